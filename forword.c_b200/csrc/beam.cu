@@ -1,0 +1,222 @@
+// beam.cu — C ABI of the beam-search operators: argument checks and launches.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdio>
+
+#include "../../include/forword_b200.h"
+#include "beam_attn.cuh"
+#include "beam_reorder.cuh"
+#include "beam_select.cuh"
+#include "status.h"
+
+namespace fwb {
+namespace {
+
+bool fail(const char *text) {
+    set_last_error(text);
+    return false;
+}
+
+bool launched(cudaError_t e, const char *who) {
+    if (e == cudaSuccess) return true;
+    char b[160];
+    snprintf(b, sizeof b, "%s: %s", who, cudaGetErrorString(e));
+    return fail(b);
+}
+
+uint32_t elem_bytes(uint32_t type) { return type == 0 ? 4u : type == 1 || type == 30 ? 2u : 0u; }
+
+// --- prefix attention --------------------------------------------------------
+bool attn_sizes_ok(const fwb_prefix_attn_t *a) {
+    if (!a) return fail("fwb_prefix_attention: null arguments");
+    if (!elem_bytes(a->type)) return fail("fwb_prefix_attention: type must be 0 (F32), 1 (F16) or 30 (BF16)");
+    if (!a->n_group || !a->n_beam || !a->n_query || !a->n_head || !a->n_head_kv)
+        return fail("fwb_prefix_attention: zero groups, beams, query tokens or heads");
+    if (a->n_head % a->n_head_kv) return fail("fwb_prefix_attention: n_head must be a multiple of n_head_kv");
+    if (!a->head_dim || a->head_dim % 16 || a->head_dim > 128)
+        return fail("fwb_prefix_attention: head_dim must be a multiple of 16, at most 128");
+    if (a->prefix_cap > 0x7fffffffu || a->suffix_cap > 0x7fffffffu)
+        return fail("fwb_prefix_attention: capacities must fit an int32");
+    const uint64_t rows = (uint64_t)a->n_group * a->n_beam;
+    if (rows > 0xffffffu || rows * a->n_query > 0xffffffu || rows * a->n_query * a->n_head > 0x7fffffffu ||
+        a->n_head > 65535)
+        return fail("fwb_prefix_attention: too many sequences, tokens or heads");
+    return true;
+}
+
+bool attn_args(const fwb_prefix_attn_t *a, BeamAttnArgs &k) {
+    if (!attn_sizes_ok(a)) return false;
+    const uint64_t e = elem_bytes(a->type);
+    if (!a->q || !a->out) return fail("fwb_prefix_attention: null q or out");
+    if ((a->prefix_cap && (!a->prefix_k || !a->prefix_v)) || (a->suffix_cap && (!a->suffix_k || !a->suffix_v)))
+        return fail("fwb_prefix_attention: null K or V");
+    uint64_t odd = (uintptr_t)a->q | a->q_seq_stride * e | a->q_token_stride * e | a->q_head_stride * e |
+                   (uintptr_t)a->out;
+    if (a->prefix_cap)
+        odd |= (uintptr_t)a->prefix_k | (uintptr_t)a->prefix_v | a->prefix_group_stride * e |
+               a->prefix_head_stride * e | a->prefix_pos_stride * e;
+    if (a->suffix_cap)
+        odd |= (uintptr_t)a->suffix_k | (uintptr_t)a->suffix_v | a->suffix_seq_stride * e |
+               a->suffix_head_stride * e | a->suffix_pos_stride * e;
+    if (odd % 16) return fail("fwb_prefix_attention: q, K, V and out and their strides must be multiples of 16 bytes");
+    if (((uintptr_t)a->lse | (uintptr_t)a->prefix_len | (uintptr_t)a->suffix_len | (uintptr_t)a->slots) % 4)
+        return fail("fwb_prefix_attention: lse, lengths and slots must be 4-byte aligned");
+    k = {};
+    k.q = a->q; k.pk = a->prefix_k; k.pv = a->prefix_v; k.sk = a->suffix_k; k.sv = a->suffix_v;
+    k.out = a->out; k.lse = a->lse;
+    k.plen = a->prefix_len; k.slen = a->suffix_len; k.slots = a->slots;
+    k.q_seq = a->q_seq_stride; k.q_tok = a->q_token_stride; k.q_head = a->q_head_stride;
+    k.p_group = a->prefix_group_stride; k.p_head = a->prefix_head_stride; k.p_pos = a->prefix_pos_stride;
+    k.s_seq = a->suffix_seq_stride; k.s_head = a->suffix_head_stride; k.s_pos = a->suffix_pos_stride;
+    k.slot_seq = a->slots_stride;
+    k.n_group = a->n_group; k.n_beam = a->n_beam; k.n_query = a->n_query;
+    k.n_head = a->n_head; k.n_kv = a->n_head_kv; k.gq = a->n_head / a->n_head_kv; k.hd = a->head_dim;
+    k.pcap = a->prefix_cap; k.scap = a->suffix_cap;
+    k.scale = a->scale != 0.f ? a->scale : 1.0f / sqrtf((float)a->head_dim);
+    return true;
+}
+
+size_t attn_workspace(const fwb_prefix_attn_t *) { return 16; }
+
+template <typename T>
+bool run_attn(const BeamAttnArgs &k, cudaStream_t st) {
+    beam_attn_rows_kernel<T><<<dim3(k.n_group * k.n_beam * k.n_query, k.n_head), kBaThreads, 0, st>>>(k);
+    return launched(cudaGetLastError(), "fwb_prefix_attention launch");
+}
+
+// --- selection ------------------------------------------------------------------
+constexpr size_t kMaxSelect = 128, kMaxSelectBeams = 64;
+
+bool select_sizes_ok(uint32_t type, size_t n_group, size_t n_beam, size_t n_vocab, size_t n_select) {
+    if (!elem_bytes(type)) return fail("fwb_beam_select: type must be 0 (F32), 1 (F16) or 30 (BF16)");
+    if (!n_group || !n_beam || !n_vocab || !n_select)
+        return fail("fwb_beam_select: zero groups, beams, tokens or selected entries");
+    if (n_beam > kMaxSelectBeams || n_group > 0x7fffffffu / kMaxSelectBeams || n_vocab > 0x7fffffffu / n_beam)
+        return fail("fwb_beam_select: more than 64 beams, or more than 2^31 - 1 scores in a group");
+    if (n_select > kMaxSelect || n_select > n_beam * n_vocab)
+        return fail("fwb_beam_select: n_select must be at most 128 and at most n_beam * n_vocab");
+    return true;
+}
+
+size_t select_workspace() { return 16; }
+
+template <typename T>
+bool run_select(const BeamSelectArgs &k, cudaStream_t st) {
+    beam_select_passes_kernel<T><<<k.n_group, kBsThreads, 0, st>>>(k);
+    return launched(cudaGetLastError(), "fwb_beam_select launch");
+}
+
+// --- reordering -------------------------------------------------------------------
+template <typename V>
+bool run_reorder(BeamReorderArgs &k, size_t run_bytes, cudaStream_t st) {
+    const size_t n_col = run_bytes / sizeof(V);
+    if (n_col > 0x7fffffffu) return fail("fwb_beam_reorder: run too long");
+    k.n_col = (uint32_t)n_col;
+    const uint64_t n = (uint64_t)k.n_outer * k.n_group * k.n_inner * n_col;
+    const unsigned grid = (unsigned)std::min<uint64_t>((n + kBrThreads - 1) / kBrThreads, 148 * 16);
+    if (k.n_beam <= 8) beam_reorder_kernel<V, 8><<<grid, kBrThreads, 0, st>>>(k);
+    else beam_reorder_kernel<V, 64><<<grid, kBrThreads, 0, st>>>(k);
+    return launched(cudaGetLastError(), "fwb_beam_reorder launch");
+}
+
+}  // namespace
+}  // namespace fwb
+
+using namespace fwb;
+
+extern "C" {
+
+size_t fwb_prefix_attention_workspace(const fwb_prefix_attn_t *a) {
+    return attn_sizes_ok(a) ? attn_workspace(a) : 0;
+}
+
+int fwb_prefix_attention_dev(const fwb_prefix_attn_t *a, void *workspace, size_t workspace_bytes, void *stream) {
+    BeamAttnArgs k;
+    if (!attn_args(a, k)) return -1;
+    if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < attn_workspace(a)) {
+        fail("fwb_prefix_attention: workspace missing, misaligned or smaller than fwb_prefix_attention_workspace");
+        return -1;
+    }
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool ok = a->type == 0 ? run_attn<float>(k, st)
+                  : a->type == 1 ? run_attn<__half>(k, st) : run_attn<__nv_bfloat16>(k, st);
+    return ok ? 0 : -1;
+}
+
+size_t fwb_beam_select_workspace(uint32_t type, size_t n_group, size_t n_beam, size_t n_vocab, size_t n_select) {
+    return select_sizes_ok(type, n_group, n_beam, n_vocab, n_select) ? select_workspace() : 0;
+}
+
+int fwb_beam_select_dev(const void *d_logits, uint32_t type, size_t n_group, size_t n_beam, size_t n_vocab,
+                        size_t row_stride, const float *d_scores, size_t n_select, float *d_out_scores,
+                        int32_t *d_parent, int32_t *d_token, void *workspace, size_t workspace_bytes, void *stream) {
+    if (!select_sizes_ok(type, n_group, n_beam, n_vocab, n_select)) return -1;
+    if (!d_logits || !d_scores || !d_out_scores || !d_parent || !d_token) {
+        fail("fwb_beam_select: null pointer");
+        return -1;
+    }
+    if (row_stride < n_vocab) { fail("fwb_beam_select: row_stride smaller than n_vocab"); return -1; }
+    if ((uintptr_t)d_logits % elem_bytes(type) ||
+        ((uintptr_t)d_scores | (uintptr_t)d_out_scores | (uintptr_t)d_parent | (uintptr_t)d_token) % 4) {
+        fail("fwb_beam_select: misaligned pointer");
+        return -1;
+    }
+    if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < select_workspace()) {
+        fail("fwb_beam_select: workspace missing, misaligned or smaller than fwb_beam_select_workspace");
+        return -1;
+    }
+    BeamSelectArgs k{};
+    k.logits = d_logits; k.scores = d_scores;
+    k.out_scores = d_out_scores; k.parent = d_parent; k.token = d_token;
+    k.row_stride = row_stride;
+    k.n_group = (uint32_t)n_group; k.n_beam = (uint32_t)n_beam; k.n_vocab = (uint32_t)n_vocab;
+    k.n_select = (uint32_t)n_select;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool ok = type == 0 ? run_select<float>(k, st)
+                  : type == 1 ? run_select<__half>(k, st) : run_select<__nv_bfloat16>(k, st);
+    return ok ? 0 : -1;
+}
+
+int fwb_beam_reorder_dev(const void *d_src, void *d_dst, const int32_t *d_parent, size_t n_outer, size_t n_group,
+                         size_t n_beam, size_t n_inner, size_t run_bytes, size_t src_outer_stride,
+                         size_t src_slot_stride, size_t src_inner_stride, size_t dst_outer_stride,
+                         size_t dst_slot_stride, size_t dst_inner_stride, void *stream) {
+    if (!d_src || !d_dst || !d_parent) { fail("fwb_beam_reorder: null pointer"); return -1; }
+    if (!n_outer || !n_group || !n_beam || !n_inner || !run_bytes) { fail("fwb_beam_reorder: zero size"); return -1; }
+    if (n_beam > kBrMaxBeams) { fail("fwb_beam_reorder: more than 64 beams"); return -1; }
+    if (n_outer > 0x7fffffffu || n_group > 0x7fffffffu / kBrMaxBeams || n_inner > 0x7fffffffu) {
+        fail("fwb_beam_reorder: sizes too large");
+        return -1;
+    }
+    if ((uintptr_t)d_parent % 4) { fail("fwb_beam_reorder: misaligned parents"); return -1; }
+    // the bytes from the first to the last that each side touches
+    const size_t src_span = (n_outer - 1) * src_outer_stride + (n_group * n_beam - 1) * src_slot_stride +
+                            (n_inner - 1) * src_inner_stride + run_bytes;
+    const size_t dst_span = (n_outer - 1) * dst_outer_stride + (n_group * n_beam - 1) * dst_slot_stride +
+                            (n_inner - 1) * dst_inner_stride + run_bytes;
+    const uintptr_t s0 = (uintptr_t)d_src, d0 = (uintptr_t)d_dst;
+    const bool same = s0 == d0 && src_outer_stride == dst_outer_stride && src_slot_stride == dst_slot_stride &&
+                      src_inner_stride == dst_inner_stride;
+    if (!same && s0 < d0 + dst_span && d0 < s0 + src_span) {
+        fail("fwb_beam_reorder: source and destination overlap without being the same");
+        return -1;
+    }
+    BeamReorderArgs k{};
+    k.src = static_cast<const uint8_t *>(d_src);
+    k.dst = static_cast<uint8_t *>(d_dst);
+    k.parent = d_parent;
+    k.src_outer = src_outer_stride; k.src_slot = src_slot_stride; k.src_inner = src_inner_stride;
+    k.dst_outer = dst_outer_stride; k.dst_slot = dst_slot_stride; k.dst_inner = dst_inner_stride;
+    k.n_group = (uint32_t)n_group; k.n_beam = (uint32_t)n_beam;
+    k.n_outer = (uint32_t)n_outer; k.n_inner = (uint32_t)n_inner;
+    const uint64_t mix = s0 | d0 | run_bytes | src_outer_stride | src_slot_stride | src_inner_stride |
+                         dst_outer_stride | dst_slot_stride | dst_inner_stride;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool ok = mix % 16 == 0 ? run_reorder<uint4>(k, run_bytes, st)
+                  : mix % 4 == 0 ? run_reorder<uint32_t>(k, run_bytes, st) : run_reorder<uint8_t>(k, run_bytes, st);
+    return ok ? 0 : -1;
+}
+
+}  // extern "C"

@@ -87,7 +87,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
 // `code` in *err) when the bound is exceeded or another thread already
 // flagged an error.  The first poll is inline (the phase has normally
 // completed already); the polling loop is out of line.
-__device__ __noinline__ bool mbar_wait_slow(uint64_t *bar, uint32_t parity, uint32_t *err, uint32_t code) {
+inline __device__ __noinline__ bool mbar_wait_slow(uint64_t *bar, uint32_t parity, uint32_t *err, uint32_t code) {
     for (uint32_t i = 0; i < kMaxPolls; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if (i > 64) __nanosleep(i < 4096 ? 32 : 256);

@@ -22,6 +22,7 @@
 #include "attention.cuh"
 #include "gemv.cuh"
 #include "gguf_reader.h"
+#include "status.h"
 #include "tp_shard.h"
 #include "upload.h"
 #include "decode.cuh"
@@ -34,6 +35,12 @@ namespace fwb {
 
 static thread_local std::string g_err;
 static void set_err(const std::string &e) { g_err = e; }
+void set_last_error(const char *text) noexcept {
+    try {
+        g_err = text;
+    } catch (...) {  // no memory for the text: the return code still tells
+    }
+}
 
 #define CK(x)                                                                            \
     do {                                                                                 \

@@ -96,3 +96,8 @@ def _declare(lib) -> None:
     sig("fwb_tp_handle", _i32, _vp, _vp)
     sig("fwb_tp_connect", _i32, _vp, _vp)
     sig("fwb_tp_shard", _i32, _c.c_char_p, _c.c_char_p, _i32, _i32, _i32, _vp, _sz, _c.POINTER(_sz))
+    sig("fwb_prefix_attention_dev", _i32, _vp, _vp, _sz, _vp)
+    sig("fwb_prefix_attention_workspace", _sz, _vp)
+    sig("fwb_beam_select_dev", _i32, _vp, _u32, _sz, _sz, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp)
+    sig("fwb_beam_select_workspace", _sz, _u32, _sz, _sz, _sz, _sz)
+    sig("fwb_beam_reorder_dev", _i32, _vp, _vp, _vp, *[_sz] * 11, _vp)

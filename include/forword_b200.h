@@ -141,6 +141,94 @@ int quant_dequant_dev(const void *d_weights, size_t weights_size, uint32_t ggml_
                       float *d_out, size_t n_values, void *stream);
 
 /* ------------------------------------------------------------------------
+ * Beam search and parallel continuations of one prompt (no reference
+ * counterpart: forword.c keeps one sequence).  Sequences come in n_group
+ * groups of n_beam; sequence s = group * n_beam + beam.  The operators take
+ * device pointers, run on the current device, enqueue on `stream` (a
+ * cudaStream_t, NULL = legacy default stream) and return without waiting;
+ * they allocate nothing and may be captured into a CUDA graph.  Element
+ * types are GGML's ids: 0 (F32), 1 (F16), 30 (BF16).
+ * ------------------------------------------------------------------------ */
+
+/* Arguments of fwb_prefix_attention_dev.  Strides are in elements, the
+ * head_dim values of a row are contiguous; q, K and V addresses and the byte
+ * strides of K and V are multiples of 16, those of q too. */
+typedef struct fwb_prefix_attn {
+    uint32_t type;                     /* of q, K, V and out: 0, 1 or 30 */
+    uint32_t n_group, n_beam, n_query; /* n_query new tokens per sequence */
+    uint32_t n_head, n_head_kv;        /* n_head a multiple of n_head_kv */
+    uint32_t head_dim;                 /* a multiple of 16, at most 128 */
+    uint32_t prefix_cap, suffix_cap;   /* positions that the caches hold (0: none) */
+    float scale;                       /* of the scores; 0 -> 1/sqrt(head_dim) */
+    const void *q;                     /* [n_seq][n_query][n_head][head_dim] */
+    uint64_t q_seq_stride, q_token_stride, q_head_stride;
+    const void *prefix_k, *prefix_v;   /* [n_group][n_head_kv][prefix_cap][head_dim] */
+    uint64_t prefix_group_stride, prefix_head_stride, prefix_pos_stride;
+    const void *suffix_k, *suffix_v;   /* [n_seq][n_head_kv][suffix_cap][head_dim] */
+    uint64_t suffix_seq_stride, suffix_head_stride, suffix_pos_stride;
+    const int32_t *prefix_len;         /* [n_group], or NULL: prefix_cap each */
+    const int32_t *suffix_len;         /* [n_seq], the new tokens included, or NULL: suffix_cap each */
+    const int32_t *slots;              /* [n_seq][suffix_cap], or NULL: every position its own */
+    uint64_t slots_stride;
+    void *out;                         /* [n_seq][n_query][n_head][head_dim], contiguous */
+    float *lse;                        /* [n_seq][n_query][n_head], or NULL */
+} fwb_prefix_attn_t;
+
+/*
+ * Attention of every new token over its group's prefix (held once and read
+ * once for all its beams) and its own sequence's suffix.  Token t of n_query
+ * sees the prefix and the first suffix_len - (n_query - 1 - t) suffix
+ * positions.  slots[s][p] = b: suffix position p of sequence s is row p of
+ * sequence group * n_beam + b, the beam that computed it, so that a beam
+ * step re-orders this table instead of the cache (an entry outside
+ * 0..n_beam-1 counts as the sequence's own beam).  lse receives log sum exp
+ * of the scaled scores.  A token that sees no position gets out 0 and lse
+ * -inf.  Lengths are held to 0..cap; rows at and past a length are never
+ * used, whatever they hold.  Scores, softmax and sums are fp32.
+ * workspace: fwb_prefix_attention_workspace(a) bytes of device memory,
+ * 16-byte aligned, that no other call uses meanwhile; its contents matter to
+ * nobody between calls.  -1 with fwb_last_error() for arguments outside the
+ * above.
+ */
+int fwb_prefix_attention_dev(const fwb_prefix_attn_t *a, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Bytes of workspace that fwb_prefix_attention_dev needs for a's type, sizes
+ * and capacities (its pointers, lengths and strides are not looked at); 0
+ * with fwb_last_error() for sizes that it does not take. */
+size_t fwb_prefix_attention_workspace(const fwb_prefix_attn_t *a);
+
+/*
+ * Selection of a beam step: of the n_beam * n_vocab scores of a group,
+ * score[w][v] = d_scores[w] + logits[w][v] - logsumexp(logits[w]), the
+ * n_select largest in descending order, the lowest index w * n_vocab + v
+ * first among equals: their scores, beams (0..n_beam-1) and tokens, each
+ * [n_group][n_select].  d_logits holds n_group * n_beam rows of n_vocab
+ * elements of `type`, row_stride elements apart; d_scores [n_group * n_beam].
+ * A logit of -inf bars its token.  A row that is barred throughout, holds a
+ * NaN or +inf, or has a d_scores entry that is not finite offers no
+ * candidate (its scores are -inf, and still rank by index).  n_beam at most
+ * 64, n_select at most 128 and at most n_beam * n_vocab, which is at most
+ * 2^31 - 1.  workspace as above, of fwb_beam_select_workspace bytes.
+ */
+int fwb_beam_select_dev(const void *d_logits, uint32_t type, size_t n_group, size_t n_beam, size_t n_vocab,
+                        size_t row_stride, const float *d_scores, size_t n_select, float *d_out_scores,
+                        int32_t *d_parent, int32_t *d_token, void *workspace, size_t workspace_bytes, void *stream);
+size_t fwb_beam_select_workspace(uint32_t type, size_t n_group, size_t n_beam, size_t n_vocab, size_t n_select);
+
+/*
+ * Per-beam state moved by the parents of a beam step:
+ * dst[o][g * n_beam + b][i] = src[o][g * n_beam + parent[g][b]][i] for runs
+ * of run_bytes bytes, o < n_outer, i < n_inner, all strides in bytes.
+ * d_dst == d_src with equal strides works in place; otherwise the two must
+ * not overlap.  A parent outside 0..n_beam-1 counts as b itself.  n_beam at
+ * most 64.
+ */
+int fwb_beam_reorder_dev(const void *d_src, void *d_dst, const int32_t *d_parent, size_t n_outer, size_t n_group,
+                         size_t n_beam, size_t n_inner, size_t run_bytes, size_t src_outer_stride,
+                         size_t src_slot_stride, size_t src_inner_stride, size_t dst_outer_stride,
+                         size_t dst_slot_stride, size_t dst_inner_stride, void *stream);
+
+/* ------------------------------------------------------------------------
  * Decode model (transformer.h:39-48 semantics).
  * ------------------------------------------------------------------------ */
 
