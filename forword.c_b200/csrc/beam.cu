@@ -39,6 +39,7 @@ bool attn_sizes_ok(const fwb_prefix_attn_t *a) {
         return fail("fwb_prefix_attention: head_dim must be a multiple of 16, at most 128");
     if (a->prefix_cap > 0x7fffffffu || a->suffix_cap > 0x7fffffffu)
         return fail("fwb_prefix_attention: capacities must fit an int32");
+    if (!(a->scale >= 0.f) || a->scale > 3e38f) return fail("fwb_prefix_attention: scale must be positive, or 0 for the default");
     const uint64_t rows = (uint64_t)a->n_group * a->n_beam;
     if (rows > 0xffffffu || rows * a->n_query > 0xffffffu || rows * a->n_query * a->n_head > 0x7fffffffu ||
         a->n_head > 65535)
@@ -78,12 +79,101 @@ bool attn_args(const fwb_prefix_attn_t *a, BeamAttnArgs &k) {
     return true;
 }
 
-size_t attn_workspace(const fwb_prefix_attn_t *) { return 16; }
+uint32_t device_sms() {
+    static int n[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if (!n[dev]) {
+        int v = 0;
+        if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v < 1) return 148;
+        n[dev] = v;
+    }
+    return (uint32_t)n[dev];
+}
+
+// Row tiles and the workspace's layout; returns its bytes.
+struct AttnLayout {
+    uint32_t prg, srg;  // row groups of 16 of a prefix / suffix tile: 1, 2 or 4
+    uint32_t ptiles, stiles, ctas;
+    size_t pitems, sitems, bytes;
+    size_t po, so, pml, sml, pcta, scta;
+};
+
+bool attn_layout(const fwb_prefix_attn_t *a, AttnLayout &L) {
+    const uint64_t gq = a->n_head / a->n_head_kv, srows = gq * a->n_query, prows = srows * a->n_beam;
+    const uint32_t hd = a->head_dim <= 64 ? 64 : 128;
+    auto groups = [](uint64_t rows) { return rows <= 16 ? 1u : rows <= 32 ? 2u : 4u; };
+    L.prg = groups(prows);
+    L.srg = srows <= 16 ? 1u : L.prg;
+    L.ptiles = (uint32_t)((prows + L.prg * 16 - 1) / (L.prg * 16));
+    L.stiles = (uint32_t)((srows + L.srg * 16 - 1) / (L.srg * 16));
+    L.pitems = a->prefix_cap ? (size_t)a->n_group * a->n_head_kv * L.ptiles : 0;
+    L.sitems = a->suffix_cap ? (size_t)a->n_group * a->n_beam * a->n_head_kv * L.stiles : 0;
+    const uint64_t units = L.pitems * ((a->prefix_cap + 15) / 16) + L.sitems * ((a->suffix_cap + 15) / 16);
+    if (L.pitems + L.sitems > 0x3fffffffu || units >> 40)
+        return fail("fwb_prefix_attention: too many rows times positions");
+    L.ctas = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(2 * device_sms(), units));
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        const size_t here = at;
+        at += (n + 255) & ~(size_t)255;
+        return here;
+    };
+    const size_t pslots = (L.pitems + L.ctas) * L.prg * 16, sslots = (L.sitems + L.ctas) * L.srg * 16;
+    L.po = take(pslots * hd * 4);
+    L.so = take(sslots * hd * 4);
+    L.pml = take(pslots * 8);
+    L.sml = take(sslots * 8);
+    L.pcta = take(L.pitems * 8);
+    L.scta = take(L.sitems * 8);
+    L.bytes = at;
+    return true;
+}
+
+template <typename T, int HD, int RWP, int RWS>
+bool launch_attn(const BeamAttnArgs &k, const BeamAttnPlan &p, cudaStream_t st) {
+    static bool ready[64] = {};
+    constexpr uint32_t smem = beam_attn_smem<T, HD>();
+    int dev = 0;
+    if (!launched(cudaGetDevice(&dev), "fwb_prefix_attention")) return false;
+    if (dev >= 64 || !ready[dev]) {
+        if (!launched(cudaFuncSetAttribute(beam_attn_kernel<T, HD, RWP, RWS>,
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
+                      "fwb_prefix_attention"))
+            return false;
+        if (dev < 64) ready[dev] = true;
+    }
+    beam_attn_kernel<T, HD, RWP, RWS><<<p.ctas, kBaThreads, smem, st>>>(k, p);
+    beam_attn_join_kernel<T, HD><<<dim3(k.n_group * k.n_beam * k.n_query, k.n_head), kBaThreads, 0, st>>>(k, p);
+    return launched(cudaGetLastError(), "fwb_prefix_attention launch");
+}
+
+template <typename T, int HD>
+bool pick_attn(const BeamAttnArgs &k, const BeamAttnPlan &p, uint32_t prg, uint32_t srg, cudaStream_t st) {
+    switch (prg * 8 + srg) {
+    case 1 * 8 + 1: return launch_attn<T, HD, 1, 1>(k, p, st);
+    case 2 * 8 + 1: return launch_attn<T, HD, 2, 1>(k, p, st);
+    case 2 * 8 + 2: return launch_attn<T, HD, 2, 2>(k, p, st);
+    case 4 * 8 + 1: return launch_attn<T, HD, 4, 1>(k, p, st);
+    default: return launch_attn<T, HD, 4, 4>(k, p, st);
+    }
+}
 
 template <typename T>
-bool run_attn(const BeamAttnArgs &k, cudaStream_t st) {
-    beam_attn_rows_kernel<T><<<dim3(k.n_group * k.n_beam * k.n_query, k.n_head), kBaThreads, 0, st>>>(k);
-    return launched(cudaGetLastError(), "fwb_prefix_attention launch");
+bool run_attn(const BeamAttnArgs &k, const AttnLayout &L, uint8_t *ws, cudaStream_t st) {
+    BeamAttnPlan p;
+    p.po = reinterpret_cast<float *>(ws + L.po);
+    p.so = reinterpret_cast<float *>(ws + L.so);
+    p.pml = reinterpret_cast<float2 *>(ws + L.pml);
+    p.sml = reinterpret_cast<float2 *>(ws + L.sml);
+    p.pcta = reinterpret_cast<uint2 *>(ws + L.pcta);
+    p.scta = reinterpret_cast<uint2 *>(ws + L.scta);
+    p.prow = L.prg * 16;
+    p.srow = L.srg * 16;
+    p.ptiles = L.ptiles;
+    p.stiles = L.stiles;
+    p.ctas = L.ctas;
+    return k.hd <= 64 ? pick_attn<T, 64>(k, p, L.prg, L.srg, st) : pick_attn<T, 128>(k, p, L.prg, L.srg, st);
 }
 
 // --- selection ------------------------------------------------------------------
@@ -129,19 +219,22 @@ using namespace fwb;
 extern "C" {
 
 size_t fwb_prefix_attention_workspace(const fwb_prefix_attn_t *a) {
-    return attn_sizes_ok(a) ? attn_workspace(a) : 0;
+    AttnLayout L;
+    return attn_sizes_ok(a) && attn_layout(a, L) ? L.bytes : 0;
 }
 
 int fwb_prefix_attention_dev(const fwb_prefix_attn_t *a, void *workspace, size_t workspace_bytes, void *stream) {
     BeamAttnArgs k;
-    if (!attn_args(a, k)) return -1;
-    if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < attn_workspace(a)) {
+    AttnLayout L;
+    if (!attn_args(a, k) || !attn_layout(a, L)) return -1;
+    if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < L.bytes) {
         fail("fwb_prefix_attention: workspace missing, misaligned or smaller than fwb_prefix_attention_workspace");
         return -1;
     }
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool ok = a->type == 0 ? run_attn<float>(k, st)
-                  : a->type == 1 ? run_attn<__half>(k, st) : run_attn<__nv_bfloat16>(k, st);
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    const bool ok = a->type == 0 ? run_attn<float>(k, L, ws, st)
+                  : a->type == 1 ? run_attn<__half>(k, L, ws, st) : run_attn<__nv_bfloat16>(k, L, ws, st);
     return ok ? 0 : -1;
 }
 

@@ -51,71 +51,666 @@ __device__ __forceinline__ uint32_t beam_len(const int32_t *len, uint32_t i, uin
     return n < 0 ? 0u : min((uint32_t)n, cap);
 }
 
-constexpr int kBaThreads = 128;
+// ---------------------------------------------------------------------------
+// The split of the work.  A "part" is one group's prefix (rows: the query
+// heads of one KV head of all its beams and new tokens) or one sequence's
+// suffix; an item is a part, a KV head and a tile of rows.  Every item is a
+// run of units of 16 positions; all items' U units stand in one line, and CTA c
+// of C <= U takes units [c U / C, (c + 1) U / C).  So every CTA reads as many
+// positions as any other, whatever the lengths are, and an item that several
+// CTAs share leaves one partial result (sum, maximum, weighted values) per
+// CTA.  A second kernel joins a row's partial results of prefix and suffix.
+// ---------------------------------------------------------------------------
+constexpr uint32_t kBaUnit = 16;      // positions
+constexpr int kBaThreads = 128;       // four warps
+constexpr int kBaStages = 3;
+constexpr uint32_t kBaSRows = 16;     // least rows of a tile
 
-// One block per (query token, query head): its warps take the positions in
-// turn, each with its own running maximum, sum and weighted values.
-template <typename T>
-__global__ void __launch_bounds__(kBaThreads) beam_attn_rows_kernel(BeamAttnArgs a) {
-    constexpr int NW = kBaThreads / 32;
-    __shared__ float part[NW][128], pm[NW], pl[NW];
+struct BeamAttnPlan {
+    float *po, *so;        // partial weighted values of prefix and suffix items: [slot][rows][HD]
+    float2 *pml, *sml;     // their (maximum in units of log2, sum): [slot][rows]
+    uint2 *pcta, *scta;    // (first, last) CTA of each item
+    uint32_t prow, srow;   // rows of a prefix / suffix tile
+    uint32_t ptiles, stiles;  // row tiles of a group / of a sequence
+    uint32_t ctas;
+};
+
+// Where a CTA stands in the line of units.
+struct BeamCursor {
+    uint32_t part;         // 0..n_group-1: prefixes, then the sequences
+    uint32_t kvh, tile;
+    uint32_t pos, len;     // the item's next position and its length
+    uint32_t left;         // positions that this CTA still takes, counted in whole units
+};
+
+__device__ __forceinline__ uint32_t beam_part_len(const BeamAttnArgs &a, uint32_t part) {
+    return part < a.n_group ? beam_len(a.plen, part, a.pcap) : beam_len(a.slen, part - a.n_group, a.scap);
+}
+__device__ __forceinline__ uint32_t beam_units(uint32_t len) { return (len + kBaUnit - 1) / kBaUnit; }
+
+// The cursor of this CTA's first unit; false when it has none.  One scan of
+// the parts' lengths by the whole block.
+__device__ inline bool beam_first(const BeamAttnArgs &a, const BeamAttnPlan &p, BeamCursor &c) {
+    __shared__ uint64_t s_warp[kBaThreads / 32];
+    __shared__ uint32_t s_part;
+    __shared__ uint64_t s_off;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t row = blockIdx.x, h = blockIdx.y, kvh = h / a.gq;
-    const uint32_t s = row / a.n_query, t = row % a.n_query, grp = s / a.n_beam;
-    const T *q = static_cast<const T *>(a.q) + s * a.q_seq + t * a.q_tok + h * a.q_head;
-    const T *pk = static_cast<const T *>(a.pk) + grp * a.p_group + kvh * a.p_head;
-    const T *pv = static_cast<const T *>(a.pv) + grp * a.p_group + kvh * a.p_head;
-    const uint32_t np = beam_len(a.plen, grp, a.pcap), ns = beam_len(a.slen, s, a.scap);
-    const uint32_t hidden = a.n_query - 1 - t;
-    const uint32_t n = np + (ns > hidden ? ns - hidden : 0);
-    float qv[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
+    const uint32_t parts = a.n_group + a.n_group * a.n_beam;
+    uint64_t sum = 0;
+    for (uint32_t i = threadIdx.x; i < parts; i += kBaThreads)
+        sum += (uint64_t)beam_units(beam_part_len(a, i)) * a.n_kv * (i < a.n_group ? p.ptiles : p.stiles);
+    uint64_t t = sum;
+    for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if (lane == 0) s_warp[warp] = t;
+    __syncthreads();
+    uint64_t total = 0;
+    for (int w = 0; w < kBaThreads / 32; ++w) total += s_warp[w];
+    // with fewer units than CTAs the first ones take one each, so that the
+    // CTAs of an item are neighbours
+    const uint64_t ctas = total < p.ctas ? total : p.ctas;
+    if (blockIdx.x >= ctas) return false;  // the same in every thread
+    const uint64_t lo = blockIdx.x * total / ctas, hi = (blockIdx.x + 1) * total / ctas;
+    uint64_t base = 0;
+    for (uint32_t i0 = 0; i0 < parts; i0 += kBaThreads) {
+        const uint32_t i = i0 + threadIdx.x;
+        uint64_t w = 0;
+        if (i < parts) w = (uint64_t)beam_units(beam_part_len(a, i)) * a.n_kv * (i < a.n_group ? p.ptiles : p.stiles);
+        uint64_t inc = w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) qv[i] = lane + 32 * i < a.hd ? beam_to_f32(q[lane + 32 * i]) : 0.f;
-    for (uint32_t j = warp; j < n; j += NW) {
-        const T *k, *v;
-        if (j < np) {
-            k = pk + j * a.p_pos;
-            v = pv + j * a.p_pos;
-        } else {
-            const uint32_t at = j - np;
-            uint32_t b = s % a.n_beam;
-            if (a.slots) {
-                const uint32_t from = (uint32_t)a.slots[s * a.slot_seq + at];
-                if (from < a.n_beam) b = from;
-            }
-            const size_t off = (size_t)(grp * a.n_beam + b) * a.s_seq + kvh * a.s_head + at * a.s_pos;
-            k = static_cast<const T *>(a.sk) + off;
-            v = static_cast<const T *>(a.sv) + off;
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= (uint32_t)o) inc += v;
         }
-        float x = 0.f;
+        __syncthreads();
+        if (lane == 31) s_warp[warp] = inc;
+        __syncthreads();
+        uint64_t before = base;
+        for (uint32_t v = 0; v < warp; ++v) before += s_warp[v];
+        const uint64_t first = before + inc - w;
+        if (w && lo >= first && lo < first + w) { s_part = i; s_off = lo - first; }
+        for (int v = 0; v < kBaThreads / 32; ++v) base += s_warp[v];
+        if (base > lo) break;  // the same in every thread
+    }
+    __syncthreads();
+    c.part = s_part;
+    c.len = beam_part_len(a, c.part);
+    const uint32_t units = beam_units(c.len), tiles = c.part < a.n_group ? p.ptiles : p.stiles;
+    const uint32_t item = (uint32_t)(s_off / units);
+    c.kvh = item / tiles;
+    c.tile = item % tiles;
+    c.pos = (uint32_t)(s_off % units) * kBaUnit;
+    c.left = (uint32_t)(hi - lo);
+    return true;
+}
+
+// To the item after the cursor's (its positions are used up, units are left).
+__device__ __forceinline__ void beam_next_item(const BeamAttnArgs &a, const BeamAttnPlan &p, BeamCursor &c) {
+    c.pos = 0;
+    if (++c.tile < (c.part < a.n_group ? p.ptiles : p.stiles)) return;
+    c.tile = 0;
+    if (++c.kvh < a.n_kv) return;
+    c.kvh = 0;
+    do {
+        if (++c.part >= a.n_group + a.n_group * a.n_beam) {  // lengths that changed under the call
+            c.left = 0;
+            return;
+        }
+        c.len = beam_part_len(a, c.part);
+    } while (c.len == 0);
+}
+
+// --- matrix instructions of a warp --------------------------------------------
+__device__ __forceinline__ void ldm_x4(uint32_t *r, uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldm_x4_t(uint32_t *r, uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void mma16(float *c, const uint32_t *a, uint32_t b0, uint32_t b1, __half) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16(float *c, const uint32_t *a, uint32_t b0, uint32_t b1, __nv_bfloat16) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x = hi + lo: hi rounded to tf32's 11 significant bits, lo the exact rest
+// (13 bits; the product takes its first 11).
+__device__ __forceinline__ void tf32_split(float x, uint32_t &hi, uint32_t &lo) {
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+    lo = __float_as_uint(x - __uint_as_float(hi));
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// 16 bytes global -> shared, or zeros (the source is not read then).
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src, bool take) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// Shared-memory tile: KT rows of HD elements in 16-byte chunks, the chunk
+// index xor-ed by a function of the row so that the reads below touch all
+// banks.  16-bit types: ldmatrix reads 8 consecutive rows of one chunk.
+// fp32: a quarter-warp reads 4 chunks of 2 rows (K), or 2 chunks of the rows
+// 2t, t = 0..3 (V).
+template <typename T, int HD>
+struct BeamTile {
+    static constexpr int kEs = sizeof(T), kChunks = HD * kEs / 16, kKeys = kEs == 2 ? 64 : 32;
+    static constexpr uint32_t kBytes = kKeys * HD * kEs;  // of K; V the same
+    static __device__ __forceinline__ uint32_t k_at(uint32_t row, uint32_t chunk) {
+        return (row * kChunks + (chunk ^ (kEs == 2 ? row & 7 : (row & 1) << 2))) * 16;
+    }
+    static __device__ __forceinline__ uint32_t v_at(uint32_t row, uint32_t chunk) {
+        return (row * kChunks + (chunk ^ (kEs == 2 ? row & 7 : row & 6))) * 16;
+    }
+};
+
+template <typename T, int HD>
+constexpr uint32_t beam_attn_smem() {
+    return 2 * BeamTile<T, HD>::kBytes * kBaStages + 2 * 16 * HD * 4 + 2 * 16 * 8;
+}
+
+// This CTA's next tile of positions from the cursor into stage `st`: K and V
+// rows by 16-byte asynchronous copies (gathered through the slot table in a
+// suffix).  V rows past the part's positions are zeros: their probabilities
+// are zero, and zero times whatever the shared memory held must be zero.
+template <typename T, int HD>
+__device__ __forceinline__ void beam_load(const BeamAttnArgs &a, const BeamCursor &c, uint32_t n, uint32_t st) {
+    using Tl = BeamTile<T, HD>;
+    constexpr int CH = Tl::kChunks, RP = kBaThreads / CH;  // rows per pass of the block
+    const uint32_t ch = threadIdx.x % CH, r0 = threadIdx.x / CH;
+    const uint32_t ks = st, vs = st + Tl::kBytes;
+    if (ch * (16 / Tl::kEs) >= a.hd) return;  // the padding of the head stays zero
+    const size_t col = (size_t)ch * (16 / Tl::kEs);
+    if (c.part < a.n_group) {
+        const size_t off = c.part * a.p_group + c.kvh * a.p_head + (size_t)(c.pos + r0) * a.p_pos + col;
+        const T *k = static_cast<const T *>(a.pk) + off, *v = static_cast<const T *>(a.pv) + off;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 32 * i < a.hd) x = fmaf(qv[i], beam_to_f32(k[lane + 32 * i]), x);
+        for (int i = 0; i < Tl::kKeys / RP; ++i) {
+            const uint32_t row = r0 + i * RP;
+            const size_t step = (size_t)i * RP * a.p_pos;
+            const bool in = row < n;
+            if (in) cp_async16_or_zero(ks + Tl::k_at(row, ch), k + step, true);
+            cp_async16_or_zero(vs + Tl::v_at(row, ch), in ? v + step : v, in);
+        }
+    } else {
+        const uint32_t s = c.part - a.n_group, b0 = s / a.n_beam * a.n_beam;
+        const int32_t *slots = a.slots ? a.slots + s * a.slot_seq + c.pos : nullptr;
+        const size_t head = c.kvh * a.s_head + (size_t)c.pos * a.s_pos + col;
 #pragma unroll
-        for (int w = 16; w; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
-        x *= a.scale;
-        const float mn = fmaxf(m, x);
-        const float al = m == -INFINITY ? 0.f : expf(m - mn), e = x == -INFINITY ? 0.f : expf(x - mn);
-        l = fmaf(l, al, e);
+        for (int i = 0; i < Tl::kKeys / RP; ++i) {
+            const uint32_t row = r0 + i * RP;
+            const bool in = row < n;
+            uint32_t seq = s;
+            if (slots && in) {
+                const uint32_t from = (uint32_t)slots[row];
+                if (from < a.n_beam) seq = b0 + from;
+            }
+            const size_t off = in ? seq * a.s_seq + head + (size_t)row * a.s_pos : 0;
+            if (in) cp_async16_or_zero(ks + Tl::k_at(row, ch), static_cast<const T *>(a.sk) + off, true);
+            cp_async16_or_zero(vs + Tl::v_at(row, ch), static_cast<const T *>(a.sv) + off, in);
+        }
+    }
+}
+
+// The online softmax of a warp's 16 rows: thread rows g and g + 8 (g = lane
+// / 4).  Scores come in sc (raw products), leave as probabilities relative
+// to the new maximum; returns the factors of the earlier sums.
+template <int NB>
+__device__ __forceinline__ void beam_softmax(float (*sc)[4], float sl2, float *m, float *l, float *al) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 32 * i < a.hd) o[i] = fmaf(e, beam_to_f32(v[lane + 32 * i]), o[i] * al);
-        m = mn;
+    for (int h = 0; h < 2; ++h) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) mx = fmaxf(mx, fmaxf(sc[j][2 * h], sc[j][2 * h + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mn = fmaxf(m[h], mx * sl2), safe = mn == -INFINITY ? 0.f : mn;
+        al[h] = exp2_fast(m[h] - safe);
+        m[h] = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+            for (int e = 2 * h; e < 2 * h + 2; ++e) {
+                sc[j][e] = exp2_fast(fmaf(sc[j][e], sl2, -safe));
+                sum += sc[j][e];
+            }
+        l[h] = fmaf(l[h], al[h], sum);  // the lanes' shares are joined at the end
+    }
+}
+
+// Rows of one warp: 16 query rows in registers, their output, maximum, sum.
+template <typename T, int HD>
+struct BeamRows {
+    uint32_t q[HD * sizeof(T) / 8];  // matrix operand A: 16-bit pairs, or fp32 values
+    float o[HD / 8][4];
+    float m[2], l[2];
+    int32_t lim[2];                  // positions that rows g and g + 8 see (-1: no such row)
+};
+
+// Query rows of an item: row r of the tile, as the operand of lane (g, t).
+template <typename T, int HD>
+__device__ __forceinline__ const T *beam_q_row(const BeamAttnArgs &a, const BeamCursor &c, uint32_t r, int32_t &lim) {
+    lim = -1;
+    const uint32_t rows = (c.part < a.n_group ? a.n_beam : 1) * a.n_query * a.gq;
+    if (r >= rows) return nullptr;
+    const uint32_t h = c.kvh * a.gq + r % a.gq, t = r / a.gq % a.n_query;
+    uint32_t s = c.part - a.n_group;
+    if (c.part < a.n_group) {
+        s = c.part * a.n_beam + r / (a.gq * a.n_query);
+        lim = 0x7fffffff;
+    } else {
+        const uint32_t hidden = a.n_query - 1 - t;
+        lim = c.len > hidden ? (int32_t)(c.len - hidden) : 0;
+    }
+    return static_cast<const T *>(a.q) + s * a.q_seq + t * a.q_tok + h * a.q_head;
+}
+
+template <typename T, int HD>
+__device__ __forceinline__ void beam_rows_init(const BeamAttnArgs &a, const BeamCursor &c, uint32_t r0,
+                                               BeamRows<T, HD> &w) {
+    const uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const T *q[2];
+    q[0] = beam_q_row<T, HD>(a, c, r0 + g, w.lim[0]);
+    q[1] = beam_q_row<T, HD>(a, c, r0 + g + 8, w.lim[1]);
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {  // a0: (g, 2t), a1: (g + 8, 2t), a2: (g, 2t + 8), a3: (g + 8, 2t + 8)
+                const uint32_t d = 16 * k + 2 * t + (e >= 2 ? 8 : 0);
+                const T *p = q[e & 1];
+                w.q[4 * k + e] = p && d < a.hd ? *reinterpret_cast<const uint32_t *>(p + d) : 0u;
+            }
+    } else {
+        // the 16 dimensions 16 k ..: lane t takes 4 t .. 4 t + 3, the first two
+        // as columns t and t + 4 of one product and the others of the next
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t d = 16 * k + 4 * t;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (q[e] && d < a.hd) v = *reinterpret_cast<const uint4 *>(q[e] + d);
+                w.q[8 * k + e] = v.x;
+                w.q[8 * k + 2 + e] = v.y;
+                w.q[8 * k + 4 + e] = v.z;
+                w.q[8 * k + 6 + e] = v.w;
+            }
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) part[warp][lane + 32 * i] = o[i];
+    for (int j = 0; j < HD / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w.o[j][e] = 0.f;
+    w.m[0] = w.m[1] = -INFINITY;
+    w.l[0] = w.l[1] = 0.f;
+}
+
+// One tile: KW positions of it, from row k0 on, for this warp's 16 rows.
+// `at`: the part's position of the tile's first row; `end`: the positions
+// that this segment takes.
+template <typename T, int HD, int KW>
+__device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t ks, uint32_t vs, uint32_t k0, uint32_t at,
+                                          uint32_t end, float sl2) {
+    using Tl = BeamTile<T, HD>;
+    const uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    float sc[KW / 8][4];
+#pragma unroll
+    for (int j = 0; j < KW / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[j][e] = 0.f;
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+            for (int j = 0; j < KW / 16; ++j) {
+                uint32_t b[4];
+                ldm_x4(b, ks + Tl::k_at(k0 + 16 * j + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+                mma16(sc[2 * j], w.q + 4 * k, b[0], b[1], T{});
+                mma16(sc[2 * j + 1], w.q + 4 * k, b[2], b[3], T{});
+            }
+    } else {
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+            uint32_t ah[8], al[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) tf32_split(__uint_as_float(w.q[8 * k + e]), ah[e], al[e]);
+#pragma unroll
+            for (int j = 0; j < KW / 8; ++j) {
+                float4 v;
+                const uint32_t ad = ks + Tl::k_at(k0 + 8 * j + g, 4 * k + t);
+                asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(ad));
+                uint32_t bh[4], bl[4];
+                tf32_split(v.x, bh[0], bl[0]);
+                tf32_split(v.y, bh[1], bl[1]);
+                tf32_split(v.z, bh[2], bl[2]);
+                tf32_split(v.w, bh[3], bl[3]);
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {  // the small products first
+                    mma8(sc[j], al + 4 * s, bh[2 * s], bh[2 * s + 1]);
+                    mma8(sc[j], ah + 4 * s, bl[2 * s], bl[2 * s + 1]);
+                    mma8(sc[j], ah + 4 * s, bh[2 * s], bh[2 * s + 1]);
+                }
+            }
+        }
+    }
+    // positions that a row does not see
+    const uint32_t first = at + k0, lim0 = min((uint32_t)w.lim[0], end), lim1 = min((uint32_t)w.lim[1], end);
+    if (first + KW > min(lim0, lim1)) {
+#pragma unroll
+        for (int j = 0; j < KW / 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (first + 8 * j + 2 * t + (e & 1) >= (e < 2 ? lim0 : lim1)) sc[j][e] = -INFINITY;
+    }
+    float al[2];
+    beam_softmax<KW / 8>(sc, sl2, w.m, w.l, al);
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int j = 0; j < HD / 8; ++j) {
+            w.o[j][0] *= al[0];
+            w.o[j][1] *= al[0];
+            w.o[j][2] *= al[1];
+            w.o[j][3] *= al[1];
+        }
+#pragma unroll
+        for (int k = 0; k < KW / 16; ++k) {
+            uint32_t p[4];
+            p[0] = pack2(sc[2 * k][0], sc[2 * k][1], T{});
+            p[1] = pack2(sc[2 * k][2], sc[2 * k][3], T{});
+            p[2] = pack2(sc[2 * k + 1][0], sc[2 * k + 1][1], T{});
+            p[3] = pack2(sc[2 * k + 1][2], sc[2 * k + 1][3], T{});
+#pragma unroll
+            for (int j = 0; j < HD / 16; ++j) {
+                uint32_t b[4];
+                ldm_x4_t(b, vs + Tl::v_at(k0 + 16 * k + (lane & 7) + ((lane >> 3) & 1) * 8, 2 * j + (lane >> 4)));
+                mma16(w.o[2 * j], p, b[0], b[1], T{});
+                mma16(w.o[2 * j + 1], p, b[2], b[3], T{});
+            }
+        }
+    } else {
+        // The tensor cores' fp32 sums truncate: a tile's products are summed
+        // from zero and added to the output with one rounded fma, the rescaling
+        // in the same instruction.
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) {
+            float acc[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
+#pragma unroll
+            for (int k = 0; k < KW / 8; ++k) {
+                uint32_t ph[4], pl[4];  // columns t, t + 4: positions 2 t, 2 t + 1
+                tf32_split(sc[k][0], ph[0], pl[0]);
+                tf32_split(sc[k][2], ph[1], pl[1]);
+                tf32_split(sc[k][1], ph[2], pl[2]);
+                tf32_split(sc[k][3], ph[3], pl[3]);
+                float v[2][4];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const uint32_t ad = vs + Tl::v_at(k0 + 8 * k + 2 * t + r, 8 * j + g);
+                    asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];"
+                                 : "=f"(v[r][0]), "=f"(v[r][1]), "=f"(v[r][2]), "=f"(v[r][3]) : "r"(ad));
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {  // column g of product i: dimension 32 j + 4 g + i
+                    uint32_t h0, l0, h1, l1;
+                    tf32_split(v[0][i], h0, l0);
+                    tf32_split(v[1][i], h1, l1);
+                    mma8(acc[i], pl, h0, h1);
+                    mma8(acc[i], ph, l0, l1);
+                    mma8(acc[i], ph, h0, h1);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w.o[4 * j + i][e] = fmaf(w.o[4 * j + i][e], al[e >> 1], acc[i][e]);
+        }
+    }
+}
+
+// Joins the rows of the warps that share them (the upper half gives, the
+// lower half takes, twice with four), then the first writes the item's
+// partial result.  buf: two warps' outputs.
+template <typename T, int HD, int RW>
+__device__ __forceinline__ void beam_flush(const BeamAttnArgs &a, const BeamAttnPlan &p, const BeamCursor &c,
+                                           BeamRows<T, HD> &w, float *buf) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rg = warp % RW, kg = warp / RW;
+    const uint32_t g = lane >> 2, t = lane & 3;
+    float2 *bml = reinterpret_cast<float2 *>(buf + 2 * 16 * HD);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        w.l[h] += __shfl_xor_sync(0xffffffffu, w.l[h], 1);
+        w.l[h] += __shfl_xor_sync(0xffffffffu, w.l[h], 2);
+    }
+#pragma unroll
+    for (int half = 4 / RW / 2; half >= 1; half >>= 1) {
+        const uint32_t at = (kg % half) * RW + rg;
+        float *ob = buf + at * 16 * HD;
+        if (kg >= half && kg < 2 * half) {
+#pragma unroll
+            for (int j = 0; j < HD / 8; ++j)
+                *reinterpret_cast<float4 *>(ob + (j * 32 + lane) * 4) =
+                    make_float4(w.o[j][0], w.o[j][1], w.o[j][2], w.o[j][3]);
+            if (t == 0) {
+                bml[at * 16 + g] = make_float2(w.m[0], w.l[0]);
+                bml[at * 16 + g + 8] = make_float2(w.m[1], w.l[1]);
+            }
+        }
+        __syncthreads();
+        if (kg < half) {
+            float mine[2], other[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float2 ml = bml[at * 16 + g + 8 * h];
+                const float mn = fmaxf(w.m[h], ml.x), safe = mn == -INFINITY ? 0.f : mn;
+                mine[h] = exp2_fast(w.m[h] - safe);
+                other[h] = exp2_fast(ml.x - safe);
+                w.m[h] = mn;
+                w.l[h] = w.l[h] * mine[h] + ml.y * other[h];
+            }
+#pragma unroll
+            for (int j = 0; j < HD / 8; ++j) {
+                const float4 v = *reinterpret_cast<const float4 *>(ob + (j * 32 + lane) * 4);
+                w.o[j][0] = w.o[j][0] * mine[0] + v.x * other[0];
+                w.o[j][1] = w.o[j][1] * mine[0] + v.y * other[0];
+                w.o[j][2] = w.o[j][2] * mine[1] + v.z * other[1];
+                w.o[j][3] = w.o[j][3] * mine[1] + v.w * other[1];
+            }
+        }
+        __syncthreads();
+    }
+    if (kg == 0) {
+        const bool pre = c.part < a.n_group;
+        const uint32_t item = ((pre ? c.part : c.part - a.n_group) * a.n_kv + c.kvh) * (pre ? p.ptiles : p.stiles) + c.tile;
+        const size_t row = (size_t)(item + blockIdx.x) * (pre ? p.prow : p.srow) + rg * 16;
+        float *o = (pre ? p.po : p.so) + row * HD;
+        float2 *ml = (pre ? p.pml : p.sml) + row;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (w.lim[h] < 0) continue;  // no such row
+            float *r = o + (size_t)(g + 8 * h) * HD;
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int j = 0; j < HD / 8; ++j)
+                    *reinterpret_cast<float2 *>(r + 8 * j + 2 * t) = make_float2(w.o[j][2 * h], w.o[j][2 * h + 1]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < HD / 32; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        *reinterpret_cast<float4 *>(r + 32 * j + 8 * t + 4 * e) =
+                            make_float4(w.o[4 * j][2 * h + e], w.o[4 * j + 1][2 * h + e], w.o[4 * j + 2][2 * h + e],
+                                        w.o[4 * j + 3][2 * h + e]);
+            }
+            if (t == 0) ml[g + 8 * h] = make_float2(w.m[h], w.l[h]);
+        }
+    }
+}
+
+// The positions of the cursor's next tile: within the item and this CTA's units.
+template <typename T, int HD>
+__device__ __forceinline__ uint32_t beam_take(const BeamCursor &c) {
+    return min(min((uint32_t)BeamTile<T, HD>::kKeys, c.len - c.pos), c.left * kBaUnit);
+}
+__device__ __forceinline__ void beam_advance(BeamCursor &c, uint32_t n) {
+    c.pos += n;
+    c.left -= (n + kBaUnit - 1) / kBaUnit;
+}
+
+// One segment: the tiles of one item that this CTA takes.  RW warps hold the
+// row groups of 16, and 4 / RW warps share each tile's positions.
+template <typename T, int HD, int RW>
+__device__ __forceinline__ void beam_segment(const BeamAttnArgs &a, const BeamAttnPlan &p, BeamCursor &c,
+                                             BeamCursor &ahead, uint32_t smem, float *buf, uint32_t &stage,
+                                             uint32_t &astage) {
+    using Tl = BeamTile<T, HD>;
+    constexpr int KW = Tl::kKeys / (4 / RW);
+    const uint32_t warp = threadIdx.x >> 5, rg = warp % RW, kg = warp / RW;
+    const BeamCursor seg = c;
+    BeamRows<T, HD> w;
+    beam_rows_init<T, HD>(a, seg, seg.tile * RW * 16 + rg * 16, w);
+    const uint32_t end = min(seg.len, seg.pos + seg.left * kBaUnit);
+    const float sl2 = a.scale * 1.4426950408889634f;
+    const bool some = __any_sync(0xffffffffu, w.lim[0] >= 0 || w.lim[1] >= 0);
+    while (c.pos < end) {
+        cp_async_wait<kBaStages - 2>();
+        __syncthreads();  // the tile is there for all, and the stage that is filled next is free
+        if (ahead.left) {
+            const uint32_t n = beam_take<T, HD>(ahead);
+            beam_load<T, HD>(a, ahead, n, smem + astage * 2 * Tl::kBytes);
+            beam_advance(ahead, n);
+            if (ahead.left && ahead.pos >= ahead.len) beam_next_item(a, p, ahead);
+            astage = astage + 1 == kBaStages ? 0 : astage + 1;
+        }
+        cp_async_commit();
+        const uint32_t ks = smem + stage * 2 * Tl::kBytes;
+        const uint32_t n = beam_take<T, HD>(c);
+        if (some && kg * KW < n) beam_tile<T, HD, KW>(w, ks, ks + Tl::kBytes, kg * KW, c.pos, end, sl2);
+        beam_advance(c, n);
+        stage = stage + 1 == kBaStages ? 0 : stage + 1;
+    }
+    beam_flush<T, HD, RW>(a, p, seg, w, buf);
+    if (threadIdx.x == 0) {
+        const bool pre = seg.part < a.n_group;
+        const uint32_t item = ((pre ? seg.part : seg.part - a.n_group) * a.n_kv + seg.kvh) * (pre ? p.ptiles : p.stiles) + seg.tile;
+        uint2 *cta = (pre ? p.pcta : p.scta) + item;
+        if (seg.pos == 0) cta->x = blockIdx.x;
+        if (end == seg.len) cta->y = blockIdx.x;
+    }
+    if (c.left) beam_next_item(a, p, c);
+}
+
+// RWP, RWS: row groups of 16 of a prefix / suffix tile.
+template <typename T, int HD, int RWP, int RWS>
+__global__ void __launch_bounds__(kBaThreads, 2) beam_attn_kernel(BeamAttnArgs a, BeamAttnPlan p) {
+    using Tl = BeamTile<T, HD>;
+    extern __shared__ __align__(128) uint8_t beam_smem[];
+    const uint32_t smem = smem_u32(beam_smem);
+    float *buf = reinterpret_cast<float *>(beam_smem + 2 * Tl::kBytes * kBaStages);
+    BeamCursor c;
+    if (!beam_first(a, p, c)) return;
+    if (a.hd < HD) {  // the padding of the heads
+        for (uint32_t i = threadIdx.x; i < 2 * Tl::kBytes * kBaStages / 16; i += kBaThreads)
+            reinterpret_cast<uint4 *>(beam_smem)[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+    }
+    BeamCursor ahead = c;
+    uint32_t stage = 0, astage = 0;
+#pragma unroll
+    for (int i = 0; i < kBaStages - 1; ++i) {
+        if (ahead.left) {
+            const uint32_t n = beam_take<T, HD>(ahead);
+            beam_load<T, HD>(a, ahead, n, smem + astage * 2 * Tl::kBytes);
+            beam_advance(ahead, n);
+            if (ahead.left && ahead.pos >= ahead.len) beam_next_item(a, p, ahead);
+            ++astage;
+        }
+        cp_async_commit();
+    }
+    if (astage == kBaStages) astage = 0;
+    while (c.left) {
+        if (RWP == RWS || c.part < a.n_group)
+            beam_segment<T, HD, RWP>(a, p, c, ahead, smem, buf, stage, astage);
+        else
+            beam_segment<T, HD, RWS>(a, p, c, ahead, smem, buf, stage, astage);
+    }
+    cp_async_wait<0>();
+}
+
+// Joins a row's partial results: block (row, head), the warps take the
+// segments in turn, lanes the dimensions.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kBaThreads) beam_attn_join_kernel(BeamAttnArgs a, BeamAttnPlan p) {
+    constexpr int NW = kBaThreads / 32, V = HD / 32;
+    __shared__ float part[NW][HD], pm[NW], pl[NW];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t h = blockIdx.y, kvh = h / a.gq, hg = h % a.gq;
+    const uint32_t s = blockIdx.x / a.n_query, t = blockIdx.x % a.n_query, grp = s / a.n_beam;
+    const uint32_t pr = ((s % a.n_beam) * a.n_query + t) * a.gq + hg, sr = t * a.gq + hg;
+    const uint32_t pi = (grp * a.n_kv + kvh) * p.ptiles + pr / p.prow, si = (s * a.n_kv + kvh) * p.stiles + sr / p.srow;
+    uint2 pc = make_uint2(1, 0), sc = make_uint2(1, 0);
+    if (beam_part_len(a, grp)) pc = p.pcta[pi];
+    if (beam_part_len(a, a.n_group + s)) sc = p.scta[si];
+    const uint32_t np = pc.y + 1 - pc.x, n = np + (sc.y + 1 - sc.x);
+    float m = -INFINITY, l = 0.f, o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = 0.f;
+    for (uint32_t j = warp; j < n; j += NW) {
+        const size_t row = j < np ? (size_t)(pi + pc.x + j) * p.prow + pr % p.prow
+                                  : (size_t)(si + sc.x + j - np) * p.srow + sr % p.srow;
+        const float2 ml = (j < np ? p.pml : p.sml)[row];
+        const float *src = (j < np ? p.po : p.so) + row * HD + lane;
+        const float mn = fmaxf(m, ml.x), safe = mn == -INFINITY ? 0.f : mn;
+        const float mine = exp2_fast(m - safe), other = exp2_fast(ml.x - safe);
+        m = mn;
+        l = l * mine + ml.y * other;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = o[i] * mine + src[32 * i] * other;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) part[warp][lane + 32 * i] = o[i];
     if (lane == 0) { pm[warp] = m; pl[warp] = l; }
     __syncthreads();
     float M = -INFINITY, L = 0.f;
+#pragma unroll
     for (int w = 0; w < NW; ++w) M = fmaxf(M, pm[w]);
-    for (int w = 0; w < NW; ++w) L += pm[w] == -INFINITY ? 0.f : pl[w] * expf(pm[w] - M);
-    const size_t at = (size_t)row * a.n_head + h;
-    for (uint32_t d = threadIdx.x; d < a.hd; d += kBaThreads) {
-        float v = 0.f;
-        for (int w = 0; w < NW; ++w) v += pm[w] == -INFINITY ? 0.f : part[w][d] * expf(pm[w] - M);
-        static_cast<T *>(a.out)[at * a.hd + d] = beam_from_f32<T>(L > 0.f ? v / L : 0.f);
+    const float safe = M == -INFINITY ? 0.f : M;
+    const uint32_t d = threadIdx.x;
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+        const float f = exp2_fast(pm[w] - safe);
+        L += pl[w] * f;
+        if (d < HD) v += part[w][d] * f;
     }
-    if (a.lse && threadIdx.x == 0) a.lse[at] = L > 0.f ? M + logf(L) : -INFINITY;
+    const size_t at = (size_t)blockIdx.x * a.n_head + h;
+    if (d < a.hd) static_cast<T *>(a.out)[at * a.hd + d] = beam_from_f32<T>(L == 0.f ? 0.f : v / L);
+    if (a.lse && d == 0) a.lse[at] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
 }  // namespace fwb

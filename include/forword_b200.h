@@ -159,7 +159,7 @@ typedef struct fwb_prefix_attn {
     uint32_t n_head, n_head_kv;        /* n_head a multiple of n_head_kv */
     uint32_t head_dim;                 /* a multiple of 16, at most 128 */
     uint32_t prefix_cap, suffix_cap;   /* positions that the caches hold (0: none) */
-    float scale;                       /* of the scores; 0 -> 1/sqrt(head_dim) */
+    float scale;                       /* of the scores, positive; 0 -> 1/sqrt(head_dim) */
     const void *q;                     /* [n_seq][n_query][n_head][head_dim] */
     uint64_t q_seq_stride, q_token_stride, q_head_stride;
     const void *prefix_k, *prefix_v;   /* [n_group][n_head_kv][prefix_cap][head_dim] */
