@@ -177,7 +177,7 @@ bool run_attn(const BeamAttnArgs &k, const AttnLayout &L, uint8_t *ws, cudaStrea
 }
 
 // --- selection ------------------------------------------------------------------
-constexpr size_t kMaxSelect = 128, kMaxSelectBeams = 64;
+constexpr size_t kMaxSelect = kBsMaxSelect, kMaxSelectBeams = kBsMaxBeams;
 
 bool select_sizes_ok(uint32_t type, size_t n_group, size_t n_beam, size_t n_vocab, size_t n_select) {
     if (!elem_bytes(type)) return fail("fwb_beam_select: type must be 0 (F32), 1 (F16) or 30 (BF16)");
@@ -185,16 +185,53 @@ bool select_sizes_ok(uint32_t type, size_t n_group, size_t n_beam, size_t n_voca
         return fail("fwb_beam_select: zero groups, beams, tokens or selected entries");
     if (n_beam > kMaxSelectBeams || n_group > 0x7fffffffu / kMaxSelectBeams || n_vocab > 0x7fffffffu / n_beam)
         return fail("fwb_beam_select: more than 64 beams, or more than 2^31 - 1 scores in a group");
+    if (n_group * n_beam > (size_t)0x7fffffff / (n_vocab / 2048 + 1))
+        return fail("fwb_beam_select: too many rows");
     if (n_select > kMaxSelect || n_select > n_beam * n_vocab)
         return fail("fwb_beam_select: n_select must be at most 128 and at most n_beam * n_vocab");
     return true;
 }
 
-size_t select_workspace() { return 16; }
+// The chunks of a row and the workspace's layout.  A block holds 8, 32 or 64
+// logits per thread: the largest chunk that still makes two blocks per SM.
+struct SelectLayout {
+    uint32_t per_thread, n_chunk, chunk, cap;
+    size_t cand, count, stat, bytes;
+};
+
+void select_layout(size_t n_group, size_t n_beam, size_t n_vocab, size_t n_select, SelectLayout &L) {
+    const size_t rows = n_group * n_beam;
+    for (uint32_t e : {64u, 32u, 8u}) {
+        L.per_thread = e;
+        L.n_chunk = (uint32_t)((n_vocab + e * kBsThreads - 1) / (e * kBsThreads));
+        if (rows * L.n_chunk >= 2 * device_sms()) break;
+    }
+    L.chunk = (uint32_t)(((n_vocab + L.n_chunk - 1) / L.n_chunk + 7) / 8 * 8);
+    L.n_chunk = (uint32_t)((n_vocab + L.chunk - 1) / L.chunk);
+    L.cap = (uint32_t)(2 * n_select + 32);
+    const size_t lists = rows * L.n_chunk;
+    L.cand = 0;
+    L.count = (lists * L.cap * sizeof(float2) + 255) & ~(size_t)255;
+    L.stat = L.count + ((lists * 4 + 255) & ~(size_t)255);
+    L.bytes = L.stat + lists * sizeof(float2);
+}
+
+template <typename T, int E>
+void launch_chunks(const BeamSelectArgs &k, bool vec, cudaStream_t st) {
+    const uint32_t grid = k.n_group * k.n_beam * k.n_chunk;
+    if (vec) beam_select_chunk_kernel<T, E, true><<<grid, kBsThreads, 0, st>>>(k);
+    else beam_select_chunk_kernel<T, E, false><<<grid, kBsThreads, 0, st>>>(k);
+}
 
 template <typename T>
-bool run_select(const BeamSelectArgs &k, cudaStream_t st) {
-    beam_select_passes_kernel<T><<<k.n_group, kBsThreads, 0, st>>>(k);
+bool run_select(const BeamSelectArgs &k, uint32_t per_thread, cudaStream_t st) {
+    // 16-byte loads when every row allows them (not row by row: rows with equal
+    // logits must have equal sums)
+    const bool vec = ((uintptr_t)k.logits | k.row_stride * sizeof(T)) % 16 == 0;
+    if (per_thread == 64) launch_chunks<T, 64>(k, vec, st);
+    else if (per_thread == 32) launch_chunks<T, 32>(k, vec, st);
+    else launch_chunks<T, 8>(k, vec, st);
+    beam_select_join_kernel<<<k.n_group, kBsJoinThreads, 0, st>>>(k);
     return launched(cudaGetLastError(), "fwb_beam_select launch");
 }
 
@@ -239,7 +276,10 @@ int fwb_prefix_attention_dev(const fwb_prefix_attn_t *a, void *workspace, size_t
 }
 
 size_t fwb_beam_select_workspace(uint32_t type, size_t n_group, size_t n_beam, size_t n_vocab, size_t n_select) {
-    return select_sizes_ok(type, n_group, n_beam, n_vocab, n_select) ? select_workspace() : 0;
+    SelectLayout L;
+    if (!select_sizes_ok(type, n_group, n_beam, n_vocab, n_select)) return 0;
+    select_layout(n_group, n_beam, n_vocab, n_select, L);
+    return L.bytes;
 }
 
 int fwb_beam_select_dev(const void *d_logits, uint32_t type, size_t n_group, size_t n_beam, size_t n_vocab,
@@ -256,7 +296,9 @@ int fwb_beam_select_dev(const void *d_logits, uint32_t type, size_t n_group, siz
         fail("fwb_beam_select: misaligned pointer");
         return -1;
     }
-    if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < select_workspace()) {
+    SelectLayout L;
+    select_layout(n_group, n_beam, n_vocab, n_select, L);
+    if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < L.bytes) {
         fail("fwb_beam_select: workspace missing, misaligned or smaller than fwb_beam_select_workspace");
         return -1;
     }
@@ -266,9 +308,15 @@ int fwb_beam_select_dev(const void *d_logits, uint32_t type, size_t n_group, siz
     k.row_stride = row_stride;
     k.n_group = (uint32_t)n_group; k.n_beam = (uint32_t)n_beam; k.n_vocab = (uint32_t)n_vocab;
     k.n_select = (uint32_t)n_select;
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    k.cand = reinterpret_cast<float2 *>(ws + L.cand);
+    k.count = reinterpret_cast<uint32_t *>(ws + L.count);
+    k.stat = reinterpret_cast<float2 *>(ws + L.stat);
+    k.n_chunk = L.n_chunk; k.chunk = L.chunk; k.cap = L.cap;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool ok = type == 0 ? run_select<float>(k, st)
-                  : type == 1 ? run_select<__half>(k, st) : run_select<__nv_bfloat16>(k, st);
+    const bool ok = type == 0 ? run_select<float>(k, L.per_thread, st)
+                  : type == 1 ? run_select<__half>(k, L.per_thread, st)
+                              : run_select<__nv_bfloat16>(k, L.per_thread, st);
     return ok ? 0 : -1;
 }
 

@@ -392,6 +392,11 @@ __device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t ks, uint3
                 mma16(sc[2 * j + 1], w.q + 4 * k, b[2], b[3], T{});
             }
     } else {
+        float lo[KW / 8][4];
+#pragma unroll
+        for (int j = 0; j < KW / 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) lo[j][e] = 0.f;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
             uint32_t ah[8], al[8];
@@ -407,14 +412,25 @@ __device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t ks, uint3
                 tf32_split(v.y, bh[1], bl[1]);
                 tf32_split(v.z, bh[2], bl[2]);
                 tf32_split(v.w, bh[3], bl[3]);
+                // The tensor cores' fp32 sums truncate: the large products are
+                // summed from zero over 16 dimensions and added with one
+                // rounded addition; the small ones, 2^-11 of them, in their
+                // own sum.
+                float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int s = 0; s < 2; ++s) {  // the small products first
-                    mma8(sc[j], al + 4 * s, bh[2 * s], bh[2 * s + 1]);
-                    mma8(sc[j], ah + 4 * s, bl[2 * s], bl[2 * s + 1]);
-                    mma8(sc[j], ah + 4 * s, bh[2 * s], bh[2 * s + 1]);
+                for (int s = 0; s < 2; ++s) {
+                    mma8(lo[j], al + 4 * s, bh[2 * s], bh[2 * s + 1]);
+                    mma8(lo[j], ah + 4 * s, bl[2 * s], bl[2 * s + 1]);
+                    mma8(acc, ah + 4 * s, bh[2 * s], bh[2 * s + 1]);
                 }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[j][e] += acc[e];
             }
         }
+#pragma unroll
+        for (int j = 0; j < KW / 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[j][e] += lo[j][e];
     }
     // positions that a row does not see
     const uint32_t first = at + k0, lim0 = min((uint32_t)w.lim[0], end), lim1 = min((uint32_t)w.lim[1], end);
@@ -451,9 +467,8 @@ __device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t ks, uint3
             }
         }
     } else {
-        // The tensor cores' fp32 sums truncate: a tile's products are summed
-        // from zero and added to the output with one rounded fma, the rescaling
-        // in the same instruction.
+        // Again from zero for each tile, added to the output with one rounded
+        // fma that does the rescaling too.
 #pragma unroll
         for (int j = 0; j < HD / 32; ++j) {
             float acc[4][4];
