@@ -26,6 +26,25 @@ bool launched(cudaError_t e, const char *who) {
     return fail(b);
 }
 
+// A kernel whose blocks may be placed while the stream's kernel before it
+// ends (it waits for that one's results itself).
+template <typename F, typename... A>
+cudaError_t launch_after(F *fn, dim3 grid, unsigned threads, unsigned cluster, cudaStream_t st, const A &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, fn, args...);
+}
+
 uint32_t elem_bytes(uint32_t type) { return type == 0 ? 4u : type == 1 || type == 30 ? 2u : 0u; }
 
 // --- prefix attention --------------------------------------------------------
@@ -185,54 +204,58 @@ bool select_sizes_ok(uint32_t type, size_t n_group, size_t n_beam, size_t n_voca
         return fail("fwb_beam_select: zero groups, beams, tokens or selected entries");
     if (n_beam > kMaxSelectBeams || n_group > 0x7fffffffu / kMaxSelectBeams || n_vocab > 0x7fffffffu / n_beam)
         return fail("fwb_beam_select: more than 64 beams, or more than 2^31 - 1 scores in a group");
-    if (n_group * n_beam > (size_t)0x7fffffff / (n_vocab / 2048 + 1))
+    if (n_group * n_beam > (size_t)0x7fffffff / (n_vocab / 2048 + 2))
         return fail("fwb_beam_select: too many rows");
     if (n_select > kMaxSelect || n_select > n_beam * n_vocab)
         return fail("fwb_beam_select: n_select must be at most 128 and at most n_beam * n_vocab");
     return true;
 }
 
-// The chunks of a row and the workspace's layout.  A block holds 8, 32 or 64
-// logits per thread: the largest chunk that still makes two blocks per SM.
+// The parts of a row and the workspace's layout.  A piece is what a block
+// holds in registers: 16 logits per thread, 8 when the rows are few.
 struct SelectLayout {
-    uint32_t per_thread, n_chunk, chunk, cap;
-    size_t cand, count, stat, bytes;
+    bool small;
+    uint32_t n_part, part, cap;
+    size_t cand, stat, bytes;
 };
 
 void select_layout(size_t n_group, size_t n_beam, size_t n_vocab, size_t n_select, SelectLayout &L) {
-    const size_t rows = n_group * n_beam;
-    for (uint32_t e : {64u, 32u, 8u}) {
-        L.per_thread = e;
-        L.n_chunk = (uint32_t)((n_vocab + e * kBsThreads - 1) / (e * kBsThreads));
-        if (rows * L.n_chunk >= 2 * device_sms()) break;
-    }
-    L.chunk = (uint32_t)(((n_vocab + L.n_chunk - 1) / L.n_chunk + 7) / 8 * 8);
-    L.n_chunk = (uint32_t)((n_vocab + L.chunk - 1) / L.chunk);
-    L.cap = (uint32_t)(2 * n_select + 32);
-    const size_t lists = rows * L.n_chunk;
+    const size_t rows = n_group * n_beam, piece = 16 * kBsThreads;
+    // about four blocks per SM, of one to four pieces
+    const size_t even = rows * n_vocab / (4 * device_sms());
+    L.small = even < piece;
+    const size_t want = L.small ? piece / 2 : std::min(4 * piece, even / piece * piece);
+    L.n_part = (uint32_t)((n_vocab + want - 1) / want);
+    L.part = (uint32_t)(((n_vocab + L.n_part - 1) / L.n_part + 7) / 8 * 8);
+    L.n_part = (uint32_t)((n_vocab + L.part - 1) / L.part);
+    L.cap = (uint32_t)((n_select + n_select / 2 + 8 + 31) / 32 * 32);
+    const size_t lists = rows * L.n_part;
     L.cand = 0;
-    L.count = (lists * L.cap * sizeof(float2) + 255) & ~(size_t)255;
-    L.stat = L.count + ((lists * 4 + 255) & ~(size_t)255);
+    L.stat = (lists * L.cap * sizeof(float2) + 255) & ~(size_t)255;
     L.bytes = L.stat + lists * sizeof(float2);
 }
 
 template <typename T, int E>
-void launch_chunks(const BeamSelectArgs &k, bool vec, cudaStream_t st) {
-    const uint32_t grid = k.n_group * k.n_beam * k.n_chunk;
-    if (vec) beam_select_chunk_kernel<T, E, true><<<grid, kBsThreads, 0, st>>>(k);
-    else beam_select_chunk_kernel<T, E, false><<<grid, kBsThreads, 0, st>>>(k);
+void launch_parts(const BeamSelectArgs &k, bool vec, cudaStream_t st) {
+    const uint32_t grid = k.n_group * k.n_beam * k.n_part;
+    if (vec) beam_select_part_kernel<T, E, true><<<grid, kBsThreads, 0, st>>>(k);
+    else beam_select_part_kernel<T, E, false><<<grid, kBsThreads, 0, st>>>(k);
 }
 
 template <typename T>
-bool run_select(const BeamSelectArgs &k, uint32_t per_thread, cudaStream_t st) {
+bool run_select(const BeamSelectArgs &k, bool small, cudaStream_t st) {
     // 16-byte loads when every row allows them (not row by row: rows with equal
     // logits must have equal sums)
     const bool vec = ((uintptr_t)k.logits | k.row_stride * sizeof(T)) % 16 == 0;
-    if (per_thread == 64) launch_chunks<T, 64>(k, vec, st);
-    else if (per_thread == 32) launch_chunks<T, 32>(k, vec, st);
-    else launch_chunks<T, 8>(k, vec, st);
-    beam_select_join_kernel<<<k.n_group, kBsJoinThreads, 0, st>>>(k);
-    return launched(cudaGetLastError(), "fwb_beam_select launch");
+    if (small) launch_parts<T, 8>(k, vec, st);
+    else launch_parts<T, 16>(k, vec, st);
+    if (!launched(cudaGetLastError(), "fwb_beam_select launch")) return false;
+    // as many blocks per group as have a batch of slices for every warp
+    const uint64_t batches = ((uint64_t)k.n_beam * k.n_part * (k.cap / 32) + 31) / 32;
+    uint32_t cluster = 1;
+    while (cluster < kBsJoinCluster && cluster < batches) cluster *= 2;
+    return launched(launch_after(beam_select_join_kernel, dim3(k.n_group * cluster), kBsJoinThreads, cluster, st, k),
+                    "fwb_beam_select launch");
 }
 
 // --- reordering -------------------------------------------------------------------
@@ -310,13 +333,12 @@ int fwb_beam_select_dev(const void *d_logits, uint32_t type, size_t n_group, siz
     k.n_select = (uint32_t)n_select;
     uint8_t *ws = static_cast<uint8_t *>(workspace);
     k.cand = reinterpret_cast<float2 *>(ws + L.cand);
-    k.count = reinterpret_cast<uint32_t *>(ws + L.count);
     k.stat = reinterpret_cast<float2 *>(ws + L.stat);
-    k.n_chunk = L.n_chunk; k.chunk = L.chunk; k.cap = L.cap;
+    k.n_part = L.n_part; k.part = L.part; k.cap = L.cap;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool ok = type == 0 ? run_select<float>(k, L.per_thread, st)
-                  : type == 1 ? run_select<__half>(k, L.per_thread, st)
-                              : run_select<__nv_bfloat16>(k, L.per_thread, st);
+    const bool ok = type == 0 ? run_select<float>(k, L.small, st)
+                  : type == 1 ? run_select<__half>(k, L.small, st)
+                              : run_select<__nv_bfloat16>(k, L.small, st);
     return ok ? 0 : -1;
 }
 

@@ -11,21 +11,25 @@
 // its scores are -inf.
 //
 // The logits are read once.  Within a row the scores order as the logits do,
-// so a chunk's candidates need no lse: a first kernel takes each row in
-// chunks that one block holds in registers, writes the chunk's maximum and
-// sum of exponentials and every logit that can be among the row's best; a
-// second kernel (one block per group) joins the sums, scores the candidates
-// and ranks them.  Scores rank in 64 bits, so that logits of one row never
-// tie by rounding.
+// so the candidates of a part of a row need no lse: a first kernel streams
+// parts of rows, keeping the running maximum and sum of exponentials per
+// thread and the logits that can still be among the part's best; a second
+// kernel (one block per group) joins the sums, scores the candidates and
+// ranks them.  Scores rank in 64 bits, so that logits of one row never tie by
+// rounding.
 #pragma once
+#include <cooperative_groups.h>
+
 #include "beam_attn.cuh"
 
 namespace fwb {
 
-constexpr int kBsThreads = 256;       // of a chunk's block
-constexpr int kBsJoinThreads = 512;
+constexpr int kBsThreads = 256;       // of a part's block
+constexpr int kBsJoinThreads = 256;
+constexpr uint32_t kBsJoinCluster = 8;  // most blocks of a group's join
 constexpr uint32_t kBsMaxSelect = 128, kBsMaxBeams = 64;
-constexpr uint32_t kBsPool = 1024;    // candidates that the second kernel ranks
+constexpr uint32_t kBsList = 1024;    // candidates that a block of the first kernel holds
+constexpr uint32_t kBsPool = 2048;    // candidates that the second kernel ranks
 
 struct BeamSelectArgs {
     const void *logits;     // [n_group * n_beam] rows, row_stride elements apart
@@ -34,36 +38,45 @@ struct BeamSelectArgs {
     int32_t *parent, *token;
     uint64_t row_stride;
     uint32_t n_group, n_beam, n_vocab, n_select;
-    // workspace: per chunk (row-major [row][chunk]) its candidates (logit,
-    // token), their number, and (maximum, sum of exp(x - maximum))
+    // workspace: per part (row-major [row][part]) `cap` candidates (logit,
+    // token; a NaN logit in unused places) and (b, sum of 2^(x log2(e) - b))
     float2 *cand;
-    uint32_t *count;
     float2 *stat;
-    uint32_t n_chunk, chunk, cap;
+    uint32_t n_part, part, cap;
 };
 
-// Orders like the float, as an unsigned integer (NaN is not passed).
+// Orders like the float, as an unsigned integer (NaN is not passed; -0 and 0
+// are equal).
 __device__ __forceinline__ uint32_t beam_order(float v) {
-    const uint32_t b = __float_as_uint(v);
+    const uint32_t b = __float_as_uint(v + 0.f);
     return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float beam_unorder(uint32_t u) {
+    return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 constexpr uint32_t kBsNone = 0x007fffffu;  // beam_order(-inf): entries at or below it are no candidates
 
 // A value t such that at least `want` of the block's N values in `vals`
 // (beam_order of each thread's best) are >= t, and few more; kBsNone + 1 if
-// not as many are above kBsNone.  One warp; bisection that stops at up to
-// want / 2 + 8 too many.
+// not as many are above kBsNone.  One warp; bisection between the least and
+// the largest value that stops at up to want / 2 + 8 too many.
 template <int N>
 __device__ __forceinline__ uint32_t beam_threshold(const uint32_t *vals, uint32_t want) {
     const uint32_t lane = threadIdx.x & 31;
-    uint32_t v[N / 32], top = 0;
+    uint32_t v[N / 32], top = 0, least = 0xffffffffu, some = 0;
 #pragma unroll
     for (int i = 0; i < N / 32; ++i) {
         v[i] = vals[32 * i + lane];
         top = max(top, v[i]);
+        if (v[i] > kBsNone) {
+            least = min(least, v[i]);
+            ++some;
+        }
     }
     top = __reduce_max_sync(0xffffffffu, top);
-    uint32_t lo = kBsNone + 1, hi = top;  // count(lo) >= want, or all there is
+    least = __reduce_min_sync(0xffffffffu, least);
+    if (__reduce_add_sync(0xffffffffu, some) < want) return kBsNone + 1;
+    uint32_t lo = least, hi = top;  // count(lo) >= want
     while (lo < hi) {
         const uint32_t mid = lo + (hi - lo + 1) / 2;
         uint32_t n = 0;
@@ -80,207 +93,412 @@ __device__ __forceinline__ uint32_t beam_threshold(const uint32_t *vals, uint32_
     return lo;
 }
 
+// A piece: E logits of each thread, 16 bytes at a time (VEC) or one.
 template <typename T, int E, bool VEC>
-__device__ __forceinline__ void beam_load_chunk(const T *x, uint32_t n, float *v) {
-    constexpr int PV = VEC ? 16 / (int)sizeof(T) : 1;  // elements per load
+struct BeamPiece {
+    static constexpr int PV = VEC ? 16 / (int)sizeof(T) : 1;  // elements per load
+    static __device__ __forceinline__ uint32_t at(int e) { return ((e / PV) * kBsThreads + threadIdx.x) * PV + e % PV; }
+    // x: the piece's first logit; n: logits from there on, the rest -inf
+    static __device__ __forceinline__ void load(const T *x, uint32_t n, float *v) {
+        if (n >= E * kBsThreads) {
+            if constexpr (VEC) {
+                uint4 raw[E / PV];
 #pragma unroll
-    for (int i = 0; i < E / PV; ++i) {
-        const uint32_t at = (i * kBsThreads + threadIdx.x) * PV;
-        if constexpr (VEC) {
-            uint4 raw = make_uint4(0, 0, 0, 0);
-            if (at + PV <= n) raw = __ldcs(reinterpret_cast<const uint4 *>(x + at));
-            else if (at < n) {
-                T *part = reinterpret_cast<T *>(&raw);
-                for (int e = 0; e < PV; ++e)
-                    if (at + e < n) part[e] = x[at + e];
+                for (int i = 0; i < E / PV; ++i) raw[i] = __ldcs(reinterpret_cast<const uint4 *>(x + at(i * PV)));
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = beam_to_f32(reinterpret_cast<const T *>(&raw[e / PV])[e % PV]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < E; ++e) v[e] = beam_to_f32(x[at(e)]);
             }
-            const T *e16 = reinterpret_cast<const T *>(&raw);
-#pragma unroll
-            for (int e = 0; e < PV; ++e) v[i * PV + e] = at + e < n ? beam_to_f32(e16[e]) : -INFINITY;
         } else {
-            v[i] = at < n ? beam_to_f32(x[at]) : -INFINITY;
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[e] = at(e) < n ? beam_to_f32(x[at(e)]) : -INFINITY;
         }
+    }
+};
+
+// The candidates that a block has gathered so far.
+struct BeamList {
+    float x[kBsList];
+    uint32_t tok[kBsList];
+    uint32_t n, thr;
+    uint32_t best[kBsThreads];
+    uint64_t key[kBsThreads / 32];
+};
+
+// Raises thr to about the n_select-th best of the list and drops what is
+// below; a list that equal logits keep long is cut to exactly n_select (the
+// pieces come in the order of the tokens, so later equals cannot displace
+// them, and thr excludes these).  The whole block.
+__device__ __forceinline__ void beam_trim(BeamList &l, uint32_t want) {
+    constexpr uint32_t PT = kBsList / kBsThreads;
+    const uint32_t n = min(l.n, kBsList);
+    float x[PT];
+    uint32_t tok[PT];
+#pragma unroll
+    for (uint32_t i = 0; i < PT; ++i) {
+        const uint32_t j = i * kBsThreads + threadIdx.x;
+        x[i] = j < n ? l.x[j] : -INFINITY;
+        tok[i] = j < n ? l.tok[j] : 0;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < PT; ++i)  // the list's own memory, as ordered integers, for the search
+        reinterpret_cast<uint32_t *>(l.x)[i * kBsThreads + threadIdx.x] = x[i] == -INFINITY ? 0u : beam_order(x[i]);
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const uint32_t thr = beam_threshold<kBsList>(reinterpret_cast<const uint32_t *>(l.x), want);
+        if (threadIdx.x == 0) {
+            l.thr = max(l.thr, thr);
+            l.n = 0;
+        }
+    }
+    __syncthreads();
+    const uint32_t thr = l.thr;
+#pragma unroll
+    for (uint32_t i = 0; i < PT; ++i)
+        if (x[i] > -INFINITY && beam_order(x[i]) >= thr) {
+            const uint32_t at = atomicAdd(&l.n, 1);
+            l.x[at] = x[i];
+            l.tok[at] = tok[i];
+        }
+    __syncthreads();
+    const uint32_t kept = l.n;
+    if (kept <= kBsList / 2) return;
+    uint32_t rank[PT];
+#pragma unroll
+    for (uint32_t i = 0; i < PT; ++i) {
+        const uint32_t j = i * kBsThreads + threadIdx.x;
+        rank[i] = kept;
+        if (j < kept) {
+            x[i] = l.x[j];
+            tok[i] = l.tok[j];
+            rank[i] = 0;
+            for (uint32_t k = 0; k < kept; ++k) rank[i] += l.x[k] > x[i] || (l.x[k] == x[i] && l.tok[k] < tok[i]);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < PT; ++i)
+        if (rank[i] < want) {
+            l.x[rank[i]] = x[i];
+            l.tok[rank[i]] = tok[i];
+            if (rank[i] == want - 1) {
+                l.n = want;
+                l.thr = max(l.thr, beam_order(x[i]) + 1);
+            }
+        }
+    __syncthreads();
+}
+
+// The n_select best of a piece (more than that many) behind the first `old`
+// entries of the list, one after the other, read from memory again.  The
+// whole block.
+template <typename T>
+__device__ __noinline__ void beam_take_best(BeamList &l, const T *x, uint32_t n, uint32_t tok0, uint32_t old,
+                                            uint32_t want) {
+    constexpr uint32_t NW = kBsThreads / 32;
+    uint64_t last = ~0ull;
+    for (uint32_t k = 0; k < want; ++k) {
+        uint64_t best = 0;
+        for (uint32_t i = threadIdx.x; i < n; i += kBsThreads) {
+            const float v = beam_to_f32(x[i]);
+            const uint64_t key = (uint64_t)beam_order(v) << 32 | (0xffffffffu - (tok0 + i));
+            if (v > -INFINITY && key < last && key > best) best = key;
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
+            best = other > best ? other : best;
+        }
+        if (threadIdx.x % 32 == 0) l.key[threadIdx.x / 32] = best;
+        __syncthreads();
+        for (uint32_t w = 0; w < NW; ++w) best = l.key[w] > best ? l.key[w] : best;
+        if (threadIdx.x == 0) {
+            const uint32_t u = (uint32_t)(best >> 32);
+            l.x[old + k] = beam_unorder(u);
+            l.tok[old + k] = 0xffffffffu - (uint32_t)best;
+            l.n = old + k + 1;
+            // later pieces' equals of the last one taken cannot displace it
+            if (k + 1 == want) l.thr = max(l.thr, u + 1);
+        }
+        last = best;
+        __syncthreads();
     }
 }
 
-// One chunk of a row per block, E logits per thread.
-template <typename T, int E, bool VEC>
-__global__ void __launch_bounds__(kBsThreads) beam_select_chunk_kernel(BeamSelectArgs a) {
-    constexpr int NW = kBsThreads / 32, PV = VEC ? 16 / (int)sizeof(T) : 1;
-    __shared__ float s_max[NW], s_sum[NW];
-    __shared__ uint32_t s_best[kBsThreads], s_thr, s_n;
-    __shared__ uint64_t s_key[NW];
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t row = blockIdx.x / a.n_chunk, ck = blockIdx.x % a.n_chunk;
-    const uint32_t v0 = ck * a.chunk, n = min(a.chunk, a.n_vocab - v0);
-    const T *x = static_cast<const T *>(a.logits) + row * a.row_stride + v0;
-    float v[E];
-    beam_load_chunk<T, E, VEC>(x, n, v);
+// A piece with more logits at or above the threshold than the list has room
+// for (rising logits; equal ones): the list without this piece's, then a
+// threshold from this piece, or else its n_select best, read from memory
+// again.  The whole block.
+template <typename T>
+__device__ __noinline__ void beam_overflow(BeamList &l, const T *x, uint32_t n, uint32_t tok0, uint32_t want) {
+    constexpr uint32_t PT = kBsList / kBsThreads;
+    float keep[PT];
+    uint32_t tok[PT];
+#pragma unroll
+    for (uint32_t i = 0; i < PT; ++i) {
+        keep[i] = l.x[i * kBsThreads + threadIdx.x];
+        tok[i] = l.tok[i * kBsThreads + threadIdx.x];
+    }
     float m = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < E; ++e) m = fmaxf(m, v[e]);
-    s_best[threadIdx.x] = m == -INFINITY ? kBsNone : beam_order(m);
-    if (threadIdx.x == 0) s_n = 0;
-    float bm = m;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) bm = fmaxf(bm, __shfl_xor_sync(0xffffffffu, bm, o));
-    if (lane == 0) s_max[warp] = bm;
+    for (uint32_t i = threadIdx.x; i < n; i += kBsThreads) m = fmaxf(m, beam_to_f32(x[i]));
+    l.best[threadIdx.x] = m == -INFINITY ? kBsNone : beam_order(m);
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const uint32_t t = beam_threshold<kBsThreads>(l.best, want);
+        if (threadIdx.x == 0) {
+            l.thr = max(l.thr, t);
+            l.n = 0;
+        }
+    }
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NW; ++w) bm = fmaxf(bm, s_max[w]);
-    const float base = bm == -INFINITY ? 0.f : bm;
-    if (warp == 0) {
-        const uint32_t thr = beam_threshold<kBsThreads>(s_best, a.n_select);
-        if (lane == 0) s_thr = thr;
+    for (uint32_t i = 0; i < PT; ++i)
+        if (tok[i] < tok0) {
+            const uint32_t at = atomicAdd(&l.n, 1);
+            l.x[at] = keep[i];
+            l.tok[at] = tok[i];
+        }
+    __syncthreads();
+    const uint32_t old = l.n;
+    const float thr = beam_unorder(l.thr);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += kBsThreads) {
+        const float v = beam_to_f32(x[i]);
+        if (v >= thr) {
+            const uint32_t at = atomicAdd(&l.n, 1);
+            if (at < kBsList) {
+                l.x[at] = v;
+                l.tok[at] = tok0 + i;
+            }
+        }
     }
-    float sum = 0.f;  // a NaN or +inf among the logits makes it NaN
+    __syncthreads();
+    const bool still = l.n > kBsList;
+    __syncthreads();
+    if (still) beam_take_best(l, x, n, tok0, old, want);
+}
+
+// One part of a row per block.
+template <typename T, int E, bool VEC>
+__global__ void __launch_bounds__(kBsThreads, 5) beam_select_part_kernel(BeamSelectArgs a) {
+    constexpr int NW = kBsThreads / 32;
+    constexpr uint32_t kPiece = E * kBsThreads;
+    constexpr float kLog2e = 1.4426950408889634f;
+    using Piece = BeamPiece<T, E, VEC>;
+    __shared__ BeamList l;
+    __shared__ float s_max[NW], s_sum[NW];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t row = blockIdx.x / a.n_part;
+    const uint32_t v0 = blockIdx.x % a.n_part * a.part, n = min(a.part, a.n_vocab - v0);
+    const T *x = static_cast<const T *>(a.logits) + row * a.row_stride + v0;
+    pdl_launch();
+    if (threadIdx.x == 0) l.n = 0;
+    // of this thread's logits so far: the maximum, b = maximum * log2(e) as
+    // rounded, and the sum of 2^(x log2(e) - b); a NaN or +inf makes the sum NaN
+    float m = -INFINITY, b = 0.f, sum = 0.f, thr = 0.f;
+    for (uint32_t p0 = 0; p0 < n; p0 += kPiece) {
+        float v[E];
+        Piece::load(x + p0, n - p0, v);
+        float pm = v[0];
 #pragma unroll
-    for (int e = 0; e < E; ++e) sum += exp2_fast((v[e] - base) * 1.4426950408889634f);
+        for (int e = 1; e < E; ++e) pm = fmaxf(pm, v[e]);
+        if (p0 == 0) {  // the first threshold: about the n_select-th best of the threads' best
+            l.best[threadIdx.x] = pm == -INFINITY ? kBsNone : beam_order(pm);
+            __syncthreads();
+            if (warp == 0) {
+                const uint32_t t = beam_threshold<kBsThreads>(l.best, a.n_select);
+                if (lane == 0) l.thr = t;
+            }
+        }
+        if (pm > m) {
+            const float nb = pm * kLog2e;
+            sum *= exp2_fast(b - nb);  // (0 so far without a maximum)
+            m = pm;
+            b = nb;
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum += exp2_fast(fmaf(v[e], kLog2e, -b));
+        if (p0 == 0) {
+            __syncthreads();
+            thr = beam_unorder(l.thr);  // finite: -inf and NaN are below
+        }
+        bool full = false;
+        if (pm >= thr) {
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+                if (v[e] >= thr) {
+                    const uint32_t at = atomicAdd(&l.n, 1);
+                    full |= at >= kBsList / 2;
+                    if (at < kBsList) {
+                        l.x[at] = v[e];
+                        l.tok[at] = v0 + p0 + Piece::at(e);
+                    }
+                }
+        }
+        if (__syncthreads_or(full)) {
+            const bool over = l.n > kBsList;
+            __syncthreads();
+            if (over) beam_overflow(l, x + p0, min(n - p0, kPiece), v0 + p0, a.n_select);
+            if (l.n > kBsList / 2) beam_trim(l, a.n_select);
+            thr = beam_unorder(l.thr);
+            __syncthreads();
+        }
+    }
+    if (l.n > a.cap) beam_trim(l, a.n_select);
+    float2 *cand = a.cand + (size_t)blockIdx.x * a.cap;
+    const uint32_t cnt = l.n;
+    if (cnt <= a.cap) {
+        for (uint32_t i = threadIdx.x; i < a.cap; i += kBsThreads)
+            cand[i] = i < cnt ? make_float2(l.x[i], __uint_as_float(l.tok[i])) : make_float2(NAN, 0.f);
+    } else {  // many equal logits: the n_select best by rank
+        for (uint32_t i = threadIdx.x; i < cnt; i += kBsThreads) {
+            const float xi = l.x[i];
+            const uint32_t ti = l.tok[i];
+            uint32_t rank = 0;
+            for (uint32_t j = 0; j < cnt; ++j) rank += l.x[j] > xi || (l.x[j] == xi && l.tok[j] < ti);
+            if (rank < a.n_select) cand[rank] = make_float2(xi, __uint_as_float(ti));
+        }
+        for (uint32_t i = a.n_select + threadIdx.x; i < a.cap; i += kBsThreads) cand[i] = make_float2(NAN, 0.f);
+    }
+    float bb = m == -INFINITY ? -INFINITY : b;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) bb = fmaxf(bb, __shfl_xor_sync(0xffffffffu, bb, o));
+    if (lane == 0) s_max[warp] = bb;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) bb = fmaxf(bb, s_max[w]);
+    // a thread without finite logits has sum 0, or NaN
+    if (m > -INFINITY) sum *= exp2_fast(b - bb);
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) s_sum[warp] = sum;
     __syncthreads();
-    const uint32_t thr = s_thr;
-    const size_t list = blockIdx.x;
-    float2 *cand = a.cand + list * a.cap;
-    if (beam_order(m) >= thr && m > -INFINITY) {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (v[e] > -INFINITY && beam_order(v[e]) >= thr) {
-                const uint32_t at = atomicAdd(&s_n, 1);
-                const uint32_t tok = v0 + ((e / PV) * kBsThreads + threadIdx.x) * PV + e % PV;
-                if (at < a.cap) cand[at] = make_float2(v[e], __uint_as_float(tok));
-            }
-    }
-    __syncthreads();
-    uint32_t cnt = s_n;
-    if (cnt > a.cap) {  // many equal logits, or the best in few threads: exactly n_select, one after the other
-        uint64_t last = ~0ull;
-        for (cnt = 0; cnt < a.n_select; ++cnt) {
-            uint64_t best = 0;
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (v[e] > -INFINITY) {
-                    float now = v[e] + 0.f;              // (-0 ties with 0)
-                    asm volatile("" : "+f"(now));        // keep the keys out of registers between rounds
-                    const uint32_t tok = v0 + ((e / PV) * kBsThreads + threadIdx.x) * PV + e % PV;
-                    const uint64_t key = (uint64_t)beam_order(now) << 32 | (0xffffffffu - tok);
-                    if (key < last && key > best) best = key;
-                }
-#pragma unroll
-            for (int o = 16; o; o >>= 1) {
-                const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
-                best = other > best ? other : best;
-            }
-            if (lane == 0) s_key[warp] = best;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < NW; ++w) best = s_key[w] > best ? s_key[w] : best;
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                const uint32_t u = (uint32_t)(best >> 32);
-                cand[cnt] = make_float2(__uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u),
-                                        __uint_as_float(0xffffffffu - (uint32_t)best));
-            }
-            last = best;
-        }
-    }
     if (threadIdx.x == 0) {
         float t = 0.f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) t += s_sum[w];
-        a.stat[list] = make_float2(bm, t);
-        a.count[list] = cnt;
+        a.stat[blockIdx.x] = make_float2(bb, t);
     }
 }
 
-// One block per group: the rows' log-sums, the candidates' scores, their ranks.
+// Orders like the double, as an unsigned integer.
+__device__ __forceinline__ uint64_t beam_order64(double v) {
+    const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
+    return b >> 63 ? ~b : b | 1ull << 63;
+}
+__device__ __forceinline__ double beam_unorder64(uint64_t u) {
+    return __longlong_as_double((long long)(u >> 63 ? u & ~(1ull << 63) : ~u));
+}
+
+// A cluster of blocks per group: the rows' log-sums and the scores of the
+// candidates; each block gives about the n_select best of its share to the
+// first block's pool, which is cut and ranked.
 __global__ void __launch_bounds__(kBsJoinThreads) beam_select_join_kernel(BeamSelectArgs a) {
-    __shared__ double s_off[kBsMaxBeams];     // c - lse; NaN: a row without candidates
+    namespace cg = cooperative_groups;
+    const cg::cluster_group cluster = cg::this_cluster();
+    __shared__ double s_off[kBsMaxBeams];     // c - lse
+    __shared__ float s_offf[kBsMaxBeams];     // the same rounded; NaN: a row without candidates
     __shared__ uint32_t s_best[kBsJoinThreads], s_thr, s_n;
-    __shared__ double s_score[kBsPool];
+    __shared__ uint64_t s_key[kBsPool];       // beam_order64 of the score
     __shared__ uint32_t s_flat[kBsPool];
-    __shared__ double s_kd[kBsJoinThreads / 32];
+    __shared__ uint64_t s_kd[kBsJoinThreads / 32];
     __shared__ uint32_t s_ki[kBsJoinThreads / 32];
     constexpr uint32_t NT = kBsJoinThreads, NW = NT / 32;
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.x;
-    const size_t list0 = (size_t)g * a.n_beam * a.n_chunk;
-    const uint32_t lists = a.n_beam * a.n_chunk;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint32_t cs = cluster.num_blocks(), cr = cluster.block_rank(), g = blockIdx.x / cs;
+    const size_t list0 = (size_t)g * a.n_beam * a.n_part;
+    if (threadIdx.x == 0) s_n = 0;
+    pdl_wait();
     for (uint32_t w = warp; w < a.n_beam; w += NW) {
-        const float2 *st = a.stat + list0 + (size_t)w * a.n_chunk;
+        const float2 *st = a.stat + list0 + (size_t)w * a.n_part;
+        const float c = a.scores[g * a.n_beam + w];
         float m = -INFINITY;
-        for (uint32_t i = lane; i < a.n_chunk; i += 32) m = fmaxf(m, st[i].x);
+        for (uint32_t i = lane; i < a.n_part; i += 32) m = fmaxf(m, st[i].x);
 #pragma unroll
         for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        double sum = 0;
-        for (uint32_t i = lane; i < a.n_chunk; i += 32) {
-            const float2 v = st[i];  // a chunk of barred tokens has sum 0 (or NaN)
-            sum += v.x == -INFINITY ? (double)v.y : (double)v.y * (double)expf(v.x - m);
+        float sum = 0.f;
+        for (uint32_t i = lane; i < a.n_part; i += 32) {
+            const float2 v = st[i];  // a part of barred tokens has sum 0 (or NaN)
+            sum += v.x == -INFINITY ? v.y : v.y * exp2_fast(v.x - m);
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) {
-            const float c = a.scores[g * a.n_beam + w];
             const bool live = isfinite(c) && isfinite(m) && sum > 0 && isfinite(sum);
-            s_off[w] = live ? (double)c - ((double)m + log(sum)) : nan("");
+            const double off = (double)c - ((double)m * 0.69314718055994531 + (double)logf(sum));
+            s_off[w] = off;
+            s_offf[w] = live ? (float)off : NAN;
         }
     }
-    if (threadIdx.x == 0) s_n = 0;
-    __syncthreads();
-    const uint64_t slots = (uint64_t)lists * a.cap;
-    auto score_of = [&](uint64_t i, double &s, uint32_t &flat) {
-        const uint32_t list = (uint32_t)(i / a.cap), w = list / a.n_chunk;
-        if ((uint32_t)(i % a.cap) >= a.count[list0 + list]) return false;
-        const float2 c = a.cand[list0 * a.cap + i];
-        s = s_off[w] + (double)c.x;
-        flat = w * a.n_vocab + __float_as_uint(c.y);
-        return s == s;
+    cluster.sync();  // the offsets, and the first block's pool counter, are there
+    uint32_t *pool_n = cluster.map_shared_rank(&s_n, 0);
+    uint64_t *pool_key = cluster.map_shared_rank(s_key, 0);
+    uint32_t *pool_flat = cluster.map_shared_rank(s_flat, 0);
+    // The candidates in slices of 32 places, `step` warps in turn, four slices
+    // at a time.  visit(logit, row, token) is called for each place (unused
+    // ones and dead rows give NaN scores).
+    const uint32_t per = a.cap / 32, slices = a.n_beam * a.n_part * per;
+    const float2 *cand = a.cand + list0 * a.cap;
+    auto each = [&](uint32_t first, uint32_t step, auto visit) {
+        for (uint32_t s0 = first; s0 < slices; s0 += 4 * step) {
+            float2 c[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) c[u] = cand[(size_t)min(s0 + u * step, slices - 1) * 32 + lane];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (s0 + u * step < slices)
+                    visit(c[u].x, (s0 + u * step) / per / a.n_part, __float_as_uint(c[u].y));
+        }
     };
-    uint32_t best = kBsNone;
-    for (uint64_t i = threadIdx.x; i < slots; i += NT) {
-        double s;
-        uint32_t flat;
-        if (score_of(i, s, flat)) best = max(best, beam_order((float)s));
-    }
-    s_best[threadIdx.x] = best;
+    float best = -INFINITY;
+    each(cr * NW + warp, cs * NW, [&](float x, uint32_t w, uint32_t) { best = fmaxf(best, x + s_offf[w]); });
+    s_best[threadIdx.x] = best == -INFINITY ? kBsNone : beam_order(best);
     __syncthreads();
     if (warp == 0) {
         const uint32_t thr = beam_threshold<kBsJoinThreads>(s_best, a.n_select);
         if (lane == 0) s_thr = thr;
     }
+    // The scores compared here are rounded twice in 32 bits, the offset and the
+    // sum: a candidate counts as below the threshold only by more than both
+    // roundings of both sides.
+    float off_max = 0.f;
+    for (uint32_t w = 0; w < a.n_beam; ++w) off_max = fmaxf(off_max, fabsf(s_offf[w]));
     __syncthreads();
-    const uint32_t thr = s_thr;
-    if (best >= thr)
-        for (uint64_t i = threadIdx.x; i < slots; i += NT) {
-            double s;
-            uint32_t flat;
-            if (score_of(i, s, flat) && beam_order((float)s) >= thr) {
-                const uint32_t at = atomicAdd(&s_n, 1);
-                if (at < kBsPool) {
-                    s_score[at] = s;
-                    s_flat[at] = flat;
-                }
+    float thr = beam_unorder(s_thr);
+    thr -= 2.4e-7f * (2.f * fabsf(thr) + off_max);  // (-FLT_MAX or -inf takes all)
+    if (__any_sync(0xffffffffu, best >= thr))
+        each(cr * NW + warp, cs * NW, [&](float x, uint32_t w, uint32_t tok) {
+            if (!(x + s_offf[w] >= thr)) return;
+            const uint32_t at = atomicAdd(pool_n, 1);
+            if (at < kBsPool) {
+                pool_key[at] = beam_order64(s_off[w] + (double)x);
+                pool_flat[at] = w * a.n_vocab + tok;
             }
-        }
-    __syncthreads();
+        });
+    cluster.sync();
+    if (cr != 0) return;
     uint32_t n = s_n;
     __syncthreads();
-    if (n > kBsPool) {  // the best in few threads: one after the other
-        double ls = INFINITY;
+    if (n > kBsPool) {  // the best in few threads, or many equal scores: one after the other
+        uint64_t ls = ~0ull;
         uint32_t li = 0;
         for (n = 0; n < a.n_select; ++n) {
-            double bs = -INFINITY;
+            uint64_t bs = 0;
             uint32_t bi = 0xffffffffu;
-            for (uint64_t i = threadIdx.x; i < slots; i += NT) {
-                double s;
-                uint32_t flat;
-                if (!score_of(i, s, flat)) continue;
-                if (n && !(s < ls || (s == ls && flat > li))) continue;
+            each(warp, NW, [&](float x, uint32_t w, uint32_t tok) {
+                const float f = x + s_offf[w];
+                if (f != f) return;
+                const uint64_t s = beam_order64(s_off[w] + (double)x);
+                const uint32_t flat = w * a.n_vocab + tok;
+                if (n && !(s < ls || (s == ls && flat > li))) return;
                 if (s > bs || (s == bs && flat < bi)) { bs = s; bi = flat; }
-            }
+            });
 #pragma unroll
             for (int o = 16; o; o >>= 1) {
-                const double os = __shfl_xor_sync(0xffffffffu, bs, o);
+                const uint64_t os = __shfl_xor_sync(0xffffffffu, bs, o);
                 const uint32_t oi = __shfl_xor_sync(0xffffffffu, bi, o);
                 if (os > bs || (os == bs && oi < bi)) { bs = os; bi = oi; }
             }
@@ -288,20 +506,50 @@ __global__ void __launch_bounds__(kBsJoinThreads) beam_select_join_kernel(BeamSe
             __syncthreads();
             for (uint32_t w = 0; w < NW; ++w)
                 if (s_kd[w] > bs || (s_kd[w] == bs && s_ki[w] < bi)) { bs = s_kd[w]; bi = s_ki[w]; }
-            if (threadIdx.x == 0) { s_score[n] = bs; s_flat[n] = bi; }
+            if (threadIdx.x == 0) { s_key[n] = bs; s_flat[n] = bi; }
             __syncthreads();
             ls = bs;
             li = bi;
         }
+    } else if (n > 2 * a.n_select + 64) {  // many blocks' shares: cut once more, on the key's upper half
+        constexpr uint32_t PT = kBsPool / NT;
+        uint64_t key[PT];
+        uint32_t flat[PT], top = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < PT; ++i) {
+            const uint32_t j = i * NT + threadIdx.x;
+            key[i] = j < n ? s_key[j] : 0;
+            flat[i] = j < n ? s_flat[j] : 0;
+            top = max(top, (uint32_t)(key[i] >> 32));
+        }
+        s_best[threadIdx.x] = top;
+        if (threadIdx.x == 0) s_n = 0;
+        __syncthreads();
+        if (warp == 0) {
+            const uint32_t t = beam_threshold<kBsJoinThreads>(s_best, a.n_select);
+            if (lane == 0) s_thr = t;
+        }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < PT; ++i)
+            if (key[i] && (uint32_t)(key[i] >> 32) >= s_thr) {
+                const uint32_t at = atomicAdd(&s_n, 1);
+                s_key[at] = key[i];
+                s_flat[at] = flat[i];
+            }
+        __syncthreads();
+        n = s_n;
     }
+    // each warp ranks one entry at a time against all
     const size_t out = (size_t)g * a.n_select;
-    for (uint32_t i = threadIdx.x; i < n; i += NT) {
-        const double s = s_score[i];
+    for (uint32_t i = warp; i < n; i += NW) {
+        const uint64_t s = s_key[i];
         const uint32_t flat = s_flat[i];
         uint32_t rank = 0;
-        for (uint32_t j = 0; j < n; ++j) rank += s_score[j] > s || (s_score[j] == s && s_flat[j] < flat);
-        if (rank < a.n_select) {
-            a.out_scores[out + rank] = (float)s;
+        for (uint32_t j = lane; j < n; j += 32) rank += s_key[j] > s || (s_key[j] == s && s_flat[j] < flat);
+        rank = __reduce_add_sync(0xffffffffu, rank);
+        if (lane == 0 && rank < a.n_select) {
+            a.out_scores[out + rank] = (float)beam_unorder64(s);
             a.parent[out + rank] = (int32_t)(flat / a.n_vocab);
             a.token[out + rank] = (int32_t)(flat % a.n_vocab);
         }
