@@ -45,6 +45,17 @@ cudaError_t launch_after(F *fn, dim3 grid, unsigned threads, unsigned cluster, c
     return cudaLaunchKernelEx(&cfg, fn, args...);
 }
 
+// Dynamic shared memory past the default limit, once per kernel and device.
+template <typename F>
+bool opt_in(F *fn, uint32_t smem, bool (&ready)[64], const char *who) {
+    int dev = 0;
+    if (!launched(cudaGetDevice(&dev), who)) return false;
+    if (dev < 64 && ready[dev]) return true;
+    if (!launched(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem), who)) return false;
+    if (dev < 64) ready[dev] = true;
+    return true;
+}
+
 uint32_t elem_bytes(uint32_t type) { return type == 0 ? 4u : type == 1 || type == 30 ? 2u : 0u; }
 
 // --- prefix attention --------------------------------------------------------
@@ -153,15 +164,7 @@ template <typename T, int HD, int RWP, int RWS>
 bool launch_attn(const BeamAttnArgs &k, const BeamAttnPlan &p, cudaStream_t st) {
     static bool ready[64] = {};
     constexpr uint32_t smem = beam_attn_smem<T, HD>();
-    int dev = 0;
-    if (!launched(cudaGetDevice(&dev), "fwb_prefix_attention")) return false;
-    if (dev >= 64 || !ready[dev]) {
-        if (!launched(cudaFuncSetAttribute(beam_attn_kernel<T, HD, RWP, RWS>,
-                                           cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem),
-                      "fwb_prefix_attention"))
-            return false;
-        if (dev < 64) ready[dev] = true;
-    }
+    if (!opt_in(beam_attn_kernel<T, HD, RWP, RWS>, smem, ready, "fwb_prefix_attention")) return false;
     beam_attn_kernel<T, HD, RWP, RWS><<<p.ctas, kBaThreads, smem, st>>>(k, p);
     beam_attn_join_kernel<T, HD><<<dim3(k.n_group * k.n_beam * k.n_query, k.n_head), kBaThreads, 0, st>>>(k, p);
     return launched(cudaGetLastError(), "fwb_prefix_attention launch");
@@ -204,56 +207,68 @@ bool select_sizes_ok(uint32_t type, size_t n_group, size_t n_beam, size_t n_voca
         return fail("fwb_beam_select: zero groups, beams, tokens or selected entries");
     if (n_beam > kMaxSelectBeams || n_group > 0x7fffffffu / kMaxSelectBeams || n_vocab > 0x7fffffffu / n_beam)
         return fail("fwb_beam_select: more than 64 beams, or more than 2^31 - 1 scores in a group");
-    if (n_group * n_beam > (size_t)0x7fffffff / (n_vocab / 2048 + 2))
+    if (n_group * n_beam > (size_t)0x7fffffff / 1025)
         return fail("fwb_beam_select: too many rows");
     if (n_select > kMaxSelect || n_select > n_beam * n_vocab)
         return fail("fwb_beam_select: n_select must be at most 128 and at most n_beam * n_vocab");
     return true;
 }
 
-// The parts of a row and the workspace's layout.  A piece is what a block
-// holds in registers: 16 logits per thread, 8 when the rows are few.
+// The parts of a row and the workspace's layout.
 struct SelectLayout {
-    bool small;
     uint32_t n_part, part, cap;
     size_t cand, stat, bytes;
 };
 
+// How many parts a row is read in.  More parts use more SMs; each costs about
+// 7000 cycles besides its pieces (first loads, first threshold, output), and
+// leaves candidates to the join (about 3000 cycles for every 512 slices of
+// 32).  A piece takes a block 1800 cycles, and an SM 825 when its up to five
+// blocks keep the memory busy.  The cheapest count by these figures is taken.
+// Measured: 256 fp32 rows of 128256 in 1 / 2 / 4 / 8 parts a row 45 / 39 / 43 /
+// 48 us (2 taken); 16 bf16 rows in 2 / 5 / 8 / 16 / 32 parts 33 / 24 / 21 / 21
+// / 24 us (8); 4 fp32 rows of 32000 in 2 / 4 / 8 parts 12.3 / 10.1 / 9.0 us (8).
 void select_layout(size_t n_group, size_t n_beam, size_t n_vocab, size_t n_select, SelectLayout &L) {
-    const size_t rows = n_group * n_beam, piece = 16 * kBsThreads;
-    // about four blocks per SM, of one to four pieces
-    const size_t even = rows * n_vocab / (4 * device_sms());
-    L.small = even < piece;
-    const size_t want = L.small ? piece / 2 : std::min(4 * piece, even / piece * piece);
-    L.n_part = (uint32_t)((n_vocab + want - 1) / want);
-    L.part = (uint32_t)(((n_vocab + L.n_part - 1) / L.n_part + 7) / 8 * 8);
+    const uint64_t rows = (uint64_t)n_group * n_beam, sms = device_sms(), piece = kBsLogits * kBsThreads;
+    L.cap = (uint32_t)((2 * n_select + 16 + 31) / 32 * 32);
+    uint64_t cheapest = ~0ull, count = 1;
+    for (uint64_t n = 1; n <= std::min<uint64_t>(1024, (n_vocab + piece - 1) / piece); n = n < 16 ? n + 1 : n + n / 8) {
+        const uint64_t pieces = ((n_vocab + n - 1) / n + piece - 1) / piece, per_sm = (rows * n + sms - 1) / sms;
+        auto wave = [&](uint64_t blocks) { return blocks ? 7000 + pieces * std::max<uint64_t>(1800, 825 * blocks) : 0; };
+        const uint64_t cost = per_sm / 5 * wave(5) + wave(per_sm % 5) + 3000 * ((n_beam * n * (L.cap / 32) + 511) / 512);
+        if (cost < cheapest) {
+            cheapest = cost;
+            count = n;
+        }
+    }
+    L.part = (uint32_t)(((n_vocab + count - 1) / count + 7) / 8 * 8);
     L.n_part = (uint32_t)((n_vocab + L.part - 1) / L.part);
-    L.cap = (uint32_t)((n_select + n_select / 2 + 8 + 31) / 32 * 32);
     const size_t lists = rows * L.n_part;
     L.cand = 0;
     L.stat = (lists * L.cap * sizeof(float2) + 255) & ~(size_t)255;
     L.bytes = L.stat + lists * sizeof(float2);
 }
 
-template <typename T, int E>
-void launch_parts(const BeamSelectArgs &k, bool vec, cudaStream_t st) {
-    const uint32_t grid = k.n_group * k.n_beam * k.n_part;
-    if (vec) beam_select_part_kernel<T, E, true><<<grid, kBsThreads, 0, st>>>(k);
-    else beam_select_part_kernel<T, E, false><<<grid, kBsThreads, 0, st>>>(k);
+template <typename T, bool VEC>
+bool launch_parts(const BeamSelectArgs &k, cudaStream_t st) {
+    static bool ready[64] = {};
+    constexpr uint32_t smem = BeamPiece<T, VEC>::kSmem;
+    if (!opt_in(beam_select_part_kernel<T, VEC>, smem, ready, "fwb_beam_select")) return false;
+    beam_select_part_kernel<T, VEC><<<k.n_group * k.n_beam * k.n_part, kBsThreads, smem, st>>>(k);
+    return launched(cudaGetLastError(), "fwb_beam_select launch");
 }
 
 template <typename T>
-bool run_select(const BeamSelectArgs &k, bool small, cudaStream_t st) {
+bool run_select(const BeamSelectArgs &k, cudaStream_t st) {
     // 16-byte loads when every row allows them (not row by row: rows with equal
     // logits must have equal sums)
     const bool vec = ((uintptr_t)k.logits | k.row_stride * sizeof(T)) % 16 == 0;
-    if (small) launch_parts<T, 8>(k, vec, st);
-    else launch_parts<T, 16>(k, vec, st);
-    if (!launched(cudaGetLastError(), "fwb_beam_select launch")) return false;
-    // as many blocks per group as have a batch of slices for every warp
-    const uint64_t batches = ((uint64_t)k.n_beam * k.n_part * (k.cap / 32) + 31) / 32;
+    if (!(vec ? launch_parts<T, true>(k, st) : launch_parts<T, false>(k, st))) return false;
+    // more than one block per group when one would look at more than two
+    // batches of slices: the cluster's two barriers cost about a batch
+    const uint64_t batches = ((uint64_t)k.n_beam * k.n_part * (k.cap / 32) + 63) / 64;
     uint32_t cluster = 1;
-    while (cluster < kBsJoinCluster && cluster < batches) cluster *= 2;
+    while (cluster < kBsJoinCluster && 2 * cluster < batches) cluster *= 2;
     return launched(launch_after(beam_select_join_kernel, dim3(k.n_group * cluster), kBsJoinThreads, cluster, st, k),
                     "fwb_beam_select launch");
 }
@@ -336,9 +351,9 @@ int fwb_beam_select_dev(const void *d_logits, uint32_t type, size_t n_group, siz
     k.stat = reinterpret_cast<float2 *>(ws + L.stat);
     k.n_part = L.n_part; k.part = L.part; k.cap = L.cap;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool ok = type == 0 ? run_select<float>(k, L.small, st)
-                  : type == 1 ? run_select<__half>(k, L.small, st)
-                              : run_select<__nv_bfloat16>(k, L.small, st);
+    const bool ok = type == 0 ? run_select<float>(k, st)
+                  : type == 1 ? run_select<__half>(k, st)
+                              : run_select<__nv_bfloat16>(k, st);
     return ok ? 0 : -1;
 }
 

@@ -25,11 +25,12 @@
 namespace fwb {
 
 constexpr int kBsThreads = 256;       // of a part's block
-constexpr int kBsJoinThreads = 256;
+constexpr int kBsJoinThreads = 512;
 constexpr uint32_t kBsJoinCluster = 8;  // most blocks of a group's join
 constexpr uint32_t kBsMaxSelect = 128, kBsMaxBeams = 64;
 constexpr uint32_t kBsList = 1024;    // candidates that a block of the first kernel holds
 constexpr uint32_t kBsPool = 2048;    // candidates that the second kernel ranks
+constexpr int kBsLogits = 16;         // of a thread and piece
 
 struct BeamSelectArgs {
     const void *logits;     // [n_group * n_beam] rows, row_stride elements apart
@@ -93,24 +94,42 @@ __device__ __forceinline__ uint32_t beam_threshold(const uint32_t *vals, uint32_
     return lo;
 }
 
-// A piece: E logits of each thread, 16 bytes at a time (VEC) or one.
-template <typename T, int E, bool VEC>
+// A piece: E logits of each thread, loaded 16 bytes at a time (VEC) or one.  With
+// VEC the pieces ahead are copied asynchronously into shared memory; every
+// thread reads only what it copied itself, so that needs no barrier.  One
+// piece ahead, so that five blocks fit an SM.
+constexpr int kBsStages = 2;
+template <typename T, bool VEC>
 struct BeamPiece {
-    static constexpr int PV = VEC ? 16 / (int)sizeof(T) : 1;  // elements per load
+    static constexpr int E = kBsLogits, PV = VEC ? 16 / (int)sizeof(T) : 1;  // elements per load
+    static constexpr uint32_t kLogits = E * kBsThreads;
+    static constexpr uint32_t kSmem = VEC ? kBsStages * kLogits * sizeof(T) : 0;
     static __device__ __forceinline__ uint32_t at(int e) { return ((e / PV) * kBsThreads + threadIdx.x) * PV + e % PV; }
-    // x: the piece's first logit; n: logits from there on, the rest -inf
-    static __device__ __forceinline__ void load(const T *x, uint32_t n, float *v) {
-        if (n >= E * kBsThreads) {
-            if constexpr (VEC) {
-                uint4 raw[E / PV];
+    // starts the copies of a piece; x: its first logit, n: logits from there on
+    static __device__ __forceinline__ void start(const T *x, uint32_t n, T *stage) {
+        if constexpr (VEC) {
 #pragma unroll
-                for (int i = 0; i < E / PV; ++i) raw[i] = __ldcs(reinterpret_cast<const uint4 *>(x + at(i * PV)));
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[e] = beam_to_f32(reinterpret_cast<const T *>(&raw[e / PV])[e % PV]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; ++e) v[e] = beam_to_f32(x[at(e)]);
+            for (int i = 0; i < E / PV; ++i) {
+                const uint32_t p = at(i * PV);
+                if (p + PV <= n) cp_async16(stage + p, x + p);
             }
+            cp_async_commit();
+        }
+    }
+    // the piece's logits, -inf past n
+    static __device__ __forceinline__ void load(const T *x, uint32_t n, const T *stage, float *v) {
+        if constexpr (VEC) {
+            cp_async_wait<1>();
+#pragma unroll
+            for (int i = 0; i < E / PV; ++i) {
+                const uint4 raw = *reinterpret_cast<const uint4 *>(stage + at(i * PV));
+#pragma unroll
+                for (int e = 0; e < PV; ++e) v[i * PV + e] = beam_to_f32(reinterpret_cast<const T *>(&raw)[e]);
+            }
+            if (n < kLogits)
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    if (at(e - e % PV) + PV > n) v[e] = at(e) < n ? beam_to_f32(x[at(e)]) : -INFINITY;
         } else {
 #pragma unroll
             for (int e = 0; e < E; ++e) v[e] = at(e) < n ? beam_to_f32(x[at(e)]) : -INFINITY;
@@ -131,34 +150,32 @@ struct BeamList {
 // below; a list that equal logits keep long is cut to exactly n_select (the
 // pieces come in the order of the tokens, so later equals cannot displace
 // them, and thr excludes these).  The whole block.
-__device__ __forceinline__ void beam_trim(BeamList &l, uint32_t want) {
+__device__ __noinline__ void beam_trim(BeamList &l, uint32_t want) {
     constexpr uint32_t PT = kBsList / kBsThreads;
     const uint32_t n = min(l.n, kBsList);
-    float x[PT];
+    float x[PT], best = -INFINITY;
     uint32_t tok[PT];
 #pragma unroll
     for (uint32_t i = 0; i < PT; ++i) {
         const uint32_t j = i * kBsThreads + threadIdx.x;
         x[i] = j < n ? l.x[j] : -INFINITY;
         tok[i] = j < n ? l.tok[j] : 0;
+        best = fmaxf(best, x[i]);
     }
-    __syncthreads();
-#pragma unroll
-    for (uint32_t i = 0; i < PT; ++i)  // the list's own memory, as ordered integers, for the search
-        reinterpret_cast<uint32_t *>(l.x)[i * kBsThreads + threadIdx.x] = x[i] == -INFINITY ? 0u : beam_order(x[i]);
+    l.best[threadIdx.x] = best == -INFINITY ? kBsNone : beam_order(best);
     __syncthreads();
     if (threadIdx.x < 32) {
-        const uint32_t thr = beam_threshold<kBsList>(reinterpret_cast<const uint32_t *>(l.x), want);
+        const uint32_t thr = beam_threshold<kBsThreads>(l.best, want);
         if (threadIdx.x == 0) {
             l.thr = max(l.thr, thr);
             l.n = 0;
         }
     }
     __syncthreads();
-    const uint32_t thr = l.thr;
+    const float thr = beam_unorder(l.thr);
 #pragma unroll
     for (uint32_t i = 0; i < PT; ++i)
-        if (x[i] > -INFINITY && beam_order(x[i]) >= thr) {
+        if (x[i] >= thr) {
             const uint32_t at = atomicAdd(&l.n, 1);
             l.x[at] = x[i];
             l.tok[at] = tok[i];
@@ -175,7 +192,8 @@ __device__ __forceinline__ void beam_trim(BeamList &l, uint32_t want) {
             x[i] = l.x[j];
             tok[i] = l.tok[j];
             rank[i] = 0;
-            for (uint32_t k = 0; k < kept; ++k) rank[i] += l.x[k] > x[i] || (l.x[k] == x[i] && l.tok[k] < tok[i]);
+            for (uint32_t k = 0; k < kept; ++k)
+                rank[i] += (uint32_t)(l.x[k] > x[i]) | ((uint32_t)(l.x[k] == x[i]) & (uint32_t)(l.tok[k] < tok[i]));
         }
     }
     __syncthreads();
@@ -282,12 +300,14 @@ __device__ __noinline__ void beam_overflow(BeamList &l, const T *x, uint32_t n, 
 }
 
 // One part of a row per block.
-template <typename T, int E, bool VEC>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(kBsThreads, 5) beam_select_part_kernel(BeamSelectArgs a) {
-    constexpr int NW = kBsThreads / 32;
-    constexpr uint32_t kPiece = E * kBsThreads;
+    using Piece = BeamPiece<T, VEC>;
+    constexpr int NW = kBsThreads / 32, E = Piece::E;
+    constexpr uint32_t kPiece = Piece::kLogits;
     constexpr float kLog2e = 1.4426950408889634f;
-    using Piece = BeamPiece<T, E, VEC>;
+    extern __shared__ __align__(16) uint8_t bs_stages[];
+    T *stages = reinterpret_cast<T *>(bs_stages);
     __shared__ BeamList l;
     __shared__ float s_max[NW], s_sum[NW];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -296,15 +316,26 @@ __global__ void __launch_bounds__(kBsThreads, 5) beam_select_part_kernel(BeamSel
     const T *x = static_cast<const T *>(a.logits) + row * a.row_stride + v0;
     pdl_launch();
     if (threadIdx.x == 0) l.n = 0;
+    Piece::start(x, n, stages);
+    uint32_t stage = 0;
+    const uint32_t limit = min(kBsList / 2, 3 * a.n_select + 64);  // a longer list is trimmed, which raises the threshold
     // of this thread's logits so far: the maximum, b = maximum * log2(e) as
     // rounded, and the sum of 2^(x log2(e) - b); a NaN or +inf makes the sum NaN
     float m = -INFINITY, b = 0.f, sum = 0.f, thr = 0.f;
     for (uint32_t p0 = 0; p0 < n; p0 += kPiece) {
         float v[E];
-        Piece::load(x + p0, n - p0, v);
-        float pm = v[0];
+        {
+            const uint32_t next = p0 + kPiece;
+            Piece::start(x + next, n > next ? n - next : 0, stages + (stage ^ 1) * kPiece);
+            Piece::load(x + p0, n - p0, stages + stage * kPiece, v);
+            stage ^= 1;
+        }
+        float qm[E / 4], pm = -INFINITY;  // of four logits, of all
 #pragma unroll
-        for (int e = 1; e < E; ++e) pm = fmaxf(pm, v[e]);
+        for (int q = 0; q < E / 4; ++q) {
+            qm[q] = fmaxf(fmaxf(v[4 * q], v[4 * q + 1]), fmaxf(v[4 * q + 2], v[4 * q + 3]));
+            pm = fmaxf(pm, qm[q]);
+        }
         if (p0 == 0) {  // the first threshold: about the n_select-th best of the threads' best
             l.best[threadIdx.x] = pm == -INFINITY ? kBsNone : beam_order(pm);
             __syncthreads();
@@ -328,21 +359,24 @@ __global__ void __launch_bounds__(kBsThreads, 5) beam_select_part_kernel(BeamSel
         bool full = false;
         if (pm >= thr) {
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-                if (v[e] >= thr) {
-                    const uint32_t at = atomicAdd(&l.n, 1);
-                    full |= at >= kBsList / 2;
-                    if (at < kBsList) {
-                        l.x[at] = v[e];
-                        l.tok[at] = v0 + p0 + Piece::at(e);
-                    }
-                }
+            for (int q = 0; q < E / 4; ++q)
+                if (qm[q] >= thr)
+#pragma unroll
+                    for (int e = 4 * q; e < 4 * q + 4; ++e)
+                        if (v[e] >= thr) {
+                            const uint32_t at = atomicAdd(&l.n, 1);
+                            full |= at >= limit;
+                            if (at < kBsList) {
+                                l.x[at] = v[e];
+                                l.tok[at] = v0 + p0 + Piece::at(e);
+                            }
+                        }
         }
         if (__syncthreads_or(full)) {
             const bool over = l.n > kBsList;
             __syncthreads();
             if (over) beam_overflow(l, x + p0, min(n - p0, kPiece), v0 + p0, a.n_select);
-            if (l.n > kBsList / 2) beam_trim(l, a.n_select);
+            if (l.n > limit) beam_trim(l, a.n_select);
             thr = beam_unorder(l.thr);
             __syncthreads();
         }
@@ -358,7 +392,8 @@ __global__ void __launch_bounds__(kBsThreads, 5) beam_select_part_kernel(BeamSel
             const float xi = l.x[i];
             const uint32_t ti = l.tok[i];
             uint32_t rank = 0;
-            for (uint32_t j = 0; j < cnt; ++j) rank += l.x[j] > xi || (l.x[j] == xi && l.tok[j] < ti);
+            for (uint32_t j = 0; j < cnt; ++j)
+                rank += (uint32_t)(l.x[j] > xi) | ((uint32_t)(l.x[j] == xi) & (uint32_t)(l.tok[j] < ti));
             if (rank < a.n_select) cand[rank] = make_float2(xi, __uint_as_float(ti));
         }
         for (uint32_t i = a.n_select + threadIdx.x; i < a.cap; i += kBsThreads) cand[i] = make_float2(NAN, 0.f);
@@ -433,7 +468,8 @@ __global__ void __launch_bounds__(kBsJoinThreads) beam_select_join_kernel(BeamSe
             s_offf[w] = live ? (float)off : NAN;
         }
     }
-    cluster.sync();  // the offsets, and the first block's pool counter, are there
+    if (cs > 1) cluster.sync();  // the offsets, and the first block's pool counter, are there
+    else __syncthreads();
     uint32_t *pool_n = cluster.map_shared_rank(&s_n, 0);
     uint64_t *pool_key = cluster.map_shared_rank(s_key, 0);
     uint32_t *pool_flat = cluster.map_shared_rank(s_flat, 0);
@@ -441,6 +477,7 @@ __global__ void __launch_bounds__(kBsJoinThreads) beam_select_join_kernel(BeamSe
     // at a time.  visit(logit, row, token) is called for each place (unused
     // ones and dead rows give NaN scores).
     const uint32_t per = a.cap / 32, slices = a.n_beam * a.n_part * per;
+    const uint32_t places = per * a.n_part;  // slices of a row
     const float2 *cand = a.cand + list0 * a.cap;
     auto each = [&](uint32_t first, uint32_t step, auto visit) {
         for (uint32_t s0 = first; s0 < slices; s0 += 4 * step) {
@@ -450,7 +487,7 @@ __global__ void __launch_bounds__(kBsJoinThreads) beam_select_join_kernel(BeamSe
 #pragma unroll
             for (int u = 0; u < 4; ++u)
                 if (s0 + u * step < slices)
-                    visit(c[u].x, (s0 + u * step) / per / a.n_part, __float_as_uint(c[u].y));
+                    visit(c[u].x, (s0 + u * step) / places, __float_as_uint(c[u].y));
         }
     };
     float best = -INFINITY;
@@ -478,7 +515,8 @@ __global__ void __launch_bounds__(kBsJoinThreads) beam_select_join_kernel(BeamSe
                 pool_flat[at] = w * a.n_vocab + tok;
             }
         });
-    cluster.sync();
+    if (cs > 1) cluster.sync();
+    else __syncthreads();
     if (cr != 0) return;
     uint32_t n = s_n;
     __syncthreads();
@@ -540,18 +578,18 @@ __global__ void __launch_bounds__(kBsJoinThreads) beam_select_join_kernel(BeamSe
         __syncthreads();
         n = s_n;
     }
-    // each warp ranks one entry at a time against all
     const size_t out = (size_t)g * a.n_select;
-    for (uint32_t i = warp; i < n; i += NW) {
+    for (uint32_t i = threadIdx.x; i < n; i += NT) {
         const uint64_t s = s_key[i];
         const uint32_t flat = s_flat[i];
         uint32_t rank = 0;
-        for (uint32_t j = lane; j < n; j += 32) rank += s_key[j] > s || (s_key[j] == s && s_flat[j] < flat);
-        rank = __reduce_add_sync(0xffffffffu, rank);
-        if (lane == 0 && rank < a.n_select) {
+#pragma unroll 4
+        for (uint32_t j = 0; j < n; ++j) rank += (uint32_t)(s_key[j] > s) | ((uint32_t)(s_key[j] == s) & (uint32_t)(s_flat[j] < flat));
+        if (rank < a.n_select) {
+            const uint32_t w = flat / a.n_vocab;
             a.out_scores[out + rank] = (float)beam_unorder64(s);
-            a.parent[out + rank] = (int32_t)(flat / a.n_vocab);
-            a.token[out + rank] = (int32_t)(flat % a.n_vocab);
+            a.parent[out + rank] = (int32_t)w;
+            a.token[out + rank] = (int32_t)(flat - w * a.n_vocab);
         }
     }
     if (n < a.n_select && threadIdx.x < a.n_select) {

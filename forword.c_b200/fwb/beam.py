@@ -14,6 +14,7 @@ workspace of its own.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -39,33 +40,44 @@ class PrefixAttnArgs(ctypes.Structure):
                    ("out", _vp), ("lse", _vp)])
 
 
-def _check(t, what: str, shape, dtype, device: int, last: bool = True) -> None:
-    if t.dtype is not dtype or t.shape != shape or not t.is_cuda or t.get_device() != device:
+# the current stream of torch as a cudaStream_t (the public call builds an object, 3 us)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+def _refuse(t, what: str, shape, dtype, device: int):
+    if t is None:
+        raise ValueError(f"{what} is missing")
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != device:
         raise ValueError(f"{what}: expected {dtype} {tuple(shape)} on cuda:{device}, "
                          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-    if last and t.stride(-1) != 1 and t.shape[-1] > 1:
-        raise ValueError(f"{what}: the last dimension must be contiguous")
+    raise ValueError(f"{what}: the last dimension must be contiguous" if t.dim() > 1 and t.stride(-1) != 1
+                     else f"{what} must be contiguous")
 
 
 class _Plan:
     def __init__(self, device: int | None, bytes_of):
         self.lib = native.product()
         self.device = torch.cuda.current_device() if device is None else int(device)
-        self.workspace_bytes = int(bytes_of())
+        if not 0 <= self.device < torch.cuda.device_count():
+            raise ValueError(f"no device cuda:{self.device}")
+        with torch.cuda.device(self.device):
+            self.workspace_bytes = int(bytes_of())
         if not self.workspace_bytes:
             raise FwbError(_err(self.lib))
         self._ws: dict[int, torch.Tensor] = {}
 
-    def _stream(self) -> tuple[int, int]:
-        """The current stream and the address of this plan's workspace for it."""
+    def _workspace(self, stream: int) -> int:
+        """The address of this plan's workspace for a stream."""
+        ws = self._ws.get(stream)
+        if ws is None:
+            ws = self._ws[stream] = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=f"cuda:{self.device}")
+        return ws.data_ptr()
+
+    def _on_device(self) -> None:
         if torch.cuda.current_device() != self.device:
             raise ValueError(f"the plan is for cuda:{self.device}, the current device is "
                              f"cuda:{torch.cuda.current_device()}")
-        st = torch.cuda.current_stream().cuda_stream
-        ws = self._ws.get(st)
-        if ws is None:
-            ws = self._ws[st] = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=f"cuda:{self.device}")
-        return st, ws.data_ptr()
 
 
 class PrefixAttention(_Plan):
@@ -103,54 +115,78 @@ class PrefixAttention(_Plan):
         self._s = torch.Size((n, n_head_kv, suffix_cap, head_dim))
         self._plen, self._slen = torch.Size((n_group,)), torch.Size((n,))
         self._slots = torch.Size((n, suffix_cap))
+        self._lse = self._q[:3]
+        self._strides = [None, None, None]     # of q, prefix and suffix, as the arguments hold them
 
     def __call__(self, q, prefix_k, prefix_v, suffix_k, suffix_v, prefix_len=None, suffix_len=None, slots=None,
                  out=None, lse=None):
-        a, dt, dev = self.a, self.dtype, self.device
-        _check(q, "q", self._q, dt, dev)
+        a, dt, dev, seen = self.a, self.dtype, self.device, self._strides
+        st = q.stride()
+        if q.dtype is not dt or q.shape != self._q or q.get_device() != dev or st[3] != 1:
+            _refuse(q, "q", self._q, dt, dev)
+        if st != seen[0]:
+            a.q_seq_stride, a.q_token_stride, a.q_head_stride, _ = seen[0] = st
         a.q = q.data_ptr()
-        a.q_seq_stride, a.q_token_stride, a.q_head_stride, _ = q.stride()
         if a.prefix_cap:
-            _check(prefix_k, "prefix_k", self._p, dt, dev)
-            _check(prefix_v, "prefix_v", self._p, dt, dev)
-            st = prefix_k.stride()
-            if prefix_v.stride() != st:
+            k, v, shape = prefix_k, prefix_v, self._p
+            st = k.stride()
+            if k.dtype is not dt or k.shape != shape or k.get_device() != dev or st[3] != 1:
+                _refuse(k, "prefix_k", shape, dt, dev)
+            if v.dtype is not dt or v.shape != shape or v.get_device() != dev:
+                _refuse(v, "prefix_v", shape, dt, dev)
+            if v.stride() != st:
                 raise ValueError("prefix_k and prefix_v must have equal strides")
-            a.prefix_k, a.prefix_v = prefix_k.data_ptr(), prefix_v.data_ptr()
-            a.prefix_group_stride, a.prefix_head_stride, a.prefix_pos_stride, _ = st
+            if st != seen[1]:
+                a.prefix_group_stride, a.prefix_head_stride, a.prefix_pos_stride, _ = seen[1] = st
+            a.prefix_k, a.prefix_v = k.data_ptr(), v.data_ptr()
         if a.suffix_cap:
-            _check(suffix_k, "suffix_k", self._s, dt, dev)
-            _check(suffix_v, "suffix_v", self._s, dt, dev)
-            st = suffix_k.stride()
-            if suffix_v.stride() != st:
+            k, v, shape = suffix_k, suffix_v, self._s
+            st = k.stride()
+            if k.dtype is not dt or k.shape != shape or k.get_device() != dev or st[3] != 1:
+                _refuse(k, "suffix_k", shape, dt, dev)
+            if v.dtype is not dt or v.shape != shape or v.get_device() != dev:
+                _refuse(v, "suffix_v", shape, dt, dev)
+            if v.stride() != st:
                 raise ValueError("suffix_k and suffix_v must have equal strides")
-            a.suffix_k, a.suffix_v = suffix_k.data_ptr(), suffix_v.data_ptr()
-            a.suffix_seq_stride, a.suffix_head_stride, a.suffix_pos_stride, _ = st
-        a.prefix_len = a.suffix_len = a.slots = None
-        if prefix_len is not None:
-            _check(prefix_len, "prefix_len", self._plen, torch.int32, dev)
-            a.prefix_len = prefix_len.data_ptr()
-        if suffix_len is not None:
-            _check(suffix_len, "suffix_len", self._slen, torch.int32, dev)
-            a.suffix_len = suffix_len.data_ptr()
-        if slots is not None and a.suffix_cap:
-            _check(slots, "slots", self._slots, torch.int32, dev)
-            a.slots, a.slots_stride = slots.data_ptr(), slots.stride(0)
+            if st != seen[2]:
+                a.suffix_seq_stride, a.suffix_head_stride, a.suffix_pos_stride, _ = seen[2] = st
+            a.suffix_k, a.suffix_v = k.data_ptr(), v.data_ptr()
+        i32 = torch.int32
+        if prefix_len is None:
+            a.prefix_len = None
+        else:
+            t = prefix_len
+            if t.dtype is not i32 or t.shape != self._plen or t.get_device() != dev or not t.is_contiguous():
+                _refuse(t, "prefix_len", self._plen, i32, dev)
+            a.prefix_len = t.data_ptr()
+        if suffix_len is None:
+            a.suffix_len = None
+        else:
+            t = suffix_len
+            if t.dtype is not i32 or t.shape != self._slen or t.get_device() != dev or not t.is_contiguous():
+                _refuse(t, "suffix_len", self._slen, i32, dev)
+            a.suffix_len = t.data_ptr()
+        if slots is None or not a.suffix_cap:
+            a.slots = None
+        else:
+            t = slots
+            st = t.stride()
+            if t.dtype is not i32 or t.shape != self._slots or t.get_device() != dev or st[1] != 1:
+                _refuse(t, "slots", self._slots, i32, dev)
+            a.slots, a.slots_stride = t.data_ptr(), st[0]
         if out is None:
             out = torch.empty(self._q, dtype=dt, device=q.device)
-        else:
-            _check(out, "out", self._q, dt, dev)
-            if not out.is_contiguous():
-                raise ValueError("out must be contiguous")
+        elif out.dtype is not dt or out.shape != self._q or out.get_device() != dev or not out.is_contiguous():
+            _refuse(out, "out", self._q, dt, dev)
         if lse is None:
-            lse = torch.empty(self._q[:3], dtype=torch.float32, device=q.device)
-        else:
-            _check(lse, "lse", self._q[:3], torch.float32, dev)
-            if not lse.is_contiguous():
-                raise ValueError("lse must be contiguous")
+            lse = torch.empty(self._lse, dtype=torch.float32, device=q.device)
+        elif (lse.dtype is not torch.float32 or lse.shape != self._lse or lse.get_device() != dev
+              or not lse.is_contiguous()):
+            _refuse(lse, "lse", self._lse, torch.float32, dev)
         a.out, a.lse = out.data_ptr(), lse.data_ptr()
-        stream, ws = self._stream()
-        if self.lib.fwb_prefix_attention_dev(self._ref, ws, self.workspace_bytes, stream) != 0:
+        self._on_device()
+        stream = _raw_stream(dev)
+        if self.lib.fwb_prefix_attention_dev(self._ref, self._workspace(stream), self.workspace_bytes, stream) != 0:
             raise FwbError(_err(self.lib))
         return out, lse
 
@@ -176,53 +212,59 @@ class BeamSelect(_Plan):
         self._o = torch.Size((n_group, n_select))
 
     def __call__(self, logits, scores, out_scores=None, parent=None, token=None):
-        dev = self.device
-        _check(logits, "logits", self._x, self.dtype, dev)
-        _check(scores, "scores", self._c, torch.float32, dev)
-        sg, sw, _ = logits.stride()
-        if self._x[1] == 1:
-            sw = sg if self._x[0] > 1 else self._x[2]
-        elif self._x[0] > 1 and sg != self._x[1] * sw:
+        dev, o, f32, i32 = self.device, self._o, torch.float32, torch.int32
+        sg, sw, sv = logits.stride()
+        n_group, n_beam, n_vocab = self._x
+        if (logits.dtype is not self.dtype or logits.shape != self._x or logits.get_device() != dev
+                or (sv != 1 and n_vocab > 1)):
+            _refuse(logits, "logits", self._x, self.dtype, dev)
+        if n_beam == 1:
+            sw = sg if n_group > 1 else n_vocab
+        elif n_group > 1 and sg != n_beam * sw:
             raise ValueError("logits: all rows must be equally far apart")
-        if not scores.is_contiguous():
-            raise ValueError("scores must be contiguous")
+        if scores.dtype is not f32 or scores.shape != self._c or scores.get_device() != dev or not scores.is_contiguous():
+            _refuse(scores, "scores", self._c, f32, dev)
         if out_scores is None:
-            out_scores = torch.empty(self._o, dtype=torch.float32, device=logits.device)
+            out_scores = torch.empty(o, dtype=f32, device=logits.device)
+        elif (out_scores.dtype is not f32 or out_scores.shape != o or out_scores.get_device() != dev
+              or not out_scores.is_contiguous()):
+            _refuse(out_scores, "out_scores", o, f32, dev)
         if parent is None:
-            parent = torch.empty(self._o, dtype=torch.int32, device=logits.device)
+            parent = torch.empty(o, dtype=i32, device=logits.device)
+        elif parent.dtype is not i32 or parent.shape != o or parent.get_device() != dev or not parent.is_contiguous():
+            _refuse(parent, "parent", o, i32, dev)
         if token is None:
-            token = torch.empty(self._o, dtype=torch.int32, device=logits.device)
-        for t, what, dt in ((out_scores, "out_scores", torch.float32), (parent, "parent", torch.int32),
-                            (token, "token", torch.int32)):
-            _check(t, what, self._o, dt, dev)
-            if not t.is_contiguous():
-                raise ValueError(f"{what} must be contiguous")
-        stream, ws = self._stream()
+            token = torch.empty(o, dtype=i32, device=logits.device)
+        elif token.dtype is not i32 or token.shape != o or token.get_device() != dev or not token.is_contiguous():
+            _refuse(token, "token", o, i32, dev)
+        self._on_device()
+        stream = _raw_stream(dev)
         if self.lib.fwb_beam_select_dev(logits.data_ptr(), *self._sizes, sw, scores.data_ptr(), self.n_select,
-                                        out_scores.data_ptr(), parent.data_ptr(), token.data_ptr(), ws,
-                                        self.workspace_bytes, stream) != 0:
+                                        out_scores.data_ptr(), parent.data_ptr(), token.data_ptr(),
+                                        self._workspace(stream), self.workspace_bytes, stream) != 0:
             raise FwbError(_err(self.lib))
         return out_scores, parent, token
 
 
-def _runs(shape, strides, size: int):
-    """State [n_outer, slots, ...] of one or two tensors (their strides) as
-    (n_inner, run bytes, inner stride of each in bytes): the trailing
-    dimensions as one level of equally spaced runs."""
+@functools.lru_cache(maxsize=256)
+def _runs(shape, st, dt, size: int):
+    """State [n_outer, slots, ...] with the strides st and dt of its source and
+    destination as (n_inner, run bytes, inner stride of each in bytes): the
+    trailing dimensions as one level of equally spaced runs."""
     run, d = 1, len(shape) - 1
-    while d >= 2 and (shape[d] == 1 or all(st[d] == run for st in strides)):  # contiguous in each
+    while d >= 2 and (shape[d] == 1 or st[d] == dt[d] == run):  # contiguous in both
         run *= shape[d]
         d -= 1
     if d < 2:
-        return 1, run * size, [0] * len(strides)
-    n, inner = shape[d], [st[d] for st in strides]
-    for k in range(d - 1, 1, -1):                                             # dimensions that nest into that spacing
+        return 1, run * size, 0, 0
+    n = shape[d]
+    for k in range(d - 1, 1, -1):                               # dimensions that nest into that spacing
         if shape[k] == 1:
             continue
-        if any(st[k] != i * n for st, i in zip(strides, inner)):
+        if st[k] != st[d] * n or dt[k] != dt[d] * n:
             raise ValueError("reorder: the dimensions after the slots must be contiguous runs at one spacing")
         n *= shape[k]
-    return n, run * size, [i * size for i in inner]
+    return n, run * size, st[d] * size, dt[d] * size
 
 
 def reorder(src, parent, dst=None):
@@ -233,24 +275,22 @@ def reorder(src, parent, dst=None):
     runs).  parent int32 [n_group, n_beam].  dst None: in place."""
     if dst is None:
         dst = src
-    if not src.is_cuda or src.dim() < 2 or dst.shape != src.shape or dst.dtype is not src.dtype:
+    shape, st, dt, dev = src.shape, src.stride(), dst.stride(), src.get_device()
+    if len(shape) < 2 or dev < 0 or dst.shape != shape or dst.dtype is not src.dtype:
         raise ValueError("reorder: src and dst must be CUDA tensors of the same shape and type, [n_outer, slots, ...]")
-    dev = src.get_device()
     if dst.get_device() != dev or torch.cuda.current_device() != dev:
         raise ValueError("reorder: src, dst and the current device differ")
-    if parent.dim() != 2 or parent.numel() != src.shape[1]:
+    ps = parent.shape
+    if len(ps) != 2 or ps[0] * ps[1] != shape[1]:
         raise ValueError("reorder: parent must be [n_group, n_beam] with n_group * n_beam slots")
-    _check(parent, "parent", parent.shape, torch.int32, dev)
-    if not parent.is_contiguous():
-        raise ValueError("parent must be contiguous")
+    if parent.dtype is not torch.int32 or parent.get_device() != dev or not parent.is_contiguous():
+        _refuse(parent, "parent", ps, torch.int32, dev)
     if src.numel() == 0:
         return dst
     size = src.element_size()
-    st, dt = src.stride(), dst.stride()
-    n_in, run, inner = _runs(src.shape, (st, dt), size)
+    n_in, run, si, di = _runs(shape, st, dt, size)
     lib = native.product()
-    if lib.fwb_beam_reorder_dev(src.data_ptr(), dst.data_ptr(), parent.data_ptr(), src.shape[0], *parent.shape, n_in,
-                                run, st[0] * size, st[1] * size, inner[0], dt[0] * size, dt[1] * size, inner[1],
-                                torch.cuda.current_stream().cuda_stream) != 0:
+    if lib.fwb_beam_reorder_dev(src.data_ptr(), dst.data_ptr(), parent.data_ptr(), shape[0], ps[0], ps[1], n_in, run,
+                                st[0] * size, st[1] * size, si, dt[0] * size, dt[1] * size, di, _raw_stream(dev)) != 0:
         raise FwbError(_err(lib))
     return dst
