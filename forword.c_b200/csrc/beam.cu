@@ -274,16 +274,30 @@ bool run_select(const BeamSelectArgs &k, cudaStream_t st) {
 }
 
 // --- reordering -------------------------------------------------------------------
+template <typename V, int NB>
+bool launch_reorder(const BeamReorderArgs &k, uint64_t n, cudaStream_t st) {
+    const uint64_t grid = (n + kBrThreads - 1) / kBrThreads;
+    if (n + kBrThreads <= 0xffffffffu)
+        beam_reorder_kernel<V, NB, uint32_t><<<(unsigned)grid, kBrThreads, 0, st>>>(k);
+    else
+        beam_reorder_kernel<V, NB, uint64_t><<<(unsigned)grid, kBrThreads, 0, st>>>(k);
+    return launched(cudaGetLastError(), "fwb_beam_reorder launch");
+}
+
 template <typename V>
 bool run_reorder(BeamReorderArgs &k, size_t run_bytes, cudaStream_t st) {
     const size_t n_col = run_bytes / sizeof(V);
-    if (n_col > 0x7fffffffu) return fail("fwb_beam_reorder: run too long");
+    const uint64_t rows = (uint64_t)k.n_outer * k.n_inner;  // below 2^62
+    if (n_col > 0xffffffffu || rows > ((uint64_t)1 << 38) / k.n_group || rows * k.n_group > ((uint64_t)1 << 38) / n_col)
+        return fail("fwb_beam_reorder: state too large");
     k.n_col = (uint32_t)n_col;
-    const uint64_t n = (uint64_t)k.n_outer * k.n_group * k.n_inner * n_col;
-    const unsigned grid = (unsigned)std::min<uint64_t>((n + kBrThreads - 1) / kBrThreads, 148 * 16);
-    if (k.n_beam <= 8) beam_reorder_kernel<V, 8><<<grid, kBrThreads, 0, st>>>(k);
-    else beam_reorder_kernel<V, 64><<<grid, kBrThreads, 0, st>>>(k);
-    return launched(cudaGetLastError(), "fwb_beam_reorder launch");
+    const uint64_t n = rows * k.n_group * n_col;
+    if (k.n_beam <= 4) return launch_reorder<V, 4>(k, n, st);
+    if (k.n_beam <= 8) return launch_reorder<V, 8>(k, n, st);
+    if (k.n_beam <= 16) return launch_reorder<V, 16>(k, n, st);
+    if constexpr (sizeof(V) < 16)
+        if (k.n_beam > 32) return launch_reorder<V, 64>(k, n, st);
+    return launch_reorder<V, 32>(k, n, st);
 }
 
 }  // namespace
@@ -392,8 +406,12 @@ int fwb_beam_reorder_dev(const void *d_src, void *d_dst, const int32_t *d_parent
     const uint64_t mix = s0 | d0 | run_bytes | src_outer_stride | src_slot_stride | src_inner_stride |
                          dst_outer_stride | dst_slot_stride | dst_inner_stride;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const bool ok = mix % 16 == 0 ? run_reorder<uint4>(k, run_bytes, st)
-                  : mix % 4 == 0 ? run_reorder<uint32_t>(k, run_bytes, st) : run_reorder<uint8_t>(k, run_bytes, st);
+    // 16 bytes a column where everything allows it, 8 for the largest groups,
+    // whose columns a thread could not hold otherwise
+    const bool ok = mix % 16 == 0 && n_beam <= 32 ? run_reorder<uint4>(k, run_bytes, st)
+                  : mix % 8 == 0                  ? run_reorder<uint2>(k, run_bytes, st)
+                  : mix % 4 == 0                  ? run_reorder<uint32_t>(k, run_bytes, st)
+                                                  : run_reorder<uint8_t>(k, run_bytes, st);
     return ok ? 0 : -1;
 }
 

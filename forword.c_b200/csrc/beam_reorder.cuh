@@ -26,30 +26,37 @@ struct BeamReorderArgs {
 constexpr int kBrThreads = 256;
 constexpr uint32_t kBrMaxBeams = 64;
 
-// V: the column's type (16, 4 or 1 bytes); NB: the most beams of a group.
-template <typename V, int NB>
+// V: the column's type; NB: the most beams of a group; I: the type that
+// counts all columns.  One column per thread: a thread has the loads of all
+// moved beams in flight at once, which is what the memory needs.  Slots that
+// keep their own state in place are neither read nor written.
+template <typename V, int NB, typename I>
 __global__ void __launch_bounds__(kBrThreads) beam_reorder_kernel(BeamReorderArgs a) {
-    const uint64_t n = (uint64_t)a.n_outer * a.n_group * a.n_inner * a.n_col;
-    for (uint64_t i = (uint64_t)blockIdx.x * kBrThreads + threadIdx.x; i < n; i += (uint64_t)gridDim.x * kBrThreads) {
-        const uint32_t col = i % a.n_col;
-        uint64_t r = i / a.n_col;
-        const uint32_t in = r % a.n_inner;
-        r /= a.n_inner;
-        const uint32_t g = r % a.n_group, o = r / a.n_group;
-        const uint8_t *src = a.src + o * a.src_outer + in * a.src_inner + (size_t)col * sizeof(V);
-        uint8_t *dst = a.dst + o * a.dst_outer + in * a.dst_inner + (size_t)col * sizeof(V);
-        const int32_t *par = a.parent + (size_t)g * a.n_beam;
-        V v[NB];
+    const I i = (I)blockIdx.x * kBrThreads + threadIdx.x;
+    I r = i / a.n_col;
+    const uint32_t col = (uint32_t)(i - r * a.n_col);
+    I t = r / a.n_inner;
+    const uint32_t in = (uint32_t)(r - t * a.n_inner);
+    const uint32_t o = (uint32_t)(t / a.n_group), g = (uint32_t)(t - (I)o * a.n_group);
+    if (o >= a.n_outer) return;
+    const uint8_t *src = a.src + o * a.src_outer + in * a.src_inner + (size_t)col * sizeof(V) +
+                         (size_t)g * a.n_beam * a.src_slot;
+    uint8_t *dst = a.dst + o * a.dst_outer + in * a.dst_inner + (size_t)col * sizeof(V) +
+                   (size_t)g * a.n_beam * a.dst_slot;
+    const int32_t *par = a.parent + (size_t)g * a.n_beam;
+    const bool in_place = a.src == a.dst;
+    V v[NB];
+    uint32_t from[NB];
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-            if (b < a.n_beam) {
-                const uint32_t p = (uint32_t)par[b] < a.n_beam ? (uint32_t)par[b] : (uint32_t)b;
-                v[b] = *reinterpret_cast<const V *>(src + ((size_t)g * a.n_beam + p) * a.src_slot);
-            }
+    for (int b = 0; b < NB; ++b)
+        if (b < a.n_beam) {
+            const uint32_t p = (uint32_t)par[b];
+            from[b] = p < a.n_beam ? p : (uint32_t)b;
+            if (!in_place || from[b] != b) v[b] = *reinterpret_cast<const V *>(src + from[b] * a.src_slot);
+        }
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-            if (b < a.n_beam) *reinterpret_cast<V *>(dst + ((size_t)g * a.n_beam + b) * a.dst_slot) = v[b];
-    }
+    for (int b = 0; b < NB; ++b)
+        if (b < a.n_beam && (!in_place || from[b] != b)) *reinterpret_cast<V *>(dst + b * a.dst_slot) = v[b];
 }
 
 }  // namespace fwb
