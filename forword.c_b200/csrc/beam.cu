@@ -33,7 +33,7 @@ cudaError_t launch_after(F *fn, dim3 grid, unsigned threads, unsigned cluster, c
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
-    cfg.stream = st;
+    cfg.stream = st;  // (no dynamic shared memory)
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -140,7 +140,7 @@ bool attn_layout(const fwb_prefix_attn_t *a, AttnLayout &L) {
     L.pitems = a->prefix_cap ? (size_t)a->n_group * a->n_head_kv * L.ptiles : 0;
     L.sitems = a->suffix_cap ? (size_t)a->n_group * a->n_beam * a->n_head_kv * L.stiles : 0;
     const uint64_t units = L.pitems * ((a->prefix_cap + 15) / 16) + L.sitems * ((a->suffix_cap + 15) / 16);
-    if (L.pitems + L.sitems > 0x3fffffffu || units >> 40)
+    if (L.pitems + L.sitems > 0x3fffffffu || units > 0x7fffffffu)
         return fail("fwb_prefix_attention: too many rows times positions");
     L.ctas = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(2 * device_sms(), units));
     size_t at = 0;
@@ -163,11 +163,13 @@ bool attn_layout(const fwb_prefix_attn_t *a, AttnLayout &L) {
 template <typename T, int HD, int RWP, int RWS>
 bool launch_attn(const BeamAttnArgs &k, const BeamAttnPlan &p, cudaStream_t st) {
     static bool ready[64] = {};
-    constexpr uint32_t smem = beam_attn_smem<T, HD>();
+    constexpr uint32_t smem = beam_attn_smem<T, HD, RWP, RWS>();
     if (!opt_in(beam_attn_kernel<T, HD, RWP, RWS>, smem, ready, "fwb_prefix_attention")) return false;
     beam_attn_kernel<T, HD, RWP, RWS><<<p.ctas, kBaThreads, smem, st>>>(k, p);
-    beam_attn_join_kernel<T, HD><<<dim3(k.n_group * k.n_beam * k.n_query, k.n_head), kBaThreads, 0, st>>>(k, p);
-    return launched(cudaGetLastError(), "fwb_prefix_attention launch");
+    if (!launched(cudaGetLastError(), "fwb_prefix_attention launch")) return false;
+    return launched(launch_after(beam_attn_join_kernel<T, HD>, dim3(k.n_group * k.n_beam * k.n_query, k.n_head),
+                                 kBaThreads, 1, st, k, p),
+                    "fwb_prefix_attention launch");
 }
 
 template <typename T, int HD>

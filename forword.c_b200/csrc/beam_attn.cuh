@@ -63,7 +63,6 @@ __device__ __forceinline__ uint32_t beam_len(const int32_t *len, uint32_t i, uin
 // ---------------------------------------------------------------------------
 constexpr uint32_t kBaUnit = 16;      // positions
 constexpr int kBaThreads = 128;       // four warps
-constexpr int kBaStages = 3;
 constexpr uint32_t kBaSRows = 16;     // least rows of a tile
 
 struct BeamAttnPlan {
@@ -88,58 +87,50 @@ __device__ __forceinline__ uint32_t beam_part_len(const BeamAttnArgs &a, uint32_
 }
 __device__ __forceinline__ uint32_t beam_units(uint32_t len) { return (len + kBaUnit - 1) / kBaUnit; }
 
-// The cursor of this CTA's first unit; false when it has none.  One scan of
-// the parts' lengths by the whole block.
-__device__ inline bool beam_first(const BeamAttnArgs &a, const BeamAttnPlan &p, BeamCursor &c) {
-    __shared__ uint64_t s_warp[kBaThreads / 32];
-    __shared__ uint32_t s_part;
-    __shared__ uint64_t s_off;
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t parts = a.n_group + a.n_group * a.n_beam;
-    uint64_t sum = 0;
-    for (uint32_t i = threadIdx.x; i < parts; i += kBaThreads)
-        sum += (uint64_t)beam_units(beam_part_len(a, i)) * a.n_kv * (i < a.n_group ? p.ptiles : p.stiles);
-    uint64_t t = sum;
-    for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-    if (lane == 0) s_warp[warp] = t;
-    __syncthreads();
-    uint64_t total = 0;
-    for (int w = 0; w < kBaThreads / 32; ++w) total += s_warp[w];
+// Units of a part in the line.
+__device__ __forceinline__ uint32_t beam_part_units(const BeamAttnArgs &a, const BeamAttnPlan &p, uint32_t part) {
+    return beam_units(beam_part_len(a, part)) * a.n_kv * (part < a.n_group ? p.ptiles : p.stiles);
+}
+
+// The cursor of this CTA's first unit; false when it has none.  Every warp
+// scans the parts' lengths for itself, so no barrier is waited for.
+__device__ __forceinline__ bool beam_first(const BeamAttnArgs &a, const BeamAttnPlan &p, BeamCursor &c) {
+    const uint32_t lane = threadIdx.x & 31, parts = a.n_group + a.n_group * a.n_beam;
+    uint32_t mine = lane < parts ? beam_part_units(a, p, lane) : 0, total = mine;  // of the first 32 parts
+    for (uint32_t i = lane + 32; i < parts; i += 32) total += beam_part_units(a, p, i);
+    total = __reduce_add_sync(0xffffffffu, total);
     // with fewer units than CTAs the first ones take one each, so that the
     // CTAs of an item are neighbours
-    const uint64_t ctas = total < p.ctas ? total : p.ctas;
-    if (blockIdx.x >= ctas) return false;  // the same in every thread
-    const uint64_t lo = blockIdx.x * total / ctas, hi = (blockIdx.x + 1) * total / ctas;
-    uint64_t base = 0;
-    for (uint32_t i0 = 0; i0 < parts; i0 += kBaThreads) {
-        const uint32_t i = i0 + threadIdx.x;
-        uint64_t w = 0;
-        if (i < parts) w = (uint64_t)beam_units(beam_part_len(a, i)) * a.n_kv * (i < a.n_group ? p.ptiles : p.stiles);
-        uint64_t inc = w;
+    const uint32_t ctas = min(total, p.ctas);
+    if (blockIdx.x >= ctas) return false;
+    const uint32_t per = total / ctas, more = total - per * ctas;  // the first `more` CTAs take one more
+    uint32_t off = blockIdx.x * per + min(blockIdx.x, more);
+    c.left = per + (blockIdx.x < more);
+    for (uint32_t i0 = 0;; i0 += 32) {
+        if (i0) mine = i0 + lane < parts ? beam_part_units(a, p, i0 + lane) : 0;
+        uint32_t upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const uint64_t v = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= (uint32_t)o) inc += v;
+            const uint32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= (uint32_t)o) upto += v;
         }
-        __syncthreads();
-        if (lane == 31) s_warp[warp] = inc;
-        __syncthreads();
-        uint64_t before = base;
-        for (uint32_t v = 0; v < warp; ++v) before += s_warp[v];
-        const uint64_t first = before + inc - w;
-        if (w && lo >= first && lo < first + w) { s_part = i; s_off = lo - first; }
-        for (int v = 0; v < kBaThreads / 32; ++v) base += s_warp[v];
-        if (base > lo) break;  // the same in every thread
+        const uint32_t hit = __ballot_sync(0xffffffffu, off < upto);
+        if (hit) {
+            const int at = __ffs(hit) - 1;
+            c.part = i0 + at;
+            off -= __shfl_sync(0xffffffffu, upto - mine, at);
+            break;
+        }
+        off -= __shfl_sync(0xffffffffu, upto, 31);
+        if (i0 + 32 >= parts) return false;  // lengths that changed under the call
     }
-    __syncthreads();
-    c.part = s_part;
     c.len = beam_part_len(a, c.part);
     const uint32_t units = beam_units(c.len), tiles = c.part < a.n_group ? p.ptiles : p.stiles;
-    const uint32_t item = (uint32_t)(s_off / units);
+    if (units == 0) return false;            // likewise
+    const uint32_t item = off / units;
     c.kvh = item / tiles;
-    c.tile = item % tiles;
-    c.pos = (uint32_t)(s_off % units) * kBaUnit;
-    c.left = (uint32_t)(hi - lo);
+    c.tile = item - c.kvh * tiles;
+    c.pos = (off - item * units) * kBaUnit;
     return true;
 }
 
@@ -226,9 +217,21 @@ struct BeamTile {
     }
 };
 
-template <typename T, int HD>
+// Stages of tiles: fp32 has the query rows in shared memory too (their
+// registers would be twice the 16-bit types'), and two stages leave room for
+// three CTAs.
+template <typename T>
+constexpr int kBaStages = sizeof(T) == 2 ? 3 : 2;
+// Behind them: fp32 query rows of the tile's row groups, and in the same place
+// the outputs that warps sharing rows hand over at an item's end.
+template <typename T, int HD, int RW>
+constexpr uint32_t beam_attn_rows_smem() {
+    return sizeof(T) == 4 ? RW * 16 * HD * 4 : RW < 4 ? RW * 16 * HD * 4 : 0;
+}
+template <typename T, int HD, int RWP, int RWS>
 constexpr uint32_t beam_attn_smem() {
-    return 2 * BeamTile<T, HD>::kBytes * kBaStages + 2 * 16 * HD * 4 + 2 * 16 * 8;
+    constexpr uint32_t p = beam_attn_rows_smem<T, HD, RWP>(), s = beam_attn_rows_smem<T, HD, RWS>();
+    return 2 * BeamTile<T, HD>::kBytes * kBaStages<T> + (p > s ? p : s);
 }
 
 // This CTA's next tile of positions from the cursor into stage `st`: K and V
@@ -304,7 +307,7 @@ __device__ __forceinline__ void beam_softmax(float (*sc)[4], float sl2, float *m
 // Rows of one warp: 16 query rows in registers, their output, maximum, sum.
 template <typename T, int HD>
 struct BeamRows {
-    uint32_t q[HD * sizeof(T) / 8];  // matrix operand A: 16-bit pairs, or fp32 values
+    uint32_t q[sizeof(T) == 2 ? HD / 4 : 1];  // matrix operand A, 16-bit types (fp32: in shared memory)
     float o[HD / 8][4];
     float m[2], l[2];
     int32_t lim[2];                  // positions that rows g and g + 8 see (-1: no such row)
@@ -329,7 +332,7 @@ __device__ __forceinline__ const T *beam_q_row(const BeamAttnArgs &a, const Beam
 }
 
 template <typename T, int HD>
-__device__ __forceinline__ void beam_rows_init(const BeamAttnArgs &a, const BeamCursor &c, uint32_t r0,
+__device__ __forceinline__ void beam_rows_init(const BeamAttnArgs &a, const BeamCursor &c, uint32_t r0, uint32_t qs,
                                                BeamRows<T, HD> &w) {
     const uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const T *q[2];
@@ -345,19 +348,17 @@ __device__ __forceinline__ void beam_rows_init(const BeamAttnArgs &a, const Beam
                 w.q[4 * k + e] = p && d < a.hd ? *reinterpret_cast<const uint32_t *>(p + d) : 0u;
             }
     } else {
-        // the 16 dimensions 16 k ..: lane t takes 4 t .. 4 t + 3, the first two
-        // as columns t and t + 4 of one product and the others of the next
+        // Warps that share rows write the same values to the same places, and
+        // each lane reads back only what it wrote.
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const uint32_t d = 16 * k + 4 * t;
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (q[e] && d < a.hd) v = *reinterpret_cast<const uint4 *>(q[e] + d);
-                w.q[8 * k + e] = v.x;
-                w.q[8 * k + 2 + e] = v.y;
-                w.q[8 * k + 4 + e] = v.z;
-                w.q[8 * k + 6 + e] = v.w;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (q[e] && d < a.hd) v = *reinterpret_cast<const float4 *>(q[e] + d);
+                asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(qs + BeamTile<T, HD>::k_at(g + 8 * e, 4 * k + t)),
+                             "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
             }
     }
 #pragma unroll
@@ -372,8 +373,8 @@ __device__ __forceinline__ void beam_rows_init(const BeamAttnArgs &a, const Beam
 // `at`: the part's position of the tile's first row; `end`: the positions
 // that this segment takes.
 template <typename T, int HD, int KW>
-__device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t ks, uint32_t vs, uint32_t k0, uint32_t at,
-                                          uint32_t end, float sl2) {
+__device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t qs, uint32_t ks, uint32_t vs, uint32_t k0,
+                                          uint32_t at, uint32_t end, float sl2) {
     using Tl = BeamTile<T, HD>;
     const uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     float sc[KW / 8][4];
@@ -392,16 +393,29 @@ __device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t ks, uint3
                 mma16(sc[2 * j + 1], w.q + 4 * k, b[2], b[3], T{});
             }
     } else {
-        float lo[KW / 8][4];
+        // The 16 dimensions 16 k ..: lane t takes 4 t .. 4 t + 3, the first two as
+        // columns t and t + 4 of one product and the others of the next.  The
+        // tensor cores' fp32 sums truncate: the large products are summed from
+        // zero over 16 dimensions and added with one rounded addition; the
+        // small ones, 2^-11 of them, have sums of their own.
+        float lq[KW / 8][4], lk[KW / 8][4];
 #pragma unroll
         for (int j = 0; j < KW / 8; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) lo[j][e] = 0.f;
+            for (int e = 0; e < 4; ++e) lq[j][e] = lk[j][e] = 0.f;
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
             uint32_t ah[8], al[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) tf32_split(__uint_as_float(w.q[8 * k + e]), ah[e], al[e]);
+            for (int e = 0; e < 2; ++e) {
+                float4 v;
+                const uint32_t ad = qs + Tl::k_at(g + 8 * e, 4 * k + t);
+                asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(ad));
+                tf32_split(v.x, ah[e], al[e]);
+                tf32_split(v.y, ah[2 + e], al[2 + e]);
+                tf32_split(v.z, ah[4 + e], al[4 + e]);
+                tf32_split(v.w, ah[6 + e], al[6 + e]);
+            }
 #pragma unroll
             for (int j = 0; j < KW / 8; ++j) {
                 float4 v;
@@ -412,15 +426,11 @@ __device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t ks, uint3
                 tf32_split(v.y, bh[1], bl[1]);
                 tf32_split(v.z, bh[2], bl[2]);
                 tf32_split(v.w, bh[3], bl[3]);
-                // The tensor cores' fp32 sums truncate: the large products are
-                // summed from zero over 16 dimensions and added with one
-                // rounded addition; the small ones, 2^-11 of them, in their
-                // own sum.
                 float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
-                    mma8(lo[j], al + 4 * s, bh[2 * s], bh[2 * s + 1]);
-                    mma8(lo[j], ah + 4 * s, bl[2 * s], bl[2 * s + 1]);
+                    mma8(lq[j], al + 4 * s, bh[2 * s], bh[2 * s + 1]);
+                    mma8(lk[j], ah + 4 * s, bl[2 * s], bl[2 * s + 1]);
                     mma8(acc, ah + 4 * s, bh[2 * s], bh[2 * s + 1]);
                 }
 #pragma unroll
@@ -430,7 +440,7 @@ __device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t ks, uint3
 #pragma unroll
         for (int j = 0; j < KW / 8; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sc[j][e] += lo[j][e];
+            for (int e = 0; e < 4; ++e) sc[j][e] += lq[j][e] + lk[j][e];
     }
     // positions that a row does not see
     const uint32_t first = at + k0, lim0 = min((uint32_t)w.lim[0], end), lim1 = min((uint32_t)w.lim[1], end);
@@ -469,6 +479,14 @@ __device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t ks, uint3
     } else {
         // Again from zero for each tile, added to the output with one rounded
         // fma that does the rescaling too.
+        uint32_t ph[KW / 8][4], pl[KW / 8][4];  // columns t, t + 4: positions 2 t, 2 t + 1
+#pragma unroll
+        for (int k = 0; k < KW / 8; ++k) {
+            tf32_split(sc[k][0], ph[k][0], pl[k][0]);
+            tf32_split(sc[k][2], ph[k][1], pl[k][1]);
+            tf32_split(sc[k][1], ph[k][2], pl[k][2]);
+            tf32_split(sc[k][3], ph[k][3], pl[k][3]);
+        }
 #pragma unroll
         for (int j = 0; j < HD / 32; ++j) {
             float acc[4][4];
@@ -478,11 +496,6 @@ __device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t ks, uint3
                 for (int e = 0; e < 4; ++e) acc[i][e] = 0.f;
 #pragma unroll
             for (int k = 0; k < KW / 8; ++k) {
-                uint32_t ph[4], pl[4];  // columns t, t + 4: positions 2 t, 2 t + 1
-                tf32_split(sc[k][0], ph[0], pl[0]);
-                tf32_split(sc[k][2], ph[1], pl[1]);
-                tf32_split(sc[k][1], ph[2], pl[2]);
-                tf32_split(sc[k][3], ph[3], pl[3]);
                 float v[2][4];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
@@ -495,9 +508,9 @@ __device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t ks, uint3
                     uint32_t h0, l0, h1, l1;
                     tf32_split(v[0][i], h0, l0);
                     tf32_split(v[1][i], h1, l1);
-                    mma8(acc[i], pl, h0, h1);
-                    mma8(acc[i], ph, l0, l1);
-                    mma8(acc[i], ph, h0, h1);
+                    mma8(acc[i], pl[k], h0, h1);
+                    mma8(acc[i], ph[k], l0, l1);
+                    mma8(acc[i], ph[k], h0, h1);
                 }
             }
 #pragma unroll
@@ -508,40 +521,39 @@ __device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t ks, uint3
     }
 }
 
-// Joins the rows of the warps that share them (the upper half gives, the
-// lower half takes, twice with four), then the first writes the item's
-// partial result.  buf: two warps' outputs.
+// Joins the rows of the warps that share them (one after the other hands
+// over to the first), which then writes the item's partial result.  buf: an
+// output of every row group.
 template <typename T, int HD, int RW>
 __device__ __forceinline__ void beam_flush(const BeamAttnArgs &a, const BeamAttnPlan &p, const BeamCursor &c,
-                                           BeamRows<T, HD> &w, float *buf) {
+                                           BeamRows<T, HD> &w, float *buf, float2 *bml) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rg = warp % RW, kg = warp / RW;
     const uint32_t g = lane >> 2, t = lane & 3;
-    float2 *bml = reinterpret_cast<float2 *>(buf + 2 * 16 * HD);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         w.l[h] += __shfl_xor_sync(0xffffffffu, w.l[h], 1);
         w.l[h] += __shfl_xor_sync(0xffffffffu, w.l[h], 2);
     }
-#pragma unroll
-    for (int half = 4 / RW / 2; half >= 1; half >>= 1) {
-        const uint32_t at = (kg % half) * RW + rg;
-        float *ob = buf + at * 16 * HD;
-        if (kg >= half && kg < 2 * half) {
+#pragma unroll 1
+    for (uint32_t from = 1; from < 4 / RW; ++from) {
+        float *ob = buf + rg * 16 * HD;
+        __syncthreads();  // what was here is read
+        if (kg == from) {
 #pragma unroll
             for (int j = 0; j < HD / 8; ++j)
                 *reinterpret_cast<float4 *>(ob + (j * 32 + lane) * 4) =
                     make_float4(w.o[j][0], w.o[j][1], w.o[j][2], w.o[j][3]);
             if (t == 0) {
-                bml[at * 16 + g] = make_float2(w.m[0], w.l[0]);
-                bml[at * 16 + g + 8] = make_float2(w.m[1], w.l[1]);
+                bml[rg * 16 + g] = make_float2(w.m[0], w.l[0]);
+                bml[rg * 16 + g + 8] = make_float2(w.m[1], w.l[1]);
             }
         }
         __syncthreads();
-        if (kg < half) {
+        if (kg == 0) {
             float mine[2], other[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float2 ml = bml[at * 16 + g + 8 * h];
+                const float2 ml = bml[rg * 16 + g + 8 * h];
                 const float mn = fmaxf(w.m[h], ml.x), safe = mn == -INFINITY ? 0.f : mn;
                 mine[h] = exp2_fast(w.m[h] - safe);
                 other[h] = exp2_fast(ml.x - safe);
@@ -557,7 +569,6 @@ __device__ __forceinline__ void beam_flush(const BeamAttnArgs &a, const BeamAttn
                 w.o[j][3] = w.o[j][3] * mine[1] + v.w * other[1];
             }
         }
-        __syncthreads();
     }
     if (kg == 0) {
         const bool pre = c.part < a.n_group;
@@ -590,125 +601,133 @@ __device__ __forceinline__ void beam_flush(const BeamAttnArgs &a, const BeamAttn
 // The positions of the cursor's next tile: within the item and this CTA's units.
 template <typename T, int HD>
 __device__ __forceinline__ uint32_t beam_take(const BeamCursor &c) {
-    return min(min((uint32_t)BeamTile<T, HD>::kKeys, c.len - c.pos), c.left * kBaUnit);
+    return min(min((uint32_t)BeamTile<T, HD>::kKeys, c.len - c.pos), min(c.left, 4u) * kBaUnit);
 }
 __device__ __forceinline__ void beam_advance(BeamCursor &c, uint32_t n) {
     c.pos += n;
     c.left -= (n + kBaUnit - 1) / kBaUnit;
 }
 
-// One segment: the tiles of one item that this CTA takes.  RW warps hold the
-// row groups of 16, and 4 / RW warps share each tile's positions.
+// One tile of the cursor's item: the item's first of this CTA brings in its
+// query rows, the last writes the partial result.  RW warps hold the row
+// groups of 16, and 4 / RW warps share each tile's positions.
 template <typename T, int HD, int RW>
-__device__ __forceinline__ void beam_segment(const BeamAttnArgs &a, const BeamAttnPlan &p, BeamCursor &c,
-                                             BeamCursor &ahead, uint32_t smem, float *buf, uint32_t &stage,
-                                             uint32_t &astage) {
+__device__ __forceinline__ void beam_step(const BeamAttnArgs &a, const BeamAttnPlan &p, BeamCursor &c, bool &fresh,
+                                          BeamRows<T, HD> &w, uint32_t stage, uint32_t rows, float *buf, float2 *bml) {
     using Tl = BeamTile<T, HD>;
     constexpr int KW = Tl::kKeys / (4 / RW);
     const uint32_t warp = threadIdx.x >> 5, rg = warp % RW, kg = warp / RW;
-    const BeamCursor seg = c;
-    BeamRows<T, HD> w;
-    beam_rows_init<T, HD>(a, seg, seg.tile * RW * 16 + rg * 16, w);
-    const uint32_t end = min(seg.len, seg.pos + seg.left * kBaUnit);
-    const float sl2 = a.scale * 1.4426950408889634f;
-    const bool some = __any_sync(0xffffffffu, w.lim[0] >= 0 || w.lim[1] >= 0);
-    while (c.pos < end) {
-        cp_async_wait<kBaStages - 2>();
-        __syncthreads();  // the tile is there for all, and the stage that is filled next is free
-        if (ahead.left) {
-            const uint32_t n = beam_take<T, HD>(ahead);
-            beam_load<T, HD>(a, ahead, n, smem + astage * 2 * Tl::kBytes);
-            beam_advance(ahead, n);
-            if (ahead.left && ahead.pos >= ahead.len) beam_next_item(a, p, ahead);
-            astage = astage + 1 == kBaStages ? 0 : astage + 1;
-        }
-        cp_async_commit();
-        const uint32_t ks = smem + stage * 2 * Tl::kBytes;
-        const uint32_t n = beam_take<T, HD>(c);
-        if (some && kg * KW < n) beam_tile<T, HD, KW>(w, ks, ks + Tl::kBytes, kg * KW, c.pos, end, sl2);
-        beam_advance(c, n);
-        stage = stage + 1 == kBaStages ? 0 : stage + 1;
-    }
-    beam_flush<T, HD, RW>(a, p, seg, w, buf);
-    if (threadIdx.x == 0) {
-        const bool pre = seg.part < a.n_group;
-        const uint32_t item = ((pre ? seg.part : seg.part - a.n_group) * a.n_kv + seg.kvh) * (pre ? p.ptiles : p.stiles) + seg.tile;
+    const uint32_t qs = rows + rg * 16 * HD * 4;
+    if (fresh) beam_rows_init<T, HD>(a, c, c.tile * RW * 16 + rg * 16, qs, w);
+    const bool first = c.pos == 0;
+    const uint32_t n = beam_take<T, HD>(c);
+    if (kg * KW < n && __any_sync(0xffffffffu, w.lim[0] >= 0 || w.lim[1] >= 0))
+        beam_tile<T, HD, KW>(w, qs, stage, stage + Tl::kBytes, kg * KW, c.pos, c.pos + n, a.scale * 1.4426950408889634f);
+    beam_advance(c, n);
+    fresh = c.pos >= c.len || c.left == 0;
+    if (fresh) beam_flush<T, HD, RW>(a, p, c, w, buf, bml);
+    if (threadIdx.x == 0 && (first || c.pos >= c.len)) {
+        const bool pre = c.part < a.n_group;
+        const uint32_t item = ((pre ? c.part : c.part - a.n_group) * a.n_kv + c.kvh) * (pre ? p.ptiles : p.stiles) + c.tile;
         uint2 *cta = (pre ? p.pcta : p.scta) + item;
-        if (seg.pos == 0) cta->x = blockIdx.x;
-        if (end == seg.len) cta->y = blockIdx.x;
+        if (first) cta->x = blockIdx.x;
+        if (c.pos >= c.len) cta->y = blockIdx.x;
     }
-    if (c.left) beam_next_item(a, p, c);
+    if (fresh && c.left) beam_next_item(a, p, c);
 }
 
 // RWP, RWS: row groups of 16 of a prefix / suffix tile.
 template <typename T, int HD, int RWP, int RWS>
-__global__ void __launch_bounds__(kBaThreads, 2) beam_attn_kernel(BeamAttnArgs a, BeamAttnPlan p) {
+__global__ void __launch_bounds__(kBaThreads, sizeof(T) == 4 && RWP == 1 ? 3 : 2)
+    beam_attn_kernel(BeamAttnArgs a, BeamAttnPlan p) {
     using Tl = BeamTile<T, HD>;
+    constexpr int S = kBaStages<T>;
     extern __shared__ __align__(128) uint8_t beam_smem[];
-    const uint32_t smem = smem_u32(beam_smem);
-    float *buf = reinterpret_cast<float *>(beam_smem + 2 * Tl::kBytes * kBaStages);
+    __shared__ float2 bml[2 * 16];
+    const uint32_t smem = smem_u32(beam_smem), rows = smem + 2 * Tl::kBytes * S;
+    float *buf = reinterpret_cast<float *>(beam_smem + 2 * Tl::kBytes * S);
+    pdl_launch();
     BeamCursor c;
     if (!beam_first(a, p, c)) return;
     if (a.hd < HD) {  // the padding of the heads
-        for (uint32_t i = threadIdx.x; i < 2 * Tl::kBytes * kBaStages / 16; i += kBaThreads)
+        for (uint32_t i = threadIdx.x; i < 2 * Tl::kBytes * S / 16; i += kBaThreads)
             reinterpret_cast<uint4 *>(beam_smem)[i] = make_uint4(0, 0, 0, 0);
         __syncthreads();
     }
-    BeamCursor ahead = c;
-    uint32_t stage = 0, astage = 0;
-#pragma unroll
-    for (int i = 0; i < kBaStages - 1; ++i) {
+    BeamCursor ahead = c;  // of the loads
+    BeamRows<T, HD> w;
+    bool fresh = true;
+    uint32_t to = 0, from = 0;  // stages
+#pragma unroll 1
+    for (int i = 0; c.left; ++i) {
+        if (i >= S - 1) {
+            cp_async_wait<S - 2>();
+            __syncthreads();  // the tile is there for all, and the stage that is filled next is free
+        }
         if (ahead.left) {
             const uint32_t n = beam_take<T, HD>(ahead);
-            beam_load<T, HD>(a, ahead, n, smem + astage * 2 * Tl::kBytes);
+            beam_load<T, HD>(a, ahead, n, smem + to * 2 * Tl::kBytes);
             beam_advance(ahead, n);
             if (ahead.left && ahead.pos >= ahead.len) beam_next_item(a, p, ahead);
-            ++astage;
+            to = to + 1 == S ? 0 : to + 1;
         }
         cp_async_commit();
-    }
-    if (astage == kBaStages) astage = 0;
-    while (c.left) {
-        if (RWP == RWS || c.part < a.n_group)
-            beam_segment<T, HD, RWP>(a, p, c, ahead, smem, buf, stage, astage);
-        else
-            beam_segment<T, HD, RWS>(a, p, c, ahead, smem, buf, stage, astage);
+        if (i < S - 1) continue;
+        const uint32_t stage = smem + from * 2 * Tl::kBytes;
+        from = from + 1 == S ? 0 : from + 1;
+        if (RWP == RWS || c.part < a.n_group) beam_step<T, HD, RWP>(a, p, c, fresh, w, stage, rows, buf, bml);
+        else beam_step<T, HD, RWS>(a, p, c, fresh, w, stage, rows, buf, bml);
     }
     cp_async_wait<0>();
 }
 
 // Joins a row's partial results: block (row, head), the warps take the
-// segments in turn, lanes the dimensions.
+// segments in turn, four at a time, lanes the dimensions.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kBaThreads) beam_attn_join_kernel(BeamAttnArgs a, BeamAttnPlan p) {
     constexpr int NW = kBaThreads / 32, V = HD / 32;
-    __shared__ float part[NW][HD], pm[NW], pl[NW];
+    struct alignas(4 * V) Vec { float v[V]; };
+    __shared__ Vec part[NW][32];
+    __shared__ float pm[NW], pl[NW];
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t h = blockIdx.y, kvh = h / a.gq, hg = h % a.gq;
-    const uint32_t s = blockIdx.x / a.n_query, t = blockIdx.x % a.n_query, grp = s / a.n_beam;
-    const uint32_t pr = ((s % a.n_beam) * a.n_query + t) * a.gq + hg, sr = t * a.gq + hg;
-    const uint32_t pi = (grp * a.n_kv + kvh) * p.ptiles + pr / p.prow, si = (s * a.n_kv + kvh) * p.stiles + sr / p.srow;
+    const uint32_t h = blockIdx.y, kvh = h / a.gq, hg = h - kvh * a.gq;
+    const uint32_t s = blockIdx.x / a.n_query, t = blockIdx.x - s * a.n_query, grp = s / a.n_beam;
+    const uint32_t pr = ((s - grp * a.n_beam) * a.n_query + t) * a.gq + hg, sr = t * a.gq + hg;
+    const uint32_t ptile = pr / p.prow, stile = sr / p.srow;
+    const uint32_t pi = (grp * a.n_kv + kvh) * p.ptiles + ptile, si = (s * a.n_kv + kvh) * p.stiles + stile;
+    const bool some_p = beam_part_len(a, grp) != 0, some_s = beam_part_len(a, a.n_group + s) != 0;
+    pdl_wait();
     uint2 pc = make_uint2(1, 0), sc = make_uint2(1, 0);
-    if (beam_part_len(a, grp)) pc = p.pcta[pi];
-    if (beam_part_len(a, a.n_group + s)) sc = p.scta[si];
+    if (some_p) pc = p.pcta[pi];
+    if (some_s) sc = p.scta[si];
     const uint32_t np = pc.y + 1 - pc.x, n = np + (sc.y + 1 - sc.x);
-    float m = -INFINITY, l = 0.f, o[V];
+    // the rows' first slots: of a prefix segment j, and of a suffix segment
+    const size_t prow = (size_t)(pi + pc.x) * p.prow + (pr - ptile * p.prow);
+    const size_t srow = (size_t)(si + sc.x) * p.srow + (sr - stile * p.srow);
+    float m = -INFINITY, l = 0.f;
+    Vec o{};
+    for (uint32_t j0 = warp; j0 < n; j0 += 4 * NW) {
+        float2 ml[4];
+        Vec v[4];
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = 0.f;
-    for (uint32_t j = warp; j < n; j += NW) {
-        const size_t row = j < np ? (size_t)(pi + pc.x + j) * p.prow + pr % p.prow
-                                  : (size_t)(si + sc.x + j - np) * p.srow + sr % p.srow;
-        const float2 ml = (j < np ? p.pml : p.sml)[row];
-        const float *src = (j < np ? p.po : p.so) + row * HD + lane;
-        const float mn = fmaxf(m, ml.x), safe = mn == -INFINITY ? 0.f : mn;
-        const float mine = exp2_fast(m - safe), other = exp2_fast(ml.x - safe);
-        m = mn;
-        l = l * mine + ml.y * other;
+        for (int u = 0; u < 4; ++u) {
+            const uint32_t j = min(j0 + u * NW, n - 1);
+            const size_t row = j < np ? prow + (size_t)j * p.prow : srow + (size_t)(j - np) * p.srow;
+            ml[u] = (j < np ? p.pml : p.sml)[row];
+            v[u] = *reinterpret_cast<const Vec *>((j < np ? p.po : p.so) + row * HD + lane * V);
+        }
 #pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = o[i] * mine + src[32 * i] * other;
+        for (int u = 0; u < 4; ++u) {
+            if (j0 + u * NW >= n) break;
+            const float mn = fmaxf(m, ml[u].x), safe = mn == -INFINITY ? 0.f : mn;
+            const float mine = exp2_fast(m - safe), other = exp2_fast(ml[u].x - safe);
+            m = mn;
+            l = l * mine + ml[u].y * other;
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.v[i] = o.v[i] * mine + v[u].v[i] * other;
+        }
     }
-#pragma unroll
-    for (int i = 0; i < V; ++i) part[warp][lane + 32 * i] = o[i];
+    part[warp][lane] = o;
     if (lane == 0) { pm[warp] = m; pl[warp] = l; }
     __syncthreads();
     float M = -INFINITY, L = 0.f;
@@ -721,7 +740,7 @@ __global__ void __launch_bounds__(kBaThreads) beam_attn_join_kernel(BeamAttnArgs
     for (int w = 0; w < NW; ++w) {
         const float f = exp2_fast(pm[w] - safe);
         L += pl[w] * f;
-        if (d < HD) v += part[w][d] * f;
+        if (d < HD) v += reinterpret_cast<const float *>(part[w])[d] * f;
     }
     const size_t at = (size_t)blockIdx.x * a.n_head + h;
     if (d < a.hd) static_cast<T *>(a.out)[at * a.hd + d] = beam_from_f32<T>(L == 0.f ? 0.f : v / L);
