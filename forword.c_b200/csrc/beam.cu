@@ -160,12 +160,42 @@ bool attn_layout(const fwb_prefix_attn_t *a, AttnLayout &L) {
     return true;
 }
 
+decltype(&cuTensorMapEncodeTiled) map_encoder() {
+    static const auto fn = [] {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                        q == cudaDriverEntryPointSuccess;
+        return ok ? reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(p) : nullptr;
+    }();
+    return fn;
+}
+
+// A cache as a 4-D tensor; false where the copy engine does not take its
+// strides (a head or group repeated by a stride of 0, say).
+bool cache_map(const void *base, size_t e, uint64_t hd, uint64_t cap, uint64_t n_kv, uint64_t outer, uint64_t pos,
+               uint64_t head, uint64_t out, CUtensorMap &map) {
+    const auto enc = map_encoder();
+    if (!cap || !enc) return false;
+    const cuuint64_t dims[4] = {hd, cap, n_kv, outer};
+    cuuint64_t strides[3] = {pos * e, head * e, out * e};
+    for (int i = 0; i < 3; ++i) {
+        if (dims[i + 1] == 1) strides[i] = hd * e;  // never used
+        if (!strides[i] || strides[i] >= (cuuint64_t)1 << 40) return false;
+    }
+    const cuuint32_t box[4] = {(cuuint32_t)(128 / e), kBaUnit, 1, 1}, one[4] = {1, 1, 1, 1};
+    const CUtensorMapDataType type = e == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+    return enc(&map, type, 4, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int HD, int RWP, int RWS>
-bool launch_attn(const BeamAttnArgs &k, const BeamAttnPlan &p, cudaStream_t st) {
+bool launch_attn(const BeamAttnArgs &k, const BeamAttnPlan &p, const BeamMaps &maps, cudaStream_t st) {
     static bool ready[64] = {};
     constexpr uint32_t smem = beam_attn_smem<T, HD, RWP, RWS>();
     if (!opt_in(beam_attn_kernel<T, HD, RWP, RWS>, smem, ready, "fwb_prefix_attention")) return false;
-    beam_attn_kernel<T, HD, RWP, RWS><<<p.ctas, kBaThreads, smem, st>>>(k, p);
+    beam_attn_kernel<T, HD, RWP, RWS><<<p.ctas, kBaThreads + kBaLoader, smem, st>>>(k, p, maps);
     if (!launched(cudaGetLastError(), "fwb_prefix_attention launch")) return false;
     return launched(launch_after(beam_attn_join_kernel<T, HD>, dim3(k.n_group * k.n_beam * k.n_query, k.n_head),
                                  kBaThreads, 1, st, k, p),
@@ -173,13 +203,14 @@ bool launch_attn(const BeamAttnArgs &k, const BeamAttnPlan &p, cudaStream_t st) 
 }
 
 template <typename T, int HD>
-bool pick_attn(const BeamAttnArgs &k, const BeamAttnPlan &p, uint32_t prg, uint32_t srg, cudaStream_t st) {
+bool pick_attn(const BeamAttnArgs &k, const BeamAttnPlan &p, const BeamMaps &maps, uint32_t prg, uint32_t srg,
+               cudaStream_t st) {
     switch (prg * 8 + srg) {
-    case 1 * 8 + 1: return launch_attn<T, HD, 1, 1>(k, p, st);
-    case 2 * 8 + 1: return launch_attn<T, HD, 2, 1>(k, p, st);
-    case 2 * 8 + 2: return launch_attn<T, HD, 2, 2>(k, p, st);
-    case 4 * 8 + 1: return launch_attn<T, HD, 4, 1>(k, p, st);
-    default: return launch_attn<T, HD, 4, 4>(k, p, st);
+    case 1 * 8 + 1: return launch_attn<T, HD, 1, 1>(k, p, maps, st);
+    case 2 * 8 + 1: return launch_attn<T, HD, 2, 1>(k, p, maps, st);
+    case 2 * 8 + 2: return launch_attn<T, HD, 2, 2>(k, p, maps, st);
+    case 4 * 8 + 1: return launch_attn<T, HD, 4, 1>(k, p, maps, st);
+    default: return launch_attn<T, HD, 4, 4>(k, p, maps, st);
     }
 }
 
@@ -197,7 +228,14 @@ bool run_attn(const BeamAttnArgs &k, const AttnLayout &L, uint8_t *ws, cudaStrea
     p.ptiles = L.ptiles;
     p.stiles = L.stiles;
     p.ctas = L.ctas;
-    return k.hd <= 64 ? pick_attn<T, 64>(k, p, L.prg, L.srg, st) : pick_attn<T, 128>(k, p, L.prg, L.srg, st);
+    BeamMaps maps{};
+    p.tma = (cache_map(k.pk, sizeof(T), k.hd, k.pcap, k.n_kv, k.n_group, k.p_pos, k.p_head, k.p_group, maps.pk) &&
+             cache_map(k.pv, sizeof(T), k.hd, k.pcap, k.n_kv, k.n_group, k.p_pos, k.p_head, k.p_group, maps.pv)) |
+            (cache_map(k.sk, sizeof(T), k.hd, k.scap, k.n_kv, k.n_group * k.n_beam, k.s_pos, k.s_head, k.s_seq, maps.sk) &&
+             cache_map(k.sv, sizeof(T), k.hd, k.scap, k.n_kv, k.n_group * k.n_beam, k.s_pos, k.s_head, k.s_seq, maps.sv))
+                << 1;
+    return k.hd <= 64 ? pick_attn<T, 64>(k, p, maps, L.prg, L.srg, st)
+                      : pick_attn<T, 128>(k, p, maps, L.prg, L.srg, st);
 }
 
 // --- selection ------------------------------------------------------------------

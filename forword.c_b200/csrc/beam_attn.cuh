@@ -13,6 +13,7 @@
 //
 // with no visible position: out = 0, lse = -inf.
 #pragma once
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -62,7 +63,8 @@ __device__ __forceinline__ uint32_t beam_len(const int32_t *len, uint32_t i, uin
 // CTA.  A second kernel joins a row's partial results of prefix and suffix.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kBaUnit = 16;      // positions
-constexpr int kBaThreads = 128;       // four warps
+constexpr int kBaThreads = 128;       // four warps that compute
+constexpr int kBaLoader = 32;         // and one that loads
 constexpr uint32_t kBaSRows = 16;     // least rows of a tile
 
 struct BeamAttnPlan {
@@ -72,6 +74,7 @@ struct BeamAttnPlan {
     uint32_t prow, srow;   // rows of a prefix / suffix tile
     uint32_t ptiles, stiles;  // row tiles of a group / of a sequence
     uint32_t ctas;
+    uint32_t tma;          // bit 0: tensor maps of the prefix, 1: of the suffix
 };
 
 // Where a CTA stands in the line of units.
@@ -200,20 +203,21 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// Shared-memory tile: KT rows of HD elements in 16-byte chunks, the chunk
-// index xor-ed by a function of the row so that the reads below touch all
-// banks.  16-bit types: ldmatrix reads 8 consecutive rows of one chunk.
-// fp32: a quarter-warp reads 4 chunks of 2 rows (K), or 2 chunks of the rows
-// 2t, t = 0..3 (V).
+// Set when a bounded wait of the attention kernel ran out; stays until read.
+__device__ uint32_t g_beam_err;
+
+// Shared-memory tile: sub-tiles of 128 bytes of every row, [sub][row][128 B],
+// the 16-byte chunk index xor-ed by the row's low three bits, as the copy
+// engine's 128-byte swizzle does.  ldmatrix (8 rows of one chunk) and the fp32
+// reads of V (2 chunks of the rows 2 t) touch all banks; the fp32 reads of K
+// (4 chunks of 2 rows) take two rounds.
 template <typename T, int HD>
 struct BeamTile {
     static constexpr int kEs = sizeof(T), kChunks = HD * kEs / 16, kKeys = kEs == 2 ? 64 : 32;
+    static constexpr int kSub = HD * kEs / 128;
     static constexpr uint32_t kBytes = kKeys * HD * kEs;  // of K; V the same
-    static __device__ __forceinline__ uint32_t k_at(uint32_t row, uint32_t chunk) {
-        return (row * kChunks + (chunk ^ (kEs == 2 ? row & 7 : (row & 1) << 2))) * 16;
-    }
-    static __device__ __forceinline__ uint32_t v_at(uint32_t row, uint32_t chunk) {
-        return (row * kChunks + (chunk ^ (kEs == 2 ? row & 7 : row & 6))) * 16;
+    static __device__ __forceinline__ uint32_t at(uint32_t row, uint32_t chunk) {
+        return (chunk >> 3) * (kKeys * 128) + row * 128 + (((chunk ^ row) & 7) << 4);
     }
 };
 
@@ -225,56 +229,102 @@ constexpr int kBaStages = sizeof(T) == 2 ? 3 : 2;
 // Behind them: fp32 query rows of the tile's row groups, and in the same place
 // the outputs that warps sharing rows hand over at an item's end.
 template <typename T, int HD, int RW>
-constexpr uint32_t beam_attn_rows_smem() {
+constexpr uint32_t beam_attn_rows_smem() {  // (a row group: 16 rows in the tiles' chunk order)
     return sizeof(T) == 4 ? RW * 16 * HD * 4 : RW < 4 ? RW * 16 * HD * 4 : 0;
 }
+constexpr uint32_t kBaTail = 2 * 3 * 8 + 2 * 16 * 8;  // barriers; maxima and sums that are handed over
 template <typename T, int HD, int RWP, int RWS>
 constexpr uint32_t beam_attn_smem() {
     constexpr uint32_t p = beam_attn_rows_smem<T, HD, RWP>(), s = beam_attn_rows_smem<T, HD, RWS>();
-    return 2 * BeamTile<T, HD>::kBytes * kBaStages<T> + (p > s ? p : s);
+    return 2 * BeamTile<T, HD>::kBytes * kBaStages<T> + (p > s ? p : s) + kBaTail;
 }
 
-// This CTA's next tile of positions from the cursor into stage `st`: K and V
-// rows by 16-byte asynchronous copies (gathered through the slot table in a
-// suffix).  V rows past the part's positions are zeros: their probabilities
-// are zero, and zero times whatever the shared memory held must be zero.
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int32_t x, int32_t y, int32_t z,
+                                            int32_t u, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(u), "r"(smem_u32(bar)) : "memory");
+}
+
+// The caches as 4-D tensors [group or sequence][kv_head][position][dim],
+// boxes of 16 positions and 128 bytes, 128-byte swizzle, zeros past the
+// dimensions.
+struct BeamMaps {
+    CUtensorMap pk, pv, sk, sv;
+};
+
+// n positions of a part into stage `st`, by the loading warp: units of 16
+// positions that stand together by the copy engine (where the strides allow
+// tensor maps), others -- a unit of a suffix whose slots differ -- row by row
+// with 16-byte asynchronous copies.  The stage's barrier takes 32 arrivals.
 template <typename T, int HD>
-__device__ __forceinline__ void beam_load(const BeamAttnArgs &a, const BeamCursor &c, uint32_t n, uint32_t st) {
+__device__ __forceinline__ void beam_load(const BeamAttnArgs &a, const BeamAttnPlan &p, const BeamMaps &maps,
+                                          const BeamCursor &c, uint32_t n, uint32_t st, uint64_t *bar) {
     using Tl = BeamTile<T, HD>;
-    constexpr int CH = Tl::kChunks, RP = kBaThreads / CH;  // rows per pass of the block
-    const uint32_t ch = threadIdx.x % CH, r0 = threadIdx.x / CH;
-    const uint32_t ks = st, vs = st + Tl::kBytes;
-    if (ch * (16 / Tl::kEs) >= a.hd) return;  // the padding of the head stays zero
-    const size_t col = (size_t)ch * (16 / Tl::kEs);
-    if (c.part < a.n_group) {
-        const size_t off = c.part * a.p_group + c.kvh * a.p_head + (size_t)(c.pos + r0) * a.p_pos + col;
-        const T *k = static_cast<const T *>(a.pk) + off, *v = static_cast<const T *>(a.pv) + off;
+    constexpr int NU = Tl::kKeys / kBaUnit, CH = Tl::kChunks, RP = CH < 32 ? 32 / CH : 1;
+    const uint32_t lane = threadIdx.x & 31, ks = st, vs = st + Tl::kBytes, units = (n + kBaUnit - 1) / kBaUnit;
+    const bool pre = c.part < a.n_group;
+    const uint32_t s = c.part - a.n_group;
+    // the cache row's sequence, or group, of rows lane and lane + 32
+    uint32_t seq[(Tl::kKeys + 31) / 32], single = pre ? p.tma & 1 ? 0xfu : 0u : p.tma & 2 ? 0xfu : 0u;
 #pragma unroll
-        for (int i = 0; i < Tl::kKeys / RP; ++i) {
-            const uint32_t row = r0 + i * RP;
-            const size_t step = (size_t)i * RP * a.p_pos;
-            const bool in = row < n;
-            if (in) cp_async16_or_zero(ks + Tl::k_at(row, ch), k + step, true);
-            cp_async16_or_zero(vs + Tl::v_at(row, ch), in ? v + step : v, in);
-        }
-    } else {
-        const uint32_t s = c.part - a.n_group, b0 = s / a.n_beam * a.n_beam;
-        const int32_t *slots = a.slots ? a.slots + s * a.slot_seq + c.pos : nullptr;
-        const size_t head = c.kvh * a.s_head + (size_t)c.pos * a.s_pos + col;
+    for (int i = 0; i < (Tl::kKeys + 31) / 32; ++i) seq[i] = pre ? c.part : s;
+    if (!pre && a.slots) {
+        const uint32_t b0 = s / a.n_beam * a.n_beam;
+        const int32_t *slots = a.slots + s * a.slot_seq + c.pos;
 #pragma unroll
-        for (int i = 0; i < Tl::kKeys / RP; ++i) {
-            const uint32_t row = r0 + i * RP;
-            const bool in = row < n;
-            uint32_t seq = s;
-            if (slots && in) {
+        for (int i = 0; i < (Tl::kKeys + 31) / 32; ++i) {
+            const uint32_t row = lane + 32 * i;
+            if (row < n) {
                 const uint32_t from = (uint32_t)slots[row];
-                if (from < a.n_beam) seq = b0 + from;
+                if (from < a.n_beam) seq[i] = b0 + from;
             }
-            const size_t off = in ? seq * a.s_seq + head + (size_t)row * a.s_pos : 0;
-            if (in) cp_async16_or_zero(ks + Tl::k_at(row, ch), static_cast<const T *>(a.sk) + off, true);
-            cp_async16_or_zero(vs + Tl::v_at(row, ch), static_cast<const T *>(a.sv) + off, in);
+        }
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {  // units whose rows differ
+            const uint32_t row = (u & 1) * kBaUnit, v = seq[u / 2];
+            const uint32_t lead = __shfl_sync(0xffffffffu, v, row);
+            const uint32_t off = __ballot_sync(0xffffffffu, v != lead && lane + (u & ~1) * kBaUnit < n);
+            if (off >> row & 0xffffu) single &= ~(1u << u);
         }
     }
+    uint32_t bytes = 0;
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+        if (u < units && single >> u & 1) bytes += 2 * Tl::kSub * kBaUnit * 128;
+    if (lane == 0 && bytes)
+        asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+#pragma unroll 1
+    for (uint32_t u = 0; u < units; ++u) {
+        const uint32_t r0 = u * kBaUnit;
+        if (single >> u & 1) {
+            const uint32_t from = __shfl_sync(0xffffffffu, u < 2 ? seq[0] : seq[(Tl::kKeys + 31) / 32 - 1], r0 & 31);
+            // one box per lane: K and V, each sub-tile
+            if (lane < 2 * Tl::kSub) {
+                const uint32_t h = lane % Tl::kSub, to = h * (Tl::kKeys * 128) + r0 * 128;
+                const bool k = lane < Tl::kSub;
+                tma_load_4d((k ? ks : vs) + to, pre ? k ? &maps.pk : &maps.pv : k ? &maps.sk : &maps.sv,
+                            (int32_t)(h * (128 / Tl::kEs)), (int32_t)(c.pos + r0), (int32_t)c.kvh, (int32_t)from, bar);
+            }
+            continue;
+        }
+        const uint32_t ch = lane % CH;
+        const bool held = ch * (16 / Tl::kEs) < a.hd;
+        const size_t outer = pre ? a.p_group : a.s_seq, step = pre ? a.p_pos : a.s_pos;
+        const size_t col = (pre ? c.kvh * a.p_head : c.kvh * a.s_head) + (held ? (size_t)ch * (16 / Tl::kEs) : 0);
+        const T *kb = static_cast<const T *>(pre ? a.pk : a.sk) + col, *vb = static_cast<const T *>(pre ? a.pv : a.sv) + col;
+#pragma unroll 4
+        for (uint32_t i = 0; i < kBaUnit; i += RP) {
+            const uint32_t row = r0 + i + lane / CH;
+            const uint32_t from = __shfl_sync(0xffffffffu, u < 2 ? seq[0] : seq[(Tl::kKeys + 31) / 32 - 1], row & 31);
+            if (row < n) {
+                const size_t off = from * outer + (size_t)(c.pos + row) * step;
+                cp_async16_or_zero(ks + Tl::at(row, ch), kb + off, held);
+                cp_async16_or_zero(vs + Tl::at(row, ch), vb + off, held);
+            }
+        }
+    }
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
 // The online softmax of a warp's 16 rows: thread rows g and g + 8 (g = lane
@@ -331,6 +381,12 @@ __device__ __forceinline__ const T *beam_q_row(const BeamAttnArgs &a, const Beam
     return static_cast<const T *>(a.q) + s * a.q_seq + t * a.q_tok + h * a.q_head;
 }
 
+// fp32 query row and chunk: quarter-warps read 4 chunks of 2 rows.
+template <int HD>
+__device__ __forceinline__ uint32_t beam_q_at(uint32_t row, uint32_t chunk) {
+    return (row * (HD / 4) + (chunk ^ ((row & 1) << 2))) * 16;
+}
+
 template <typename T, int HD>
 __device__ __forceinline__ void beam_rows_init(const BeamAttnArgs &a, const BeamCursor &c, uint32_t r0, uint32_t qs,
                                                BeamRows<T, HD> &w) {
@@ -357,7 +413,7 @@ __device__ __forceinline__ void beam_rows_init(const BeamAttnArgs &a, const Beam
                 const uint32_t d = 16 * k + 4 * t;
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (q[e] && d < a.hd) v = *reinterpret_cast<const float4 *>(q[e] + d);
-                asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(qs + BeamTile<T, HD>::k_at(g + 8 * e, 4 * k + t)),
+                asm volatile("st.shared.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(qs + beam_q_at<HD>(g + 8 * e, 4 * k + t)),
                              "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
             }
     }
@@ -370,8 +426,8 @@ __device__ __forceinline__ void beam_rows_init(const BeamAttnArgs &a, const Beam
 }
 
 // One tile: KW positions of it, from row k0 on, for this warp's 16 rows.
-// `at`: the part's position of the tile's first row; `end`: the positions
-// that this segment takes.
+// `at`: the part's position of the tile's first row; `end`: the first
+// position past the tile.
 template <typename T, int HD, int KW>
 __device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t qs, uint32_t ks, uint32_t vs, uint32_t k0,
                                           uint32_t at, uint32_t end, float sl2) {
@@ -388,7 +444,7 @@ __device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t qs, uint3
 #pragma unroll
             for (int j = 0; j < KW / 16; ++j) {
                 uint32_t b[4];
-                ldm_x4(b, ks + Tl::k_at(k0 + 16 * j + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
+                ldm_x4(b, ks + Tl::at(k0 + 16 * j + (lane & 7) + ((lane >> 4) << 3), 2 * k + ((lane >> 3) & 1)));
                 mma16(sc[2 * j], w.q + 4 * k, b[0], b[1], T{});
                 mma16(sc[2 * j + 1], w.q + 4 * k, b[2], b[3], T{});
             }
@@ -409,7 +465,7 @@ __device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t qs, uint3
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 float4 v;
-                const uint32_t ad = qs + Tl::k_at(g + 8 * e, 4 * k + t);
+                const uint32_t ad = qs + beam_q_at<HD>(g + 8 * e, 4 * k + t);
                 asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(ad));
                 tf32_split(v.x, ah[e], al[e]);
                 tf32_split(v.y, ah[2 + e], al[2 + e]);
@@ -419,7 +475,7 @@ __device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t qs, uint3
 #pragma unroll
             for (int j = 0; j < KW / 8; ++j) {
                 float4 v;
-                const uint32_t ad = ks + Tl::k_at(k0 + 8 * j + g, 4 * k + t);
+                const uint32_t ad = ks + Tl::at(k0 + 8 * j + g, 4 * k + t);
                 asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(ad));
                 uint32_t bh[4], bl[4];
                 tf32_split(v.x, bh[0], bl[0]);
@@ -453,13 +509,27 @@ __device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t qs, uint3
     }
     float al[2];
     beam_softmax<KW / 8>(sc, sl2, w.m, w.l, al);
+    if (first + KW > end) {
+        // V rows past the end: their probabilities are zero, and zero times
+        // whatever the memory holds must be zero.  (The warps that share these
+        // rows write the same zeros.)
+        for (uint32_t i = lane; i < KW * Tl::kChunks; i += 32) {
+            const uint32_t row = i / Tl::kChunks;
+            if (first + row >= end)
+                asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(vs + Tl::at(k0 + row, i % Tl::kChunks)), "r"(0) : "memory");
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before the copy engine writes there again
+        __syncwarp();
+    }
     if constexpr (sizeof(T) == 2) {
+        if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {  // rare once the maxima are found
 #pragma unroll
-        for (int j = 0; j < HD / 8; ++j) {
-            w.o[j][0] *= al[0];
-            w.o[j][1] *= al[0];
-            w.o[j][2] *= al[1];
-            w.o[j][3] *= al[1];
+            for (int j = 0; j < HD / 8; ++j) {
+                w.o[j][0] *= al[0];
+                w.o[j][1] *= al[0];
+                w.o[j][2] *= al[1];
+                w.o[j][3] *= al[1];
+            }
         }
 #pragma unroll
         for (int k = 0; k < KW / 16; ++k) {
@@ -471,7 +541,7 @@ __device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t qs, uint3
 #pragma unroll
             for (int j = 0; j < HD / 16; ++j) {
                 uint32_t b[4];
-                ldm_x4_t(b, vs + Tl::v_at(k0 + 16 * k + (lane & 7) + ((lane >> 3) & 1) * 8, 2 * j + (lane >> 4)));
+                ldm_x4_t(b, vs + Tl::at(k0 + 16 * k + (lane & 7) + ((lane >> 3) & 1) * 8, 2 * j + (lane >> 4)));
                 mma16(w.o[2 * j], p, b[0], b[1], T{});
                 mma16(w.o[2 * j + 1], p, b[2], b[3], T{});
             }
@@ -499,7 +569,7 @@ __device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t qs, uint3
                 float v[2][4];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                    const uint32_t ad = vs + Tl::v_at(k0 + 8 * k + 2 * t + r, 8 * j + g);
+                    const uint32_t ad = vs + Tl::at(k0 + 8 * k + 2 * t + r, 8 * j + g);
                     asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];"
                                  : "=f"(v[r][0]), "=f"(v[r][1]), "=f"(v[r][2]), "=f"(v[r][3]) : "r"(ad));
                 }
@@ -537,7 +607,7 @@ __device__ __forceinline__ void beam_flush(const BeamAttnArgs &a, const BeamAttn
 #pragma unroll 1
     for (uint32_t from = 1; from < 4 / RW; ++from) {
         float *ob = buf + rg * 16 * HD;
-        __syncthreads();  // what was here is read
+        bar_sync(1, kBaThreads);  // what was here is read
         if (kg == from) {
 #pragma unroll
             for (int j = 0; j < HD / 8; ++j)
@@ -548,7 +618,7 @@ __device__ __forceinline__ void beam_flush(const BeamAttnArgs &a, const BeamAttn
                 bml[rg * 16 + g + 8] = make_float2(w.m[1], w.l[1]);
             }
         }
-        __syncthreads();
+        bar_sync(1, kBaThreads);
         if (kg == 0) {
             float mine[2], other[2];
 #pragma unroll
@@ -570,6 +640,7 @@ __device__ __forceinline__ void beam_flush(const BeamAttnArgs &a, const BeamAttn
             }
         }
     }
+    if (RW < 4) bar_sync(1, kBaThreads);  // before the next item's rows come into the same place
     if (kg == 0) {
         const bool pre = c.part < a.n_group;
         const uint32_t item = ((pre ? c.part : c.part - a.n_group) * a.n_kv + c.kvh) * (pre ? p.ptiles : p.stiles) + c.tile;
@@ -613,7 +684,8 @@ __device__ __forceinline__ void beam_advance(BeamCursor &c, uint32_t n) {
 // groups of 16, and 4 / RW warps share each tile's positions.
 template <typename T, int HD, int RW>
 __device__ __forceinline__ void beam_step(const BeamAttnArgs &a, const BeamAttnPlan &p, BeamCursor &c, bool &fresh,
-                                          BeamRows<T, HD> &w, uint32_t stage, uint32_t rows, float *buf, float2 *bml) {
+                                          BeamRows<T, HD> &w, uint32_t stage, uint64_t *full, uint64_t *empty,
+                                          uint32_t phase, bool &ok, uint32_t rows, float *buf, float2 *bml) {
     using Tl = BeamTile<T, HD>;
     constexpr int KW = Tl::kKeys / (4 / RW);
     const uint32_t warp = threadIdx.x >> 5, rg = warp % RW, kg = warp / RW;
@@ -621,8 +693,13 @@ __device__ __forceinline__ void beam_step(const BeamAttnArgs &a, const BeamAttnP
     if (fresh) beam_rows_init<T, HD>(a, c, c.tile * RW * 16 + rg * 16, qs, w);
     const bool first = c.pos == 0;
     const uint32_t n = beam_take<T, HD>(c);
-    if (kg * KW < n && __any_sync(0xffffffffu, w.lim[0] >= 0 || w.lim[1] >= 0))
+    // (after a wait that ran out: the same steps and barriers without the work)
+    ok = mbar_wait(full, phase, &g_beam_err, ERR_WAIT_FULL) && ok;
+    __syncwarp();
+    if (ok && kg * KW < n && __any_sync(0xffffffffu, w.lim[0] >= 0 || w.lim[1] >= 0))
         beam_tile<T, HD, KW>(w, qs, stage, stage + Tl::kBytes, kg * KW, c.pos, c.pos + n, a.scale * 1.4426950408889634f);
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(empty);
     beam_advance(c, n);
     fresh = c.pos >= c.len || c.left == 0;
     if (fresh) beam_flush<T, HD, RW>(a, p, c, w, buf, bml);
@@ -638,47 +715,68 @@ __device__ __forceinline__ void beam_step(const BeamAttnArgs &a, const BeamAttnP
 
 // RWP, RWS: row groups of 16 of a prefix / suffix tile.
 template <typename T, int HD, int RWP, int RWS>
-__global__ void __launch_bounds__(kBaThreads, sizeof(T) == 4 && RWP == 1 ? 3 : 2)
-    beam_attn_kernel(BeamAttnArgs a, BeamAttnPlan p) {
+__global__ void __launch_bounds__(kBaThreads + kBaLoader, sizeof(T) == 4 && RWP == 1 ? 3 : 2)
+    beam_attn_kernel(const BeamAttnArgs a, const BeamAttnPlan p, const __grid_constant__ BeamMaps maps) {
     using Tl = BeamTile<T, HD>;
     constexpr int S = kBaStages<T>;
-    extern __shared__ __align__(128) uint8_t beam_smem[];
-    __shared__ float2 bml[2 * 16];
+    // (the 128-byte swizzle counts rows from 1024-byte boundaries; nothing
+    // static stands before this)
+    extern __shared__ __align__(1024) uint8_t beam_smem[];
+    uint64_t *full = reinterpret_cast<uint64_t *>(beam_smem + beam_attn_smem<T, HD, RWP, RWS>() - kBaTail);
+    uint64_t *empty = full + S;
+    float2 *bml = reinterpret_cast<float2 *>(empty + S);
     const uint32_t smem = smem_u32(beam_smem), rows = smem + 2 * Tl::kBytes * S;
     float *buf = reinterpret_cast<float *>(beam_smem + 2 * Tl::kBytes * S);
     pdl_launch();
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            mbar_init(&full[i], 32);
+            mbar_init(&empty[i], kBaThreads / 32);
+        }
+        fence_mbar_init();
+    }
     BeamCursor c;
-    if (!beam_first(a, p, c)) return;
-    if (a.hd < HD) {  // the padding of the heads
-        for (uint32_t i = threadIdx.x; i < 2 * Tl::kBytes * S / 16; i += kBaThreads)
-            reinterpret_cast<uint4 *>(beam_smem)[i] = make_uint4(0, 0, 0, 0);
-        __syncthreads();
+    const bool any = beam_first(a, p, c);
+    __syncthreads();
+    if (!any) return;
+    uint32_t s = 0, phase = 0;
+    if (threadIdx.x >= kBaThreads) {
+        uint32_t issued = 0;
+        bool ok = true;
+        while (c.left) {
+            if (issued >= S && !(ok = mbar_wait(&empty[s], phase ^ 1, &g_beam_err, ERR_WAIT_EMPTY))) break;
+            const uint32_t n = beam_take<T, HD>(c);
+            beam_load<T, HD>(a, p, maps, c, n, smem + s * 2 * Tl::kBytes, &full[s]);
+            ++issued;
+            beam_advance(c, n);
+            if (c.left && c.pos >= c.len) beam_next_item(a, p, c);
+            if (++s == S) {
+                s = 0;
+                phase ^= 1;
+            }
+        }
+        // no copy is in flight when this CTA's shared memory is given back
+        for (uint32_t i = 0; i < min(issued, (uint32_t)S); ++i) {
+            const uint32_t t = issued - 1 - i;
+            mbar_wait(&full[t % S], t / S & 1, &g_beam_err, ERR_WAIT_DRAIN);
+        }
+        return;
     }
-    BeamCursor ahead = c;  // of the loads
     BeamRows<T, HD> w;
-    bool fresh = true;
-    uint32_t to = 0, from = 0;  // stages
+    bool fresh = true, ok = true;
 #pragma unroll 1
-    for (int i = 0; c.left; ++i) {
-        if (i >= S - 1) {
-            cp_async_wait<S - 2>();
-            __syncthreads();  // the tile is there for all, and the stage that is filled next is free
+    while (c.left) {
+        const uint32_t stage = smem + s * 2 * Tl::kBytes;
+        if (RWP == RWS || c.part < a.n_group)
+            beam_step<T, HD, RWP>(a, p, c, fresh, w, stage, &full[s], &empty[s], phase, ok, rows, buf, bml);
+        else
+            beam_step<T, HD, RWS>(a, p, c, fresh, w, stage, &full[s], &empty[s], phase, ok, rows, buf, bml);
+        if (++s == S) {
+            s = 0;
+            phase ^= 1;
         }
-        if (ahead.left) {
-            const uint32_t n = beam_take<T, HD>(ahead);
-            beam_load<T, HD>(a, ahead, n, smem + to * 2 * Tl::kBytes);
-            beam_advance(ahead, n);
-            if (ahead.left && ahead.pos >= ahead.len) beam_next_item(a, p, ahead);
-            to = to + 1 == S ? 0 : to + 1;
-        }
-        cp_async_commit();
-        if (i < S - 1) continue;
-        const uint32_t stage = smem + from * 2 * Tl::kBytes;
-        from = from + 1 == S ? 0 : from + 1;
-        if (RWP == RWS || c.part < a.n_group) beam_step<T, HD, RWP>(a, p, c, fresh, w, stage, rows, buf, bml);
-        else beam_step<T, HD, RWS>(a, p, c, fresh, w, stage, rows, buf, bml);
     }
-    cp_async_wait<0>();
 }
 
 // Joins a row's partial results: block (row, head), the warps take the
@@ -700,6 +798,9 @@ __global__ void __launch_bounds__(kBaThreads) beam_attn_join_kernel(BeamAttnArgs
     uint2 pc = make_uint2(1, 0), sc = make_uint2(1, 0);
     if (some_p) pc = p.pcta[pi];
     if (some_s) sc = p.scta[si];
+    // (after a wait that ran out these may be anything)
+    if (pc.y >= p.ctas || pc.x > pc.y + 1) pc = make_uint2(1, 0);
+    if (sc.y >= p.ctas || sc.x > sc.y + 1) sc = make_uint2(1, 0);
     const uint32_t np = pc.y + 1 - pc.x, n = np + (sc.y + 1 - sc.x);
     // the rows' first slots: of a prefix segment j, and of a suffix segment
     const size_t prow = (size_t)(pi + pc.x) * p.prow + (pr - ptile * p.prow);
