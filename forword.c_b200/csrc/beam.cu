@@ -4,9 +4,11 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdio>
+#include <cstdlib>
 
 #include "../../include/forword_b200.h"
 #include "beam_attn.cuh"
+#include "beam_attn_tc.cuh"
 #include "beam_reorder.cuh"
 #include "beam_select.cuh"
 #include "status.h"
@@ -121,9 +123,10 @@ uint32_t device_sms() {
     return (uint32_t)n[dev];
 }
 
-// Row tiles and the workspace's layout; returns its bytes.
+// Row tiles and the workspace's layout.
 struct AttnLayout {
-    uint32_t prg, srg;  // row groups of 16 of a prefix / suffix tile: 1, 2 or 4
+    bool tc;            // on the 5th-generation tensor cores (beam_attn_tc.cuh)
+    uint32_t prow, srow;  // rows of a prefix / suffix tile
     uint32_t ptiles, stiles, ctas;
     size_t pitems, sitems, bytes;
     size_t po, so, pml, sml, pcta, scta;
@@ -132,24 +135,28 @@ struct AttnLayout {
 bool attn_layout(const fwb_prefix_attn_t *a, AttnLayout &L) {
     const uint64_t gq = a->n_head / a->n_head_kv, srows = gq * a->n_query, prows = srows * a->n_beam;
     const uint32_t hd = a->head_dim <= 64 ? 64 : 128;
-    auto groups = [](uint64_t rows) { return rows <= 16 ? 1u : rows <= 32 ? 2u : 4u; };
-    L.prg = groups(prows);
-    L.srg = srows <= 16 ? 1u : L.prg;
-    L.ptiles = (uint32_t)((prows + L.prg * 16 - 1) / (L.prg * 16));
-    L.stiles = (uint32_t)((srows + L.srg * 16 - 1) / (L.srg * 16));
+    static const int force = getenv("BTC") ? atoi(getenv("BTC")) : -1;
+    L.tc = a->type != 0 && (force < 0 || force != 0);
+    auto tile = [&](uint64_t rows) {
+        return rows <= 16 ? 16u : rows <= 32 ? 32u : rows <= 64 || !L.tc ? 64u : 128u;
+    };
+    L.prow = tile(prows);
+    L.srow = srows <= 16 ? 16u : L.prow;
+    L.ptiles = (uint32_t)((prows + L.prow - 1) / L.prow);
+    L.stiles = (uint32_t)((srows + L.srow - 1) / L.srow);
     L.pitems = a->prefix_cap ? (size_t)a->n_group * a->n_head_kv * L.ptiles : 0;
     L.sitems = a->suffix_cap ? (size_t)a->n_group * a->n_beam * a->n_head_kv * L.stiles : 0;
     const uint64_t units = L.pitems * ((a->prefix_cap + 15) / 16) + L.sitems * ((a->suffix_cap + 15) / 16);
     if (L.pitems + L.sitems > 0x3fffffffu || units > 0x7fffffffu)
         return fail("fwb_prefix_attention: too many rows times positions");
-    L.ctas = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(2 * device_sms(), units));
+    L.ctas = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((L.tc ? 1 : 2) * device_sms(), units));
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t here = at;
         at += (n + 255) & ~(size_t)255;
         return here;
     };
-    const size_t pslots = (L.pitems + L.ctas) * L.prg * 16, sslots = (L.sitems + L.ctas) * L.srg * 16;
+    const size_t pslots = (L.pitems + L.ctas) * L.prow, sslots = (L.sitems + L.ctas) * L.srow;
     L.po = take(pslots * hd * 4);
     L.so = take(sslots * hd * 4);
     L.pml = take(pslots * 8);
@@ -190,27 +197,52 @@ bool cache_map(const void *base, size_t e, uint64_t hd, uint64_t cap, uint64_t n
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int HD, int RWP, int RWS>
-bool launch_attn(const BeamAttnArgs &k, const BeamAttnPlan &p, const BeamMaps &maps, cudaStream_t st) {
-    static bool ready[64] = {};
-    constexpr uint32_t smem = beam_attn_smem<T, HD, RWP, RWS>();
-    if (!opt_in(beam_attn_kernel<T, HD, RWP, RWS>, smem, ready, "fwb_prefix_attention")) return false;
-    beam_attn_kernel<T, HD, RWP, RWS><<<p.ctas, kBaThreads + kBaLoader, smem, st>>>(k, p, maps);
+template <typename T, int HD>
+bool launch_join(const BeamAttnArgs &k, const BeamAttnPlan &p, cudaStream_t st) {
     if (!launched(cudaGetLastError(), "fwb_prefix_attention launch")) return false;
     return launched(launch_after(beam_attn_join_kernel<T, HD>, dim3(k.n_group * k.n_beam * k.n_query, k.n_head),
                                  kBaThreads, 1, st, k, p),
                     "fwb_prefix_attention launch");
 }
 
+// PR, SR: rows of a prefix / suffix tile.
+template <typename T, int HD, int PR, int SR>
+bool launch_attn(const BeamAttnArgs &k, const BeamAttnPlan &p, const BeamMaps &maps, cudaStream_t st) {
+    static bool ready[64] = {};
+    constexpr uint32_t smem = beam_attn_smem<T, HD, PR / 16, SR / 16>();
+    if (!opt_in(beam_attn_kernel<T, HD, PR / 16, SR / 16>, smem, ready, "fwb_prefix_attention")) return false;
+    beam_attn_kernel<T, HD, PR / 16, SR / 16><<<p.ctas, kBaThreads + kBaLoader, smem, st>>>(k, p, maps);
+    return launch_join<T, HD>(k, p, st);
+}
+
+template <typename T, int HD, int PR, int SR>
+bool launch_attn_tc(const BeamAttnArgs &k, const BeamAttnPlan &p, const BeamMaps &maps, cudaStream_t st) {
+    static bool ready[64] = {};
+    constexpr uint32_t smem = beam_tc_smem<HD, PR>();
+    static_assert(smem <= 227 * 1024, "shared memory");
+    if (!opt_in(beam_attn_tc_kernel<T, HD, PR, SR>, smem, ready, "fwb_prefix_attention")) return false;
+    beam_attn_tc_kernel<T, HD, PR, SR><<<p.ctas, kBtThreads, smem, st>>>(k, p, maps);
+    return launch_join<T, HD>(k, p, st);
+}
+
 template <typename T, int HD>
-bool pick_attn(const BeamAttnArgs &k, const BeamAttnPlan &p, const BeamMaps &maps, uint32_t prg, uint32_t srg,
-               cudaStream_t st) {
-    switch (prg * 8 + srg) {
-    case 1 * 8 + 1: return launch_attn<T, HD, 1, 1>(k, p, maps, st);
-    case 2 * 8 + 1: return launch_attn<T, HD, 2, 1>(k, p, maps, st);
-    case 2 * 8 + 2: return launch_attn<T, HD, 2, 2>(k, p, maps, st);
-    case 4 * 8 + 1: return launch_attn<T, HD, 4, 1>(k, p, maps, st);
-    default: return launch_attn<T, HD, 4, 4>(k, p, maps, st);
+bool pick_attn(const BeamAttnArgs &k, const BeamAttnPlan &p, const BeamMaps &maps, bool tc, cudaStream_t st) {
+    if constexpr (sizeof(T) == 2)
+        if (tc) switch (p.prow + p.srow) {
+            case 16 + 16: return launch_attn_tc<T, HD, 16, 16>(k, p, maps, st);
+            case 32 + 16: return launch_attn_tc<T, HD, 32, 16>(k, p, maps, st);
+            case 32 + 32: return launch_attn_tc<T, HD, 32, 32>(k, p, maps, st);
+            case 64 + 16: return launch_attn_tc<T, HD, 64, 16>(k, p, maps, st);
+            case 64 + 64: return launch_attn_tc<T, HD, 64, 64>(k, p, maps, st);
+            case 128 + 16: return launch_attn_tc<T, HD, 128, 16>(k, p, maps, st);
+            default: return launch_attn_tc<T, HD, 128, 128>(k, p, maps, st);
+            }
+    switch (p.prow + p.srow) {
+    case 16 + 16: return launch_attn<T, HD, 16, 16>(k, p, maps, st);
+    case 32 + 16: return launch_attn<T, HD, 32, 16>(k, p, maps, st);
+    case 32 + 32: return launch_attn<T, HD, 32, 32>(k, p, maps, st);
+    case 64 + 16: return launch_attn<T, HD, 64, 16>(k, p, maps, st);
+    default: return launch_attn<T, HD, 64, 64>(k, p, maps, st);
     }
 }
 
@@ -223,8 +255,8 @@ bool run_attn(const BeamAttnArgs &k, const AttnLayout &L, uint8_t *ws, cudaStrea
     p.sml = reinterpret_cast<float2 *>(ws + L.sml);
     p.pcta = reinterpret_cast<uint2 *>(ws + L.pcta);
     p.scta = reinterpret_cast<uint2 *>(ws + L.scta);
-    p.prow = L.prg * 16;
-    p.srow = L.srg * 16;
+    p.prow = L.prow;
+    p.srow = L.srow;
     p.ptiles = L.ptiles;
     p.stiles = L.stiles;
     p.ctas = L.ctas;
@@ -234,8 +266,7 @@ bool run_attn(const BeamAttnArgs &k, const AttnLayout &L, uint8_t *ws, cudaStrea
             (cache_map(k.sk, sizeof(T), k.hd, k.scap, k.n_kv, k.n_group * k.n_beam, k.s_pos, k.s_head, k.s_seq, maps.sk) &&
              cache_map(k.sv, sizeof(T), k.hd, k.scap, k.n_kv, k.n_group * k.n_beam, k.s_pos, k.s_head, k.s_seq, maps.sv))
                 << 1;
-    return k.hd <= 64 ? pick_attn<T, 64>(k, p, maps, L.prg, L.srg, st)
-                      : pick_attn<T, 128>(k, p, maps, L.prg, L.srg, st);
+    return k.hd <= 64 ? pick_attn<T, 64>(k, p, maps, L.tc, st) : pick_attn<T, 128>(k, p, maps, L.tc, st);
 }
 
 // --- selection ------------------------------------------------------------------

@@ -45,6 +45,9 @@ template <> __device__ __forceinline__ __nv_bfloat16 beam_from_f32<__nv_bfloat16
     return __float2bfloat16_rn(v);
 }
 
+__device__ __forceinline__ constexpr bool beam_is_bf16(__half) { return false; }
+__device__ __forceinline__ constexpr bool beam_is_bf16(__nv_bfloat16) { return true; }
+
 // A length read from the device, held to the positions that the cache has.
 __device__ __forceinline__ uint32_t beam_len(const int32_t *len, uint32_t i, uint32_t cap) {
     if (!len) return cap;

@@ -1,0 +1,513 @@
+// beam_attn_tc.cuh — the shared-prefix attention of beam_attn.cuh on the
+// 5th-generation tensor cores, for fp16 and bf16.
+//
+// The products are transposed so that few query rows still fill the machine:
+// a tile's 128 positions are the M dimension of S^T = K Q^T (N: the query
+// rows, 16 to 128), and the head's dimensions that of O^T += V^T P.  A thread
+// of the softmax owns one position and half of the rows, so every thread has
+// the same work whatever the number of rows is, and the sums over positions
+// are kept per thread and joined once per item.
+//
+// The running maximum of a row is a reference that need not be exact: it is
+// raised, and O^T rescaled in tensor memory, only when a score exceeds it by
+// more than 8 in units of log2; probabilities then stay below 2^8.  So a tile
+// costs no reduction over positions, only one vote of the threads that share
+// the rows.
+//
+// One CTA per SM: a warp that loads (copy engine), one thread that issues the
+// products, and two groups of four warps for the softmax, each with half of
+// the rows.  The products of tile i + 1 run while tile i's softmax does.
+#pragma once
+#include "beam_attn.cuh"
+
+namespace fwb {
+
+constexpr int kBtKeys = 128;
+constexpr int kBtSoft = 256;                 // threads of the softmax
+constexpr int kBtThreads = 64 + kBtSoft;
+constexpr float kBtRaise = 8.f;              // log2
+
+// Shared memory: stages of K and V tiles, query rows, probabilities, then the
+// small things.
+template <int HD, int RT>
+struct BeamTc {
+    static constexpr int kSub = HD / 64;                           // sub-tiles of 128 bytes
+    static constexpr uint32_t kSubBytes = kBtKeys * 128;           // of K, V
+    static constexpr uint32_t kTile = kSub * kSubBytes;
+    static constexpr int kStages = RT == 128 ? 2 : 3;
+    static constexpr int kPBufs = RT == 128 ? 2 : 1;
+    static constexpr uint32_t kQ = RT * HD * 2, kP = (RT > 64 ? 2 : 1) * kSubBytes;
+    static constexpr uint32_t kOffQ = 2 * kTile * kStages, kOffP = kOffQ + kQ, kOffTail = kOffP + kPBufs * kP;
+    static constexpr uint32_t kTmem = RT == 128 ? 512 : RT == 64 ? 256 : RT == 32 ? 128 : 64;  // >= 3 RT columns
+};
+struct BeamTcTail {
+    uint64_t kfull[3], vfull[3], empty[3], sfull[2], sfree[2], pfull[2], odone[2], ofree, qfull;
+    uint32_t tmem;
+    alignas(16) float nm[128];  // minus the rows' references; +inf: none yet
+    float alpha[128];
+    uint32_t lim[128];          // positions that a row sees
+    uint32_t top[128];          // the tile's maxima, as ordered integers; 0 between uses
+};
+template <int HD, int RT>
+constexpr uint32_t beam_tc_smem() { return BeamTc<HD, RT>::kOffTail + sizeof(BeamTcTail); }
+
+__device__ __forceinline__ void bt_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void bt_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void bt_fence_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void bt_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// Shared-memory matrix descriptor, 128-byte swizzle: rows of 128 bytes, eight
+// of them (1024 bytes) an atom.  K-major operands: the next 8 rows 1024 bytes
+// on; MN-major ones: the next 8 k 1024 bytes on, the next 64 of M or N `lead`.
+__device__ __forceinline__ uint64_t bt_desc(uint32_t addr, uint32_t lead) {
+    return (uint64_t)((addr & 0x3ffffu) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024u >> 4) << 32 |
+           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// fp32 accumulator, A and B of type T (M 128, N n), both K-major or both MN-major.
+template <typename T>
+__device__ __forceinline__ uint32_t bt_idesc(uint32_t n, bool mn_major) {
+    const uint32_t t = beam_is_bf16(T{}) ? 1u : 0u;
+    return 1u << 4 | t << 7 | t << 10 | (mn_major ? 3u << 15 : 0u) | (n >> 3) << 17 | (128u >> 4) << 24;
+}
+__device__ __forceinline__ void bt_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+
+// 8 accumulator columns of this thread's lane (not waited for) / back.
+__device__ __forceinline__ void bt_ld8(uint32_t addr, float *v) {
+    uint32_t r[8];
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void bt_ld32(uint32_t addr, float *v) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void bt_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Keeps uses of loaded values behind the wait before it.
+template <int N>
+__device__ __forceinline__ void bt_here(float *v) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+f"(v[i]));
+}
+__device__ __forceinline__ void bt_st8(uint32_t addr, const float *v) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr),
+                 "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])),
+                 "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])),
+                 "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7])) : "memory");
+}
+__device__ __forceinline__ bool bt_any(uint32_t barrier, bool v) {  // of the 128 threads of a group
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+                 "barrier.cta.red.or.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"((uint32_t)v), "r"(barrier) : "memory");
+    return r != 0;
+}
+
+// A tile's K or V: n positions of a part, as beam_load does.
+template <typename T, int HD>
+__device__ __forceinline__ void bt_copy(const BeamAttnArgs &a, const BeamCursor &c, uint32_t n, bool pre,
+                                        const uint32_t *seq, uint32_t single, uint32_t dst, const void *base,
+                                        const CUtensorMap *map, uint64_t *bar) {
+    constexpr int kSub = HD / 64, CH = HD / 8, RP = 32 / CH;
+    const uint32_t lane = threadIdx.x & 31, units = (n + kBaUnit - 1) / kBaUnit;
+    single &= (1u << units) - 1;
+    if (lane == 0 && single)
+        asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                     "r"(__popc(single) * kSub * kBaUnit * 128) : "memory");
+    const uint32_t u = lane / kSub, h = lane % kSub;  // one box per lane
+    uint32_t from = 0;
+#pragma unroll
+    for (int i = 0; i < kBtKeys / 32; ++i) {
+        const uint32_t v = __shfl_sync(0xffffffffu, seq[i], (u & 1) * kBaUnit);
+        if ((u >> 1) == i) from = v;
+    }
+    __syncwarp();
+    if (u < units && single >> u & 1)
+        tma_load_4d(dst + h * (kBtKeys * 128) + u * kBaUnit * 128, map, (int32_t)(h * 64), (int32_t)(c.pos + u * kBaUnit),
+                    (int32_t)c.kvh, (int32_t)from, bar);
+    if (single != (1u << units) - 1) {
+        const uint32_t ch = lane % CH;
+        const bool held = ch * 8 < a.hd;
+        const size_t outer = pre ? a.p_group : a.s_seq, step = pre ? a.p_pos : a.s_pos;
+        const T *b = static_cast<const T *>(base) + (pre ? c.kvh * a.p_head : c.kvh * a.s_head) + (held ? ch * 8 : 0);
+#pragma unroll
+        for (int i = 0; i < kBtKeys / 32; ++i)
+            for (uint32_t r = 0; r < 32; r += RP) {
+                const uint32_t row = 32 * i + r + lane / CH;
+                const uint32_t s = __shfl_sync(0xffffffffu, seq[i], row & 31);
+                if (row < n && !(single >> (row / kBaUnit) & 1))
+                    cp_async16_or_zero(dst + (ch >> 3) * (kBtKeys * 128) + row * 128 + (((ch ^ row) & 7) << 4),
+                                       b + s * outer + (size_t)(c.pos + row) * step, held);
+            }
+    }
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ uint32_t bt_take(const BeamCursor &c) {
+    return min(min((uint32_t)kBtKeys, c.len - c.pos), min(c.left, kBtKeys / kBaUnit) * kBaUnit);
+}
+
+// The CTA's tile i by the softmax threads.  RT: rows of the item's tiles.
+template <typename T, int HD, int RTP, int RT>
+__device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPlan &p, BeamCursor &c, bool &fresh,
+                                        float *l, uint32_t i, uint8_t *sm, BeamTcTail &t, uint32_t tmem,
+                                        bool &ok) {
+    using Sm = BeamTc<HD, RTP>;
+    constexpr int NC = RT / 2, S = Sm::kStages, PB = Sm::kPBufs;
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = warp & 3, wg = (warp - 2) >> 2;
+    const uint32_t tid = threadIdx.x - 64, wt = tid & 127, col0 = wg * NC, bar = 2 + wg;
+    const uint32_t key = quad * 32 + lane, lanes = (quad * 32) << 16;
+    const bool pre = c.part < a.n_group;
+    const uint32_t rows = (pre ? a.n_beam : 1) * a.n_query * a.gq;
+    const float sl2 = a.scale * 1.4426950408889634f;
+    const bool limits = !pre && a.n_query > 1;
+    if (fresh) {
+        // query rows, K-major with the 128-byte swizzle; rows past the item's are zeros
+        constexpr int CH = HD / 8;
+        const uint32_t qs = smem_u32(sm + Sm::kOffQ);
+        for (uint32_t j = tid; j < RT * CH; j += kBtSoft) {
+            const uint32_t r = j / CH, ch = j % CH;
+            int32_t lim;
+            const T *q = beam_q_row<T, HD>(a, c, c.tile * RT + r, lim);
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (q && ch * 8 < a.hd) v = *reinterpret_cast<const uint4 *>(q + ch * 8);
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(qs + (ch >> 3) * (RT * 128) + r * 128 + (((ch ^ r) & 7) << 4)),
+                         "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+            if (ch == 0) t.lim[r] = (uint32_t)lim;  // (-1: no such row, sees all and is not written)
+        }
+        if (wt < NC) t.nm[col0 + wt] = INFINITY;
+#pragma unroll
+        for (int j = 0; j < NC; ++j) l[j] = 0.f;
+        bt_fence_proxy();
+        bar_sync(1, kBtSoft);
+        if (tid == 0) mbar_arrive(&t.qfull);
+    }
+    const bool first = fresh, start = c.pos == 0;
+    const uint32_t n = bt_take(c), sb = i & 1, pb = i % PB, st = i % S;
+    ok = mbar_wait(&t.sfull[sb], i >> 1 & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
+    __syncwarp();
+    bt_fence_after();
+    float s[NC];
+    const uint32_t ts = tmem + sb * RTP + lanes + col0;
+    if constexpr (NC >= 32) {
+#pragma unroll
+        for (int j = 0; j < NC; j += 32) bt_ld32(ts + j, s + j);
+    } else {
+#pragma unroll
+        for (int j = 0; j < NC; j += 8) bt_ld8(ts + j, s + j);
+    }
+    bt_ld_wait();
+    bt_here<NC>(s);
+    bt_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&t.sfree[sb]);
+    const bool live = key < n;
+    if (limits)
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+            if (c.pos + key >= t.lim[col0 + j]) s[j] = -INFINITY;
+    // against the rows' references
+    float over = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < NC; j += 4) {
+        const float4 nm = *reinterpret_cast<const float4 *>(&t.nm[col0 + j]);
+        over = fmaxf(over, fmaxf(fmaxf(fmaf(s[j], sl2, nm.x), fmaf(s[j + 1], sl2, nm.y)),
+                                 fmaxf(fmaf(s[j + 2], sl2, nm.z), fmaf(s[j + 3], sl2, nm.w))));
+    }
+    if (bt_any(bar, live && over > kBtRaise)) {
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+            const float x = live ? s[j] * sl2 : -INFINITY;
+            const uint32_t o = __float_as_uint(x) & 0x80000000u ? ~__float_as_uint(x) : __float_as_uint(x) | 0x80000000u;
+            const uint32_t m = __reduce_max_sync(0xffffffffu, o);
+            if (lane == 0) atomicMax(&t.top[col0 + j], m);
+        }
+        bar_sync(bar, 128);
+        if (wt < NC) {
+            const uint32_t r = col0 + wt;
+            const uint32_t m = t.top[r];
+            t.top[r] = 0;
+            const float x = __uint_as_float(m & 0x80000000u ? m & 0x7fffffffu : ~m), old = -t.nm[r];
+            const float now = fmaxf(old, x);
+            t.alpha[r] = old == -INFINITY ? 0.f : exp2_fast(old - now);
+            t.nm[r] = -now;  // (+inf while the row has seen nothing)
+        }
+        bar_sync(bar, 128);
+#pragma unroll
+        for (int j = 0; j < NC; ++j) l[j] *= t.alpha[col0 + j];
+        if (!first) {  // the output so far
+            ok = mbar_wait(&t.odone[(i - 1) & 1], (i - 1) >> 1 & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
+            __syncwarp();
+            bt_fence_after();
+            const uint32_t to = tmem + 2 * RTP + lanes + col0;
+#pragma unroll 1
+            for (uint32_t j = 0; j < NC; j += 8) {
+                float o[8];
+                bt_ld8(to + j, o);
+                bt_ld_wait();
+                bt_here<8>(o);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] *= t.alpha[col0 + j + e];
+                bt_st8(to + j, o);
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        }
+    }
+    // the buffer's last reader; in order for every tile, so that the phases of
+    // these barriers are never two ahead of what was seen
+    if (i >= PB) ok = mbar_wait(&t.odone[(i - PB) & 1], (i - PB) >> 1 & 1, &g_beam_err, ERR_WAIT_EMPTY) && ok;
+    const uint32_t ps = smem_u32(sm + Sm::kOffP + pb * Sm::kP) + key * 128;
+#pragma unroll
+    for (int j = 0; j < NC; j += 8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+            const float4 nm = *reinterpret_cast<const float4 *>(&t.nm[col0 + j + e]);
+            float q[4] = {fmaf(s[j + e], sl2, nm.x), fmaf(s[j + e + 1], sl2, nm.y), fmaf(s[j + e + 2], sl2, nm.z),
+                          fmaf(s[j + e + 3], sl2, nm.w)};
+#pragma unroll
+            for (int f = 0; f < 4; ++f) {
+                const bool seen = live && (!limits || s[j + e + f] != -INFINITY);
+                q[f] = seen ? exp2_fast(q[f]) : 0.f;
+                l[j + e + f] += q[f];
+            }
+            w[e / 2] = pack2(q[0], q[1], T{});
+            w[e / 2 + 1] = pack2(q[2], q[3], T{});
+        }
+        const uint32_t col = col0 + j;
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(ps + (col >> 6) * Sm::kSubBytes + ((((col >> 3) ^ key) & 7) << 4)),
+                     "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+    }
+    if (n & (kBaUnit - 1)) {
+        // V rows of the last unit past the end: their probabilities are zero,
+        // and zero times whatever the memory holds must be zero
+        ok = mbar_wait(&t.vfull[st], i / S & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
+        const uint32_t vs = smem_u32(sm + (2 * st + 1) * Sm::kTile);
+        const uint32_t end = (n + kBaUnit - 1) / kBaUnit * kBaUnit;
+        for (uint32_t j = tid; j < (end - n) * (HD / 8); j += kBtSoft) {
+            const uint32_t row = n + j / (HD / 8), ch = j % (HD / 8);
+            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(vs + (ch >> 3) * Sm::kSubBytes + row * 128 + ((ch & 7) << 4)),
+                         "r"(0) : "memory");  // (whole rows: their swizzle does not matter)
+        }
+    }
+    bt_fence_proxy();
+    bt_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&t.pfull[pb]);
+    beam_advance(c, n);
+    fresh = c.pos >= c.len || c.left == 0;
+    const uint32_t item = ((pre ? c.part : c.part - a.n_group) * a.n_kv + c.kvh) * (pre ? p.ptiles : p.stiles) + c.tile;
+    if (fresh) {
+        ok = mbar_wait(&t.odone[i & 1], i >> 1 & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
+        __syncwarp();
+        bt_fence_after();
+        const size_t row0 = (size_t)(item + blockIdx.x) * RT;
+        float *o = (pre ? p.po : p.so) + row0 * HD + key;
+        const uint32_t to = tmem + 2 * RTP + lanes + col0, held = rows - min(rows, c.tile * RT);
+#pragma unroll 1
+        for (uint32_t j = 0; j < NC; j += 8) {
+            float v[8];
+            bt_ld8(to + j, v);
+            bt_ld_wait();
+            bt_here<8>(v);
+            if (key < HD)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (col0 + j + e < held) o[(size_t)(col0 + j + e) * HD] = v[e];
+        }
+        bt_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&t.ofree);
+        // the sums over the 128 positions, through the probabilities' place
+        float *sum = reinterpret_cast<float *>(sm + Sm::kOffP);
+#pragma unroll
+        for (int j = 0; j < NC; ++j) {
+#pragma unroll
+            for (int d = 16; d; d >>= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], d);
+            if (lane == 0) sum[quad * RT + col0 + j] = l[j];
+        }
+        bar_sync(bar, 128);
+        if (wt < NC && col0 + wt < held) {
+            const uint32_t r = col0 + wt;
+            (pre ? p.pml : p.sml)[row0 + r] =
+                make_float2(-t.nm[r], (sum[r] + sum[RT + r]) + (sum[2 * RT + r] + sum[3 * RT + r]));
+        }
+        bar_sync(1, kBtSoft);  // before the next item's rows come into the same places
+    }
+    if (tid == 0 && (start || c.pos >= c.len)) {
+        uint2 *cta = (pre ? p.pcta : p.scta) + item;
+        if (start) cta->x = blockIdx.x;
+        if (c.pos >= c.len) cta->y = blockIdx.x;
+    }
+    if (fresh && c.left) beam_next_item(a, p, c);
+}
+
+// RTP, RTS: rows of a prefix / suffix tile.
+template <typename T, int HD, int RTP, int RTS>
+__global__ void __launch_bounds__(kBtThreads, 1)
+    beam_attn_tc_kernel(const BeamAttnArgs a, const BeamAttnPlan p, const __grid_constant__ BeamMaps maps) {
+    using Sm = BeamTc<HD, RTP>;
+    constexpr int S = Sm::kStages, PB = Sm::kPBufs;
+    extern __shared__ __align__(1024) uint8_t bt_sm[];
+    BeamTcTail &t = *reinterpret_cast<BeamTcTail *>(bt_sm + Sm::kOffTail);
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_launch();
+    BeamCursor c;
+    const bool any = beam_first(a, p, c);
+    if (!any) return;  // the same in every thread
+    if (threadIdx.x < 128) t.top[threadIdx.x] = 0;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S; ++i) {
+            mbar_init(&t.kfull[i], 32);
+            mbar_init(&t.vfull[i], 32);
+            mbar_init(&t.empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&t.sfull[i], 1);
+            mbar_init(&t.sfree[i], kBtSoft / 32);
+            mbar_init(&t.pfull[i], kBtSoft / 32);
+            mbar_init(&t.odone[i], 1);
+        }
+        mbar_init(&t.ofree, kBtSoft / 32);
+        mbar_init(&t.qfull, 1);
+        fence_mbar_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&t.tmem)), "r"(Sm::kTmem) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    bt_fence_before();
+    __syncthreads();
+    bt_fence_after();
+    const uint32_t tmem = t.tmem;
+    if (warp == 0) {
+        uint32_t i = 0;
+        for (; c.left; ++i) {
+            const uint32_t s = i % S;
+            if (i >= S && !mbar_wait(&t.empty[s], (i / S - 1) & 1, &g_beam_err, ERR_WAIT_EMPTY)) break;
+            __syncwarp();
+            const uint32_t n = bt_take(c);
+            const bool pre = c.part < a.n_group;
+            const uint32_t sq = c.part - a.n_group;
+            // the cache row's sequence, or group, of rows lane, lane + 32, ...
+            uint32_t seq[kBtKeys / 32], single = p.tma >> (pre ? 0 : 1) & 1 ? 0xffu : 0u;
+#pragma unroll
+            for (int j = 0; j < kBtKeys / 32; ++j) seq[j] = pre ? c.part : sq;
+            if (!pre && a.slots) {
+                const uint32_t b0 = sq / a.n_beam * a.n_beam;
+                const int32_t *slots = a.slots + sq * a.slot_seq + c.pos;
+#pragma unroll
+                for (int j = 0; j < kBtKeys / 32; ++j)
+                    if (lane + 32 * j < n) {
+                        const uint32_t from = (uint32_t)slots[lane + 32 * j];
+                        if (from < a.n_beam) seq[j] = b0 + from;
+                    }
+#pragma unroll
+                for (int j = 0; j < kBtKeys / 32; ++j) {  // units whose rows differ
+                    const uint32_t lead = __shfl_sync(0xffffffffu, seq[j], lane & 16);
+                    const uint32_t off = __ballot_sync(0xffffffffu, seq[j] != lead && lane + 32 * j < n);
+                    if (off & 0xffffu) single &= ~(1u << 2 * j);
+                    if (off >> 16) single &= ~(2u << 2 * j);
+                }
+            }
+            const uint32_t ks = smem_u32(bt_sm + 2 * s * Sm::kTile);
+            bt_copy<T, HD>(a, c, n, pre, seq, single, ks, pre ? a.pk : a.sk, pre ? &maps.pk : &maps.sk, &t.kfull[s]);
+            bt_copy<T, HD>(a, c, n, pre, seq, single, ks + Sm::kTile, pre ? a.pv : a.sv, pre ? &maps.pv : &maps.sv, &t.vfull[s]);
+            beam_advance(c, n);
+            if (c.left && c.pos >= c.len) beam_next_item(a, p, c);
+        }
+        // no copy is in flight when this CTA's shared memory is given back
+        for (uint32_t j = 0; j < min(i, (uint32_t)S); ++j) {
+            const uint32_t w = i - 1 - j;
+            mbar_wait(&t.kfull[w % S], w / S & 1, &g_beam_err, ERR_WAIT_DRAIN);
+            mbar_wait(&t.vfull[w % S], w / S & 1, &g_beam_err, ERR_WAIT_DRAIN);
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            const uint32_t q = smem_u32(bt_sm + Sm::kOffQ);
+            uint32_t seg = 0;
+            bool ok = true;
+            // S^T = K Q^T of tile i, the first of an item or not
+            auto scores = [&](uint32_t i, bool first, uint32_t rt) {
+                const uint32_t s = i % S, b = i & 1;
+                if (first) ok = mbar_wait(&t.qfull, seg & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
+                ok = mbar_wait(&t.kfull[s], i / S & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
+                if (i >= 2) ok = mbar_wait(&t.sfree[b], (i / 2 - 1) & 1, &g_beam_err, ERR_WAIT_EMPTY) && ok;
+                bt_fence_after();
+                bt_fence_proxy();
+                const uint32_t k = smem_u32(bt_sm + 2 * s * Sm::kTile), id = bt_idesc<T>(rt, false);
+                if (ok)
+#pragma unroll
+                    for (int d = 0; d < HD / 16; ++d)
+                        bt_mma(tmem + b * RTP, bt_desc(k + (d / 4) * Sm::kSubBytes + (d % 4) * 32, 16),
+                               bt_desc(q + (d / 4) * (rt * 128) + (d % 4) * 32, 16), id, d != 0);
+                bt_commit(&t.sfull[b]);
+            };
+            bool first = true;
+            scores(0, true, c.part < a.n_group ? RTP : RTS);
+            for (uint32_t i = 0; c.left; ++i) {
+                const uint32_t n = bt_take(c), rt = c.part < a.n_group ? RTP : RTS;
+                beam_advance(c, n);
+                const bool last = c.left == 0, turn = !last && c.pos >= c.len;
+                if (!last && !turn) scores(i + 1, false, rt);
+                // O^T += V^T P
+                const uint32_t s = i % S, pb = i % PB;
+                ok = mbar_wait(&t.vfull[s], i / S & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
+                ok = mbar_wait(&t.pfull[pb], i / PB & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
+                if (first && seg) ok = mbar_wait(&t.ofree, (seg - 1) & 1, &g_beam_err, ERR_WAIT_EMPTY) && ok;
+                bt_fence_after();
+                bt_fence_proxy();
+                const uint32_t v = smem_u32(bt_sm + (2 * s + 1) * Sm::kTile), ps = smem_u32(bt_sm + Sm::kOffP + pb * Sm::kP);
+                const uint32_t id = bt_idesc<T>(rt, true), units = (n + kBaUnit - 1) / kBaUnit;
+                if (ok)
+                    for (uint32_t u = 0; u < units; ++u)  // (a 64-wide head: its dimensions twice)
+                        bt_mma(tmem + 2 * RTP, bt_desc(v + u * 2048, HD == 64 ? 0 : Sm::kSubBytes),
+                               bt_desc(ps + u * 2048, Sm::kSubBytes), id, !first || u);
+                bt_commit(&t.empty[s]);
+                bt_commit(&t.odone[i & 1]);
+                first = false;
+                if (turn) {
+                    beam_next_item(a, p, c);
+                    ++seg;
+                    first = true;
+                    if (c.left) scores(i + 1, true, c.part < a.n_group ? RTP : RTS);
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        float l[(RTP > RTS ? RTP : RTS) / 2];
+        bool fresh = true, ok = true;
+#pragma unroll 1
+        for (uint32_t i = 0; c.left; ++i) {
+            if (RTP == RTS || c.part < a.n_group) bt_step<T, HD, RTP, RTP>(a, p, c, fresh, l, i, bt_sm, t, tmem, ok);
+            else bt_step<T, HD, RTP, RTS>(a, p, c, fresh, l, i, bt_sm, t, tmem, ok);
+        }
+    }
+    // every product is complete: the softmax waited for the last one's commit
+    // (or the wait ran out after its bound)
+    bt_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        bt_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Sm::kTmem) : "memory");
+    }
+}
+
+}  // namespace fwb
