@@ -127,7 +127,7 @@ uint32_t device_sms() {
 struct AttnLayout {
     bool tc;            // on the 5th-generation tensor cores (beam_attn_tc.cuh)
     uint32_t prow, srow;  // rows of a prefix / suffix tile
-    uint32_t ptiles, stiles, ctas;
+    uint32_t ptiles, stiles, ctas, cost;
     size_t pitems, sitems, bytes;
     size_t po, so, pml, sml, pcta, scta;
 };
@@ -146,7 +146,8 @@ bool attn_layout(const fwb_prefix_attn_t *a, AttnLayout &L) {
     L.stiles = (uint32_t)((srows + L.srow - 1) / L.srow);
     L.pitems = a->prefix_cap ? (size_t)a->n_group * a->n_head_kv * L.ptiles : 0;
     L.sitems = a->suffix_cap ? (size_t)a->n_group * a->n_beam * a->n_head_kv * L.stiles : 0;
-    const uint64_t units = L.pitems * ((a->prefix_cap + 15) / 16) + L.sitems * ((a->suffix_cap + 15) / 16);
+    L.cost = L.tc ? getenv("BCOST") ? atoi(getenv("BCOST")) : 20 : 4;
+    const uint64_t units = L.pitems * ((a->prefix_cap + 15) / 16 + L.cost) + L.sitems * ((a->suffix_cap + 15) / 16 + L.cost);
     if (L.pitems + L.sitems > 0x3fffffffu || units > 0x7fffffffu)
         return fail("fwb_prefix_attention: too many rows times positions");
     L.ctas = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((L.tc ? 1 : 2) * device_sms(), units));
@@ -260,6 +261,7 @@ bool run_attn(const BeamAttnArgs &k, const AttnLayout &L, uint8_t *ws, cudaStrea
     p.ptiles = L.ptiles;
     p.stiles = L.stiles;
     p.ctas = L.ctas;
+    p.cost = L.cost;
     BeamMaps maps{};
     p.tma = (cache_map(k.pk, sizeof(T), k.hd, k.pcap, k.n_kv, k.n_group, k.p_pos, k.p_head, k.p_group, maps.pk) &&
              cache_map(k.pv, sizeof(T), k.hd, k.pcap, k.n_kv, k.n_group, k.p_pos, k.p_head, k.p_group, maps.pv)) |

@@ -63,7 +63,8 @@ __device__ __forceinline__ uint32_t beam_len(const int32_t *len, uint32_t i, uin
 // of C <= U takes units [c U / C, (c + 1) U / C).  So every CTA reads as many
 // positions as any other, whatever the lengths are, and an item that several
 // CTAs share leaves one partial result (sum, maximum, weighted values) per
-// CTA.  A second kernel joins a row's partial results of prefix and suffix.
+// CTA.  An item's beginning and end cost time of their own: it stands in the
+// line with `cost` units more in front, in which nothing is read.  A second kernel joins a row's partial results of prefix and suffix.
 // ---------------------------------------------------------------------------
 constexpr uint32_t kBaUnit = 16;      // positions
 constexpr int kBaThreads = 128;       // four warps that compute
@@ -77,6 +78,7 @@ struct BeamAttnPlan {
     uint32_t prow, srow;   // rows of a prefix / suffix tile
     uint32_t ptiles, stiles;  // row tiles of a group / of a sequence
     uint32_t ctas;
+    uint32_t cost;         // units that an item's own work is worth
     uint32_t tma;          // bit 0: tensor maps of the prefix, 1: of the suffix
 };
 
@@ -95,7 +97,8 @@ __device__ __forceinline__ uint32_t beam_units(uint32_t len) { return (len + kBa
 
 // Units of a part in the line.
 __device__ __forceinline__ uint32_t beam_part_units(const BeamAttnArgs &a, const BeamAttnPlan &p, uint32_t part) {
-    return beam_units(beam_part_len(a, part)) * a.n_kv * (part < a.n_group ? p.ptiles : p.stiles);
+    const uint32_t units = beam_units(beam_part_len(a, part));
+    return units ? (units + p.cost) * a.n_kv * (part < a.n_group ? p.ptiles : p.stiles) : 0;
 }
 
 // The cursor of this CTA's first unit; false when it has none.  Every warp
@@ -131,18 +134,21 @@ __device__ __forceinline__ bool beam_first(const BeamAttnArgs &a, const BeamAttn
         if (i0 + 32 >= parts) return false;  // lengths that changed under the call
     }
     c.len = beam_part_len(a, c.part);
-    const uint32_t units = beam_units(c.len), tiles = c.part < a.n_group ? p.ptiles : p.stiles;
-    if (units == 0) return false;            // likewise
+    const uint32_t units = beam_units(c.len) + p.cost, tiles = c.part < a.n_group ? p.ptiles : p.stiles;
+    if (c.len == 0) return false;            // likewise
     const uint32_t item = off / units;
+    off -= item * units;
     c.kvh = item / tiles;
     c.tile = item - c.kvh * tiles;
-    c.pos = (off - item * units) * kBaUnit;
-    return true;
+    c.pos = off > p.cost ? (off - p.cost) * kBaUnit : 0;
+    if (off < p.cost) c.left -= min(c.left, p.cost - off);
+    return c.left != 0;
 }
 
 // To the item after the cursor's (its positions are used up, units are left).
 __device__ __forceinline__ void beam_next_item(const BeamAttnArgs &a, const BeamAttnPlan &p, BeamCursor &c) {
     c.pos = 0;
+    c.left -= min(c.left, p.cost);
     if (++c.tile < (c.part < a.n_group ? p.ptiles : p.stiles)) return;
     c.tile = 0;
     if (++c.kvh < a.n_kv) return;

@@ -119,6 +119,42 @@ __device__ __forceinline__ bool bt_any(uint32_t barrier, bool v) {  // of the 12
     return r != 0;
 }
 
+// Two fp32 at once: a = a * s + b, and a += b.
+__device__ __forceinline__ void bt_fma2(float &a0, float &a1, float s, float b0, float b1) {
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\tmov.b64 z, {%3, %4};\n\t"
+        "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "+f"(a0), "+f"(a1) : "f"(s), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void bt_add2(float &a0, float &a1, float b0, float b1) {
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
+        "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "+f"(a0), "+f"(a1) : "f"(b0), "f"(b1));
+}
+
+// Joins N values of every lane over the warp: each step keeps half of the
+// values and hands the other half to the lane across.  Lane ends with values
+// first .. first + max(1, N / 32) - 1 (lanes may hold the same ones) in v.
+template <int N, int D = 16, typename Op>
+__device__ __forceinline__ uint32_t bt_join(float *v, Op op) {
+    uint32_t first = 0;
+    if constexpr (N > 1) {
+        constexpr int H = N / 2;
+        const bool up = threadIdx.x & D;
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+            const float a = v[j], b = v[j + H];
+            const float give = up ? a : b, keep = up ? b : a;
+            v[j] = op(keep, __shfl_xor_sync(0xffffffffu, give, D));
+        }
+        first = up ? H : 0;
+        if constexpr (D > 1) first += bt_join<H, D / 2>(v, op);
+    } else {
+        v[0] = op(v[0], __shfl_xor_sync(0xffffffffu, v[0], D));
+        if constexpr (D > 1) bt_join<1, D / 2>(v, op);
+    }
+    return first;
+}
+
 // A tile's K or V: n positions of a part, as beam_load does.
 template <typename T, int HD>
 __device__ __forceinline__ void bt_copy(const BeamAttnArgs &a, const BeamCursor &c, uint32_t n, bool pre,
@@ -179,17 +215,24 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
     const bool limits = !pre && a.n_query > 1;
     if (fresh) {
         // query rows, K-major with the 128-byte swizzle; rows past the item's are zeros
-        constexpr int CH = HD / 8;
-        const uint32_t qs = smem_u32(sm + Sm::kOffQ);
-        for (uint32_t j = tid; j < RT * CH; j += kBtSoft) {
-            const uint32_t r = j / CH, ch = j % CH;
-            int32_t lim;
-            const T *q = beam_q_row<T, HD>(a, c, c.tile * RT + r, lim);
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (q && ch * 8 < a.hd) v = *reinterpret_cast<const uint4 *>(q + ch * 8);
-            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(qs + (ch >> 3) * (RT * 128) + r * 128 + (((ch ^ r) & 7) << 4)),
-                         "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-            if (ch == 0) t.lim[r] = (uint32_t)lim;  // (-1: no such row, sees all and is not written)
+        constexpr int CH = HD / 8, RPP = kBtSoft / CH, NR = (RT + RPP - 1) / RPP;  // rows of a pass; passes
+        const uint32_t qs = smem_u32(sm + Sm::kOffQ), ch = tid % CH, r0 = tid / CH;
+        uint4 v[NR];
+#pragma unroll
+        for (int j = 0; j < NR; ++j) {
+            const uint32_t r = r0 + j * RPP;
+            int32_t lim = -1;
+            const T *q = r < RT ? beam_q_row<T, HD>(a, c, c.tile * RT + r, lim) : nullptr;
+            v[j] = make_uint4(0, 0, 0, 0);
+            if (q && ch * 8 < a.hd) v[j] = *reinterpret_cast<const uint4 *>(q + ch * 8);
+            if (ch == 0 && r < RT) t.lim[r] = (uint32_t)lim;  // (-1: no such row, sees all and is not written)
+        }
+#pragma unroll
+        for (int j = 0; j < NR; ++j) {
+            const uint32_t r = r0 + j * RPP;
+            if (r < RT)
+                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(qs + (ch >> 3) * (RT * 128) + r * 128 + (((ch ^ r) & 7) << 4)),
+                             "r"(v[j].x), "r"(v[j].y), "r"(v[j].z), "r"(v[j].w) : "memory");
         }
         if (wt < NC) t.nm[col0 + wt] = INFINITY;
 #pragma unroll
@@ -203,54 +246,65 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
     ok = mbar_wait(&t.sfull[sb], i >> 1 & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
     __syncwarp();
     bt_fence_after();
-    float s[NC];
+    float y[NC];
     const uint32_t ts = tmem + sb * RTP + lanes + col0;
-    if constexpr (NC >= 32) {
-#pragma unroll
-        for (int j = 0; j < NC; j += 32) bt_ld32(ts + j, s + j);
-    } else {
-#pragma unroll
-        for (int j = 0; j < NC; j += 8) bt_ld8(ts + j, s + j);
-    }
-    bt_ld_wait();
-    bt_here<NC>(s);
-    bt_fence_before();
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&t.sfree[sb]);
     const bool live = key < n;
-    if (limits)
+    auto load = [&] {  // the scores
+        if constexpr (NC >= 32) {
 #pragma unroll
-        for (int j = 0; j < NC; ++j)
-            if (c.pos + key >= t.lim[col0 + j]) s[j] = -INFINITY;
-    // against the rows' references
+            for (int j = 0; j < NC; j += 32) bt_ld32(ts + j, y + j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NC; j += 8) bt_ld8(ts + j, y + j);
+        }
+        bt_ld_wait();
+        bt_here<NC>(y);
+    };
+    auto hide = [&] {  // positions past the end, or that a row does not see
+        if (n < kBtKeys && !live)
+#pragma unroll
+            for (int j = 0; j < NC; ++j) y[j] = -INFINITY;
+        if (limits)
+#pragma unroll
+            for (int j = 0; j < NC; ++j)
+                if (c.pos + key >= t.lim[col0 + j]) y[j] = -INFINITY;
+    };
+    auto refer = [&] {  // against the rows' references
+#pragma unroll
+        for (int j = 0; j < NC; j += 4) {
+            const float4 nm = *reinterpret_cast<const float4 *>(&t.nm[col0 + j]);
+            bt_fma2(y[j], y[j + 1], sl2, nm.x, nm.y);
+            bt_fma2(y[j + 2], y[j + 3], sl2, nm.z, nm.w);
+        }
+        hide();
+    };
+    load();
+    refer();
     float over = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < NC; j += 4) {
-        const float4 nm = *reinterpret_cast<const float4 *>(&t.nm[col0 + j]);
-        over = fmaxf(over, fmaxf(fmaxf(fmaf(s[j], sl2, nm.x), fmaf(s[j + 1], sl2, nm.y)),
-                                 fmaxf(fmaf(s[j + 2], sl2, nm.z), fmaf(s[j + 3], sl2, nm.w))));
-    }
-    if (bt_any(bar, live && over > kBtRaise)) {
+    for (int j = 0; j < NC; ++j) over = fmaxf(over, y[j]);
+    if (bt_any(bar, over > kBtRaise)) {
+        load();
+        hide();
+        const uint32_t at = bt_join<NC>(y, [](float u, float v) { return fmaxf(u, v); });
 #pragma unroll
-        for (int j = 0; j < NC; ++j) {
-            const float x = live ? s[j] * sl2 : -INFINITY;
-            const uint32_t o = __float_as_uint(x) & 0x80000000u ? ~__float_as_uint(x) : __float_as_uint(x) | 0x80000000u;
-            const uint32_t m = __reduce_max_sync(0xffffffffu, o);
-            if (lane == 0) atomicMax(&t.top[col0 + j], m);
+        for (int j = 0; j < (NC > 32 ? NC / 32 : 1); ++j) {
+            const uint32_t u = __float_as_uint(y[j] * sl2);
+            atomicMax(&t.top[col0 + at + j], u & 0x80000000u ? ~u : u | 0x80000000u);
         }
         bar_sync(bar, 128);
         if (wt < NC) {
-            const uint32_t r = col0 + wt;
-            const uint32_t m = t.top[r];
+            const uint32_t r = col0 + wt, m = t.top[r];
             t.top[r] = 0;
-            const float x = __uint_as_float(m & 0x80000000u ? m & 0x7fffffffu : ~m), old = -t.nm[r];
-            const float now = fmaxf(old, x);
-            t.alpha[r] = old == -INFINITY ? 0.f : exp2_fast(old - now);
+            const float now = fmaxf(-t.nm[r], __uint_as_float(m & 0x80000000u ? m & 0x7fffffffu : ~m));
+            t.alpha[r] = t.nm[r] == INFINITY ? 0.f : exp2_fast(-t.nm[r] - now);
             t.nm[r] = -now;  // (+inf while the row has seen nothing)
         }
         bar_sync(bar, 128);
 #pragma unroll
         for (int j = 0; j < NC; ++j) l[j] *= t.alpha[col0 + j];
+        load();
+        refer();
         if (!first) {  // the output so far
             ok = mbar_wait(&t.odone[(i - 1) & 1], (i - 1) >> 1 & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
             __syncwarp();
@@ -269,6 +323,9 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         }
     }
+    bt_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&t.sfree[sb]);
     // the buffer's last reader; in order for every tile, so that the phases of
     // these barriers are never two ahead of what was seen
     if (i >= PB) ok = mbar_wait(&t.odone[(i - PB) & 1], (i - PB) >> 1 & 1, &g_beam_err, ERR_WAIT_EMPTY) && ok;
@@ -277,18 +334,10 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
     for (int j = 0; j < NC; j += 8) {
         uint32_t w[4];
 #pragma unroll
-        for (int e = 0; e < 8; e += 4) {
-            const float4 nm = *reinterpret_cast<const float4 *>(&t.nm[col0 + j + e]);
-            float q[4] = {fmaf(s[j + e], sl2, nm.x), fmaf(s[j + e + 1], sl2, nm.y), fmaf(s[j + e + 2], sl2, nm.z),
-                          fmaf(s[j + e + 3], sl2, nm.w)};
-#pragma unroll
-            for (int f = 0; f < 4; ++f) {
-                const bool seen = live && (!limits || s[j + e + f] != -INFINITY);
-                q[f] = seen ? exp2_fast(q[f]) : 0.f;
-                l[j + e + f] += q[f];
-            }
-            w[e / 2] = pack2(q[0], q[1], T{});
-            w[e / 2 + 1] = pack2(q[2], q[3], T{});
+        for (int e = 0; e < 4; ++e) {
+            const float q0 = exp2_fast(y[j + 2 * e]), q1 = exp2_fast(y[j + 2 * e + 1]);
+            bt_add2(l[j + 2 * e], l[j + 2 * e + 1], q0, q1);
+            w[e] = pack2(q0, q1, T{});
         }
         const uint32_t col = col0 + j;
         asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(ps + (col >> 6) * Sm::kSubBytes + ((((col >> 3) ^ key) & 7) << 4)),
@@ -336,12 +385,9 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
         if (lane == 0) mbar_arrive(&t.ofree);
         // the sums over the 128 positions, through the probabilities' place
         float *sum = reinterpret_cast<float *>(sm + Sm::kOffP);
+        const uint32_t at = bt_join<NC>(l, [](float u, float v) { return u + v; });
 #pragma unroll
-        for (int j = 0; j < NC; ++j) {
-#pragma unroll
-            for (int d = 16; d; d >>= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], d);
-            if (lane == 0) sum[quad * RT + col0 + j] = l[j];
-        }
+        for (int j = 0; j < (NC > 32 ? NC / 32 : 1); ++j) sum[quad * RT + col0 + at + j] = l[j];
         bar_sync(bar, 128);
         if (wt < NC && col0 + wt < held) {
             const uint32_t r = col0 + wt;
@@ -443,12 +489,9 @@ __global__ void __launch_bounds__(kBtThreads, 1)
             const uint32_t q = smem_u32(bt_sm + Sm::kOffQ);
             uint32_t seg = 0;
             bool ok = true;
-            // S^T = K Q^T of tile i, the first of an item or not
-            auto scores = [&](uint32_t i, bool first, uint32_t rt) {
+            // S^T = K Q^T of tile i
+            auto scores = [&](uint32_t i, uint32_t rt) {
                 const uint32_t s = i % S, b = i & 1;
-                if (first) ok = mbar_wait(&t.qfull, seg & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
-                ok = mbar_wait(&t.kfull[s], i / S & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
-                if (i >= 2) ok = mbar_wait(&t.sfree[b], (i / 2 - 1) & 1, &g_beam_err, ERR_WAIT_EMPTY) && ok;
                 bt_fence_after();
                 bt_fence_proxy();
                 const uint32_t k = smem_u32(bt_sm + 2 * s * Sm::kTile), id = bt_idesc<T>(rt, false);
@@ -459,18 +502,36 @@ __global__ void __launch_bounds__(kBtThreads, 1)
                                bt_desc(q + (d / 4) * (rt * 128) + (d % 4) * 32, 16), id, d != 0);
                 bt_commit(&t.sfull[b]);
             };
+            auto scores_ready = [&](uint32_t i) {  // its K is there and its place in tensor memory is free
+                return mbar_try_wait(&t.kfull[i % S], i / S & 1) && (i < 2 || mbar_try_wait(&t.sfree[i & 1], (i / 2 - 1) & 1));
+            };
+            auto scores_wait = [&](uint32_t i) {
+                ok = mbar_wait(&t.kfull[i % S], i / S & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
+                if (i >= 2) ok = mbar_wait(&t.sfree[i & 1], (i / 2 - 1) & 1, &g_beam_err, ERR_WAIT_EMPTY) && ok;
+            };
             bool first = true;
-            scores(0, true, c.part < a.n_group ? RTP : RTS);
+            ok = mbar_wait(&t.qfull, 0, &g_beam_err, ERR_WAIT_FULL);
+            scores_wait(0);
+            scores(0, c.part < a.n_group ? RTP : RTS);
             for (uint32_t i = 0; c.left; ++i) {
                 const uint32_t n = bt_take(c), rt = c.part < a.n_group ? RTP : RTS;
                 beam_advance(c, n);
-                const bool last = c.left == 0, turn = !last && c.pos >= c.len;
-                if (!last && !turn) scores(i + 1, false, rt);
-                // O^T += V^T P
+                const bool turn = c.pos >= c.len;             // the item ends here
+                bool ahead = c.left != 0 && !turn;            // the next tile's scores come first, if its K is there
                 const uint32_t s = i % S, pb = i % PB;
+                if (first && seg) ok = mbar_wait(&t.ofree, (seg - 1) & 1, &g_beam_err, ERR_WAIT_EMPTY) && ok;
+                if (ahead)
+                    for (uint32_t polls = 0; polls < 4096; ++polls) {
+                        if (scores_ready(i + 1)) {
+                            scores(i + 1, rt);
+                            ahead = false;
+                            break;
+                        }
+                        if (mbar_try_wait(&t.pfull[pb], i / PB & 1)) break;
+                    }
+                // O^T += V^T P
                 ok = mbar_wait(&t.vfull[s], i / S & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
                 ok = mbar_wait(&t.pfull[pb], i / PB & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
-                if (first && seg) ok = mbar_wait(&t.ofree, (seg - 1) & 1, &g_beam_err, ERR_WAIT_EMPTY) && ok;
                 bt_fence_after();
                 bt_fence_proxy();
                 const uint32_t v = smem_u32(bt_sm + (2 * s + 1) * Sm::kTile), ps = smem_u32(bt_sm + Sm::kOffP + pb * Sm::kP);
@@ -482,17 +543,21 @@ __global__ void __launch_bounds__(kBtThreads, 1)
                 bt_commit(&t.empty[s]);
                 bt_commit(&t.odone[i & 1]);
                 first = false;
-                if (turn) {
+                if (turn && c.left) {
                     beam_next_item(a, p, c);
                     ++seg;
-                    first = true;
-                    if (c.left) scores(i + 1, true, c.part < a.n_group ? RTP : RTS);
+                    first = ahead = true;
+                    if (c.left) ok = mbar_wait(&t.qfull, seg & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
+                }
+                if (ahead && c.left) {
+                    scores_wait(i + 1);
+                    scores(i + 1, c.part < a.n_group ? RTP : RTS);
                 }
             }
         }
         __syncwarp();
     } else {
-        float l[(RTP > RTS ? RTP : RTS) / 2];
+        float l[(RTP > RTS ? RTP : RTS) / 2];  // the sums of this thread's position, for half of the rows
         bool fresh = true, ok = true;
 #pragma unroll 1
         for (uint32_t i = 0; c.left; ++i) {
