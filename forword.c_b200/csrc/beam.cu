@@ -76,6 +76,8 @@ bool attn_sizes_ok(const fwb_prefix_attn_t *a) {
     if (rows > 0xffffffu || rows * a->n_query > 0xffffffu || rows * a->n_query * a->n_head > 0x7fffffffu ||
         a->n_head > 65535)
         return fail("fwb_prefix_attention: too many sequences, tokens or heads");
+    if ((uint64_t)a->n_beam * a->n_query * (a->n_head / a->n_head_kv) > 65535)
+        return fail("fwb_prefix_attention: n_beam * n_query * (n_head / n_head_kv) must be at most 65535");
     return true;
 }
 
@@ -150,7 +152,7 @@ bool attn_layout(const fwb_prefix_attn_t *a, AttnLayout &L) {
     const uint64_t units = L.pitems * ((a->prefix_cap + 15) / 16 + L.cost) + L.sitems * ((a->suffix_cap + 15) / 16 + L.cost);
     if (L.pitems + L.sitems > 0x3fffffffu || units > 0x7fffffffu)
         return fail("fwb_prefix_attention: too many rows times positions");
-    L.ctas = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((L.tc ? 1 : 2) * device_sms(), units));
+    L.ctas = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((L.tc ? 1 : a->type == 0 && L.prow == 16 ? 3 : 2) * device_sms(), units));
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t here = at;
@@ -182,7 +184,7 @@ decltype(&cuTensorMapEncodeTiled) map_encoder() {
 // A cache as a 4-D tensor; false where the copy engine does not take its
 // strides (a head or group repeated by a stride of 0, say).
 bool cache_map(const void *base, size_t e, uint64_t hd, uint64_t cap, uint64_t n_kv, uint64_t outer, uint64_t pos,
-               uint64_t head, uint64_t out, CUtensorMap &map) {
+               uint64_t head, uint64_t out, uint32_t positions, CUtensorMap &map) {
     const auto enc = map_encoder();
     if (!cap || !enc) return false;
     const cuuint64_t dims[4] = {hd, cap, n_kv, outer};
@@ -191,7 +193,7 @@ bool cache_map(const void *base, size_t e, uint64_t hd, uint64_t cap, uint64_t n
         if (dims[i + 1] == 1) strides[i] = hd * e;  // never used
         if (!strides[i] || strides[i] >= (cuuint64_t)1 << 40) return false;
     }
-    const cuuint32_t box[4] = {(cuuint32_t)(128 / e), kBaUnit, 1, 1}, one[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {(cuuint32_t)(128 / e), positions, 1, 1}, one[4] = {1, 1, 1, 1};
     const CUtensorMapDataType type = e == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
     return enc(&map, type, 4, const_cast<void *>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -263,11 +265,20 @@ bool run_attn(const BeamAttnArgs &k, const AttnLayout &L, uint8_t *ws, cudaStrea
     p.ctas = L.ctas;
     p.cost = L.cost;
     BeamMaps maps{};
-    p.tma = (cache_map(k.pk, sizeof(T), k.hd, k.pcap, k.n_kv, k.n_group, k.p_pos, k.p_head, k.p_group, maps.pk) &&
-             cache_map(k.pv, sizeof(T), k.hd, k.pcap, k.n_kv, k.n_group, k.p_pos, k.p_head, k.p_group, maps.pv)) |
-            (cache_map(k.sk, sizeof(T), k.hd, k.scap, k.n_kv, k.n_group * k.n_beam, k.s_pos, k.s_head, k.s_seq, maps.sk) &&
-             cache_map(k.sv, sizeof(T), k.hd, k.scap, k.n_kv, k.n_group * k.n_beam, k.s_pos, k.s_head, k.s_seq, maps.sv))
-                << 1;
+    auto prefix = [&](const void *base, uint32_t positions, CUtensorMap &m) {
+        return cache_map(base, sizeof(T), k.hd, k.pcap, k.n_kv, k.n_group, k.p_pos, k.p_head, k.p_group, positions, m);
+    };
+    auto suffix = [&](const void *base, CUtensorMap &m) {
+        return cache_map(base, sizeof(T), k.hd, k.scap, k.n_kv, k.n_group * k.n_beam, k.s_pos, k.s_head, k.s_seq,
+                         kBaUnit, m);
+    };
+    const uint32_t whole = L.tc ? kBtKeys : sizeof(T) == 2 ? 64 : 32;
+    p.tma = (prefix(k.pk, kBaUnit, maps.pk) && prefix(k.pv, kBaUnit, maps.pv) && prefix(k.pk, whole, maps.wk) &&
+             prefix(k.pv, whole, maps.wv)) |
+            (suffix(k.sk, maps.sk) && suffix(k.sv, maps.sv)) << 1;
+    auto by = [](uint64_t d) { return d == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + d - 1) / d); };
+    p.by_gq = by(k.gq);
+    p.by_query = by(k.n_query);
     return k.hd <= 64 ? pick_attn<T, 64>(k, p, maps, L.tc, st) : pick_attn<T, 128>(k, p, maps, L.tc, st);
 }
 

@@ -79,6 +79,7 @@ struct BeamAttnPlan {
     uint32_t ptiles, stiles;  // row tiles of a group / of a sequence
     uint32_t ctas;
     uint32_t cost;         // units that an item's own work is worth
+    uint32_t by_gq, by_query;  // 2^32 / d rounded up, of row numbers below 2^16 (0: d = 1)
     uint32_t tma;          // bit 0: tensor maps of the prefix, 1: of the suffix
 };
 
@@ -256,10 +257,10 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
 }
 
 // The caches as 4-D tensors [group or sequence][kv_head][position][dim],
-// boxes of 16 positions and 128 bytes, 128-byte swizzle, zeros past the
-// dimensions.
+// boxes of 16 positions (a unit) and 128 bytes, 128-byte swizzle, zeros past
+// the dimensions; wk, wv: the prefix in boxes of a whole tile's positions.
 struct BeamMaps {
-    CUtensorMap pk, pv, sk, sv;
+    CUtensorMap pk, pv, sk, sv, wk, wv;
 };
 
 // n positions of a part into stage `st`, by the loading warp: units of 16
@@ -296,6 +297,19 @@ __device__ __forceinline__ void beam_load(const BeamAttnArgs &a, const BeamAttnP
             const uint32_t off = __ballot_sync(0xffffffffu, v != lead && lane + (u & ~1) * kBaUnit < n);
             if (off >> row & 0xffffu) single &= ~(1u << u);
         }
+    }
+    if (pre && single && units == NU) {  // a whole tile: one box per sub-tile
+        if (lane == 0)
+            asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(2 * Tl::kBytes) : "memory");
+        __syncwarp();
+        if (lane < 2 * Tl::kSub) {
+            const uint32_t h = lane % Tl::kSub;
+            const bool k = lane < Tl::kSub;
+            tma_load_4d((k ? ks : vs) + h * (Tl::kKeys * 128), k ? &maps.wk : &maps.wv, (int32_t)(h * (128 / Tl::kEs)),
+                        (int32_t)c.pos, (int32_t)c.kvh, (int32_t)c.part, bar);
+        }
+        mbar_arrive(bar);
+        return;
     }
     uint32_t bytes = 0;
 #pragma unroll
@@ -372,16 +386,21 @@ struct BeamRows {
     int32_t lim[2];                  // positions that rows g and g + 8 see (-1: no such row)
 };
 
-// Query rows of an item: row r of the tile, as the operand of lane (g, t).
+__device__ __forceinline__ uint32_t beam_div(uint32_t n, uint32_t by) { return by ? __umulhi(n, by) : n; }
+
+// Query row r of an item (row = (beam * n_query + token) * gq + head of the
+// group), and the positions that it sees.
 template <typename T, int HD>
-__device__ __forceinline__ const T *beam_q_row(const BeamAttnArgs &a, const BeamCursor &c, uint32_t r, int32_t &lim) {
+__device__ __forceinline__ const T *beam_q_row(const BeamAttnArgs &a, const BeamAttnPlan &p, const BeamCursor &c,
+                                               uint32_t r, int32_t &lim) {
     lim = -1;
     const uint32_t rows = (c.part < a.n_group ? a.n_beam : 1) * a.n_query * a.gq;
     if (r >= rows) return nullptr;
-    const uint32_t h = c.kvh * a.gq + r % a.gq, t = r / a.gq % a.n_query;
+    const uint32_t st = beam_div(r, p.by_gq), sb = beam_div(st, p.by_query);
+    const uint32_t h = c.kvh * a.gq + r - st * a.gq, t = st - sb * a.n_query;
     uint32_t s = c.part - a.n_group;
     if (c.part < a.n_group) {
-        s = c.part * a.n_beam + r / (a.gq * a.n_query);
+        s = c.part * a.n_beam + sb;
         lim = 0x7fffffff;
     } else {
         const uint32_t hidden = a.n_query - 1 - t;
@@ -397,12 +416,12 @@ __device__ __forceinline__ uint32_t beam_q_at(uint32_t row, uint32_t chunk) {
 }
 
 template <typename T, int HD>
-__device__ __forceinline__ void beam_rows_init(const BeamAttnArgs &a, const BeamCursor &c, uint32_t r0, uint32_t qs,
-                                               BeamRows<T, HD> &w) {
+__device__ __forceinline__ void beam_rows_init(const BeamAttnArgs &a, const BeamAttnPlan &p, const BeamCursor &c,
+                                               uint32_t r0, uint32_t qs, BeamRows<T, HD> &w) {
     const uint32_t lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const T *q[2];
-    q[0] = beam_q_row<T, HD>(a, c, r0 + g, w.lim[0]);
-    q[1] = beam_q_row<T, HD>(a, c, r0 + g + 8, w.lim[1]);
+    q[0] = beam_q_row<T, HD>(a, p, c, r0 + g, w.lim[0]);
+    q[1] = beam_q_row<T, HD>(a, p, c, r0 + g + 8, w.lim[1]);
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k)
@@ -699,7 +718,7 @@ __device__ __forceinline__ void beam_step(const BeamAttnArgs &a, const BeamAttnP
     constexpr int KW = Tl::kKeys / (4 / RW);
     const uint32_t warp = threadIdx.x >> 5, rg = warp % RW, kg = warp / RW;
     const uint32_t qs = rows + rg * 16 * HD * 4;
-    if (fresh) beam_rows_init<T, HD>(a, c, c.tile * RW * 16 + rg * 16, qs, w);
+    if (fresh) beam_rows_init<T, HD>(a, p, c, c.tile * RW * 16 + rg * 16, qs, w);
     const bool first = c.pos == 0;
     const uint32_t n = beam_take<T, HD>(c);
     // (after a wait that ran out: the same steps and barriers without the work)

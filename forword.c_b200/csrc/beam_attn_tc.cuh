@@ -159,9 +159,20 @@ __device__ __forceinline__ uint32_t bt_join(float *v, Op op) {
 template <typename T, int HD>
 __device__ __forceinline__ void bt_copy(const BeamAttnArgs &a, const BeamCursor &c, uint32_t n, bool pre,
                                         const uint32_t *seq, uint32_t single, uint32_t dst, const void *base,
-                                        const CUtensorMap *map, uint64_t *bar) {
+                                        const CUtensorMap *map, const CUtensorMap *wide, uint64_t *bar) {
     constexpr int kSub = HD / 64, CH = HD / 8, RP = 32 / CH;
     const uint32_t lane = threadIdx.x & 31, units = (n + kBaUnit - 1) / kBaUnit;
+    if (pre && single && units == kBtKeys / kBaUnit) {  // a whole tile: one box per sub-tile
+        if (lane == 0)
+            asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)),
+                         "r"(kSub * kBtKeys * 128) : "memory");
+        __syncwarp();
+        if (lane < kSub)
+            tma_load_4d(dst + lane * (kBtKeys * 128), wide, (int32_t)(lane * 64), (int32_t)c.pos, (int32_t)c.kvh,
+                        (int32_t)c.part, bar);
+        mbar_arrive(bar);
+        return;
+    }
     single &= (1u << units) - 1;
     if (lane == 0 && single)
         asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)),
@@ -222,7 +233,7 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
         for (int j = 0; j < NR; ++j) {
             const uint32_t r = r0 + j * RPP;
             int32_t lim = -1;
-            const T *q = r < RT ? beam_q_row<T, HD>(a, c, c.tile * RT + r, lim) : nullptr;
+            const T *q = r < RT ? beam_q_row<T, HD>(a, p, c, c.tile * RT + r, lim) : nullptr;
             v[j] = make_uint4(0, 0, 0, 0);
             if (q && ch * 8 < a.hd) v[j] = *reinterpret_cast<const uint4 *>(q + ch * 8);
             if (ch == 0 && r < RT) t.lim[r] = (uint32_t)lim;  // (-1: no such row, sees all and is not written)
@@ -279,12 +290,16 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
         hide();
     };
     load();
-    refer();
-    float over = -INFINITY;
+    bool raise = first;
+    if (!first) {
+        refer();
+        float over = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < NC; ++j) over = fmaxf(over, y[j]);
-    if (bt_any(bar, over > kBtRaise)) {
-        load();
+        for (int j = 0; j < NC; ++j) over = fmaxf(over, y[j]);
+        raise = bt_any(bar, over > kBtRaise);
+        if (raise) load();
+    }
+    if (raise) {
         hide();
         const uint32_t at = bt_join<NC>(y, [](float u, float v) { return fmaxf(u, v); });
 #pragma unroll
@@ -301,11 +316,11 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
             t.nm[r] = -now;  // (+inf while the row has seen nothing)
         }
         bar_sync(bar, 128);
-#pragma unroll
-        for (int j = 0; j < NC; ++j) l[j] *= t.alpha[col0 + j];
         load();
         refer();
-        if (!first) {  // the output so far
+        if (!first) {  // the sums and the output so far
+#pragma unroll
+            for (int j = 0; j < NC; ++j) l[j] *= t.alpha[col0 + j];
             ok = mbar_wait(&t.odone[(i - 1) & 1], (i - 1) >> 1 & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
             __syncwarp();
             bt_fence_after();
@@ -369,15 +384,17 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
         const size_t row0 = (size_t)(item + blockIdx.x) * RT;
         float *o = (pre ? p.po : p.so) + row0 * HD + key;
         const uint32_t to = tmem + 2 * RTP + lanes + col0, held = rows - min(rows, c.tile * RT);
+        constexpr int NV = NC < 32 ? 8 : 32;
 #pragma unroll 1
-        for (uint32_t j = 0; j < NC; j += 8) {
-            float v[8];
-            bt_ld8(to + j, v);
+        for (uint32_t j = 0; j < NC; j += NV) {
+            float v[NV];
+            if constexpr (NV == 32) bt_ld32(to + j, v);
+            else bt_ld8(to + j, v);
             bt_ld_wait();
-            bt_here<8>(v);
+            bt_here<NV>(v);
             if (key < HD)
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
+                for (int e = 0; e < NV; ++e)
                     if (col0 + j + e < held) o[(size_t)(col0 + j + e) * HD] = v[e];
         }
         bt_fence_before();
@@ -473,8 +490,9 @@ __global__ void __launch_bounds__(kBtThreads, 1)
                 }
             }
             const uint32_t ks = smem_u32(bt_sm + 2 * s * Sm::kTile);
-            bt_copy<T, HD>(a, c, n, pre, seq, single, ks, pre ? a.pk : a.sk, pre ? &maps.pk : &maps.sk, &t.kfull[s]);
-            bt_copy<T, HD>(a, c, n, pre, seq, single, ks + Sm::kTile, pre ? a.pv : a.sv, pre ? &maps.pv : &maps.sv, &t.vfull[s]);
+            bt_copy<T, HD>(a, c, n, pre, seq, single, ks, pre ? a.pk : a.sk, pre ? &maps.pk : &maps.sk, &maps.wk, &t.kfull[s]);
+            bt_copy<T, HD>(a, c, n, pre, seq, single, ks + Sm::kTile, pre ? a.pv : a.sv, pre ? &maps.pv : &maps.sv, &maps.wv,
+                           &t.vfull[s]);
             beam_advance(c, n);
             if (c.left && c.pos >= c.len) beam_next_item(a, p, c);
         }

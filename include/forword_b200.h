@@ -156,7 +156,7 @@ int quant_dequant_dev(const void *d_weights, size_t weights_size, uint32_t ggml_
 typedef struct fwb_prefix_attn {
     uint32_t type;                     /* of q, K, V and out: 0, 1 or 30 */
     uint32_t n_group, n_beam, n_query; /* n_query new tokens per sequence */
-    uint32_t n_head, n_head_kv;        /* n_head a multiple of n_head_kv */
+    uint32_t n_head, n_head_kv;        /* n_head a multiple of n_head_kv; n_beam * n_query * (their ratio) <= 65535 */
     uint32_t head_dim;                 /* a multiple of 16, at most 128 */
     uint32_t prefix_cap, suffix_cap;   /* positions that the caches hold (0: none) */
     float scale;                       /* of the scores, positive; 0 -> 1/sqrt(head_dim) */
