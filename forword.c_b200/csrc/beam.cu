@@ -4,7 +4,6 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdio>
-#include <cstdlib>
 
 #include "../../include/forword_b200.h"
 #include "beam_attn.cuh"
@@ -137,18 +136,26 @@ struct AttnLayout {
 bool attn_layout(const fwb_prefix_attn_t *a, AttnLayout &L) {
     const uint64_t gq = a->n_head / a->n_head_kv, srows = gq * a->n_query, prows = srows * a->n_beam;
     const uint32_t hd = a->head_dim <= 64 ? 64 : 128;
-    static const int force = getenv("BTC") ? atoi(getenv("BTC")) : -1;
-    L.tc = a->type != 0 && (force < 0 || force != 0);
-    auto tile = [&](uint64_t rows) {
-        return rows <= 16 ? 16u : rows <= 32 ? 32u : rows <= 64 || !L.tc ? 64u : 128u;
-    };
-    L.prow = tile(prows);
-    L.srow = srows <= 16 ? 16u : L.prow;
+    // More than 64 rows over a long prefix go to the 5th-generation tensor
+    // cores.  Measured (fp16, 8 KV heads of 128, one group, us for warp-level
+    // products against tcgen05): 64 rows 49 / 47 over 30000 positions and
+    // 19 / 21 over 4000; 128 rows 77 / 57, 25 / 29; 256 rows 138 / 96, 38 / 43.
+    // A tile of 64 rows and 1000 positions costs the one what 128 rows cost the
+    // other, about 1 us, and the other begins and ends some 7 to 12 us later.
+    const uint64_t spared = (prows + 63) / 64 - (prows + 127) / 128;
+    L.tc = a->type != 0 &&
+           (uint64_t)a->n_group * a->n_head_kv * a->prefix_cap * spared >=
+               (32000 + 280 * std::min<uint64_t>(prows, 256)) * device_sms() / 148;
+    const uint32_t most = L.tc ? 128 : 64;
+    auto tile = [&](uint64_t rows) { return rows <= 16 ? 16u : rows <= 32 ? 32u : most; };
+    L.prow = L.tc ? 128 : tile(prows);
+    L.srow = tile(srows);
     L.ptiles = (uint32_t)((prows + L.prow - 1) / L.prow);
     L.stiles = (uint32_t)((srows + L.srow - 1) / L.srow);
     L.pitems = a->prefix_cap ? (size_t)a->n_group * a->n_head_kv * L.ptiles : 0;
     L.sitems = a->suffix_cap ? (size_t)a->n_group * a->n_beam * a->n_head_kv * L.stiles : 0;
-    L.cost = L.tc ? getenv("BCOST") ? atoi(getenv("BCOST")) : 20 : 4;
+    // measured: 4 / 20 against 0 save a third where suffixes are many and short
+    L.cost = L.tc ? 20 : 4;
     const uint64_t units = L.pitems * ((a->prefix_cap + 15) / 16 + L.cost) + L.sitems * ((a->suffix_cap + 15) / 16 + L.cost);
     if (L.pitems + L.sitems > 0x3fffffffu || units > 0x7fffffffu)
         return fail("fwb_prefix_attention: too many rows times positions");
@@ -231,20 +238,17 @@ bool launch_attn_tc(const BeamAttnArgs &k, const BeamAttnPlan &p, const BeamMaps
 template <typename T, int HD>
 bool pick_attn(const BeamAttnArgs &k, const BeamAttnPlan &p, const BeamMaps &maps, bool tc, cudaStream_t st) {
     if constexpr (sizeof(T) == 2)
-        if (tc) switch (p.prow + p.srow) {
-            case 16 + 16: return launch_attn_tc<T, HD, 16, 16>(k, p, maps, st);
-            case 32 + 16: return launch_attn_tc<T, HD, 32, 16>(k, p, maps, st);
-            case 32 + 32: return launch_attn_tc<T, HD, 32, 32>(k, p, maps, st);
-            case 64 + 16: return launch_attn_tc<T, HD, 64, 16>(k, p, maps, st);
-            case 64 + 64: return launch_attn_tc<T, HD, 64, 64>(k, p, maps, st);
-            case 128 + 16: return launch_attn_tc<T, HD, 128, 16>(k, p, maps, st);
+        if (tc) switch (p.srow) {
+            case 16: return launch_attn_tc<T, HD, 128, 16>(k, p, maps, st);
+            case 32: return launch_attn_tc<T, HD, 128, 32>(k, p, maps, st);
             default: return launch_attn_tc<T, HD, 128, 128>(k, p, maps, st);
             }
-    switch (p.prow + p.srow) {
-    case 16 + 16: return launch_attn<T, HD, 16, 16>(k, p, maps, st);
-    case 32 + 16: return launch_attn<T, HD, 32, 16>(k, p, maps, st);
-    case 32 + 32: return launch_attn<T, HD, 32, 32>(k, p, maps, st);
-    case 64 + 16: return launch_attn<T, HD, 64, 16>(k, p, maps, st);
+    switch (p.prow * 256 + p.srow) {
+    case 16 * 256 + 16: return launch_attn<T, HD, 16, 16>(k, p, maps, st);
+    case 32 * 256 + 16: return launch_attn<T, HD, 32, 16>(k, p, maps, st);
+    case 32 * 256 + 32: return launch_attn<T, HD, 32, 32>(k, p, maps, st);
+    case 64 * 256 + 16: return launch_attn<T, HD, 64, 16>(k, p, maps, st);
+    case 64 * 256 + 32: return launch_attn<T, HD, 64, 32>(k, p, maps, st);
     default: return launch_attn<T, HD, 64, 64>(k, p, maps, st);
     }
 }

@@ -3,7 +3,7 @@
 //
 // The products are transposed so that few query rows still fill the machine:
 // a tile's 128 positions are the M dimension of S^T = K Q^T (N: the query
-// rows, 16 to 128), and the head's dimensions that of O^T += V^T P.  A thread
+// rows, 16, 32 or 128), and the head's dimensions that of O^T += V^T P.  A thread
 // of the softmax owns one position and half of the rows, so every thread has
 // the same work whatever the number of rows is, and the sums over positions
 // are kept per thread and joined once per item.
@@ -34,14 +34,13 @@ struct BeamTc {
     static constexpr int kSub = HD / 64;                           // sub-tiles of 128 bytes
     static constexpr uint32_t kSubBytes = kBtKeys * 128;           // of K, V
     static constexpr uint32_t kTile = kSub * kSubBytes;
-    static constexpr int kStages = RT == 128 ? 2 : 3;
-    static constexpr int kPBufs = RT == 128 ? 2 : 1;
-    static constexpr uint32_t kQ = RT * HD * 2, kP = (RT > 64 ? 2 : 1) * kSubBytes;
+    static constexpr int kStages = 2, kPBufs = 2;
+    static constexpr uint32_t kQ = RT * HD * 2, kP = 2 * kSubBytes;
     static constexpr uint32_t kOffQ = 2 * kTile * kStages, kOffP = kOffQ + kQ, kOffTail = kOffP + kPBufs * kP;
-    static constexpr uint32_t kTmem = RT == 128 ? 512 : RT == 64 ? 256 : RT == 32 ? 128 : 64;  // >= 3 RT columns
+    static constexpr uint32_t kTmem = 512;                         // a power of two, at least 3 RT columns
 };
 struct BeamTcTail {
-    uint64_t kfull[3], vfull[3], empty[3], sfull[2], sfree[2], pfull[2], odone[2], ofree, qfull;
+    uint64_t kfull[2], vfull[2], empty[2], sfull[2], sfree[2], pfull[2], odone[2], ofree, qfull;
     uint32_t tmem;
     alignas(16) float nm[128];  // minus the rows' references; +inf: none yet
     float alpha[128];
