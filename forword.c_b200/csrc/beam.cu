@@ -395,6 +395,22 @@ using namespace fwb;
 
 extern "C" {
 
+int fwb_beam_status(void *stream) {
+    uint32_t e = 0;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (!launched(cudaMemcpyFromSymbolAsync(&e, g_beam_err, 4, 0, cudaMemcpyDeviceToHost, st), "fwb_beam_status") ||
+        !launched(cudaStreamSynchronize(st), "fwb_beam_status"))
+        return -1;
+    if (!e) return 0;
+    const uint32_t zero = 0;
+    cudaMemcpyToSymbolAsync(g_beam_err, &zero, 4, 0, cudaMemcpyHostToDevice, st);
+    cudaStreamSynchronize(st);
+    char b[96];
+    snprintf(b, sizeof b, "fwb_beam_status: device error word 0x%x (a bounded wait in the kernel ran out)", e);
+    fail(b);
+    return -1;
+}
+
 size_t fwb_prefix_attention_workspace(const fwb_prefix_attn_t *a) {
     AttnLayout L;
     return attn_sizes_ok(a) && attn_layout(a, L) ? L.bytes : 0;

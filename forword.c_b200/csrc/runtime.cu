@@ -29,6 +29,7 @@
 #include "misc_kernels.cuh"
 #include "gemm_tc.cuh"
 #include "prefill.cuh"
+#include "beam_step.cuh"
 #include "sampler.cuh"
 
 namespace fwb {
@@ -1721,6 +1722,243 @@ int fwb_prefill(fwb_model_t *m, const uint32_t *tokens, size_t n, size_t pos0, f
     }
     // the last token through the decode step gives the logits
     return fwb_forward(m, tokens[n - 1], pos0 + n - 1, logits_host);
+}
+
+}  // extern "C"
+
+// --- beam search ------------------------------------------------------------------
+// Device memory of one call.
+struct BeamBuffers {
+    std::vector<void *> held;
+    ~BeamBuffers() {
+        for (void *p : held) cudaFree(p);
+    }
+    template <typename T>
+    bool get(T **p, size_t n) {
+        CK(cudaMalloc((void **)p, std::max<size_t>(n, 1) * sizeof(T)));
+        held.push_back(*p);
+        return true;
+    }
+};
+
+struct BeamRun {
+    fwb_model *m;
+    BeamBuffers mem;
+    uint32_t W, cap, pos0;  // beams, suffix positions, prompt length
+    float *ks, *vs;         // suffix caches [layer][beam][kv_head][cap][hd]
+    int32_t *slots;         // [beam][cap]: the beam slot that holds a position
+    int32_t *len;           // [0] prompt length, [1..W] suffix lengths
+    float *att, *logits, *scores, *best;
+    int32_t *parent, *token;
+    uint8_t *attn_ws, *select_ws;
+    size_t attn_bytes, select_bytes;
+    fwb_prefix_attn_t args;
+};
+
+// tokens[b] of every beam at suffix position `at` through the model: their
+// logits in r.logits.
+static bool beam_forward(BeamRun &r, const uint32_t *tokens, uint32_t at) {
+    fwb_model *m = r.m;
+    const ModelConfig &c = m->cfg;
+    const uint32_t E = c.n_embd, F = c.n_ff, hd = c.head_dim, H = c.n_head, KV = c.n_head_kv, W = r.W;
+    const uint32_t NQ = H * hd, NKV = KV * hd, NQKV = NQ + 2 * NKV, pos = r.pos0 + at;
+    cudaStream_t st = m->st;
+    CK(cudaMemcpyAsync(m->pf_tok, tokens, (size_t)W * 4, cudaMemcpyHostToDevice, st));
+    pf_embed_kernel<<<W, 256, 0, st>>>(m->embd.p, m->embd.type, E, m->embd.row_bytes, m->pf_tok, m->pf_x);
+    const size_t layer_kv = (size_t)KV * m->kv_ctx * hd, layer_sfx = (size_t)W * KV * r.cap * hd;
+    auto gemm = [&](const Mat &t, const __half *x, float *y, size_t K, size_t N, uint32_t mode, int i, uint32_t l) {
+        const __half *w16 = i < 0 || m->pf_w16.empty() ? nullptr : m->pf_w16[5 * l + i];
+        return launch_tc_gemm(t.p, (size_t)t.rows * t.row_bytes, t.type, x, y, K, N, W, N, mode, st, m->err, w16);
+    };
+    auto f16 = [&](const float *x, size_t n, __half *h) {
+        beam_f16_kernel<<<(unsigned)std::min<size_t>(592, (n / 2 + 255) / 256), 256, 0, st>>>(x, n, h);
+    };
+    for (uint32_t l = 0; l < c.n_layer; ++l) {
+        const LayerW &w = m->layers[l];
+        float *ks = r.ks + l * layer_sfx, *vs = r.vs + l * layer_sfx;
+        pf_rmsnorm_f16_kernel<<<W, 256, 0, st>>>(m->pf_x, w.attn_norm, c.norm_eps, E, m->pf_h16);
+        if (!gemm(w.qkv, m->pf_h16, m->pf_qkv, E, NQKV, TC_STORE, 0, l)) return false;
+        beam_rope_kv_kernel<<<W, 256, 0, st>>>(m->pf_qkv, pos, at, r.cap, NQ, NKV, hd, m->rope_cos, m->rope_sin,
+                                               m->pf_q, ks, vs);
+        fwb_prefix_attn_t &a = r.args;
+        a.prefix_k = m->kc + l * layer_kv;
+        a.prefix_v = m->vc + l * layer_kv;
+        a.suffix_k = ks;
+        a.suffix_v = vs;
+        if (fwb_prefix_attention_dev(&a, r.attn_ws, r.attn_bytes, st) != 0) return false;
+        f16(r.att, (size_t)W * NQ, m->pf_a16);
+        if (!gemm(w.o, m->pf_a16, m->pf_x, NQ, E, TC_ADD, 1, l)) return false;
+        pf_rmsnorm_f16_kernel<<<W, 256, 0, st>>>(m->pf_x, w.ffn_norm, c.norm_eps, E, m->pf_h16);
+        if (!gemm(w.gate, m->pf_h16, m->pf_g, E, F, TC_STORE, 2, l) || !gemm(w.up, m->pf_h16, m->pf_u, E, F, TC_STORE, 3, l))
+            return false;
+        pf_swiglu_kernel<<<(unsigned)std::min<size_t>(4 * 148, ((size_t)W * F / 4 + 255) / 256), 256, 0, st>>>(
+            m->pf_g, m->pf_u, (size_t)W * F, m->pf_h16);
+        if (!gemm(w.down, m->pf_h16, m->pf_x, F, E, TC_ADD, 4, l)) return false;
+    }
+    if (m->out_norm) pf_rmsnorm_f16_kernel<<<W, 256, 0, st>>>(m->pf_x, m->out_norm, c.norm_eps, E, m->pf_h16);
+    else f16(m->pf_x, (size_t)W * E, m->pf_h16);
+    if (!gemm(m->head, m->pf_h16, r.logits, E, c.n_vocab, TC_STORE, -1, 0)) return false;
+    CK(cudaGetLastError());
+    return true;
+}
+
+struct BeamHyp {
+    std::vector<uint32_t> tokens;
+    double sum = 0, rank = 0;  // accumulated log-probability; the same with the length's penalty
+};
+
+static bool beam_search(fwb_model *m, const uint32_t *prompt, size_t n, size_t n_beam, size_t max_new, int64_t eos,
+                        float length_penalty, std::vector<BeamHyp> &done) {
+    const ModelConfig &c = m->cfg;
+    BeamRun r{};
+    r.m = m;
+    r.W = (uint32_t)n_beam;
+    r.cap = (uint32_t)max_new;
+    r.pos0 = (uint32_t)n;
+    const uint32_t W = r.W, V = c.n_vocab, K = std::min<uint32_t>(2 * W, V), hd = c.head_dim;
+    const size_t sfx = (size_t)c.n_layer * W * c.n_head_kv * r.cap * hd;
+    fwb_prefix_attn_t &a = r.args;
+    a.n_group = a.n_query = 1;
+    a.n_beam = W;
+    a.n_head = c.n_head;
+    a.n_head_kv = c.n_head_kv;
+    a.head_dim = hd;
+    a.prefix_cap = m->kv_ctx;
+    a.suffix_cap = r.cap;
+    r.attn_bytes = fwb_prefix_attention_workspace(&a);
+    const size_t first = fwb_beam_select_workspace(0, 1, 1, V, K), later = fwb_beam_select_workspace(0, 1, W, V, K);
+    if (!r.attn_bytes || !first || !later) return false;
+    r.select_bytes = std::max(first, later);
+    if (!prefill_alloc(m) || !r.mem.get(&r.ks, sfx) || !r.mem.get(&r.vs, sfx) || !r.mem.get(&r.slots, (size_t)W * r.cap) ||
+        !r.mem.get(&r.len, 1 + W) || !r.mem.get(&r.att, (size_t)W * c.n_head * hd) ||
+        !r.mem.get(&r.logits, (size_t)W * V) || !r.mem.get(&r.scores, W) || !r.mem.get(&r.best, K) ||
+        !r.mem.get(&r.parent, K) || !r.mem.get(&r.token, K) || !r.mem.get(&r.attn_ws, r.attn_bytes) ||
+        !r.mem.get(&r.select_ws, r.select_bytes))
+        return false;
+    a.q = m->pf_q;
+    a.q_seq_stride = a.q_token_stride = (uint64_t)c.n_head * hd;
+    a.q_head_stride = hd;
+    a.prefix_pos_stride = a.suffix_pos_stride = hd;
+    a.prefix_head_stride = (uint64_t)m->kv_ctx * hd;
+    a.prefix_group_stride = a.prefix_head_stride * c.n_head_kv;
+    a.suffix_head_stride = (uint64_t)r.cap * hd;
+    a.suffix_seq_stride = a.suffix_head_stride * c.n_head_kv;
+    a.prefix_len = r.len;
+    a.suffix_len = r.len + 1;
+    a.slots = r.slots;
+    a.slots_stride = r.cap;
+    a.out = r.att;
+    if (fwb_prefill(m, prompt, n, 0, nullptr) != 0) return false;
+    cudaStream_t st = m->st;
+    {  // every position starts as its own beam's
+        std::vector<int32_t> own((size_t)W * r.cap);
+        for (size_t i = 0; i < own.size(); ++i) own[i] = (int32_t)(i / r.cap);
+        CK(cudaMemcpyAsync(r.slots, own.data(), own.size() * 4, cudaMemcpyHostToDevice, st));
+        CK(cudaStreamSynchronize(st));
+    }
+    std::vector<BeamHyp> live(1);
+    std::vector<float> score(K), sum(W, 0.f);
+    std::vector<int32_t> parent(K), token(K), next_parent(W), lens(1 + W);
+    std::vector<uint32_t> next_token(W);
+    auto penalised = [&](double s, size_t len) { return length_penalty == 0.f ? s : s / std::pow((double)len, (double)length_penalty); };
+    auto worst = [&] {  // of the W best
+        std::vector<double> ranks;
+        for (const BeamHyp &h : done) ranks.push_back(h.rank);
+        std::nth_element(ranks.begin(), ranks.begin() + (W - 1), ranks.end(), std::greater<double>());
+        return ranks[W - 1];
+    };
+    CK(cudaMemsetAsync(m->err, 0, 4, st));
+    for (uint32_t t = 0; t < r.cap && !live.empty(); ++t) {
+        // the prompt's logits are one row; later every beam has one
+        const uint32_t rows = t == 0 ? 1 : W;
+        CK(cudaMemcpyAsync(r.scores, sum.data(), rows * 4, cudaMemcpyHostToDevice, st));
+        if (fwb_beam_select_dev(t == 0 ? m->logits : r.logits, 0, 1, rows, V, V, r.scores, K, r.best, r.parent, r.token,
+                                r.select_ws, r.select_bytes, st) != 0)
+            return false;
+        CK(cudaMemcpyAsync(score.data(), r.best, K * 4, cudaMemcpyDeviceToHost, st));
+        CK(cudaMemcpyAsync(parent.data(), r.parent, K * 4, cudaMemcpyDeviceToHost, st));
+        CK(cudaMemcpyAsync(token.data(), r.token, K * 4, cudaMemcpyDeviceToHost, st));
+        if (!finish(m)) return false;  // (waits; a GEMM's bounded wait that ran out)
+        if (fwb_beam_status(st) != 0) return false;
+        std::vector<BeamHyp> next;
+        for (uint32_t i = 0; i < K && next.size() < W; ++i) {
+            if (!std::isfinite(score[i])) break;
+            BeamHyp h = live[(size_t)parent[i]];
+            h.tokens.push_back((uint32_t)token[i]);
+            h.sum = score[i];
+            h.rank = penalised(h.sum, h.tokens.size());
+            if (token[i] == eos) {
+                if (i < W) done.push_back(std::move(h));  // (an end of a beam that would not survive does not count)
+                continue;
+            }
+            next_parent[next.size()] = parent[i];
+            next_token[next.size()] = (uint32_t)token[i];
+            next.push_back(std::move(h));
+        }
+        live.swap(next);
+        if (done.size() >= W) {
+            // no live beam can pass the W found (for a length penalty of at most 0
+            // scores only fall; otherwise the search ends here, as is usual)
+            if (length_penalty != 0.f || live.empty() || live[0].rank <= worst()) break;
+        }
+        if (t + 1 == r.cap || live.empty()) break;
+        for (uint32_t b = 0; b < W; ++b) {
+            const bool alive = b < live.size();
+            if (!alive) { next_parent[b] = 0; next_token[b] = 0; }
+            sum[b] = alive ? (float)live[b].sum : -INFINITY;
+        }
+        // the slots of the positions so far follow their beams; position t is
+        // each beam's own
+        CK(cudaMemcpyAsync(r.parent, next_parent.data(), W * 4, cudaMemcpyHostToDevice, st));
+        if (t && fwb_beam_reorder_dev(r.slots, r.slots, r.parent, 1, 1, W, 1, (size_t)t * 4, 0, (size_t)r.cap * 4, 0, 0,
+                                      (size_t)r.cap * 4, 0, st) != 0)
+            return false;
+        lens[0] = (int32_t)n;
+        for (uint32_t b = 0; b < W; ++b) lens[1 + b] = (int32_t)t + 1;
+        CK(cudaMemcpyAsync(r.len, lens.data(), (1 + W) * 4, cudaMemcpyHostToDevice, st));
+        live.resize(W);  // (dead beams have score -inf and offer nothing)
+        if (!beam_forward(r, next_token.data(), t)) return false;
+    }
+    for (BeamHyp &h : live)
+        if (!h.tokens.empty()) done.push_back(std::move(h));
+    std::stable_sort(done.begin(), done.end(), [](const BeamHyp &x, const BeamHyp &y) { return x.rank > y.rank; });
+    if (done.size() > W) done.resize(W);
+    CK(cudaStreamSynchronize(st));
+    return true;
+}
+
+extern "C" {
+
+int fwb_beam_search(fwb_model_t *m, const uint32_t *prompt, size_t n, size_t n_beam, size_t max_new, int64_t eos,
+                    float length_penalty, uint32_t *tokens_out, uint32_t *lengths_out, float *scores_out) {
+    if (!m || !prompt || !n || !tokens_out || !lengths_out || !scores_out) {
+        set_err("fwb_beam_search: null argument or empty prompt");
+        return -1;
+    }
+    if (!n_beam || n_beam > 64 || !max_new) { set_err("fwb_beam_search: n_beam must be 1..64 and max_new positive"); return -1; }
+    if (n > m->kv_ctx || max_new > m->kv_ctx - n) { set_err("fwb_beam_search: positions exceed the KV cache"); return -1; }
+    if (!(std::isfinite(length_penalty))) { set_err("fwb_beam_search: length_penalty must be finite"); return -1; }
+    for (size_t i = 0; i < n; ++i)
+        if (prompt[i] >= m->cfg.n_vocab) { set_err("fwb_beam_search: token ID out of range"); return -1; }
+    if (!prefill_eligible(m) || m->head.type != 2 || m->head.cols % kTcK || (uintptr_t)m->head.p % 4 || m->cfg.head_dim % 16) {
+        set_err("fwb_beam_search: needs a model on one GPU whose layers and LM head are Q4_0 and whose head_dim is a multiple of 16");
+        return -1;
+    }
+    cudaSetDevice(m->dev);
+    try {
+        std::vector<BeamHyp> done;
+        if (!beam_search(m, prompt, n, n_beam, max_new, eos, length_penalty, done)) return -1;
+        for (size_t b = 0; b < n_beam; ++b) {
+            const bool have = b < done.size();
+            lengths_out[b] = have ? (uint32_t)done[b].tokens.size() : 0;
+            scores_out[b] = have ? (float)done[b].rank : -INFINITY;
+            if (have) std::copy(done[b].tokens.begin(), done[b].tokens.end(), tokens_out + b * max_new);
+        }
+    } catch (const std::exception &) {
+        set_err("fwb_beam_search: out of host memory");
+        return -1;
+    }
+    return 0;
 }
 
 int fwb_forward(fwb_model_t *m, uint32_t token, size_t pos, float *logits_host) {

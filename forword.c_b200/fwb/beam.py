@@ -4,6 +4,9 @@ include/forword_b200.h on torch CUDA tensors.
 ``PrefixAttention``  attention of sequences that share a prefix
 ``BeamSelect``       the best of beams x vocabulary
 ``reorder``          per-beam state moved by the selected parents
+``check_status``     whether every attention kernel so far completed
+
+(``Model.beam_search`` runs them on a model.)
 
 Thin plumbing over the CUDA library (no CPU fallback): a plan checks sizes
 once and keeps its workspace; a call checks its tensors and enqueues on the
@@ -294,3 +297,11 @@ def reorder(src, parent, dst=None):
                                 st[0] * size, st[1] * size, si, dt[0] * size, dt[1] * size, di, _raw_stream(dev)) != 0:
         raise FwbError(_err(lib))
     return dst
+
+
+def check_status() -> None:
+    """Waits for the current stream and raises FwbError if a bounded wait of an
+    attention kernel on this device ran out since the last look (fwb_beam_status)."""
+    lib = native.product()
+    if lib.fwb_beam_status(_raw_stream(torch.cuda.current_device())) != 0:
+        raise FwbError(_err(lib))

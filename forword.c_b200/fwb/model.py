@@ -142,6 +142,21 @@ class Model:
             raise FwbError(f"fwb_sample: {_err(self.lib)}")
         return int(tok.value), int(st.value)
 
+    def beam_search(self, prompt, n_beam: int, max_new: int, eos: int | None = None,
+                    length_penalty: float = 0.0) -> list[tuple[np.ndarray, float]]:
+        """fwb_beam_search: the continuations found, best first, as (tokens, score)."""
+        p = np.ascontiguousarray(prompt, dtype=np.uint32)
+        tok = np.zeros((n_beam, max_new), dtype=np.uint32)
+        n = np.zeros(n_beam, dtype=np.uint32)
+        score = np.zeros(n_beam, dtype=np.float32)
+        u32 = ctypes.POINTER(ctypes.c_uint32)
+        rc = self.lib.fwb_beam_search(self.h, p.ctypes.data_as(u32), p.size, n_beam, max_new, -1 if eos is None else eos,
+                                      length_penalty, tok.ctypes.data_as(u32), n.ctypes.data_as(u32),
+                                      score.ctypes.data_as(ctypes.POINTER(ctypes.c_float)))
+        if rc != 0:
+            raise FwbError(f"fwb_beam_search: {_err(self.lib)}")
+        return [(tok[b, :n[b]].copy(), float(score[b])) for b in range(n_beam) if n[b]]
+
     def kv_load(self, layer: int, pos0: int, k: np.ndarray, v: np.ndarray) -> None:
         k = np.ascontiguousarray(k, dtype=np.float32)
         v = np.ascontiguousarray(v, dtype=np.float32)

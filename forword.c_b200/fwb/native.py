@@ -101,3 +101,6 @@ def _declare(lib) -> None:
     sig("fwb_beam_select_dev", _i32, _vp, _u32, _sz, _sz, _sz, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _sz, _vp)
     sig("fwb_beam_select_workspace", _sz, _u32, _sz, _sz, _sz, _sz)
     sig("fwb_beam_reorder_dev", _i32, _vp, _vp, _vp, *[_sz] * 11, _vp)
+    sig("fwb_beam_status", _i32, _vp)
+    sig("fwb_beam_search", _i32, _vp, _c.POINTER(_u32), _sz, _sz, _sz, _c.c_int64, _c.c_float, _c.POINTER(_u32),
+        _c.POINTER(_u32), _fp)

@@ -192,6 +192,14 @@ typedef struct fwb_prefix_attn {
  */
 int fwb_prefix_attention_dev(const fwb_prefix_attn_t *a, void *workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * Status of the fwb_prefix_attention_dev calls on the current device since
+ * the last look, after the work queued on `stream` (synchronises it): 0, or
+ * -1 if one of the kernel's bounded waits ran out (its outputs are then not
+ * valid); looking clears it.
+ */
+int fwb_beam_status(void *stream);
+
 /* Bytes of workspace that fwb_prefix_attention_dev needs for a's type, sizes
  * and capacities (its pointers, lengths and strides are not looked at); 0
  * with fwb_last_error() for sizes that it does not take. */
@@ -407,6 +415,22 @@ int fwb_tp_connect(fwb_model_t *m, const void *handles);
  */
 int fwb_tp_shard(const char *gguf_path, const char *tensor, int as_head, int rank, int world,
                  void *out, size_t cap, size_t *out_bytes);
+
+/*
+ * Beam search: prompt[0..n) once through fwb_prefill (positions 0..n-1 of the
+ * model's cache, which every beam then shares), and up to max_new tokens of
+ * n_beam continuations together, with the operators above: their suffix keys
+ * and values live in buffers of the call.  A continuation ends with token
+ * `eos` (-1: none does) or at max_new tokens; the search ends when n_beam
+ * ended ones are found and, without a length penalty, no live one can pass
+ * them.  Results are sorted by the sum of log-probabilities, divided by
+ * length^length_penalty (0: not divided): tokens_out [n_beam][max_new],
+ * lengths_out and scores_out [n_beam] (length 0 and score -inf where there
+ * are fewer).  For models on one GPU whose layers and LM head are Q4_0, with
+ * n + max_new <= kv_ctx and n_beam at most 64; -1 otherwise.  Synchronous.
+ */
+int fwb_beam_search(fwb_model_t *m, const uint32_t *prompt, size_t n, size_t n_beam, size_t max_new, int64_t eos,
+                    float length_penalty, uint32_t *tokens_out, uint32_t *lengths_out, float *scores_out);
 
 /* Device logits of the last step (n_vocab fp32) and the model's CUDA stream. */
 const float *fwb_logits_dev(fwb_model_t *m);
