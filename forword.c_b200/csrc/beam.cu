@@ -30,11 +30,12 @@ bool launched(cudaError_t e, const char *who) {
 // A kernel whose blocks may be placed while the stream's kernel before it
 // ends (it waits for that one's results itself).
 template <typename F, typename... A>
-cudaError_t launch_after(F *fn, dim3 grid, unsigned threads, unsigned cluster, cudaStream_t st, const A &...args) {
+cudaError_t launch_after(F *fn, dim3 grid, unsigned threads, unsigned smem, unsigned cluster, cudaStream_t st, const A &...args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
-    cfg.stream = st;  // (no dynamic shared memory)
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -128,7 +129,7 @@ uint32_t device_sms() {
 struct AttnLayout {
     bool tc;            // on the 5th-generation tensor cores (beam_attn_tc.cuh)
     uint32_t prow, srow;  // rows of a prefix / suffix tile
-    uint32_t ptiles, stiles, ctas, cost;
+    uint32_t ptiles, stiles, ctas, tctas, cost;  // (tctas: of the tcgen05 kernel, the others then the suffixes')
     size_t pitems, sitems, bytes;
     size_t po, so, pml, sml, pcta, scta;
 };
@@ -146,27 +147,29 @@ bool attn_layout(const fwb_prefix_attn_t *a, AttnLayout &L) {
     L.tc = a->type != 0 &&
            (uint64_t)a->n_group * a->n_head_kv * a->prefix_cap * spared >=
                (32000 + 280 * std::min<uint64_t>(prows, 256)) * device_sms() / 148;
-    const uint32_t most = L.tc ? 128 : 64;
-    auto tile = [&](uint64_t rows) { return rows <= 16 ? 16u : rows <= 32 ? 32u : most; };
-    L.prow = L.tc ? 128 : tile(prows);
+    auto tile = [&](uint64_t rows) { return rows <= 16 ? 16u : rows <= 32 ? 32u : 64u; };
+    L.prow = L.tc ? kBtRows : tile(prows);
     L.srow = tile(srows);
     L.ptiles = (uint32_t)((prows + L.prow - 1) / L.prow);
     L.stiles = (uint32_t)((srows + L.srow - 1) / L.srow);
     L.pitems = a->prefix_cap ? (size_t)a->n_group * a->n_head_kv * L.ptiles : 0;
     L.sitems = a->suffix_cap ? (size_t)a->n_group * a->n_beam * a->n_head_kv * L.stiles : 0;
-    // measured: 4 / 20 against 0 save a third where suffixes are many and short
+    // (measured: 4 and 20 against 0 save a third where suffixes are many and short)
     L.cost = L.tc ? 20 : 4;
-    const uint64_t units = L.pitems * ((a->prefix_cap + 15) / 16 + L.cost) + L.sitems * ((a->suffix_cap + 15) / 16 + L.cost);
+    const uint64_t punits = L.pitems * ((a->prefix_cap + 15) / 16 + L.cost),
+                   sunits = L.sitems * ((a->suffix_cap + 15) / 16 + 4), units = punits + sunits;
     if (L.pitems + L.sitems > 0x3fffffffu || units > 0x7fffffffu)
         return fail("fwb_prefix_attention: too many rows times positions");
-    L.ctas = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>((L.tc ? 1 : a->type == 0 && L.prow == 16 ? 3 : 2) * device_sms(), units));
+    const uint64_t sms = device_sms();
+    L.ctas = (uint32_t)std::max<uint64_t>(1, std::min(a->type == 0 && L.prow == 16 ? 3 * sms : 2 * sms, L.tc ? sunits : units));
+    L.tctas = L.tc ? (uint32_t)std::min(sms, punits) : 0;
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t here = at;
         at += (n + 255) & ~(size_t)255;
         return here;
     };
-    const size_t pslots = (L.pitems + L.ctas) * L.prow, sslots = (L.sitems + L.ctas) * L.srow;
+    const size_t pslots = (L.pitems + std::max(L.ctas, L.tctas)) * L.prow, sslots = (L.sitems + L.ctas) * L.srow;
     L.po = take(pslots * hd * 4);
     L.so = take(sslots * hd * 4);
     L.pml = take(pslots * 8);
@@ -207,14 +210,6 @@ bool cache_map(const void *base, size_t e, uint64_t hd, uint64_t cap, uint64_t n
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int HD>
-bool launch_join(const BeamAttnArgs &k, const BeamAttnPlan &p, cudaStream_t st) {
-    if (!launched(cudaGetLastError(), "fwb_prefix_attention launch")) return false;
-    return launched(launch_after(beam_attn_join_kernel<T, HD>, dim3(k.n_group * k.n_beam * k.n_query, k.n_head),
-                                 kBaThreads, 1, st, k, p),
-                    "fwb_prefix_attention launch");
-}
-
 // PR, SR: rows of a prefix / suffix tile.
 template <typename T, int HD, int PR, int SR>
 bool launch_attn(const BeamAttnArgs &k, const BeamAttnPlan &p, const BeamMaps &maps, cudaStream_t st) {
@@ -222,27 +217,21 @@ bool launch_attn(const BeamAttnArgs &k, const BeamAttnPlan &p, const BeamMaps &m
     constexpr uint32_t smem = beam_attn_smem<T, HD, PR / 16, SR / 16>();
     if (!opt_in(beam_attn_kernel<T, HD, PR / 16, SR / 16>, smem, ready, "fwb_prefix_attention")) return false;
     beam_attn_kernel<T, HD, PR / 16, SR / 16><<<p.ctas, kBaThreads + kBaLoader, smem, st>>>(k, p, maps);
-    return launch_join<T, HD>(k, p, st);
-}
-
-template <typename T, int HD, int PR, int SR>
-bool launch_attn_tc(const BeamAttnArgs &k, const BeamAttnPlan &p, const BeamMaps &maps, cudaStream_t st) {
-    static bool ready[64] = {};
-    constexpr uint32_t smem = beam_tc_smem<HD, PR>();
-    static_assert(smem <= 227 * 1024, "shared memory");
-    if (!opt_in(beam_attn_tc_kernel<T, HD, PR, SR>, smem, ready, "fwb_prefix_attention")) return false;
-    beam_attn_tc_kernel<T, HD, PR, SR><<<p.ctas, kBtThreads, smem, st>>>(k, p, maps);
-    return launch_join<T, HD>(k, p, st);
+    return launched(cudaGetLastError(), "fwb_prefix_attention launch");
 }
 
 template <typename T, int HD>
-bool pick_attn(const BeamAttnArgs &k, const BeamAttnPlan &p, const BeamMaps &maps, bool tc, cudaStream_t st) {
-    if constexpr (sizeof(T) == 2)
-        if (tc) switch (p.srow) {
-            case 16: return launch_attn_tc<T, HD, 128, 16>(k, p, maps, st);
-            case 32: return launch_attn_tc<T, HD, 128, 32>(k, p, maps, st);
-            default: return launch_attn_tc<T, HD, 128, 128>(k, p, maps, st);
-            }
+bool launch_attn_tc(const BeamAttnArgs &k, const BeamAttnPlan &p, const BeamMaps &maps, cudaStream_t st) {
+    static bool ready[64] = {};
+    constexpr uint32_t smem = beam_tc_smem<HD>();
+    static_assert(smem <= 227 * 1024, "shared memory");
+    if (!opt_in(beam_attn_tc_kernel<T, HD>, smem, ready, "fwb_prefix_attention")) return false;
+    return launched(launch_after(beam_attn_tc_kernel<T, HD>, dim3(p.ctas), kBtThreads, smem, 1, st, k, p, maps),
+                    "fwb_prefix_attention launch");
+}
+
+template <typename T, int HD>
+bool pick_attn(const BeamAttnArgs &k, const BeamAttnPlan &p, const BeamMaps &maps, cudaStream_t st) {
     switch (p.prow * 256 + p.srow) {
     case 16 * 256 + 16: return launch_attn<T, HD, 16, 16>(k, p, maps, st);
     case 32 * 256 + 16: return launch_attn<T, HD, 32, 16>(k, p, maps, st);
@@ -253,9 +242,34 @@ bool pick_attn(const BeamAttnArgs &k, const BeamAttnPlan &p, const BeamMaps &map
     }
 }
 
+// The kernels of a call: all parts by one, or the suffixes by that and the
+// prefixes by the tcgen05 kernel; then the join.
+template <typename T, int HD>
+bool run_parts(const BeamAttnArgs &k, BeamAttnPlan p, const BeamMaps &maps, const AttnLayout &L, cudaStream_t st) {
+    const uint32_t seqs = k.n_group * k.n_beam;
+    p.part0 = L.tc ? k.n_group : 0;
+    p.parts = k.n_group + seqs;
+    p.cost = 4;
+    p.ctas = L.ctas;
+    if (L.tc) p.prow = p.srow;  // (its kernel has no prefix part)
+    if (!pick_attn<T, HD>(k, p, maps, st)) return false;
+    p.prow = L.prow;
+    if constexpr (sizeof(T) == 2)
+        if (L.tc) {
+            p.part0 = 0;
+            p.parts = k.n_group;
+            p.cost = L.cost;
+            p.ctas = L.tctas;
+            if (!launch_attn_tc<T, HD>(k, p, maps, st)) return false;
+            p.ctas = std::max(L.ctas, L.tctas);
+        }
+    return launched(launch_after(beam_attn_join_kernel<T, HD>, dim3(seqs * k.n_query, k.n_head), kBaThreads, 0, 1, st, k, p),
+                    "fwb_prefix_attention launch");
+}
+
 template <typename T>
 bool run_attn(const BeamAttnArgs &k, const AttnLayout &L, uint8_t *ws, cudaStream_t st) {
-    BeamAttnPlan p;
+    BeamAttnPlan p{};
     p.po = reinterpret_cast<float *>(ws + L.po);
     p.so = reinterpret_cast<float *>(ws + L.so);
     p.pml = reinterpret_cast<float2 *>(ws + L.pml);
@@ -266,8 +280,6 @@ bool run_attn(const BeamAttnArgs &k, const AttnLayout &L, uint8_t *ws, cudaStrea
     p.srow = L.srow;
     p.ptiles = L.ptiles;
     p.stiles = L.stiles;
-    p.ctas = L.ctas;
-    p.cost = L.cost;
     BeamMaps maps{};
     auto prefix = [&](const void *base, uint32_t positions, CUtensorMap &m) {
         return cache_map(base, sizeof(T), k.hd, k.pcap, k.n_kv, k.n_group, k.p_pos, k.p_head, k.p_group, positions, m);
@@ -283,7 +295,7 @@ bool run_attn(const BeamAttnArgs &k, const AttnLayout &L, uint8_t *ws, cudaStrea
     auto by = [](uint64_t d) { return d == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + d - 1) / d); };
     p.by_gq = by(k.gq);
     p.by_query = by(k.n_query);
-    return k.hd <= 64 ? pick_attn<T, 64>(k, p, maps, L.tc, st) : pick_attn<T, 128>(k, p, maps, L.tc, st);
+    return k.hd <= 64 ? run_parts<T, 64>(k, p, maps, L, st) : run_parts<T, 128>(k, p, maps, L, st);
 }
 
 // --- selection ------------------------------------------------------------------
@@ -357,7 +369,7 @@ bool run_select(const BeamSelectArgs &k, cudaStream_t st) {
     const uint64_t batches = ((uint64_t)k.n_beam * k.n_part * (k.cap / 32) + 63) / 64;
     uint32_t cluster = 1;
     while (cluster < kBsJoinCluster && 2 * cluster < batches) cluster *= 2;
-    return launched(launch_after(beam_select_join_kernel, dim3(k.n_group * cluster), kBsJoinThreads, cluster, st, k),
+    return launched(launch_after(beam_select_join_kernel, dim3(k.n_group * cluster), kBsJoinThreads, 0, cluster, st, k),
                     "fwb_beam_select launch");
 }
 

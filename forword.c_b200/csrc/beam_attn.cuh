@@ -78,6 +78,7 @@ struct BeamAttnPlan {
     uint32_t prow, srow;   // rows of a prefix / suffix tile
     uint32_t ptiles, stiles;  // row tiles of a group / of a sequence
     uint32_t ctas;
+    uint32_t part0, parts;  // the parts that a kernel takes: part0 .. parts - 1
     uint32_t cost;         // units that an item's own work is worth
     uint32_t by_gq, by_query;  // 2^32 / d rounded up, of row numbers below 2^16 (0: d = 1)
     uint32_t tma;          // bit 0: tensor maps of the prefix, 1: of the suffix
@@ -105,9 +106,9 @@ __device__ __forceinline__ uint32_t beam_part_units(const BeamAttnArgs &a, const
 // The cursor of this CTA's first unit; false when it has none.  Every warp
 // scans the parts' lengths for itself, so no barrier is waited for.
 __device__ __forceinline__ bool beam_first(const BeamAttnArgs &a, const BeamAttnPlan &p, BeamCursor &c) {
-    const uint32_t lane = threadIdx.x & 31, parts = a.n_group + a.n_group * a.n_beam;
-    uint32_t mine = lane < parts ? beam_part_units(a, p, lane) : 0, total = mine;  // of the first 32 parts
-    for (uint32_t i = lane + 32; i < parts; i += 32) total += beam_part_units(a, p, i);
+    const uint32_t lane = threadIdx.x & 31, first = p.part0 + lane;
+    uint32_t mine = first < p.parts ? beam_part_units(a, p, first) : 0, total = mine;  // of the first 32 parts
+    for (uint32_t i = first + 32; i < p.parts; i += 32) total += beam_part_units(a, p, i);
     total = __reduce_add_sync(0xffffffffu, total);
     // with fewer units than CTAs the first ones take one each, so that the
     // CTAs of an item are neighbours
@@ -116,8 +117,8 @@ __device__ __forceinline__ bool beam_first(const BeamAttnArgs &a, const BeamAttn
     const uint32_t per = total / ctas, more = total - per * ctas;  // the first `more` CTAs take one more
     uint32_t off = blockIdx.x * per + min(blockIdx.x, more);
     c.left = per + (blockIdx.x < more);
-    for (uint32_t i0 = 0;; i0 += 32) {
-        if (i0) mine = i0 + lane < parts ? beam_part_units(a, p, i0 + lane) : 0;
+    for (uint32_t i0 = p.part0;; i0 += 32) {
+        if (i0 != p.part0) mine = i0 + lane < p.parts ? beam_part_units(a, p, i0 + lane) : 0;
         uint32_t upto = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -132,7 +133,7 @@ __device__ __forceinline__ bool beam_first(const BeamAttnArgs &a, const BeamAttn
             break;
         }
         off -= __shfl_sync(0xffffffffu, upto, 31);
-        if (i0 + 32 >= parts) return false;  // lengths that changed under the call
+        if (i0 + 32 >= p.parts) return false;  // lengths that changed under the call
     }
     c.len = beam_part_len(a, c.part);
     const uint32_t units = beam_units(c.len) + p.cost, tiles = c.part < a.n_group ? p.ptiles : p.stiles;
@@ -155,7 +156,7 @@ __device__ __forceinline__ void beam_next_item(const BeamAttnArgs &a, const Beam
     if (++c.kvh < a.n_kv) return;
     c.kvh = 0;
     do {
-        if (++c.part >= a.n_group + a.n_group * a.n_beam) {  // lengths that changed under the call
+        if (++c.part >= p.parts) {  // lengths that changed under the call
             c.left = 0;
             return;
         }
@@ -827,8 +828,8 @@ __global__ void __launch_bounds__(kBaThreads) beam_attn_join_kernel(BeamAttnArgs
     if (some_p) pc = p.pcta[pi];
     if (some_s) sc = p.scta[si];
     // (after a wait that ran out these may be anything)
-    if (pc.y >= p.ctas || pc.x > pc.y + 1) pc = make_uint2(1, 0);
-    if (sc.y >= p.ctas || sc.x > sc.y + 1) sc = make_uint2(1, 0);
+    if (pc.y >= p.ctas || pc.x > pc.y) pc = make_uint2(1, 0);
+    if (sc.y >= p.ctas || sc.x > sc.y) sc = make_uint2(1, 0);
     const uint32_t np = pc.y + 1 - pc.x, n = np + (sc.y + 1 - sc.x);
     // the rows' first slots: of a prefix segment j, and of a suffix segment
     const size_t prow = (size_t)(pi + pc.x) * p.prow + (pr - ptile * p.prow);

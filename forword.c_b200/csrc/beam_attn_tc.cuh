@@ -1,12 +1,13 @@
-// beam_attn_tc.cuh — the shared-prefix attention of beam_attn.cuh on the
-// 5th-generation tensor cores, for fp16 and bf16.
+// beam_attn_tc.cuh — the prefix part of the shared-prefix attention
+// (beam_attn.cuh) on the 5th-generation tensor cores, for fp16 and bf16 and
+// many rows.  The suffixes, short and with few rows each, stay with
+// beam_attn.cuh's kernel, launched before this one and running beside it.
 //
-// The products are transposed so that few query rows still fill the machine:
-// a tile's 128 positions are the M dimension of S^T = K Q^T (N: the query
-// rows, 16, 32 or 128), and the head's dimensions that of O^T += V^T P.  A thread
-// of the softmax owns one position and half of the rows, so every thread has
-// the same work whatever the number of rows is, and the sums over positions
-// are kept per thread and joined once per item.
+// The products are transposed: a tile's 128 positions are the M dimension of
+// S^T = K Q^T (N: 128 query rows), and the head's dimensions that of
+// O^T += V^T P.  A thread of the softmax owns one position and half of the
+// rows, so the sums over positions are kept per thread and joined once per
+// item.
 //
 // The running maximum of a row is a reference that need not be exact: it is
 // raised, and O^T rescaled in tensor memory, only when a score exceeds it by
@@ -16,7 +17,10 @@
 //
 // One CTA per SM: a warp that loads (copy engine), one thread that issues the
 // products, and two groups of four warps for the softmax, each with half of
-// the rows.  The products of tile i + 1 run while tile i's softmax does.
+// the rows.  The scores of tile i + 1 are formed while tile i's softmax runs.
+// K and V have rings of their own: a K tile is done with as soon as its
+// scores are formed, so the next but one is on its way a whole softmax earlier
+// than V's.
 #pragma once
 #include "beam_attn.cuh"
 
@@ -26,29 +30,28 @@ constexpr int kBtKeys = 128;
 constexpr int kBtSoft = 256;                 // threads of the softmax
 constexpr int kBtThreads = 64 + kBtSoft;
 constexpr float kBtRaise = 8.f;              // log2
+constexpr int kBtRows = 128;                 // query rows of a tile
 
-// Shared memory: stages of K and V tiles, query rows, probabilities, then the
-// small things.
-template <int HD, int RT>
+// Shared memory: two stages of K and two of V, query rows, two buffers of
+// probabilities, then the small things.
+template <int HD>
 struct BeamTc {
     static constexpr int kSub = HD / 64;                           // sub-tiles of 128 bytes
     static constexpr uint32_t kSubBytes = kBtKeys * 128;           // of K, V
     static constexpr uint32_t kTile = kSub * kSubBytes;
-    static constexpr int kStages = 2, kPBufs = 2;
-    static constexpr uint32_t kQ = RT * HD * 2, kP = 2 * kSubBytes;
-    static constexpr uint32_t kOffQ = 2 * kTile * kStages, kOffP = kOffQ + kQ, kOffTail = kOffP + kPBufs * kP;
-    static constexpr uint32_t kTmem = 512;                         // a power of two, at least 3 RT columns
+    static constexpr uint32_t kQ = kBtRows * HD * 2, kP = 2 * kSubBytes;
+    static constexpr uint32_t kOffV = 2 * kTile, kOffQ = 4 * kTile, kOffP = kOffQ + kQ, kOffTail = kOffP + 2 * kP;
+    static constexpr uint32_t kTmem = 512;                         // a power of two, at least 3 x 128 columns
 };
 struct BeamTcTail {
-    uint64_t kfull[2], vfull[2], empty[2], sfull[2], sfree[2], pfull[2], odone[2], ofree, qfull;
+    uint64_t kfull[2], vfull[2], kempty[2], vempty[2], sfull[2], sfree[2], pfull[2], odone[2], ofree, qfull;
     uint32_t tmem;
     alignas(16) float nm[128];  // minus the rows' references; +inf: none yet
     float alpha[128];
-    uint32_t lim[128];          // positions that a row sees
     uint32_t top[128];          // the tile's maxima, as ordered integers; 0 between uses
 };
-template <int HD, int RT>
-constexpr uint32_t beam_tc_smem() { return BeamTc<HD, RT>::kOffTail + sizeof(BeamTcTail); }
+template <int HD>
+constexpr uint32_t beam_tc_smem() { return BeamTc<HD>::kOffTail + sizeof(BeamTcTail); }
 
 __device__ __forceinline__ void bt_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void bt_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -154,54 +157,34 @@ __device__ __forceinline__ uint32_t bt_join(float *v, Op op) {
     return first;
 }
 
-// A tile's K or V: n positions of a part, as beam_load does.
+// n positions of a prefix, K or V, into a stage: by the copy engine, or where
+// the strides do not allow its maps by 16-byte asynchronous copies.  The
+// barrier takes 32 arrivals.
 template <typename T, int HD>
-__device__ __forceinline__ void bt_copy(const BeamAttnArgs &a, const BeamCursor &c, uint32_t n, bool pre,
-                                        const uint32_t *seq, uint32_t single, uint32_t dst, const void *base,
-                                        const CUtensorMap *map, const CUtensorMap *wide, uint64_t *bar) {
+__device__ __forceinline__ void bt_copy(const BeamAttnArgs &a, const BeamCursor &c, uint32_t n, bool tma, uint32_t dst,
+                                        const void *base, const CUtensorMap *map, const CUtensorMap *wide, uint64_t *bar) {
     constexpr int kSub = HD / 64, CH = HD / 8, RP = 32 / CH;
     const uint32_t lane = threadIdx.x & 31, units = (n + kBaUnit - 1) / kBaUnit;
-    if (pre && single && units == kBtKeys / kBaUnit) {  // a whole tile: one box per sub-tile
+    if (tma) {
+        const bool whole = units == kBtKeys / kBaUnit;  // one box per sub-tile, else one per unit and sub-tile
         if (lane == 0)
             asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)),
-                         "r"(kSub * kBtKeys * 128) : "memory");
+                         "r"(units * kSub * kBaUnit * 128) : "memory");
         __syncwarp();
-        if (lane < kSub)
-            tma_load_4d(dst + lane * (kBtKeys * 128), wide, (int32_t)(lane * 64), (int32_t)c.pos, (int32_t)c.kvh,
-                        (int32_t)c.part, bar);
+        const uint32_t u = lane / kSub, h = lane % kSub;
+        if (u < (whole ? 1 : units))
+            tma_load_4d(dst + h * (kBtKeys * 128) + u * kBaUnit * 128, whole ? wide : map, (int32_t)(h * 64),
+                        (int32_t)(c.pos + u * kBaUnit), (int32_t)c.kvh, (int32_t)c.part, bar);
         mbar_arrive(bar);
         return;
     }
-    single &= (1u << units) - 1;
-    if (lane == 0 && single)
-        asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)),
-                     "r"(__popc(single) * kSub * kBaUnit * 128) : "memory");
-    const uint32_t u = lane / kSub, h = lane % kSub;  // one box per lane
-    uint32_t from = 0;
-#pragma unroll
-    for (int i = 0; i < kBtKeys / 32; ++i) {
-        const uint32_t v = __shfl_sync(0xffffffffu, seq[i], (u & 1) * kBaUnit);
-        if ((u >> 1) == i) from = v;
-    }
-    __syncwarp();
-    if (u < units && single >> u & 1)
-        tma_load_4d(dst + h * (kBtKeys * 128) + u * kBaUnit * 128, map, (int32_t)(h * 64), (int32_t)(c.pos + u * kBaUnit),
-                    (int32_t)c.kvh, (int32_t)from, bar);
-    if (single != (1u << units) - 1) {
-        const uint32_t ch = lane % CH;
-        const bool held = ch * 8 < a.hd;
-        const size_t outer = pre ? a.p_group : a.s_seq, step = pre ? a.p_pos : a.s_pos;
-        const T *b = static_cast<const T *>(base) + (pre ? c.kvh * a.p_head : c.kvh * a.s_head) + (held ? ch * 8 : 0);
-#pragma unroll
-        for (int i = 0; i < kBtKeys / 32; ++i)
-            for (uint32_t r = 0; r < 32; r += RP) {
-                const uint32_t row = 32 * i + r + lane / CH;
-                const uint32_t s = __shfl_sync(0xffffffffu, seq[i], row & 31);
-                if (row < n && !(single >> (row / kBaUnit) & 1))
-                    cp_async16_or_zero(dst + (ch >> 3) * (kBtKeys * 128) + row * 128 + (((ch ^ row) & 7) << 4),
-                                       b + s * outer + (size_t)(c.pos + row) * step, held);
-            }
-    }
+    const uint32_t ch = lane % CH;
+    const bool held = ch * 8 < a.hd;
+    const T *b = static_cast<const T *>(base) + c.part * a.p_group + c.kvh * a.p_head + (held ? ch * 8 : 0);
+#pragma unroll 4
+    for (uint32_t row = lane / CH; row < n; row += RP)
+        cp_async16_or_zero(dst + (ch >> 3) * (kBtKeys * 128) + row * 128 + (((ch ^ row) & 7) << 4),
+                           b + (size_t)(c.pos + row) * a.p_pos, held);
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
@@ -209,40 +192,36 @@ __device__ __forceinline__ uint32_t bt_take(const BeamCursor &c) {
     return min(min((uint32_t)kBtKeys, c.len - c.pos), min(c.left, kBtKeys / kBaUnit) * kBaUnit);
 }
 
-// The CTA's tile i by the softmax threads.  RT: rows of the item's tiles.
-template <typename T, int HD, int RTP, int RT>
+// The CTA's tile i by the softmax threads.
+template <typename T, int HD>
 __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPlan &p, BeamCursor &c, bool &fresh,
                                         float *l, uint32_t i, uint8_t *sm, BeamTcTail &t, uint32_t tmem,
                                         bool &ok) {
-    using Sm = BeamTc<HD, RTP>;
-    constexpr int NC = RT / 2, S = Sm::kStages, PB = Sm::kPBufs;
+    using Sm = BeamTc<HD>;
+    constexpr int RT = kBtRows, NC = RT / 2;
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, quad = warp & 3, wg = (warp - 2) >> 2;
     const uint32_t tid = threadIdx.x - 64, wt = tid & 127, col0 = wg * NC, bar = 2 + wg;
     const uint32_t key = quad * 32 + lane, lanes = (quad * 32) << 16;
-    const bool pre = c.part < a.n_group;
-    const uint32_t rows = (pre ? a.n_beam : 1) * a.n_query * a.gq;
+    const uint32_t rows = a.n_beam * a.n_query * a.gq;
     const float sl2 = a.scale * 1.4426950408889634f;
-    const bool limits = !pre && a.n_query > 1;
     if (fresh) {
         // query rows, K-major with the 128-byte swizzle; rows past the item's are zeros
-        constexpr int CH = HD / 8, RPP = kBtSoft / CH, NR = (RT + RPP - 1) / RPP;  // rows of a pass; passes
+        constexpr int CH = HD / 8, RPP = kBtSoft / CH, NR = RT / RPP;  // rows of a pass; passes
         const uint32_t qs = smem_u32(sm + Sm::kOffQ), ch = tid % CH, r0 = tid / CH;
         uint4 v[NR];
 #pragma unroll
         for (int j = 0; j < NR; ++j) {
             const uint32_t r = r0 + j * RPP;
-            int32_t lim = -1;
-            const T *q = r < RT ? beam_q_row<T, HD>(a, p, c, c.tile * RT + r, lim) : nullptr;
-            v[j] = make_uint4(0, 0, 0, 0);
+            int32_t lim;
+            const T *q = beam_q_row<T, HD>(a, p, c, c.tile * RT + r, lim);
+            v[j] = make_uint4(0, 0, 0, 0);  // (rows past the item's: zeros, and not written at the end)
             if (q && ch * 8 < a.hd) v[j] = *reinterpret_cast<const uint4 *>(q + ch * 8);
-            if (ch == 0 && r < RT) t.lim[r] = (uint32_t)lim;  // (-1: no such row, sees all and is not written)
         }
 #pragma unroll
         for (int j = 0; j < NR; ++j) {
             const uint32_t r = r0 + j * RPP;
-            if (r < RT)
-                asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(qs + (ch >> 3) * (RT * 128) + r * 128 + (((ch ^ r) & 7) << 4)),
-                             "r"(v[j].x), "r"(v[j].y), "r"(v[j].z), "r"(v[j].w) : "memory");
+            asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(qs + (ch >> 3) * (RT * 128) + r * 128 + (((ch ^ r) & 7) << 4)),
+                         "r"(v[j].x), "r"(v[j].y), "r"(v[j].z), "r"(v[j].w) : "memory");
         }
         if (wt < NC) t.nm[col0 + wt] = INFINITY;
 #pragma unroll
@@ -252,32 +231,23 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
         if (tid == 0) mbar_arrive(&t.qfull);
     }
     const bool first = fresh, start = c.pos == 0;
-    const uint32_t n = bt_take(c), sb = i & 1, pb = i % PB, st = i % S;
-    ok = mbar_wait(&t.sfull[sb], i >> 1 & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
+    const uint32_t n = bt_take(c), b = i & 1, ph = i >> 1 & 1;
+    ok = mbar_wait(&t.sfull[b], ph, &g_beam_err, ERR_WAIT_FULL) && ok;
     __syncwarp();
     bt_fence_after();
     float y[NC];
-    const uint32_t ts = tmem + sb * RTP + lanes + col0;
+    const uint32_t ts = tmem + b * RT + lanes + col0;
     const bool live = key < n;
     auto load = [&] {  // the scores
-        if constexpr (NC >= 32) {
 #pragma unroll
-            for (int j = 0; j < NC; j += 32) bt_ld32(ts + j, y + j);
-        } else {
-#pragma unroll
-            for (int j = 0; j < NC; j += 8) bt_ld8(ts + j, y + j);
-        }
+        for (int j = 0; j < NC; j += 32) bt_ld32(ts + j, y + j);
         bt_ld_wait();
         bt_here<NC>(y);
     };
-    auto hide = [&] {  // positions past the end, or that a row does not see
+    auto hide = [&] {  // positions past the end
         if (n < kBtKeys && !live)
 #pragma unroll
             for (int j = 0; j < NC; ++j) y[j] = -INFINITY;
-        if (limits)
-#pragma unroll
-            for (int j = 0; j < NC; ++j)
-                if (c.pos + key >= t.lim[col0 + j]) y[j] = -INFINITY;
     };
     auto refer = [&] {  // against the rows' references
 #pragma unroll
@@ -302,7 +272,7 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
         hide();
         const uint32_t at = bt_join<NC>(y, [](float u, float v) { return fmaxf(u, v); });
 #pragma unroll
-        for (int j = 0; j < (NC > 32 ? NC / 32 : 1); ++j) {
+        for (int j = 0; j < NC / 32; ++j) {
             const uint32_t u = __float_as_uint(y[j] * sl2);
             atomicMax(&t.top[col0 + at + j], u & 0x80000000u ? ~u : u | 0x80000000u);
         }
@@ -323,7 +293,7 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
             ok = mbar_wait(&t.odone[(i - 1) & 1], (i - 1) >> 1 & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
             __syncwarp();
             bt_fence_after();
-            const uint32_t to = tmem + 2 * RTP + lanes + col0;
+            const uint32_t to = tmem + 2 * RT + lanes + col0;
 #pragma unroll 1
             for (uint32_t j = 0; j < NC; j += 8) {
                 float o[8];
@@ -339,11 +309,11 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
     }
     bt_fence_before();
     __syncwarp();
-    if (lane == 0) mbar_arrive(&t.sfree[sb]);
+    if (lane == 0) mbar_arrive(&t.sfree[b]);
     // the buffer's last reader; in order for every tile, so that the phases of
     // these barriers are never two ahead of what was seen
-    if (i >= PB) ok = mbar_wait(&t.odone[(i - PB) & 1], (i - PB) >> 1 & 1, &g_beam_err, ERR_WAIT_EMPTY) && ok;
-    const uint32_t ps = smem_u32(sm + Sm::kOffP + pb * Sm::kP) + key * 128;
+    if (i >= 2) ok = mbar_wait(&t.odone[b], ph ^ 1, &g_beam_err, ERR_WAIT_EMPTY) && ok;
+    const uint32_t ps = smem_u32(sm + Sm::kOffP + b * Sm::kP) + key * 128;
 #pragma unroll
     for (int j = 0; j < NC; j += 8) {
         uint32_t w[4];
@@ -360,8 +330,8 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
     if (n & (kBaUnit - 1)) {
         // V rows of the last unit past the end: their probabilities are zero,
         // and zero times whatever the memory holds must be zero
-        ok = mbar_wait(&t.vfull[st], i / S & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
-        const uint32_t vs = smem_u32(sm + (2 * st + 1) * Sm::kTile);
+        ok = mbar_wait(&t.vfull[b], ph, &g_beam_err, ERR_WAIT_FULL) && ok;
+        const uint32_t vs = smem_u32(sm + Sm::kOffV + b * Sm::kTile);
         const uint32_t end = (n + kBaUnit - 1) / kBaUnit * kBaUnit;
         for (uint32_t j = tid; j < (end - n) * (HD / 8); j += kBtSoft) {
             const uint32_t row = n + j / (HD / 8), ch = j % (HD / 8);
@@ -372,28 +342,26 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
     bt_fence_proxy();
     bt_fence_before();
     __syncwarp();
-    if (lane == 0) mbar_arrive(&t.pfull[pb]);
+    if (lane == 0) mbar_arrive(&t.pfull[b]);
     beam_advance(c, n);
     fresh = c.pos >= c.len || c.left == 0;
-    const uint32_t item = ((pre ? c.part : c.part - a.n_group) * a.n_kv + c.kvh) * (pre ? p.ptiles : p.stiles) + c.tile;
+    const uint32_t item = (c.part * a.n_kv + c.kvh) * p.ptiles + c.tile;
     if (fresh) {
-        ok = mbar_wait(&t.odone[i & 1], i >> 1 & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
+        ok = mbar_wait(&t.odone[b], ph, &g_beam_err, ERR_WAIT_FULL) && ok;
         __syncwarp();
         bt_fence_after();
         const size_t row0 = (size_t)(item + blockIdx.x) * RT;
-        float *o = (pre ? p.po : p.so) + row0 * HD + key;
-        const uint32_t to = tmem + 2 * RTP + lanes + col0, held = rows - min(rows, c.tile * RT);
-        constexpr int NV = NC < 32 ? 8 : 32;
+        float *o = p.po + row0 * HD + key;
+        const uint32_t to = tmem + 2 * RT + lanes + col0, held = rows - min(rows, c.tile * RT);
 #pragma unroll 1
-        for (uint32_t j = 0; j < NC; j += NV) {
-            float v[NV];
-            if constexpr (NV == 32) bt_ld32(to + j, v);
-            else bt_ld8(to + j, v);
+        for (uint32_t j = 0; j < NC; j += 32) {
+            float v[32];
+            bt_ld32(to + j, v);
             bt_ld_wait();
-            bt_here<NV>(v);
+            bt_here<32>(v);
             if (key < HD)
 #pragma unroll
-                for (int e = 0; e < NV; ++e)
+                for (int e = 0; e < 32; ++e)
                     if (col0 + j + e < held) o[(size_t)(col0 + j + e) * HD] = v[e];
         }
         bt_fence_before();
@@ -403,44 +371,44 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
         float *sum = reinterpret_cast<float *>(sm + Sm::kOffP);
         const uint32_t at = bt_join<NC>(l, [](float u, float v) { return u + v; });
 #pragma unroll
-        for (int j = 0; j < (NC > 32 ? NC / 32 : 1); ++j) sum[quad * RT + col0 + at + j] = l[j];
+        for (int j = 0; j < NC / 32; ++j) sum[quad * RT + col0 + at + j] = l[j];
         bar_sync(bar, 128);
         if (wt < NC && col0 + wt < held) {
             const uint32_t r = col0 + wt;
-            (pre ? p.pml : p.sml)[row0 + r] =
+            p.pml[row0 + r] =
                 make_float2(-t.nm[r], (sum[r] + sum[RT + r]) + (sum[2 * RT + r] + sum[3 * RT + r]));
         }
         bar_sync(1, kBtSoft);  // before the next item's rows come into the same places
     }
     if (tid == 0 && (start || c.pos >= c.len)) {
-        uint2 *cta = (pre ? p.pcta : p.scta) + item;
+        uint2 *cta = p.pcta + item;
         if (start) cta->x = blockIdx.x;
         if (c.pos >= c.len) cta->y = blockIdx.x;
     }
     if (fresh && c.left) beam_next_item(a, p, c);
 }
 
-// RTP, RTS: rows of a prefix / suffix tile.
-template <typename T, int HD, int RTP, int RTS>
+template <typename T, int HD>
 __global__ void __launch_bounds__(kBtThreads, 1)
     beam_attn_tc_kernel(const BeamAttnArgs a, const BeamAttnPlan p, const __grid_constant__ BeamMaps maps) {
-    using Sm = BeamTc<HD, RTP>;
-    constexpr int S = Sm::kStages, PB = Sm::kPBufs;
+    using Sm = BeamTc<HD>;
+    constexpr int RT = kBtRows;
     extern __shared__ __align__(1024) uint8_t bt_sm[];
     BeamTcTail &t = *reinterpret_cast<BeamTcTail *>(bt_sm + Sm::kOffTail);
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_launch();
     BeamCursor c;
-    const bool any = beam_first(a, p, c);
-    if (!any) return;  // the same in every thread
+    if (!beam_first(a, p, c)) {  // the same in every thread
+        pdl_wait();
+        return;
+    }
     if (threadIdx.x < 128) t.top[threadIdx.x] = 0;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < S; ++i) {
+        for (int i = 0; i < 2; ++i) {
             mbar_init(&t.kfull[i], 32);
             mbar_init(&t.vfull[i], 32);
-            mbar_init(&t.empty[i], 1);
-        }
-        for (int i = 0; i < 2; ++i) {
+            mbar_init(&t.kempty[i], 1);
+            mbar_init(&t.vempty[i], 1);
             mbar_init(&t.sfull[i], 1);
             mbar_init(&t.sfree[i], kBtSoft / 32);
             mbar_init(&t.pfull[i], kBtSoft / 32);
@@ -459,106 +427,89 @@ __global__ void __launch_bounds__(kBtThreads, 1)
     bt_fence_after();
     const uint32_t tmem = t.tmem;
     if (warp == 0) {
-        uint32_t i = 0;
-        for (; c.left; ++i) {
-            const uint32_t s = i % S;
-            if (i >= S && !mbar_wait(&t.empty[s], (i / S - 1) & 1, &g_beam_err, ERR_WAIT_EMPTY)) break;
+        // K of tile i + 1 before V of tile i
+        BeamCursor v = c;
+        uint32_t nk = 0, nv = 0;
+        const bool tma = p.tma & 1;
+        bool ok = true;
+        auto next = [&](BeamCursor &at, uint32_t &count, const void *base, uint32_t off, const CUtensorMap *map,
+                        const CUtensorMap *wide, uint64_t *full, uint64_t *empty) {
+            const uint32_t s = count & 1;
+            if (count >= 2) ok = mbar_wait(&empty[s], (count >> 1 & 1) ^ 1, &g_beam_err, ERR_WAIT_EMPTY);
             __syncwarp();
-            const uint32_t n = bt_take(c);
-            const bool pre = c.part < a.n_group;
-            const uint32_t sq = c.part - a.n_group;
-            // the cache row's sequence, or group, of rows lane, lane + 32, ...
-            uint32_t seq[kBtKeys / 32], single = p.tma >> (pre ? 0 : 1) & 1 ? 0xffu : 0u;
-#pragma unroll
-            for (int j = 0; j < kBtKeys / 32; ++j) seq[j] = pre ? c.part : sq;
-            if (!pre && a.slots) {
-                const uint32_t b0 = sq / a.n_beam * a.n_beam;
-                const int32_t *slots = a.slots + sq * a.slot_seq + c.pos;
-#pragma unroll
-                for (int j = 0; j < kBtKeys / 32; ++j)
-                    if (lane + 32 * j < n) {
-                        const uint32_t from = (uint32_t)slots[lane + 32 * j];
-                        if (from < a.n_beam) seq[j] = b0 + from;
-                    }
-#pragma unroll
-                for (int j = 0; j < kBtKeys / 32; ++j) {  // units whose rows differ
-                    const uint32_t lead = __shfl_sync(0xffffffffu, seq[j], lane & 16);
-                    const uint32_t off = __ballot_sync(0xffffffffu, seq[j] != lead && lane + 32 * j < n);
-                    if (off & 0xffffu) single &= ~(1u << 2 * j);
-                    if (off >> 16) single &= ~(2u << 2 * j);
-                }
-            }
-            const uint32_t ks = smem_u32(bt_sm + 2 * s * Sm::kTile);
-            bt_copy<T, HD>(a, c, n, pre, seq, single, ks, pre ? a.pk : a.sk, pre ? &maps.pk : &maps.sk, &maps.wk, &t.kfull[s]);
-            bt_copy<T, HD>(a, c, n, pre, seq, single, ks + Sm::kTile, pre ? a.pv : a.sv, pre ? &maps.pv : &maps.sv, &maps.wv,
-                           &t.vfull[s]);
-            beam_advance(c, n);
-            if (c.left && c.pos >= c.len) beam_next_item(a, p, c);
+            if (!ok) return;
+            const uint32_t n = bt_take(at);
+            bt_copy<T, HD>(a, at, n, tma, smem_u32(bt_sm + off + s * Sm::kTile), base, map, wide, &full[s]);
+            ++count;
+            beam_advance(at, n);
+            if (at.left && at.pos >= at.len) beam_next_item(a, p, at);
+        };
+        while (ok && v.left) {
+            while (ok && c.left && nk <= nv + 1) next(c, nk, a.pk, 0, &maps.pk, &maps.wk, t.kfull, t.kempty);
+            if (ok) next(v, nv, a.pv, Sm::kOffV, &maps.pv, &maps.wv, t.vfull, t.vempty);
         }
         // no copy is in flight when this CTA's shared memory is given back
-        for (uint32_t j = 0; j < min(i, (uint32_t)S); ++j) {
-            const uint32_t w = i - 1 - j;
-            mbar_wait(&t.kfull[w % S], w / S & 1, &g_beam_err, ERR_WAIT_DRAIN);
-            mbar_wait(&t.vfull[w % S], w / S & 1, &g_beam_err, ERR_WAIT_DRAIN);
-        }
+        for (uint32_t j = 0; j < min(nk, 2u); ++j)
+            mbar_wait(&t.kfull[(nk - 1 - j) & 1], (nk - 1 - j) >> 1 & 1, &g_beam_err, ERR_WAIT_DRAIN);
+        for (uint32_t j = 0; j < min(nv, 2u); ++j)
+            mbar_wait(&t.vfull[(nv - 1 - j) & 1], (nv - 1 - j) >> 1 & 1, &g_beam_err, ERR_WAIT_DRAIN);
     } else if (warp == 1) {
         if (lane == 0) {
             const uint32_t q = smem_u32(bt_sm + Sm::kOffQ);
+            const uint32_t ids = bt_idesc<T>(RT, false), ido = bt_idesc<T>(RT, true);
             uint32_t seg = 0;
             bool ok = true;
             // S^T = K Q^T of tile i
-            auto scores = [&](uint32_t i, uint32_t rt) {
-                const uint32_t s = i % S, b = i & 1;
+            auto scores = [&](uint32_t i) {
+                const uint32_t b = i & 1, k = smem_u32(bt_sm + b * Sm::kTile);
                 bt_fence_after();
                 bt_fence_proxy();
-                const uint32_t k = smem_u32(bt_sm + 2 * s * Sm::kTile), id = bt_idesc<T>(rt, false);
                 if (ok)
 #pragma unroll
                     for (int d = 0; d < HD / 16; ++d)
-                        bt_mma(tmem + b * RTP, bt_desc(k + (d / 4) * Sm::kSubBytes + (d % 4) * 32, 16),
-                               bt_desc(q + (d / 4) * (rt * 128) + (d % 4) * 32, 16), id, d != 0);
+                        bt_mma(tmem + b * RT, bt_desc(k + (d / 4) * Sm::kSubBytes + (d % 4) * 32, 16),
+                               bt_desc(q + (d / 4) * (RT * 128) + (d % 4) * 32, 16), ids, d != 0);
                 bt_commit(&t.sfull[b]);
+                bt_commit(&t.kempty[b]);
             };
             auto scores_ready = [&](uint32_t i) {  // its K is there and its place in tensor memory is free
-                return mbar_try_wait(&t.kfull[i % S], i / S & 1) && (i < 2 || mbar_try_wait(&t.sfree[i & 1], (i / 2 - 1) & 1));
+                return mbar_try_wait(&t.kfull[i & 1], i >> 1 & 1) && (i < 2 || mbar_try_wait(&t.sfree[i & 1], (i >> 1 & 1) ^ 1));
             };
             auto scores_wait = [&](uint32_t i) {
-                ok = mbar_wait(&t.kfull[i % S], i / S & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
-                if (i >= 2) ok = mbar_wait(&t.sfree[i & 1], (i / 2 - 1) & 1, &g_beam_err, ERR_WAIT_EMPTY) && ok;
+                ok = mbar_wait(&t.kfull[i & 1], i >> 1 & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
+                if (i >= 2) ok = mbar_wait(&t.sfree[i & 1], (i >> 1 & 1) ^ 1, &g_beam_err, ERR_WAIT_EMPTY) && ok;
             };
             bool first = true;
             ok = mbar_wait(&t.qfull, 0, &g_beam_err, ERR_WAIT_FULL);
             scores_wait(0);
-            scores(0, c.part < a.n_group ? RTP : RTS);
+            scores(0);
             for (uint32_t i = 0; c.left; ++i) {
-                const uint32_t n = bt_take(c), rt = c.part < a.n_group ? RTP : RTS;
+                const uint32_t n = bt_take(c), b = i & 1, ph = i >> 1 & 1;
                 beam_advance(c, n);
                 const bool turn = c.pos >= c.len;             // the item ends here
                 bool ahead = c.left != 0 && !turn;            // the next tile's scores come first, if its K is there
-                const uint32_t s = i % S, pb = i % PB;
                 if (first && seg) ok = mbar_wait(&t.ofree, (seg - 1) & 1, &g_beam_err, ERR_WAIT_EMPTY) && ok;
                 if (ahead)
                     for (uint32_t polls = 0; polls < 4096; ++polls) {
                         if (scores_ready(i + 1)) {
-                            scores(i + 1, rt);
+                            scores(i + 1);
                             ahead = false;
                             break;
                         }
-                        if (mbar_try_wait(&t.pfull[pb], i / PB & 1)) break;
+                        if (mbar_try_wait(&t.pfull[b], ph)) break;
                     }
                 // O^T += V^T P
-                ok = mbar_wait(&t.vfull[s], i / S & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
-                ok = mbar_wait(&t.pfull[pb], i / PB & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
+                ok = mbar_wait(&t.vfull[b], ph, &g_beam_err, ERR_WAIT_FULL) && ok;
+                ok = mbar_wait(&t.pfull[b], ph, &g_beam_err, ERR_WAIT_FULL) && ok;
                 bt_fence_after();
                 bt_fence_proxy();
-                const uint32_t v = smem_u32(bt_sm + (2 * s + 1) * Sm::kTile), ps = smem_u32(bt_sm + Sm::kOffP + pb * Sm::kP);
-                const uint32_t id = bt_idesc<T>(rt, true), units = (n + kBaUnit - 1) / kBaUnit;
+                const uint32_t v = smem_u32(bt_sm + Sm::kOffV + b * Sm::kTile), ps = smem_u32(bt_sm + Sm::kOffP + b * Sm::kP);
                 if (ok)
-                    for (uint32_t u = 0; u < units; ++u)  // (a 64-wide head: its dimensions twice)
-                        bt_mma(tmem + 2 * RTP, bt_desc(v + u * 2048, HD == 64 ? 0 : Sm::kSubBytes),
-                               bt_desc(ps + u * 2048, Sm::kSubBytes), id, !first || u);
-                bt_commit(&t.empty[s]);
-                bt_commit(&t.odone[i & 1]);
+                    for (uint32_t u = 0; u < (n + kBaUnit - 1) / kBaUnit; ++u)  // (a 64-wide head: its dimensions twice)
+                        bt_mma(tmem + 2 * RT, bt_desc(v + u * 2048, HD == 64 ? 0 : Sm::kSubBytes),
+                               bt_desc(ps + u * 2048, Sm::kSubBytes), ido, !first || u);
+                bt_commit(&t.vempty[b]);
+                bt_commit(&t.odone[b]);
                 first = false;
                 if (turn && c.left) {
                     beam_next_item(a, p, c);
@@ -568,19 +519,16 @@ __global__ void __launch_bounds__(kBtThreads, 1)
                 }
                 if (ahead && c.left) {
                     scores_wait(i + 1);
-                    scores(i + 1, c.part < a.n_group ? RTP : RTS);
+                    scores(i + 1);
                 }
             }
         }
         __syncwarp();
     } else {
-        float l[(RTP > RTS ? RTP : RTS) / 2];  // the sums of this thread's position, for half of the rows
+        float l[RT / 2];  // the sums of this thread's position, for half of the rows
         bool fresh = true, ok = true;
 #pragma unroll 1
-        for (uint32_t i = 0; c.left; ++i) {
-            if (RTP == RTS || c.part < a.n_group) bt_step<T, HD, RTP, RTP>(a, p, c, fresh, l, i, bt_sm, t, tmem, ok);
-            else bt_step<T, HD, RTP, RTS>(a, p, c, fresh, l, i, bt_sm, t, tmem, ok);
-        }
+        for (uint32_t i = 0; c.left; ++i) bt_step<T, HD>(a, p, c, fresh, l, i, bt_sm, t, tmem, ok);
     }
     // every product is complete: the softmax waited for the last one's commit
     // (or the wait ran out after its bound)
@@ -590,6 +538,7 @@ __global__ void __launch_bounds__(kBtThreads, 1)
         bt_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Sm::kTmem) : "memory");
     }
+    pdl_wait();  // the suffixes' kernel, so that what waits for this one has both
 }
 
 }  // namespace fwb
