@@ -139,14 +139,13 @@ bool attn_layout(const fwb_prefix_attn_t *a, AttnLayout &L) {
     const uint32_t hd = a->head_dim <= 64 ? 64 : 128;
     // More than 64 rows over a long prefix go to the 5th-generation tensor
     // cores.  Measured (fp16, 8 KV heads of 128, one group, us for warp-level
-    // products against tcgen05): 64 rows 49 / 47 over 30000 positions and
-    // 19 / 21 over 4000; 128 rows 77 / 57, 25 / 29; 256 rows 138 / 96, 38 / 43.
-    // A tile of 64 rows and 1000 positions costs the one what 128 rows cost the
-    // other, about 1 us, and the other begins and ends some 7 to 12 us later.
+    // products / tcgen05 over 500, 4000 and 30000 positions): 96 rows 15 / 21,
+    // 24 / 24, 75 / 50; 128 rows 15 / 23, 25 / 26, 77 / 51; 256 rows 21 / 26,
+    // 38 / 33, 138 / 77.  1000 positions cost the one 1 us per 64 rows and the
+    // other as much per 128, and the other, two kernels, begins 5 us later.
     const uint64_t spared = (prows + 63) / 64 - (prows + 127) / 128;
     L.tc = a->type != 0 &&
-           (uint64_t)a->n_group * a->n_head_kv * a->prefix_cap * spared >=
-               (32000 + 280 * std::min<uint64_t>(prows, 256)) * device_sms() / 148;
+           (uint64_t)a->n_group * a->n_head_kv * a->prefix_cap * spared >= (uint64_t)36000 * device_sms() / 148;
     auto tile = [&](uint64_t rows) { return rows <= 16 ? 16u : rows <= 32 ? 32u : 64u; };
     L.prow = L.tc ? kBtRows : tile(prows);
     L.srow = tile(srows);

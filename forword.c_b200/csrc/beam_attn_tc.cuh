@@ -53,6 +53,13 @@ struct BeamTcTail {
 template <int HD>
 constexpr uint32_t beam_tc_smem() { return BeamTc<HD>::kOffTail + sizeof(BeamTcTail); }
 
+// Whether a phase is over, without waiting at all.
+__device__ __forceinline__ bool bt_test(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ void bt_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void bt_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void bt_fence_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -473,7 +480,7 @@ __global__ void __launch_bounds__(kBtThreads, 1)
                 bt_commit(&t.kempty[b]);
             };
             auto scores_ready = [&](uint32_t i) {  // its K is there and its place in tensor memory is free
-                return mbar_try_wait(&t.kfull[i & 1], i >> 1 & 1) && (i < 2 || mbar_try_wait(&t.sfree[i & 1], (i >> 1 & 1) ^ 1));
+                return bt_test(&t.kfull[i & 1], i >> 1 & 1) && (i < 2 || bt_test(&t.sfree[i & 1], (i >> 1 & 1) ^ 1));
             };
             auto scores_wait = [&](uint32_t i) {
                 ok = mbar_wait(&t.kfull[i & 1], i >> 1 & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
@@ -496,7 +503,7 @@ __global__ void __launch_bounds__(kBtThreads, 1)
                             ahead = false;
                             break;
                         }
-                        if (mbar_try_wait(&t.pfull[b], ph)) break;
+                        if (bt_test(&t.pfull[b], ph)) break;
                     }
                 // O^T += V^T P
                 ok = mbar_wait(&t.vfull[b], ph, &g_beam_err, ERR_WAIT_FULL) && ok;
