@@ -262,8 +262,15 @@ bool run_parts(const BeamAttnArgs &k, BeamAttnPlan p, const BeamMaps &maps, cons
             if (!launch_attn_tc<T, HD>(k, p, maps, st)) return false;
             p.ctas = std::max(L.ctas, L.tctas);
         }
-    return launched(launch_after(beam_attn_join_kernel<T, HD>, dim3(seqs * k.n_query, k.n_head), kBaThreads, 0, 1, st, k, p),
-                    "fwb_prefix_attention launch");
+    const uint32_t rows = seqs * k.n_query * k.n_head, sms = device_sms();
+    auto join = [&](auto fn, uint32_t blocks, unsigned threads) {
+        return launched(launch_after(fn, dim3(blocks), threads, 0, 1, st, k, p), "fwb_prefix_attention launch");
+    };
+    // (measured, all of a call in us with 8 / 4 / 1 warps a row: 128 rows of 55
+    // segments 30.0 / 31.2 / -, 960 of 10 - / 39.8 / 42.1, 4096 of 6 - / 142.4 / 139.4)
+    if (rows <= 4 * sms) return join(beam_attn_join_kernel<T, HD, 8>, rows, kBjThreads<8>);
+    if (rows <= 16 * sms) return join(beam_attn_join_kernel<T, HD, 4>, rows, kBjThreads<4>);
+    return join(beam_attn_join_kernel<T, HD, 1>, (rows + 7) / 8, kBjThreads<1>);
 }
 
 template <typename T>

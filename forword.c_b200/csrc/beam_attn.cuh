@@ -808,17 +808,23 @@ __global__ void __launch_bounds__(kBaThreads + kBaLoader, sizeof(T) == 4 && RWP 
     }
 }
 
-// Joins a row's partial results: block (row, head), the warps take the
-// segments in turn, four at a time, lanes the dimensions.
-template <typename T, int HD>
-__global__ void __launch_bounds__(kBaThreads) beam_attn_join_kernel(BeamAttnArgs a, BeamAttnPlan p) {
-    constexpr int NW = kBaThreads / 32, V = HD / 32;
+// Joins a row's partial results.  WPR warps a row (token and head) take its
+// segments in turn, four at a time, lanes the dimensions; their results are
+// joined through shared memory.  More where the rows are few and so have many
+// segments each; a block has one row, or eight with one warp each.
+template <int WPR>
+constexpr int kBjThreads = WPR > 1 ? 32 * WPR : 256;
+template <typename T, int HD, int WPR>
+__global__ void __launch_bounds__(kBjThreads<WPR>) beam_attn_join_kernel(BeamAttnArgs a, BeamAttnPlan p) {
+    constexpr int V = HD / 32, RPB = kBjThreads<WPR> / 32 / WPR;  // rows of a block
     struct alignas(4 * V) Vec { float v[V]; };
-    __shared__ Vec part[NW][32];
-    __shared__ float pm[NW], pl[NW];
-    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const uint32_t h = blockIdx.y, kvh = h / a.gq, hg = h - kvh * a.gq;
-    const uint32_t s = blockIdx.x / a.n_query, t = blockIdx.x - s * a.n_query, grp = s / a.n_beam;
+    __shared__ Vec part[WPR > 1 ? WPR : 1][32];
+    __shared__ float pm[WPR], pl[WPR];
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, w = warp % WPR;
+    const uint32_t row = blockIdx.x * RPB + warp / WPR;
+    if (row >= a.n_group * a.n_beam * a.n_query * a.n_head) return;  // (one row per block where there is a barrier)
+    const uint32_t st = row / a.n_head, h = row - st * a.n_head, kvh = beam_div(h, p.by_gq), hg = h - kvh * a.gq;
+    const uint32_t s = st / a.n_query, t = st - s * a.n_query, grp = s / a.n_beam;
     const uint32_t pr = ((s - grp * a.n_beam) * a.n_query + t) * a.gq + hg, sr = t * a.gq + hg;
     const uint32_t ptile = pr / p.prow, stile = sr / p.srow;
     const uint32_t pi = (grp * a.n_kv + kvh) * p.ptiles + ptile, si = (s * a.n_kv + kvh) * p.stiles + stile;
@@ -836,19 +842,19 @@ __global__ void __launch_bounds__(kBaThreads) beam_attn_join_kernel(BeamAttnArgs
     const size_t srow = (size_t)(si + sc.x) * p.srow + (sr - stile * p.srow);
     float m = -INFINITY, l = 0.f;
     Vec o{};
-    for (uint32_t j0 = warp; j0 < n; j0 += 4 * NW) {
+    for (uint32_t j0 = w; j0 < n; j0 += 4 * WPR) {
         float2 ml[4];
         Vec v[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const uint32_t j = min(j0 + u * NW, n - 1);
-            const size_t row = j < np ? prow + (size_t)j * p.prow : srow + (size_t)(j - np) * p.srow;
-            ml[u] = (j < np ? p.pml : p.sml)[row];
-            v[u] = *reinterpret_cast<const Vec *>((j < np ? p.po : p.so) + row * HD + lane * V);
+            const uint32_t j = min(j0 + u * WPR, n - 1);
+            const size_t at = j < np ? prow + (size_t)j * p.prow : srow + (size_t)(j - np) * p.srow;
+            ml[u] = (j < np ? p.pml : p.sml)[at];
+            v[u] = *reinterpret_cast<const Vec *>((j < np ? p.po : p.so) + at * HD + lane * V);
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            if (j0 + u * NW >= n) break;
+            if (j0 + u * WPR >= n) break;
             const float mn = fmaxf(m, ml[u].x), safe = mn == -INFINITY ? 0.f : mn;
             const float mine = exp2_fast(m - safe), other = exp2_fast(ml[u].x - safe);
             m = mn;
@@ -857,24 +863,31 @@ __global__ void __launch_bounds__(kBaThreads) beam_attn_join_kernel(BeamAttnArgs
             for (int i = 0; i < V; ++i) o.v[i] = o.v[i] * mine + v[u].v[i] * other;
         }
     }
-    part[warp][lane] = o;
-    if (lane == 0) { pm[warp] = m; pl[warp] = l; }
-    __syncthreads();
-    float M = -INFINITY, L = 0.f;
+    if constexpr (WPR > 1) {
+        part[w][lane] = o;
+        if (lane == 0) { pm[w] = m; pl[w] = l; }
+        __syncthreads();
+        if (w) return;
+        m = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < NW; ++w) M = fmaxf(M, pm[w]);
-    const float safe = M == -INFINITY ? 0.f : M;
-    const uint32_t d = threadIdx.x;
-    float v = 0.f;
+        for (int u = 0; u < WPR; ++u) m = fmaxf(m, pm[u]);
+        const float safe = m == -INFINITY ? 0.f : m;
+        l = 0.f;
+        o = Vec{};
 #pragma unroll
-    for (int w = 0; w < NW; ++w) {
-        const float f = exp2_fast(pm[w] - safe);
-        L += pl[w] * f;
-        if (d < HD) v += reinterpret_cast<const float *>(part[w])[d] * f;
+        for (int u = 0; u < WPR; ++u) {
+            const float f = exp2_fast(pm[u] - safe);
+            const Vec x = part[u][lane];
+            l += pl[u] * f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) o.v[i] += x.v[i] * f;
+        }
     }
-    const size_t at = (size_t)blockIdx.x * a.n_head + h;
-    if (d < a.hd) static_cast<T *>(a.out)[at * a.hd + d] = beam_from_f32<T>(L == 0.f ? 0.f : v / L);
-    if (a.lse && d == 0) a.lse[at] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+    T *out = static_cast<T *>(a.out) + (size_t)row * a.hd;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+        if (lane * V + i < a.hd) out[lane * V + i] = beam_from_f32<T>(l == 0.f ? 0.f : o.v[i] / l);
+    if (a.lse && lane == 0) a.lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 }  // namespace fwb
