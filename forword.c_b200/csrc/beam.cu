@@ -129,7 +129,7 @@ uint32_t device_sms() {
 struct AttnLayout {
     bool tc;            // on the 5th-generation tensor cores (beam_attn_tc.cuh)
     uint32_t prow, srow;  // rows of a prefix / suffix tile
-    uint32_t ptiles, stiles, ctas, tctas, cost;  // (tctas: of the tcgen05 kernel, the others then the suffixes')
+    uint32_t ptiles, stiles, ctas, tctas, cost, tcost;  // (tctas, tcost: of the tcgen05 kernel, the others then the suffixes')
     size_t pitems, sitems, bytes;
     size_t po, so, pml, sml, pcta, scta;
 };
@@ -153,10 +153,16 @@ bool attn_layout(const fwb_prefix_attn_t *a, AttnLayout &L) {
     L.stiles = (uint32_t)((srows + L.srow - 1) / L.srow);
     L.pitems = a->prefix_cap ? (size_t)a->n_group * a->n_head_kv * L.ptiles : 0;
     L.sitems = a->suffix_cap ? (size_t)a->n_group * a->n_beam * a->n_head_kv * L.stiles : 0;
-    // (measured: 4 and 20 against 0 save a third where suffixes are many and short)
-    L.cost = L.tc ? 20 : 4;
-    const uint64_t punits = L.pitems * ((a->prefix_cap + 15) / 16 + L.cost),
-                   sunits = L.sitems * ((a->suffix_cap + 15) / 16 + 4), units = punits + sunits;
+    // What an item's beginning and end cost, in units.  Measured with 4 / 12 / 16:
+    // 6 groups of 5 fp16 beams 40 / 32 / 32 us, 4 beams over 30000 positions 38 /
+    // 30 / 31; fp32, whose units take three times as long, 30 / 31 / 32 for 4
+    // beams over 8000.  Units of 64 rows take longer too: 48 beams over 500 and
+    // 4000 positions 17 / 23 / - and 31 / 36 / -.  The tcgen05 kernel 20 / 40: 9
+    // beams of 7 tokens 30.5 / 28.1.
+    L.cost = a->type == 0 ? 4 : L.prow == 64 ? 6 : 12;
+    L.tcost = 40;
+    const uint64_t punits = L.pitems * ((a->prefix_cap + 15) / 16 + (L.tc ? L.tcost : L.cost)),
+                   sunits = L.sitems * ((a->suffix_cap + 15) / 16 + L.cost), units = punits + sunits;
     if (L.pitems + L.sitems > 0x3fffffffu || units > 0x7fffffffu)
         return fail("fwb_prefix_attention: too many rows times positions");
     const uint64_t sms = device_sms();
@@ -248,7 +254,7 @@ bool run_parts(const BeamAttnArgs &k, BeamAttnPlan p, const BeamMaps &maps, cons
     const uint32_t seqs = k.n_group * k.n_beam;
     p.part0 = L.tc ? k.n_group : 0;
     p.parts = k.n_group + seqs;
-    p.cost = 4;
+    p.cost = L.cost;
     p.ctas = L.ctas;
     if (L.tc) p.prow = p.srow;  // (its kernel has no prefix part)
     if (!pick_attn<T, HD>(k, p, maps, st)) return false;
@@ -257,7 +263,7 @@ bool run_parts(const BeamAttnArgs &k, BeamAttnPlan p, const BeamMaps &maps, cons
         if (L.tc) {
             p.part0 = 0;
             p.parts = k.n_group;
-            p.cost = L.cost;
+            p.cost = L.tcost;
             p.ctas = L.tctas;
             if (!launch_attn_tc<T, HD>(k, p, maps, st)) return false;
             p.ctas = std::max(L.ctas, L.tctas);
