@@ -30,6 +30,8 @@ constexpr uint32_t kBrMaxBeams = 64;
 // counts all columns.  One column per thread: a thread has the loads of all
 // moved beams in flight at once, which is what the memory needs.  Slots that
 // keep their own state in place are neither read nor written.
+// Bound: DRAM.  K/V rows of 32 layers for 8 beams, half of them moved in place
+// (183 MB read and written): 35.7 us, 5.1 TB/s, of a copy's 6.5.
 template <typename V, int NB, typename I>
 __global__ void __launch_bounds__(kBrThreads) beam_reorder_kernel(BeamReorderArgs a) {
     const I i = (I)blockIdx.x * kBrThreads + threadIdx.x;
