@@ -189,9 +189,11 @@ __device__ __forceinline__ void mma8(float *c, const uint32_t *a, uint32_t b0, u
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // x = hi + lo: hi rounded to tf32's 11 significant bits, lo the exact rest
-// (13 bits; the product takes its first 11).
+// (12 bits and a sign; the product takes its first 11).  By integer addition:
+// the conversion instruction has a quarter of its rate (4 beams over 30000
+// positions 70 us with it, 61 without).
 __device__ __forceinline__ void tf32_split(float x, uint32_t &hi, uint32_t &lo) {
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
     lo = __float_as_uint(x - __uint_as_float(hi));
 }
 __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
@@ -241,7 +243,7 @@ constexpr int kBaStages = sizeof(T) == 2 ? 3 : 2;
 // the outputs that warps sharing rows hand over at an item's end.
 template <typename T, int HD, int RW>
 constexpr uint32_t beam_attn_rows_smem() {  // (a row group: 16 rows in the tiles' chunk order)
-    return sizeof(T) == 4 ? RW * 16 * HD * 4 : RW < 4 ? RW * 16 * HD * 4 : 0;
+    return sizeof(T) == 4 ? RW * 16 * HD * 4 : RW < 4 ? 2 * 16 * HD * 4 : 0;
 }
 constexpr uint32_t kBaTail = 2 * 3 * 8 + 2 * 16 * 8;  // barriers; maxima and sums that are handed over
 template <typename T, int HD, int RWP, int RWS>
@@ -620,12 +622,14 @@ __device__ __forceinline__ void beam_tile(BeamRows<T, HD> &w, uint32_t qs, uint3
     }
 }
 
-// Joins the rows of the warps that share them (one after the other hands
-// over to the first), which then writes the item's partial result.  buf: an
-// output of every row group.
+// Joins the rows of the warps that share them -- the upper half of those that
+// had positions hands over to the lower, in 16-bit types; in fp32, where there
+// is room for one, one after the other hands over to the first -- which then
+// writes the item's partial result.  buf: outputs of two warps (fp32: one for
+// every row group).  busy: warps that share rows and had positions.
 template <typename T, int HD, int RW>
 __device__ __forceinline__ void beam_flush(const BeamAttnArgs &a, const BeamAttnPlan &p, const BeamCursor &c,
-                                           BeamRows<T, HD> &w, float *buf, float2 *bml) {
+                                           BeamRows<T, HD> &w, uint32_t busy, float *buf, float2 *bml) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5, rg = warp % RW, kg = warp / RW;
     const uint32_t g = lane >> 2, t = lane & 3;
 #pragma unroll
@@ -633,26 +637,30 @@ __device__ __forceinline__ void beam_flush(const BeamAttnArgs &a, const BeamAttn
         w.l[h] += __shfl_xor_sync(0xffffffffu, w.l[h], 1);
         w.l[h] += __shfl_xor_sync(0xffffffffu, w.l[h], 2);
     }
+    constexpr bool kPairs = sizeof(T) == 2 && RW == 1;  // two hand over at once
 #pragma unroll 1
-    for (uint32_t from = 1; from < 4 / RW; ++from) {
-        float *ob = buf + rg * 16 * HD;
+    for (uint32_t i = 1; i < (kPairs ? 3u : 4u / RW); ++i) {
+        const uint32_t half = kPairs ? 4 >> i : 1, from = kPairs ? half : i;
+        if (from >= busy) continue;
+        const uint32_t at = kPairs ? kg & (half - 1) : rg;
+        float *ob = buf + at * 16 * HD;
         bar_sync(1, kBaThreads);  // what was here is read
-        if (kg == from) {
+        if (kg >= from && kg < from + half) {
 #pragma unroll
             for (int j = 0; j < HD / 8; ++j)
                 *reinterpret_cast<float4 *>(ob + (j * 32 + lane) * 4) =
                     make_float4(w.o[j][0], w.o[j][1], w.o[j][2], w.o[j][3]);
             if (t == 0) {
-                bml[rg * 16 + g] = make_float2(w.m[0], w.l[0]);
-                bml[rg * 16 + g + 8] = make_float2(w.m[1], w.l[1]);
+                bml[at * 16 + g] = make_float2(w.m[0], w.l[0]);
+                bml[at * 16 + g + 8] = make_float2(w.m[1], w.l[1]);
             }
         }
         bar_sync(1, kBaThreads);
-        if (kg == 0) {
+        if (kg < half) {
             float mine[2], other[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float2 ml = bml[rg * 16 + g + 8 * h];
+                const float2 ml = bml[at * 16 + g + 8 * h];
                 const float mn = fmaxf(w.m[h], ml.x), safe = mn == -INFINITY ? 0.f : mn;
                 mine[h] = exp2_fast(w.m[h] - safe);
                 other[h] = exp2_fast(ml.x - safe);
@@ -713,15 +721,19 @@ __device__ __forceinline__ void beam_advance(BeamCursor &c, uint32_t n) {
 // groups of 16, and 4 / RW warps share each tile's positions.
 template <typename T, int HD, int RW>
 __device__ __forceinline__ void beam_step(const BeamAttnArgs &a, const BeamAttnPlan &p, BeamCursor &c, bool &fresh,
-                                          BeamRows<T, HD> &w, uint32_t stage, uint64_t *full, uint64_t *empty,
+                                          uint32_t &most, BeamRows<T, HD> &w, uint32_t stage, uint64_t *full, uint64_t *empty,
                                           uint32_t phase, bool &ok, uint32_t rows, float *buf, float2 *bml) {
     using Tl = BeamTile<T, HD>;
     constexpr int KW = Tl::kKeys / (4 / RW);
     const uint32_t warp = threadIdx.x >> 5, rg = warp % RW, kg = warp / RW;
     const uint32_t qs = rows + rg * 16 * HD * 4;
-    if (fresh) beam_rows_init<T, HD>(a, p, c, c.tile * RW * 16 + rg * 16, qs, w);
+    if (fresh) {
+        beam_rows_init<T, HD>(a, p, c, c.tile * RW * 16 + rg * 16, qs, w);
+        most = 0;
+    }
     const bool first = c.pos == 0;
     const uint32_t n = beam_take<T, HD>(c);
+    most = max(most, n);  // positions of the item's longest tile here
     // (after a wait that ran out: the same steps and barriers without the work)
     ok = mbar_wait(full, phase, &g_beam_err, ERR_WAIT_FULL) && ok;
     __syncwarp();
@@ -731,7 +743,7 @@ __device__ __forceinline__ void beam_step(const BeamAttnArgs &a, const BeamAttnP
     if ((threadIdx.x & 31) == 0) mbar_arrive(empty);
     beam_advance(c, n);
     fresh = c.pos >= c.len || c.left == 0;
-    if (fresh) beam_flush<T, HD, RW>(a, p, c, w, buf, bml);
+    if (fresh) beam_flush<T, HD, RW>(a, p, c, w, (most + KW - 1) / KW, buf, bml);
     if (threadIdx.x == 0 && (first || c.pos >= c.len)) {
         const bool pre = c.part < a.n_group;
         const uint32_t item = ((pre ? c.part : c.part - a.n_group) * a.n_kv + c.kvh) * (pre ? p.ptiles : p.stiles) + c.tile;
@@ -806,13 +818,14 @@ __global__ void __launch_bounds__(kBaThreads + kBaLoader, sizeof(T) == 4 && RWP 
     }
     BeamRows<T, HD> w;
     bool fresh = true, ok = true;
+    uint32_t most = 0;
 #pragma unroll 1
     while (c.left) {
         const uint32_t stage = smem + s * 2 * Tl::kBytes;
         if (RWP == RWS || c.part < a.n_group)
-            beam_step<T, HD, RWP>(a, p, c, fresh, w, stage, &full[s], &empty[s], phase, ok, rows, buf, bml);
+            beam_step<T, HD, RWP>(a, p, c, fresh, most, w, stage, &full[s], &empty[s], phase, ok, rows, buf, bml);
         else
-            beam_step<T, HD, RWS>(a, p, c, fresh, w, stage, &full[s], &empty[s], phase, ok, rows, buf, bml);
+            beam_step<T, HD, RWS>(a, p, c, fresh, most, w, stage, &full[s], &empty[s], phase, ok, rows, buf, bml);
         if (++s == S) {
             s = 0;
             phase ^= 1;
