@@ -518,3 +518,70 @@ def test_refusals(torch, beam):
         beam.reorder(x[:, :3], torch.zeros(1, 3, dtype=torch.int32, device="cuda"), x[:, 1:])
     with pytest.raises(FwbError):
         beam.reorder(torch.zeros(1, 65, 4, device="cuda"), torch.zeros(1, 65, dtype=torch.int32, device="cuda"))
+
+
+# --- many rows over long prefixes: the tcgen05 kernel -------------------------------------
+# n_group * n_head_kv * prefix_cap * (rows / 64 - rows / 128, each rounded up) is at least
+# 36000 in all of these, which is where that kernel takes the prefixes over.
+LONG = [
+    # G  W   nq nh nkv  hd    P    S
+    (1, 40, 2, 8, 4, 128, 9001, 6),
+    (1, 9, 7, 32, 4, 128, 2611, 71),
+    (2, 33, 1, 16, 4, 64, 4609, 5),
+    (1, 20, 4, 8, 8, 96, 4513, 12),
+    (1, 64, 1, 8, 1, 48, 9100, 3),
+    (3, 128, 1, 2, 2, 16, 6144, 0),
+    (1, 300, 1, 4, 2, 112, 4096, 1),
+]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("shape", LONG, ids=lambda s: "x".join(map(str, s)))
+def test_attention_many_rows(torch, beam, dtype, shape):
+    attn_check(torch, beam, attn_case(torch, dtype, *shape, seed=sum(shape)))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_attention_many_rows_short_lengths(torch, beam, dtype):
+    """Lengths of a tile's fractions in a large cache, of nothing, and past it; poison behind them."""
+    for plen in ([0, 1, 15], [127, 128, 129], [16, 0, 20000], [-3, 4100, 500]):
+        c = attn_case(torch, dtype, 3, 24, 1, 32, 8, 128, 4100, 9, plen=plen, slen=[i % 10 for i in range(72)])
+        clean = attn_check(torch, beam, c)
+        for g in range(3):
+            for k in ("pk", "pv"):
+                for i, b in enumerate((math.nan, math.inf, -math.inf)):
+                    c[k][g, :, max(0, plen[g]) + i::3] = b
+        dirty = attn_check(torch, beam, c)
+        assert torch.equal(clean[0], dirty[0]) and torch.equal(clean[1], dirty[1])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_attention_many_rows_rising_scores(torch, beam, dtype):
+    """Tiles that raise the references again and again, by little and by much, for some rows only."""
+    c = attn_case(torch, dtype, 1, 48, 1, 16, 4, 128, 9500, 8)
+    c["q"].fill_(0)
+    c["q"][..., 0] = torch.linspace(0, 1, 48, device="cuda")[:, None, None].to(c["q"].dtype)
+    c["q"][..., 1] = 0.25
+    at = torch.arange(9500, device="cuda")
+    c["pk"][..., 0] = (at / 95.0).to(c["pk"].dtype)
+    c["pk"][..., 1] = (((at * 7919) % 9500) / 40.0).to(c["pk"].dtype)
+    attn_check(torch, beam, c, scale=1.0)
+    c["pk"][..., 0] = (-at / 50.0).to(c["pk"].dtype)
+    attn_check(torch, beam, c, scale=1.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("W,P", [(3, 150), (32, 2400)])
+def test_attention_broadcast_caches(torch, beam, dtype, W, P):
+    """One prefix for all groups and one KV head for all (strides of 0), one suffix for all sequences."""
+    c = attn_case(torch, dtype, 2, W, 1, 32, 8, 128, P, 20, slots=False)
+    for k in ("pk", "pv"):
+        c[k] = c[k][:1, :1].expand(2, 8, -1, -1)
+    for k in ("sk", "sv"):
+        c[k] = c[k][:1].expand(2 * W, -1, -1, -1)
+    c["plen"] = [P, P - 1]
+    attn_check(torch, beam, c)
+
+
+def test_attention_status(torch, beam):
+    beam.check_status()
