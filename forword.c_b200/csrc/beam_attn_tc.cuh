@@ -19,7 +19,7 @@
 // the exponentials 1024 (16 a cycle and SM), shared memory about 2000 (both
 // operands of both products, the copies, P); measured 4000, with eight softmax
 // warps waiting on one another and on short chains.  64 bf16 samples (512 rows
-// for each of 8 KV heads) over 32763 positions: 136 us with their suffixes, 500
+// for each of 8 KV heads) over 32763 positions: 134 us with their suffixes, 515
 // TFLOP/s, against 276 with warp-level products.
 //
 // One CTA per SM: a warp that loads (copy engine), one thread that issues the

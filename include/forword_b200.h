@@ -184,9 +184,9 @@ typedef struct fwb_prefix_attn {
  * 0..n_beam-1 counts as the sequence's own beam).  lse receives log sum exp
  * of the scaled scores.  A token that sees no position gets out 0 and lse
  * -inf.  Lengths are held to 0..cap; rows at and past a length are never
- * used, whatever they hold; rows below it hold finite values (a new token's V
- * that is not finite also spoils the sequence's earlier new tokens).  Scores,
- * softmax and sums are fp32, the probabilities of fp16 and bf16 calls are
+ * used, whatever they hold; K or V below it that is infinite or NaN reaches
+ * the tokens that see its position and no others.  Scores, softmax and sums
+ * are fp32, the probabilities of fp16 and bf16 calls are
  * rounded to that type for the products with V.
  * workspace: fwb_prefix_attention_workspace(a) bytes of device memory,
  * 16-byte aligned, that no other call uses meanwhile; its contents matter to

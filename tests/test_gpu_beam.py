@@ -185,6 +185,36 @@ def test_attention_ignores_what_lies_past_the_lengths(torch, beam, dtype, rows):
     assert torch.equal(clean[0], dirty[0]) and torch.equal(clean[1], dirty[1])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", [(1, 3, 5, 8, 2, 128, 70, 40), (2, 2, 40, 8, 2, 64, 190, 64), (1, 2, 17, 6, 6, 48, 0, 33),
+                                   (1, 2, 3, 4, 4, 16, 5, 19)], ids=lambda s: "x".join(map(str, s)))
+def test_attention_keeps_values_from_tokens_that_do_not_see_them(torch, beam, dtype, shape):
+    """Infinite and NaN V (and NaN K) of a new token reach that token and later ones, and no earlier one."""
+    nq, nh, nkv, hd, n = shape[2], shape[3], shape[4], shape[5], shape[0] * shape[1]
+    c = attn_case(torch, dtype, *shape, slots=False, slen=[shape[7] - 3 * i for i in range(n)])
+    clean, lse = attn_check(torch, beam, c)
+    plan = beam.PrefixAttention(n_group=shape[0], n_beam=shape[1], n_query=nq, n_head=nh, n_head_kv=nkv, head_dim=hd,
+                                dtype=c["q"].dtype, prefix_cap=shape[6], suffix_cap=shape[7])
+    kw = {"suffix_len": torch.tensor(c["slen"], dtype=torch.int32, device="cuda")}
+    if shape[6]:
+        kw["prefix_len"] = torch.tensor(c["plen"], dtype=torch.int32, device="cuda")
+    sv, sk, from_t = c["sv"].clone(), c["sk"].clone(), nq // 2
+    hit = torch.zeros(n, nq, nh, hd, dtype=torch.bool, device="cuda")
+    for s in range(n):
+        for i, b in enumerate((math.nan, math.inf, -math.inf)):
+            t, h, d = min(nq - 1, from_t + i), i % nkv, (5 * i + 3 * s) % hd
+            sv[s, h, c["slen"][s] - nq + t, d] = b
+            hit[s, t:, h * (nh // nkv):(h + 1) * (nh // nkv), d] = True
+    out, l = plan(c["q"], c["pk"], c["pv"], sk, sv, **kw)
+    assert torch.equal(out[~hit], clean[~hit]) and torch.equal(l, lse)
+    assert not torch.isfinite(out[hit]).any()
+    for s in range(n):
+        sk[s, :, c["slen"][s] - nq + from_t] = math.nan
+    out, l = plan(c["q"], c["pk"], c["pv"], sk, c["sv"], **kw)
+    assert torch.equal(out[:, :from_t], clean[:, :from_t]) and torch.equal(l[:, :from_t], lse[:, :from_t])
+    assert torch.isnan(out[:, from_t:]).all()
+
+
 def test_attention_slots_out_of_range_count_as_own(torch, beam):
     c = attn_case(torch, "f16", 2, 4, 1, 8, 2, 128, 33, 30)
     c["slots"][:, ::3] = -1
