@@ -40,7 +40,8 @@ struct BeamSelectArgs {
     uint64_t row_stride;
     uint32_t n_group, n_beam, n_vocab, n_select;
     // workspace: per part (row-major [row][part]) `cap` candidates (logit,
-    // token; a NaN logit in unused places) and (b, sum of 2^(x log2(e) - b))
+    // token; a NaN logit in unused places) and (m, sum of exp(x - m)), m the
+    // largest logit
     float2 *cand;
     float2 *stat;
     uint32_t n_part, part, cap;
@@ -299,12 +300,24 @@ __device__ __noinline__ void beam_overflow(BeamList &l, const T *x, uint32_t n, 
     if (still) beam_take_best(l, x, n, tok0, old, want);
 }
 
+// Two fp32 at once: x = (x + a) * s, and x += y.
+__device__ __forceinline__ void beam_scaled2(float &x0, float &x1, float a, float s) {
+    asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %2};\n\tmov.b64 z, {%3, %3};\n\t"
+        "add.rn.f32x2 x, x, y;\n\tmul.rn.f32x2 x, x, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "+f"(x0), "+f"(x1) : "f"(a), "f"(s));
+}
+__device__ __forceinline__ void beam_add2(float &x0, float &x1, float y0, float y1) {
+    asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%0, %1};\n\tmov.b64 y, {%2, %3};\n\t"
+        "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+        : "+f"(x0), "+f"(x1) : "f"(y0), "f"(y1));
+}
+
 // One part of a row per block.
 //
 // Bound: the logits once from DRAM.  Five blocks per SM with one piece ahead
 // each keep about 80 KB of loads in flight; a logit costs about seven
-// instructions (maximum, 2^x with one fma and one MUFU, the sum, a compare per
-// four).  256 fp32 rows of 128256: 38 us with the join (3.5 TB/s); the blocks
+// instructions (maximum, 2^x with half of a packed addition and product and one
+// MUFU, half of a packed sum, a compare per four).  256 fp32 rows of 128256: 38 us with the join (3.5 TB/s); the blocks
 // are 3.5 per SM on average and 4 on the busiest.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kBsThreads, 5) beam_select_part_kernel(BeamSelectArgs a) {
@@ -325,9 +338,10 @@ __global__ void __launch_bounds__(kBsThreads, 5) beam_select_part_kernel(BeamSel
     Piece::start(x, n, stages);
     uint32_t stage = 0;
     const uint32_t limit = min(kBsList / 2, 3 * a.n_select + 64);  // a longer list is trimmed, which raises the threshold
-    // of this thread's logits so far: the maximum, b = maximum * log2(e) as
-    // rounded, and the sum of 2^(x log2(e) - b); a NaN or +inf makes the sum NaN
-    float m = -INFINITY, b = 0.f, sum = 0.f, thr = 0.f;
+    // of this thread's logits so far: the maximum and the sum of exp(x - m), of
+    // every other one apart; a NaN or +inf makes it NaN.  In the logits' own units: a maximum times
+    // log2(e) would overflow at the type's lowest value, which bars tokens too.
+    float m = -INFINITY, sum = 0.f, odd = 0.f, thr = 0.f;
     for (uint32_t p0 = 0; p0 < n; p0 += kPiece) {
         float v[E];
         {
@@ -351,13 +365,20 @@ __global__ void __launch_bounds__(kBsThreads, 5) beam_select_part_kernel(BeamSel
             }
         }
         if (pm > m) {
-            const float nb = pm * kLog2e;
-            sum *= exp2_fast(b - nb);  // (0 so far without a maximum)
+            if (m > -INFINITY) {  // (without a maximum so far: 0, or NaN)
+                const float f = exp2_fast((m - pm) * kLog2e);
+                sum *= f;
+                odd *= f;
+            }
             m = pm;
-            b = nb;
         }
+        const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-        for (int e = 0; e < E; ++e) sum += exp2_fast(fmaf(v[e], kLog2e, -b));
+        for (int e = 0; e < E; e += 2) {
+            float x0 = v[e], x1 = v[e + 1];
+            beam_scaled2(x0, x1, -ref, kLog2e);
+            beam_add2(sum, odd, exp2_fast(x0), exp2_fast(x1));
+        }
         if (p0 == 0) {
             __syncthreads();
             thr = beam_unorder(l.thr);  // finite: -inf and NaN are below
@@ -404,7 +425,7 @@ __global__ void __launch_bounds__(kBsThreads, 5) beam_select_part_kernel(BeamSel
         }
         for (uint32_t i = a.n_select + threadIdx.x; i < a.cap; i += kBsThreads) cand[i] = make_float2(NAN, 0.f);
     }
-    float bb = m == -INFINITY ? -INFINITY : b;
+    float bb = m;
 #pragma unroll
     for (int o = 16; o; o >>= 1) bb = fmaxf(bb, __shfl_xor_sync(0xffffffffu, bb, o));
     if (lane == 0) s_max[warp] = bb;
@@ -412,7 +433,8 @@ __global__ void __launch_bounds__(kBsThreads, 5) beam_select_part_kernel(BeamSel
 #pragma unroll
     for (int w = 0; w < NW; ++w) bb = fmaxf(bb, s_max[w]);
     // a thread without finite logits has sum 0, or NaN
-    if (m > -INFINITY) sum *= exp2_fast(b - bb);
+    sum += odd;
+    if (m > -INFINITY) sum *= exp2_fast((m - bb) * kLog2e);
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (lane == 0) s_sum[warp] = sum;
@@ -440,7 +462,11 @@ __device__ __forceinline__ double beam_unorder64(uint64_t u) {
 __global__ void __launch_bounds__(kBsJoinThreads) beam_select_join_kernel(BeamSelectArgs a) {
     namespace cg = cooperative_groups;
     const cg::cluster_group cluster = cg::this_cluster();
-    __shared__ double s_off[kBsMaxBeams];     // c - lse
+    constexpr float kLog2e = 1.4426950408889634f;
+    // a score is (x - m) + (c - log sum exp(x - m)), m the row's largest logit: x -
+    // m first, since lse itself may be too large to hold the logarithm
+    __shared__ float s_top[kBsMaxBeams];      // m
+    __shared__ double s_off[kBsMaxBeams];     // c - log sum
     __shared__ float s_offf[kBsMaxBeams];     // the same rounded; NaN: a row without candidates
     __shared__ uint32_t s_best[kBsJoinThreads], s_thr, s_n;
     __shared__ uint64_t s_key[kBsPool];       // beam_order64 of the score
@@ -463,13 +489,14 @@ __global__ void __launch_bounds__(kBsJoinThreads) beam_select_join_kernel(BeamSe
         float sum = 0.f;
         for (uint32_t i = lane; i < a.n_part; i += 32) {
             const float2 v = st[i];  // a part of barred tokens has sum 0 (or NaN)
-            sum += v.x == -INFINITY ? v.y : v.y * exp2_fast(v.x - m);
+            sum += v.x == -INFINITY ? v.y : v.y * exp2_fast((v.x - m) * kLog2e);
         }
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         if (lane == 0) {
             const bool live = isfinite(c) && isfinite(m) && sum > 0 && isfinite(sum);
-            const double off = (double)c - ((double)m * 0.69314718055994531 + (double)logf(sum));
+            const double off = (double)c - (double)logf(sum);
+            s_top[w] = m;
             s_off[w] = off;
             s_offf[w] = live ? (float)off : NAN;
         }
@@ -497,15 +524,16 @@ __global__ void __launch_bounds__(kBsJoinThreads) beam_select_join_kernel(BeamSe
         }
     };
     float best = -INFINITY;
-    each(cr * NW + warp, cs * NW, [&](float x, uint32_t w, uint32_t) { best = fmaxf(best, x + s_offf[w]); });
+    each(cr * NW + warp, cs * NW, [&](float x, uint32_t w, uint32_t) { best = fmaxf(best, (x - s_top[w]) + s_offf[w]); });
     s_best[threadIdx.x] = best == -INFINITY ? kBsNone : beam_order(best);
     __syncthreads();
     if (warp == 0) {
         const uint32_t thr = beam_threshold<kBsJoinThreads>(s_best, a.n_select);
         if (lane == 0) s_thr = thr;
     }
-    // The scores compared here are rounded twice in 32 bits, the offset and the
-    // sum: a candidate counts as below the threshold only by more than both
+    // The scores compared here are rounded three times in 32 bits, the
+    // difference, the offset and the sum, together by at most 2^-23 of |score| +
+    // |offset|: a candidate counts as below the threshold only by more than the
     // roundings of both sides.
     float off_max = 0.f;
     for (uint32_t w = 0; w < a.n_beam; ++w) off_max = fmaxf(off_max, fabsf(s_offf[w]));
@@ -514,10 +542,10 @@ __global__ void __launch_bounds__(kBsJoinThreads) beam_select_join_kernel(BeamSe
     thr -= 2.4e-7f * (2.f * fabsf(thr) + off_max);  // (-FLT_MAX or -inf takes all)
     if (__any_sync(0xffffffffu, best >= thr))
         each(cr * NW + warp, cs * NW, [&](float x, uint32_t w, uint32_t tok) {
-            if (!(x + s_offf[w] >= thr)) return;
+            if (!((x - s_top[w]) + s_offf[w] >= thr)) return;
             const uint32_t at = atomicAdd(pool_n, 1);
             if (at < kBsPool) {
-                pool_key[at] = beam_order64(s_off[w] + (double)x);
+                pool_key[at] = beam_order64(((double)x - (double)s_top[w]) + s_off[w]);
                 pool_flat[at] = w * a.n_vocab + tok;
             }
         });
@@ -533,9 +561,9 @@ __global__ void __launch_bounds__(kBsJoinThreads) beam_select_join_kernel(BeamSe
             uint64_t bs = 0;
             uint32_t bi = 0xffffffffu;
             each(warp, NW, [&](float x, uint32_t w, uint32_t tok) {
-                const float f = x + s_offf[w];
+                const float f = (x - s_top[w]) + s_offf[w];
                 if (f != f) return;
-                const uint64_t s = beam_order64(s_off[w] + (double)x);
+                const uint64_t s = beam_order64(((double)x - (double)s_top[w]) + s_off[w]);
                 const uint32_t flat = w * a.n_vocab + tok;
                 if (n && !(s < ls || (s == ls && flat > li))) return;
                 if (s > bs || (s == bs && flat < bi)) { bs = s; bi = flat; }

@@ -1,0 +1,91 @@
+"""GPU: the beam-search operators (fwb.beam) on extreme values: logits far below
+zero and masks of the type's lowest value, against the definition in 64 bits."""
+import math
+
+import numpy as np
+import pytest
+
+from test_gpu_beam import beam, decided, dtype_of, select_decided, select_inputs, torch  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# --- selection ----------------------------------------------------------------------
+def stable_scores(x, c):
+    """c + ((x - max) - log sum exp(x - max)) in 64 bits, flat per group: logsumexp by itself may be too large to hold the logarithm."""
+    x = x.astype(np.float64)
+    d = x - x.max(2, keepdims=True)
+    s = (d - np.log(np.exp(d).sum(2, keepdims=True))) + c.astype(np.float64)[:, :, None]
+    return s.reshape(x.shape[0], -1)
+
+
+def check_scores(torch, beam, x, c, K, dtype):
+    """The selection of x (values of the type) and its scores.
+
+    A score's logarithm of a sum of V terms rounds 16 times by 2^-24 of 1 + log V, the score's own sum once of its size."""
+    G, W, V = x.shape
+    s = stable_scores(x, c)
+    at = np.argsort(-s, axis=1, kind="stable")[:, :K]
+    plan = beam.BeamSelect(n_group=G, n_beam=W, n_vocab=V, n_select=K, dtype=dtype_of(torch, dtype))
+    t = torch.from_numpy(x).to(dtype_of(torch, dtype)).cuda()
+    assert np.array_equal(t.float().cpu().numpy(), x)
+    got, par, tok = plan(t, torch.from_numpy(c).cuda())
+    assert np.array_equal(par.cpu().numpy().astype(np.int64) * V + tok.cpu().numpy(), at)
+    want = np.take_along_axis(s, at, 1)
+    tol = 16 * 2.0 ** -24 * (1 + math.log(V) + np.abs(c).max() + np.abs(want))
+    assert (np.abs(got.cpu().numpy() - want) <= tol).all()
+
+
+def spoil(kind, x, low, seed):
+    r = np.random.default_rng(seed)
+    if kind == "by -100":
+        return x - 100
+    if kind == "by -1e4":
+        return x - 10000
+    if kind == "masked -1e4":
+        return np.where(r.random(x.shape) < 0.75, -1e4, x)
+    if kind == "masked lowest":
+        return np.where(r.random(x.shape) < 0.95, low, x)
+    if kind == "first half":
+        return np.where(np.arange(x.shape[2]) < x.shape[2] // 2, low, x)
+    if kind == "few allowed":
+        y = np.full_like(x, low)
+        for g in range(x.shape[0]):
+            for w in range(x.shape[1]):
+                at = r.choice(x.shape[2], 12, replace=False)
+                y[g, w, at] = x[g, w, at]
+        return y
+    assert kind == "with barred"
+    u = r.random(x.shape)
+    return np.where(u < 0.5, -np.inf, np.where(u < 0.9, low, x))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("kind", ["by -100", "by -1e4", "masked -1e4", "masked lowest", "first half", "few allowed", "with barred"])
+@pytest.mark.parametrize("G,W,V", [(1, 4, 4000), (2, 3, 32003), (1, 1, 500)])
+def test_select_far_below_zero(torch, beam, dtype, kind, G, W, V):
+    """Finite logits, however low, are candidates with finite scores."""
+    low = torch.finfo(dtype_of(torch, dtype)).min
+    for seed in range(50):
+        x, c = select_inputs(G, W, V, 1000 * seed + V)
+        x = torch.from_numpy(spoil(kind, x, low, seed).astype(np.float32)).to(dtype_of(torch, dtype)).float().numpy()
+        s = stable_scores(x, c)
+        if select_decided(x, s, np.argsort(-s, axis=1, kind="stable")[:, :6], V):
+            check_scores(torch, beam, x, c, 6, dtype)
+            return
+    raise AssertionError("no decided input")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("V", [7, 5000, 40000])
+@pytest.mark.parametrize("value", ["lowest", "highest", -1000.0])
+def test_select_equal_extreme_logits(torch, beam, dtype, V, value):
+    """A row of one value, the type's lowest or highest, is uniform: score c - log V, lowest tokens first."""
+    info = torch.finfo(dtype_of(torch, dtype))
+    value = {"lowest": info.min, "highest": info.max}.get(value, value)
+    x = np.full((1, 1, V), value, np.float32)
+    check_scores(torch, beam, x, np.array([[-2.5]], np.float32), 5, dtype)
+    # beside an ordinary row that is better, and one that is worse
+    y = np.concatenate([x, np.zeros((1, 1, V), np.float32), x], axis=1)
+    check_scores(torch, beam, y, np.array([[-2.5, -1.0, -9.0]], np.float32), 5, dtype)
+    check_scores(torch, beam, y, np.array([[-2.5, -7.0, -9.0]], np.float32), 5, dtype)
