@@ -1897,8 +1897,8 @@ static bool beam_search(fwb_model *m, const uint32_t *prompt, size_t n, size_t n
         }
         live.swap(next);
         if (done.size() >= W) {
-            // no live beam can pass the W found (for a length penalty of at most 0
-            // scores only fall; otherwise the search ends here, as is usual)
+            // without a length penalty scores only fall: the search goes on while a
+            // live beam can still pass the W found; with one it ends here
             if (length_penalty != 0.f || live.empty() || live[0].rank <= worst()) break;
         }
         if (t + 1 == r.cap || live.empty()) break;
@@ -1919,8 +1919,9 @@ static bool beam_search(fwb_model *m, const uint32_t *prompt, size_t n, size_t n
         live.resize(W);  // (dead beams have score -inf and offer nothing)
         if (!beam_forward(r, next_token.data(), t)) return false;
     }
+    // a live beam is a result once it has all its tokens, not where the search ended before
     for (BeamHyp &h : live)
-        if (!h.tokens.empty()) done.push_back(std::move(h));
+        if (h.tokens.size() == r.cap) done.push_back(std::move(h));
     std::stable_sort(done.begin(), done.end(), [](const BeamHyp &x, const BeamHyp &y) { return x.rank > y.rank; });
     if (done.size() > W) done.resize(W);
     CK(cudaStreamSynchronize(st));

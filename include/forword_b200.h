@@ -426,7 +426,7 @@ int fwb_tp_shard(const char *gguf_path, const char *tensor, int as_head, int ran
  * and values live in buffers of the call.  A continuation ends with token
  * `eos` (-1: none does) or at max_new tokens; the search ends when n_beam
  * ended ones are found and, without a length penalty, no live one can pass
- * them.  Results are sorted by the sum of log-probabilities, divided by
+ * them; live ones that are shorter than max_new then are no results.  Results are sorted by the sum of log-probabilities, divided by
  * length^length_penalty (0: not divided): tokens_out [n_beam][max_new],
  * lengths_out and scores_out [n_beam] (length 0 and score -inf where there
  * are fewer).  For models on one GPU whose layers and LM head are Q4_0, with
