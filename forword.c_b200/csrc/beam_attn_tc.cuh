@@ -38,6 +38,10 @@ constexpr int kBtSoft = 256;                 // threads of the softmax
 constexpr int kBtThreads = 64 + kBtSoft;
 constexpr float kBtRaise = 8.f;              // log2
 constexpr int kBtRows = 128;                 // query rows of a tile
+// Minus the reference of a row that has seen no score above -inf: finite, so
+// that a score of -inf stays one against it, and so large that any other
+// exceeds it and raises it.
+constexpr float kBtUnset = 3.4028234664e38f;
 
 // Shared memory: two stages of K and two of V, query rows, two buffers of
 // probabilities, then the small things.
@@ -53,7 +57,7 @@ struct BeamTc {
 struct BeamTcTail {
     uint64_t kfull[2], vfull[2], kempty[2], vempty[2], sfull[2], sfree[2], pfull[2], odone[2], ofree, qfull;
     uint32_t tmem;
-    alignas(16) float nm[128];  // minus the rows' references; +inf: none yet
+    alignas(16) float nm[128];  // minus the rows' references; kBtUnset: none yet
     float alpha[128];
     uint32_t top[128];          // the tile's maxima, as ordered integers; 0 between uses
 };
@@ -237,7 +241,7 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
             asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(qs + (ch >> 3) * (RT * 128) + r * 128 + (((ch ^ r) & 7) << 4)),
                          "r"(v[j].x), "r"(v[j].y), "r"(v[j].z), "r"(v[j].w) : "memory");
         }
-        if (wt < NC) t.nm[col0 + wt] = INFINITY;
+        if (wt < NC) t.nm[col0 + wt] = kBtUnset;
 #pragma unroll
         for (int j = 0; j < NC; ++j) l[j] = 0.f;
         bt_fence_proxy();
@@ -295,8 +299,8 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
             const uint32_t r = col0 + wt, m = t.top[r];
             t.top[r] = 0;
             const float now = fmaxf(-t.nm[r], __uint_as_float(m & 0x80000000u ? m & 0x7fffffffu : ~m));
-            t.alpha[r] = t.nm[r] == INFINITY ? 0.f : exp2_fast(-t.nm[r] - now);
-            t.nm[r] = -now;  // (+inf while the row has seen nothing)
+            t.alpha[r] = exp2_fast(-t.nm[r] - now);
+            t.nm[r] = -now;  // (kBtUnset while the row has seen nothing)
         }
         bar_sync(bar, 128);
         load();

@@ -182,8 +182,8 @@ typedef struct fwb_prefix_attn {
  * sequence group * n_beam + b, the beam that computed it, so that a beam
  * step re-orders this table instead of the cache (an entry outside
  * 0..n_beam-1 counts as the sequence's own beam).  lse receives log sum exp
- * of the scaled scores.  A token that sees no position gets out 0 and lse
- * -inf.  Lengths are held to 0..cap; rows at and past a length are never
+ * of the scaled scores.  A token that sees no position, or only ones whose
+ * scores are -inf, gets out 0 and lse -inf.  Lengths are held to 0..cap; rows at and past a length are never
  * used, whatever they hold; K or V below it that is infinite or NaN reaches
  * the tokens that see its position and no others.  Scores, softmax and sums
  * are fp32, the probabilities of fp16 and bf16 calls are

@@ -5,7 +5,8 @@ import math
 import numpy as np
 import pytest
 
-from test_gpu_beam import beam, decided, dtype_of, select_decided, select_inputs, torch  # noqa: F401
+from test_gpu_beam import (ROUND, attn_case, attn_ref, beam, dtype_of, select_decided, select_inputs,  # noqa: F401
+                           torch)
 
 pytestmark = pytest.mark.gpu
 
@@ -89,3 +90,62 @@ def test_select_equal_extreme_logits(torch, beam, dtype, V, value):
     y = np.concatenate([x, np.zeros((1, 1, V), np.float32), x], axis=1)
     check_scores(torch, beam, y, np.array([[-2.5, -1.0, -9.0]], np.float32), 5, dtype)
     check_scores(torch, beam, y, np.array([[-2.5, -7.0, -9.0]], np.float32), 5, dtype)
+
+
+# --- attention ------------------------------------------------------------------------
+# G  W  nq  nh nkv  hd    P   S: warp-level products with 16, 32 and 64 rows a tile, and the tcgen05 kernel in 16-bit types
+ATTENTION = [(1, 4, 1, 8, 2, 128, 300, 40), (2, 3, 2, 8, 2, 64, 400, 9), (1, 12, 1, 16, 4, 128, 700, 20),
+             (1, 9, 7, 4, 2, 48, 333, 30), (1, 40, 2, 8, 4, 128, 9001, 6), (1, 66, 1, 8, 8, 64, 4700, 3)]
+
+
+def run_attention(torch, beam, c):
+    n, nq, nh, hd = c["q"].shape
+    W = c["n_beam"]
+    plan = beam.PrefixAttention(n_group=n // W, n_beam=W, n_query=nq, n_head=nh, n_head_kv=c["pk"].shape[1], head_dim=hd,
+                                dtype=c["q"].dtype, prefix_cap=c["pk"].shape[2], suffix_cap=c["sk"].shape[2])
+    return plan(c["q"], c["pk"], c["pv"], c["sk"], c["sv"],
+                prefix_len=torch.tensor(c["plen"], dtype=torch.int32, device="cuda"),
+                suffix_len=torch.tensor(c["slen"], dtype=torch.int32, device="cuda"), slots=c["slots"])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("shape", ATTENTION, ids=lambda s: "x".join(map(str, s)))
+def test_attention_keys_that_score_minus_infinity(torch, beam, dtype, shape):
+    """Visible keys whose scores are -inf change nothing: not in a row's first
+    tile, not in whole tiles, in no kernel."""
+    G, W, nq, nh, nkv, hd, P, S = shape
+    c = attn_case(torch, dtype, *shape, slots=False, plen=[P] * G, slen=[S] * (G * W), seed=sum(shape))
+    c["q"][..., 0] = c["q"][..., 0].abs() + 0.5
+    at = torch.arange(P, device="cuda")
+    hit = (at < 170) | (at % 3 == 1)
+    late = torch.arange(S, device="cuda") < (S - nq) // 2
+    want, wl, tol, dl = attn_ref(torch, c["q"], c["pk"][:, :, ~hit], c["pv"][:, :, ~hit], c["sk"][:, :, ~late],
+                                 c["sv"][:, :, ~late], [int((~hit).sum())] * G, [int((~late).sum())] * (G * W), None, W,
+                                 1 / math.sqrt(hd))
+    c["pk"][:, :, hit, 0] = -math.inf
+    c["sk"][:, :, late, 0] = -math.inf
+    out, lse = run_attention(torch, beam, c)
+    tol = tol + ROUND[str(c["q"].dtype)] * want.abs() + 2.0 ** -25
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    assert bool(((out.double() - want).abs() <= tol).all())
+    assert bool(((lse.double() - wl).abs() <= dl).all())
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("shape", ATTENTION, ids=lambda s: "x".join(map(str, s)))
+def test_attention_all_scores_minus_infinity(torch, beam, dtype, shape):
+    """A token all of whose scores are -inf is one that sees nothing."""
+    G, W, nq, nh, nkv, hd, P, S = shape
+    c = attn_case(torch, dtype, *shape, slots=False, plen=[P] * G, slen=[S] * (G * W), seed=sum(shape))
+    c["q"][..., 0] = c["q"][..., 0].abs() + 0.5
+    c["pk"][..., 0] = -math.inf
+    c["sk"][..., 0] = -math.inf
+    out, lse = run_attention(torch, beam, c)
+    assert (out == 0).all() and torch.isneginf(lse).all()
+    c["sk"][W - 1, :, 0, 0] = 1   # one position of one sequence is seen after all
+    out, lse = run_attention(torch, beam, c)
+    mine = torch.zeros(G * W, dtype=torch.bool, device="cuda")
+    mine[W - 1] = True
+    assert (out[~mine] == 0).all() and torch.isneginf(lse[~mine]).all()
+    v = c["sv"][W - 1, :, 0].repeat_interleave(nh // nkv, 0).expand(nq, -1, -1)
+    assert torch.equal(out[W - 1], v) and torch.isfinite(lse[W - 1]).all()
