@@ -882,6 +882,75 @@ __global__ void __launch_bounds__(kBaThreads + kBaLoader, sizeof(T) == 4 && RWP 
     }
 }
 
+// A row of an fp32 call by plain fp32 arithmetic, one warp, V dimensions a
+// lane.  An infinite operand, or one within 2^-12 of the largest float, has no
+// split into two tf32 numbers (infinity minus infinity): the products are NaN
+// there, and a row whose joined result holds a NaN is computed again here, as
+// scores and values are in the definition.  Rare; four positions at a time, so
+// that their loads overlap (about 200 cycles a position); a row that a NaN
+// score has spoilt for good ends early.
+template <int V>
+__device__ __forceinline__ void beam_row_plain(const BeamAttnArgs &a, uint32_t s, uint32_t t, uint32_t h, uint32_t kvh,
+                                               float &m, float &l, float *o) {
+    const uint32_t grp = s / a.n_beam, d0 = (threadIdx.x & 31) * V;
+    const bool held = d0 < a.hd;
+    struct alignas(4 * V) Vec { float v[V]; };
+    auto row = [&](const void *base, size_t at) {
+        return held ? *reinterpret_cast<const Vec *>(static_cast<const float *>(base) + at + d0) : Vec{};
+    };
+    Vec q = row(a.q, s * a.q_seq + t * a.q_tok + h * a.q_head);
+#pragma unroll
+    for (int i = 0; i < V; ++i) q.v[i] *= a.scale, o[i] = 0.f;
+    m = -INFINITY;
+    l = 0.f;
+    const uint32_t np = beam_part_len(a, grp), ns = beam_part_len(a, a.n_group + s), hidden = a.n_query - 1 - t;
+    const uint32_t n = np + (ns > hidden ? ns - hidden : 0);
+#pragma unroll 1
+    for (uint32_t j0 = 0; j0 < n && l == l; j0 += 4) {
+        Vec k[4], v[4];
+        float x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const uint32_t j = min(j0 + u, n - 1), r = j - np;
+            if (j < np) {
+                const size_t at = grp * a.p_group + kvh * a.p_head + j * a.p_pos;
+                k[u] = row(a.pk, at);
+                v[u] = row(a.pv, at);
+            } else {
+                uint32_t from = s;
+                if (a.slots) {
+                    const uint32_t b = (uint32_t)a.slots[s * a.slot_seq + r];
+                    if (b < a.n_beam) from = grp * a.n_beam + b;
+                }
+                const size_t at = from * a.s_seq + kvh * a.s_head + r * a.s_pos;
+                k[u] = row(a.sk, at);
+                v[u] = row(a.sv, at);
+            }
+            x[u] = 0.f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) x[u] = fmaf(q.v[i], k[u].v[i], x[u]);
+        }
+#pragma unroll
+        for (int w = 16; w; w >>= 1)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) x[u] += __shfl_xor_sync(0xffffffffu, x[u], w);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (j0 + u >= n) break;
+            x[u] = __fmul_rn(x[u], 1.4426950408889634f);  // (rounded here, so that the maximum minus itself is 0)
+            const float mn = fmaxf(m, x[u]), safe = mn == -INFINITY ? 0.f : mn;
+            const float al = exp2_fast(m - safe), p = exp2_fast(x[u] - safe);
+            m = mn;
+            l = fmaf(l, al, p);
+#pragma unroll
+            for (int i = 0; i < V; ++i) o[i] = fmaf(o[i], al, p * v[u].v[i]);
+        }
+    }
+    if (l != l)
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = l;
+}
+
 // Joins a row's partial results.  WPR warps a row (token and head) take its
 // segments in turn, four at a time, lanes the dimensions; their results are
 // joined through shared memory.  More where the rows are few and so have many
@@ -958,6 +1027,15 @@ __global__ void __launch_bounds__(kBjThreads<WPR>) beam_attn_join_kernel(BeamAtt
             wild |= __float_as_uint(pl[u]);
 #pragma unroll
             for (int i = 0; i < V; ++i) o.v[i] += x.v[i] * f;
+        }
+    }
+    if constexpr (sizeof(T) == 4) {
+        bool again = l != l;
+#pragma unroll
+        for (int i = 0; i < V; ++i) again |= o.v[i] != o.v[i];  // (past head_dim: zeros)
+        if (__any_sync(0xffffffffu, again)) {
+            beam_row_plain<V>(a, s, t, h, kvh, m, l, o.v);
+            wild = 0;
         }
     }
     if (wild >> 31) {

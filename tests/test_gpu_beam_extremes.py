@@ -108,7 +108,7 @@ def run_attention(torch, beam, c):
                 suffix_len=torch.tensor(c["slen"], dtype=torch.int32, device="cuda"), slots=c["slots"])
 
 
-@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("shape", ATTENTION, ids=lambda s: "x".join(map(str, s)))
 def test_attention_keys_that_score_minus_infinity(torch, beam, dtype, shape):
     """Visible keys whose scores are -inf change nothing: not in a row's first
@@ -131,7 +131,7 @@ def test_attention_keys_that_score_minus_infinity(torch, beam, dtype, shape):
     assert bool(((lse.double() - wl).abs() <= dl).all())
 
 
-@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("shape", ATTENTION, ids=lambda s: "x".join(map(str, s)))
 def test_attention_all_scores_minus_infinity(torch, beam, dtype, shape):
     """A token all of whose scores are -inf is one that sees nothing."""
@@ -149,3 +149,32 @@ def test_attention_all_scores_minus_infinity(torch, beam, dtype, shape):
     assert (out[~mine] == 0).all() and torch.isneginf(lse[~mine]).all()
     v = c["sv"][W - 1, :, 0].repeat_interleave(nh // nkv, 0).expand(nq, -1, -1)
     assert torch.equal(out[W - 1], v) and torch.isfinite(lse[W - 1]).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", ATTENTION, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("where", ["prefix", "suffix"])
+def test_attention_infinite_and_largest_values(torch, beam, dtype, shape, where):
+    """Visible values of V: infinite ones keep their sign, opposite ones and NaN give NaN, the largest finite ones a
+    finite result, and the other dimensions are as if they were not there."""
+    G, W, nq, nh, nkv, hd, P, S = shape
+    c = attn_case(torch, dtype, *shape, slots=False, plen=[P] * G, slen=[S] * (G * W), seed=sum(shape))
+    k, v, at = (c["pk"], c["pv"], (P // 2, P - 1)) if where == "prefix" else (c["sk"], c["sv"], (0, (S - nq) // 2))
+    for i in at:
+        k[:, :, i] = 0            # a weight that is not lost in any type
+    big = torch.finfo(v.dtype).max
+    v[:, :, at[0], 1], v[:, :, at[1], 2] = big, -big
+    want, wl, tol, dl = attn_ref(torch, c["q"], c["pk"], c["pv"], c["sk"], c["sv"], c["plen"], c["slen"], None, W,
+                                 1 / math.sqrt(hd))
+    tol = tol + ROUND[str(v.dtype)] * want.abs() + 2.0 ** -25
+    v[:, :, at[0], 3] = math.inf
+    v[:, :, at[1], 5] = -math.inf
+    v[:, :, at[0], 7] = math.nan
+    if at[0] != at[1]:
+        v[:, :, at[0], 9], v[:, :, at[1], 9] = math.inf, -math.inf
+    out, lse = run_attention(torch, beam, c)
+    assert torch.isposinf(out[..., 3]).all() and torch.isneginf(out[..., 5]).all() and torch.isnan(out[..., 7]).all()
+    assert at[0] == at[1] or torch.isnan(out[..., 9]).all()
+    rest = [d for d in range(hd) if d not in (3, 5, 7, 9)]
+    assert bool(((out.double() - want).abs() <= tol)[..., rest].all())
+    assert bool(((lse.double() - wl).abs() <= dl).all())
