@@ -680,7 +680,9 @@ __device__ __forceinline__ void beam_flush(const BeamAttnArgs &a, const BeamAttn
             }
         }
     }
-    if (RW < 4) bar_sync(1, kBaThreads);  // before the next item's rows come into the same place
+    // before the next item's rows come into the same place: these outputs', and
+    // fp32 query rows of other warps where a suffix tile has fewer row groups
+    if (RW < 4 || sizeof(T) == 4) bar_sync(1, kBaThreads);
     if (kg == 0) {
         const bool pre = c.part < a.n_group;
         const uint32_t item = ((pre ? c.part : c.part - a.n_group) * a.n_kv + c.kvh) * (pre ? p.ptiles : p.stiles) + c.tile;
