@@ -884,40 +884,52 @@ __global__ void __launch_bounds__(kBaThreads + kBaLoader, sizeof(T) == 4 && RWP 
     }
 }
 
-// A row of an fp32 call by plain fp32 arithmetic, one warp, V dimensions a
-// lane.  An infinite operand, or one within 2^-12 of the largest float, has no
-// split into two tf32 numbers (infinity minus infinity): the products are NaN
-// there, and a row whose joined result holds a NaN is computed again here, as
-// scores and values are in the definition.  Rare; four positions at a time, so
-// that their loads overlap (about 200 cycles a position); a row that a NaN
-// score has spoilt for good ends early.
-template <int V>
+// A row by plain fp32 arithmetic, V dimensions a lane; warp w of WPR takes
+// every WPR-th four positions, whose loads overlap.  For rows that the kernels'
+// arithmetic cannot form, which the joining kernel finds by its partial results:
+// - fp32: an infinite operand, or one within 2^-12 of the largest float, has no
+//   split into two tf32 numbers (infinity minus infinity); the products are NaN.
+// - scores of 2^16 and more in units of log2, keys near the largest float among
+//   them: a maximum is a scaled score as rounded, and the exact product that a
+//   fused multiply-add takes differs from it by up to 2^-24 of it.  That shifts
+//   a row's probabilities by a common factor, which for still larger scores is
+//   a power of two past the types' range.  (Rounding every product in the
+//   kernels: 64 bf16 samples 147 us for 134.)
+// Rare and slow: 4 fp32 beams over 8000 positions 465 us for 28.  A row that a
+// NaN score has spoilt for good ends early.
+template <typename T, int V, int WPR>
 __device__ __forceinline__ void beam_row_plain(const BeamAttnArgs &a, uint32_t s, uint32_t t, uint32_t h, uint32_t kvh,
-                                               float &m, float &l, float *o) {
+                                               uint32_t w, float &m, float &l, float *o) {
     const uint32_t grp = s / a.n_beam, d0 = (threadIdx.x & 31) * V;
     const bool held = d0 < a.hd;
-    struct alignas(4 * V) Vec { float v[V]; };
-    auto row = [&](const void *base, size_t at) {
-        return held ? *reinterpret_cast<const Vec *>(static_cast<const float *>(base) + at + d0) : Vec{};
-    };
-    Vec q = row(a.q, s * a.q_seq + t * a.q_tok + h * a.q_head);
+    struct alignas(sizeof(T) * V) Vec { T v[V]; };
+    auto row = [&](const void *base, size_t at, float *x) {
+        Vec r{};
+        if (held) r = *reinterpret_cast<const Vec *>(static_cast<const T *>(base) + at + d0);
 #pragma unroll
-    for (int i = 0; i < V; ++i) q.v[i] *= a.scale, o[i] = 0.f;
+        for (int i = 0; i < V; ++i) x[i] = beam_to_f32(r.v[i]);
+    };
+    float q[V];
+    row(a.q, s * a.q_seq + t * a.q_tok + h * a.q_head, q);
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        q[i] *= a.scale;
+        o[i] = 0.f;
+    }
     m = -INFINITY;
     l = 0.f;
     const uint32_t np = beam_part_len(a, grp), ns = beam_part_len(a, a.n_group + s), hidden = a.n_query - 1 - t;
     const uint32_t n = np + (ns > hidden ? ns - hidden : 0);
 #pragma unroll 1
-    for (uint32_t j0 = 0; j0 < n && l == l; j0 += 4) {
-        Vec k[4], v[4];
-        float x[4];
+    for (uint32_t j0 = 4 * w; j0 < n && l == l; j0 += 4 * WPR) {
+        float k[4][V], v[4][V], x[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             const uint32_t j = min(j0 + u, n - 1), r = j - np;
             if (j < np) {
                 const size_t at = grp * a.p_group + kvh * a.p_head + j * a.p_pos;
-                k[u] = row(a.pk, at);
-                v[u] = row(a.pv, at);
+                row(a.pk, at, k[u]);
+                row(a.pv, at, v[u]);
             } else {
                 uint32_t from = s;
                 if (a.slots) {
@@ -925,17 +937,17 @@ __device__ __forceinline__ void beam_row_plain(const BeamAttnArgs &a, uint32_t s
                     if (b < a.n_beam) from = grp * a.n_beam + b;
                 }
                 const size_t at = from * a.s_seq + kvh * a.s_head + r * a.s_pos;
-                k[u] = row(a.sk, at);
-                v[u] = row(a.sv, at);
+                row(a.sk, at, k[u]);
+                row(a.sv, at, v[u]);
             }
             x[u] = 0.f;
 #pragma unroll
-            for (int i = 0; i < V; ++i) x[u] = fmaf(q.v[i], k[u].v[i], x[u]);
+            for (int i = 0; i < V; ++i) x[u] = fmaf(q[i], k[u][i], x[u]);
         }
 #pragma unroll
-        for (int w = 16; w; w >>= 1)
+        for (int d = 16; d; d >>= 1)
 #pragma unroll
-            for (int u = 0; u < 4; ++u) x[u] += __shfl_xor_sync(0xffffffffu, x[u], w);
+            for (int u = 0; u < 4; ++u) x[u] += __shfl_xor_sync(0xffffffffu, x[u], d);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             if (j0 + u >= n) break;
@@ -945,7 +957,7 @@ __device__ __forceinline__ void beam_row_plain(const BeamAttnArgs &a, uint32_t s
             m = mn;
             l = fmaf(l, al, p);
 #pragma unroll
-            for (int i = 0; i < V; ++i) o[i] = fmaf(o[i], al, p * v[u].v[i]);
+            for (int i = 0; i < V; ++i) o[i] = fmaf(o[i], al, p * v[u][i]);
         }
     }
     if (l != l)
@@ -1010,10 +1022,20 @@ __global__ void __launch_bounds__(kBjThreads<WPR>) beam_attn_join_kernel(BeamAtt
             for (int i = 0; i < V; ++i) o.v[i] = o.v[i] * mine + v[u].v[i] * other;
         }
     }
+    bool again = !(l < INFINITY) || (l > 0.f && fabsf(m) > 65536.f);
+    if constexpr (sizeof(T) == 4)
+#pragma unroll
+        for (int i = 0; i < V; ++i) again |= o.v[i] != o.v[i];  // (past head_dim: zeros)
     if constexpr (WPR > 1) {
         part[w][lane] = o;
         if (lane == 0) { pm[w] = m; pl[w] = __uint_as_float(__float_as_uint(l) | (wild & 0x80000000u)); }
-        __syncthreads();
+        if (__syncthreads_or(again)) {
+            beam_row_plain<T, V, WPR>(a, s, t, h, kvh, w, m, l, o.v);
+            wild = 0;
+            part[w][lane] = o;
+            if (lane == 0) { pm[w] = m; pl[w] = l; }
+            __syncthreads();
+        }
         if (w) return;
         m = -INFINITY;
 #pragma unroll
@@ -1030,15 +1052,9 @@ __global__ void __launch_bounds__(kBjThreads<WPR>) beam_attn_join_kernel(BeamAtt
 #pragma unroll
             for (int i = 0; i < V; ++i) o.v[i] += x.v[i] * f;
         }
-    }
-    if constexpr (sizeof(T) == 4) {
-        bool again = l != l;
-#pragma unroll
-        for (int i = 0; i < V; ++i) again |= o.v[i] != o.v[i];  // (past head_dim: zeros)
-        if (__any_sync(0xffffffffu, again)) {
-            beam_row_plain<V>(a, s, t, h, kvh, m, l, o.v);
-            wild = 0;
-        }
+    } else if (__any_sync(0xffffffffu, again)) {
+        beam_row_plain<T, V, 1>(a, s, t, h, kvh, 0, m, l, o.v);
+        wild = 0;
     }
     if (wild >> 31) {
         // values of suffix positions that other tokens do not see were left out:

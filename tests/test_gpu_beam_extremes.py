@@ -110,8 +110,9 @@ def run_attention(torch, beam, c):
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("shape", ATTENTION, ids=lambda s: "x".join(map(str, s)))
-def test_attention_keys_that_score_minus_infinity(torch, beam, dtype, shape):
-    """Visible keys whose scores are -inf change nothing: not in a row's first
+@pytest.mark.parametrize("value", ["-inf", "lowest"])
+def test_attention_keys_that_score_minus_infinity(torch, beam, dtype, shape, value):
+    """Visible keys whose scores are -inf, or so low that their weight is 0, change nothing: not in a row's first
     tile, not in whole tiles, in no kernel."""
     G, W, nq, nh, nkv, hd, P, S = shape
     c = attn_case(torch, dtype, *shape, slots=False, plen=[P] * G, slen=[S] * (G * W), seed=sum(shape))
@@ -122,8 +123,9 @@ def test_attention_keys_that_score_minus_infinity(torch, beam, dtype, shape):
     want, wl, tol, dl = attn_ref(torch, c["q"], c["pk"][:, :, ~hit], c["pv"][:, :, ~hit], c["sk"][:, :, ~late],
                                  c["sv"][:, :, ~late], [int((~hit).sum())] * G, [int((~late).sum())] * (G * W), None, W,
                                  1 / math.sqrt(hd))
-    c["pk"][:, :, hit, 0] = -math.inf
-    c["sk"][:, :, late, 0] = -math.inf
+    low = -math.inf if value == "-inf" else torch.finfo(c["q"].dtype).min
+    c["pk"][:, :, hit, 0] = low
+    c["sk"][:, :, late, 0] = low
     out, lse = run_attention(torch, beam, c)
     tol = tol + ROUND[str(c["q"].dtype)] * want.abs() + 2.0 ** -25
     assert torch.isfinite(out).all() and torch.isfinite(lse).all()
@@ -178,3 +180,28 @@ def test_attention_infinite_and_largest_values(torch, beam, dtype, shape, where)
     rest = [d for d in range(hd) if d not in (3, 5, 7, 9)]
     assert bool(((out.double() - want).abs() <= tol)[..., rest].all())
     assert bool(((lse.double() - wl).abs() <= dl).all())
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("shape", ATTENTION, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("low,high", [(2.0, 9.0), (-9.0, -2.0)])
+def test_attention_enormous_scores(torch, beam, dtype, shape, low, high):
+    """Scores of 2^28 to 2^40: the largest one takes all the weight, whatever its sign."""
+    G, W, nq, nh, nkv, hd, P, S = shape
+    c = attn_case(torch, dtype, *shape, slots=False, plen=[P] * G, slen=[S] * (G * W), seed=sum(shape))
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    c["q"].zero_()
+    c["q"][..., 0] = torch.randint(1, 5, c["q"].shape[:3], device="cuda", generator=gen).to(c["q"].dtype)
+    for k in ("pk", "sk"):
+        c[k][..., 0] = low
+    c["pk"][:, :, P // 3, 0] = high
+    if high < 0:
+        c["pk"][:, :, P // 3 + 1:, 0] = low - 1
+    scale = 1e9 / 3
+    plan = beam.PrefixAttention(n_group=G, n_beam=W, n_query=nq, n_head=nh, n_head_kv=nkv, head_dim=hd, dtype=c["q"].dtype,
+                                prefix_cap=P, suffix_cap=S, scale=scale)
+    out, lse = plan(c["q"], c["pk"], c["pv"], c["sk"], c["sv"])
+    want = c["pv"][:, :, P // 3].repeat_interleave(nh // nkv, 1).repeat_interleave(W, 0)[:, None].expand(-1, nq, -1, -1)
+    assert torch.equal(out, want)
+    top = c["q"][..., 0].double() * high * scale
+    assert bool(((lse.double() - top).abs() <= 2.0 ** -21 * top.abs()).all())
