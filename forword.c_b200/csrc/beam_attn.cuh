@@ -785,8 +785,7 @@ __device__ __forceinline__ void beam_step(const BeamAttnArgs &a, const BeamAttnP
     const uint32_t n = beam_take<T, HD>(c);
     most = max(most, n);  // positions of the item's longest tile here
     // (after a wait that ran out: the same steps and barriers without the work)
-    ok = mbar_wait(full, phase, &g_beam_err, ERR_WAIT_FULL) && ok;
-    __syncwarp();
+    ok = mbar_wait_warp(full, phase, &g_beam_err, ERR_WAIT_FULL) && ok;
     if (c.part >= a.n_group && c.pos + n + a.n_query > c.len + 1) wild |= beam_tame<T, HD>(stage + Tl::kBytes, n);
     if (ok && kg * KW < n && __any_sync(0xffffffffu, w.lim[0] >= 0 || w.lim[1] >= 0))
         beam_tile<T, HD, KW>(w, qs, stage, stage + Tl::kBytes, kg * KW, c.pos, c.pos + n, a.scale * 1.4426950408889634f);
@@ -849,7 +848,7 @@ __global__ void __launch_bounds__(kBaThreads + kBaLoader, sizeof(T) == 4 && RWP 
         uint32_t issued = 0;
         bool ok = true;
         while (c.left) {
-            if (issued >= S && !(ok = mbar_wait(&empty[s], phase ^ 1, &g_beam_err, ERR_WAIT_EMPTY))) break;
+            if (issued >= S && !(ok = mbar_wait_warp(&empty[s], phase ^ 1, &g_beam_err, ERR_WAIT_EMPTY))) break;
             const uint32_t n = beam_take<T, HD>(c);
             beam_load<T, HD>(a, p, maps, c, n, smem + s * 2 * Tl::kBytes, &full[s]);
             ++issued;

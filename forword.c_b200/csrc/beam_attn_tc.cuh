@@ -250,8 +250,7 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
     }
     const bool first = fresh, start = c.pos == 0;
     const uint32_t n = bt_take(c), b = i & 1, ph = i >> 1 & 1;
-    ok = mbar_wait(&t.sfull[b], ph, &g_beam_err, ERR_WAIT_FULL) && ok;
-    __syncwarp();
+    ok = mbar_wait_warp(&t.sfull[b], ph, &g_beam_err, ERR_WAIT_FULL) && ok;
     bt_fence_after();
     float y[NC];
     const uint32_t ts = tmem + b * RT + lanes + col0;
@@ -308,8 +307,7 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
         if (!first) {  // the sums and the output so far
 #pragma unroll
             for (int j = 0; j < NC; ++j) l[j] *= t.alpha[col0 + j];
-            ok = mbar_wait(&t.odone[(i - 1) & 1], (i - 1) >> 1 & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
-            __syncwarp();
+            ok = mbar_wait_warp(&t.odone[(i - 1) & 1], (i - 1) >> 1 & 1, &g_beam_err, ERR_WAIT_FULL) && ok;
             bt_fence_after();
             const uint32_t to = tmem + 2 * RT + lanes + col0;
 #pragma unroll 1
@@ -330,7 +328,7 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
     if (lane == 0) mbar_arrive(&t.sfree[b]);
     // the buffer's last reader; in order for every tile, so that the phases of
     // these barriers are never two ahead of what was seen
-    if (i >= 2) ok = mbar_wait(&t.odone[b], ph ^ 1, &g_beam_err, ERR_WAIT_EMPTY) && ok;
+    if (i >= 2) ok = mbar_wait_warp(&t.odone[b], ph ^ 1, &g_beam_err, ERR_WAIT_EMPTY) && ok;
     const uint32_t ps = smem_u32(sm + Sm::kOffP + b * Sm::kP) + key * 128;
 #pragma unroll
     for (int j = 0; j < NC; j += 8) {
@@ -348,7 +346,7 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
     if (n & (kBaUnit - 1)) {
         // V rows of the last unit past the end: their probabilities are zero,
         // and zero times whatever the memory holds must be zero
-        ok = mbar_wait(&t.vfull[b], ph, &g_beam_err, ERR_WAIT_FULL) && ok;
+        ok = mbar_wait_warp(&t.vfull[b], ph, &g_beam_err, ERR_WAIT_FULL) && ok;
         const uint32_t vs = smem_u32(sm + Sm::kOffV + b * Sm::kTile);
         const uint32_t end = (n + kBaUnit - 1) / kBaUnit * kBaUnit;
         for (uint32_t j = tid; j < (end - n) * (HD / 8); j += kBtSoft) {
@@ -365,8 +363,7 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
     fresh = c.pos >= c.len || c.left == 0;
     const uint32_t item = (c.part * a.n_kv + c.kvh) * p.ptiles + c.tile;
     if (fresh) {
-        ok = mbar_wait(&t.odone[b], ph, &g_beam_err, ERR_WAIT_FULL) && ok;
-        __syncwarp();
+        ok = mbar_wait_warp(&t.odone[b], ph, &g_beam_err, ERR_WAIT_FULL) && ok;
         bt_fence_after();
         const size_t row0 = (size_t)(item + blockIdx.x) * RT;
         float *o = p.po + row0 * HD + key;
@@ -453,8 +450,7 @@ __global__ void __launch_bounds__(kBtThreads, 1)
         auto next = [&](BeamCursor &at, uint32_t &count, const void *base, uint32_t off, const CUtensorMap *map,
                         const CUtensorMap *wide, uint64_t *full, uint64_t *empty) {
             const uint32_t s = count & 1;
-            if (count >= 2) ok = mbar_wait(&empty[s], (count >> 1 & 1) ^ 1, &g_beam_err, ERR_WAIT_EMPTY);
-            __syncwarp();
+            if (count >= 2) ok = mbar_wait_warp(&empty[s], (count >> 1 & 1) ^ 1, &g_beam_err, ERR_WAIT_EMPTY);
             if (!ok) return;
             const uint32_t n = bt_take(at);
             bt_copy<T, HD>(a, at, n, tma, smem_u32(bt_sm + off + s * Sm::kTile), base, map, wide, &full[s]);

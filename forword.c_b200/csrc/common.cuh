@@ -102,6 +102,13 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, uint32
     return mbar_wait_slow(bar, parity, err, code);
 }
 
+// The same by a whole warp, with one answer for all its lanes: a lane by
+// itself may give up just before the phase ends, and lanes that went on
+// without it would wait for it in the next warp-wide step.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t *bar, uint32_t parity, uint32_t *err, uint32_t code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, err, code));
+}
+
 // 1-D bulk copy global -> this CTA's shared memory, completing `bytes` of
 // transaction count on `bar`.  src, dst 16-byte aligned; bytes % 16 == 0.
 __device__ __forceinline__ void bulk_g2s(void *dst, const void *src, uint32_t bytes,
