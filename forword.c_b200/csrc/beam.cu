@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdio>
+#include <exception>
 
 #include "../../include/forword_b200.h"
 #include "beam_attn.cuh"
@@ -421,14 +422,13 @@ extern "C" {
 
 int fwb_beam_status(void *stream) {
     uint32_t e = 0;
-    const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (!launched(cudaMemcpyFromSymbolAsync(&e, g_beam_err, 4, 0, cudaMemcpyDeviceToHost, st), "fwb_beam_status") ||
-        !launched(cudaStreamSynchronize(st), "fwb_beam_status"))
+    try {
+        if (!launched(beam_take_status(static_cast<cudaStream_t>(stream), e), "fwb_beam_status")) return -1;
+    } catch (const std::exception &) {
+        fail("fwb_beam_status: the lock failed");
         return -1;
+    }
     if (!e) return 0;
-    const uint32_t zero = 0;
-    cudaMemcpyToSymbolAsync(g_beam_err, &zero, 4, 0, cudaMemcpyHostToDevice, st);
-    cudaStreamSynchronize(st);
     char b[96];
     snprintf(b, sizeof b, "fwb_beam_status: device error word 0x%x (a bounded wait in the kernel ran out)", e);
     fail(b);

@@ -17,6 +17,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "beam_status.cuh"
 #include "common.cuh"
 
 namespace fwb {
@@ -216,9 +217,6 @@ __device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void *src
 }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// Set when a bounded wait of the attention kernel ran out; stays until read.
-__device__ uint32_t g_beam_err;
 
 // Shared-memory tile: sub-tiles of 128 bytes of every row, [sub][row][128 B],
 // the 16-byte chunk index xor-ed by the row's low three bits, as the copy

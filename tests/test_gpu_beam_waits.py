@@ -1,7 +1,7 @@
 """GPU: the bounded waits of the beam-search kernels when they run out.  A small
 kernel built from the library's own headers waits for a barrier that completes
 late or not at all; the error word is set beforehand, so that a wait gives up
-after its first thousand polls."""
+after its first thousand polls.  And the error word itself (beam_status.cuh)."""
 import ctypes
 import os
 import shutil
@@ -14,6 +14,7 @@ pytestmark = pytest.mark.gpu
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "forword.c_b200", "csrc")
 
 SOURCE = r"""
+#include "beam_status.cuh"
 #include "common.cuh"
 using namespace fwb;
 
@@ -45,6 +46,34 @@ extern "C" int wait_run(unsigned preset, long long delay, uint32_t *answers, uin
     const cudaError_t e = cudaMemcpy(err, d + 32, 4, cudaMemcpyDeviceToHost);
     cudaFree(d);
     return (int)e;
+}
+
+__global__ void set_kernel(uint32_t bit) { atomicOr(&g_beam_err, 1u << bit); }
+
+// Errors set one after the other on one stream while another looks: all that was seen.
+extern "C" int status_run(int rounds, uint32_t *seen, uint32_t *left) {
+    cudaStream_t a, b;
+    if (cudaStreamCreateWithFlags(&a, cudaStreamNonBlocking) != cudaSuccess ||
+        cudaStreamCreateWithFlags(&b, cudaStreamNonBlocking) != cudaSuccess)
+        return -1;
+    int bad = 0;
+    for (int r = 0; r < rounds; ++r) {
+        uint32_t all = 0, word = 0;
+        for (uint32_t bit = 0; bit < 32; ++bit) {
+            set_kernel<<<1, 1, 0, b>>>(bit);
+            if (beam_take_status(a, word) != cudaSuccess) return -1;
+            all |= word;
+        }
+        if (cudaStreamSynchronize(b) != cudaSuccess || beam_take_status(a, word) != cudaSuccess) return -1;
+        all |= word;
+        bad += all != 0xffffffffu;
+        *seen = all;
+        if (beam_take_status(b, *left) != cudaSuccess) return -1;
+        bad += *left != 0;
+    }
+    cudaStreamDestroy(a);
+    cudaStreamDestroy(b);
+    return bad;
 }
 """
 
@@ -91,3 +120,10 @@ def test_lanes_answer_alike(lib):
         assert len(answers) == 1 and answers <= {0, 1}
         seen |= answers
     assert 1 in seen
+
+
+def test_no_error_is_lost_between_streams(lib):
+    """Each look takes what was set until then, and leaves what is set later to the next."""
+    seen, left = ctypes.c_uint32(), ctypes.c_uint32(1)
+    assert lib.status_run(200, ctypes.byref(seen), ctypes.byref(left)) == 0
+    assert seen.value == 0xffffffff and left.value == 0
