@@ -12,7 +12,8 @@ Thin plumbing over the CUDA library (no CPU fallback): a plan checks sizes
 once and keeps its workspace; a call checks its tensors and enqueues on the
 current stream of torch.  Plans and calls work on the current device.  One
 plan is used from one thread at a time; each stream that it is used on gets a
-workspace of its own.
+workspace of its own, and so does each call captured into a CUDA graph, from
+the graph's memory pool.
 """
 from __future__ import annotations
 
@@ -46,6 +47,7 @@ class PrefixAttnArgs(ctypes.Structure):
 # the current stream of torch as a cudaStream_t (the public call builds an object, 3 us)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda device: torch.cuda.current_stream(device).cuda_stream)
+_capturing = torch.cuda.is_current_stream_capturing
 
 
 def _refuse(t, what: str, shape, dtype, device: int):
@@ -70,12 +72,15 @@ class _Plan:
             raise FwbError(_err(self.lib))
         self._ws: dict[int, torch.Tensor] = {}
 
-    def _workspace(self, stream: int) -> int:
-        """The address of this plan's workspace for a stream."""
+    def _workspace(self, stream: int) -> torch.Tensor:
+        """This plan's workspace for a stream.  A captured call's belongs to its graph, which may be replayed on any
+        stream beside other graphs and calls of this plan: it is not kept here, the graph's memory pool holds it."""
+        if _capturing():
+            return torch.empty(self.workspace_bytes, dtype=torch.uint8, device=f"cuda:{self.device}")
         ws = self._ws.get(stream)
         if ws is None:
             ws = self._ws[stream] = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=f"cuda:{self.device}")
-        return ws.data_ptr()
+        return ws
 
     def _on_device(self) -> None:
         if torch.cuda.current_device() != self.device:
@@ -189,7 +194,8 @@ class PrefixAttention(_Plan):
         a.out, a.lse = out.data_ptr(), lse.data_ptr()
         self._on_device()
         stream = _raw_stream(dev)
-        if self.lib.fwb_prefix_attention_dev(self._ref, self._workspace(stream), self.workspace_bytes, stream) != 0:
+        ws = self._workspace(stream)
+        if self.lib.fwb_prefix_attention_dev(self._ref, ws.data_ptr(), self.workspace_bytes, stream) != 0:
             raise FwbError(_err(self.lib))
         return out, lse
 
@@ -242,9 +248,10 @@ class BeamSelect(_Plan):
             _refuse(token, "token", o, i32, dev)
         self._on_device()
         stream = _raw_stream(dev)
+        ws = self._workspace(stream)
         if self.lib.fwb_beam_select_dev(logits.data_ptr(), *self._sizes, sw, scores.data_ptr(), self.n_select,
                                         out_scores.data_ptr(), parent.data_ptr(), token.data_ptr(),
-                                        self._workspace(stream), self.workspace_bytes, stream) != 0:
+                                        ws.data_ptr(), self.workspace_bytes, stream) != 0:
             raise FwbError(_err(self.lib))
         return out_scores, parent, token
 
