@@ -387,6 +387,33 @@ bool run_select(const BeamSelectArgs &k, cudaStream_t st) {
 }
 
 // --- reordering -------------------------------------------------------------------
+// A state's three levels of runs, widest stride first; levels of one are left
+// out.  false: its runs may overlap one another, each level not reaching past
+// the stride of the next.
+struct ReorderRuns {
+    uint64_t n[3], stride[3], span;  // span: bytes from the first to the last
+    int levels = 0;
+    bool nested(uint64_t run, const size_t (&counts)[3], const size_t (&strides)[3]) {
+        for (int i = 0; i < 3; ++i) {
+            if (counts[i] == 1) continue;
+            int at = levels++;
+            for (; at > 0 && stride[at - 1] < strides[i]; --at) {
+                n[at] = n[at - 1];
+                stride[at] = stride[at - 1];
+            }
+            n[at] = counts[i];
+            stride[at] = strides[i];
+        }
+        span = run;
+        for (int i = levels - 1; i >= 0; --i) {
+            uint64_t over;
+            if (stride[i] < span || __builtin_mul_overflow(n[i] - 1, stride[i], &over) || over > (uint64_t)1 << 62) return false;
+            span += over;
+        }
+        return true;
+    }
+};
+
 template <typename V, int NB>
 bool launch_reorder(const BeamReorderArgs &k, uint64_t n, cudaStream_t st) {
     const uint64_t grid = (n + kBrThreads - 1) / kBrThreads;
@@ -510,12 +537,16 @@ int fwb_beam_reorder_dev(const void *d_src, void *d_dst, const int32_t *d_parent
         fail("fwb_beam_reorder: sizes too large");
         return -1;
     }
-    if ((uintptr_t)d_parent % 4) { fail("fwb_beam_reorder: misaligned parents"); return -1; }
+    ReorderRuns to;
+    if (run_bytes > (uint64_t)1 << 62 ||
+        !to.nested(run_bytes, {n_outer, n_group * n_beam, n_inner}, {dst_outer_stride, dst_slot_stride, dst_inner_stride})) {
+        fail("fwb_beam_reorder: the destination's runs overlap one another");
+        return -1;
+    }
     // the bytes from the first to the last that each side touches
     const size_t src_span = (n_outer - 1) * src_outer_stride + (n_group * n_beam - 1) * src_slot_stride +
                             (n_inner - 1) * src_inner_stride + run_bytes;
-    const size_t dst_span = (n_outer - 1) * dst_outer_stride + (n_group * n_beam - 1) * dst_slot_stride +
-                            (n_inner - 1) * dst_inner_stride + run_bytes;
+    const size_t dst_span = to.span;
     const uintptr_t s0 = (uintptr_t)d_src, d0 = (uintptr_t)d_dst;
     const bool same = s0 == d0 && src_outer_stride == dst_outer_stride && src_slot_stride == dst_slot_stride &&
                       src_inner_stride == dst_inner_stride;
@@ -523,6 +554,7 @@ int fwb_beam_reorder_dev(const void *d_src, void *d_dst, const int32_t *d_parent
         fail("fwb_beam_reorder: source and destination overlap without being the same");
         return -1;
     }
+    if ((uintptr_t)d_parent % 4) { fail("fwb_beam_reorder: misaligned parents"); return -1; }
     BeamReorderArgs k{};
     k.src = static_cast<const uint8_t *>(d_src);
     k.dst = static_cast<uint8_t *>(d_dst);
