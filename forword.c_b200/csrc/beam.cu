@@ -412,6 +412,15 @@ struct ReorderRuns {
         }
         return true;
     }
+    // Whether a state of the same layout, its first run `off` bytes on, shares a byte with this one.
+    bool meets(int64_t off, uint64_t run, int level = 0) const {
+        if (level == levels) return off < (int64_t)run && off > -(int64_t)run;
+        // the two multiples of the stride around it: the smaller levels reach no further than one stride
+        const int64_t st = (int64_t)stride[level], q = off / st - (off % st < 0), most = (int64_t)n[level] - 1;
+        for (int64_t i = q; i <= q + 1; ++i)
+            if (i >= -most && i <= most && meets(off - i * st, run, level + 1)) return true;
+        return false;
+    }
 };
 
 template <typename V, int NB>
@@ -548,9 +557,10 @@ int fwb_beam_reorder_dev(const void *d_src, void *d_dst, const int32_t *d_parent
                             (n_inner - 1) * src_inner_stride + run_bytes;
     const size_t dst_span = to.span;
     const uintptr_t s0 = (uintptr_t)d_src, d0 = (uintptr_t)d_dst;
-    const bool same = s0 == d0 && src_outer_stride == dst_outer_stride && src_slot_stride == dst_slot_stride &&
-                      src_inner_stride == dst_inner_stride;
-    if (!same && s0 < d0 + dst_span && d0 < s0 + src_span) {
+    const bool alike = src_outer_stride == dst_outer_stride && src_slot_stride == dst_slot_stride &&
+                       src_inner_stride == dst_inner_stride;
+    const bool near = s0 < d0 + dst_span && d0 < s0 + src_span;
+    if ((!alike && near) || (alike && near && s0 != d0 && to.meets((int64_t)(d0 - s0), run_bytes))) {
         fail("fwb_beam_reorder: source and destination overlap without being the same");
         return -1;
     }

@@ -231,7 +231,8 @@ size_t fwb_beam_select_workspace(uint32_t type, size_t n_group, size_t n_beam, s
  * dst[o][g * n_beam + b][i] = src[o][g * n_beam + parent[g][b]][i] for runs
  * of run_bytes bytes, o < n_outer, i < n_inner, all strides in bytes.
  * d_dst == d_src with equal strides works in place; otherwise the two must
- * not overlap.  The destination's runs must not overlap one another: sorted,
+ * not overlap: with equal strides, in no byte (one may lie in the other's
+ * gaps); with others, not from first byte to last.  The destination's runs must not overlap one another: sorted,
  * each stride reaches past the runs of the smaller ones.  A parent outside 0..n_beam-1 counts as b itself.  n_beam at
  * most 64.
  */

@@ -25,3 +25,28 @@ def test_a_destination_that_overlaps_itself(lib, state, place):
         bad = {**{k: v for k, v in bad.items() if k[0] == "d"}, "dst": PTR << 20}
     assert lib.fwb_beam_reorder_dev(*{**ARGS, **bad}.values(), None) == -1
     assert "overlap one another" in lib.fwb_last_error().decode()
+
+
+def touched(base, a):
+    return {base + o * a["so"] + s * a["ss"] + i * a["si"] + b for o in range(a["n_outer"])
+            for s in range(a["n_group"] * a["n_beam"]) for i in range(a["n_inner"]) for b in range(a["run"])}
+
+
+@pytest.mark.parametrize("layout", [
+    dict(n_outer=2, n_beam=3, n_inner=2, run=4, so=60, ss=20, si=8), dict(n_outer=3, n_beam=2, n_inner=1, run=4, so=16, ss=8, si=0),
+    dict(n_outer=2, n_beam=3, n_inner=2, run=4, so=8, ss=48, si=20), dict(n_outer=1, n_beam=4, n_inner=3, run=8, so=0, ss=64, si=16),
+], ids=str)
+def test_states_in_each_others_gaps(lib, layout):
+    """Refused exactly where a byte is shared; the others come to the parents' address."""
+    a = {**ARGS, **layout}
+    a.update(do=a["so"], ds=a["ss"], di=a["si"])
+    mine = touched(0, a)
+    seen = set()
+    for off in range(-200, 201):
+        if off == 0:
+            continue
+        meet = bool(mine & touched(off, a))
+        assert lib.fwb_beam_reorder_dev(*{**a, "dst": PTR + off}.values(), None) == -1
+        assert ("overlap" in lib.fwb_last_error().decode()) == meet, off
+        seen.add(meet)
+    assert seen == {False, True}
