@@ -129,18 +129,16 @@ class PrefixAttention(_Plan):
     def __call__(self, q, prefix_k, prefix_v, suffix_k, suffix_v, prefix_len=None, suffix_len=None, slots=None,
                  out=None, lse=None):
         a, dt, dev, seen = self.a, self.dtype, self.device, self._strides
-        st = q.stride()
-        if q.dtype is not dt or q.shape != self._q or q.get_device() != dev or st[3] != 1:
+        if q is None or q.dtype is not dt or q.shape != self._q or q.get_device() != dev or (st := q.stride())[3] != 1:
             _refuse(q, "q", self._q, dt, dev)
         if st != seen[0]:
             a.q_seq_stride, a.q_token_stride, a.q_head_stride, _ = seen[0] = st
         a.q = q.data_ptr()
         if a.prefix_cap:
             k, v, shape = prefix_k, prefix_v, self._p
-            st = k.stride()
-            if k.dtype is not dt or k.shape != shape or k.get_device() != dev or st[3] != 1:
+            if k is None or k.dtype is not dt or k.shape != shape or k.get_device() != dev or (st := k.stride())[3] != 1:
                 _refuse(k, "prefix_k", shape, dt, dev)
-            if v.dtype is not dt or v.shape != shape or v.get_device() != dev:
+            if v is None or v.dtype is not dt or v.shape != shape or v.get_device() != dev:
                 _refuse(v, "prefix_v", shape, dt, dev)
             if v.stride() != st:
                 raise ValueError("prefix_k and prefix_v must have equal strides")
@@ -149,10 +147,9 @@ class PrefixAttention(_Plan):
             a.prefix_k, a.prefix_v = k.data_ptr(), v.data_ptr()
         if a.suffix_cap:
             k, v, shape = suffix_k, suffix_v, self._s
-            st = k.stride()
-            if k.dtype is not dt or k.shape != shape or k.get_device() != dev or st[3] != 1:
+            if k is None or k.dtype is not dt or k.shape != shape or k.get_device() != dev or (st := k.stride())[3] != 1:
                 _refuse(k, "suffix_k", shape, dt, dev)
-            if v.dtype is not dt or v.shape != shape or v.get_device() != dev:
+            if v is None or v.dtype is not dt or v.shape != shape or v.get_device() != dev:
                 _refuse(v, "suffix_v", shape, dt, dev)
             if v.stride() != st:
                 raise ValueError("suffix_k and suffix_v must have equal strides")
@@ -222,16 +219,17 @@ class BeamSelect(_Plan):
 
     def __call__(self, logits, scores, out_scores=None, parent=None, token=None):
         dev, o, f32, i32 = self.device, self._o, torch.float32, torch.int32
-        sg, sw, sv = logits.stride()
         n_group, n_beam, n_vocab = self._x
-        if (logits.dtype is not self.dtype or logits.shape != self._x or logits.get_device() != dev
-                or (sv != 1 and n_vocab > 1)):
+        if (logits is None or logits.dtype is not self.dtype or logits.shape != self._x or logits.get_device() != dev
+                or (logits.stride(2) != 1 and n_vocab > 1)):
             _refuse(logits, "logits", self._x, self.dtype, dev)
+        sg, sw, _ = logits.stride()
         if n_beam == 1:
             sw = sg if n_group > 1 else n_vocab
         elif n_group > 1 and sg != n_beam * sw:
             raise ValueError("logits: all rows must be equally far apart")
-        if scores.dtype is not f32 or scores.shape != self._c or scores.get_device() != dev or not scores.is_contiguous():
+        if (scores is None or scores.dtype is not f32 or scores.shape != self._c or scores.get_device() != dev
+                or not scores.is_contiguous()):
             _refuse(scores, "scores", self._c, f32, dev)
         if out_scores is None:
             out_scores = torch.empty(o, dtype=f32, device=logits.device)
@@ -283,6 +281,8 @@ def reorder(src, parent, dst=None):
     src [n_outer, n_group*n_beam, ...] of any type; views are moved as views
     (the dimensions after the slots must form equally spaced contiguous
     runs).  parent int32 [n_group, n_beam].  dst None: in place."""
+    if src is None or parent is None:
+        raise ValueError("reorder: src or parent is missing")
     if dst is None:
         dst = src
     shape, st, dt, dev = src.shape, src.stride(), dst.stride(), src.get_device()
