@@ -1735,7 +1735,12 @@ struct BeamBuffers {
     }
     template <typename T>
     bool get(T **p, size_t n) {
-        CK(cudaMalloc((void **)p, std::max<size_t>(n, 1) * sizeof(T)));
+        const cudaError_t e = cudaMalloc((void **)p, std::max<size_t>(n, 1) * sizeof(T));
+        if (e != cudaSuccess) {
+            cudaGetLastError();  // or the next call's launch check would find it
+            set_err(std::string("fwb_beam_search: device memory: ") + cudaGetErrorString(e));
+            return false;
+        }
         held.push_back(*p);
         return true;
     }
