@@ -88,14 +88,16 @@ bool attn_args(const fwb_prefix_attn_t *a, BeamAttnArgs &k) {
     if (!a->q || !a->out) return fail("fwb_prefix_attention: null q or out");
     if ((a->prefix_cap && (!a->prefix_k || !a->prefix_v)) || (a->suffix_cap && (!a->suffix_k || !a->suffix_v)))
         return fail("fwb_prefix_attention: null K or V");
-    uint64_t odd = (uintptr_t)a->q | a->q_seq_stride * e | a->q_token_stride * e | a->q_head_stride * e |
-                   (uintptr_t)a->out;
+    auto step = [&](uint64_t n, uint64_t stride) { return n > 1 ? stride * e : 0; };  // (never used where n is 1)
+    const uint64_t seqs = (uint64_t)a->n_group * a->n_beam;
+    uint64_t odd = (uintptr_t)a->q | step(seqs, a->q_seq_stride) | step(a->n_query, a->q_token_stride) |
+                   step(a->n_head, a->q_head_stride) | (uintptr_t)a->out;
     if (a->prefix_cap)
-        odd |= (uintptr_t)a->prefix_k | (uintptr_t)a->prefix_v | a->prefix_group_stride * e |
-               a->prefix_head_stride * e | a->prefix_pos_stride * e;
+        odd |= (uintptr_t)a->prefix_k | (uintptr_t)a->prefix_v | step(a->n_group, a->prefix_group_stride) |
+               step(a->n_head_kv, a->prefix_head_stride) | step(a->prefix_cap, a->prefix_pos_stride);
     if (a->suffix_cap)
-        odd |= (uintptr_t)a->suffix_k | (uintptr_t)a->suffix_v | a->suffix_seq_stride * e |
-               a->suffix_head_stride * e | a->suffix_pos_stride * e;
+        odd |= (uintptr_t)a->suffix_k | (uintptr_t)a->suffix_v | step(seqs, a->suffix_seq_stride) |
+               step(a->n_head_kv, a->suffix_head_stride) | step(a->suffix_cap, a->suffix_pos_stride);
     if (odd % 16) return fail("fwb_prefix_attention: q, K, V and out and their strides must be multiples of 16 bytes");
     if (((uintptr_t)a->lse | (uintptr_t)a->prefix_len | (uintptr_t)a->suffix_len | (uintptr_t)a->slots) % 4)
         return fail("fwb_prefix_attention: lse, lengths and slots must be 4-byte aligned");

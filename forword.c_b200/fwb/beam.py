@@ -60,6 +60,11 @@ def _refuse(t, what: str, shape, dtype, device: int):
                      else f"{what} must be contiguous")
 
 
+def _apart(shape, one, other) -> bool:
+    """Whether the strides of two tensors of this shape differ where they matter."""
+    return any(n > 1 and x != y for n, x, y in zip(shape, one, other))
+
+
 class _Plan:
     def __init__(self, device: int | None, bytes_of):
         self.lib = native.product()
@@ -140,7 +145,7 @@ class PrefixAttention(_Plan):
                 _refuse(k, "prefix_k", shape, dt, dev)
             if v is None or v.dtype is not dt or v.shape != shape or v.get_device() != dev:
                 _refuse(v, "prefix_v", shape, dt, dev)
-            if v.stride() != st:
+            if v.stride() != st and _apart(shape, v.stride(), st):
                 raise ValueError("prefix_k and prefix_v must have equal strides")
             if st != seen[1]:
                 a.prefix_group_stride, a.prefix_head_stride, a.prefix_pos_stride, _ = seen[1] = st
@@ -151,7 +156,7 @@ class PrefixAttention(_Plan):
                 _refuse(k, "suffix_k", shape, dt, dev)
             if v is None or v.dtype is not dt or v.shape != shape or v.get_device() != dev:
                 _refuse(v, "suffix_v", shape, dt, dev)
-            if v.stride() != st:
+            if v.stride() != st and _apart(shape, v.stride(), st):
                 raise ValueError("suffix_k and suffix_v must have equal strides")
             if st != seen[2]:
                 a.suffix_seq_stride, a.suffix_head_stride, a.suffix_pos_stride, _ = seen[2] = st
@@ -176,7 +181,8 @@ class PrefixAttention(_Plan):
         else:
             t = slots
             st = t.stride()
-            if t.dtype is not i32 or t.shape != self._slots or t.get_device() != dev or st[1] != 1:
+            if (t.dtype is not i32 or t.shape != self._slots or t.get_device() != dev
+                    or (st[1] != 1 and a.suffix_cap > 1)):
                 _refuse(t, "slots", self._slots, i32, dev)
             a.slots, a.slots_stride = t.data_ptr(), st[0]
         if out is None:

@@ -152,7 +152,8 @@ int quant_dequant_dev(const void *d_weights, size_t weights_size, uint32_t ggml_
 
 /* Arguments of fwb_prefix_attention_dev.  Strides are in elements, the
  * head_dim values of a row are contiguous; q, K and V addresses and the byte
- * strides of K and V are multiples of 16, those of q too. */
+ * strides of K and V are multiples of 16, those of q too (those of a dimension
+ * of one element are not looked at). */
 typedef struct fwb_prefix_attn {
     uint32_t type;                     /* of q, K, V and out: 0, 1 or 30 */
     uint32_t n_group, n_beam, n_query; /* n_query new tokens per sequence */
