@@ -845,8 +845,11 @@ __global__ void __launch_bounds__(kBaThreads + kBaLoader, sizeof(T) == 4 && RWP 
     if (threadIdx.x >= kBaThreads) {
         uint32_t issued = 0;
         bool ok = true;
+        // stages that 16-byte copies have filled are the copy engine's next
+        const bool mixed = p.tma && (p.tma != 3 || a.slots);
         while (c.left) {
             if (issued >= S && !(ok = mbar_wait_warp(&empty[s], phase ^ 1, &g_beam_err, ERR_WAIT_EMPTY))) break;
+            if (mixed) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             const uint32_t n = beam_take<T, HD>(c);
             beam_load<T, HD>(a, p, maps, c, n, smem + s * 2 * Tl::kBytes, &full[s]);
             ++issued;

@@ -41,3 +41,23 @@ def test_attention_repeats(torch, beam, dtype, pair, broadcast):
         o, l = plan(c["q"], c["pk"], c["pv"], c["sk"], c["sv"], prefix_len=plen, suffix_len=slen)
         differ += (o != out).sum() + (l != lse).sum()
     assert int(differ) == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("W,nq,S", [(4, 1, 500), (3, 2, 333)])
+def test_slots_that_change_by_units(torch, beam, dtype, W, nq, S):
+    """Units of 16 positions from one beam, which the copy engine brings, and units from several, which come row by row,
+    in turn and through the same stages."""
+    c = attn_case(torch, dtype, 2, W, nq, 8, 2, 128, 100, S, slen=[S - i for i in range(2 * W)], seed=S)
+    unit = torch.arange(S, device="cuda") // 16
+    c["slots"] = torch.where(unit % 3 != 1, (unit * 7 // 3) % W, c["slots"]).to(torch.int32)
+    out, lse = attn_check(torch, beam, c)
+    plan = beam.PrefixAttention(n_group=2, n_beam=W, n_query=nq, n_head=8, n_head_kv=2, head_dim=128, dtype=c["q"].dtype,
+                                prefix_cap=100, suffix_cap=S)
+    plen = torch.tensor(c["plen"], dtype=torch.int32, device="cuda")
+    slen = torch.tensor(c["slen"], dtype=torch.int32, device="cuda")
+    differ = torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(100):
+        o, l = plan(c["q"], c["pk"], c["pv"], c["sk"], c["sv"], prefix_len=plen, suffix_len=slen, slots=c["slots"])
+        differ += (o != out).sum() + (l != lse).sum()
+    assert int(differ) == 0
