@@ -12,6 +12,7 @@
 #include "beam_reorder.cuh"
 #include "beam_select.cuh"
 #include "status.h"
+#include "tensor_map.h"
 
 namespace fwb {
 namespace {
@@ -188,22 +189,11 @@ bool attn_layout(const fwb_prefix_attn_t *a, AttnLayout &L) {
     return true;
 }
 
-decltype(&cuTensorMapEncodeTiled) map_encoder() {
-    static const auto fn = [] {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q{};
-        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-                        q == cudaDriverEntryPointSuccess;
-        return ok ? reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(p) : nullptr;
-    }();
-    return fn;
-}
-
 // A cache as a 4-D tensor; false where the copy engine does not take its
 // strides (a head or group repeated by a stride of 0, say).
 bool cache_map(const void *base, size_t e, uint64_t hd, uint64_t cap, uint64_t n_kv, uint64_t outer, uint64_t pos,
                uint64_t head, uint64_t out, uint32_t positions, CUtensorMap &map) {
-    const auto enc = map_encoder();
+    const auto enc = tensor_map_encoder();
     if (!cap || !enc) return false;
     const cuuint64_t dims[4] = {hd, cap, n_kv, outer};
     cuuint64_t strides[3] = {pos * e, head * e, out * e};

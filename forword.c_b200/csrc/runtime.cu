@@ -23,6 +23,7 @@
 #include "gemv.cuh"
 #include "gguf_reader.h"
 #include "status.h"
+#include "tensor_map.h"
 #include "tp_shard.h"
 #include "upload.h"
 #include "decode.cuh"
@@ -1284,20 +1285,6 @@ int quant_matvec_dev(const void *d_weights, size_t weights_size, uint32_t ggml_t
 
 int quant_device_status(void *stream) {
     return device_status(static_cast<cudaStream_t>(stream), "quant_device_status") ? 0 : -1;
-}
-
-// cuTensorMapEncodeTiled from the driver (through the runtime's entry-point
-// query, so the library does not link libcuda itself).
-static decltype(&cuTensorMapEncodeTiled) tensor_map_encoder() {
-    static decltype(&cuTensorMapEncodeTiled) fn = nullptr;
-    if (!fn) {
-        void *p = nullptr;
-        cudaDriverEntryPointQueryResult q{};
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(p);
-    }
-    return fn;
 }
 
 // Tensor-core dequant-GEMM launch (gemm_tc.cuh): Y[m][0..N) (row stride ldy)
