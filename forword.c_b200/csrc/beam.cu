@@ -147,6 +147,9 @@ bool attn_layout(const fwb_prefix_attn_t *a, AttnLayout &L) {
     // 24 / 24, 75 / 50; 128 rows 15 / 23, 25 / 26, 77 / 51; 256 rows 21 / 26,
     // 38 / 33, 138 / 77.  1000 positions cost the one 1 us per 64 rows and the
     // other as much per 128, and the other, two kernels, begins 5 us later.
+    // (Device times of full caches.  The rule goes by the capacity, since the
+    // host does not know the lengths: a cache much longer than what it holds
+    // takes this path for 5 to 8 us more, by these figures.)
     const uint64_t spared = (prows + 63) / 64 - (prows + 127) / 128;
     L.tc = a->type != 0 &&
            (uint64_t)a->n_group * a->n_head_kv * a->prefix_cap * spared >= (uint64_t)36000 * device_sms() / 148;
@@ -265,7 +268,7 @@ bool run_parts(const BeamAttnArgs &k, BeamAttnPlan p, const BeamMaps &maps, cons
     auto join = [&](auto fn, uint32_t blocks, unsigned threads) {
         return launched(launch_after(fn, dim3(blocks), threads, 0, 1, st, k, p), "fwb_prefix_attention launch");
     };
-    // (measured, all of a call in us with 8 / 4 / 1 warps a row: 128 rows of 55
+    // (measured, all of a call on the device in us with 8 / 4 / 1 warps a row: 128 rows of 55
     // segments 30.0 / 31.2 / -, 960 of 10 - / 39.8 / 42.1, 4096 of 6 - / 142.4 / 139.4)
     if (rows <= 4 * sms) return join(beam_attn_join_kernel<T, HD, 8>, rows, kBjThreads<8>);
     if (rows <= 16 * sms) return join(beam_attn_join_kernel<T, HD, 4>, rows, kBjThreads<4>);
@@ -330,9 +333,10 @@ struct SelectLayout {
 // leaves candidates to the join (about 3000 cycles for every 512 slices of
 // 32).  A piece takes a block 1800 cycles, and an SM 825 when its up to five
 // blocks keep the memory busy.  The cheapest count by these figures is taken.
-// Measured: 256 fp32 rows of 128256 in 1 / 2 / 4 / 8 parts a row 45 / 39 / 43 /
-// 48 us (2 taken); 16 bf16 rows in 2 / 5 / 8 / 16 / 32 parts 33 / 24 / 21 / 21
-// / 24 us (8); 4 fp32 rows of 32000 in 2 / 4 / 8 parts 12.3 / 10.1 / 9.0 us (8).
+// Measured on the device: 256 fp32 rows of 128256 in 1 / 2 / 4 / 8 parts a row
+// 45 / 38 / 40 / 45 us (2 taken); 16 bf16 rows in 2 / 5 / 8 / 16 / 32 parts 31 /
+// 23 / 19 / 16 / 17 us (16); 4 fp32 rows of 32000 in 2 / 4 / 8 parts 11.8 / 9.5 /
+// 8.1 us (8).
 void select_layout(size_t n_group, size_t n_beam, size_t n_vocab, size_t n_select, SelectLayout &L) {
     const uint64_t rows = (uint64_t)n_group * n_beam, sms = device_sms(), piece = kBsLogits * kBsThreads;
     L.cap = (uint32_t)((2 * n_select + 16 + 31) / 32 * 32);

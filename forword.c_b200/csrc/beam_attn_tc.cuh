@@ -1,7 +1,8 @@
 // beam_attn_tc.cuh — the prefix part of the shared-prefix attention
 // (beam_attn.cuh) on the 5th-generation tensor cores, for fp16 and bf16 and
 // many rows.  The suffixes, short and with few rows each, stay with
-// beam_attn.cuh's kernel, launched before this one and running beside it.
+// beam_attn.cuh's kernel, launched before this one; a CTA of each does not fit
+// an SM together, so an SM takes up its prefixes when its suffixes are done.
 //
 // The products are transposed: a tile's 128 positions are the M dimension of
 // S^T = K Q^T (N: 128 query rows), and the head's dimensions that of
@@ -19,8 +20,8 @@
 // the exponentials 1024 (16 a cycle and SM), shared memory about 2000 (both
 // operands of both products, the copies, P); measured 4000, with eight softmax
 // warps waiting on one another and on short chains.  64 bf16 samples (512 rows
-// for each of 8 KV heads) over 32763 positions: 134 us with their suffixes, 515
-// TFLOP/s, against 276 with warp-level products.
+// for each of 8 KV heads) over 32763 positions: 135 us on the device with their
+// suffixes, 510 TFLOP/s, against 276 with warp-level products.
 //
 // One CTA per SM: a warp that loads (copy engine), one thread that issues the
 // products, and two groups of four warps for the softmax, each with half of
@@ -330,6 +331,7 @@ __device__ __forceinline__ void bt_step(const BeamAttnArgs &a, const BeamAttnPla
     // these barriers are never two ahead of what was seen
     if (i >= 2) ok = mbar_wait_warp(&t.odone[b], ph ^ 1, &g_beam_err, ERR_WAIT_EMPTY) && ok;
     const uint32_t ps = smem_u32(sm + Sm::kOffP + b * Sm::kP) + key * 128;
+    // (in V's type, as the products take them: beam_tile has what that costs)
 #pragma unroll
     for (int j = 0; j < NC; j += 8) {
         uint32_t w[4];

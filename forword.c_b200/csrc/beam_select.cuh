@@ -317,7 +317,7 @@ __device__ __forceinline__ void beam_add2(float &x0, float &x1, float y0, float 
 // Bound: the logits once from DRAM.  Five blocks per SM with one piece ahead
 // each keep about 80 KB of loads in flight; a logit costs about seven
 // instructions (maximum, 2^x with half of a packed addition and product and one
-// MUFU, half of a packed sum, a compare per four).  256 fp32 rows of 128256: 38 us with the join (3.5 TB/s); the blocks
+// MUFU, half of a packed sum, a compare per four).  256 fp32 rows of 128256: 38 us on the device with the join (3.5 TB/s); the blocks
 // are 3.5 per SM on average and 4 on the busiest.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kBsThreads, 5) beam_select_part_kernel(BeamSelectArgs a) {

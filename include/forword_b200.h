@@ -190,8 +190,8 @@ typedef struct fwb_prefix_attn {
  * are fp32, the probabilities of fp16 and bf16 calls are
  * rounded to that type for the products with V.
  * workspace: fwb_prefix_attention_workspace(a) bytes of device memory,
- * 16-byte aligned, that no other call uses meanwhile; its contents matter to
- * nobody between calls.  -1 with fwb_last_error() for arguments outside the
+ * 16-byte aligned, that no other call uses meanwhile (a captured call's: at
+ * every replay); its contents matter to nobody between calls.  -1 with fwb_last_error() for arguments outside the
  * above.
  */
 int fwb_prefix_attention_dev(const fwb_prefix_attn_t *a, void *workspace, size_t workspace_bytes, void *stream);
@@ -429,10 +429,13 @@ int fwb_tp_shard(const char *gguf_path, const char *tensor, int as_head, int ran
  * and values live in buffers of the call.  A continuation ends with token
  * `eos` (-1: none does) or at max_new tokens; the search ends when n_beam
  * ended ones are found and, without a length penalty, no live one can pass
- * them; live ones that are shorter than max_new then are no results.  Results are sorted by the sum of log-probabilities, divided by
+ * them; live ones that are shorter than max_new then are no results.  Results
+ * are sorted by the sum of log-probabilities, divided by
  * length^length_penalty (0: not divided): tokens_out [n_beam][max_new],
  * lengths_out and scores_out [n_beam] (length 0 and score -inf where there
- * are fewer).  For models on one GPU whose layers and LM head are Q4_0, with
+ * are fewer).  As in fwb_prefill, and unlike the decode step, the inputs of
+ * every weight product are rounded to fp16, the attention's output and the LM
+ * head's input among them.  For models on one GPU whose layers and LM head are Q4_0, with
  * n + max_new <= kv_ctx and n_beam at most 64; -1 otherwise.  Synchronous.
  */
 int fwb_beam_search(fwb_model_t *m, const uint32_t *prompt, size_t n, size_t n_beam, size_t max_new, int64_t eos,
