@@ -1,0 +1,279 @@
+// kv4.cu — C ABI of the paged 4-bit cache: argument checks and launches.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <exception>
+#include <mutex>
+
+#include "../../include/forword_b200.h"
+#include "kv4_append.cuh"
+#include "kv4_attn.cuh"
+#include "launch.h"
+
+namespace fwb {
+namespace {
+
+__device__ uint32_t g_kv4_err;  // kKvBad... bits, until taken
+
+__global__ void kv4_status_kernel(uint32_t *out) { *out = atomicExch(&g_kv4_err, 0u); }
+
+uint32_t *error_word() {
+    static uint32_t *at[64] = {};
+    int dev = 0;
+    if (!launched(cudaGetDevice(&dev), "fwb_kv4")) return nullptr;
+    if (dev < 64 && at[dev]) return at[dev];
+    void *p = nullptr;
+    if (!launched(cudaGetSymbolAddress(&p, g_kv4_err), "fwb_kv4")) return nullptr;
+    if (dev < 64) at[dev] = static_cast<uint32_t *>(p);
+    return static_cast<uint32_t *>(p);
+}
+
+// The error word after the work queued on `st`, cleared in the same step.
+cudaError_t take_status(cudaStream_t st, uint32_t &word) {
+    static std::mutex one;  // look at a time: they share the place that the kernel writes
+    static uint32_t *place = nullptr;
+    const std::lock_guard<std::mutex> lock(one);
+    cudaError_t e = place ? cudaSuccess : cudaHostAlloc(&place, sizeof *place, cudaHostAllocPortable);
+    if (e != cudaSuccess) return e;
+    kv4_status_kernel<<<1, 1, 0, st>>>(place);
+    e = cudaGetLastError();
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e == cudaSuccess) word = *static_cast<volatile uint32_t *>(place);
+    return e;
+}
+
+bool refuse(const char *who, const char *what) {
+    char b[200];
+    snprintf(b, sizeof b, "%s: %s", who, what);
+    return fail(b);
+}
+
+uint32_t log2_of(uint32_t page_size) {
+    uint32_t n = 0;
+    while (1u << n < page_size) ++n;
+    return n;
+}
+
+bool page_ok(const char *who, uint32_t hd, uint32_t page_size) {
+    if (!hd || hd % 16 || hd > 32 * kKvMaxBlocks) return refuse(who, "head_dim must be a multiple of 16, at most 128");
+    if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
+        return refuse(who, "page_size must be 16, 32, 64, 128 or 256");
+    return true;
+}
+
+bool cache_ok(const char *who, uint32_t type, uint32_t n_seq, uint32_t n_tok, uint32_t n_kv, uint32_t hd, uint32_t page_size,
+              uint32_t n_page, uint32_t max_pages) {
+    if (!elem_bytes(type)) return refuse(who, "type must be 0 (F32), 1 (F16) or 30 (BF16)");
+    if (!n_seq || !n_tok || !n_kv || !n_page || !max_pages) return refuse(who, "zero sequences, tokens, heads or pages");
+    if (!page_ok(who, hd, page_size)) return false;
+    if (n_page > 0x7fffffffu || (uint64_t)max_pages * page_size > 0x40000000u)
+        return refuse(who, "more than 2^30 positions in a page table, or too many pages");
+    if (n_kv > 65535 || n_seq > 0xffffffu || (uint64_t)n_seq * n_tok > 0xffffffu)
+        return refuse(who, "too many sequences, tokens or heads");
+    return true;
+}
+
+bool tables_ok(const char *who, const void *cache, const void *pages, const void *a, const void *b) {
+    if (!cache || !pages || !a) return refuse(who, "null cache, pages or lengths");
+    if ((uintptr_t)cache % 16) return refuse(who, "the cache must be 16-byte aligned");
+    if (((uintptr_t)pages | (uintptr_t)a | (uintptr_t)b) % 4) return refuse(who, "tables and lengths must be 4-byte aligned");
+    return true;
+}
+
+// Rows [n_seq][n_tok][heads][head_dim] whose addresses and byte strides are
+// multiples of 16 (those of a dimension of one element are not looked at).
+bool rows_ok(const char *who, uint32_t type, uint32_t n_seq, uint32_t n_tok, uint32_t heads, const Kv4Rows &r) {
+    const uint64_t e = elem_bytes(type);
+    auto step = [&](uint64_t n, uint64_t stride) { return n > 1 ? stride * e : 0; };
+    if (((uintptr_t)r.p | step(n_seq, r.seq) | step(n_tok, r.tok) | step(heads, r.head)) % 16)
+        return refuse(who, "rows and their strides must be multiples of 16 bytes");
+    return true;
+}
+
+// --- attention ---------------------------------------------------------------
+constexpr const char *kAttn = "fwb_kv4_attention";
+
+bool attn_sizes_ok(const fwb_kv4_attn_t *a) {
+    if (!a) return refuse(kAttn, "null arguments");
+    if (!cache_ok(kAttn, a->type, a->n_seq, a->n_query, a->n_head_kv, a->head_dim, a->page_size, a->n_page, a->max_pages)) return false;
+    if (!a->n_head || a->n_head % a->n_head_kv) return refuse(kAttn, "n_head must be a multiple of n_head_kv");
+    if (!(a->scale >= 0.f) || a->scale > 3e38f) return refuse(kAttn, "scale must be positive, or 0 for the default");
+    if (a->n_head > 65535 || (uint64_t)a->n_seq * a->n_query * a->n_head > 0x7fffffffu)
+        return refuse(kAttn, "too many sequences, tokens or heads");
+    return true;
+}
+
+struct AttnLayout {
+    uint32_t nt, nb, rtiles, ctas;  // column tiles of 8 rows, blocks of a row, row tiles, CTAs
+    size_t po, pml, ticket, bytes;
+};
+
+bool attn_layout(const fwb_kv4_attn_t *a, AttnLayout &L) {
+    const uint64_t rows = (uint64_t)a->n_query * (a->n_head / a->n_head_kv);
+    L.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+    L.nb = kv4_blocks(a->head_dim);
+    L.rtiles = (uint32_t)((rows + 8 * L.nt - 1) / (8 * L.nt));
+    const uint64_t units = (uint64_t)a->n_seq * L.rtiles * a->n_head_kv * ((uint64_t)a->max_pages * a->page_size / kKvTile + 64);
+    if (units > 0x7fffffffu) return refuse(kAttn, "too many rows times positions");
+    L.ctas = device_sms() * (L.nt == 1 ? 2 : 1);
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        const size_t here = at;
+        at += (n + 255) & ~(size_t)255;
+        return here;
+    };
+    L.ticket = take(device_sms() * 2 * 4);  // (in the same place for all sizes: it is zero between calls)
+    L.pml = take((size_t)2 * L.ctas * 8 * L.nt * 8);
+    L.po = take((size_t)2 * L.ctas * 8 * L.nt * 32 * L.nb * 4);
+    L.bytes = at;
+    return true;
+}
+
+template <bool SPLIT, int NB, int NT>
+bool launch_attn(const Kv4AttnArgs &k, uint32_t ctas, cudaStream_t st) {
+    static bool ready[64] = {};
+    constexpr uint32_t smem = KaSmem<NB, NT>::kBytes;
+    if (!opt_in(kv4_attn_kernel<SPLIT, NB, NT>, smem, ready, kAttn)) return false;
+    return launched(launch_after(kv4_attn_kernel<SPLIT, NB, NT>, dim3(ctas), kKaThreads, smem, 1, st, k), kAttn);
+}
+
+template <bool SPLIT, int NB>
+bool pick_rows(const Kv4AttnArgs &k, const AttnLayout &L, cudaStream_t st) {
+    return L.nt == 1 ? launch_attn<SPLIT, NB, 1>(k, L.ctas, st)
+         : L.nt == 2 ? launch_attn<SPLIT, NB, 2>(k, L.ctas, st) : launch_attn<SPLIT, NB, 4>(k, L.ctas, st);
+}
+
+template <bool SPLIT>
+bool pick_blocks(const Kv4AttnArgs &k, const AttnLayout &L, cudaStream_t st) {
+    switch (L.nb) {
+    case 1: return pick_rows<SPLIT, 1>(k, L, st);
+    case 2: return pick_rows<SPLIT, 2>(k, L, st);
+    case 3: return pick_rows<SPLIT, 3>(k, L, st);
+    default: return pick_rows<SPLIT, 4>(k, L, st);
+    }
+}
+
+}  // namespace
+}  // namespace fwb
+
+using namespace fwb;
+
+extern "C" {
+
+size_t fwb_kv4_page_bytes(uint32_t head_dim, uint32_t page_size) {
+    return page_ok("fwb_kv4_page_bytes", head_dim, page_size) ? (size_t)page_size / kKvTile * kv4_tile(kv4_blocks(head_dim)) : 0;
+}
+
+int fwb_kv4_status(void *stream) {
+    uint32_t e = 0;
+    try {
+        if (!launched(take_status(static_cast<cudaStream_t>(stream), e), "fwb_kv4_status")) return -1;
+    } catch (const std::exception &) {
+        fail("fwb_kv4_status: the lock failed");
+        return -1;
+    }
+    if (!e) return 0;
+    char b[160];
+    snprintf(b, sizeof b, "fwb_kv4_status:%s%s", e & kKvBadPage ? " a page outside the cache" : "",
+             e & kKvBadPosition ? " a position past the page table or the rotation's tables" : "");
+    fail(b);
+    return -1;
+}
+
+int fwb_kv4_append_dev(const fwb_kv4_append_t *a, void *stream) {
+    constexpr const char *who = "fwb_kv4_append";
+    if (!a) { refuse(who, "null arguments"); return -1; }
+    if (!cache_ok(who, a->type, a->n_seq, a->n_query, a->n_head_kv, a->head_dim, a->page_size, a->n_page, a->max_pages) ||
+        !tables_ok(who, a->cache, a->pages, a->lengths, a->n_new))
+        return -1;
+    if (!a->k || !a->v || !a->q != !a->q_out || (a->q && !a->n_head)) {
+        refuse(who, "null k or v, or only one of q and q_out");
+        return -1;
+    }
+    if (!a->cos != !a->sin || (a->cos && !a->n_pos) || ((uintptr_t)a->cos | (uintptr_t)a->sin) % 16) {
+        refuse(who, "cos and sin must both be given, 16-byte aligned, with n_pos rows, or both be null");
+        return -1;
+    }
+    const uint32_t heads = a->q ? a->n_head : 0;
+    Kv4AppendArgs k{};
+    k.q = {a->q, a->q_seq_stride, a->q_token_stride, a->q_head_stride};
+    k.k = {a->k, a->k_seq_stride, a->k_token_stride, a->k_head_stride};
+    k.v = {a->v, a->v_seq_stride, a->v_token_stride, a->v_head_stride};
+    k.q_out = {a->q_out, a->q_out_seq_stride, a->q_out_token_stride, a->q_out_head_stride};
+    if (!rows_ok(who, a->type, a->n_seq, a->n_query, a->n_head_kv, k.k) || !rows_ok(who, a->type, a->n_seq, a->n_query, a->n_head_kv, k.v) ||
+        (heads && (!rows_ok(who, a->type, a->n_seq, a->n_query, heads, k.q) || !rows_ok(who, a->type, a->n_seq, a->n_query, heads, k.q_out))))
+        return -1;
+    const uint64_t tokens = (uint64_t)a->n_seq * a->n_query, lanes_q = tokens * heads * (a->head_dim / 8),
+                   lanes_kv = tokens * 2 * a->n_head_kv * kv4_blocks(a->head_dim) * 8;
+    if (heads > 65535 || lanes_q > 0xffffff00u || lanes_kv > 0xffffff00u) { refuse(who, "too many tokens or heads"); return -1; }
+    k.cache = static_cast<uint8_t *>(a->cache);
+    k.pages = a->pages; k.len = a->lengths; k.n_new = a->n_new;
+    k.cos = a->cos; k.sin = a->sin;
+    k.pages_seq = a->pages_stride;
+    k.type = a->type; k.n_seq = a->n_seq; k.n_query = a->n_query; k.n_head = heads ? heads : 1; k.n_kv = a->n_head_kv; k.hd = a->head_dim;
+    k.page_log2 = log2_of(a->page_size); k.n_page = a->n_page; k.max_pages = a->max_pages; k.n_pos = a->n_pos; k.halves = a->halves;
+    k.q_blocks = (uint32_t)((lanes_q + kKpThreads - 1) / kKpThreads);
+    if (!(k.err = error_word())) return -1;
+    const uint32_t blocks = k.q_blocks + (uint32_t)((lanes_kv + kKpThreads - 1) / kKpThreads);
+    return launched(launch_after(kv4_append_kernel, dim3(blocks), kKpThreads, 0, 1, static_cast<cudaStream_t>(stream), k), who) ? 0 : -1;
+}
+
+int fwb_kv4_read_dev(const fwb_kv4_read_t *a, void *stream) {
+    constexpr const char *who = "fwb_kv4_read";
+    if (!a) { refuse(who, "null arguments"); return -1; }
+    if (!cache_ok(who, a->type, a->n_seq, a->n, a->n_head_kv, a->head_dim, a->page_size, a->n_page, a->max_pages) ||
+        !tables_ok(who, a->cache, a->pages, a->start, a->lengths))
+        return -1;
+    if (!a->k || !a->v || ((uintptr_t)a->k | (uintptr_t)a->v) % 16) { refuse(who, "null or misaligned k or v"); return -1; }
+    const uint64_t lanes = (uint64_t)a->n_seq * a->n * 2 * a->n_head_kv * (a->head_dim / 4);
+    if (lanes > 0xffffff00u) { refuse(who, "too many positions or heads"); return -1; }
+    Kv4ReadArgs k{};
+    k.cache = static_cast<const uint8_t *>(a->cache);
+    k.pages = a->pages; k.start = a->start; k.len = a->lengths;
+    k.k = a->k; k.v = a->v;
+    k.pages_seq = a->pages_stride;
+    k.type = a->type; k.n_seq = a->n_seq; k.n = a->n; k.n_kv = a->n_head_kv; k.hd = a->head_dim;
+    k.page_log2 = log2_of(a->page_size); k.n_page = a->n_page; k.max_pages = a->max_pages;
+    if (!(k.err = error_word())) return -1;
+    const uint32_t blocks = (uint32_t)((lanes + kKpThreads - 1) / kKpThreads);
+    return launched(launch_after(kv4_read_kernel, dim3(blocks), kKpThreads, 0, 1, static_cast<cudaStream_t>(stream), k), who) ? 0 : -1;
+}
+
+size_t fwb_kv4_attention_workspace(const fwb_kv4_attn_t *a) {
+    AttnLayout L;
+    return attn_sizes_ok(a) && attn_layout(a, L) ? L.bytes : 0;
+}
+
+int fwb_kv4_attention_dev(const fwb_kv4_attn_t *a, void *workspace, size_t workspace_bytes, void *stream) {
+    AttnLayout L;
+    if (!attn_sizes_ok(a) || !attn_layout(a, L) || !tables_ok(kAttn, a->cache, a->pages, a->lengths, a->n_new)) return -1;
+    if (!a->q || !a->out) { refuse(kAttn, "null q or out"); return -1; }
+    if (!rows_ok(kAttn, a->type, a->n_seq, a->n_query, a->n_head, {a->q, a->q_seq_stride, a->q_token_stride, a->q_head_stride})) return -1;
+    if ((uintptr_t)a->out % 16 || (uintptr_t)a->lse % 4) { refuse(kAttn, "out must be 16-byte and lse 4-byte aligned"); return -1; }
+    if (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < L.bytes) {
+        refuse(kAttn, "workspace missing, misaligned or smaller than fwb_kv4_attention_workspace");
+        return -1;
+    }
+    uint8_t *ws = static_cast<uint8_t *>(workspace);
+    Kv4AttnArgs k{};
+    k.q = a->q; k.cache = static_cast<const uint8_t *>(a->cache);
+    k.pages = a->pages; k.len = a->lengths; k.n_new = a->n_new;
+    k.out = a->out; k.lse = a->lse;
+    k.q_seq = a->q_seq_stride; k.q_tok = a->q_token_stride; k.q_head = a->q_head_stride; k.pages_seq = a->pages_stride;
+    k.type = a->type; k.n_seq = a->n_seq; k.n_query = a->n_query; k.n_head = a->n_head; k.n_kv = a->n_head_kv;
+    k.gq = a->n_head / a->n_head_kv; k.hd = a->head_dim;
+    k.tpp_log2 = log2_of(a->page_size) - 4; k.n_page = a->n_page; k.max_pages = a->max_pages;
+    k.rtiles = L.rtiles;
+    k.cost = 8;
+    k.least = 16;
+    k.scale = a->scale != 0.f ? a->scale : 1.0f / sqrtf((float)a->head_dim);
+    k.po = reinterpret_cast<float *>(ws + L.po);
+    k.pml = reinterpret_cast<float2 *>(ws + L.pml);
+    k.ticket = reinterpret_cast<uint32_t *>(ws + L.ticket);
+    if (!(k.err = error_word())) return -1;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return (a->type == 0 ? pick_blocks<true>(k, L, st) : pick_blocks<false>(k, L, st)) ? 0 : -1;
+}
+
+}  // extern "C"

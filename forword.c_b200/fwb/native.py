@@ -104,3 +104,10 @@ def _declare(lib) -> None:
     sig("fwb_beam_status", _i32, _vp)
     sig("fwb_beam_search", _i32, _vp, _c.POINTER(_u32), _sz, _sz, _sz, _c.c_int64, _c.c_float, _c.POINTER(_u32),
         _c.POINTER(_u32), _fp)
+    sig("fwb_kv4_page_bytes", _sz, _u32, _u32)
+    sig("fwb_kv4_status", _i32, _vp)
+    sig("fwb_kv4_append_dev", _i32, _vp, _vp)
+    sig("fwb_kv4_read_dev", _i32, _vp, _vp)
+    sig("fwb_kv4_attention_dev", _i32, _vp, _vp, _sz, _vp)
+    sig("fwb_kv4_attention_workspace", _sz, _vp)
+    sig("fwb_sample_rows_dev", _i32, _vp, _u32, _sz, _sz, _sz, *[_vp] * 8)

@@ -243,6 +243,155 @@ int fwb_beam_reorder_dev(const void *d_src, void *d_dst, const int32_t *d_parent
                          size_t dst_slot_stride, size_t dst_inner_stride, void *stream);
 
 /* ------------------------------------------------------------------------
+ * Several sequences served from one cache of 4-bit pages (no reference
+ * counterpart: forword.c keeps one sequence, in fp32).  As above the
+ * operators take device pointers, run on the current device, enqueue on
+ * `stream`, allocate nothing and may be captured into a CUDA graph.
+ *
+ * The cache is [n_page][n_head_kv] lines of fwb_kv4_page_bytes(head_dim,
+ * page_size) bytes, 16-byte aligned.  A position's keys and values are held in
+ * blocks of 32 values, each with an fp16 scale d and codes 0..15 that stand
+ * for (code - 8) * d: 4.5 bits a value (head_dim is filled up to a multiple of
+ * 32).  Memory that nothing was appended to may hold anything.  pages[s][i]
+ * is the page that holds positions i * page_size .. of sequence s; several
+ * sequences may share pages that they only read.  lengths[s] counts the
+ * positions of a sequence, its new tokens included: token t of n_new[s] (at
+ * most n_query; NULL: n_query each) has position lengths[s] - n_new[s] + t,
+ * and the rows of tokens t >= n_new[s] of a padded batch are neither read nor
+ * written.  page_size is 16, 32, 64, 128 or 256; head_dim a multiple of 16, at
+ * most 128; a page table holds at most 2^30 positions.
+ *
+ * A page outside 0..n_page-1 is neither read nor written: its positions are
+ * not appended, count as not seen, and read as zeros.  The same holds for
+ * positions below 0, and for the append for positions past the page table or
+ * the rotation's tables (a token's q_out row is then not written).  All but
+ * those below 0 set an error word, which fwb_kv4_status takes.
+ * ------------------------------------------------------------------------ */
+
+/* Bytes of a page's line for one head; 0 for sizes that are not taken. */
+size_t fwb_kv4_page_bytes(uint32_t head_dim, uint32_t page_size);
+
+/* Status of the fwb_kv4 calls on the current device since the last look,
+ * after the work queued on `stream` (synchronises it): 0, or -1 if one met a
+ * page or position outside its tables; looking clears it. */
+int fwb_kv4_status(void *stream);
+
+/* Arguments of fwb_kv4_append_dev.  Strides are in elements, the head_dim
+ * values of a row are contiguous; addresses and byte strides of rows are
+ * multiples of 16 (those of a dimension of one element are not looked at). */
+typedef struct fwb_kv4_append {
+    uint32_t type;                      /* of q, k, v and q_out: 0, 1 or 30 */
+    uint32_t n_seq, n_query, n_head, n_head_kv, head_dim;
+    uint32_t page_size, n_page, max_pages; /* max_pages: pages of a row of the table */
+    uint32_t n_pos;                     /* rows of cos and sin */
+    uint32_t halves;                    /* pairs (i, i + head_dim / 2) are turned, not (2i, 2i + 1) */
+    const void *q;                      /* [n_seq][n_query][n_head][head_dim], or NULL (with q_out) */
+    uint64_t q_seq_stride, q_token_stride, q_head_stride;
+    const void *k, *v;                  /* [n_seq][n_query][n_head_kv][head_dim] */
+    uint64_t k_seq_stride, k_token_stride, k_head_stride;
+    uint64_t v_seq_stride, v_token_stride, v_head_stride;
+    void *q_out;                        /* as q; q itself, or memory apart from it */
+    uint64_t q_out_seq_stride, q_out_token_stride, q_out_head_stride;
+    void *cache;
+    const int32_t *pages;               /* [n_seq][max_pages], pages_stride apart */
+    uint64_t pages_stride;
+    const int32_t *lengths, *n_new;     /* [n_seq] */
+    const float *cos, *sin;             /* [n_pos][head_dim / 2], contiguous, 16-byte aligned; NULL: no rotation */
+} fwb_kv4_append_t;
+
+/*
+ * New tokens' queries rotated by position into q_out, their keys rotated and
+ * quantised, their values quantised, into the cache.  (a, b) becomes (a cos -
+ * b sin, a sin + b cos) as in rope.c:28-53.  A block's scale is d = fp16(-m /
+ * 8) for its value m of largest magnitude (the positive one of two), its codes
+ * floor(y / d + 8.5) held to 0..15; a key's y is the fp32 value nearest to the
+ * exact rotation.  Magnitudes past 524032 are held to what the largest fp16
+ * scale reaches; a block with a value that is not finite reads as NaN
+ * throughout.  No two tokens of a call may have the same position of the same
+ * page, and no other work may use that position meanwhile.
+ */
+int fwb_kv4_append_dev(const fwb_kv4_append_t *a, void *stream);
+
+/* Arguments of fwb_kv4_read_dev. */
+typedef struct fwb_kv4_read {
+    uint32_t type;                      /* of k and v */
+    uint32_t n_seq, n, n_head_kv, head_dim;
+    uint32_t page_size, n_page, max_pages;
+    const void *cache;
+    const int32_t *pages;
+    uint64_t pages_stride;
+    const int32_t *start;               /* [n_seq] */
+    const int32_t *lengths;             /* [n_seq], or NULL: no limit but the page table */
+    void *k, *v;                        /* [n_seq][n][n_head_kv][head_dim], contiguous */
+} fwb_kv4_read_t;
+
+/*
+ * What the cache holds at positions start[s] .. start[s] + n - 1, rounded once
+ * to the type (fwb_kv_read's counterpart; row order [n][n_head_kv][head_dim]).
+ * Zeros below position 0 and at and past a length or the page table.
+ */
+int fwb_kv4_read_dev(const fwb_kv4_read_t *a, void *stream);
+
+/* Arguments of fwb_kv4_attention_dev (strides as in fwb_kv4_append_t). */
+typedef struct fwb_kv4_attn {
+    uint32_t type;                      /* of q and out: 0, 1 or 30 */
+    uint32_t n_seq, n_query, n_head, n_head_kv, head_dim; /* n_head a multiple of n_head_kv */
+    uint32_t page_size, n_page, max_pages;
+    float scale;                        /* of the scores, positive; 0 -> 1/sqrt(head_dim) */
+    const void *q;                      /* [n_seq][n_query][n_head][head_dim] */
+    uint64_t q_seq_stride, q_token_stride, q_head_stride;
+    const void *cache;
+    const int32_t *pages;               /* [n_seq][max_pages], pages_stride apart */
+    uint64_t pages_stride;
+    const int32_t *lengths, *n_new;     /* [n_seq]; held to 0..max_pages * page_size and 0..n_query */
+    void *out;                          /* [n_seq][n_query][n_head][head_dim], contiguous */
+    float *lse;                         /* [n_seq][n_query][n_head], or NULL */
+} fwb_kv4_attn_t;
+
+/*
+ * Attention of every sequence's new tokens over its pages: token t of n_new
+ * sees the first lengths[s] - (n_new[s] - 1 - t) positions.  lse receives log
+ * sum exp of the scaled scores.  A token that sees no position gets out 0 and
+ * lse -inf; one whose query is not finite, or that sees a NaN key or value,
+ * gets NaN; what lies past the positions that a token sees reaches it in no
+ * way.  fp16 and bf16 queries are exact in the products, weighted
+ * probabilities are rounded to fp16; fp32 calls carry 22 bits of both.
+ * workspace: fwb_kv4_attention_workspace(a) bytes of device memory, 16-byte
+ * aligned, that no other call uses meanwhile (a captured call's: at every
+ * replay).  It must be all zeros before its first use; calls leave it fit for
+ * the next one, of any sizes.
+ */
+int fwb_kv4_attention_dev(const fwb_kv4_attn_t *a, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Bytes of workspace that fwb_kv4_attention_dev needs for a's type and sizes
+ * (its pointers, lengths and strides are not looked at); 0 with
+ * fwb_last_error() for sizes that it does not take. */
+size_t fwb_kv4_attention_workspace(const fwb_kv4_attn_t *a);
+
+/*
+ * A token for each of n_row rows of logits (fwb_sample's counterpart for many
+ * rows and given random numbers).  d_logits holds rows of n_vocab elements of
+ * `type`, row_stride elements apart.  Of a row, ranked by logit and among
+ * equals by the lower index, with weights exp((logit - max) / temperature):
+ * the first top_k stay (0 or less: all); of these, the ones before which less
+ * than top_p of their mass lies (1 or more: all); of these, the ones of weight
+ * at least min_p; the first one always.  The token is the first whose running
+ * mass among them exceeds d_uniform * their mass (the last of them from 1 on).
+ * d_logprob (may be NULL) receives the log of its share of their mass.
+ * d_temperature, d_top_k, d_top_p and d_min_p hold a value for each row; NULL:
+ * 1, 0, 1 and 0.  A temperature of 0 or less takes the largest logit (log 1).
+ * A logit of -inf bars its token.  A row that holds a NaN or +inf, is barred
+ * throughout, or has a temperature or uniform number that is NaN gets token -1
+ * and -inf.  Entries of weight below 2^-64 count as nothing, neither for top_k
+ * nor in a mass.  Weights carry 22 bits and are added exactly, so a token can
+ * differ from exact arithmetic's only where a limit falls within about 2^-22
+ * of the mass of a border.  n_vocab at most 262144.
+ */
+int fwb_sample_rows_dev(const void *d_logits, uint32_t type, size_t n_row, size_t n_vocab, size_t row_stride,
+                        const float *d_uniform, const float *d_temperature, const int32_t *d_top_k, const float *d_top_p,
+                        const float *d_min_p, int32_t *d_token, float *d_logprob, void *stream);
+
+/* ------------------------------------------------------------------------
  * Decode model (transformer.h:39-48 semantics).
  * ------------------------------------------------------------------------ */
 
