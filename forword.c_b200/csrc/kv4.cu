@@ -133,7 +133,7 @@ bool attn_layout(const fwb_kv4_attn_t *a, AttnLayout &L) {
 template <bool SPLIT, int NB, int NT>
 bool launch_attn(const Kv4AttnArgs &k, uint32_t ctas, cudaStream_t st) {
     static bool ready[64] = {};
-    constexpr uint32_t smem = KaSmem<NB, NT>::kBytes;
+    constexpr uint32_t smem = KaSmem<SPLIT, NB, NT>::kBytes;
     if (!opt_in(kv4_attn_kernel<SPLIT, NB, NT>, smem, ready, kAttn)) return false;
     return launched(launch_after(kv4_attn_kernel<SPLIT, NB, NT>, dim3(ctas), kKaThreads, smem, 1, st, k), kAttn);
 }
@@ -265,8 +265,16 @@ int fwb_kv4_attention_dev(const fwb_kv4_attn_t *a, void *workspace, size_t works
     k.gq = a->n_head / a->n_head_kv; k.hd = a->head_dim;
     k.tpp_log2 = log2_of(a->page_size) - 4; k.n_page = a->n_page; k.max_pages = a->max_pages;
     k.rtiles = L.rtiles;
-    k.cost = 8;
+    // How the line is cut, in pairs of tiles.  Measured (us on the device): an
+    // item's ends counted as 8 / 16 / 24 / 32 pairs, 64 sequences of up to 8191
+    // 110 / 87 / 81 / 83; parts of at least 16 / 24 / 40 pairs, one sequence of
+    // 4000 positions 11.9 / 15.3 / 16.3, of 16000 15.9 / 18.3 / 17.1; items of up
+    // to 48 pairs left whole where there is a CTA for each: 1000 positions 11.3,
+    // cut 13.0 (2000: whole 16.3, cut 12.3).
+    k.cost = 24;
+    k.snap = 8;
     k.least = 16;
+    k.whole = 48;
     k.scale = a->scale != 0.f ? a->scale : 1.0f / sqrtf((float)a->head_dim);
     k.po = reinterpret_cast<float *>(ws + L.po);
     k.pml = reinterpret_cast<float2 *>(ws + L.pml);

@@ -29,9 +29,11 @@
 
 namespace fwb {
 
-constexpr int kKaWarps = 8, kKaThreads = 32 * kKaWarps, kKaStages = 4;
-constexpr float kKaLazy = 7.f;  // log2 of how far a score may exceed its row's reference
-constexpr float kKaHead = 256.f;  // largest product of a probability and a scale when references are exact
+constexpr int kKaWarps = 8, kKaThreads = 32 * kKaWarps, kKaStages = 3;
+constexpr uint32_t kKaPair = 2 * kKvTile;  // positions that a warp takes at a time
+// Weights are formed as 2^8 exp2(score - reference), and a reference is raised
+// when a score exceeds it by 2^7: they stay below 2^15, which fp16 holds.
+constexpr float kKaHead = 8.f, kKaLazy = 7.f;
 
 struct Kv4AttnArgs {
     const void *q;
@@ -42,7 +44,8 @@ struct Kv4AttnArgs {
     uint64_t q_seq, q_tok, q_head, pages_seq;  // strides in elements
     uint32_t type, n_seq, n_query, n_head, n_kv, gq, hd;
     uint32_t tpp_log2, n_page, max_pages;  // tiles of a page
-    uint32_t rtiles, cost, least;          // row tiles; units of an item's ends; units worth a CTA
+    uint32_t rtiles;                       // row tiles
+    uint32_t cost, snap, least, whole;     // of an item's ends; see ka_cut; worth a CTA; not worth cutting (pairs of tiles)
     float scale;
     float *po;        // [2 CTAs][rows][32 NB] parts of cut items
     float2 *pml;      // [2 CTAs][rows] their references and sums
@@ -55,10 +58,14 @@ __device__ __forceinline__ float ka_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ void ka_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ void ka_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1,
+                                       float c2, float c3) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+__device__ __forceinline__ void ka_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    ka_mma(d, a, b0, b1, d[0], d[1], d[2], d[3]);
 }
 // The 8x8 halves that a warp holds as rows, as columns.
 __device__ __forceinline__ uint32_t ka_transpose(uint32_t x) {
@@ -66,18 +73,18 @@ __device__ __forceinline__ uint32_t ka_transpose(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-// The codes less 8 of nibbles (0, 4), (1, 5), (2, 6), (3, 7) as pairs of
-// halves: 0x6400 is 1024, whose last bit is worth 1 (16 for the upper nibble
-// of a byte), so 1024 + q and 1024 + 16 q need only their mask, and each
-// subtraction or fma is exact.
+// (code - 8) * 2^-9 of nibbles (0, 4), (1, 5), (2, 6), (3, 7) as pairs of
+// halves.  A nibble in the low bits of a half is the subnormal code * 2^-24 (16
+// times that in bits 4..7), so it needs its mask and one fma, which is exact.
+constexpr float kKaCode = 512.f;
 __device__ __forceinline__ void ka_codes(uint32_t w, uint32_t (&h)[4]) {
-    const __half2 k1032 = __half2half2(__ushort_as_half(0x6408)), k16 = __half2half2(__ushort_as_half(0x2c00)),
-                  k72 = __half2half2(__ushort_as_half(0xd480));
+    const __half2 up = __half2half2(__ushort_as_half(0x7800)), up16 = __half2half2(__ushort_as_half(0x6800)),
+                  eight = __half2half2(__ushort_as_half(0xa400));  // 2^15, 2^11, -2^-6
 #pragma unroll
     for (int i = 0; i < 2; ++i, w >>= 8) {
-        const uint32_t lo = (w & 0x000f000fu) | 0x64006400u, hi = (w & 0x00f000f0u) | 0x64006400u;
-        const __half2 a = __hsub2(*reinterpret_cast<const __half2 *>(&lo), k1032),
-                      b = __hfma2(*reinterpret_cast<const __half2 *>(&hi), k16, k72);
+        const uint32_t lo = w & 0x000f000fu, hi = w & 0x00f000f0u;
+        const __half2 a = __hfma2(*reinterpret_cast<const __half2 *>(&lo), up, eight),
+                      b = __hfma2(*reinterpret_cast<const __half2 *>(&hi), up16, eight);
         h[2 * i] = *reinterpret_cast<const uint32_t *>(&a);
         h[2 * i + 1] = *reinterpret_cast<const uint32_t *>(&b);
     }
@@ -138,80 +145,132 @@ __device__ __forceinline__ bool ka_tiles(const Kv4AttnArgs &a, uint32_t rt, int3
     return true;
 }
 
-template <int NB, int NT>
+template <bool SPLIT, int NB, int NT>
 struct KaSmem {
-    static constexpr uint32_t kRows = 8 * NT, kTile = kv4_tile(NB), kStride = 32 * NB + 4;
-    static constexpr uint32_t kRing = kKaWarps * kKaStages * kTile, kJoin = kKaWarps * kRows * kStride * 4;
-    static constexpr uint32_t kBytes = kRing > kJoin ? kRing : kJoin;
+    static constexpr uint32_t kRows = 8 * NT, kTile = kv4_tile(NB), kStage = 2 * kTile, kStride = 32 * NB + 4;
+    static constexpr uint32_t kRing = kKaWarps * kKaStages * kStage, kJoin = kKaWarps * kRows * kStride * 4;
+    static constexpr uint32_t kQueries = NT * NB * (SPLIT ? 2 : 1) * 32 * 16;  // after the ring
+    static constexpr uint32_t kRingBytes = kRing > kJoin ? kRing : kJoin, kBytes = kRingBytes + kQueries;
 };
 
-// One tile of 16 positions.  EDGE: some rows may not see all of them.
+// Where the line's even cuts fall within an item of `units` units: one in its
+// first `head` + 1 moves to its beginning, one at `tail` or later to its end.
+struct KaCut {
+    uint32_t head, tail;
+};
+__device__ __forceinline__ KaCut ka_cut(uint32_t units, uint32_t snap) {
+    const uint32_t head = min(snap, units / 2);
+    return {head, max(units > snap ? units - snap : 0u, head + 1)};
+}
+
+// Two tiles of 16 positions.  Keys' codes go into the products as they lie,
+// under a mask: a nibble in the low bits of a half is the subnormal code * 2^-24
+// (16 times that in bits 4..7), so a pair costs one instruction, and the sums
+// begin at -8 in every place.  Values, whose sums run on, and all codes of fp32
+// calls (the tensor cores' sums truncate at their largest term: 3e-6 of the
+// result instead of 3e-7) are unpacked to code - 8.  EDGE: some rows may not see all of them, or a
+// tile is not there.  q: the queries' B operand [n][hi, lo][b] for each lane in shared memory (NT > 1); r: in registers.
 template <bool SPLIT, int NB, int NT, bool EDGE>
-__device__ __forceinline__ void ka_tile(const uint8_t *tile, const uint32_t (&qh)[NT][NB][4], const uint32_t (&ql)[SPLIT ? NT : 1][NB][4],
-                                        const float (&qs)[NT][2], const int32_t (&lim)[NT][2], int32_t pos0, int32_t limit,
-                                        float (&o)[NT][NB][2][4], float (&m)[NT][2], float (&l)[NT][2], float &vref) {
+__device__ __forceinline__ void ka_pair(const uint8_t *pair, const uint4 *sq, 
+                                        const float *soff, const float (&qs)[NT][2], const int32_t (&lim)[NT][2],
+                                        const int32_t (&limt)[NT], int32_t pos0, int32_t limit, uint32_t there,
+                                        float (&o)[NT][NB][2][4], float (&mm)[NT][2], float (&thr)[NT][2], float (&l)[NT][2],
+                                        float &vref) {
+    constexpr uint32_t TB = kv4_tile(NB);
     const uint32_t lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const uint32_t p0 = (g >> 1) + 4 * (g & 1), p1 = p0 + 8;  // the positions of this lane's rows of the scores
-    float s[NT][4];
+    float s[2][NT][4];
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[h][n][0] = s[h][n][1] = s[h][n][2] = s[h][n][3] = 0.f;
     {
-        uint32_t w0[NB], w1[NB], d0[(NB + 1) / 2], d1[(NB + 1) / 2];
-        ka_words<NB>(tile + p0 * 16 * NB + c * 4 * NB, w0);
-        ka_words<NB>(tile + p1 * 16 * NB + c * 4 * NB, w1);
-        ka_halves<NB>(tile + kv4_codes(NB) + p0 * 2 * NB, d0);
-        ka_halves<NB>(tile + kv4_codes(NB) + p1 * 2 * NB, d1);
+        uint32_t w0[2][NB], w1[2][NB], d0[2][(NB + 1) / 2], d1[2][(NB + 1) / 2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint8_t *tile = pair + h * TB;
+            ka_words<NB>(tile + p0 * 16 * NB + c * 4 * NB, w0[h]);
+            ka_words<NB>(tile + p1 * 16 * NB + c * 4 * NB, w1[h]);
+            ka_halves<NB>(tile + kv4_codes(NB) + p0 * 2 * NB, d0[h]);
+            ka_halves<NB>(tile + kv4_codes(NB) + p1 * 2 * NB, d1[h]);
+        }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            uint32_t x[4], y[4];
-            ka_codes(w0[b], x);
-            ka_codes(w1[b], y);
-            const float2 e0 = kv4_unpack(d0[b / 2]), e1 = kv4_unpack(d1[b / 2]);
-            const float k0 = b % 2 ? e0.y : e0.x, k1 = b % 2 ? e1.y : e1.x;
-            const uint32_t a0[4] = {x[0], y[0], x[1], y[1]}, a1[4] = {x[2], y[2], x[3], y[3]};
+            uint32_t a0[2][4], a1[2][4];
+            float k0[2], k1[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if constexpr (SPLIT) {
+                    uint32_t x[4], y[4];
+                    ka_codes(w0[h][b], x);
+                    ka_codes(w1[h][b], y);
+                    a0[h][0] = x[0]; a0[h][1] = y[0]; a0[h][2] = x[1]; a0[h][3] = y[1];
+                    a1[h][0] = x[2]; a1[h][1] = y[2]; a1[h][2] = x[3]; a1[h][3] = y[3];
+                } else {
+                    const uint32_t x = w0[h][b], y = w1[h][b];
+                    a0[h][0] = x & 0x000f000fu; a0[h][1] = y & 0x000f000fu;
+                    a0[h][2] = x & 0x00f000f0u; a0[h][3] = y & 0x00f000f0u;
+                    a1[h][0] = x >> 8 & 0x000f000fu; a1[h][1] = y >> 8 & 0x000f000fu;
+                    a1[h][2] = x >> 8 & 0x00f000f0u; a1[h][3] = y >> 8 & 0x00f000f0u;
+                }
+                const float2 e0 = kv4_unpack(d0[h][b / 2]), e1 = kv4_unpack(d1[h][b / 2]);
+                k0[h] = b % 2 ? e0.y : e0.x;
+                k1[h] = b % 2 ? e1.y : e1.x;
+            }
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                if constexpr (SPLIT) {
-                    ka_mma(acc, a0, ql[n][b][0], ql[n][b][1]);
-                    ka_mma(acc, a1, ql[n][b][2], ql[n][b][3]);
+                uint4 q, r = {};
+                float2 off = {};
+                {
+                    if constexpr (!SPLIT) off = *reinterpret_cast<const float2 *>(soff + (n * NB + b) * 8 + 2 * c);
+                    q = sq[((n * (SPLIT ? 2 : 1)) * NB + b) * 32 + lane];
+                    if constexpr (SPLIT) r = sq[((n * 2 + 1) * NB + b) * 32 + lane];
                 }
-                ka_mma(acc, a0, qh[n][b][0], qh[n][b][1]);
-                ka_mma(acc, a1, qh[n][b][2], qh[n][b][3]);
-                s[n][0] = fmaf(k0, acc[0], s[n][0]);
-                s[n][1] = fmaf(k0, acc[1], s[n][1]);
-                s[n][2] = fmaf(k1, acc[2], s[n][2]);
-                s[n][3] = fmaf(k1, acc[3], s[n][3]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float acc[4];
+                    if constexpr (SPLIT) {
+                        ka_mma(acc, a0[h], r.x, r.y, 0.f, 0.f, 0.f, 0.f);
+                        ka_mma(acc, a1[h], r.z, r.w);
+                        ka_mma(acc, a0[h], q.x, q.y);
+                    } else {
+                        ka_mma(acc, a0[h], q.x, q.y, off.x, off.y, off.x, off.y);
+                    }
+                    ka_mma(acc, a1[h], q.z, q.w);
+                    s[h][n][0] = fmaf(k0[h], acc[0], s[h][n][0]);
+                    s[h][n][1] = fmaf(k0[h], acc[1], s[h][n][1]);
+                    s[h][n][2] = fmaf(k1[h], acc[2], s[h][n][2]);
+                    s[h][n][3] = fmaf(k1[h], acc[3], s[h][n][3]);
+                }
             }
         }
     }
-    bool seen[NT][4];
     bool raise = false;
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            s[n][i] *= qs[n][i & 1];
-            if constexpr (EDGE) {
-                seen[n][i] = pos0 + (int32_t)(i < 2 ? p0 : p1) < lim[n][i & 1];
-                if (!seen[n][i]) s[n][i] = -INFINITY;
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (EDGE)
+                    if (!(there >> h & 1) || pos0 + (int32_t)(16 * h + (i < 2 ? p0 : p1)) >= lim[n][i & 1]) s[h][n][i] = -INFINITY;
+                raise |= s[h][n][i] > thr[n][i & 1];
             }
-            raise |= s[n][i] > m[n][i & 1] + kKaLazy;
-        }
-    // References follow the scores only when one exceeds its own by 2^7: the
-    // products below stay under 2^15, which fp16 holds.
+    // References follow the scores only when one exceeds its own by 2^7.
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                float top = fmaxf(s[n][j], s[n][j + 2]);
+                float top = fmaxf(fmaxf(s[0][n][j], s[0][n][j + 2]), fmaxf(s[1][n][j], s[1][n][j + 2]));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                if (top > m[n][j]) {
-                    const float f = ka_exp2(m[n][j] - top);
-                    m[n][j] = top;
+                top *= qs[n][j];
+                if (top > (thr[n][j] == -INFINITY ? -INFINITY : mm[n][j] + kKaHead)) {
+                    const float now = top - kKaHead, f = thr[n][j] == -INFINITY ? 0.f : ka_exp2(mm[n][j] - now);
+                    mm[n][j] = now;
+                    thr[n][j] = (top + kKaLazy) / qs[n][j];
                     l[n][j] *= f;
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
@@ -224,143 +283,217 @@ __device__ __forceinline__ void ka_tile(const uint8_t *tile, const uint32_t (&qh
             }
     }
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float ref = m[n][j] == -INFINITY ? 0.f : m[n][j];  // nothing seen yet: every score is -inf
-            s[n][j] = ka_exp2(s[n][j] - ref);
-            s[n][j + 2] = ka_exp2(s[n][j + 2] - ref);
-            l[n][j] += s[n][j] + s[n][j + 2];
-        }
-    const uint8_t *vt = tile + kv4_codes(NB) + kv4_scales(NB);
-    // The values' scales relative to the largest so far (as a power of two).
-    float v0[NB], v1[NB];
-    {
-        uint32_t d0[(NB + 1) / 2], d1[(NB + 1) / 2];
-        ka_halves<NB>(vt + kv4_codes(NB) + p0 * 2 * NB, d0);
-        ka_halves<NB>(vt + kv4_codes(NB) + p1 * 2 * NB, d1);
-        float top = 0.f;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const float2 e0 = kv4_unpack(d0[b / 2]), e1 = kv4_unpack(d1[b / 2]);
-            v0[b] = b % 2 ? e0.y : e0.x;
-            v1[b] = b % 2 ? e1.y : e1.x;
-            if constexpr (EDGE) {  // past the last row's positions lies anything
-                if (pos0 + (int32_t)p0 >= limit) v0[b] = 0.f;
-                if (pos0 + (int32_t)p1 >= limit) v1[b] = 0.f;
+            for (int i = 0; i < 4; ++i) {
+                float p = ka_exp2(fmaf(s[h][n][i], qs[n][i & 1], -mm[n][i & 1]));
+                if constexpr (EDGE)
+                    if (s[h][n][i] == -INFINITY) p = 0.f;
+                s[h][n][i] = p;
+                l[n][i & 1] += p;
             }
-            top = fmaxf(top, fmaxf(fabsf(v0[b]), fabsf(v1[b])));
+    // The values' scales; what lies past the last row's positions is anything.
+    uint32_t v[2][NB][2];  // of positions (c, c + 4) and (c + 8, c + 12): the rows of the transposed weights
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint8_t *vd = pair + h * TB + 2 * kv4_codes(NB) + kv4_scales(NB);
+        uint32_t d[4][(NB + 1) / 2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ka_halves<NB>(vd + (c + 4 * j) * 2 * NB, d[j]);
+        uint32_t m0 = 0xffffffffu, m1 = 0xffffffffu;
+        if constexpr (EDGE) {
+            const int32_t left = there >> h & 1 ? limit - pos0 - (int32_t)(16 * h + c) : 0;
+            m0 = (left > 0 ? 0xffffu : 0u) | (left > 4 ? 0xffff0000u : 0u);
+            m1 = (left > 8 ? 0xffffu : 0u) | (left > 12 ? 0xffff0000u : 0u);
         }
-        if (__any_sync(0xffffffffu, top > vref)) {
-            const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(fminf(top, 65536.f)));
-            const float now = fmaxf(vref, __uint_as_float((bits + 0x7fffffu) & 0xff800000u));
-            const float f = vref * __uint_as_float((254u << 23) - __float_as_uint(now));  // of powers of two
-            vref = now;
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) o[n][b][t][i] *= f;
-        }
-        // kKaHead / vref
-        const float inv = __uint_as_float(((254u + 8u) << 23) - __float_as_uint(vref));
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            v0[b] *= inv;
-            v1[b] *= inv;
+            const uint32_t pick = b % 2 ? 0x7632u : 0x5410u;
+            v[h][b][0] = __byte_perm(d[0][b / 2], d[1][b / 2], pick) & m0;
+            v[h][b][1] = __byte_perm(d[2][b / 2], d[3][b / 2], pick) & m1;
         }
     }
-    uint32_t u[4][(NB + 1) / 2];
+    // They go into the products relative to vref, a power of two not below the
+    // largest so far (each lane looks at a word of each tile's scales).
+    float top = 0.f;
+    if (lane < 8 * NB)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) ka_halves<NB>(vt + (c + 4 * j) * 16 * NB + (g ^ (c & 2 ? 4u : 0u)) * 2 * NB, u[j]);
+        for (int h = 0; h < 2; ++h) {
+            uint32_t word = *reinterpret_cast<const uint32_t *>(pair + h * TB + 2 * kv4_codes(NB) + kv4_scales(NB) + 4 * lane);
+            if constexpr (EDGE) {
+                const int32_t left = there >> h & 1 ? limit - pos0 - 16 * h : 0;
+                if ((int32_t)(2 * lane / NB) >= left) word = 0;
+                if ((int32_t)((2 * lane + 1) / NB) >= left) word &= 0xffffu;
+            }
+            const float2 f = kv4_unpack(word);
+            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+    if (__any_sync(0xffffffffu, top > vref)) {
+        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(fminf(top, 65536.f)));
+        const float now = fmaxf(vref, __uint_as_float((bits + 0x7fffffu) & 0xff800000u));
+        const float f = vref * __uint_as_float((254u << 23) - __float_as_uint(now));  // of powers of two
+        vref = now;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        const uint32_t pick = b % 2 ? 0x7632u : 0x5410u;
-        uint32_t x[4], y[4];
-        ka_codes(__byte_perm(u[0][b / 2], u[1][b / 2], pick), x);
-        ka_codes(__byte_perm(u[2][b / 2], u[3][b / 2], pick), y);
-        const uint32_t a0[4] = {x[0], x[1], y[0], y[1]}, a1[4] = {x[2], x[3], y[2], y[3]};
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            float w[4] = {s[n][0] * v0[b], s[n][1] * v0[b], s[n][2] * v1[b], s[n][3] * v1[b]};
-            if constexpr (EDGE)
+            for (int b = 0; b < NB; ++b)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (!seen[n][i]) w[i] = 0.f;  // (its scale may be NaN)
-            const uint32_t h0 = kv4_pack(w[0], w[1]), h1 = kv4_pack(w[2], w[3]);
-            const uint32_t b0 = ka_transpose(h0), b1 = ka_transpose(h1);
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[n][b][t][i] *= f;
+    }
+    const float inv = __uint_as_float((254u << 23) - __float_as_uint(vref));  // 1 / vref, at most 2^14
+    const __half2 inv2 = __half2half2(__float2half_rn(inv));
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        // the weights' transposes: rows as columns g, positions as above
+        uint32_t w[NT][2], rest[NT][2];  // in two halves
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const uint32_t x = kv4_pack(s[h][n][2 * e], s[h][n][2 * e + 1]);
+                const float2 f = kv4_unpack(x);
+                w[n][e] = ka_transpose(x);
+                rest[n][e] = ka_transpose(kv4_pack(s[h][n][2 * e] - f.x, s[h][n][2 * e + 1] - f.y));
+            }
+        uint32_t mask[NT][2];
+        if constexpr (EDGE)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int32_t left = there >> h & 1 ? limt[n] - pos0 - (int32_t)(16 * h + c) : 0;
+                mask[n][0] = (left > 0 ? 0xffffu : 0u) | (left > 4 ? 0xffff0000u : 0u);
+                mask[n][1] = (left > 8 ? 0xffffu : 0u) | (left > 12 ? 0xffff0000u : 0u);
+            }
+        const uint8_t *vt = pair + h * TB + kv4_codes(NB) + kv4_scales(NB);
+        uint32_t u[4][(NB + 1) / 2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ka_halves<NB>(vt + (c + 4 * j) * 16 * NB + (g ^ (c & 2 ? 4u : 0u)) * 2 * NB, u[j]);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const uint32_t pick = b % 2 ? 0x7632u : 0x5410u;
+            uint32_t x[4], y[4];
+            ka_codes(__byte_perm(u[0][b / 2], u[1][b / 2], pick), x);
+            ka_codes(__byte_perm(u[2][b / 2], u[3][b / 2], pick), y);
+            const uint32_t a0[4] = {x[0], x[1], y[0], y[1]}, a1[4] = {x[2], x[3], y[2], y[3]};
             if constexpr (SPLIT) {
-                // The rest of each product as a second half, and sums of 16
+                // Each weight times its scale in two halves, and sums of 16
                 // positions added in rounded fp32: the tensor cores' own
                 // additions truncate.
-                const float2 f0 = kv4_unpack(h0), f1 = kv4_unpack(h1);
-                const uint32_t r0 = ka_transpose(kv4_pack(w[0] - f0.x, w[1] - f0.y)),
-                               r1 = ka_transpose(kv4_pack(w[2] - f1.x, w[3] - f1.y));
-                float t0[4] = {0.f, 0.f, 0.f, 0.f}, t1[4] = {0.f, 0.f, 0.f, 0.f};
-                ka_mma(t0, a0, r0, r1);
-                ka_mma(t1, a1, r0, r1);
-                ka_mma(t0, a0, b0, b1);
-                ka_mma(t1, a1, b0, b1);
+                const float2 v0 = kv4_unpack(v[h][b][0]), v1 = kv4_unpack(v[h][b][1]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    o[n][b][0][i] += t0[i];
-                    o[n][b][1][i] += t1[i];
+                for (int n = 0; n < NT; ++n) {
+                    const float2 x0 = kv4_unpack(w[n][0]), x1 = kv4_unpack(w[n][1]), y0 = kv4_unpack(rest[n][0]), y1 = kv4_unpack(rest[n][1]);
+                    const float f0 = (x0.x + y0.x) * (v0.x * inv), f1 = (x0.y + y0.y) * (v0.y * inv),
+                                f2 = (x1.x + y1.x) * (v1.x * inv), f3 = (x1.y + y1.y) * (v1.y * inv);
+                    uint32_t b0 = kv4_pack(f0, f1), b1 = kv4_pack(f2, f3);
+                    const float2 h0 = kv4_unpack(b0), h1 = kv4_unpack(b1);
+                    uint32_t r0 = kv4_pack(f0 - h0.x, f1 - h0.y), r1 = kv4_pack(f2 - h1.x, f3 - h1.y);
+                    if constexpr (EDGE) {  // (a scale may be NaN)
+                        b0 &= mask[n][0]; r0 &= mask[n][0];
+                        b1 &= mask[n][1]; r1 &= mask[n][1];
+                    }
+                    float t0[4], t1[4];
+                    ka_mma(t0, a0, r0, r1, 0.f, 0.f, 0.f, 0.f);
+                    ka_mma(t1, a1, r0, r1, 0.f, 0.f, 0.f, 0.f);
+                    ka_mma(t0, a0, b0, b1);
+                    ka_mma(t1, a1, b0, b1);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        o[n][b][0][i] += t0[i];
+                        o[n][b][1][i] += t1[i];
+                    }
                 }
             } else {
-                ka_mma(o[n][b][0], a0, b0, b1);
-                ka_mma(o[n][b][1], a1, b0, b1);
+                // a weight times its scale, rounded to fp16 once (the rest of the
+                // weight is below its last bit, so its own product's rounding is nothing)
+                const __half2 v0 = __hmul2(*reinterpret_cast<const __half2 *>(&v[h][b][0]), inv2),
+                              v1 = __hmul2(*reinterpret_cast<const __half2 *>(&v[h][b][1]), inv2);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const __half2 x0 = __hfma2(*reinterpret_cast<const __half2 *>(&w[n][0]), v0,
+                                               __hmul2(*reinterpret_cast<const __half2 *>(&rest[n][0]), v0)),
+                                  x1 = __hfma2(*reinterpret_cast<const __half2 *>(&w[n][1]), v1,
+                                               __hmul2(*reinterpret_cast<const __half2 *>(&rest[n][1]), v1));
+                    uint32_t b0 = *reinterpret_cast<const uint32_t *>(&x0), b1 = *reinterpret_cast<const uint32_t *>(&x1);
+                    if constexpr (EDGE) {
+                        b0 &= mask[n][0];
+                        b1 &= mask[n][1];
+                    }
+                    ka_mma(o[n][b][0], a0, b0, b1);
+                    ka_mma(o[n][b][1], a1, b0, b1);
+                }
             }
         }
     }
 }
 
-// SPLIT: fp32 calls, whose queries and weighted probabilities go through the
-// products as two halves each.  NT: column tiles of 8 query rows.
+// SPLIT: fp32 calls, whose queries and weights go through the products as two
+// halves each.  NT: column tiles of 8 query rows.
 template <bool SPLIT, int NB, int NT>
 __global__ void __launch_bounds__(kKaThreads, NT == 1 ? 2 : 1) kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
-    using S = KaSmem<NB, NT>;
+    using S = KaSmem<SPLIT, NB, NT>;
     constexpr uint32_t ROWS = S::kRows;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ float2 sml[kKaWarps][ROWS];
     __shared__ float sref[kKaWarps];
     __shared__ float sw[kKaWarps][ROWS];   // weights of the warps' results
     __shared__ float2 srow[ROWS];          // an item's references and sums
-    __shared__ uint32_t scan[kKaWarps + 1], sfind[3], slast;
+    __shared__ __align__(8) float soff[NT * NB * 8];
+    __shared__ float sqs[ROWS];            // of its queries
+    __shared__ uint32_t scan[kKaWarps], most[kKaWarps], sfind[3], slast;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+    uint4 *const sq = reinterpret_cast<uint4 *>(ring + S::kRingBytes);
     pdl_wait();
 
     // --- this CTA's part of the line ---
     const uint32_t entries = a.n_seq * a.rtiles, per = (entries + kKaThreads - 1) / kKaThreads;
+    bool whole = false;  // items count alike, and go to a CTA each
     auto units_of = [&](uint32_t e) -> uint32_t {
         int32_t len, fresh, limit;
         ka_lengths(a, e / a.rtiles, len, fresh);
-        return ka_tiles<ROWS>(a, e % a.rtiles, len, fresh, limit) ? (uint32_t)(limit + kKvTile - 1) / kKvTile + a.cost : 0;
+        return !ka_tiles<ROWS>(a, e % a.rtiles, len, fresh, limit) ? 0
+               : whole ? 1 : (uint32_t)(limit + kKaPair - 1) / kKaPair + a.cost;
     };
-    uint32_t mine = 0;
-    for (uint32_t e = tid * per; e < min(entries, (tid + 1) * per); ++e) mine += units_of(e) * a.n_kv;
+    uint32_t mine = 0, top = 0, have = 0;
+    for (uint32_t e = tid * per; e < min(entries, (tid + 1) * per); ++e) {
+        const uint32_t n = units_of(e);
+        mine += n * a.n_kv;
+        have += n ? a.n_kv : 0;
+        top = max(top, n);
+    }
+    if (entries * a.n_kv <= gridDim.x) {
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0) most[warp] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kKaWarps; ++w) top = max(top, most[w]);
+        if (top <= a.whole + a.cost) {
+            whole = true;
+            mine = have;
+        }
+    }
     uint32_t before = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
         const uint32_t x = __shfl_up_sync(0xffffffffu, before, d);
         if (lane >= (uint32_t)d) before += x;
     }
-    if (lane == 31) scan[warp + 1] = before;
-    if (tid == 0) scan[0] = 0;
+    if (lane == 31) scan[warp] = before;
     __syncthreads();
     uint32_t total = 0, base = 0;
 #pragma unroll
     for (int w = 0; w < kKaWarps; ++w) {
         if (w == (int)warp) base = total;
-        total += scan[w + 1];
+        total += scan[w];
     }
     before += base - mine;
-    const uint32_t chunk = max((total + gridDim.x - 1) / gridDim.x, a.least);
+    const uint32_t chunk = whole ? 1 : max((total + gridDim.x - 1) / gridDim.x, a.least);
     const uint64_t lo64 = (uint64_t)blockIdx.x * chunk;
     if (lo64 >= total) return;
-    const uint32_t lo = (uint32_t)lo64, hi = min(total, lo + chunk);
+    const uint32_t lo = (uint32_t)lo64;
     if (mine && before <= lo && lo < before + mine) {
         uint32_t at = before, e = tid * per, n;
         while (at + (n = units_of(e) * a.n_kv) <= lo) at += n, ++e;
@@ -373,65 +506,122 @@ __global__ void __launch_bounds__(kKaThreads, NT == 1 ? 2 : 1) kv4_attn_kernel(c
     uint32_t start = sfind[1] + head * units;  // of the item
 
     while (true) {
-        const uint32_t seq = entry / a.rtiles, rt = entry % a.rtiles;
-        int32_t len, fresh, limit = 0;
-        ka_lengths(a, seq, len, fresh);
-        ka_tiles<ROWS>(a, rt, len, fresh, limit);
-        const uint32_t tiles = (uint32_t)(limit + kKvTile - 1) / kKvTile;
-        const uint32_t from = min(max(lo, start) - start, tiles), to = min(min(hi, start + units) - start, tiles);
-        if (from < to || (tiles == 0 && lo <= start)) {
-            // --- queries: the products' B operand, columns of 8 rows ---
-            uint32_t qh[NT][NB][4], ql[SPLIT ? NT : 1][NB][4];
-            float qs[NT][2], m[NT][2], l[NT][2], o[NT][NB][2][4], vref = 5.9604645e-8f;  // 2^-24
-            int32_t lim[NT][2];
+        // the CTAs that share the item, `first` to `last`
+        const KaCut cut = ka_cut(units, a.snap);
+        const uint32_t first = (start + cut.head) / chunk, last = (start + cut.tail - 1) / chunk;
+        if (first > blockIdx.x) break;
+        if (last >= blockIdx.x) {
+            const uint32_t seq = entry / a.rtiles, rt = entry % a.rtiles;
+            int32_t len, fresh, limit = 0;
+            ka_lengths(a, seq, len, fresh);
+            ka_tiles<ROWS>(a, rt, len, fresh, limit);
+            const uint32_t pairs = (uint32_t)(limit + kKaPair - 1) / kKaPair;
+            const uint32_t from = first == blockIdx.x ? 0 : min(blockIdx.x * chunk - start, pairs),
+                           to = last == blockIdx.x ? pairs : min((blockIdx.x + 1) * chunk - start, pairs);
             const uint32_t rows = a.n_query * a.gq;
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const uint32_t row = rt * ROWS + n * 8 + g, t = row / a.gq;
-                float x[NB][8];
-                float top = 0.f, odd = 0.f;
-#pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    const uint32_t d = 32 * b + 8 * c;
-                    float4 v0 = {0.f, 0.f, 0.f, 0.f}, v1 = v0;
-                    if (row < rows && (int32_t)t < fresh && d < a.hd) {
-                        const uint64_t at = seq * a.q_seq + t * a.q_tok + (head * a.gq + row % a.gq) * a.q_head + d;
-                        v0 = kv4_load4(a.q, at, a.type);
-                        v1 = kv4_load4(a.q, at + 4, a.type);
-                    }
-                    x[b][0] = v0.x; x[b][1] = v0.y; x[b][2] = v0.z; x[b][3] = v0.w;
-                    x[b][4] = v1.x; x[b][5] = v1.y; x[b][6] = v1.z; x[b][7] = v1.w;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        top = fmaxf(top, fabsf(x[b][i]));
-                        odd += x[b][i] * 0.f;  // NaN where something is not finite
-                    }
-                }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                odd += __shfl_xor_sync(0xffffffffu, odd, 1);
-                odd += __shfl_xor_sync(0xffffffffu, odd, 2);
-                // the row times a power of two, its largest value in [2^13, 2^14)
-                const uint32_t ex = min(max(__float_as_uint(top) >> 23, 14u), 254u);
-                const float up = __uint_as_float((267u - ex) << 23), down = __uint_as_float((ex - 13u) << 23) + odd;
-#pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float y0 = x[b][2 * i] * up, y1 = x[b][2 * i + 1] * up;
-                        qh[n][b][i] = kv4_pack(y0, y1);
-                        if constexpr (SPLIT) {
-                            const float2 f = kv4_unpack(qh[n][b][i]);
-                            ql[n][b][i] = kv4_pack(y0 - f.x, y1 - f.y);
+
+            // --- the warp's positions: their pages, and the first copies ---
+            uint8_t *const mine_ring = ring + warp * (kKaStages * S::kStage);
+            const uint32_t count = from + warp < to ? (to - from - warp + kKaWarps - 1) / kKaWarps : 0;
+            const int32_t *const table = a.pages + seq * a.pages_seq;
+            // where the next 32 pairs' tiles lie, in 64-byte steps from the cache's
+            // beginning (each lane a pair), and which tiles of the ring's pairs there are
+            constexpr uint32_t kNone = 0xffffffffu;
+            uint32_t at0 = 0, at1 = 0, there = 0;
+            auto fill = [&](uint32_t i) {
+                if (i < count) {
+                    if (i % 32 == 0) {
+                        const uint32_t t = 2 * (from + warp + (i + lane) * kKaWarps);  // the first tile
+                        at0 = at1 = kNone;
+                        if (i + lane < count) {
+                            const bool two = (t + 1) * kKvTile < (uint32_t)limit;
+                            const uint32_t page0 = (uint32_t)table[t >> a.tpp_log2],
+                                           page1 = two ? (uint32_t)table[(t + 1) >> a.tpp_log2] : 0,
+                                           in = (1u << a.tpp_log2) - 1;
+                            if (page0 < a.n_page) at0 = (((page0 * a.n_kv + head) << a.tpp_log2) + (t & in)) * (S::kTile / 64);
+                            if (two && page1 < a.n_page) at1 = (((page1 * a.n_kv + head) << a.tpp_log2) + ((t + 1) & in)) * (S::kTile / 64);
+                            if (page0 >= a.n_page || page1 >= a.n_page) atomicOr(a.err, kKvBadPage);
                         }
                     }
+                    const uint32_t stage = i % kKaStages, s0 = __shfl_sync(0xffffffffu, at0, i % 32),
+                                   s1 = __shfl_sync(0xffffffffu, at1, i % 32);
+                    const bool ok0 = s0 != kNone, ok1 = s1 != kNone;
+                    there = (there & ~(3u << 2 * stage)) | ((ok0 ? 1u : 0u) | (ok1 ? 2u : 0u)) << 2 * stage;
+                    constexpr uint32_t kChunks = S::kTile / 16;
+                    const uint8_t *src0 = a.cache + (uint64_t)s0 * 64 + lane * 16,
+                                  *src1 = a.cache + (uint64_t)s1 * 64 + lane * 16 - S::kTile;
+                    uint8_t *dst = mine_ring + stage * S::kStage + lane * 16;
+#pragma unroll
+                    for (uint32_t k = 0; k < (2 * kChunks + 31) / 32; ++k) {
+                        const uint32_t c0 = k * 32 + lane;
+                        if (c0 < kChunks ? ok0 : ok1 && c0 < 2 * kChunks) cp_async16(dst + k * 512, (c0 < kChunks ? src0 : src1) + k * 512);
+                    }
+                }
+                cp_async_commit();
+            };
+#pragma unroll
+            for (uint32_t i = 0; i < kKaStages - 1; ++i) fill(i);
+
+            // --- queries: the products' B operand, columns of 8 rows ---
+            // 16 threads a row, 8 dimensions each.  A row is taken times a power
+            // of two, its largest value in [2^13, 2^14); but for SPLIT pairs 1 and 3
+            // of each eight, whose codes weigh 16 times as much, 1/16 of that.
+            for (uint32_t i = tid; i < ROWS * 16; i += kKaThreads) {
+                const uint32_t r = i / 16, ch = i % 16, b = ch / 4, row = rt * ROWS + r, t = row / a.gq, d = 8 * ch;
+                float4 v0 = {0.f, 0.f, 0.f, 0.f}, v1 = v0;
+                if (row < rows && (int32_t)t < fresh && d < a.hd) {
+                    const uint64_t at = seq * a.q_seq + t * a.q_tok + (head * a.gq + row % a.gq) * a.q_head + d;
+                    v0 = kv4_load4(a.q, at, a.type);
+                    v1 = kv4_load4(a.q, at + 4, a.type);
+                }
+                const float x[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+                float top = 0.f, odd = 0.f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    top = fmaxf(top, fabsf(x[k]));
+                    odd += x[k] * 0.f;  // NaN where something is not finite
+                }
+#pragma unroll
+                for (int k = 1; k < 16; k <<= 1) {
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+                    odd += __shfl_xor_sync(0xffffffffu, odd, k);
+                }
+                const uint32_t ex = min(max(__float_as_uint(top) >> 23, 14u), 254u);
+                const float up = __uint_as_float((267u - ex) << 23);
+                uint32_t hi[4], lo[4];
+                float sum = 0.f;  // as the products have them
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float by = !SPLIT && k & 1 ? up * 0.0625f : up, y0 = x[2 * k] * by, y1 = x[2 * k + 1] * by;
+                    hi[k] = kv4_pack(y0, y1);
+                    const float2 f = kv4_unpack(hi[k]);
+                    lo[k] = kv4_pack(y0 - f.x, y1 - f.y);
+                    sum += (k & 1 ? 16.f : 1.f) * (f.x + f.y);
+                }
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                if (b < NB) {
+                    const uint32_t at = ((r / 8) * (SPLIT ? 2 : 1) * NB + b) * 32 + r % 8 * 4 + ch % 4;
+                    sq[at] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                    if constexpr (SPLIT) sq[at + NB * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    if (ch % 4 == 0) soff[(r / 8 * NB + b) * 8 + r % 8] = sum * (-8.f / 16777216.f);
+                }
+                // codes stand there as multiples of 2^-24 (SPLIT: of 2^-9); past 2^100 the factor would not be finite
+                if (ch == 0) sqs[r] = (__uint_as_float((ex - 13u) << 23) + (ex < 227 ? odd : NAN)) * (a.scale * 1.4426950408889634f) * (SPLIT ? kKaCode : 16777216.f);
+            }
+            float qs[NT][2], mm[NT][2], thr[NT][2], l[NT][2], o[NT][NB][2][4], vref = 6.103515625e-05f;  // 2^-14
+            int32_t lim[NT][2], limt[NT];
+            __syncthreads();
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    qs[n][j] = __shfl_sync(0xffffffffu, down, 4 * (2 * c + j)) * (a.scale * 1.4426950408889634f);
+                    qs[n][j] = sqs[n * 8 + 2 * c + j];
                     lim[n][j] = ka_limit(a, len, fresh, rt * ROWS + n * 8 + 2 * c + j);
-                    m[n][j] = -INFINITY;
-                    l[n][j] = 0.f;
+                    thr[n][j] = -INFINITY;  // nothing seen yet
+                    mm[n][j] = l[n][j] = 0.f;
                 }
+                limt[n] = ka_limit(a, len, fresh, rt * ROWS + n * 8 + g);
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
@@ -439,47 +629,16 @@ __global__ void __launch_bounds__(kKaThreads, NT == 1 ? 2 : 1) kv4_attn_kernel(c
             }
             const int32_t least = ka_limit(a, len, fresh, rt * ROWS);  // of the first row: the fewest positions
 
-            // --- the warp's tiles ---
-            uint8_t *const mine_ring = ring + warp * (kKaStages * S::kTile);
-            const uint32_t count = from + warp < to ? (to - from - warp + kKaWarps - 1) / kKaWarps : 0;
-            const int32_t *const table = a.pages + seq * a.pages_seq;
-            uint32_t ids = 0, good = 0;
-            auto fill = [&](uint32_t i) {
-                if (i < count) {
-                    if (i % 32 == 0)
-                        ids = i + lane < count ? (uint32_t)table[(from + warp + (i + lane) * kKaWarps) >> a.tpp_log2] : 0;
-                    const uint32_t page = __shfl_sync(0xffffffffu, ids, i % 32), stage = i % kKaStages;
-                    good &= ~(1u << stage);
-                    if (page < a.n_page) {
-                        good |= 1u << stage;
-                        const uint32_t t = from + warp + i * kKaWarps;
-                        const uint8_t *src = a.cache + ((((uint64_t)page * a.n_kv + head) << a.tpp_log2) +
-                                                        (t & ((1u << a.tpp_log2) - 1))) * S::kTile;
-                        uint8_t *dst = mine_ring + stage * S::kTile;
-                        constexpr uint32_t kChunks = S::kTile / 16;
-#pragma unroll
-                        for (uint32_t k = 0; k < (kChunks + 31) / 32; ++k)
-                            if (k * 32 + lane < kChunks) cp_async16(dst + (k * 32 + lane) * 16, src + (k * 32 + lane) * 16);
-                    } else if (lane == 0) {
-                        atomicOr(a.err, kKvBadPage);
-                    }
-                }
-                cp_async_commit();
-            };
-#pragma unroll
-            for (uint32_t i = 0; i < kKaStages - 1; ++i) fill(i);
             for (uint32_t i = 0; i < count; ++i) {
                 asm volatile("cp.async.wait_group %0;" ::"n"(kKaStages - 2) : "memory");
                 __syncwarp();
-                const uint32_t stage = i % kKaStages, t = from + warp + i * kKaWarps;
-                if (good >> stage & 1) {
-                    const uint8_t *tile = mine_ring + stage * S::kTile;
-                    const int32_t pos0 = (int32_t)(t * kKvTile);
-                    if (pos0 + (int32_t)kKvTile > least)
-                        ka_tile<SPLIT, NB, NT, true>(tile, qh, ql, qs, lim, pos0, limit, o, m, l, vref);
-                    else
-                        ka_tile<SPLIT, NB, NT, false>(tile, qh, ql, qs, lim, pos0, limit, o, m, l, vref);
-                }
+                const uint32_t stage = i % kKaStages, ok = there >> 2 * stage & 3;
+                const uint8_t *pair = mine_ring + stage * S::kStage;
+                const int32_t pos0 = (int32_t)((from + warp + i * kKaWarps) * kKaPair);
+                if (pos0 + (int32_t)kKaPair > least || ok != 3)
+                    ka_pair<SPLIT, NB, NT, true>(pair, sq, soff, qs, lim, limt, pos0, limit, ok, o, mm, thr, l, vref);
+                else
+                    ka_pair<SPLIT, NB, NT, false>(pair, sq, soff, qs, lim, limt, pos0, limit, ok, o, mm, thr, l, vref);
                 __syncwarp();
                 fill(i + kKaStages - 1);
             }
@@ -497,7 +656,7 @@ __global__ void __launch_bounds__(kKaThreads, NT == 1 ? 2 : 1) kv4_attn_kernel(c
                     sum += __shfl_xor_sync(0xffffffffu, sum, 8);
                     sum += __shfl_xor_sync(0xffffffffu, sum, 16);
                     const uint32_t row = n * 8 + 2 * c + j;
-                    if (g == 0) sml[warp][row] = make_float2(m[n][j], sum);
+                    if (g == 0) sml[warp][row] = make_float2(thr[n][j] == -INFINITY ? -INFINITY : mm[n][j], sum);
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
                         *reinterpret_cast<float4 *>(so + (warp * ROWS + row) * S::kStride + 32 * b + 4 * g) =
@@ -514,13 +673,12 @@ __global__ void __launch_bounds__(kKaThreads, NT == 1 ? 2 : 1) kv4_attn_kernel(c
                 for (int w = 0; w < kKaWarps; ++w) {
                     const float f = ka_exp2(sml[w][tid].x - ref);
                     sum = fmaf(f, sml[w][tid].y, sum);
-                    sw[w][tid] = f * sref[w] * (1.f / kKaHead);
+                    sw[w][tid] = f * (sref[w] * kKaCode);
                 }
                 srow[tid] = make_float2(top, sum);
             }
             __syncthreads();
-            const uint32_t first = start / chunk, parts = (start + max(tiles, 1u) - 1) / chunk - first + 1;
-            const bool begins = first == blockIdx.x;
+            const uint32_t parts = last - first + 1;
             auto finish = [&](uint32_t r, uint32_t d, float4 v, float2 ml) {
                 const uint32_t row = rt * ROWS + r, t = row / a.gq;
                 if (row >= rows || (int32_t)t >= fresh) return;
@@ -529,7 +687,7 @@ __global__ void __launch_bounds__(kKaThreads, NT == 1 ? 2 : 1) kv4_attn_kernel(c
                 if (d < a.hd) kv4_store4(a.out, at * a.hd + d, a.type, make_float4(v.x * by, v.y * by, v.z * by, v.w * by));
                 if (d == 0 && a.lse) a.lse[at] = ml.y == 0.f ? -INFINITY : (ml.x + log2f(ml.y)) * 0.69314718055994531f;
             };
-            const uint64_t slot = 2ull * blockIdx.x + (begins ? 1 : 0);
+            auto slot_of = [&](uint32_t cta) { return 2ull * cta + (cta == first ? 1 : 0); };
             for (uint32_t i = tid; i < ROWS * 8 * NB; i += kKaThreads) {
                 const uint32_t r = i / (8 * NB), d = i % (8 * NB) * 4;
                 float4 v = {0.f, 0.f, 0.f, 0.f};
@@ -545,8 +703,8 @@ __global__ void __launch_bounds__(kKaThreads, NT == 1 ? 2 : 1) kv4_attn_kernel(c
                 if (parts == 1) {
                     finish(r, d, v, srow[r]);
                 } else {
-                    *reinterpret_cast<float4 *>(a.po + (slot * ROWS + r) * (32 * NB) + d) = v;
-                    if (d == 0) a.pml[slot * ROWS + r] = srow[r];
+                    *reinterpret_cast<float4 *>(a.po + (slot_of(blockIdx.x) * ROWS + r) * (32 * NB) + d) = v;
+                    if (d == 0) a.pml[slot_of(blockIdx.x) * ROWS + r] = srow[r];
                 }
             }
             if (parts > 1) {
@@ -557,13 +715,13 @@ __global__ void __launch_bounds__(kKaThreads, NT == 1 ? 2 : 1) kv4_attn_kernel(c
                 if (slast) {
                     __threadfence();
                     if (tid == 0) a.ticket[first] = 0;
-                    auto slot_of = [&](uint32_t p) { return 2ull * (first + p) + (p == 0 ? 1 : 0); };
                     for (uint32_t i = tid; i < ROWS * 8 * NB; i += kKaThreads) {
                         const uint32_t r = i / (8 * NB), d = i % (8 * NB) * 4;
+                        if (rt * ROWS + r >= rows) continue;
                         float2 ml = {-INFINITY, 0.f};
                         float4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-                        for (uint32_t p = 0; p < parts; ++p) {
+#pragma unroll 8
+                        for (uint32_t p = first; p <= last; ++p) {
                             const float2 y = __ldcg(a.pml + slot_of(p) * ROWS + r);
                             const float4 x = __ldcg(reinterpret_cast<const float4 *>(a.po + (slot_of(p) * ROWS + r) * (32 * NB) + d));
                             const float top = fmaxf(ml.x, y.x), ref = top == -INFINITY ? 0.f : top;
@@ -581,8 +739,9 @@ __global__ void __launch_bounds__(kKaThreads, NT == 1 ? 2 : 1) kv4_attn_kernel(c
             __syncthreads();  // the results are read: the rings may be filled again
         }
         // --- the next item ---
+        if (last > blockIdx.x) break;
         start += units;
-        if (start >= hi) break;
+        if (start >= total) break;
         if (++head == a.n_kv) {
             head = 0;
             do units = units_of(++entry);

@@ -101,7 +101,8 @@ def attention(q, k, v, lengths, n_new=None, scale=None):
 def bounds(q, out, lse, mass, reach, most):
     """How far a call's out and lse may be from these. Scores: a product of 32 exact pairs is summed in fp32 whose
     additions may truncate (2^-23 each, 32 + 4 + 2 of them, queries of fp32 calls held to 2^-22): under 2^-17 of reach.
-    The average: twice the scores' errors, probabilities held to 2^-11 (fp32 calls 2^-21) and exp2 to 2^-21, sums of `most` terms in fp32;
+    The average: twice the scores' errors, probabilities with their scales held to 2^-11 (fp32 calls 2^-21) and exp2 to
+    2^-21, sums of `most` terms in fp32;
     and the output's rounding. Products below 2^-24 of 2^8 times the largest scale are lost: 2^-20 of mass's largest covers them."""
     p = 2.0 ** -11 if q.dtype != torch.float32 else 2.0 ** -21
     ds = 2.0 ** -17 * reach
