@@ -91,6 +91,12 @@ bool rows_ok(const char *who, uint32_t type, uint32_t n_seq, uint32_t n_tok, uin
     return true;
 }
 
+template <typename T>
+bool run_append(const Kv4AppendArgs &k, bool halves, dim3 grid, cudaStream_t st) {
+    const auto fn = !k.cos ? kv4_append_kernel<T, kKpNone> : halves ? kv4_append_kernel<T, kKpHalves> : kv4_append_kernel<T, kKpNeighbours>;
+    return launched(launch_after(fn, grid, kKpThreads, 0, 1, st, k), "fwb_kv4_append launch");
+}
+
 // --- attention ---------------------------------------------------------------
 constexpr const char *kAttn = "fwb_kv4_attention";
 
@@ -204,19 +210,27 @@ int fwb_kv4_append_dev(const fwb_kv4_append_t *a, void *stream) {
     if (!rows_ok(who, a->type, a->n_seq, a->n_query, a->n_head_kv, k.k) || !rows_ok(who, a->type, a->n_seq, a->n_query, a->n_head_kv, k.v) ||
         (heads && (!rows_ok(who, a->type, a->n_seq, a->n_query, heads, k.q) || !rows_ok(who, a->type, a->n_seq, a->n_query, heads, k.q_out))))
         return -1;
-    const uint64_t tokens = (uint64_t)a->n_seq * a->n_query, lanes_q = tokens * heads * (a->head_dim / 8),
-                   lanes_kv = tokens * 2 * a->n_head_kv * kv4_blocks(a->head_dim) * 8;
-    if (heads > 65535 || lanes_q > 0xffffff00u || lanes_kv > 0xffffff00u) { refuse(who, "too many tokens or heads"); return -1; }
+    if (heads > 65535) { refuse(who, "too many heads"); return -1; }
     k.cache = static_cast<uint8_t *>(a->cache);
     k.pages = a->pages; k.len = a->lengths; k.n_new = a->n_new;
     k.cos = a->cos; k.sin = a->sin;
     k.pages_seq = a->pages_stride;
-    k.type = a->type; k.n_seq = a->n_seq; k.n_query = a->n_query; k.n_head = heads ? heads : 1; k.n_kv = a->n_head_kv; k.hd = a->head_dim;
-    k.page_log2 = log2_of(a->page_size); k.n_page = a->n_page; k.max_pages = a->max_pages; k.n_pos = a->n_pos; k.halves = a->halves;
-    k.q_blocks = (uint32_t)((lanes_q + kKpThreads - 1) / kKpThreads);
+    k.n_seq = a->n_seq; k.n_query = a->n_query; k.n_head = heads; k.n_kv = a->n_head_kv; k.hd = a->head_dim;
+    k.page_log2 = log2_of(a->page_size); k.n_page = a->n_page; k.max_pages = a->max_pages; k.n_pos = a->n_pos;
+    auto by = [](uint64_t d) { return d == 1 ? 0u : (uint32_t)((((uint64_t)1 << 32) + d - 1) / d); };
+    const uint32_t pairs = a->head_dim * elem_bytes(a->type) / 32;  // of 16-byte chunks in a query row
+    k.by_part = by(pairs);
+    k.by_blocks = by(kv4_blocks(a->head_dim));
     if (!(k.err = error_word())) return -1;
-    const uint32_t blocks = k.q_blocks + (uint32_t)((lanes_kv + kKpThreads - 1) / kKpThreads);
-    return launched(launch_after(kv4_append_kernel, dim3(blocks), kKpThreads, 0, 1, static_cast<cudaStream_t>(stream), k), who) ? 0 : -1;
+    // Blocks of a token: one where tokens fill the device; few tokens are dealt out finer.
+    const uint32_t tokens = a->n_seq * a->n_query, most = std::max(heads * pairs, 2 * a->n_head_kv * kv4_blocks(a->head_dim) * 4),
+                   parts = std::min((most + kKpThreads - 1) / kKpThreads, std::max(1u, 4 * device_sms() / tokens));
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const dim3 grid(tokens, parts);
+    const bool ok = a->type == 0 ? run_append<float>(k, a->halves != 0, grid, st)
+                  : a->type == 1 ? run_append<__half>(k, a->halves != 0, grid, st)
+                                 : run_append<__nv_bfloat16>(k, a->halves != 0, grid, st);
+    return ok ? 0 : -1;
 }
 
 int fwb_kv4_read_dev(const fwb_kv4_read_t *a, void *stream) {

@@ -15,15 +15,15 @@
 // exact comparisons, so that a cache's content does not depend on how a sum was
 // rounded.
 //
-// Bound: DRAM for prompts, the launch for steps.  Eight lanes hold a block, four
-// values each: its scale is three shuffles, and every store goes to bytes of
-// this position alone.
+// Bound: DRAM for prompts, the launch for steps.  Four lanes hold a block, eight
+// values each: its scale is two shuffles of each extreme, a lane has a whole
+// word of a key's codes, and every store goes to bytes of this position alone.
 #pragma once
 #include "kv4_format.cuh"
 
 namespace fwb {
 
-constexpr int kKpThreads = 256;
+constexpr int kKpThreads = 128;
 
 struct Kv4Rows {  // [n_seq][n_query][heads][head_dim], strides in elements
     const void *p;
@@ -36,8 +36,8 @@ struct Kv4AppendArgs {
     const int32_t *pages, *len, *n_new;
     const float *cos, *sin;  // [n_pos][hd / 2], or null: not rotated
     uint64_t pages_seq;
-    uint32_t type, n_seq, n_query, n_head, n_kv, hd, page_log2, n_page, max_pages, n_pos, halves;
-    uint32_t q_blocks;  // CTAs for queries, before those for keys and values
+    uint32_t n_seq, n_query, n_head, n_kv, hd, page_log2, n_page, max_pages, n_pos;
+    uint32_t by_part, by_blocks;  // 2^32 over the chunk pairs of a query row, and the blocks of a row, rounded up (0: over 1)
     uint32_t *err;
 };
 
@@ -54,137 +54,215 @@ __device__ __forceinline__ int32_t kp_position(const Kv4AppendArgs &a, uint32_t 
     return (int32_t)pos;
 }
 
-// A rotated pair to fp32: in fp32 for queries (two roundings), exactly and
-// then rounded for keys.
+enum KpTurn { kKpNone, kKpNeighbours, kKpHalves };
+
+// x cos - y sin, to fp32: with two roundings for queries, with one for keys.
 template <bool EXACT>
-__device__ __forceinline__ float2 kp_turn(float x, float y, float c, float s) {
-    if constexpr (EXACT)
-        return make_float2((float)((double)x * c - (double)y * s), (float)((double)x * s + (double)y * c));
-    else
-        return make_float2(fmaf(x, c, -(y * s)), fmaf(x, s, y * c));
+__device__ __forceinline__ float kp_turn(float x, float c, float y, float s) {
+    if constexpr (EXACT) return (float)((double)x * c - (double)y * s);
+    else return fmaf(x, c, -(y * s));
 }
 
-// Eight values of a query row: four pairs, so that a row may be turned in place.
-__device__ __forceinline__ void kp_query(const Kv4AppendArgs &a, uint32_t i, uint32_t &bad) {
-    const uint32_t part = a.hd / 8, j = i % part, row = i / part, h = row % a.n_head, tok = row / a.n_head,
-                   seq = tok / a.n_query, t = tok % a.n_query;
-    if (seq >= a.n_seq) return;
-    const int32_t pos = kp_position(a, seq, t, bad);
-    if (pos < 0) return;
-    const uint32_t d0 = a.halves ? 4 * j : 8 * j, d1 = a.halves ? 4 * j + a.hd / 2 : 8 * j + 4;
-    const uint64_t from = seq * a.q.seq + t * a.q.tok + h * a.q.head,
-                   to = seq * a.q_out.seq + t * a.q_out.tok + h * a.q_out.head;
-    float4 x = kv4_load4(a.q.p, from + d0, a.type), y = kv4_load4(a.q.p, from + d1, a.type);
-    if (a.cos) {
-        const uint64_t at = (uint64_t)pos * (a.hd / 2) + 4 * j;
-        const float4 c = *reinterpret_cast<const float4 *>(a.cos + at), s = *reinterpret_cast<const float4 *>(a.sin + at);
-        if (a.halves) {
-            const float2 p0 = kp_turn<false>(x.x, y.x, c.x, s.x), p1 = kp_turn<false>(x.y, y.y, c.y, s.y),
-                         p2 = kp_turn<false>(x.z, y.z, c.z, s.z), p3 = kp_turn<false>(x.w, y.w, c.w, s.w);
-            x = make_float4(p0.x, p1.x, p2.x, p3.x);
-            y = make_float4(p0.y, p1.y, p2.y, p3.y);
-        } else {
-            const float2 p0 = kp_turn<false>(x.x, x.y, c.x, s.x), p1 = kp_turn<false>(x.z, x.w, c.y, s.y),
-                         p2 = kp_turn<false>(y.x, y.y, c.z, s.z), p3 = kp_turn<false>(y.z, y.w, c.w, s.w);
-            x = make_float4(p0.x, p0.y, p1.x, p1.y);
-            y = make_float4(p2.x, p2.y, p3.x, p3.y);
-        }
+// Two chunks of 16 bytes of a query row, half a row apart: whole pairs either
+// way, so that a row may be turned in place.
+template <typename T>
+struct KpQuery {
+    static constexpr int N = 16 / sizeof(T);
+    float x[N], y[N];
+    uint32_t h, j;
+};
+template <typename T>
+__device__ __forceinline__ void kp_chunk(const void *p, uint64_t at, float (&x)[16 / sizeof(T)]) {
+    if constexpr (sizeof(T) == 2) {
+        kv4_load8<T>(p, at, x);
+    } else {
+        const float4 v = kv4_load4<T>(p, at);
+        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
     }
-    kv4_store4(const_cast<void *>(a.q_out.p), to + d0, a.type, x);
-    kv4_store4(const_cast<void *>(a.q_out.p), to + d1, a.type, y);
 }
-
-// The code of y: floor(y / d + 8.5) held to 0..15, by exact comparisons (a
-// multiple of d / 2 up to 8.5 d is exact in fp32).
-__device__ __forceinline__ uint32_t kp_code(float y, float d) {
-    if (d == 0.f) return 8;
-    const float a = fabsf(d), z = d < 0.f ? -y : y;
-    float f = fminf(fmaxf(floorf(__fdiv_rn(z, a) + 8.5f), 0.f), 15.f);
-    if (z < (f - 8.5f) * a) f -= 1.f;
-    else if (z >= (f - 7.5f) * a) f += 1.f;
-    return (uint32_t)fminf(fmaxf(f, 0.f), 15.f);
-}
-
-// A block of a key or value row, four values in each of eight lanes (all of a
-// warp's lanes come here together).
-__device__ __forceinline__ void kp_block(const Kv4AppendArgs &a, uint32_t i, uint32_t &bad) {
-    const uint32_t nb = kv4_blocks(a.hd), j = i % 8, unit = i / 8, b = unit % nb, row = unit / nb,
-                   h = row % (2 * a.n_kv), tok = row / (2 * a.n_kv), seq = tok / a.n_query, t = tok % a.n_query;
-    const bool value = h >= a.n_kv;
-    const uint32_t head = value ? h - a.n_kv : h, d0 = 32 * b + 4 * j;
-    const int32_t pos = seq < a.n_seq ? kp_position(a, seq, t, bad) : -1;
-    float y[4] = {0.f, 0.f, 0.f, 0.f};
-    if (pos >= 0 && d0 < a.hd) {
-        const Kv4Rows &src = value ? a.v : a.k;
-        const uint64_t from = seq * src.seq + t * src.tok + head * src.head;
-        const float4 x = kv4_load4(src.p, from + d0, a.type);
-        y[0] = x.x; y[1] = x.y; y[2] = x.z; y[3] = x.w;
-        if (!value && a.cos) {
-            const uint64_t at = (uint64_t)pos * (a.hd / 2);
-            if (a.halves) {
-                const bool upper = d0 >= a.hd / 2;
-                const uint32_t e = upper ? d0 - a.hd / 2 : d0;
-                const float4 z = kv4_load4(src.p, from + (upper ? e : e + a.hd / 2), a.type);
-                const float4 c = *reinterpret_cast<const float4 *>(a.cos + at + e), s = *reinterpret_cast<const float4 *>(a.sin + at + e);
-                const float2 p0 = upper ? kp_turn<true>(z.x, x.x, c.x, s.x) : kp_turn<true>(x.x, z.x, c.x, s.x),
-                             p1 = upper ? kp_turn<true>(z.y, x.y, c.y, s.y) : kp_turn<true>(x.y, z.y, c.y, s.y),
-                             p2 = upper ? kp_turn<true>(z.z, x.z, c.z, s.z) : kp_turn<true>(x.z, z.z, c.z, s.z),
-                             p3 = upper ? kp_turn<true>(z.w, x.w, c.w, s.w) : kp_turn<true>(x.w, z.w, c.w, s.w);
-                y[0] = upper ? p0.y : p0.x; y[1] = upper ? p1.y : p1.x;
-                y[2] = upper ? p2.y : p2.x; y[3] = upper ? p3.y : p3.x;
-            } else {
-                const float2 c = *reinterpret_cast<const float2 *>(a.cos + at + d0 / 2),
-                             s = *reinterpret_cast<const float2 *>(a.sin + at + d0 / 2);
-                const float2 p0 = kp_turn<true>(x.x, x.y, c.x, s.x), p1 = kp_turn<true>(x.z, x.w, c.y, s.y);
-                y[0] = p0.x; y[1] = p0.y; y[2] = p1.x; y[3] = p1.y;
-            }
-        }
+template <typename T>
+__device__ __forceinline__ void kp_query_load(const Kv4AppendArgs &a, uint32_t i, uint64_t from, KpQuery<T> &q) {
+    const uint32_t part = a.hd / (2 * q.N);
+    q.h = part == 1 ? i : __umulhi(i, a.by_part);
+    q.j = i - q.h * part;
+    if (q.h < a.n_head) {
+        kp_chunk<T>(a.q.p, from + q.h * a.q.head + q.N * q.j, q.x);
+        kp_chunk<T>(a.q.p, from + q.h * a.q.head + q.N * q.j + a.hd / 2, q.y);
     }
-    float hi = fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), lo = fminf(fminf(y[0], y[1]), fminf(y[2], y[3]));
-    uint32_t odd = !(fabsf(y[0]) < INFINITY && fabsf(y[1]) < INFINITY && fabsf(y[2]) < INFINITY && fabsf(y[3]) < INFINITY);
+}
+template <typename T>
+__device__ __forceinline__ void kp_chunk_store(void *p, uint64_t at, const float (&x)[16 / sizeof(T)]) {
+    if constexpr (sizeof(T) == 2) kv4_store8<T>(p, at, x);
+    else kv4_store4<T>(p, at, make_float4(x[0], x[1], x[2], x[3]));
+}
+// M angles' cosines and sines.
+template <int M>
+__device__ __forceinline__ void kp_angles(const Kv4AppendArgs &a, uint64_t at, float (&c)[M], float (&s)[M]) {
+    if constexpr (M == 2) {
+        const float2 u = *reinterpret_cast<const float2 *>(a.cos + at), v = *reinterpret_cast<const float2 *>(a.sin + at);
+        c[0] = u.x; c[1] = u.y; s[0] = v.x; s[1] = v.y;
+    } else {
 #pragma unroll
-    for (int m = 1; m < 8; m <<= 1) {
+        for (int m = 0; m < M; m += 4) {
+            const float4 u = kv4_load4<float>(a.cos, at + m), v = kv4_load4<float>(a.sin, at + m);
+            c[m] = u.x; c[m + 1] = u.y; c[m + 2] = u.z; c[m + 3] = u.w;
+            s[m] = v.x; s[m + 1] = v.y; s[m + 2] = v.z; s[m + 3] = v.w;
+        }
+    }
+}
+// Neighbours turned, in a chunk of N values from dimension d on.
+template <bool EXACT, int N>
+__device__ __forceinline__ void kp_neighbours(const Kv4AppendArgs &a, uint32_t pos, uint32_t d, float (&x)[N]) {
+    float c[N / 2], s[N / 2];
+    kp_angles(a, (uint64_t)pos * (a.hd / 2) + d / 2, c, s);
+#pragma unroll
+    for (int m = 0; m < N / 2; ++m) {
+        const float u = kp_turn<EXACT>(x[2 * m], c[m], x[2 * m + 1], s[m]);
+        x[2 * m + 1] = kp_turn<EXACT>(x[2 * m + 1], c[m], x[2 * m], -s[m]);
+        x[2 * m] = u;
+    }
+}
+template <typename T, KpTurn TURN>
+__device__ __forceinline__ void kp_query_store(const Kv4AppendArgs &a, KpQuery<T> &q, uint64_t to, uint32_t pos) {
+    if (q.h >= a.n_head) return;
+    constexpr int N = KpQuery<T>::N;
+    if constexpr (TURN == kKpNeighbours) {
+        kp_neighbours<false>(a, pos, N * q.j, q.x);
+        kp_neighbours<false>(a, pos, N * q.j + a.hd / 2, q.y);
+    } else if constexpr (TURN == kKpHalves) {
+        float c[N], s[N];
+        kp_angles(a, (uint64_t)pos * (a.hd / 2) + N * q.j, c, s);
+#pragma unroll
+        for (int m = 0; m < N; ++m) {
+            const float u = kp_turn<false>(q.x[m], c[m], q.y[m], s[m]);
+            q.y[m] = kp_turn<false>(q.y[m], c[m], q.x[m], -s[m]);
+            q.x[m] = u;
+        }
+    }
+    kp_chunk_store<T>(const_cast<void *>(a.q_out.p), to + q.h * a.q_out.head + N * q.j, q.x);
+    kp_chunk_store<T>(const_cast<void *>(a.q_out.p), to + q.h * a.q_out.head + N * q.j + a.hd / 2, q.y);
+}
+
+// The code of y: floor(y / d + 8.5) held to 0..15.  The integer nearest to y *
+// (1 / d) is one off at most; what is left of y beyond its code is exact in
+// fp32 (codes have 4 bits, d has 11), and a comparison with d / 2 decides.
+// a = |d| and inv = 1 / a, or where d is 0 the largest float and 0.
+__device__ __forceinline__ uint32_t kp_code(float y, float d, float a, float inv) {
+    const float z = d < 0.f ? -y : y, t = fminf(fmaxf(z * inv, -9.f), 9.f), n = rintf(t), left = fmaf(-n, a, z), half = 0.5f * a;
+    const int k = (int)n + 8 + (left >= half ? 1 : 0) - (left < -half ? 1 : 0);
+    return (uint32_t)min(max(k, 0), 15);
+}
+
+// Eight values of a block of a key or value row (zeros past its end), and where
+// halves are turned the eight that they pair with.
+struct KpBlock {
+    float x[8], z[8];
+    uint32_t head, b;
+    bool value;
+};
+template <typename T, KpTurn TURN>
+__device__ __forceinline__ void kp_block_load(const Kv4AppendArgs &a, uint32_t i, uint32_t seq, uint32_t t, bool is, KpBlock &k) {
+    const uint32_t nb = kv4_blocks(a.hd), unit = i / 4, h = nb == 1 ? unit : __umulhi(unit, a.by_blocks);
+    k.value = h >= a.n_kv;
+    k.head = k.value ? h - a.n_kv : h;
+    k.b = unit - h * nb;
+    const uint32_t d0 = 32 * k.b + 8 * (i % 4);
+#pragma unroll
+    for (int m = 0; m < 8; ++m) k.x[m] = 0.f;
+    if (is && d0 < a.hd) {
+        const Kv4Rows &src = k.value ? a.v : a.k;
+        const uint64_t from = seq * src.seq + t * src.tok + k.head * src.head;
+        kv4_load8<T>(src.p, from + d0, k.x);
+        if constexpr (TURN == kKpHalves)
+            if (!k.value) kv4_load8<T>(src.p, from + (d0 >= a.hd / 2 ? d0 - a.hd / 2 : d0 + a.hd / 2), k.z);
+    }
+}
+// The block rotated, quantised and stored, by the four lanes that hold it (all
+// of a warp's lanes come here together; is: whether this one holds any).
+template <KpTurn TURN>
+__device__ __forceinline__ void kp_block_store(const Kv4AppendArgs &a, KpBlock &k, uint32_t i, uint32_t page, uint32_t pos, bool is) {
+    const uint32_t nb = kv4_blocks(a.hd), j = i % 4, d0 = 32 * k.b + 8 * j;
+    float (&y)[8] = k.x;
+    if (TURN != kKpNone && is && !k.value && d0 < a.hd) {
+        if constexpr (TURN == kKpHalves) {
+            const uint64_t at = (uint64_t)pos * (a.hd / 2);
+            const bool upper = d0 >= a.hd / 2;
+            float c[8], s[8];
+            kp_angles(a, at + (upper ? d0 - a.hd / 2 : d0), c, s);
+#pragma unroll
+            for (int m = 0; m < 8; ++m) y[m] = kp_turn<true>(y[m], c[m], k.z[m], upper ? -s[m] : s[m]);
+        } else {
+            kp_neighbours<true>(a, pos, d0, y);
+        }
+    }
+    float hi = y[0], lo = y[0], odd = y[0] * 0.f;  // odd: NaN where something is not finite
+#pragma unroll
+    for (int m = 1; m < 8; ++m) {
+        hi = fmaxf(hi, y[m]);
+        lo = fminf(lo, y[m]);
+        odd = fmaf(y[m], 0.f, odd);
+    }
+#pragma unroll
+    for (int m = 1; m < 4; m <<= 1) {
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, m));
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, m));
-        odd |= __shfl_xor_sync(0xffffffffu, odd, m);
+        odd += __shfl_xor_sync(0xffffffffu, odd, m);
     }
     // a block with a value that is not finite is NaN throughout; past what fp16
     // scales reach (|m| > 524032) values are held to the largest
-    const __half dh = odd ? __ushort_as_half(0x7fff)
+    const bool bad = odd != odd;
+    const __half dh = bad ? __ushort_as_half(0x7fff)
                           : __float2half_rn(fminf(fmaxf((hi >= -lo ? hi : lo) * -0.125f, -65504.f), 65504.f));
-    const float d = odd ? 0.f : __half2float(dh);
-    uint32_t code[4];
+    const float d = bad ? 0.f : __half2float(dh), mag = d == 0.f ? 3e38f : fabsf(d), inv = d == 0.f ? 0.f : __frcp_rn(mag);
+    uint32_t word = 0, code[8];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) code[k] = kp_code(y[k], d);
-    // lane j's half of key word c = j / 2: nibbles 0, 4, 1, 5 or 2, 6, 3, 7
-    uint32_t word = code[0] | code[1] << 16 | code[2] << 4 | code[3] << 20;
-    if (j & 1) word <<= 8;
-    word |= __shfl_xor_sync(0xffffffffu, word, 1);
-    if (pos < 0) return;
-    const uint32_t page = (uint32_t)a.pages[seq * a.pages_seq + ((uint32_t)pos >> a.page_log2)];
-    if (page >= a.n_page) {
-        bad |= kKvBadPage;
-        return;
+    for (int m = 0; m < 8; ++m) {
+        code[m] = bad ? 8u : kp_code(y[m], d, mag, inv);
+        word |= code[m] << (4 * (m / 2) + 16 * (m % 2));
     }
-    const uint32_t in = (uint32_t)pos & ((1u << a.page_log2) - 1), p = in % kKvTile;
-    uint8_t *tile = a.cache + ((((uint64_t)page * a.n_kv + head) << (a.page_log2 - 4)) + in / kKvTile) * kv4_tile(nb) +
-                    (value ? kv4_codes(nb) + kv4_scales(nb) : 0);
-    if (value)
-        *reinterpret_cast<uint16_t *>(tile + p * 16 * nb + (j ^ (p & 2 ? 4u : 0u)) * 2 * nb + 2 * b) =
-            (uint16_t)(code[0] | code[1] << 4 | code[2] << 8 | code[3] << 12);
-    else if (!(j & 1))
-        *reinterpret_cast<uint32_t *>(tile + p * 16 * nb + (j / 2) * 4 * nb + 4 * b) = word;
-    if (j == 0) *reinterpret_cast<__half *>(tile + kv4_codes(nb) + p * 2 * nb + 2 * b) = dh;
+    if (!is) return;
+    const uint32_t in = pos & ((1u << a.page_log2) - 1), p = in % kKvTile;
+    uint8_t *tile = a.cache + ((((uint64_t)page * a.n_kv + k.head) << (a.page_log2 - 4)) + in / kKvTile) * kv4_tile(nb) +
+                    (k.value ? kv4_codes(nb) + kv4_scales(nb) : 0);
+    if (k.value) {
+        uint8_t *to = tile + p * 16 * nb + 2 * k.b + (2 * j ^ (p & 2 ? 4u : 0u)) * 2 * nb;  // and the unit after it
+        *reinterpret_cast<uint16_t *>(to) = (uint16_t)(code[0] | code[1] << 4 | code[2] << 8 | code[3] << 12);
+        *reinterpret_cast<uint16_t *>(to + 2 * nb) = (uint16_t)(code[4] | code[5] << 4 | code[6] << 8 | code[7] << 12);
+    } else {
+        *reinterpret_cast<uint32_t *>(tile + p * 16 * nb + j * 4 * nb + 4 * k.b) = word;
+    }
+    if (j == 0) *reinterpret_cast<__half *>(tile + kv4_codes(nb) + p * 2 * nb + 2 * k.b) = dh;
 }
 
-__global__ void __launch_bounds__(kKpThreads) kv4_append_kernel(const __grid_constant__ Kv4AppendArgs a) {
+// A token for each blockIdx.x, its rows dealt out over blockIdx.y.
+template <typename T, KpTurn TURN>
+__global__ void __launch_bounds__(kKpThreads, 8) kv4_append_kernel(const __grid_constant__ Kv4AppendArgs a) {
     pdl_wait();
+    const uint32_t seq = blockIdx.x / a.n_query, t = blockIdx.x - seq * a.n_query, at = blockIdx.y * kKpThreads + threadIdx.x,
+                   step = gridDim.y * kKpThreads;
     uint32_t bad = 0;
-    if (blockIdx.x < a.q_blocks)
-        kp_query(a, blockIdx.x * kKpThreads + threadIdx.x, bad);
-    else
-        kp_block(a, (blockIdx.x - a.q_blocks) * kKpThreads + threadIdx.x, bad);
-    if (bad) atomicOr(a.err, bad);
+    const int32_t pos = kp_position(a, seq, t, bad);
+    if (pos < 0) {
+        if (bad && at == 0) atomicOr(a.err, bad);
+        return;
+    }
+    const uint64_t from = seq * a.q.seq + t * a.q.tok, to = seq * a.q_out.seq + t * a.q_out.tok;
+    const uint32_t nq = a.n_head * (a.hd * sizeof(T) / 32), nkv = 2 * a.n_kv * kv4_blocks(a.hd) * 4;
+    const uint32_t page = (uint32_t)a.pages[seq * a.pages_seq + ((uint32_t)pos >> a.page_log2)];
+    KpQuery<T> q;
+    for (uint32_t i = at; i < nq; i += step) {
+        kp_query_load<T>(a, i, from, q);
+        kp_query_store<T, TURN>(a, q, to, (uint32_t)pos);
+    }
+    if (page >= a.n_page) {
+        if (at == 0) atomicOr(a.err, kKvBadPage);
+        return;
+    }
+    KpBlock k;
+    for (uint32_t i = at; i - threadIdx.x % 32 < nkv; i += step) {
+        kp_block_load<T, TURN>(a, i, seq, t, i < nkv, k);
+        kp_block_store<TURN>(a, k, i, page, (uint32_t)pos, i < nkv);
+    }
 }
 
 struct Kv4ReadArgs {

@@ -84,30 +84,30 @@ def _page_size(head_dim: int, line: int) -> int:
     raise ValueError(f"cache: a line of {line} bytes is no page of head_dim {head_dim}")
 
 
-def _cache(cache, heads: int, head_dim: int, dev: int):
-    """(page size, pages) of a cache."""
+def _refuse_cache(cache, heads: int, dev: int):
     if cache is None:
         raise ValueError("cache is missing")
-    shape = cache.shape
-    if (cache.dtype is not torch.uint8 or len(shape) != 3 or shape[1] != heads or cache.get_device() != dev
-            or not cache.is_contiguous()):
-        raise ValueError(f"cache: expected contiguous torch.uint8 [n_page, {heads}, page bytes] on cuda:{dev}, "
-                         f"got {cache.dtype} {tuple(shape)} on {cache.device}")
-    return _page_size(head_dim, shape[2]), shape[0]
+    raise ValueError(f"cache: expected contiguous torch.uint8 [n_page, {heads}, page bytes] on cuda:{dev}, "
+                     f"got {cache.dtype} {tuple(cache.shape)} on {cache.device}")
 
 
-def _table(pages, n: int, dev: int):
-    """(max_pages, row stride) of a page table."""
+def _refuse_pages(pages, n: int, dev: int):
     if pages is None:
         raise ValueError("pages is missing")
-    shape = pages.shape
-    if pages.dtype is not torch.int32 or len(shape) != 2 or shape[0] != n or pages.get_device() != dev:
-        raise ValueError(f"pages: expected torch.int32 [{n}, max_pages] on cuda:{dev}, "
-                         f"got {pages.dtype} {tuple(shape)} on {pages.device}")
-    st = pages.stride()
-    if st[1] != 1 and shape[1] > 1:
-        raise ValueError("pages: the last dimension must be contiguous")
-    return shape[1], st[0]
+    raise ValueError(f"pages: expected torch.int32 [{n}, max_pages] on cuda:{dev}, the last dimension contiguous, "
+                     f"got {pages.dtype} {tuple(pages.shape)} on {pages.device}")
+
+
+def _tables(a, cache, pages, n: int, heads: int, head_dim: int, dev: int) -> None:
+    """The arguments of a cache and its page table."""
+    if (cache is None or cache.dtype is not torch.uint8 or cache.dim() != 3 or (cs := cache.shape)[1] != heads
+            or cache.get_device() != dev or not cache.is_contiguous()):
+        _refuse_cache(cache, heads, dev)
+    a.page_size, a.n_page, a.cache = _page_size(head_dim, cs[2]), cs[0], cache.data_ptr()
+    if (pages is None or pages.dtype is not torch.int32 or pages.dim() != 2 or (ps := pages.shape)[0] != n
+            or pages.get_device() != dev or ((st := pages.stride())[1] != 1 and ps[1] > 1)):
+        _refuse_pages(pages, n, dev)
+    a.max_pages, a.pages_stride, a.pages = ps[1], st[0], pages.data_ptr()
 
 
 def _ints(t, what: str, shape, dev: int) -> int:
@@ -116,20 +116,13 @@ def _ints(t, what: str, shape, dev: int) -> int:
     return t.data_ptr()
 
 
-def _rows(t, what: str, shape, dtype, dev: int):
-    """(address, strides) of rows [n_seq, n_query, heads, head_dim]."""
-    if t is None or t.dtype is not dtype or t.shape != shape or t.get_device() != dev or (st := t.stride())[3] != 1:
-        _refuse(t, what, shape, dtype, dev)
-    return t.data_ptr(), st
-
-
 def _overlap(a, b) -> bool:
     """Whether the bytes from first to last of two tensors meet."""
-    def span(t):
-        p = t.data_ptr()
-        return p, p + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    def end(t):
+        if t.is_contiguous():
+            return t.data_ptr() + t.numel() * t.element_size()
+        return t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
 
 
 def append(q, k, v, cache, pages, lengths, cos=None, sin=None, halves: bool = False, n_new=None, q_out=None):
@@ -145,46 +138,51 @@ def append(q, k, v, cache, pages, lengths, cos=None, sin=None, halves: bool = Fa
     if k is None or k.dim() != 4:
         raise ValueError("k must be [n_seq, n_query, n_head_kv, head_dim]")
     dt, dev, shape = k.dtype, k.get_device(), k.shape
-    if dt not in TYPE_IDS:
+    kind = TYPE_IDS.get(dt)
+    if kind is None:
         raise ValueError(f"dtype must be one of {list(TYPE_IDS)}")
     if dev < 0 or torch.cuda.current_device() != dev:
         raise ValueError("append: k and the current device differ")
     n_seq, n_query, heads, hd = shape
-    a = AppendArgs()
-    a.type, a.n_seq, a.n_query, a.n_head_kv, a.head_dim = TYPE_IDS[dt], n_seq, n_query, heads, hd
-    a.k, st = _rows(k, "k", shape, dt, dev)
-    a.k_seq_stride, a.k_token_stride, a.k_head_stride, _ = st
-    a.v, st = _rows(v, "v", shape, dt, dev)
-    a.v_seq_stride, a.v_token_stride, a.v_head_stride, _ = st
-    a.page_size, a.n_page = _cache(cache, heads, hd, dev)
-    a.cache = cache.data_ptr()
-    a.max_pages, a.pages_stride = _table(pages, n_seq, dev)
-    a.pages = pages.data_ptr()
+    a = AppendArgs(kind, n_seq, n_query, 0, heads, hd)
+    if (st := k.stride())[3] != 1:
+        _refuse(k, "k", shape, dt, dev)
+    a.k, a.k_seq_stride, a.k_token_stride, a.k_head_stride = k.data_ptr(), st[0], st[1], st[2]
+    if v is None or v.dtype is not dt or v.shape != shape or v.get_device() != dev or (st := v.stride())[3] != 1:
+        _refuse(v, "v", shape, dt, dev)
+    a.v, a.v_seq_stride, a.v_token_stride, a.v_head_stride = v.data_ptr(), st[0], st[1], st[2]
+    _tables(a, cache, pages, n_seq, heads, hd, dev)
     a.lengths = _ints(lengths, "lengths", (n_seq,), dev)
     if n_new is not None:
         a.n_new = _ints(n_new, "n_new", (n_seq,), dev)
     if q is not None:
         if q.dim() != 4:
             raise ValueError("q must be [n_seq, n_query, n_head, head_dim]")
-        qs = torch.Size((n_seq, n_query, q.shape[2], hd))
-        a.n_head = qs[2]
-        a.q, st = _rows(q, "q", qs, dt, dev)
-        a.q_seq_stride, a.q_token_stride, a.q_head_stride, _ = st
+        qs = q.shape
+        if (q.dtype is not dt or qs[0] != n_seq or qs[1] != n_query or qs[3] != hd or q.get_device() != dev
+                or (st := q.stride())[3] != 1):
+            _refuse(q, "q", torch.Size((n_seq, n_query, qs[2], hd)), dt, dev)
+        a.n_head, a.q, a.q_seq_stride, a.q_token_stride, a.q_head_stride = qs[2], q.data_ptr(), st[0], st[1], st[2]
         if q_out is None:
-            q_out = torch.empty(qs, dtype=dt, device=k.device) if n_new is None else torch.zeros(qs, dtype=dt, device=k.device)
-        a.q_out, so = _rows(q_out, "q_out", qs, dt, dev)
-        a.q_out_seq_stride, a.q_out_token_stride, a.q_out_head_stride, _ = so
-        if (a.q != a.q_out or st != so) and q.numel() and _overlap(q, q_out):
+            q_out = (torch.empty if n_new is None else torch.zeros)(qs, dtype=dt, device=k.device)
+            so = q_out.stride()
+        elif q_out.dtype is not dt or q_out.shape != qs or q_out.get_device() != dev or (so := q_out.stride())[3] != 1:
+            _refuse(q_out, "q_out", qs, dt, dev)
+        elif q_out is not q and (so != st or q_out.data_ptr() != a.q) and _overlap(q, q_out):
             raise ValueError("q_out must be q itself or memory apart from it")
+        a.q_out, a.q_out_seq_stride, a.q_out_token_stride, a.q_out_head_stride = q_out.data_ptr(), so[0], so[1], so[2]
     elif q_out is not None:
         raise ValueError("q_out without q")
     if cos is not None or sin is not None:
         for t, what in ((cos, "cos"), (sin, "sin")):
-            if (t is None or t.dtype is not torch.float32 or t.dim() != 2 or t.shape != (cos if cos is not None else t).shape
-                    or t.shape[1] * 2 != hd or t.get_device() != dev or not t.is_contiguous()):
-                raise ValueError(f"{what}: expected contiguous torch.float32 [n_pos, {hd // 2}] on cuda:{dev}, cos and sin alike")
+            if (t is None or t.dtype is not torch.float32 or t.dim() != 2 or t.shape[1] * 2 != hd or t.get_device() != dev
+                    or not t.is_contiguous()):
+                raise ValueError(f"{what}: expected contiguous torch.float32 [n_pos, {hd // 2}] on cuda:{dev}")
+        if cos.shape != sin.shape:
+            raise ValueError("cos and sin must have the same shape")
         a.cos, a.sin, a.n_pos = cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-    a.halves = 1 if halves else 0
+    if halves:
+        a.halves = 1
     lib = native.product()
     if lib.fwb_kv4_append_dev(ctypes.byref(a), _raw_stream(dev)) != 0:
         raise FwbError(_err(lib))
@@ -194,7 +192,8 @@ def append(q, k, v, cache, pages, lengths, cos=None, sin=None, halves: bool = Fa
 def read(cache, pages, start, n: int, *, head_dim: int, dtype: torch.dtype, lengths=None, k=None, v=None):
     """Positions start[s] .. start[s] + n - 1 of every sequence (fwb_kv4_read_dev)
     -> (k, v), each [n_seq, n, n_head_kv, head_dim]; zeros at and past lengths."""
-    if dtype not in TYPE_IDS:
+    kind = TYPE_IDS.get(dtype)
+    if kind is None:
         raise ValueError(f"dtype must be one of {list(TYPE_IDS)}")
     if cache is None or cache.dim() != 3:
         raise ValueError("cache must be [n_page, n_head_kv, page bytes]")
@@ -205,24 +204,19 @@ def read(cache, pages, start, n: int, *, head_dim: int, dtype: torch.dtype, leng
         raise ValueError("read: the cache and the current device differ")
     if not 0 <= n < 1 << 32:
         raise ValueError(f"size {n} out of range")
-    a = ReadArgs()
-    a.type, a.n_seq, a.n, a.n_head_kv, a.head_dim = TYPE_IDS[dtype], n_seq, n, heads, head_dim
-    a.page_size, a.n_page = _cache(cache, heads, head_dim, dev)
-    a.cache = cache.data_ptr()
-    a.max_pages, a.pages_stride = _table(pages, n_seq, dev)
-    a.pages = pages.data_ptr()
+    a = ReadArgs(kind, n_seq, n, heads, head_dim)
+    _tables(a, cache, pages, n_seq, heads, head_dim, dev)
     a.start = _ints(start, "start", (n_seq,), dev)
     if lengths is not None:
         a.lengths = _ints(lengths, "lengths", (n_seq,), dev)
-    shape = torch.Size((n_seq, n, heads, head_dim))
-    if k is None:
-        k = torch.empty(shape, dtype=dtype, device=cache.device)
-    elif k.dtype is not dtype or k.shape != shape or k.get_device() != dev or not k.is_contiguous():
-        _refuse(k, "k", shape, dtype, dev)
-    if v is None:
-        v = torch.empty(shape, dtype=dtype, device=cache.device)
-    elif v.dtype is not dtype or v.shape != shape or v.get_device() != dev or not v.is_contiguous():
-        _refuse(v, "v", shape, dtype, dev)
+    if k is None and v is None:
+        k, v = cache.new_empty((2, n_seq, n, heads, head_dim), dtype=dtype).unbind()
+    else:
+        shape = torch.Size((n_seq, n, heads, head_dim))
+        k, v = (cache.new_empty(shape, dtype=dtype) if t is None else t for t in (k, v))
+        for t, what in ((k, "k"), (v, "v")):
+            if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+                _refuse(t, what, shape, dtype, dev)
     a.k, a.v = k.data_ptr(), v.data_ptr()
     lib = native.product()
     if lib.fwb_kv4_read_dev(ctypes.byref(a), _raw_stream(dev)) != 0:
