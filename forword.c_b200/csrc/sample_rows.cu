@@ -8,27 +8,21 @@
 namespace fwb {
 namespace {
 
-template <typename T, bool VEC>
-bool launch_rows(const SampleRowsArgs &k, uint32_t rows, uint32_t cluster, cudaStream_t st) {
-    static bool ready[64] = {};
-    if (!opt_in(sample_rows_kernel<T, VEC>, sizeof(SrSmem), ready, "fwb_sample_rows")) return false;
-    return launched(launch_after(sample_rows_kernel<T, VEC>, dim3(rows * cluster), kSrThreads, sizeof(SrSmem), cluster, st, k),
-                    "fwb_sample_rows launch");
-}
-
 template <typename T>
 bool run_rows(SampleRowsArgs &k, uint32_t rows, cudaStream_t st) {
-    // Blocks of a row: enough that a block's slice stays below kSrSlice, and as
-    // many as keep the device's SMs busy with the rows at hand while a slice is
-    // worth a block.
+    // Blocks of a row: as many as a slice needs, and as keep the device's SMs
+    // busy with the rows at hand while a slice is worth a block.
     const uint32_t sms = device_sms();
     uint32_t cluster = 1;
     while (cluster < kSrCluster && ((uint64_t)cluster * kSrSlice < k.n_vocab ||
                                     ((uint64_t)rows * cluster * 2 <= 2 * sms && cluster * 4096 < k.n_vocab)))
         cluster *= 2;
     k.slice = ((k.n_vocab + cluster - 1) / cluster + 7) / 8 * 8;
-    const bool vec = ((uintptr_t)k.logits | k.stride * sizeof(T)) % 16 == 0;
-    return vec ? launch_rows<T, true>(k, rows, cluster, st) : launch_rows<T, false>(k, rows, cluster, st);
+    k.vec = ((uintptr_t)k.logits | k.stride * sizeof(T)) % 16 == 0;
+    static bool ready[64] = {};
+    if (!opt_in(sample_rows_kernel<T>, sizeof(SrSmem), ready, "fwb_sample_rows")) return false;
+    return launched(launch_after(sample_rows_kernel<T>, dim3(rows * cluster), kSrThreads, sizeof(SrSmem), cluster, st, k),
+                    "fwb_sample_rows launch");
 }
 
 }  // namespace

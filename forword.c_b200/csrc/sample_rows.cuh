@@ -8,22 +8,27 @@
 // is its first entry at which the running mass exceeds u times the prefix's.
 //
 // Every question is thus where a running count or mass passes a limit, and is
-// answered without a sort.  A cluster of blocks shares a row.  The weights'
-// exponents y = (x - max) log2(e) / T fall into 2048 bins of 1/32 octave (what
-// lies 64 octaves below the maximum weighs less than 2^-46 of any sum and is
-// left out); a bin holds a count and the sum of 2^22 (1 - w / w_bin), both
-// 32-bit integers, so masses are sums of integers: exact, and the same in any
-// order.  The first block scans the bins, and only the entries of the bin
-// where a limit falls (or, where few entries come before it, of all bins up to
-// there) are gathered, sorted and walked.  A bin of more than kSrList entries
-// is first divided again by the logits' bits, and equal logits by index.
+// answered without a sort of the row.  A cluster of blocks shares a row.  The
+// weights' exponents y = (x - max) log2(e) / T fall into bins of
+// 1/32 octave (what lies 64 octaves below the maximum weighs less than 2^-46 of
+// any sum and is left out); a bin holds a count and the sum of 2^22 (1 - w /
+// w_bin), both 32-bit integers, so masses are sums of integers: exact, and the
+// same in any order.  Only the first half of the bins is filled at once; most tokens of
+// a vocabulary lie below it, and are added up by threads instead of by
+// additions in shared memory.  Every block sums a share of the bins for all, and where few
+// entries lie up to the bin that decides, these are gathered in the first
+// block, sorted and walked.  Otherwise the first block asks for more: the other
+// bins, then each limit's bin by itself; one of more than kSrList entries is
+// divided by the logits' bits, and equal logits by index.
 //
-// Bound: latency for few rows (a row is three or four rounds of the cluster),
-// the shared-memory additions for many.
+// Bound: latency for few rows (loads, four barriers of the cluster, a short
+// sort), instruction issue for many.
 #pragma once
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -32,6 +37,8 @@ namespace fwb {
 namespace cg = cooperative_groups;
 
 constexpr int kSrThreads = 512, kSrBins = 2048, kSrList = 2048;
+constexpr int kSrNear = 1024;              // bins filled at once
+constexpr int kSrKept = 1024;              // entries of the first half of these that a block keeps a list of
 constexpr uint32_t kSrSlice = 32768;       // most entries of a block: its bins' sums stay below 2^32
 constexpr uint32_t kSrCluster = 8;         // most blocks of a row
 constexpr float kSrUnit = 4194304.f;       // 2^22
@@ -39,7 +46,7 @@ constexpr float kSrUnit = 4194304.f;       // 2^22
 struct SampleRowsArgs {
     const void *logits;
     uint64_t stride;
-    uint32_t n_vocab, slice;
+    uint32_t n_vocab, slice, vec;           // vec: rows are 16-byte aligned
     const float *u, *temp, *top_p, *min_p;  // the last three and top_k may be null
     const int32_t *top_k;
     int32_t *token;
@@ -51,10 +58,10 @@ struct SampleRowsArgs {
 struct SrRange {
     uint32_t k0, k1, klo, khi, ilo, ihi;
 };
-enum SrOp : uint32_t { kSrDone, kSrHist, kSrLow, kSrCollect };
+enum SrOp : uint32_t { kSrDone, kSrFar, kSrHist, kSrLow, kSrCollect };
 
 struct SrSmem {
-    uint32_t count[kSrBins], frac[kSrBins];
+    uint2 bins[kSrBins];                 // {entries, the sum of what their weights lack}
     uint32_t cum_c[kSrBins];             // (first block) entries and mass up to and with a bin
     double cum_w[kSrBins];
     // (first block) the list, key << 32 | ~index, with the mass up to and with
@@ -69,10 +76,12 @@ struct SrSmem {
     };
     unsigned long long best[kSrCluster]; // the blocks' largest entries
     uint32_t bad[kSrCluster];
-    uint32_t op, shift, listed;
+    double far[kSrCluster];              // the blocks' masses below the near bins
+    unsigned long long kept[kSrKept];    // key << 32 | ~index
+    uint32_t op, shift, listed, n_kept;
     SrRange range;
     uint32_t found;
-    double wsum[kSrThreads / 32];
+    double wsum[kSrThreads / 32], steps[32];
     uint32_t csum[kSrThreads / 32];
     unsigned long long wbest[kSrThreads / 32];
     uint32_t wbad[kSrThreads / 32];
@@ -84,62 +93,116 @@ __device__ __forceinline__ uint32_t sr_key(float x) {
 }
 __device__ __forceinline__ float sr_value(uint32_t key) { return __uint_as_float(key >> 31 ? key & 0x7fffffffu : ~key); }
 
-template <typename T> __device__ __forceinline__ float sr_float(T x);
-template <> __device__ __forceinline__ float sr_float<float>(float x) { return x; }
-template <> __device__ __forceinline__ float sr_float<__half>(__half x) { return __half2float(x); }
-template <> __device__ __forceinline__ float sr_float<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
-
-// f(logit, index) for every entry of this block's slice.  VEC: 16-byte loads.
-template <typename T, bool VEC, typename F>
-__device__ __forceinline__ void sr_each(const T *row, uint32_t begin, uint32_t end, F f) {
-    if constexpr (VEC) {
-        constexpr uint32_t N = 16 / sizeof(T);
-        const uint32_t whole = begin + (end - begin) / N * N;  // (begin is a multiple of N)
-#pragma unroll 2
-        for (uint32_t i = begin + threadIdx.x * N; i < whole; i += kSrThreads * N) {
-            const uint4 v = *reinterpret_cast<const uint4 *>(row + i);
-            const T *x = reinterpret_cast<const T *>(&v);
+// A block's slice of a row: read again by every pass, from the caches after the
+// first (held in registers, the passes' unrolled code spilled: 2.5 times slower).
+template <typename T>
+struct SrSlice {
+    static constexpr uint32_t N = 16 / sizeof(T);
+    const T *row;
+    uint32_t begin, end, vec;
+    // 16 bytes of entries from i on, those past the end -inf
+    __device__ __forceinline__ uint4 load(uint32_t i) const {
+        if (vec && i + N <= end) return __ldg(reinterpret_cast<const uint4 *>(row + i));
+        uint32_t w[4];
 #pragma unroll
-            for (uint32_t j = 0; j < N; ++j) f(sr_float<T>(x[j]), i + j);
+        for (uint32_t j = 0; j < N; ++j) {
+            if constexpr (sizeof(T) == 4) {
+                w[j] = i + j < end ? __float_as_uint(row[i + j]) : 0xff800000u;
+            } else {
+                const uint32_t h = i + j < end ? reinterpret_cast<const uint16_t *>(row)[i + j]
+                                               : std::is_same<T, __half>::value ? 0xfc00u : 0xff80u;
+                w[j / 2] = j % 2 ? w[j / 2] | h << 16 : h;
+            }
         }
-        for (uint32_t i = whole + threadIdx.x; i < end; i += kSrThreads) f(sr_float<T>(row[i]), i);
-    } else {
-        for (uint32_t i = begin + threadIdx.x; i < end; i += kSrThreads) f(sr_float<T>(row[i]), i);
+        return make_uint4(w[0], w[1], w[2], w[3]);
     }
-}
+    // f(logit, index) for every entry, and for some of -inf past the end; U
+    // loads of a thread in flight
+    template <int U, typename F>
+    __device__ __forceinline__ void each(F f) const {
+#pragma unroll 1
+        for (uint32_t i = begin + threadIdx.x * N; i < end; i += U * kSrThreads * N) {
+            uint4 v[U];
+#pragma unroll
+            for (int m = 0; m < U; ++m) v[m] = load(i + m * kSrThreads * N);
+#pragma unroll
+            for (int m = 0; m < U; ++m) {
+                const uint32_t w[4] = {v[m].x, v[m].y, v[m].z, v[m].w};
+#pragma unroll
+                for (uint32_t j = 0; j < N; ++j) {
+                    float x;
+                    if constexpr (sizeof(T) == 4) x = __uint_as_float(w[j]);
+                    else if constexpr (std::is_same<T, __half>::value) x = __half2float(__ushort_as_half((uint16_t)(w[j / 2] >> (j % 2 * 16))));
+                    else x = __uint_as_float(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+                    f(x, i + m * kSrThreads * N + j);
+                }
+            }
+        }
+    }
+};
 
 // A row's constants and an entry's place: its bin and what its weight lacks to
 // the bin's, in units of 2^-22.  The exponent is formed as t + lo, t rounded
 // and lo its error.
 struct SrScale {
-    float top, hi, lo;  // log2(e) / T in two parts
+    float top, hi, lo;     // log2(e) / T in two parts
+    float low_hi, low_lo;  // log2(min_p)
     __device__ __forceinline__ void of(float x, float &t, float &rest) const {
         const float d = x - top;
         t = d * hi;
         rest = fmaf(d, lo, fmaf(d, hi, -t));
     }
+    __device__ __forceinline__ bool high(float t, float rest) const { return (t - low_hi) + (rest - low_lo) >= 0.f; }  // w >= min_p
     __device__ __forceinline__ uint32_t bin(float t) const { return (uint32_t)(t * -32.f); }
-    __device__ __forceinline__ uint32_t frac(float t, float rest, uint32_t k) const {
+    static __device__ __forceinline__ float weight(float y) {
         float w;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(fmaf((float)k, 1.f / 32, t) + rest));
-        return (uint32_t)fmaxf(rintf((1.f - w) * kSrUnit), 0.f);
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(y));
+        return w;
+    }
+    __device__ __forceinline__ uint32_t frac(float t, float rest, uint32_t k) const {
+        return (uint32_t)fmaxf(rintf((1.f - weight(fmaf((float)k, 1.f / 32, t) + rest)) * kSrUnit), 0.f);
     }
 };
 
-__device__ __forceinline__ double sr_mass(uint32_t bin, uint32_t count, unsigned long long frac) {
-    return exp2((double)bin * (-1. / 32)) * ((double)count - (double)frac * (1. / 4194304));
+// steps: 2^(-i / 32) for i below 32
+__device__ __forceinline__ double sr_mass(const double *steps, uint32_t bin, uint32_t count, unsigned long long frac) {
+    return steps[bin % 32] * __hiloint2double((1023 - bin / 32) << 20, 0) * ((double)count - (double)frac * (1. / 4194304));
 }
 
-// Inclusive sums over the block's threads, four values each.
-__device__ __forceinline__ void sr_scan(SrSmem &sh, uint32_t (&c)[4], double (&w)[4]) {
+// What a block does for the first one, which asked through sh.op: counts the
+// entries of a range in bins, or gives them to the first block's list.
+template <typename T>
+__device__ __noinline__ void sr_serve(SrSmem &sh, SrSmem &first, SrSlice<T> x, SrScale s) {
+    const SrRange r = sh.range;
+    const uint32_t op = sh.op, shift = sh.shift;
+    x.template each<2>([&](float v, uint32_t i) {
+        float t, rest;
+        s.of(v, t, rest);
+        const uint32_t k = s.bin(t), key = sr_key(v);
+        if (v == -INFINITY || k < r.k0 || k > r.k1 || key < r.klo || key > r.khi || i < r.ilo || i > r.ihi) return;
+        if (op == kSrCollect) {
+            const uint32_t at = atomicAdd(&first.listed, 1u);
+            if (at < kSrList) first.list[at] = (unsigned long long)key << 32 | ~i;
+            return;
+        }
+        const uint32_t at = op == kSrFar ? k : op == kSrLow ? 2 * (k - r.k0) + (s.high(t, rest) ? 0 : 1)
+                            : r.klo < r.khi ? (r.khi - key) >> shift : (i - r.ilo) >> shift;
+        atomicAdd(&sh.bins[at].x, 1u);
+        atomicAdd(&sh.bins[at].y, s.frac(t, rest, k));
+    });
+}
+
+// Inclusive sums over the block's threads, K values each.
+template <int K>
+__device__ __forceinline__ void sr_scan(SrSmem &sh, uint32_t (&c)[K], double (&w)[K]) {
     const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-    for (int i = 1; i < 4; ++i) {
+    for (int i = 1; i < K; ++i) {
         c[i] += c[i - 1];
         w[i] += w[i - 1];
     }
-    uint32_t cs = c[3];
-    double ws = w[3];
+    uint32_t cs = c[K - 1];
+    double ws = w[K - 1];
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
         const uint32_t x = __shfl_up_sync(0xffffffffu, cs, d);
@@ -155,38 +218,43 @@ __device__ __forceinline__ void sr_scan(SrSmem &sh, uint32_t (&c)[4], double (&w
         sh.wsum[warp] = ws;
     }
     __syncthreads();
-    uint32_t cb = cs - c[3];
+    uint32_t cb = lane < kSrThreads / 32 && lane < warp ? sh.csum[lane] : 0;
+    double before = lane < kSrThreads / 32 && lane < warp ? sh.wsum[lane] : 0.;
+    cb = __reduce_add_sync(0xffffffffu, cb) + cs - c[K - 1];
+#pragma unroll
+    for (int d = 8; d; d >>= 1) before += __shfl_xor_sync(0xffffffffu, before, d);
+    before = __shfl_sync(0xffffffffu, before, 0);
     double wb = __shfl_up_sync(0xffffffffu, ws, 1);
     if (!lane) wb = 0.;
-    double before = 0.;
-    for (uint32_t v = 0; v < warp; ++v) {
-        cb += sh.csum[v];
-        before += sh.wsum[v];
-    }
     wb += before;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < K; ++i) {
         c[i] += cb;
         w[i] += wb;
     }
 }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(kSrThreads) sample_rows_kernel(const __grid_constant__ SampleRowsArgs a) {
+template <typename T>
+__global__ void __launch_bounds__(kSrThreads, 2) sample_rows_kernel(const __grid_constant__ SampleRowsArgs a) {
     extern __shared__ __align__(16) uint8_t dyn[];
     SrSmem &sh = *reinterpret_cast<SrSmem *>(dyn);
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, blocks = cluster.num_blocks(),
                    rank = cluster.block_rank(), row = blockIdx.x / blocks;
     pdl_wait();
-    const T *const x = static_cast<const T *>(a.logits) + row * a.stride;
-    const uint32_t begin = min(rank * a.slice, a.n_vocab), end = min(begin + a.slice, a.n_vocab);
+    const uint32_t begin = min(rank * a.slice, a.n_vocab);
+    const SrSlice<T> x = {static_cast<const T *>(a.logits) + row * a.stride, begin, min(begin + a.slice, a.n_vocab), a.vec};
+    const float temp = a.temp ? a.temp[row] : 1.f, u = a.u[row], low = a.min_p ? a.min_p[row] : 0.f;
+    const double top_p = a.top_p ? (double)a.top_p[row] : 1.;
+    const int32_t top_k = a.top_k ? a.top_k[row] : 0;
+    for (uint32_t b = tid; b < kSrNear; b += kSrThreads) sh.bins[b] = make_uint2(0, 0);
+    if (tid == 0) sh.listed = sh.n_kept = 0;
 
     // --- the largest entry ---
     {
         float best = -INFINITY;
         uint32_t at = 0xffffffffu, bad = 0;
-        sr_each<T, VEC>(x, begin, end, [&](float v, uint32_t i) {
+        x.template each<4>([&](float v, uint32_t i) {
             bad |= !(v < INFINITY);
             if (v > best) {
                 best = v;
@@ -204,31 +272,39 @@ __global__ void __launch_bounds__(kSrThreads) sample_rows_kernel(const __grid_co
             sh.wbest[warp] = key;
             sh.wbad[warp] = bad;
         }
-        for (uint32_t b = tid; b < kSrBins; b += kSrThreads) sh.count[b] = sh.frac[b] = 0;
-        if (tid == 0) sh.listed = 0;
         __syncthreads();
-        if (tid < blocks) {
-            key = sh.wbest[0];
-            bad = sh.wbad[0];
-            for (int w = 1; w < kSrThreads / 32; ++w) {
-                key = sh.wbest[w] > key ? sh.wbest[w] : key;
-                bad |= sh.wbad[w];
+        if (warp == 0) {
+            key = lane < kSrThreads / 32 ? sh.wbest[lane] : 0;
+            bad = __any_sync(0xffffffffu, lane < kSrThreads / 32 ? sh.wbad[lane] : 0);
+#pragma unroll
+            for (int d = 8; d; d >>= 1) {
+                const unsigned long long o = __shfl_xor_sync(0xffffffffu, key, d);
+                key = o > key ? o : key;
             }
-            SrSmem &to = *cluster.map_shared_rank(&sh, tid);
-            to.best[rank] = key;
-            to.bad[rank] = bad;
+            key = __shfl_sync(0xffffffffu, key, 0);
+            if (lane < blocks) {
+                SrSmem &to = *cluster.map_shared_rank(&sh, lane);
+                to.best[rank] = key;
+                to.bad[rank] = bad;
+            }
         }
-        cluster.sync();
     }
+    SrScale s;
+    cluster.barrier_arrive();
+    const double scale = fmin(1.4426950408889634 / (double)temp, 1e30), low2 = low > 0.f ? log2((double)low) : 0.;
+    s.hi = (float)scale;
+    s.lo = (float)(scale - (double)s.hi);
+    s.low_hi = (float)low2;
+    s.low_lo = (float)(low2 - (double)s.low_hi);
+    if (tid < 32) sh.steps[tid] = exp2((double)tid * (-1. / 32));
+    cluster.barrier_wait();
     unsigned long long best = sh.best[0];
     uint32_t dead = sh.bad[0];
     for (uint32_t b = 1; b < blocks; ++b) {
         best = sh.best[b] > best ? sh.best[b] : best;
         dead |= sh.bad[b];
     }
-    SrScale s;
     s.top = sr_value((uint32_t)(best >> 32));
-    const float temp = a.temp ? a.temp[row] : 1.f, u = a.u[row];
     if (dead || s.top == -INFINITY || temp != temp || u != u || temp <= 0.f) {  // (the same in every block)
         if (rank == 0 && tid == 0) {
             const bool greedy = !dead && s.top != -INFINITY && temp <= 0.f;
@@ -237,71 +313,70 @@ __global__ void __launch_bounds__(kSrThreads) sample_rows_kernel(const __grid_co
         }
         return;
     }
+    // --- the near bins, and what lies below them ---
     {
-        const double c = fmin(1.4426950408889634 / (double)temp, 1e30);
-        s.hi = (float)c;
-        s.lo = (float)(c - (double)s.hi);
-    }
-
-    // --- the row's bins ---
-    sr_each<T, VEC>(x, begin, end, [&](float v, uint32_t) {
-        float t, rest;
-        s.of(v, t, rest);
-        const uint32_t k = s.bin(t);
-        if (k < kSrBins && v != -INFINITY) {
-            atomicAdd(&sh.count[k], 1u);
-            atomicAdd(&sh.frac[k], s.frac(t, rest, k));
-        }
-    });
-    cluster.sync();
-
-    // What the blocks do for the first one, which asks through sh.op.
-    const float low = a.min_p ? a.min_p[row] : 0.f;
-    const double low2 = low > 0.f ? log2((double)low) : 0.;
-    const float low_hi = (float)low2, low_lo = (float)(low2 - (double)low_hi);
-    auto high = [&](float t, float rest) { return (t - low_hi) + (rest - low_lo) >= 0.f; };  // w >= min_p
-    auto serve = [&]() {
-        const SrRange r = sh.range;
-        const uint32_t op = sh.op, shift = sh.shift;
-        SrSmem &first = *cluster.map_shared_rank(&sh, 0);
-        sr_each<T, VEC>(x, begin, end, [&](float v, uint32_t i) {
+        float far = 0.f;
+        x.template each<2>([&](float v, uint32_t i) {
             float t, rest;
             s.of(v, t, rest);
-            const uint32_t k = s.bin(t);
-            if (k < r.k0 || k > r.k1 || v == -INFINITY) return;
-            if (op == kSrLow) {
-                const uint32_t at = 2 * (k - r.k0) + (high(t, rest) ? 0 : 1);
-                atomicAdd(&sh.count[at], 1u);
-                atomicAdd(&sh.frac[at], s.frac(t, rest, k));
-                return;
-            }
-            const uint32_t key = sr_key(v);
-            if (key < r.klo || key > r.khi || i < r.ilo || i > r.ihi) return;
-            if (op == kSrCollect) {
-                const uint32_t at = atomicAdd(&first.listed, 1u);
-                if (at < kSrList) first.list[at] = (unsigned long long)key << 32 | ~i;
-            } else {
-                const uint32_t at = r.klo < r.khi ? (r.khi - key) >> shift : (i - r.ilo) >> shift;
-                atomicAdd(&sh.count[at], 1u);
-                atomicAdd(&sh.frac[at], s.frac(t, rest, k));
+            if (t < kSrNear * -1.f / 32) {
+                if (t > -48.f) far += s.weight(t);  // (what is less is less than 2^-30 of the mass, all of it)
+            } else if (v != -INFINITY) {
+                const uint32_t k = min(s.bin(t), kSrNear - 1u);
+                atomicAdd(&sh.bins[k].x, 1u);
+                atomicAdd(&sh.bins[k].y, s.frac(t, rest, k));
+                if (k < kSrNear / 2) {
+                    const uint32_t at = atomicAdd(&sh.n_kept, 1u);
+                    if (at < kSrKept) sh.kept[at] = (unsigned long long)sr_key(v) << 32 | ~i;
+                }
             }
         });
-    };
-    if (rank != 0) {
-        while (true) {
-            cluster.sync();  // the first block has asked
-            if (sh.op == kSrDone) break;
-            if (sh.op != kSrCollect) {
-                for (uint32_t b = tid; b < kSrBins; b += kSrThreads) sh.count[b] = sh.frac[b] = 0;
-                __syncthreads();
-            }
-            serve();
-            cluster.sync();
+        double far_w = far;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) far_w += __shfl_xor_sync(0xffffffffu, far_w, d);
+        if (lane == 0) sh.wsum[warp] = far_w;
+        __syncthreads();
+        if (tid < blocks) {
+            for (int w = 1; w < kSrThreads / 32; ++w) far_w = (w == 1 ? sh.wsum[0] : far_w) + sh.wsum[w];
+            cluster.map_shared_rank(&sh, tid)->far[rank] = far_w;
         }
-        return;
     }
+    cluster.sync();
+    // Each block sums a share of the bins, for all blocks.
+    {
+        const uint32_t share = kSrNear / blocks;
+        for (uint32_t b = tid; b < share; b += kSrThreads) {
+            const uint32_t at = rank * share + b;
+            uint2 v[kSrCluster];
+#pragma unroll
+            for (uint32_t k = 0; k < kSrCluster; ++k) v[k] = k < blocks ? cluster.map_shared_rank(&sh, k)->bins[at] : make_uint2(0, 0);
+            uint32_t c = 0;
+            unsigned long long f = 0;
+#pragma unroll
+            for (uint32_t k = 0; k < kSrCluster; ++k) {
+                c += v[k].x;
+                f += v[k].y;
+            }
+            const double w = c ? sr_mass(sh.steps, at, c, f) : 0.;
+#pragma unroll
+            for (uint32_t k = 0; k < kSrCluster; ++k)
+                if (k < blocks) {
+                    SrSmem &to = *cluster.map_shared_rank(&sh, k);
+                    to.cum_c[at] = c;
+                    to.cum_w[at] = w;
+                }
+        }
+    }
+    cluster.sync();
 
-    // --- the first block ---
+    // The bins that an operation counts in, made zeros.
+    auto clear = [&](uint32_t op) {
+        if (op == kSrCollect) return;
+        for (uint32_t b = (op == kSrFar ? kSrNear : 0) + tid; b < kSrBins; b += kSrThreads) sh.bins[b] = make_uint2(0, 0);
+        __syncthreads();
+    };
+
+    // What the first block does with the others' help.
     auto ask = [&](uint32_t op, const SrRange &r, uint32_t shift) {
         __syncthreads();
         if (tid < blocks) {
@@ -313,11 +388,8 @@ __global__ void __launch_bounds__(kSrThreads) sample_rows_kernel(const __grid_co
         if (tid == 0) sh.listed = 0;
         cluster.sync();
         if (op == kSrDone) return;
-        if (op != kSrCollect) {
-            for (uint32_t b = tid; b < kSrBins; b += kSrThreads) sh.count[b] = sh.frac[b] = 0;
-            __syncthreads();
-        }
-        serve();
+        clear(op);
+        sr_serve(sh, *cluster.map_shared_rank(&sh, 0), x, s);
         cluster.sync();
     };
     // All blocks' bins, summed up: those of the row, or of the divisions of bin `of`.
@@ -330,13 +402,13 @@ __global__ void __launch_bounds__(kSrThreads) sample_rows_kernel(const __grid_co
             unsigned long long f = 0;
             c[i] = 0;
             for (uint32_t k = 0; k < blocks; ++k) {
-                const SrSmem &from = *cluster.map_shared_rank(&sh, k);
-                c[i] += from.count[b];
-                f += from.frac[b];
+                const uint2 v = cluster.map_shared_rank(&sh, k)->bins[b];
+                c[i] += v.x;
+                f += v.y;
             }
-            w[i] = c[i] ? sr_mass(of < kSrBins ? of : b, c[i], f) : 0.;
+            w[i] = c[i] ? sr_mass(sh.steps, of < kSrBins ? of : b, c[i], f) : 0.;
         }
-        sr_scan(sh, c, w);
+        sr_scan<4>(sh, c, w);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             cum_c[4 * tid + i] = c[i];
@@ -344,21 +416,23 @@ __global__ void __launch_bounds__(kSrThreads) sample_rows_kernel(const __grid_co
         }
         __syncthreads();
     };
-    // The first bin up to and with which more than `count` entries, or more
-    // than `mass`, lie (without one, the last that holds any).
-    auto pass = [&](const uint32_t *cum_c, const double *cum_w, bool by_count, uint32_t count, double mass) {
-        if (tid == 0) sh.found = kSrBins;
+    // The first of `bins` bins up to and with which more than `count` entries, or
+    // more than `mass`, lie; without one `bins`, or with `any` the last that
+    // holds any.
+    auto pass = [&](const uint32_t *cum_c, const double *cum_w, uint32_t bins, bool by_count, uint32_t count, double mass, bool any) {
+        if (tid == 0) sh.found = bins;
         __syncthreads();
-        uint32_t at = kSrBins;
-        for (int i = 3; i >= 0; --i)
-            if (by_count ? cum_c[4 * tid + i] > count : cum_w[4 * tid + i] > mass) at = 4 * tid + i;
-        if (at < kSrBins) atomicMin(&sh.found, at);
+        const uint32_t each = bins / kSrThreads;
+        uint32_t at = bins;
+        for (int i = each - 1; i >= 0; --i)
+            if (by_count ? cum_c[each * tid + i] > count : cum_w[each * tid + i] > mass) at = each * tid + i;
+        if (at < bins) atomicMin(&sh.found, at);
         __syncthreads();
-        if (sh.found == kSrBins) {  // (read by all before it changes again)
+        if (any && sh.found == bins) {  // (read by all before it changes again)
             __syncthreads();
-            for (int i = 3; i >= 0; --i)
-                if (cum_c[4 * tid + i] == cum_c[kSrBins - 1]) at = 4 * tid + i;
-            if (at < kSrBins) atomicMin(&sh.found, at);
+            for (int i = each - 1; i >= 0; --i)
+                if (cum_c[each * tid + i] == cum_c[bins - 1]) at = each * tid + i;
+            if (at < bins) atomicMin(&sh.found, at);
         }
         __syncthreads();
         at = sh.found;
@@ -368,26 +442,35 @@ __global__ void __launch_bounds__(kSrThreads) sample_rows_kernel(const __grid_co
     uint32_t n = 0;            // entries of the list,
     uint32_t base_c = 0;       // and what comes before it
     double base_w = 0.;
-    // The entries of a range in order, with their running mass.
-    auto collect = [&](const SrRange &r) {
-        ask(kSrCollect, r, 0);
+    // The list in order, with its running mass.
+    auto order = [&]() {
         n = min(sh.listed, (uint32_t)kSrList);
-        uint32_t size = 32;
-        while (size < n) size *= 2;
-        for (uint32_t i = n + tid; i < size; i += kSrThreads) sh.list[i] = 0;
-        __syncthreads();
-        for (uint32_t k = 2; k <= size; k *= 2)
-            for (uint32_t j = k / 2; j; j /= 2) {
-                for (uint32_t p = tid; p < size / 2; p += kSrThreads) {
-                    const uint32_t i = 2 * p - (p & (j - 1)), o = i + j;
-                    const unsigned long long e = sh.list[i], f = sh.list[o];
-                    if ((e < f) == ((i & k) == 0)) {
-                        sh.list[i] = f;
-                        sh.list[o] = e;
+        if (n <= 128) {  // each entry counts the larger ones
+            const unsigned long long e = tid < n ? sh.list[tid] : 0;
+            uint32_t larger = 0;
+            if (tid < n)
+                for (uint32_t i = 0; i < n; ++i) larger += sh.list[i] > e;
+            __syncthreads();
+            if (tid < n) sh.list[larger] = e;
+            __syncthreads();
+        } else {
+            uint32_t size = 256;
+            while (size < n) size *= 2;
+            for (uint32_t i = n + tid; i < size; i += kSrThreads) sh.list[i] = 0;
+            __syncthreads();
+            for (uint32_t k = 2; k <= size; k *= 2)
+                for (uint32_t j = k / 2; j; j /= 2) {
+                    for (uint32_t p = tid; p < size / 2; p += kSrThreads) {
+                        const uint32_t i = 2 * p - (p & (j - 1)), o = i + j;
+                        const unsigned long long e = sh.list[i], f = sh.list[o];
+                        if ((e < f) == ((i & k) == 0)) {
+                            sh.list[i] = f;
+                            sh.list[o] = e;
+                        }
                     }
+                    __syncthreads();
                 }
-                __syncthreads();
-            }
+        }
         uint32_t c[4];
         double w[4];
 #pragma unroll
@@ -398,10 +481,10 @@ __global__ void __launch_bounds__(kSrThreads) sample_rows_kernel(const __grid_co
                 float t, rest;
                 s.of(sr_value((uint32_t)(sh.list[4 * tid + i] >> 32)), t, rest);
                 const uint32_t k = s.bin(t);
-                w[i] = sr_mass(k, 1, s.frac(t, rest, k));
+                w[i] = sr_mass(sh.steps, k, 1, s.frac(t, rest, k));
             }
         }
-        sr_scan(sh, c, w);
+        sr_scan<4>(sh, c, w);
 #pragma unroll
         for (int i = 0; i < 4; ++i) sh.list_w[4 * tid + i] = w[i];
         __syncthreads();
@@ -435,7 +518,7 @@ __global__ void __launch_bounds__(kSrThreads) sample_rows_kernel(const __grid_co
             while (span >> shift >= kSrBins) ++shift;
             ask(kSrHist, r, shift);
             gather(k, sh.sub_c, sh.sub_w);
-            const uint32_t b = pass(sh.sub_c, sh.sub_w, by_count, count - base_c, mass - base_w);
+            const uint32_t b = pass(sh.sub_c, sh.sub_w, kSrBins, by_count, count - base_c, mass - base_w, true);
             const uint32_t c0 = b ? sh.sub_c[b - 1] : 0;
             held = sh.sub_c[b] - c0;
             base_c += c0;
@@ -449,35 +532,86 @@ __global__ void __launch_bounds__(kSrThreads) sample_rows_kernel(const __grid_co
                 r.ihi = min(r.ihi, r.ilo + (1u << shift) - 1);
             }
         }
-        collect(r);
+        ask(kSrCollect, r, 0);
+        order();
     };
 
-    gather(kSrBins, sh.cum_c, sh.cum_w);
-    const uint32_t all = sh.cum_c[kSrBins - 1];
-    const double total = sh.cum_w[kSrBins - 1];
-    const int32_t top_k = a.top_k ? a.top_k[row] : 0;
-    const double top_p = a.top_p ? (double)a.top_p[row] : 1.;
-    const bool by_k = top_k > 0 && (uint32_t)top_k < all, by_p = top_p < 1., by_low = low > 0.f;
-    const uint32_t keep_k = by_k ? (uint32_t)top_k : all;
-    // the bin of weight min_p, give or take a rounding
-    const uint32_t low_bin = by_low ? (uint32_t)fmin(fmax(low2 * -32., 1.), kSrBins - 2.) : 0;
-    // the bin in which the last filter ends (without one, the draw)
-    uint32_t far;
-    if (by_k) {
-        far = pass(sh.cum_c, sh.cum_w, true, keep_k - 1, 0.);
-    } else if (by_p) {
-        far = pass(sh.cum_c, sh.cum_w, false, 0, top_p * total);
-        if (by_low) far = min(far, low_bin + 1);
-    } else if (by_low) {
-        far = low_bin + 1;
-    } else {
-        far = pass(sh.cum_c, sh.cum_w, false, 0, (double)u * total);
+    // --- every block: the near bins of all, and the bin in which the last filter
+    // ends (without one, the draw) ---
+    double total = 0.;
+    {
+        constexpr int K = kSrNear / kSrThreads;
+        uint32_t c[K];
+        double w[K];
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            c[i] = sh.cum_c[K * tid + i];
+            w[i] = sh.cum_w[K * tid + i];
+        }
+        sr_scan<K>(sh, c, w);
+#pragma unroll
+        for (int i = 0; i < K; ++i) {
+            sh.cum_c[K * tid + i] = c[i];
+            sh.cum_w[K * tid + i] = w[i];
+        }
+        __syncthreads();
+        for (uint32_t k = 0; k < blocks; ++k) total += sh.far[k];
     }
+    // What lies below the near bins decides nothing, and is left out, where its
+    // mass, or that of the most entries that top_k leaves of it (each below
+    // 2^-32 of the first's), is within the weights' own precision; but for a u of
+    // 1, which asks for the last entry.
+    const double near_w = sh.cum_w[kSrNear - 1];
+    const uint32_t near_c = sh.cum_c[kSrNear - 1];
+    const bool light = u < 1.f && (total <= near_w * (1. / 16777216) || (top_k > 0 && (uint32_t)top_k < near_c + 256));
+    total = light ? near_w : total + near_w;
+    uint32_t all = light ? near_c : 0xffffffffu, bins = kSrNear, keep_k;
+    bool by_k;
+    // the bin of weight min_p, give or take a rounding
+    const uint32_t low_bin = low > 0.f ? (uint32_t)fmin(fmax(low2 * -32., 1.), kSrBins - 2.) : 0;
+    const bool by_p = top_p < 1., by_low = low > 0.f && !(light && low_bin + 1 >= kSrNear);
+    auto last_bin = [&](bool any) {
+        by_k = top_k > 0 && (uint32_t)top_k < all;
+        keep_k = by_k ? (uint32_t)top_k : all;
+        if (by_k) return pass(sh.cum_c, sh.cum_w, bins, true, keep_k - 1, 0., any);
+        uint32_t at = bins;
+        if (by_p) at = pass(sh.cum_c, sh.cum_w, bins, false, 0, top_p * total, any);
+        if (by_low) at = min(at, low_bin + 1);
+        return by_p || by_low ? at : pass(sh.cum_c, sh.cum_w, bins, false, 0, (double)u * total, any);
+    };
+    uint32_t far = last_bin(light);
+    const bool few = far < kSrNear && sh.cum_c[far] <= kSrList;  // (the same in every block)
+    if (few) {
+        // they go to the first block's list
+        SrSmem &first = *cluster.map_shared_rank(&sh, 0);
+        auto give = [&](float v, unsigned long long entry) {
+            float t, rest;
+            s.of(v, t, rest);
+            if (s.bin(t) <= far && v != -INFINITY) first.list[atomicAdd(&first.listed, 1u)] = entry;
+        };
+        const uint32_t n = sh.n_kept;
+        if (far < kSrNear / 2 && n <= kSrKept)
+            for (uint32_t i = tid; i < n; i += kSrThreads) give(sr_value((uint32_t)(sh.kept[i] >> 32)), sh.kept[i]);
+        else
+            x.template each<2>([&](float v, uint32_t i) { give(v, (unsigned long long)sr_key(v) << 32 | ~i); });
+    }
+    cluster.sync();
+    if (rank != 0) {
+        while (!few) {
+            cluster.sync();  // the first block has asked
+            if (sh.op == kSrDone) break;
+            clear(sh.op);
+            sr_serve(sh, *cluster.map_shared_rank(&sh, 0), x, s);
+            cluster.sync();
+        }
+        return;
+    }
+
+    // --- the first block ---
     uint32_t pick = 0;     // the token's place in the list
     double kept = total;   // mass of what the filters leave
-    if (sh.cum_c[far] <= kSrList) {
-        // few entries: all of them up to there in one list
-        collect({0u, far, 0u, 0xffffffffu, 0u, 0xffffffffu});
+    if (few) {
+        order();
         uint32_t stay = by_k ? keep_k : n;
         if (by_k) kept = sh.list_w[keep_k - 1];
         if (by_p) {
@@ -488,13 +622,22 @@ __global__ void __launch_bounds__(kSrThreads) sample_rows_kernel(const __grid_co
             stay = min(stay, prefix([&](uint32_t i) {
                            float t, rest;
                            s.of(sr_value((uint32_t)(sh.list[i] >> 32)), t, rest);
-                           return i == 0 || high(t, rest);
+                           return i == 0 || s.high(t, rest);
                        }));
         if (by_k || by_p || by_low) kept = sh.list_w[stay - 1];
         const double limit = (double)u * kept;
         pick = min(prefix([&](uint32_t i) { return sh.list_w[i] <= limit; }), stay - 1);
     } else {
-        // each filter's end by itself, then the draw
+        // each filter's end by itself, and the draw
+        if (far == kSrNear) {  // below the near bins: all of them
+            ask(kSrFar, {kSrNear, kSrBins - 1, 0u, 0xffffffffu, 0u, 0xffffffffu}, 0);
+            gather(kSrBins, sh.cum_c, sh.cum_w);
+            bins = kSrBins;
+            all = sh.cum_c[kSrBins - 1];
+            total = sh.cum_w[kSrBins - 1];
+            far = last_bin(true);
+        }
+        kept = total;
         uint32_t stay = keep_k;
         if (by_k) {
             near(far, true, keep_k - 1, 0.);
@@ -502,26 +645,26 @@ __global__ void __launch_bounds__(kSrThreads) sample_rows_kernel(const __grid_co
         }
         if (by_p) {
             const double limit = top_p * kept;
-            near(pass(sh.cum_c, sh.cum_w, false, 0, limit), false, 0, limit);
+            near(pass(sh.cum_c, sh.cum_w, bins, false, 0, limit, true), false, 0, limit);
             const uint32_t c = prefix([&](uint32_t i) { return base_c + i == 0 || base_w + (i ? sh.list_w[i - 1] : 0.) < limit; });
             if (base_c + c < stay) {
                 stay = base_c + c;
                 kept = base_w + (c ? sh.list_w[c - 1] : 0.);
             }
         }
-        if (by_low) {
+        if (by_low && low_bin <= far + 1) {  // (else it leaves all that the others left)
             const uint32_t k0 = low_bin - 1;
             ask(kSrLow, {k0, k0 + 2, 0u, 0xffffffffu, 0u, 0xffffffffu}, 0);
             if (tid < 3) {
                 unsigned long long f = 0;
                 uint32_t c = 0;
                 for (uint32_t k = 0; k < blocks; ++k) {
-                    const SrSmem &from = *cluster.map_shared_rank(&sh, k);
-                    c += from.count[2 * tid];
-                    f += from.frac[2 * tid];
+                    const uint2 v = cluster.map_shared_rank(&sh, k)->bins[2 * tid];
+                    c += v.x;
+                    f += v.y;
                 }
                 sh.csum[tid] = c;
-                sh.wsum[tid] = sr_mass(k0 + tid, c, f);
+                sh.wsum[tid] = sr_mass(sh.steps, k0 + tid, c, f);
             }
             __syncthreads();
             const uint32_t c = (k0 ? sh.cum_c[k0 - 1] : 0) + sh.csum[0] + sh.csum[1] + sh.csum[2];
@@ -533,10 +676,10 @@ __global__ void __launch_bounds__(kSrThreads) sample_rows_kernel(const __grid_co
             __syncthreads();
         }
         const double limit = (double)u * kept;
-        near(pass(sh.cum_c, sh.cum_w, false, 0, limit), false, 0, limit);
+        near(pass(sh.cum_c, sh.cum_w, bins, false, 0, limit, true), false, 0, limit);
         pick = prefix([&](uint32_t i) { return base_w + sh.list_w[i] <= limit; });
         if (base_c + pick >= stay) {  // u is 1, or rounding: the last that stays
-            near(pass(sh.cum_c, sh.cum_w, true, stay - 1, 0.), true, stay - 1, 0.);
+            near(pass(sh.cum_c, sh.cum_w, bins, true, stay - 1, 0., true), true, stay - 1, 0.);
             pick = stay - 1 - base_c;
         }
     }
@@ -546,7 +689,7 @@ __global__ void __launch_bounds__(kSrThreads) sample_rows_kernel(const __grid_co
         a.token[row] = (int32_t)index;
         if (a.logprob) a.logprob[row] = (float)log(w / kept);
     }
-    ask(kSrDone, {}, 0);
+    if (!few) ask(kSrDone, {}, 0);
 }
 
 }  // namespace fwb

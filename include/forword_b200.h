@@ -259,7 +259,8 @@ int fwb_beam_reorder_dev(const void *d_src, void *d_dst, const int32_t *d_parent
  * most n_query; NULL: n_query each) has position lengths[s] - n_new[s] + t,
  * and the rows of tokens t >= n_new[s] of a padded batch are neither read nor
  * written.  page_size is 16, 32, 64, 128 or 256; head_dim a multiple of 16, at
- * most 128; a page table holds at most 2^30 positions.
+ * most 128; a page table holds at most 2^30 positions, and a call at most 2^24 -
+ * 1 tokens (n_seq * n_query) and 65535 heads.
  *
  * A page outside 0..n_page-1 is neither read nor written: its positions are
  * not appended, count as not seen, and read as zeros.  The same holds for
@@ -352,14 +353,16 @@ typedef struct fwb_kv4_attn {
  * Attention of every sequence's new tokens over its pages: token t of n_new
  * sees the first lengths[s] - (n_new[s] - 1 - t) positions.  lse receives log
  * sum exp of the scaled scores.  A token that sees no position gets out 0 and
- * lse -inf; one whose query is not finite, or that sees a NaN key or value,
- * gets NaN; what lies past the positions that a token sees reaches it in no
- * way.  fp16 and bf16 queries are exact in the products, weighted
+ * lse -inf; a head of it whose query holds a value that is not finite, or of
+ * 2^100 or more, gets NaN, and so does one that sees a NaN key (with a NaN value,
+ * the dimensions of its block); what lies past the positions that a token sees
+ * reaches it in no way.  fp16 and bf16 queries are exact in the products, weighted
  * probabilities are rounded to fp16; fp32 calls carry 22 bits of both.
  * workspace: fwb_kv4_attention_workspace(a) bytes of device memory, 16-byte
  * aligned, that no other call uses meanwhile (a captured call's: at every
  * replay).  It must be all zeros before its first use; calls leave it fit for
- * the next one, of any sizes.
+ * the next one, of any sizes.  n_seq * n_query * n_head is at most 2^31 - 1, and
+ * so are the query rows' tiles of 8 to 32 times the page table's tiles of 16.
  */
 int fwb_kv4_attention_dev(const fwb_kv4_attn_t *a, void *workspace, size_t workspace_bytes, void *stream);
 
@@ -383,7 +386,8 @@ size_t fwb_kv4_attention_workspace(const fwb_kv4_attn_t *a);
  * A logit of -inf bars its token.  A row that holds a NaN or +inf, is barred
  * throughout, or has a temperature or uniform number that is NaN gets token -1
  * and -inf.  Entries of weight below 2^-64 count as nothing, neither for top_k
- * nor in a mass.  Weights carry 22 bits and are added exactly, so a token can
+ * nor in a mass, and ones below 2^-32 need not, where they make up less than
+ * 2^-24 of the mass.  Weights carry 22 bits and are added exactly, so a token can
  * differ from exact arithmetic's only where a limit falls within about 2^-22
  * of the mass of a border.  n_vocab at most 262144.
  */
