@@ -122,7 +122,7 @@ bool attn_layout(const fwb_kv4_attn_t *a, AttnLayout &L) {
     L.rtiles = (uint32_t)((rows + 8 * L.nt - 1) / (8 * L.nt));
     const uint64_t units = (uint64_t)a->n_seq * L.rtiles * a->n_head_kv * ((uint64_t)a->max_pages * a->page_size / kKvTile + 64);
     if (units > 0x7fffffffu) return refuse(kAttn, "too many rows times positions");
-    L.ctas = device_sms() * (L.nt == 1 ? 2 : 1);
+    L.ctas = device_sms() * (L.nt <= 2 ? 2 : 1);
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t here = at;

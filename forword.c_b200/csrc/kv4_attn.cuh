@@ -29,7 +29,7 @@
 
 namespace fwb {
 
-constexpr int kKaWarps = 8, kKaThreads = 32 * kKaWarps, kKaStages = 3;
+constexpr int kKaWarps = 8, kKaThreads = 32 * kKaWarps;
 constexpr uint32_t kKaPair = 2 * kKvTile;  // positions that a warp takes at a time
 // Weights are formed as 2^8 exp2(score - reference), and a reference is raised
 // when a score exceeds it by 2^7: they stay below 2^15, which fp16 holds.
@@ -118,10 +118,9 @@ __device__ __forceinline__ void ka_halves(const uint8_t *p, uint32_t (&w)[(NB + 
     }
 }
 
-// What an item needs to know of its rows.
+// What a step needs to know of its item.
 struct KaItem {
-    uint32_t seq, rt, head;
-    uint32_t tiles;       // that its last row sees
+    uint32_t row0;        // its first row
     int32_t limit;        // positions that its last row sees
     int32_t len, fresh;   // of its sequence
 };
@@ -147,8 +146,9 @@ __device__ __forceinline__ bool ka_tiles(const Kv4AttnArgs &a, uint32_t rt, int3
 
 template <bool SPLIT, int NB, int NT>
 struct KaSmem {
+    static constexpr int kStages = NT == 2 ? 2 : 3;
     static constexpr uint32_t kRows = 8 * NT, kTile = kv4_tile(NB), kStage = 2 * kTile, kStride = 32 * NB + 4;
-    static constexpr uint32_t kRing = kKaWarps * kKaStages * kStage, kJoin = kKaWarps * kRows * kStride * 4;
+    static constexpr uint32_t kRing = kKaWarps * kStages * kStage, kJoin = kKaWarps * kRows * kStride * 4;
     static constexpr uint32_t kQueries = NT * NB * (SPLIT ? 2 : 1) * 32 * 16;  // after the ring
     static constexpr uint32_t kRingBytes = kRing > kJoin ? kRing : kJoin, kBytes = kRingBytes + kQueries;
 };
@@ -163,31 +163,29 @@ __device__ __forceinline__ KaCut ka_cut(uint32_t units, uint32_t snap) {
     return {head, max(units > snap ? units - snap : 0u, head + 1)};
 }
 
-// Two tiles of 16 positions.  Keys' codes go into the products as they lie,
+// H tiles of 16 positions.  Keys' codes go into the products as they lie,
 // under a mask: a nibble in the low bits of a half is the subnormal code * 2^-24
 // (16 times that in bits 4..7), so a pair costs one instruction, and the sums
 // begin at -8 in every place.  Values, whose sums run on, and all codes of fp32
 // calls (the tensor cores' sums truncate at their largest term: 3e-6 of the
 // result instead of 3e-7) are unpacked to code - 8.  EDGE: some rows may not see all of them, or a
 // tile is not there.  q: the queries' B operand [n][hi, lo][b] for each lane in shared memory (NT > 1); r: in registers.
-template <bool SPLIT, int NB, int NT, bool EDGE>
-__device__ __forceinline__ void ka_pair(const uint8_t *pair, const uint4 *sq, 
-                                        const float *soff, const float (&qs)[NT][2], const int32_t (&lim)[NT][2],
-                                        const int32_t (&limt)[NT], int32_t pos0, int32_t limit, uint32_t there,
-                                        float (&o)[NT][NB][2][4], float (&mm)[NT][2], float (&thr)[NT][2], float (&l)[NT][2],
-                                        float &vref) {
+template <bool SPLIT, int NB, int NT, int H, bool EDGE>
+__device__ __forceinline__ void ka_step(const Kv4AttnArgs &args, const uint8_t *pair, const uint4 *sq, const float *soff, const KaItem &it,
+                                        int32_t pos0, uint32_t there, const float (&qs)[NT][2], float (&o)[NT][NB][2][4],
+                                        float (&mm)[NT][2], float (&thr)[NT][2], float (&l)[NT][2], float &vref) {
     constexpr uint32_t TB = kv4_tile(NB);
     const uint32_t lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const uint32_t p0 = (g >> 1) + 4 * (g & 1), p1 = p0 + 8;  // the positions of this lane's rows of the scores
-    float s[2][NT][4];
+    float s[H][NT][4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < H; ++h)
 #pragma unroll
         for (int n = 0; n < NT; ++n) s[h][n][0] = s[h][n][1] = s[h][n][2] = s[h][n][3] = 0.f;
     {
-        uint32_t w0[2][NB], w1[2][NB], d0[2][(NB + 1) / 2], d1[2][(NB + 1) / 2];
+        uint32_t w0[H][NB], w1[H][NB], d0[H][(NB + 1) / 2], d1[H][(NB + 1) / 2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < H; ++h) {
             const uint8_t *tile = pair + h * TB;
             ka_words<NB>(tile + p0 * 16 * NB + c * 4 * NB, w0[h]);
             ka_words<NB>(tile + p1 * 16 * NB + c * 4 * NB, w1[h]);
@@ -196,10 +194,10 @@ __device__ __forceinline__ void ka_pair(const uint8_t *pair, const uint4 *sq,
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            uint32_t a0[2][4], a1[2][4];
-            float k0[2], k1[2];
+            uint32_t a0[H][4], a1[H][4];
+            float k0[H], k1[H];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < H; ++h) {
                 if constexpr (SPLIT) {
                     uint32_t x[4], y[4];
                     ka_codes(w0[h][b], x);
@@ -227,7 +225,7 @@ __device__ __forceinline__ void ka_pair(const uint8_t *pair, const uint4 *sq,
                     if constexpr (SPLIT) r = sq[((n * 2 + 1) * NB + b) * 32 + lane];
                 }
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int h = 0; h < H; ++h) {
                     float acc[4];
                     if constexpr (SPLIT) {
                         ka_mma(acc, a0[h], r.x, r.y, 0.f, 0.f, 0.f, 0.f);
@@ -247,14 +245,17 @@ __device__ __forceinline__ void ka_pair(const uint8_t *pair, const uint4 *sq,
     }
     bool raise = false;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < H; ++h)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                if constexpr (EDGE)
-                    if (!(there >> h & 1) || pos0 + (int32_t)(16 * h + (i < 2 ? p0 : p1)) >= lim[n][i & 1]) s[h][n][i] = -INFINITY;
-                raise |= s[h][n][i] > thr[n][i & 1];
+                if constexpr (EDGE) {
+                    const int32_t lim = ka_limit(args, it.len, it.fresh, it.row0 + n * 8 + 2 * c + (i & 1));
+                    if (!(there >> h & 1) || pos0 + (int32_t)(16 * h + (i < 2 ? p0 : p1)) >= lim) s[h][n][i] = -INFINITY;
+                }
+                // (thr: the same in terms of the bare score, where there are registers for it)
+                raise |= NT == 1 ? s[h][n][i] > thr[n][i & 1] : fmaf(s[h][n][i], qs[n][i & 1], -mm[n][i & 1]) > kKaHead + kKaLazy;
             }
     // References follow the scores only when one exceeds its own by 2^7.
     if (__any_sync(0xffffffffu, raise)) {
@@ -262,15 +263,16 @@ __device__ __forceinline__ void ka_pair(const uint8_t *pair, const uint4 *sq,
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                float top = fmaxf(fmaxf(s[0][n][j], s[0][n][j + 2]), fmaxf(s[1][n][j], s[1][n][j + 2]));
+                float top = fmaxf(s[0][n][j], s[0][n][j + 2]);
+                if constexpr (H == 2) top = fmaxf(top, fmaxf(s[H - 1][n][j], s[H - 1][n][j + 2]));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                top *= qs[n][j];
-                if (top > (thr[n][j] == -INFINITY ? -INFINITY : mm[n][j] + kKaHead)) {
-                    const float now = top - kKaHead, f = thr[n][j] == -INFINITY ? 0.f : ka_exp2(mm[n][j] - now);
+                const float now = fmaf(top, qs[n][j], -kKaHead);
+                if (now > mm[n][j]) {
+                    const float f = ka_exp2(mm[n][j] - now);
                     mm[n][j] = now;
-                    thr[n][j] = (top + kKaLazy) / qs[n][j];
+                    thr[n][j] = (now + (kKaHead + kKaLazy)) / qs[n][j];
                     l[n][j] *= f;
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
@@ -283,7 +285,7 @@ __device__ __forceinline__ void ka_pair(const uint8_t *pair, const uint4 *sq,
             }
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < H; ++h)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -295,16 +297,16 @@ __device__ __forceinline__ void ka_pair(const uint8_t *pair, const uint4 *sq,
                 l[n][i & 1] += p;
             }
     // The values' scales; what lies past the last row's positions is anything.
-    uint32_t v[2][NB][2];  // of positions (c, c + 4) and (c + 8, c + 12): the rows of the transposed weights
+    uint32_t v[H][NB][2];  // of positions (c, c + 4) and (c + 8, c + 12): the rows of the transposed weights
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < H; ++h) {
         const uint8_t *vd = pair + h * TB + 2 * kv4_codes(NB) + kv4_scales(NB);
         uint32_t d[4][(NB + 1) / 2];
 #pragma unroll
         for (int j = 0; j < 4; ++j) ka_halves<NB>(vd + (c + 4 * j) * 2 * NB, d[j]);
         uint32_t m0 = 0xffffffffu, m1 = 0xffffffffu;
         if constexpr (EDGE) {
-            const int32_t left = there >> h & 1 ? limit - pos0 - (int32_t)(16 * h + c) : 0;
+            const int32_t left = there >> h & 1 ? it.limit - pos0 - (int32_t)(16 * h + c) : 0;
             m0 = (left > 0 ? 0xffffu : 0u) | (left > 4 ? 0xffff0000u : 0u);
             m1 = (left > 8 ? 0xffffu : 0u) | (left > 12 ? 0xffff0000u : 0u);
         }
@@ -320,10 +322,10 @@ __device__ __forceinline__ void ka_pair(const uint8_t *pair, const uint4 *sq,
     float top = 0.f;
     if (lane < 8 * NB)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < H; ++h) {
             uint32_t word = *reinterpret_cast<const uint32_t *>(pair + h * TB + 2 * kv4_codes(NB) + kv4_scales(NB) + 4 * lane);
             if constexpr (EDGE) {
-                const int32_t left = there >> h & 1 ? limit - pos0 - 16 * h : 0;
+                const int32_t left = there >> h & 1 ? it.limit - pos0 - 16 * h : 0;
                 if ((int32_t)(2 * lane / NB) >= left) word = 0;
                 if ((int32_t)((2 * lane + 1) / NB) >= left) word &= 0xffffu;
             }
@@ -347,7 +349,7 @@ __device__ __forceinline__ void ka_pair(const uint8_t *pair, const uint4 *sq,
     const float inv = __uint_as_float((254u << 23) - __float_as_uint(vref));  // 1 / vref, at most 2^14
     const __half2 inv2 = __half2half2(__float2half_rn(inv));
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < H; ++h) {
         // the weights' transposes: rows as columns g, positions as above
         uint32_t w[NT][2], rest[NT][2];  // in two halves
 #pragma unroll
@@ -363,7 +365,8 @@ __device__ __forceinline__ void ka_pair(const uint8_t *pair, const uint4 *sq,
         if constexpr (EDGE)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const int32_t left = there >> h & 1 ? limt[n] - pos0 - (int32_t)(16 * h + c) : 0;
+                const int32_t lim = ka_limit(args, it.len, it.fresh, it.row0 + n * 8 + g);
+                const int32_t left = there >> h & 1 ? lim - pos0 - (int32_t)(16 * h + c) : 0;
                 mask[n][0] = (left > 0 ? 0xffffu : 0u) | (left > 4 ? 0xffff0000u : 0u);
                 mask[n][1] = (left > 8 ? 0xffffu : 0u) | (left > 12 ? 0xffff0000u : 0u);
             }
@@ -433,9 +436,10 @@ __device__ __forceinline__ void ka_pair(const uint8_t *pair, const uint4 *sq,
 // SPLIT: fp32 calls, whose queries and weights go through the products as two
 // halves each.  NT: column tiles of 8 query rows.
 template <bool SPLIT, int NB, int NT>
-__global__ void __launch_bounds__(kKaThreads, NT == 1 ? 2 : 1) kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
+__global__ void __launch_bounds__(kKaThreads, NT <= 2 ? 2 : 1) kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
     using S = KaSmem<SPLIT, NB, NT>;
     constexpr uint32_t ROWS = S::kRows;
+    constexpr int kKaStages = S::kStages;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ float2 sml[kKaWarps][ROWS];
     __shared__ float sref[kKaWarps];
@@ -610,23 +614,21 @@ __global__ void __launch_bounds__(kKaThreads, NT == 1 ? 2 : 1) kv4_attn_kernel(c
                 if (ch == 0) sqs[r] = (__uint_as_float((ex - 13u) << 23) + (ex < 227 ? odd : NAN)) * (a.scale * 1.4426950408889634f) * (SPLIT ? kKaCode : 16777216.f);
             }
             float qs[NT][2], mm[NT][2], thr[NT][2], l[NT][2], o[NT][NB][2][4], vref = 6.103515625e-05f;  // 2^-14
-            int32_t lim[NT][2], limt[NT];
             __syncthreads();
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     qs[n][j] = sqs[n * 8 + 2 * c + j];
-                    lim[n][j] = ka_limit(a, len, fresh, rt * ROWS + n * 8 + 2 * c + j);
-                    thr[n][j] = -INFINITY;  // nothing seen yet
-                    mm[n][j] = l[n][j] = 0.f;
+                    mm[n][j] = thr[n][j] = -INFINITY;  // nothing seen yet
+                    l[n][j] = 0.f;
                 }
-                limt[n] = ka_limit(a, len, fresh, rt * ROWS + n * 8 + g);
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) o[n][b][0][i] = o[n][b][1][i] = 0.f;
             }
+            const KaItem it = {rt * ROWS, limit, len, fresh};
             const int32_t least = ka_limit(a, len, fresh, rt * ROWS);  // of the first row: the fewest positions
 
             for (uint32_t i = 0; i < count; ++i) {
@@ -635,10 +637,17 @@ __global__ void __launch_bounds__(kKaThreads, NT == 1 ? 2 : 1) kv4_attn_kernel(c
                 const uint32_t stage = i % kKaStages, ok = there >> 2 * stage & 3;
                 const uint8_t *pair = mine_ring + stage * S::kStage;
                 const int32_t pos0 = (int32_t)((from + warp + i * kKaWarps) * kKaPair);
-                if (pos0 + (int32_t)kKaPair > least || ok != 3)
-                    ka_pair<SPLIT, NB, NT, true>(pair, sq, soff, qs, lim, limt, pos0, limit, ok, o, mm, thr, l, vref);
-                else
-                    ka_pair<SPLIT, NB, NT, false>(pair, sq, soff, qs, lim, limt, pos0, limit, ok, o, mm, thr, l, vref);
+                const bool edge = pos0 + (int32_t)kKaPair > least || ok != 3;
+                if constexpr (NT == 1) {  // both tiles at once: one look at the references for two
+                    if (edge) ka_step<SPLIT, NB, NT, 2, true>(a, pair, sq, soff, it, pos0, ok, qs, o, mm, thr, l, vref);
+                    else ka_step<SPLIT, NB, NT, 2, false>(a, pair, sq, soff, it, pos0, ok, qs, o, mm, thr, l, vref);
+                } else {                  // one after the other: registers
+#pragma unroll 1
+                    for (int h = 0; h < 2; ++h) {
+                        if (edge) ka_step<SPLIT, NB, NT, 1, true>(a, pair + h * S::kTile, sq, soff, it, pos0 + 16 * h, ok >> h, qs, o, mm, thr, l, vref);
+                        else ka_step<SPLIT, NB, NT, 1, false>(a, pair + h * S::kTile, sq, soff, it, pos0 + 16 * h, ok >> h, qs, o, mm, thr, l, vref);
+                    }
+                }
                 __syncwarp();
                 fill(i + kKaStages - 1);
             }
@@ -656,7 +665,7 @@ __global__ void __launch_bounds__(kKaThreads, NT == 1 ? 2 : 1) kv4_attn_kernel(c
                     sum += __shfl_xor_sync(0xffffffffu, sum, 8);
                     sum += __shfl_xor_sync(0xffffffffu, sum, 16);
                     const uint32_t row = n * 8 + 2 * c + j;
-                    if (g == 0) sml[warp][row] = make_float2(thr[n][j] == -INFINITY ? -INFINITY : mm[n][j], sum);
+                    if (g == 0) sml[warp][row] = make_float2(mm[n][j], sum);
 #pragma unroll
                     for (int b = 0; b < NB; ++b)
                         *reinterpret_cast<float4 *>(so + (warp * ROWS + row) * S::kStride + 32 * b + 4 * g) =
