@@ -31,6 +31,7 @@
 // than V's.
 #pragma once
 #include "beam_attn.cuh"
+#include "tcgen05.cuh"
 
 namespace fwb {
 
@@ -65,72 +66,11 @@ struct BeamTcTail {
 template <int HD>
 constexpr uint32_t beam_tc_smem() { return BeamTc<HD>::kOffTail + sizeof(BeamTcTail); }
 
-// Whether a phase is over, without waiting at all.
-__device__ __forceinline__ bool bt_test(uint64_t *bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                 : "=r"(ok) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-    return ok != 0;
-}
-__device__ __forceinline__ void bt_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void bt_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void bt_fence_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void bt_commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-// Shared-memory matrix descriptor, 128-byte swizzle: rows of 128 bytes, eight
-// of them (1024 bytes) an atom.  K-major operands: the next 8 rows 1024 bytes
-// on; MN-major ones: the next 8 k 1024 bytes on, the next 64 of M or N `lead`.
-__device__ __forceinline__ uint64_t bt_desc(uint32_t addr, uint32_t lead) {
-    return (uint64_t)((addr & 0x3ffffu) >> 4) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024u >> 4) << 32 |
-           (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
 // fp32 accumulator, A and B of type T (M 128, N n), both K-major or both MN-major.
 template <typename T>
 __device__ __forceinline__ uint32_t bt_idesc(uint32_t n, bool mn_major) {
     const uint32_t t = beam_is_bf16(T{}) ? 1u : 0u;
     return 1u << 4 | t << 7 | t << 10 | (mn_major ? 3u << 15 : 0u) | (n >> 3) << 17 | (128u >> 4) << 24;
-}
-__device__ __forceinline__ void bt_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
-}
-
-// 8 accumulator columns of this thread's lane (not waited for) / back.
-__device__ __forceinline__ void bt_ld8(uint32_t addr, float *v) {
-    uint32_t r[8];
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "r"(addr));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
-}
-__device__ __forceinline__ void bt_ld32(uint32_t addr, float *v) {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(addr));
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-__device__ __forceinline__ void bt_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-// Keeps uses of loaded values behind the wait before it.
-template <int N>
-__device__ __forceinline__ void bt_here(float *v) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) asm volatile("" : "+f"(v[i]));
-}
-__device__ __forceinline__ void bt_st8(uint32_t addr, const float *v) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr),
-                 "r"(__float_as_uint(v[0])), "r"(__float_as_uint(v[1])), "r"(__float_as_uint(v[2])),
-                 "r"(__float_as_uint(v[3])), "r"(__float_as_uint(v[4])), "r"(__float_as_uint(v[5])),
-                 "r"(__float_as_uint(v[6])), "r"(__float_as_uint(v[7])) : "memory");
 }
 __device__ __forceinline__ bool bt_any(uint32_t barrier, bool v) {  // of the 128 threads of a group
     uint32_t r;

@@ -9,14 +9,20 @@
 #include "../../include/forword_b200.h"
 #include "kv4_append.cuh"
 #include "kv4_attn.cuh"
+#include "kv4_attn_tc.cuh"
 #include "launch.h"
 
 namespace fwb {
 namespace {
 
-__device__ uint32_t g_kv4_err;  // kKvBad... bits, until taken
+// Until taken: kKvBad... bits, and what a bounded wait that ran out set (by
+// itself: once it is set, waits give up early).
+__device__ uint32_t g_kv4_err[2];
 
-__global__ void kv4_status_kernel(uint32_t *out) { *out = atomicExch(&g_kv4_err, 0u); }
+__global__ void kv4_status_kernel(uint32_t *out) {
+    out[0] = atomicExch(&g_kv4_err[0], 0u);
+    out[1] = atomicExch(&g_kv4_err[1], 0u);
+}
 
 uint32_t *error_word() {
     static uint32_t *at[64] = {};
@@ -29,17 +35,18 @@ uint32_t *error_word() {
     return static_cast<uint32_t *>(p);
 }
 
-// The error word after the work queued on `st`, cleared in the same step.
-cudaError_t take_status(cudaStream_t st, uint32_t &word) {
+// The error words after the work queued on `st`, cleared in the same step.
+cudaError_t take_status(cudaStream_t st, uint32_t (&word)[2]) {
     static std::mutex one;  // look at a time: they share the place that the kernel writes
     static uint32_t *place = nullptr;
     const std::lock_guard<std::mutex> lock(one);
-    cudaError_t e = place ? cudaSuccess : cudaHostAlloc(&place, sizeof *place, cudaHostAllocPortable);
+    cudaError_t e = place ? cudaSuccess : cudaHostAlloc(&place, 2 * sizeof *place, cudaHostAllocPortable);
     if (e != cudaSuccess) return e;
     kv4_status_kernel<<<1, 1, 0, st>>>(place);
     e = cudaGetLastError();
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-    if (e == cudaSuccess) word = *static_cast<volatile uint32_t *>(place);
+    if (e == cudaSuccess)
+        for (int i = 0; i < 2; ++i) word[i] = static_cast<volatile uint32_t *>(place)[i];
     return e;
 }
 
@@ -111,7 +118,8 @@ bool attn_sizes_ok(const fwb_kv4_attn_t *a) {
 }
 
 struct AttnLayout {
-    uint32_t nt, nb, rtiles, ctas;  // column tiles of 8 rows, blocks of a row, row tiles, CTAs
+    bool tc;                              // on the 5th-generation tensor cores (kv4_attn_tc.cuh)
+    uint32_t nt, nb, rows, rtiles, ctas;  // column tiles of 8 rows, blocks of a row, rows of a tile, row tiles, CTAs
     size_t po, pml, ticket, bytes;
 };
 
@@ -119,10 +127,20 @@ bool attn_layout(const fwb_kv4_attn_t *a, AttnLayout &L) {
     const uint64_t rows = (uint64_t)a->n_query * (a->n_head / a->n_head_kv);
     L.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
     L.nb = kv4_blocks(a->head_dim);
-    L.rtiles = (uint32_t)((rows + 8 * L.nt - 1) / (8 * L.nt));
+    // More rows than half a tile of the tcgen05 kernel, and tiles for three
+    // quarters of the SMs (their items are better left whole: a part is 64 KB).
+    // Measured, us for warp-level products / tcgen05 (fp16, 8 KV heads of 128, 4
+    // query heads each): 512 tokens at 8191 positions (128 tiles) 346 / 234, at 512
+    // 56 / 28; 16 sequences of 1000 positions with 16, 32, 64 tokens (128, 128, 256
+    // tiles) 46 / 38, 69 / 39, 124 / 73; of one sequence 32, 64, 128 tokens at 8191 (8,
+    // 16, 32 tiles) 42 / 125, 66 / 134, 105 / 143.
+    const uint64_t tiles = (uint64_t)a->n_seq * a->n_head_kv * ((rows + kKtRows - 1) / kKtRows);
+    L.tc = a->type != 0 && (L.nb == 2 || L.nb == 4) && rows >= kKtRows / 2 && 4 * tiles >= 3 * (uint64_t)device_sms();
+    L.rows = L.tc ? kKtRows : 8 * L.nt;
+    L.rtiles = (uint32_t)((rows + L.rows - 1) / L.rows);
     const uint64_t units = (uint64_t)a->n_seq * L.rtiles * a->n_head_kv * ((uint64_t)a->max_pages * a->page_size / kKvTile + 64);
     if (units > 0x7fffffffu) return refuse(kAttn, "too many rows times positions");
-    L.ctas = device_sms() * (L.nt <= 2 ? 2 : 1);
+    L.ctas = device_sms() * (!L.tc && L.nt <= 2 ? 2 : 1);
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t here = at;
@@ -130,8 +148,8 @@ bool attn_layout(const fwb_kv4_attn_t *a, AttnLayout &L) {
         return here;
     };
     L.ticket = take(device_sms() * 2 * 4);  // (in the same place for all sizes: it is zero between calls)
-    L.pml = take((size_t)2 * L.ctas * 8 * L.nt * 8);
-    L.po = take((size_t)2 * L.ctas * 8 * L.nt * 32 * L.nb * 4);
+    L.pml = take((size_t)2 * L.ctas * L.rows * 8);
+    L.po = take((size_t)2 * L.ctas * L.rows * 32 * L.nb * 4);
     L.bytes = at;
     return true;
 }
@@ -142,6 +160,15 @@ bool launch_attn(const Kv4AttnArgs &k, uint32_t ctas, cudaStream_t st) {
     constexpr uint32_t smem = KaSmem<SPLIT, NB, NT>::kBytes;
     if (!opt_in(kv4_attn_kernel<SPLIT, NB, NT>, smem, ready, kAttn)) return false;
     return launched(launch_after(kv4_attn_kernel<SPLIT, NB, NT>, dim3(ctas), kKaThreads, smem, 1, st, k), kAttn);
+}
+
+template <int NB, bool LOW>
+bool launch_attn_tc(const Kv4AttnArgs &k, uint32_t ctas, cudaStream_t st) {
+    static bool ready[64] = {};
+    constexpr uint32_t smem = kt_smem<NB, LOW>();
+    static_assert(smem <= 227 * 1024, "shared memory");
+    if (!opt_in(kv4_attn_tc_kernel<NB, LOW>, smem, ready, kAttn)) return false;
+    return launched(launch_after(kv4_attn_tc_kernel<NB, LOW>, dim3(ctas), kKtThreads, smem, 1, st, k), kAttn);
 }
 
 template <bool SPLIT, int NB>
@@ -172,17 +199,18 @@ size_t fwb_kv4_page_bytes(uint32_t head_dim, uint32_t page_size) {
 }
 
 int fwb_kv4_status(void *stream) {
-    uint32_t e = 0;
+    uint32_t e[2] = {0, 0};
     try {
         if (!launched(take_status(static_cast<cudaStream_t>(stream), e), "fwb_kv4_status")) return -1;
     } catch (const std::exception &) {
         fail("fwb_kv4_status: the lock failed");
         return -1;
     }
-    if (!e) return 0;
-    char b[160];
-    snprintf(b, sizeof b, "fwb_kv4_status:%s%s", e & kKvBadPage ? " a page outside the cache" : "",
-             e & kKvBadPosition ? " a position past the page table or the rotation's tables" : "");
+    if (!e[0] && !e[1]) return 0;
+    char b[200];
+    snprintf(b, sizeof b, "fwb_kv4_status:%s%s%s", e[0] & kKvBadPage ? " a page outside the cache" : "",
+             e[0] & kKvBadPosition ? " a position past the page table or the rotation's tables" : "",
+             e[1] ? " a bounded wait in the kernel ran out" : "");
     fail(b);
     return -1;
 }
@@ -294,7 +322,19 @@ int fwb_kv4_attention_dev(const fwb_kv4_attn_t *a, void *workspace, size_t works
     k.pml = reinterpret_cast<float2 *>(ws + L.pml);
     k.ticket = reinterpret_cast<uint32_t *>(ws + L.ticket);
     if (!(k.err = error_word())) return -1;
+    k.wait_err = k.err + 1;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (L.tc) {
+        // in tiles of 64 positions; items with a CTA each are left whole, others cut
+        // only past 16 tiles of their ends
+        k.cost = 12;
+        k.snap = 16;
+        k.least = 32;
+        k.whole = 0x3fffffff;
+        const bool ok = a->type == 1 ? (L.nb == 4 ? launch_attn_tc<4, true>(k, L.ctas, st) : launch_attn_tc<2, true>(k, L.ctas, st))
+                                     : (L.nb == 4 ? launch_attn_tc<4, false>(k, L.ctas, st) : launch_attn_tc<2, false>(k, L.ctas, st));
+        return ok ? 0 : -1;
+    }
     return (a->type == 0 ? pick_blocks<true>(k, L, st) : pick_blocks<false>(k, L, st)) ? 0 : -1;
 }
 

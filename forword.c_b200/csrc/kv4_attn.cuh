@@ -50,7 +50,7 @@ struct Kv4AttnArgs {
     float *po;        // [2 CTAs][rows][32 NB] parts of cut items
     float2 *pml;      // [2 CTAs][rows] their references and sums
     uint32_t *ticket; // [CTAs] zero between launches
-    uint32_t *err;
+    uint32_t *err, *wait_err;  // what the tables held; a bounded wait that ran out
 };
 
 __device__ __forceinline__ float ka_exp2(float x) {
@@ -144,15 +144,6 @@ __device__ __forceinline__ bool ka_tiles(const Kv4AttnArgs &a, uint32_t rt, int3
     return true;
 }
 
-template <bool SPLIT, int NB, int NT>
-struct KaSmem {
-    static constexpr int kStages = NT == 2 ? 2 : 3;
-    static constexpr uint32_t kRows = 8 * NT, kTile = kv4_tile(NB), kStage = 2 * kTile, kStride = 32 * NB + 4;
-    static constexpr uint32_t kRing = kKaWarps * kStages * kStage, kJoin = kKaWarps * kRows * kStride * 4;
-    static constexpr uint32_t kQueries = NT * NB * (SPLIT ? 2 : 1) * 32 * 16;  // after the ring
-    static constexpr uint32_t kRingBytes = kRing > kJoin ? kRing : kJoin, kBytes = kRingBytes + kQueries;
-};
-
 // Where the line's even cuts fall within an item of `units` units: one in its
 // first `head` + 1 moves to its beginning, one at `tail` or later to its end.
 struct KaCut {
@@ -162,6 +153,160 @@ __device__ __forceinline__ KaCut ka_cut(uint32_t units, uint32_t snap) {
     const uint32_t head = min(snap, units / 2);
     return {head, max(units > snap ? units - snap : 0u, head + 1)};
 }
+
+struct KaScan {
+    uint32_t sum[32], most[32], find[3];
+};
+
+// A CTA's way along the line of items, in units of UNIT positions, for row
+// tiles of ROWS.  Every thread goes it by itself.
+template <int ROWS, int UNIT>
+struct KaLine {
+    const Kv4AttnArgs &a;
+    bool whole = false;  // items count alike, and go to a CTA each
+    uint32_t total, chunk, entry, head, start, units;  // start, units: of the item
+    // the item's sequence and row tile, what its rows see, and this CTA's part
+    uint32_t seq, rt, first, last, from, to, tiles;
+    int32_t len, fresh, limit;
+
+    __device__ __forceinline__ KaLine(const Kv4AttnArgs &args) : a(args) {}
+    __device__ __forceinline__ uint32_t units_of(uint32_t e) const {
+        int32_t len, fresh, limit;
+        ka_lengths(a, e / a.rtiles, len, fresh);
+        return !ka_tiles<ROWS>(a, e % a.rtiles, len, fresh, limit) ? 0 : whole ? 1 : (uint32_t)(limit + UNIT - 1) / UNIT + a.cost;
+    }
+    // Called by all the CTA's threads (whole warps); false: no part of the line is its.
+    __device__ __forceinline__ bool begin(KaScan &sh) {
+        const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5, entries = a.n_seq * a.rtiles,
+                       per = (entries + blockDim.x - 1) / blockDim.x;
+        uint32_t mine = 0, top = 0, have = 0;
+        for (uint32_t e = tid * per; e < min(entries, (tid + 1) * per); ++e) {
+            const uint32_t n = units_of(e);
+            mine += n * a.n_kv;
+            have += n ? a.n_kv : 0;
+            top = max(top, n);
+        }
+        if (entries * a.n_kv <= gridDim.x) {
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0) sh.most[warp] = top;
+            __syncthreads();
+            for (uint32_t w = 0; w < warps; ++w) top = max(top, sh.most[w]);
+            if (top <= a.whole + a.cost) {
+                whole = true;
+                mine = have;
+            }
+        }
+        uint32_t before = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, before, d);
+            if (lane >= (uint32_t)d) before += x;
+        }
+        if (lane == 31) sh.sum[warp] = before;
+        __syncthreads();
+        total = 0;
+        uint32_t base = 0;
+        for (uint32_t w = 0; w < warps; ++w) {
+            if (w == warp) base = total;
+            total += sh.sum[w];
+        }
+        before += base - mine;
+        chunk = whole ? 1 : max((total + gridDim.x - 1) / gridDim.x, a.least);
+        const uint64_t lo = (uint64_t)blockIdx.x * chunk;
+        if (lo >= total) return false;
+        if (mine && before <= lo && lo < before + mine) {
+            uint32_t at = before, e = tid * per, n;
+            while (at + (n = units_of(e) * a.n_kv) <= lo) at += n, ++e;
+            sh.find[0] = e;
+            sh.find[1] = at;
+            sh.find[2] = ((uint32_t)lo - at) / (n / a.n_kv);
+        }
+        __syncthreads();
+        entry = sh.find[0];
+        head = sh.find[2];
+        units = units_of(entry);
+        start = sh.find[1] + head * units;
+        return true;
+    }
+    // The item's CTAs are `first` to `last`; false where they lie past this one.
+    // Otherwise it has units from..to of the item (last < this CTA: none).
+    __device__ __forceinline__ bool item() {
+        const KaCut cut = ka_cut(units, a.snap);
+        first = (start + cut.head) / chunk;
+        last = (start + cut.tail - 1) / chunk;
+        if (first > blockIdx.x) return false;
+        seq = entry / a.rtiles;
+        rt = entry % a.rtiles;
+        limit = 0;
+        ka_lengths(a, seq, len, fresh);
+        ka_tiles<ROWS>(a, rt, len, fresh, limit);
+        tiles = (uint32_t)(limit + UNIT - 1) / UNIT;
+        from = first == blockIdx.x ? 0 : min(blockIdx.x * chunk - start, tiles);
+        to = last == blockIdx.x ? tiles : min((blockIdx.x + 1) * chunk - start, tiles);
+        return true;
+    }
+    // To the next item; false at the end of this CTA's part.
+    __device__ __forceinline__ bool next() {
+        if (last > blockIdx.x) return false;
+        start += units;
+        if (start >= total) return false;
+        if (++head == a.n_kv) {
+            head = 0;
+            do units = units_of(++entry);
+            while (!units);
+        }
+        return true;
+    }
+};
+
+// The result of a row: four dimensions from d on, and its log-sum-exp.
+template <int ROWS, int UNIT>
+__device__ __forceinline__ void ka_finish(const KaLine<ROWS, UNIT> &ln, uint32_t r, uint32_t d, float4 v, float2 ml) {
+    const Kv4AttnArgs &a = ln.a;
+    const uint32_t row = ln.rt * ROWS + r, t = row / a.gq;
+    if (row >= a.n_query * a.gq || (int32_t)t >= ln.fresh) return;
+    const uint64_t at = ((uint64_t)ln.seq * a.n_query + t) * a.n_head + ln.head * a.gq + row % a.gq;
+    const float by = ml.y == 0.f ? 0.f : 1.f / ml.y;
+    if (d < a.hd) kv4_store4(a.out, at * a.hd + d, a.type, make_float4(v.x * by, v.y * by, v.z * by, v.w * by));
+    if (d == 0 && a.lse) a.lse[at] = ml.y == 0.f ? -INFINITY : (ml.x + log2f(ml.y)) * 0.69314718055994531f;
+}
+// A part's place: a CTA begins one cut item at most, and ends one.
+template <int ROWS, int UNIT>
+__device__ __forceinline__ uint64_t ka_slot(const KaLine<ROWS, UNIT> &ln, uint32_t cta) { return 2ull * cta + (cta == ln.first ? 1 : 0); }
+// The parts of an item added, in the order of the positions, by thread `tid` of THREADS.
+template <int NB, int THREADS, int ROWS, int UNIT>
+__device__ __forceinline__ void ka_add_parts(const KaLine<ROWS, UNIT> &ln, uint32_t tid) {
+    const Kv4AttnArgs &a = ln.a;
+    const uint32_t rows = a.n_query * a.gq;
+    for (uint32_t i = tid; i < ROWS * 8 * NB; i += THREADS) {
+        const uint32_t r = i / (8 * NB), d = i % (8 * NB) * 4;
+        if (ln.rt * ROWS + r >= rows) continue;
+        float2 ml = {-INFINITY, 0.f};
+        float4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+        for (uint32_t p = ln.first; p <= ln.last; ++p) {
+            const float2 y = __ldcg(a.pml + ka_slot(ln, p) * ROWS + r);
+            const float4 x = __ldcg(reinterpret_cast<const float4 *>(a.po + (ka_slot(ln, p) * ROWS + r) * (32 * NB) + d));
+            const float top = fmaxf(ml.x, y.x), ref = top == -INFINITY ? 0.f : top;
+            const float f0 = ka_exp2(ml.x - ref), f1 = ka_exp2(y.x - ref);
+            ml = make_float2(top, ml.y * f0 + y.y * f1);
+            v.x = v.x * f0 + x.x * f1;
+            v.y = v.y * f0 + x.y * f1;
+            v.z = v.z * f0 + x.z * f1;
+            v.w = v.w * f0 + x.w * f1;
+        }
+        ka_finish(ln, r, d, v, ml);
+    }
+}
+
+template <bool SPLIT, int NB, int NT>
+struct KaSmem {
+    static constexpr int kStages = NT == 2 ? 2 : 3;
+    static constexpr uint32_t kRows = 8 * NT, kTile = kv4_tile(NB), kStage = 2 * kTile, kStride = 32 * NB + 4;
+    static constexpr uint32_t kRing = kKaWarps * kStages * kStage, kJoin = kKaWarps * kRows * kStride * 4;
+    static constexpr uint32_t kQueries = NT * NB * (SPLIT ? 2 : 1) * 32 * 16;  // after the ring
+    static constexpr uint32_t kRingBytes = kRing > kJoin ? kRing : kJoin, kBytes = kRingBytes + kQueries;
+};
 
 // H tiles of 16 positions.  Keys' codes go into the products as they lie,
 // under a mask: a nibble in the low bits of a half is the subnormal code * 2^-24
@@ -447,81 +592,19 @@ __global__ void __launch_bounds__(kKaThreads, NT <= 2 ? 2 : 1) kv4_attn_kernel(c
     __shared__ float2 srow[ROWS];          // an item's references and sums
     __shared__ __align__(8) float soff[NT * NB * 8];
     __shared__ float sqs[ROWS];            // of its queries
-    __shared__ uint32_t scan[kKaWarps], most[kKaWarps], sfind[3], slast;
+    __shared__ KaScan scan;
+    __shared__ uint32_t slast;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     uint4 *const sq = reinterpret_cast<uint4 *>(ring + S::kRingBytes);
     pdl_wait();
 
-    // --- this CTA's part of the line ---
-    const uint32_t entries = a.n_seq * a.rtiles, per = (entries + kKaThreads - 1) / kKaThreads;
-    bool whole = false;  // items count alike, and go to a CTA each
-    auto units_of = [&](uint32_t e) -> uint32_t {
-        int32_t len, fresh, limit;
-        ka_lengths(a, e / a.rtiles, len, fresh);
-        return !ka_tiles<ROWS>(a, e % a.rtiles, len, fresh, limit) ? 0
-               : whole ? 1 : (uint32_t)(limit + kKaPair - 1) / kKaPair + a.cost;
-    };
-    uint32_t mine = 0, top = 0, have = 0;
-    for (uint32_t e = tid * per; e < min(entries, (tid + 1) * per); ++e) {
-        const uint32_t n = units_of(e);
-        mine += n * a.n_kv;
-        have += n ? a.n_kv : 0;
-        top = max(top, n);
-    }
-    if (entries * a.n_kv <= gridDim.x) {
-        top = __reduce_max_sync(0xffffffffu, top);
-        if (lane == 0) most[warp] = top;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kKaWarps; ++w) top = max(top, most[w]);
-        if (top <= a.whole + a.cost) {
-            whole = true;
-            mine = have;
-        }
-    }
-    uint32_t before = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const uint32_t x = __shfl_up_sync(0xffffffffu, before, d);
-        if (lane >= (uint32_t)d) before += x;
-    }
-    if (lane == 31) scan[warp] = before;
-    __syncthreads();
-    uint32_t total = 0, base = 0;
-#pragma unroll
-    for (int w = 0; w < kKaWarps; ++w) {
-        if (w == (int)warp) base = total;
-        total += scan[w];
-    }
-    before += base - mine;
-    const uint32_t chunk = whole ? 1 : max((total + gridDim.x - 1) / gridDim.x, a.least);
-    const uint64_t lo64 = (uint64_t)blockIdx.x * chunk;
-    if (lo64 >= total) return;
-    const uint32_t lo = (uint32_t)lo64;
-    if (mine && before <= lo && lo < before + mine) {
-        uint32_t at = before, e = tid * per, n;
-        while (at + (n = units_of(e) * a.n_kv) <= lo) at += n, ++e;
-        sfind[0] = e;
-        sfind[1] = at;
-        sfind[2] = (lo - at) / (n / a.n_kv);
-    }
-    __syncthreads();
-    uint32_t entry = sfind[0], head = sfind[2], units = units_of(entry);
-    uint32_t start = sfind[1] + head * units;  // of the item
-
-    while (true) {
-        // the CTAs that share the item, `first` to `last`
-        const KaCut cut = ka_cut(units, a.snap);
-        const uint32_t first = (start + cut.head) / chunk, last = (start + cut.tail - 1) / chunk;
-        if (first > blockIdx.x) break;
-        if (last >= blockIdx.x) {
-            const uint32_t seq = entry / a.rtiles, rt = entry % a.rtiles;
-            int32_t len, fresh, limit = 0;
-            ka_lengths(a, seq, len, fresh);
-            ka_tiles<ROWS>(a, rt, len, fresh, limit);
-            const uint32_t pairs = (uint32_t)(limit + kKaPair - 1) / kKaPair;
-            const uint32_t from = first == blockIdx.x ? 0 : min(blockIdx.x * chunk - start, pairs),
-                           to = last == blockIdx.x ? pairs : min((blockIdx.x + 1) * chunk - start, pairs);
+    KaLine<ROWS, kKaPair> ln(a);
+    if (!ln.begin(scan)) return;
+    do {
+        if (!ln.item()) break;
+        if (ln.last >= blockIdx.x) {
+            const uint32_t seq = ln.seq, rt = ln.rt, head = ln.head, from = ln.from, to = ln.to;
+            const int32_t len = ln.len, fresh = ln.fresh, limit = ln.limit;
             const uint32_t rows = a.n_query * a.gq;
 
             // --- the warp's positions: their pages, and the first copies ---
@@ -687,16 +770,8 @@ __global__ void __launch_bounds__(kKaThreads, NT <= 2 ? 2 : 1) kv4_attn_kernel(c
                 srow[tid] = make_float2(top, sum);
             }
             __syncthreads();
-            const uint32_t parts = last - first + 1;
-            auto finish = [&](uint32_t r, uint32_t d, float4 v, float2 ml) {
-                const uint32_t row = rt * ROWS + r, t = row / a.gq;
-                if (row >= rows || (int32_t)t >= fresh) return;
-                const uint64_t at = ((uint64_t)seq * a.n_query + t) * a.n_head + head * a.gq + row % a.gq;
-                const float by = ml.y == 0.f ? 0.f : 1.f / ml.y;
-                if (d < a.hd) kv4_store4(a.out, at * a.hd + d, a.type, make_float4(v.x * by, v.y * by, v.z * by, v.w * by));
-                if (d == 0 && a.lse) a.lse[at] = ml.y == 0.f ? -INFINITY : (ml.x + log2f(ml.y)) * 0.69314718055994531f;
-            };
-            auto slot_of = [&](uint32_t cta) { return 2ull * cta + (cta == first ? 1 : 0); };
+            const uint32_t parts = ln.last - ln.first + 1;
+            const uint64_t slot = ka_slot(ln, blockIdx.x);
             for (uint32_t i = tid; i < ROWS * 8 * NB; i += kKaThreads) {
                 const uint32_t r = i / (8 * NB), d = i % (8 * NB) * 4;
                 float4 v = {0.f, 0.f, 0.f, 0.f};
@@ -710,53 +785,26 @@ __global__ void __launch_bounds__(kKaThreads, NT <= 2 ? 2 : 1) kv4_attn_kernel(c
                     v.w = fmaf(f, x.w, v.w);
                 }
                 if (parts == 1) {
-                    finish(r, d, v, srow[r]);
+                    ka_finish(ln, r, d, v, srow[r]);
                 } else {
-                    *reinterpret_cast<float4 *>(a.po + (slot_of(blockIdx.x) * ROWS + r) * (32 * NB) + d) = v;
-                    if (d == 0) a.pml[slot_of(blockIdx.x) * ROWS + r] = srow[r];
+                    *reinterpret_cast<float4 *>(a.po + (slot * ROWS + r) * (32 * NB) + d) = v;
+                    if (d == 0) a.pml[slot * ROWS + r] = srow[r];
                 }
             }
             if (parts > 1) {
                 __threadfence();
                 __syncthreads();
-                if (tid == 0) slast = atomicAdd(a.ticket + first, 1u) == parts - 1;
+                if (tid == 0) slast = atomicAdd(a.ticket + ln.first, 1u) == parts - 1;
                 __syncthreads();
                 if (slast) {
                     __threadfence();
-                    if (tid == 0) a.ticket[first] = 0;
-                    for (uint32_t i = tid; i < ROWS * 8 * NB; i += kKaThreads) {
-                        const uint32_t r = i / (8 * NB), d = i % (8 * NB) * 4;
-                        if (rt * ROWS + r >= rows) continue;
-                        float2 ml = {-INFINITY, 0.f};
-                        float4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-                        for (uint32_t p = first; p <= last; ++p) {
-                            const float2 y = __ldcg(a.pml + slot_of(p) * ROWS + r);
-                            const float4 x = __ldcg(reinterpret_cast<const float4 *>(a.po + (slot_of(p) * ROWS + r) * (32 * NB) + d));
-                            const float top = fmaxf(ml.x, y.x), ref = top == -INFINITY ? 0.f : top;
-                            const float f0 = ka_exp2(ml.x - ref), f1 = ka_exp2(y.x - ref);
-                            ml = make_float2(top, ml.y * f0 + y.y * f1);
-                            v.x = v.x * f0 + x.x * f1;
-                            v.y = v.y * f0 + x.y * f1;
-                            v.z = v.z * f0 + x.z * f1;
-                            v.w = v.w * f0 + x.w * f1;
-                        }
-                        finish(r, d, v, ml);
-                    }
+                    if (tid == 0) a.ticket[ln.first] = 0;
+                    ka_add_parts<NB, kKaThreads>(ln, tid);
                 }
             }
             __syncthreads();  // the results are read: the rings may be filled again
         }
-        // --- the next item ---
-        if (last > blockIdx.x) break;
-        start += units;
-        if (start >= total) break;
-        if (++head == a.n_kv) {
-            head = 0;
-            do units = units_of(++entry);
-            while (!units);
-        }
-    }
+    } while (ln.next());
 }
 
 }  // namespace fwb

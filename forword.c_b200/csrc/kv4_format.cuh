@@ -69,6 +69,18 @@ template <> __device__ __forceinline__ void kv4_store4<__nv_bfloat16>(void *p, u
     *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p) + at) =
         make_uint2(*reinterpret_cast<const uint32_t *>(&a), *reinterpret_cast<const uint32_t *>(&b));
 }
+// Eight 16-bit elements.
+template <typename T>
+__device__ __forceinline__ void kv4_floats8(uint4 v, float (&x)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = std::is_same<T, __half>::value ? kv4_unpack(w[i])
+                                                        : make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
+}
 // Eight elements, 16-byte aligned.
 template <typename T>
 __device__ __forceinline__ void kv4_load8(const void *p, uint64_t at, float (&x)[8]) {
@@ -76,16 +88,7 @@ __device__ __forceinline__ void kv4_load8(const void *p, uint64_t at, float (&x)
         const float4 a = kv4_load4<float>(p, at), b = kv4_load4<float>(p, at + 4);
         x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
     } else {
-        const uint4 v = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + at);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = std::is_same<T, __half>::value
-                                 ? kv4_unpack(w[i])
-                                 : make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
-            x[2 * i] = f.x;
-            x[2 * i + 1] = f.y;
-        }
+        kv4_floats8<T>(*reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + at), x);
     }
 }
 template <typename T>

@@ -261,12 +261,13 @@ class Attention(_Plan):
         self._strides = None
 
     def _workspace(self, stream: int) -> torch.Tensor:
-        """As a plan's, but zeros at first, as the kernel wants it; a call leaves it so."""
-        if _capturing():
-            return torch.zeros(self.workspace_bytes, dtype=torch.uint8, device=f"cuda:{self.device}")
+        """As a plan's, but with zeros where the kernel counts, which a call leaves so."""
         ws = self._ws.get(stream)
-        if ws is None:
-            ws = self._ws[stream] = torch.zeros(self.workspace_bytes, dtype=torch.uint8, device=f"cuda:{self.device}")
+        if ws is None or _capturing():
+            ws = torch.empty(self.workspace_bytes, dtype=torch.uint8, device=f"cuda:{self.device}")
+            ws[:4096].zero_()
+            if not _capturing():
+                self._ws[stream] = ws
         return ws
 
     def __call__(self, q, cache, pages, lengths, n_new=None, out=None, lse=None):

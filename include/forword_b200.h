@@ -274,7 +274,8 @@ size_t fwb_kv4_page_bytes(uint32_t head_dim, uint32_t page_size);
 
 /* Status of the fwb_kv4 calls on the current device since the last look,
  * after the work queued on `stream` (synchronises it): 0, or -1 if one met a
- * page or position outside its tables; looking clears it. */
+ * page or position outside its tables, or if one of the attention kernel's
+ * bounded waits ran out (its outputs are then not valid); looking clears it. */
 int fwb_kv4_status(void *stream);
 
 /* Arguments of fwb_kv4_append_dev.  Strides are in elements, the head_dim
@@ -360,8 +361,8 @@ typedef struct fwb_kv4_attn {
  * probabilities are rounded to fp16; fp32 calls carry 22 bits of both.
  * workspace: fwb_kv4_attention_workspace(a) bytes of device memory, 16-byte
  * aligned, that no other call uses meanwhile (a captured call's: at every
- * replay).  It must be all zeros before its first use; calls leave it fit for
- * the next one, of any sizes.  n_seq * n_query * n_head is at most 2^31 - 1, and
+ * replay).  Its first 4096 bytes must be zeros before its first use; calls leave
+ * it fit for the next one, of any sizes.  n_seq * n_query * n_head is at most 2^31 - 1, and
  * so are the query rows' tiles of 8 to 32 times the page table's tiles of 16.
  */
 int fwb_kv4_attention_dev(const fwb_kv4_attn_t *a, void *workspace, size_t workspace_bytes, void *stream);

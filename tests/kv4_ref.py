@@ -98,14 +98,16 @@ def attention(q, k, v, lengths, n_new=None, scale=None):
     return out, lse, mass, reach
 
 
-def bounds(q, out, lse, mass, reach, most):
+def bounds(q, out, lse, mass, reach, most, heads):
     """How far a call's out and lse may be from these. Scores: a product of 32 exact pairs is summed in fp32 whose
     additions may truncate (2^-23 each, 32 + 4 + 2 of them, queries of fp32 calls held to 2^-22): under 2^-17 of reach.
     The average: twice the scores' errors, probabilities with their scales held to 2^-11 (fp32 calls 2^-21) and exp2 to
     2^-21, sums of `most` terms in fp32;
-    and the output's rounding. Products below 2^-24 of 2^8 times the largest scale are lost: 2^-20 of mass's largest covers them."""
+    and the output's rounding. bf16 calls of many rows hold keys and values to 2^-11 as well. Products below 2^-24 of 2^8 times the largest scale are lost: 2^-20 of mass's largest covers them."""
     p = 2.0 ** -11 if q.dtype != torch.float32 else 2.0 ** -21
     ds = 2.0 ** -17 * reach
+    if q.dtype == torch.bfloat16 and q.shape[1] * (q.shape[2] // heads) >= 64:
+        ds, p = ds + 2.0 ** -11 * reach, p + 2.0 ** -11
     rel = p + 2.0 ** -20 + 2 * ds + (most / 16 + 32) * 2.0 ** -23
     tol = mass * rel[..., None] + mass.amax(-1, keepdim=True) * 2.0 ** -20 + out.abs() * half_step(q.dtype)
     return tol, ds + 2.0 ** -20 + lse.abs() * 2.0 ** -23
@@ -113,7 +115,7 @@ def bounds(q, out, lse, mass, reach, most):
 
 def check_attention(got, got_lse, q, k, v, lengths, n_new=None, scale=None):
     out, lse, mass, reach = attention(q, k, v, lengths, n_new, scale)
-    tol, tol_lse = bounds(q, out, lse.nan_to_num(neginf=0.0), mass, reach, k.shape[1])
+    tol, tol_lse = bounds(q, out, lse.nan_to_num(neginf=0.0), mass, reach, k.shape[1], k.shape[2])
     for s in range(q.shape[0]):
         fresh = q.shape[1] if n_new is None else int(n_new[s])
         d = (got[s, :fresh].double() - out[s, :fresh]).abs()
