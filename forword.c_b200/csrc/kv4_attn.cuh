@@ -10,20 +10,29 @@
 // and the products run on the codes, which fp16 holds exactly; the scales
 // multiply the 32-wide partial scores and the probabilities in fp32.
 //
-// Bound: DRAM (72 bytes per position, head and side at head_dim 128) for large
-// batches, the ends of the launch for small ones; see the figures at the
-// kernel.  Positions are the rows of the m16n8k16 products and query rows the
-// columns: a group's few rows fill 8 columns, and an instruction multiplies
-// 256 values of K or V, which is what unpacking them at the memory's rate
-// leaves room for.  (tcgen05 would want them unpacked into shared memory.)
+// Bound: at head_dim 128 a position is 144 bytes for a KV head, 55 cycles of an
+// SM at the memory's rate, and takes a warp 25 to 30 instructions, three in ten
+// of them on codes: large batches are bound by instruction issue (the integer
+// pipe 55 % busy, 2.3 instructions a cycle), small ones by latency, a launch of
+// one item 7.5 us.  Positions are the rows of the m16n8k16 products and query
+// rows the columns: a group's few rows fill 8 columns, and an instruction
+// multiplies 256 values of K or V as they come unpacked into registers.  (On
+// tcgen05 they would pass through shared memory, which pays from 64 rows on:
+// kv4_attn_tc.cuh.)
 //
-// Work: an item is (sequence, row tile, KV head); the items' tiles of 16
+// Work: an item is (sequence, row tile, KV head); the items' pairs of tiles of 16
 // positions stand in one line that is cut evenly over the CTAs, an item's ends
-// counting as kKaCost tiles.  The eight warps of a CTA take an item's tiles in
-// turn, each with a ring of its own that it fills by 16-byte copies, and join
-// their results in shared memory at the item's end.  Where an item is cut, its
-// parts go to the workspace and the CTA that arrives last adds them, in the
-// order of the positions whichever arrives last.
+// counting as `cost` of them, and a cut near an item's end moves there.  The
+// eight warps of a CTA take an item's pairs in turn, each with a ring of its own
+// that it fills by 16-byte copies, and join their results in shared memory at
+// the item's end.  Where an item is cut, its parts go to the workspace and the
+// CTA that arrives last adds them, in the order of the positions whichever
+// arrives last.
+//
+// Measured on a B200 (us; graphs of calls on alternating inputs; heads of 128
+// dimensions): 64 bf16 sequences of up to 8191 positions, 64 heads on 8, 84 (308
+// MB: 3.7 TB/s); one fp16 token, 32 heads on 8, at 8000 positions 14.1; one fp32
+// token at 200 8.1; 9 bf16 sequences of 7 tokens at 4099 35.1.
 #pragma once
 #include "kv4_format.cuh"
 
@@ -308,15 +317,12 @@ struct KaSmem {
     static constexpr uint32_t kRingBytes = kRing > kJoin ? kRing : kJoin, kBytes = kRingBytes + kQueries;
 };
 
-// H tiles of 16 positions.  Keys' codes go into the products as they lie,
-// under a mask: a nibble in the low bits of a half is the subnormal code * 2^-24
-// (16 times that in bits 4..7), so a pair costs one instruction, and the sums
-// begin at -8 in every place.  Values, whose sums run on, and all codes of fp32
-// calls (the tensor cores' sums truncate at their largest term: 3e-6 of the
-// result instead of 3e-7) are unpacked to code - 8.  EDGE: some rows may not see all of them, or a
-// tile is not there.  q: the queries' B operand [n][hi, lo][b] for each lane in shared memory (NT > 1); r: in registers.
+// H tiles of 16 positions.  (Keys' codes as they lie under a mask, with sums that
+// begin at -8 in every place, cost the scores 1e-6: the tensor cores' sums
+// truncate at their largest term.)  EDGE: some rows may not see all positions, or
+// a tile is not there.  sq: the queries' B operand [n][hi, lo][b] for each lane.
 template <bool SPLIT, int NB, int NT, int H, bool EDGE>
-__device__ __forceinline__ void ka_step(const Kv4AttnArgs &args, const uint8_t *pair, const uint4 *sq, const float *soff, const KaItem &it,
+__device__ __forceinline__ void ka_step(const Kv4AttnArgs &args, const uint8_t *pair, const uint4 *sq, const KaItem &it,
                                         int32_t pos0, uint32_t there, const float (&qs)[NT][2], float (&o)[NT][NB][2][4],
                                         float (&mm)[NT][2], float (&thr)[NT][2], float (&l)[NT][2], float &vref) {
     constexpr uint32_t TB = kv4_tile(NB);
@@ -343,19 +349,11 @@ __device__ __forceinline__ void ka_step(const Kv4AttnArgs &args, const uint8_t *
             float k0[H], k1[H];
 #pragma unroll
             for (int h = 0; h < H; ++h) {
-                if constexpr (SPLIT) {
-                    uint32_t x[4], y[4];
-                    ka_codes(w0[h][b], x);
-                    ka_codes(w1[h][b], y);
-                    a0[h][0] = x[0]; a0[h][1] = y[0]; a0[h][2] = x[1]; a0[h][3] = y[1];
-                    a1[h][0] = x[2]; a1[h][1] = y[2]; a1[h][2] = x[3]; a1[h][3] = y[3];
-                } else {
-                    const uint32_t x = w0[h][b], y = w1[h][b];
-                    a0[h][0] = x & 0x000f000fu; a0[h][1] = y & 0x000f000fu;
-                    a0[h][2] = x & 0x00f000f0u; a0[h][3] = y & 0x00f000f0u;
-                    a1[h][0] = x >> 8 & 0x000f000fu; a1[h][1] = y >> 8 & 0x000f000fu;
-                    a1[h][2] = x >> 8 & 0x00f000f0u; a1[h][3] = y >> 8 & 0x00f000f0u;
-                }
+                uint32_t x[4], y[4];
+                ka_codes(w0[h][b], x);
+                ka_codes(w1[h][b], y);
+                a0[h][0] = x[0]; a0[h][1] = y[0]; a0[h][2] = x[1]; a0[h][3] = y[1];
+                a1[h][0] = x[2]; a1[h][1] = y[2]; a1[h][2] = x[3]; a1[h][3] = y[3];
                 const float2 e0 = kv4_unpack(d0[h][b / 2]), e1 = kv4_unpack(d1[h][b / 2]);
                 k0[h] = b % 2 ? e0.y : e0.x;
                 k1[h] = b % 2 ? e1.y : e1.x;
@@ -363,12 +361,8 @@ __device__ __forceinline__ void ka_step(const Kv4AttnArgs &args, const uint8_t *
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 uint4 q, r = {};
-                float2 off = {};
-                {
-                    if constexpr (!SPLIT) off = *reinterpret_cast<const float2 *>(soff + (n * NB + b) * 8 + 2 * c);
-                    q = sq[((n * (SPLIT ? 2 : 1)) * NB + b) * 32 + lane];
-                    if constexpr (SPLIT) r = sq[((n * 2 + 1) * NB + b) * 32 + lane];
-                }
+                q = sq[((n * (SPLIT ? 2 : 1)) * NB + b) * 32 + lane];
+                if constexpr (SPLIT) r = sq[((n * 2 + 1) * NB + b) * 32 + lane];
 #pragma unroll
                 for (int h = 0; h < H; ++h) {
                     float acc[4];
@@ -377,7 +371,7 @@ __device__ __forceinline__ void ka_step(const Kv4AttnArgs &args, const uint8_t *
                         ka_mma(acc, a1[h], r.z, r.w);
                         ka_mma(acc, a0[h], q.x, q.y);
                     } else {
-                        ka_mma(acc, a0[h], q.x, q.y, off.x, off.y, off.x, off.y);
+                        ka_mma(acc, a0[h], q.x, q.y, 0.f, 0.f, 0.f, 0.f);
                     }
                     ka_mma(acc, a1[h], q.z, q.w);
                     s[h][n][0] = fmaf(k0[h], acc[0], s[h][n][0]);
@@ -590,7 +584,6 @@ __global__ void __launch_bounds__(kKaThreads, NT <= 2 ? 2 : 1) kv4_attn_kernel(c
     __shared__ float sref[kKaWarps];
     __shared__ float sw[kKaWarps][ROWS];   // weights of the warps' results
     __shared__ float2 srow[ROWS];          // an item's references and sums
-    __shared__ __align__(8) float soff[NT * NB * 8];
     __shared__ float sqs[ROWS];            // of its queries
     __shared__ KaScan scan;
     __shared__ uint32_t slast;
@@ -651,8 +644,7 @@ __global__ void __launch_bounds__(kKaThreads, NT <= 2 ? 2 : 1) kv4_attn_kernel(c
 
             // --- queries: the products' B operand, columns of 8 rows ---
             // 16 threads a row, 8 dimensions each.  A row is taken times a power
-            // of two, its largest value in [2^13, 2^14); but for SPLIT pairs 1 and 3
-            // of each eight, whose codes weigh 16 times as much, 1/16 of that.
+            // of two, its largest value in [2^13, 2^14).
             for (uint32_t i = tid; i < ROWS * 16; i += kKaThreads) {
                 const uint32_t r = i / 16, ch = i % 16, b = ch / 4, row = rt * ROWS + r, t = row / a.gq, d = 8 * ch;
                 float4 v0 = {0.f, 0.f, 0.f, 0.f}, v1 = v0;
@@ -676,25 +668,20 @@ __global__ void __launch_bounds__(kKaThreads, NT <= 2 ? 2 : 1) kv4_attn_kernel(c
                 const uint32_t ex = min(max(__float_as_uint(top) >> 23, 14u), 254u);
                 const float up = __uint_as_float((267u - ex) << 23);
                 uint32_t hi[4], lo[4];
-                float sum = 0.f;  // as the products have them
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const float by = !SPLIT && k & 1 ? up * 0.0625f : up, y0 = x[2 * k] * by, y1 = x[2 * k + 1] * by;
+                    const float y0 = x[2 * k] * up, y1 = x[2 * k + 1] * up;
                     hi[k] = kv4_pack(y0, y1);
                     const float2 f = kv4_unpack(hi[k]);
                     lo[k] = kv4_pack(y0 - f.x, y1 - f.y);
-                    sum += (k & 1 ? 16.f : 1.f) * (f.x + f.y);
                 }
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
                 if (b < NB) {
                     const uint32_t at = ((r / 8) * (SPLIT ? 2 : 1) * NB + b) * 32 + r % 8 * 4 + ch % 4;
                     sq[at] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
                     if constexpr (SPLIT) sq[at + NB * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-                    if (ch % 4 == 0) soff[(r / 8 * NB + b) * 8 + r % 8] = sum * (-8.f / 16777216.f);
                 }
-                // codes stand there as multiples of 2^-24 (SPLIT: of 2^-9); past 2^100 the factor would not be finite
-                if (ch == 0) sqs[r] = (__uint_as_float((ex - 13u) << 23) + (ex < 227 ? odd : NAN)) * (a.scale * 1.4426950408889634f) * (SPLIT ? kKaCode : 16777216.f);
+                // codes stand there as multiples of 2^-9
+                if (ch == 0) sqs[r] = (__uint_as_float((ex - 13u) << 23) + (ex < 227 ? odd : NAN)) * (a.scale * 1.4426950408889634f) * kKaCode;
             }
             float qs[NT][2], mm[NT][2], thr[NT][2], l[NT][2], o[NT][NB][2][4], vref = 6.103515625e-05f;  // 2^-14
             __syncthreads();
@@ -722,13 +709,13 @@ __global__ void __launch_bounds__(kKaThreads, NT <= 2 ? 2 : 1) kv4_attn_kernel(c
                 const int32_t pos0 = (int32_t)((from + warp + i * kKaWarps) * kKaPair);
                 const bool edge = pos0 + (int32_t)kKaPair > least || ok != 3;
                 if constexpr (NT == 1) {  // both tiles at once: one look at the references for two
-                    if (edge) ka_step<SPLIT, NB, NT, 2, true>(a, pair, sq, soff, it, pos0, ok, qs, o, mm, thr, l, vref);
-                    else ka_step<SPLIT, NB, NT, 2, false>(a, pair, sq, soff, it, pos0, ok, qs, o, mm, thr, l, vref);
+                    if (edge) ka_step<SPLIT, NB, NT, 2, true>(a, pair, sq, it, pos0, ok, qs, o, mm, thr, l, vref);
+                    else ka_step<SPLIT, NB, NT, 2, false>(a, pair, sq, it, pos0, ok, qs, o, mm, thr, l, vref);
                 } else {                  // one after the other: registers
 #pragma unroll 1
                     for (int h = 0; h < 2; ++h) {
-                        if (edge) ka_step<SPLIT, NB, NT, 1, true>(a, pair + h * S::kTile, sq, soff, it, pos0 + 16 * h, ok >> h, qs, o, mm, thr, l, vref);
-                        else ka_step<SPLIT, NB, NT, 1, false>(a, pair + h * S::kTile, sq, soff, it, pos0 + 16 * h, ok >> h, qs, o, mm, thr, l, vref);
+                        if (edge) ka_step<SPLIT, NB, NT, 1, true>(a, pair + h * S::kTile, sq, it, pos0 + 16 * h, ok >> h, qs, o, mm, thr, l, vref);
+                        else ka_step<SPLIT, NB, NT, 1, false>(a, pair + h * S::kTile, sq, it, pos0 + 16 * h, ok >> h, qs, o, mm, thr, l, vref);
                     }
                 }
                 __syncwarp();

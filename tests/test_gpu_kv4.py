@@ -291,6 +291,31 @@ def test_one_score_far_above(torch, kv4, dtype):
         ref.check_attention(*plan(q, p.cache, p.table, p.lengths), q, k, v, [500])
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("gq", [1, 12, 30])
+def test_codes_that_are_zero_add_nothing(torch, kv4, dtype, gq):
+    """A score of a few small products keeps its digits beside large query values that meet zeros."""
+    hd, n = 64, 37
+    p = ref.Pages(kv4, [n], 1, hd, 16)
+    k = torch.zeros(1, n, 1, hd, device="cuda")
+    k[..., 5], k[..., 37] = -8.0, -8.0       # the blocks' scales are 1
+    k[..., 11], k[..., 50] = 1.0, 3.0
+    kv4.append(torch.zeros(1, n, gq, hd, device="cuda"), k, k, p.cache, p.table, p.lengths)
+    q = noise(torch, 3, 1, 1, gq, hd).abs().add(1.0)
+    q[..., 5], q[..., 37] = 0.0, 0.0
+    q[..., 11], q[..., 50] = q[..., 11] / 1024, q[..., 50] / 2048
+    q = q.to(ref.DTYPES[dtype])
+    plan = kv4.Attention(n_seq=1, n_query=1, n_head=gq, n_head_kv=1, head_dim=hd, dtype=q.dtype, page_size=16, n_page=p.cache.shape[0],
+                         max_pages=p.table.shape[1], scale=1024.0)
+    lse = torch.empty(1, 1, gq, device="cuda")
+    plan(q, p.cache, p.table, p.lengths, lse=lse)
+    want = 1024 * (q[0, 0, :, 11].double() + 3 * q[0, 0, :, 50].double()) + math.log(n)
+    # two products and their sum at 2^-23 of their size, the factor back at 2^-23, the log of the sum and its addition
+    # 2^-22: below 2^-20 of all of it (fp32 queries: their two halves carry 22 bits of the row's largest, 4 / 2^22 * 2^10 more)
+    slack = 2 * 1024 * 4 * 2.0 ** -22 if dtype == "f32" else 0.0
+    assert bool(((lse[0, 0].double() - want).abs() <= want.abs() * 2.0 ** -20 + slack).all())
+
+
 @pytest.mark.parametrize("dtype", ["f32", "f16"])
 @pytest.mark.parametrize("sizes", [(1e-4, 1e-4), (1.0, 1e4), (1e4, 1.0), (1e-3, 30.0)])
 def test_sizes_of_values(torch, kv4, dtype, sizes):
