@@ -387,10 +387,12 @@ size_t fwb_kv4_attention_workspace(const fwb_kv4_attn_t *a);
  * A logit of -inf bars its token.  A row that holds a NaN or +inf, is barred
  * throughout, or has a temperature or uniform number that is NaN gets token -1
  * and -inf.  Entries of weight below 2^-64 count as nothing, neither for top_k
- * nor in a mass, and ones below 2^-32 need not, where they make up less than
- * 2^-24 of the mass.  Weights carry 22 bits and are added exactly, so a token can
- * differ from exact arithmetic's only where a limit falls within about 2^-22
- * of the mass of a border.  n_vocab at most 262144.
+ * nor in a mass; ones below 2^-32 are not drawn where they make up less than
+ * 2^-24 of the mass, and a top_k or min_p that would keep some of them keeps none
+ * where they make up less than 2^-20 of the mass besides the first entry's.
+ * Weights carry 22 bits and are added exactly, so a token can differ from exact
+ * arithmetic's only where a limit falls within about 2^-22 of the mass of a
+ * border.  n_vocab at most 262144.
  */
 int fwb_sample_rows_dev(const void *d_logits, uint32_t type, size_t n_row, size_t n_vocab, size_t row_stride,
                         const float *d_uniform, const float *d_temperature, const int32_t *d_top_k, const float *d_top_p,

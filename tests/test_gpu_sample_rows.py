@@ -230,6 +230,52 @@ def test_repeats_graphs_and_streams(torch, sample_rows):
         assert all(torch.equal(a, b) for o in outs for a, b in zip(o, want))
 
 
+@pytest.mark.parametrize("setting", [dict(), dict(k=7), dict(k=300), dict(p=0.99999), dict(low=1e-6), dict(low=1e-12), dict(k=300, p=0.9999, low=1e-9)],
+                         ids=lambda s: "-".join(s) + str(s.get("k", s.get("low", ""))) if s else "none")
+@pytest.mark.parametrize("V", [1000, 32003])
+def test_one_token_holds_nearly_all(torch, sample_rows, setting, V):
+    """The first token's log keeps its digits where the others hold up to half and down to 2^-50 of the mass between them."""
+    gaps = [7.0, 9.0, 14.0, 18.0, 21.5, 24.0, 27.0, 31.0, 36.0]
+    n = len(gaps)
+    # multiples of 2^-8: the differences of logits are exact in 32 bits
+    x = torch.round(logits(torch, 8, n, V).clamp(-8, 5) * 256) / 256
+    x[:, V // 3] = 5 + torch.tensor(gaps, device="cuda")
+    full = {name: [setting.get(name, d)] * n for name, d in (("k", 0), ("p", 1.0), ("low", 0.0))}
+    token, logprob = sample_rows(x, torch.full((n,), 0.25, device="cuda"), top_k=torch.tensor(full["k"], dtype=torch.int32, device="cuda"),
+                                 top_p=torch.tensor(full["p"], device="cuda"), min_p=torch.tensor(full["low"], device="cuda"))
+    for i in range(n):
+        p, low = (float(torch.tensor(full[k][i])) for k in ("p", "low"))
+        s = torch.sort(x[i].double(), descending=True)[0]
+        w = torch.exp(s - s[0])
+        w = w[w > 2.0 ** -64]
+        w = w[:full["k"][i] or len(w)]
+        before = torch.cumsum(w, 0) - w
+        if p < 1:
+            border = (before - p * float(w.sum())).abs()
+            w = w[(before < p * float(w.sum())) | (before == 0)]
+            if float(border[1:].min()) < 2.0 ** -20:   # the cut may be off by an entry
+                continue
+        w = w[w >= low]
+        rest = float(w[1:].sum())
+        want = -math.log1p(rest)
+        # Each other weight: 2^-22 of the exponential, 2^-23 of its step in a bin; what lies below 2^-32 up to
+        # V / 4096 in a row in 32 bits, 8 * 2^-24; what a filter leaves of it 2^-20.  Together below 2^-19.  The mass in
+        # 64 bits, its quotient and its log: a step of 2^-52 each at most.
+        assert int(token[i]) == V // 3
+        assert abs(float(logprob[i]) - want) <= abs(want) * 2.0 ** -19 + 3 * 2.0 ** -52, (i, float(logprob[i]), want)
+
+
+@pytest.mark.parametrize("setting", [dict(), dict(k=3), dict(k=4), dict(k=40), dict(p=0.5), dict(low=2.0 ** -32), dict(low=2.0 ** -33)], ids=str)
+@pytest.mark.parametrize("u", [0.0, 0.5, 1.0])
+def test_weights_at_a_step_of_32_octaves(torch, sample_rows, setting, u):
+    """Logits whose weights are 2^-32 and its neighbours, to the last bit or nearly."""
+    x = torch.full((1, 900), -math.inf, device="cuda")
+    x[0, 10], x[0, 500] = 0.0, -1.0
+    x[0, 20], x[0, 600], x[0, 30], x[0, 800] = -32.0, -32.0, -32.0 + 2.0 ** -18, -32.0 - 2.0 ** -18
+    x[0, 700], x[0, 40] = -63.0, -40.0
+    check(torch, sample_rows, x, [u], temp=[math.log2(math.e)], **{name: [v] for name, v in setting.items()})
+
+
 def test_refusals(torch, sample_rows):
     from fwb.model import FwbError
     x, u = logits(torch, 1, 3, 100), torch.zeros(3, device="cuda")
