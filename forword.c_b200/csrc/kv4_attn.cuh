@@ -10,12 +10,12 @@
 // and the products run on the codes, which fp16 holds exactly; the scales
 // multiply the 32-wide partial scores and the probabilities in fp32.
 //
-// Bound: at head_dim 128 a position is 144 bytes for a KV head, 55 cycles of an
-// SM at the memory's rate, and takes a warp 25 to 30 instructions, three in ten
-// of them on codes: large batches are bound by instruction issue (the integer
-// pipe 55 % busy, 2.3 instructions a cycle), small ones by latency, a launch of
-// one item 7.5 us.  Positions are the rows of the m16n8k16 products and query
-// rows the columns: a group's few rows fill 8 columns, and an instruction
+// Bound: at head_dim 128 a position is 144 bytes for a KV head, 6 cycles of an SM
+// at the memory's rate, and 24 instructions of a warp, three in ten of them on
+// codes, 10 cycles at the 2.4 a cycle that issue: large batches are bound by
+// issue (integer pipe 46 % busy, tensor pipe 20 %), small ones by latency, a
+// launch of one item 7.5 us.  Positions are the rows of the m16n8k16 products and
+// query rows the columns: a group's few rows fill 8 columns, and an instruction
 // multiplies 256 values of K or V as they come unpacked into registers.  (On
 // tcgen05 they would pass through shared memory, which pays from 64 rows on:
 // kv4_attn_tc.cuh.)

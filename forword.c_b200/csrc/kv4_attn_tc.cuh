@@ -6,11 +6,12 @@
 // A CTA has 128 query rows as the M dimension of S = Q K^T (64 positions) and
 // O += P V; S, O, Q and P are in tensor memory (with Q and P in shared memory a
 // tile of 16 products of 64 columns took 1.1 us, most of it reading Q).  Eight
-// warps unpack a tile's keys and values into shared memory (a thread a position and a quarter of its dimensions), four
-// do the softmax (a thread a row), and a thread each issues the products of the
-// one and the other kind (together they took it 1.9 us a tile).  Keys and values
-// have rings of two tiles each: a tile's keys are done with as soon as its scores
-// are formed, and the scores of tile i + 1 are formed while tile i's softmax runs.
+// warps unpack a tile's keys and values into shared memory (a thread a position
+// and a quarter of its dimensions), four do the softmax (a thread a row), and a
+// thread each issues the products of the one and the other kind (one for both
+// took 1.9 us a tile for that alone).  Keys and values have rings of two tiles
+// each: a tile's keys are done with as soon as its scores are formed, and the
+// scores of tile i + 1 are formed while tile i's softmax runs.
 //
 // A position's scales are taken times a power of two of its own, which leaves
 // the largest in [2^14, 2^15) and multiplies the scores, or the weights, in fp32:
@@ -19,11 +20,11 @@
 // first's rounding; bf16 calls, whose result's rounding is 8 times one of fp16,
 // take the first alone.
 //
-// Bound: the issue of products (N = 64 columns an instruction, two of them where
-// LOW) and the softmax between them, 1.8 us a tile (bf16 1.5).  Measured on a
-// B200: 512 tokens of 32 fp16 heads on 8 of 128 at 8191 positions 234 us (285
-// TFLOP/s of the formula's, twice that in products), bf16 188 us; warp-level
-// products take 346 and 349.
+// Bound: the chain of a tile's products, softmax and products beside its
+// unpacking, 1.8 us a tile (bf16 1.5); the tensor pipe is 31 % busy, and 2.1
+// instructions issue a cycle.  Measured on a B200: 512 tokens of 32
+// fp16 heads on 8 of 128 at 8191 positions 234 us (285 TFLOP/s of the formula's,
+// twice that in products), bf16 188 us; warp-level products take 346 and 349.
 //
 // The reference of a row is raised, and its part of O rescaled in tensor memory,
 // only when a score exceeds it by 2^7 (see kv4_attn.cuh).  Values that are not
