@@ -7,8 +7,9 @@
 //
 //     s_p = scale sum_b d_kb (codes_pb . q_b),   out = sum_p (exp(s_p - m) d_vb) codes_p
 //
-// and the products run on the codes, which fp16 holds exactly; the scales
-// multiply the 32-wide partial scores and the probabilities in fp32.
+// and the products run on the codes, which 16 bits hold exactly; the scales
+// multiply the 32-wide partial scores and the probabilities in fp32, and what
+// comes of the latter goes into its products in two or three parts of bf16.
 //
 // Bound: at head_dim 128 a position is 144 bytes for a KV head, 6 cycles of an SM
 // at the memory's rate, and 24 instructions of a warp, three in ten of them on
@@ -30,9 +31,12 @@
 // arrives last.
 //
 // Measured on a B200 (us; graphs of calls on alternating inputs; heads of 128
-// dimensions): 64 bf16 sequences of up to 8191 positions, 64 heads on 8, 84 (308
-// MB: 3.7 TB/s); one fp16 token, 32 heads on 8, at 8000 positions 14.1; one fp32
-// token at 200 8.1; 9 bf16 sequences of 7 tokens at 4099 35.1.
+// dimensions): 64 bf16 sequences of up to 8191 positions, 64 heads on 8, 93 (308
+// MB: 3.3 TB/s); one fp16 token, 32 heads on 8, at 8000 positions 14.2; one fp32
+// token at 200 8.0; 9 bf16 sequences of 7 tokens at 4099 38.7.  (With weights as one
+// fp16 relative to the largest value scale 84, 14.0, 8.1, 35.1: where scales lie
+// 2^14 and more apart, in blocks beside one another or in positions that only later
+// tokens see, results were off by up to 400 times their bounds.)
 #pragma once
 #include "kv4_format.cuh"
 
@@ -41,7 +45,8 @@ namespace fwb {
 constexpr int kKaWarps = 8, kKaThreads = 32 * kKaWarps;
 constexpr uint32_t kKaPair = 2 * kKvTile;  // positions that a warp takes at a time
 // Weights are formed as 2^8 exp2(score - reference), and a reference is raised
-// when a score exceeds it by 2^7: they stay below 2^15, which fp16 holds.
+// when a score of its row exceeds it by 2^7: they stay below 2^15 (the tcgen05
+// kernel's go into fp16).
 constexpr float kKaHead = 8.f, kKaLazy = 7.f;
 
 struct Kv4AttnArgs {
@@ -76,6 +81,11 @@ __device__ __forceinline__ void ka_mma(float (&d)[4], const uint32_t (&a)[4], ui
 __device__ __forceinline__ void ka_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     ka_mma(d, a, b0, b1, d[0], d[1], d[2], d[3]);
 }
+__device__ __forceinline__ void ka_mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 // The 8x8 halves that a warp holds as rows, as columns.
 __device__ __forceinline__ uint32_t ka_transpose(uint32_t x) {
     uint32_t y;
@@ -97,6 +107,31 @@ __device__ __forceinline__ void ka_codes(uint32_t w, uint32_t (&h)[4]) {
         h[2 * i] = *reinterpret_cast<const uint32_t *>(&a);
         h[2 * i + 1] = *reinterpret_cast<const uint32_t *>(&b);
     }
+}
+
+// The same as pairs of bf16, times 2^-6 (whose subnormals have 2^-133 for a unit).
+constexpr float kKaValue = 64.f;
+__device__ __forceinline__ void ka_codes_bf16(uint32_t w, uint32_t (&h)[4]) {
+    const __nv_bfloat162 up = __bfloat162bfloat162(__ushort_as_bfloat16(0x7f00)), up16 = __bfloat162bfloat162(__ushort_as_bfloat16(0x7d00)),
+                         eight = __bfloat162bfloat162(__ushort_as_bfloat16(0xbe00));  // 2^127, 2^123, -2^-3
+#pragma unroll
+    for (int i = 0; i < 2; ++i, w >>= 8) {
+        const uint32_t lo = w & 0x000f000fu, hi = w & 0x00f000f0u;
+        const __nv_bfloat162 a = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&lo), up, eight),
+                             b = __hfma2(*reinterpret_cast<const __nv_bfloat162 *>(&hi), up16, eight);
+        h[2 * i] = *reinterpret_cast<const uint32_t *>(&a);
+        h[2 * i + 1] = *reinterpret_cast<const uint32_t *>(&b);
+    }
+}
+// The upper 16 bits of two floats, which are bf16 values, and what they leave of them.
+__device__ __forceinline__ uint32_t ka_upper(float2 x) { return __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x7632u); }
+__device__ __forceinline__ float2 ka_left(float2 x) {
+    const float2 up = make_float2(__uint_as_float(__float_as_uint(x.x) & 0xffff0000u), __uint_as_float(__float_as_uint(x.y) & 0xffff0000u));
+    return __ffma2_rn(up, make_float2(-1.f, -1.f), x);
+}
+__device__ __forceinline__ uint32_t ka_pack_bf16(float2 x) {
+    const __nv_bfloat162 h = __float22bfloat162_rn(x);
+    return *reinterpret_cast<const uint32_t *>(&h);
 }
 
 // NB 32-bit words, or the units of NB 16-bit parts.
@@ -324,7 +359,7 @@ struct KaSmem {
 template <bool SPLIT, int NB, int NT, int H, bool EDGE>
 __device__ __forceinline__ void ka_step(const Kv4AttnArgs &args, const uint8_t *pair, const uint4 *sq, const KaItem &it,
                                         int32_t pos0, uint32_t there, const float (&qs)[NT][2], float (&o)[NT][NB][2][4],
-                                        float (&mm)[NT][2], float (&thr)[NT][2], float (&l)[NT][2], float &vref) {
+                                        float (&mm)[NT][2], float (&thr)[NT][2], float (&l)[NT][2]) {
     constexpr uint32_t TB = kv4_tile(NB);
     const uint32_t lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const uint32_t p0 = (g >> 1) + 4 * (g & 1), p1 = p0 + 8;  // the positions of this lane's rows of the scores
@@ -396,7 +431,8 @@ __device__ __forceinline__ void ka_step(const Kv4AttnArgs &args, const uint8_t *
                 // (thr: the same in terms of the bare score, where there are registers for it)
                 raise |= NT == 1 ? s[h][n][i] > thr[n][i & 1] : fmaf(s[h][n][i], qs[n][i & 1], -mm[n][i & 1]) > kKaHead + kKaLazy;
             }
-    // References follow the scores only when one exceeds its own by 2^7.
+    // A row's reference follows its scores only when one of them exceeds it by 2^7
+    // (its own: what other rows see changes nothing).
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -408,7 +444,8 @@ __device__ __forceinline__ void ka_step(const Kv4AttnArgs &args, const uint8_t *
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                 const float now = fmaf(top, qs[n][j], -kKaHead);
-                if (now > mm[n][j]) {
+                const bool own = NT == 1 ? top > thr[n][j] : fmaf(top, qs[n][j], -mm[n][j]) > kKaHead + kKaLazy;
+                if (own && now > mm[n][j]) {
                     const float f = ka_exp2(mm[n][j] - now);
                     mm[n][j] = now;
                     thr[n][j] = (now + (kKaHead + kKaLazy)) / qs[n][j];
@@ -456,49 +493,20 @@ __device__ __forceinline__ void ka_step(const Kv4AttnArgs &args, const uint8_t *
             v[h][b][1] = __byte_perm(d[2][b / 2], d[3][b / 2], pick) & m1;
         }
     }
-    // They go into the products relative to vref, a power of two not below the
-    // largest so far (each lane looks at a word of each tile's scales).
-    float top = 0.f;
-    if (lane < 8 * NB)
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-            uint32_t word = *reinterpret_cast<const uint32_t *>(pair + h * TB + 2 * kv4_codes(NB) + kv4_scales(NB) + 4 * lane);
-            if constexpr (EDGE) {
-                const int32_t left = there >> h & 1 ? it.limit - pos0 - 16 * h : 0;
-                if ((int32_t)(2 * lane / NB) >= left) word = 0;
-                if ((int32_t)((2 * lane + 1) / NB) >= left) word &= 0xffffu;
-            }
-            const float2 f = kv4_unpack(word);
-            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-        }
-    if (__any_sync(0xffffffffu, top > vref)) {
-        const uint32_t bits = __reduce_max_sync(0xffffffffu, __float_as_uint(fminf(top, 65536.f)));
-        const float now = fmaxf(vref, __uint_as_float((bits + 0x7fffffu) & 0xff800000u));
-        const float f = vref * __uint_as_float((254u << 23) - __float_as_uint(now));  // of powers of two
-        vref = now;
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) o[n][b][t][i] *= f;
-    }
-    const float inv = __uint_as_float((254u << 23) - __float_as_uint(vref));  // 1 / vref, at most 2^14
-    const __half2 inv2 = __half2half2(__float2half_rn(inv));
+    // A weight times its scale goes into the products as parts in bf16, whose range is
+    // fp32's: neither a row's small scales nor a block's vanish beside larger ones (as
+    // fp16, with a reference of the largest scale, those 2^-14 of it and less lost bits).
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-        // the weights' transposes: rows as columns g, positions as above
-        uint32_t w[NT][2], rest[NT][2];  // in two halves
+        // the weights' transposes: rows as columns g, positions as above (moved as two halves of their 32 bits)
+        float2 w[NT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const uint32_t x = kv4_pack(s[h][n][2 * e], s[h][n][2 * e + 1]);
-                const float2 f = kv4_unpack(x);
-                w[n][e] = ka_transpose(x);
-                rest[n][e] = ka_transpose(kv4_pack(s[h][n][2 * e] - f.x, s[h][n][2 * e + 1] - f.y));
+                const uint32_t x = __float_as_uint(s[h][n][2 * e]), y = __float_as_uint(s[h][n][2 * e + 1]),
+                               up = ka_transpose(__byte_perm(x, y, 0x7632u)), low = ka_transpose(__byte_perm(x, y, 0x5410u));
+                w[n][e] = make_float2(__uint_as_float(__byte_perm(low, up, 0x5410u)), __uint_as_float(__byte_perm(low, up, 0x7632u)));
             }
         uint32_t mask[NT][2];
         if constexpr (EDGE)
@@ -517,63 +525,58 @@ __device__ __forceinline__ void ka_step(const Kv4AttnArgs &args, const uint8_t *
         for (int b = 0; b < NB; ++b) {
             const uint32_t pick = b % 2 ? 0x7632u : 0x5410u;
             uint32_t x[4], y[4];
-            ka_codes(__byte_perm(u[0][b / 2], u[1][b / 2], pick), x);
-            ka_codes(__byte_perm(u[2][b / 2], u[3][b / 2], pick), y);
+            ka_codes_bf16(__byte_perm(u[0][b / 2], u[1][b / 2], pick), x);
+            ka_codes_bf16(__byte_perm(u[2][b / 2], u[3][b / 2], pick), y);
             const uint32_t a0[4] = {x[0], x[1], y[0], y[1]}, a1[4] = {x[2], x[3], y[2], y[3]};
-            if constexpr (SPLIT) {
-                // Each weight times its scale in two halves, and sums of 16
-                // positions added in rounded fp32: the tensor cores' own
-                // additions truncate.
-                const float2 v0 = kv4_unpack(v[h][b][0]), v1 = kv4_unpack(v[h][b][1]);
+            const float2 v0 = kv4_unpack(v[h][b][0]), v1 = kv4_unpack(v[h][b][1]);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const float2 x0 = kv4_unpack(w[n][0]), x1 = kv4_unpack(w[n][1]), y0 = kv4_unpack(rest[n][0]), y1 = kv4_unpack(rest[n][1]);
-                    const float f0 = (x0.x + y0.x) * (v0.x * inv), f1 = (x0.y + y0.y) * (v0.y * inv),
-                                f2 = (x1.x + y1.x) * (v1.x * inv), f3 = (x1.y + y1.y) * (v1.y * inv);
-                    uint32_t b0 = kv4_pack(f0, f1), b1 = kv4_pack(f2, f3);
-                    const float2 h0 = kv4_unpack(b0), h1 = kv4_unpack(b1);
-                    uint32_t r0 = kv4_pack(f0 - h0.x, f1 - h0.y), r1 = kv4_pack(f2 - h1.x, f3 - h1.y);
-                    if constexpr (EDGE) {  // (a scale may be NaN)
-                        b0 &= mask[n][0]; r0 &= mask[n][0];
-                        b1 &= mask[n][1]; r1 &= mask[n][1];
+            for (int n = 0; n < NT; ++n) {
+                const float2 f0 = __fmul2_rn(w[n][0], v0), f1 = __fmul2_rn(w[n][1], v1), r0 = ka_left(f0), r1 = ka_left(f1);
+                // 8 bits and the rest: 8 and 8 bits in fp32 calls, all of it; 8 with a rounding, 2^-17, in the others
+                uint32_t p[3][2] = {{ka_upper(f0), ka_upper(f1)}, {}, {}};
+                if constexpr (SPLIT) {
+                    p[1][0] = ka_upper(r0);
+                    p[1][1] = ka_upper(r1);
+                    p[2][0] = ka_pack_bf16(ka_left(r0));
+                    p[2][1] = ka_pack_bf16(ka_left(r1));
+                } else {
+                    p[1][0] = ka_pack_bf16(r0);
+                    p[1][1] = ka_pack_bf16(r1);
+                }
+                constexpr int kParts = SPLIT ? 3 : 2;
+                if constexpr (EDGE)  // (a scale may be NaN)
+#pragma unroll
+                    for (int i = 0; i < kParts; ++i) {
+                        p[i][0] &= mask[n][0];
+                        p[i][1] &= mask[n][1];
                     }
-                    float t0[4], t1[4];
-                    ka_mma(t0, a0, r0, r1, 0.f, 0.f, 0.f, 0.f);
-                    ka_mma(t1, a1, r0, r1, 0.f, 0.f, 0.f, 0.f);
-                    ka_mma(t0, a0, b0, b1);
-                    ka_mma(t1, a1, b0, b1);
+                if constexpr (SPLIT) {
+                    // sums of 16 positions added in rounded fp32: the tensor cores' own additions truncate
+                    float t0[4] = {0.f, 0.f, 0.f, 0.f}, t1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = kParts - 1; i >= 0; --i) {
+                        ka_mma_bf16(t0, a0, p[i][0], p[i][1]);
+                        ka_mma_bf16(t1, a1, p[i][0], p[i][1]);
+                    }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         o[n][b][0][i] += t0[i];
                         o[n][b][1][i] += t1[i];
                     }
-                }
-            } else {
-                // a weight times its scale, rounded to fp16 once (the rest of the
-                // weight is below its last bit, so its own product's rounding is nothing)
-                const __half2 v0 = __hmul2(*reinterpret_cast<const __half2 *>(&v[h][b][0]), inv2),
-                              v1 = __hmul2(*reinterpret_cast<const __half2 *>(&v[h][b][1]), inv2);
+                } else {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const __half2 x0 = __hfma2(*reinterpret_cast<const __half2 *>(&w[n][0]), v0,
-                                               __hmul2(*reinterpret_cast<const __half2 *>(&rest[n][0]), v0)),
-                                  x1 = __hfma2(*reinterpret_cast<const __half2 *>(&w[n][1]), v1,
-                                               __hmul2(*reinterpret_cast<const __half2 *>(&rest[n][1]), v1));
-                    uint32_t b0 = *reinterpret_cast<const uint32_t *>(&x0), b1 = *reinterpret_cast<const uint32_t *>(&x1);
-                    if constexpr (EDGE) {
-                        b0 &= mask[n][0];
-                        b1 &= mask[n][1];
+                    for (int i = kParts - 1; i >= 0; --i) {
+                        ka_mma_bf16(o[n][b][0], a0, p[i][0], p[i][1]);
+                        ka_mma_bf16(o[n][b][1], a1, p[i][0], p[i][1]);
                     }
-                    ka_mma(o[n][b][0], a0, b0, b1);
-                    ka_mma(o[n][b][1], a1, b0, b1);
                 }
             }
         }
     }
 }
 
-// SPLIT: fp32 calls, whose queries and weights go through the products as two
-// halves each.  NT: column tiles of 8 query rows.
+// SPLIT: fp32 calls, whose queries go through the products as two halves and
+// whose weights as three parts.  NT: column tiles of 8 query rows.
 template <bool SPLIT, int NB, int NT>
 __global__ void __launch_bounds__(kKaThreads, NT <= 2 ? 2 : 1) kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
     using S = KaSmem<SPLIT, NB, NT>;
@@ -581,7 +584,6 @@ __global__ void __launch_bounds__(kKaThreads, NT <= 2 ? 2 : 1) kv4_attn_kernel(c
     constexpr int kKaStages = S::kStages;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ float2 sml[kKaWarps][ROWS];
-    __shared__ float sref[kKaWarps];
     __shared__ float sw[kKaWarps][ROWS];   // weights of the warps' results
     __shared__ float2 srow[ROWS];          // an item's references and sums
     __shared__ float sqs[ROWS];            // of its queries
@@ -683,7 +685,7 @@ __global__ void __launch_bounds__(kKaThreads, NT <= 2 ? 2 : 1) kv4_attn_kernel(c
                 // codes stand there as multiples of 2^-9
                 if (ch == 0) sqs[r] = (__uint_as_float((ex - 13u) << 23) + (ex < 227 ? odd : NAN)) * (a.scale * 1.4426950408889634f) * kKaCode;
             }
-            float qs[NT][2], mm[NT][2], thr[NT][2], l[NT][2], o[NT][NB][2][4], vref = 6.103515625e-05f;  // 2^-14
+            float qs[NT][2], mm[NT][2], thr[NT][2], l[NT][2], o[NT][NB][2][4];
             __syncthreads();
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -709,13 +711,13 @@ __global__ void __launch_bounds__(kKaThreads, NT <= 2 ? 2 : 1) kv4_attn_kernel(c
                 const int32_t pos0 = (int32_t)((from + warp + i * kKaWarps) * kKaPair);
                 const bool edge = pos0 + (int32_t)kKaPair > least || ok != 3;
                 if constexpr (NT == 1) {  // both tiles at once: one look at the references for two
-                    if (edge) ka_step<SPLIT, NB, NT, 2, true>(a, pair, sq, it, pos0, ok, qs, o, mm, thr, l, vref);
-                    else ka_step<SPLIT, NB, NT, 2, false>(a, pair, sq, it, pos0, ok, qs, o, mm, thr, l, vref);
+                    if (edge) ka_step<SPLIT, NB, NT, 2, true>(a, pair, sq, it, pos0, ok, qs, o, mm, thr, l);
+                    else ka_step<SPLIT, NB, NT, 2, false>(a, pair, sq, it, pos0, ok, qs, o, mm, thr, l);
                 } else {                  // one after the other: registers
 #pragma unroll 1
                     for (int h = 0; h < 2; ++h) {
-                        if (edge) ka_step<SPLIT, NB, NT, 1, true>(a, pair + h * S::kTile, sq, it, pos0 + 16 * h, ok >> h, qs, o, mm, thr, l, vref);
-                        else ka_step<SPLIT, NB, NT, 1, false>(a, pair + h * S::kTile, sq, it, pos0 + 16 * h, ok >> h, qs, o, mm, thr, l, vref);
+                        if (edge) ka_step<SPLIT, NB, NT, 1, true>(a, pair + h * S::kTile, sq, it, pos0 + 16 * h, ok >> h, qs, o, mm, thr, l);
+                        else ka_step<SPLIT, NB, NT, 1, false>(a, pair + h * S::kTile, sq, it, pos0 + 16 * h, ok >> h, qs, o, mm, thr, l);
                     }
                 }
                 __syncwarp();
@@ -741,7 +743,6 @@ __global__ void __launch_bounds__(kKaThreads, NT <= 2 ? 2 : 1) kv4_attn_kernel(c
                         *reinterpret_cast<float4 *>(so + (warp * ROWS + row) * S::kStride + 32 * b + 4 * g) =
                             make_float4(o[n][b][0][j], o[n][b][0][j + 2], o[n][b][1][j], o[n][b][1][j + 2]);
                 }
-            if (lane == 0) sref[warp] = vref;
             __syncthreads();
             if (tid < ROWS) {
                 float top = -INFINITY, sum = 0.f;
@@ -752,7 +753,7 @@ __global__ void __launch_bounds__(kKaThreads, NT <= 2 ? 2 : 1) kv4_attn_kernel(c
                 for (int w = 0; w < kKaWarps; ++w) {
                     const float f = ka_exp2(sml[w][tid].x - ref);
                     sum = fmaf(f, sml[w][tid].y, sum);
-                    sw[w][tid] = f * (sref[w] * kKaCode);
+                    sw[w][tid] = f * kKaValue;
                 }
                 srow[tid] = make_float2(top, sum);
             }
