@@ -13,21 +13,26 @@
 // each: a tile's keys are done with as soon as its scores are formed, and the
 // scores of tile i + 1 are formed while tile i's softmax runs.
 //
-// A position's scales are taken times a power of two of its own, which leaves
-// the largest in [2^14, 2^15) and multiplies the scores, or the weights, in fp32:
-// unpacked values neither overflow nor vanish.  LOW (fp16 calls): a value d *
+// The scales of a position's key are taken times a power of two, which leaves the
+// largest in [2^14, 2^15) and multiplies its scores in fp32: unpacked keys do not
+// overflow, and lose 2^-33 of the largest at most.  LOW (fp16 calls): a key d *
 // (code - 8) has up to 15 bits and goes in as two halves, the second exactly the
-// first's rounding; bf16 calls, whose result's rounding is 8 times one of fp16,
-// take the first alone.
+// first's rounding; bf16 calls take the first alone.  A position's values go in
+// as they are, in two parts of bf16 that hold them exactly, and the weights in two
+// parts, 16 bits of them (three of the four products are formed): with bf16's
+// range neither a block's small scales nor a row's vanish beside larger ones.
+// (One part of fp16 each, weights relative to the largest scale so far of all
+// rows' positions: 234 us for the 246 below, and values that only later tokens
+// see, or of other blocks, took bits of a result.)
 //
 // Bound: the chain of a tile's products, softmax and products beside its
-// unpacking, 1.8 us a tile (bf16 1.5); the tensor pipe is 31 % busy, and 2.1
+// unpacking, 1.9 us a tile (bf16 1.7); the tensor pipe is 31 % busy, and 2.1
 // instructions issue a cycle.  Measured on a B200: 512 tokens of 32
-// fp16 heads on 8 of 128 at 8191 positions 234 us (285 TFLOP/s of the formula's,
-// twice that in products), bf16 188 us; warp-level products take 346 and 349.
+// fp16 heads on 8 of 128 at 8191 positions 246 us (271 TFLOP/s of the formula's,
+// two and a half times that in products), bf16 220 us.
 //
 // The reference of a row is raised, and its part of O rescaled in tensor memory,
-// only when a score exceeds it by 2^7 (see kv4_attn.cuh).  Values that are not
+// only when a score of it exceeds it by 2^7 (see kv4_attn.cuh).  Values that are not
 // finite would reach every row of a product, seen or not: they go in as zeros,
 // and rows that see their position get NaN in their block at the end.
 #pragma once
@@ -43,15 +48,15 @@ template <int NB, bool LOW>
 struct KtSmem {
     static constexpr int kDims = 32 * NB, kSub = kDims / 64, kHalves = LOW ? 2 : 1;
     static constexpr uint32_t kSubBytes = kKtKeys * 128;               // 64 dimensions of a tile's keys or values
-    static constexpr uint32_t kPart = kSub * kSubBytes;                // one half of them all
-    static constexpr uint32_t kStage = kHalves * kPart;                // of keys or values
-    static constexpr uint32_t kOffV = 2 * kStage, kOffTail = 4 * kStage;
+    static constexpr uint32_t kPart = kSub * kSubBytes;                // one half, or part, of them all
+    static constexpr uint32_t kStage = kHalves * kPart;                // of keys
+    static constexpr uint32_t kStageV = 2 * kPart;
+    static constexpr uint32_t kOffV = 2 * kStage, kOffTail = kOffV + 2 * kStageV;
 };
 struct KtTail {
     uint64_t kfull[2], vfull[2], sfull[2], sfree[2], pfull[2], pdone[2], qfull, ofree;
     uint32_t tmem, slast;
-    alignas(16) float ek[2][kKtKeys], fv[2][kKtKeys];  // what keys' scores and values' weights are multiplied with
-    alignas(16) float vmax[2][8];                      // the largest fv of each making warp's positions
+    alignas(16) float ek[2][kKtKeys];                  // what keys' scores are multiplied with
     alignas(8) uint8_t absent[2][8];                   // positions that are not there, a bit each
     alignas(8) uint8_t odd[2][4][8];                   // values that are not finite, by block
     KaScan scan;
@@ -81,9 +86,10 @@ __device__ __forceinline__ void kt_read(const uint8_t *p, uint32_t (&w)[NB]) {
 __device__ __forceinline__ void kt_store16(uint32_t at, const uint32_t (&w)[4]) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
 }
-// fp32 accumulator, fp16 A (128 rows, K-major) and B (n columns).
-__device__ __forceinline__ uint32_t kt_idesc(uint32_t n, bool b_mn_major) {
-    return 1u << 4 | (b_mn_major ? 1u << 16 : 0u) | (n >> 3) << 17 | (128u >> 4) << 24;
+// fp32 accumulator, A (128 rows, K-major) and B (n columns): fp16, K-major B, for
+// the scores; bf16, MN-major B, for the average.
+__device__ __forceinline__ uint32_t kt_idesc(uint32_t n, bool values) {
+    return 1u << 4 | (values ? 1u << 7 | 1u << 10 | 1u << 16 : 0u) | (n >> 3) << 17 | (128u >> 4) << 24;
 }
 // The position, of the eight of a making warp's half tile, of lanes 4 q ..: two
 // neighbours lie four rows apart, so that eight lanes' 16-byte stores to swizzled
@@ -97,20 +103,15 @@ __device__ __forceinline__ uint8_t kt_positions(uint32_t votes) {
     return (uint8_t)x;
 }
 
-// One position's scales: the finite ones times the power of two that leaves the
-// largest in [2^14, 2^15); returns what undoes it (and the codes' 2^-9).
+// The scales of a position's key times the power of two that leaves the largest
+// (finite) one in [2^14, 2^15); returns what undoes it (and the codes' 2^-9).
 template <int NB>
-__device__ __forceinline__ float kt_scales(const uint32_t (&raw)[NB / 2], __half2 (&d)[NB], uint32_t &odd, bool drop) {
+__device__ __forceinline__ float kt_scales(const uint32_t (&raw)[NB / 2], __half2 (&d)[NB]) {
     float x[NB], top = 0.f;
-    odd = 0;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         const float2 f = kv4_unpack(raw[b / 2]);
         x[b] = b % 2 ? f.y : f.x;
-        if (!(fabsf(x[b]) < INFINITY)) {
-            odd |= 1u << b;
-            if (drop) x[b] = 0.f;
-        }
         if (fabsf(x[b]) < INFINITY) top = fmaxf(top, fabsf(x[b]));
     }
     const uint32_t ex = max(__float_as_uint(top) >> 23, 103u);  // (fp16's least is 2^-24)
@@ -119,10 +120,9 @@ __device__ __forceinline__ float kt_scales(const uint32_t (&raw)[NB / 2], __half
     for (int b = 0; b < NB; ++b) d[b] = __half2half2(__float2half_rn(x[b] * up));
     return top == 0.f ? 0.f : __uint_as_float((ex - 5u) << 23);
 }
-
-// Codes times a scale, in one half or two, to a swizzled row.
+// A key's codes times a scale, in one half or two, to a swizzled row.
 template <bool LOW>
-__device__ __forceinline__ void kt_values(uint32_t word, __half2 d, uint32_t at, uint32_t part) {
+__device__ __forceinline__ void kt_key(uint32_t word, __half2 d, uint32_t at, uint32_t part) {
     uint32_t code[4], hi[4], lo[4];
     ka_codes(word, code);
 #pragma unroll
@@ -134,42 +134,59 @@ __device__ __forceinline__ void kt_values(uint32_t word, __half2 d, uint32_t at,
     kt_store16(at, hi);
     if constexpr (LOW) kt_store16(at + part, lo);
 }
+// A value's in two parts of bf16.  The scale has 11 bits: 8 and what is left; the
+// first product rounded to 8, and what is left of both, which 8 hold: exact.
+__device__ __forceinline__ void kt_value(uint32_t word, float scale, uint32_t at, uint32_t part) {
+    const __nv_bfloat16 up = __float2bfloat16_rn(scale);
+    const __nv_bfloat162 d = __bfloat162bfloat162(up), e = __float2bfloat162_rn(scale - __bfloat162float(up));
+    uint32_t code[4], hi[4], lo[4];
+    ka_codes_bf16(word, code);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const __nv_bfloat162 x = *reinterpret_cast<const __nv_bfloat162 *>(&code[j]), h = __hmul2(x, d),
+                             r = __hfma2(x, e, __hfma2(x, d, __hneg2(h)));
+        hi[j] = *reinterpret_cast<const uint32_t *>(&h);
+        lo[j] = *reinterpret_cast<const uint32_t *>(&r);
+    }
+    kt_store16(at, hi);
+    kt_store16(at + part, lo);
+}
 // A position's quarter of keys into a stage; eight positions a warp at a time.
 template <int NB, bool LOW>
 __device__ __forceinline__ float kt_make_keys(const KtRaw<NB> &raw, uint32_t stage, uint32_t p, uint32_t c) {
     using S = KtSmem<NB, LOW>;
     __half2 d[NB];
-    uint32_t odd;
-    const float ek = kt_scales<NB>(raw.dk, d, odd, false);
+    const float ek = kt_scales<NB>(raw.dk, d);
 #pragma unroll
     for (int b = 0; b < NB; ++b)
-        kt_values<LOW>(raw.k[b], d[b], stage + p * 128 + (b / 2) * S::kSubBytes + (((4 * (b % 2) + c) ^ (p & 7)) << 4), S::kPart);
+        kt_key<LOW>(raw.k[b], d[b], stage + p * 128 + (b / 2) * S::kSubBytes + (((4 * (b % 2) + c) ^ (p & 7)) << 4), S::kPart);
     return ek;
 }
 // Its values, and what the softmax needs of the position (which stays until the
 // tile's weights are used, as its values do; its keys go earlier).
-template <int NB, bool LOW>
+template <int NB>
 __device__ __forceinline__ void kt_make_values(const KtRaw<NB> &raw, float ek, uint32_t stage, KtTail &t, uint32_t s, uint32_t p, uint32_t c) {
-    using S = KtSmem<NB, LOW>;
-    __half2 d[NB];
-    uint32_t odd;
-    const float fv = kt_scales<NB>(raw.dv, d, odd, true);
+    using S = KtSmem<NB, true>;
+    uint32_t odd = 0;
     const uint32_t chunk = c ^ (p & 2);  // units 2c and 2c + 1 as they lie: dimensions 8 chunk.. of every block
 #pragma unroll
-    for (int b = 0; b < NB; ++b)         // (of the eight: (0, 4), (1, 5), (2, 6), (3, 7))
-        kt_values<LOW>(__byte_perm(raw.v[b / 2], raw.v[NB / 2 + b / 2], b % 2 ? 0x7632u : 0x5410u), d[b],
-                       stage + p * 128 + (b / 2) * S::kSubBytes + (((4 * (b % 2) + chunk) ^ (p & 7)) << 4), S::kPart);
-    if (c == 0) {
-        t.ek[s][p] = ek;
-        t.fv[s][p] = fv;
+    for (int b = 0; b < NB; ++b) {       // (of the eight: (0, 4), (1, 5), (2, 6), (3, 7))
+        const float2 f = kv4_unpack(raw.dv[b / 2]);
+        float d = (b % 2 ? f.y : f.x) * kKaValue;
+        if (!(fabsf(d) < INFINITY)) {
+            odd |= 1u << b;
+            d = 0.f;
+        }
+        kt_value(__byte_perm(raw.v[b / 2], raw.v[NB / 2 + b / 2], b % 2 ? 0x7632u : 0x5410u), d,
+                 stage + p * 128 + (b / 2) * S::kSubBytes + (((4 * (b % 2) + chunk) ^ (p & 7)) << 4), S::kPart);
     }
-    const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(fv)), gone = __ballot_sync(0xffffffffu, !raw.there), any = __ballot_sync(0xffffffffu, odd != 0);
+    if (c == 0) t.ek[s][p] = ek;
+    const uint32_t gone = __ballot_sync(0xffffffffu, !raw.there), any = __ballot_sync(0xffffffffu, odd != 0);
     uint32_t bad[4] = {0, 0, 0, 0};
     if (any)
 #pragma unroll
         for (int b = 0; b < NB; ++b) bad[b] = __ballot_sync(0xffffffffu, odd >> b & 1);
     if (threadIdx.x % 32 == 0) {
-        t.vmax[s][p / 8] = __uint_as_float(most);
         t.absent[s][p / 8] = kt_positions(gone);
 #pragma unroll
         for (int b = 0; b < 4; ++b) t.odd[s][b][p / 8] = kt_positions(bad[b]);
@@ -180,7 +197,7 @@ template <int NB, bool LOW>
 __global__ void __launch_bounds__(kKtThreads, 1) kv4_attn_tc_kernel(const __grid_constant__ Kv4AttnArgs a) {
     using S = KtSmem<NB, LOW>;
     using T = typename std::conditional<LOW, __half, __nv_bfloat16>::type;
-    constexpr uint32_t kTmem = 512, kO = 2 * kKtKeys, kQ = kO + 128, kP = kQ + 64;  // columns: scores, O, queries, weights
+    constexpr uint32_t kTmem = 512, kO = 2 * kKtKeys, kQ = kO + 128, kP = kQ + 64;  // columns: scores, O, queries, weights (128)
     extern __shared__ __align__(1024) uint8_t kt_sm[];
     KtTail &t = *reinterpret_cast<KtTail *>(kt_sm + S::kOffTail);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -258,7 +275,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv4_attn_tc_kernel(const __grid
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&t.kfull[s]);
                 if (i >= 2) ok = mbar_wait_warp(&t.pdone[s], (i >> 1 & 1) ^ 1, a.wait_err, ERR_WAIT_EMPTY) && ok;
-                kt_make_values<NB, LOW>(now, ek, smem + S::kOffV + s * S::kStage, t, s, p, c);
+                kt_make_values<NB>(now, ek, smem + S::kOffV + s * S::kStageV, t, s, p, c);
                 bt_fence_proxy();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&t.vfull[s]);
@@ -304,18 +321,18 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv4_attn_tc_kernel(const __grid
                 if (seg) ok = mbar_wait(&t.ofree, (seg - 1) & 1, a.wait_err, ERR_WAIT_EMPTY) && ok;
                 ++seg;
                 for (uint32_t k = 0; k < n; ++k, ++i) {
-                    const uint32_t b = i & 1, ph = i >> 1 & 1, v = smem + S::kOffV + b * S::kStage, ps = tmem + kP + b * (kKtKeys / 2);
+                    const uint32_t b = i & 1, ph = i >> 1 & 1, v = smem + S::kOffV + b * S::kStageV, ps = tmem + kP + b * kKtKeys;
                     ok = mbar_wait(&t.vfull[b], ph, a.wait_err, ERR_WAIT_FULL) && ok;
                     ok = mbar_wait(&t.pfull[b], ph, a.wait_err, ERR_WAIT_FULL) && ok;
                     bt_fence_after();
                     bt_fence_proxy();
                     if (ok)
 #pragma unroll
-                        for (int h = S::kHalves - 1; h >= 0; --h)
+                        for (int h = 2; h >= 0; --h)  // the weights' and the values' second parts, then the first of both
 #pragma unroll
                             for (int u = 0; u < kKtKeys / 16; ++u)
-                                bt_mma_ta(tmem + kO, ps + u * 8, bt_desc(v + h * S::kPart + u * 2048, NB == 2 ? 0 : S::kSubBytes), ido,
-                                          k || u != 0 || h != S::kHalves - 1);
+                                bt_mma_ta(tmem + kO, ps + (h == 2 ? kKtKeys / 2 : 0) + u * 8,
+                                          bt_desc(v + (h == 1 ? S::kPart : 0) + u * 2048, NB == 2 ? 0 : S::kSubBytes), ido, k || u != 0 || h != 2);
                     bt_commit(&t.pdone[b]);
                 }
             } while (ln.next());
@@ -373,9 +390,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv4_attn_tc_kernel(const __grid
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&t.qfull);
             }
-            // ref: 8 less than the row's reference, plus lv = log2 of the largest fv so
-            // far: weights exp2(score - ref) times a position's fv stay below 2^15
-            float ref = -INFINITY, l = 0.f, lv = -29.f;
+            float ref = -INFINITY, l = 0.f;  // ref: 8 less than the row's reference
             uint32_t nan = 0;
             for (uint32_t k = 0; k < n; ++k, ++i) {
                 const uint32_t b = i & 1, ph = i >> 1 & 1;
@@ -417,15 +432,11 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv4_attn_tc_kernel(const __grid
                 float top = y[0];
 #pragma unroll
                 for (int j = 1; j < kKtKeys; ++j) top = fmaxf(top, y[j]);
-                const float4 v0 = *reinterpret_cast<const float4 *>(&t.vmax[b][0]), v1 = *reinterpret_cast<const float4 *>(&t.vmax[b][4]);
-                const float vtop = fmaxf(fmaxf(fmaxf(v0.x, v0.y), fmaxf(v0.z, v0.w)), fmaxf(fmaxf(v1.x, v1.y), fmaxf(v1.z, v1.w)));
-                const float vlog = (float)(int)(__float_as_uint(vtop) >> 23) - 127.f;  // (a power of two, or 0)
-                if (__any_sync(0xffffffffu, vlog > lv || fmaf(top, qs, -ref) > kKaHead + kKaLazy - lv)) {
+                const bool own = fmaf(top, qs, -ref) > kKaHead + kKaLazy;
+                if (__any_sync(0xffffffffu, own)) {
                     const float was = ref;
-                    ref += fmaxf(vlog - lv, 0.f);
-                    lv = fmaxf(lv, vlog);
-                    ref = fmaxf(ref, fmaf(top, qs, lv - kKaHead));
-                    const float f = ref == -INFINITY ? 1.f : ka_exp2(was - ref);
+                    if (own) ref = fmaf(top, qs, -kKaHead);
+                    const float f = own ? ka_exp2(was - ref) : 1.f;
                     l *= f;
                     if (k) {
                         ok = mbar_wait_warp(&t.pdone[b ^ 1], (i - 1) >> 1 & 1, a.wait_err, ERR_WAIT_FULL) && ok;
@@ -443,27 +454,26 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv4_attn_tc_kernel(const __grid
                         bt_st_wait();
                     }
                 }
-                const uint32_t ps = tmem + kP + b * (kKtKeys / 2) + lanes;
+                const uint32_t ps = tmem + kP + b * kKtKeys + lanes;
 #pragma unroll
                 for (int j = 0; j < kKtKeys; j += 16) {
-                    uint32_t w[8];
+                    uint32_t w[8], r[8];
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        const float4 f = *reinterpret_cast<const float4 *>(&t.fv[b][j + 4 * h]);
-                        const float fv[4] = {f.x, f.y, f.z, f.w};
-                        float x[4];
+                    for (int h = 0; h < 8; ++h) {
+                        float2 x;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float v = y[j + 4 * h + e];
-                            x[e] = ka_exp2(fmaf(v, qs, -ref));
-                            if (edge && v == -INFINITY) x[e] = 0.f;
-                            l += x[e];
-                            x[e] *= fv[e];
+                        for (int e = 0; e < 2; ++e) {
+                            const float v = y[j + 2 * h + e];
+                            float p = ka_exp2(fmaf(v, qs, -ref));
+                            if (edge && v == -INFINITY) p = 0.f;
+                            l += p;
+                            (e ? x.y : x.x) = p;
                         }
-                        w[2 * h] = kv4_pack(x[0], x[1]);
-                        w[2 * h + 1] = kv4_pack(x[2], x[3]);
+                        w[h] = ka_upper(x);
+                        r[h] = ka_pack_bf16(ka_left(x));
                     }
                     bt_st8(ps + j / 2, w);
+                    bt_st8(ps + kKtKeys / 2 + j / 2, r);
                 }
                 bt_st_wait();
                 bt_fence_before();

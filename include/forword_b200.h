@@ -358,8 +358,7 @@ typedef struct fwb_kv4_attn {
  * 2^100 or more, gets NaN, and so does one that sees a NaN key (with a NaN value,
  * the dimensions of its block); what lies past the positions that a token sees
  * reaches it in no way.  fp16 and bf16 queries are exact in the products, weighted
- * probabilities carry 16 bits (11 in the kernel for many rows); fp32 calls carry 22
- * and 24.
+ * probabilities carry 16 bits; fp32 calls carry 22 and 24.
  * workspace: fwb_kv4_attention_workspace(a) bytes of device memory, 16-byte
  * aligned, that no other call uses meanwhile (a captured call's: at every
  * replay).  Its first 4096 bytes must be zeros before its first use; calls leave

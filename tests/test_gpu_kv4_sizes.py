@@ -77,10 +77,7 @@ def test_blocks_beside_one_another(torch, kv4, dtype, apart, n, nq, nh, nkv, hd,
     unequal(torch, kv4, dtype, n, nq, nh, nkv, hd, length, apart)
 
 
-@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
-@pytest.mark.parametrize("n,nq,nh,nkv,hd,length", FEW)
-def test_positions_of_unequal_values(torch, kv4, dtype, n, nq, nh, nkv, hd, length):
-    """One position in nine has values of 5e4 where its score leaves it next to no weight."""
+def outweighed(torch, kv4, dtype, n, nq, nh, nkv, hd, length):
     dt = ref.DTYPES[dtype]
     q = noise(torch, 1, n, nq, nh, hd).abs().add(0.1).to(dt)       # all positive
     kv = noise(torch, 2, 2, n, length, nkv, hd)
@@ -92,3 +89,10 @@ def test_positions_of_unequal_values(torch, kv4, dtype, n, nq, nh, nkv, hd, leng
     kv4.append(None, kv[0], kv[1], p.cache, p.table, p.lengths)
     k, v = kv4.read(p.cache, p.table, torch.zeros_like(p.lengths), length, head_dim=hd, dtype=torch.float32)
     check_blocks(*call(kv4, p, q, nkv), q, k, v, [length] * n)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("n,nq,nh,nkv,hd,length", FEW)
+def test_positions_of_unequal_values(torch, kv4, dtype, n, nq, nh, nkv, hd, length):
+    """One position in nine has values of 5e4 where its score leaves it next to no weight."""
+    outweighed(torch, kv4, dtype, n, nq, nh, nkv, hd, length)
