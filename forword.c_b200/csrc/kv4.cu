@@ -162,13 +162,13 @@ bool launch_attn(const Kv4AttnArgs &k, uint32_t ctas, cudaStream_t st) {
     return launched(launch_after(kv4_attn_kernel<SPLIT, NB, NT>, dim3(ctas), kKaThreads, smem, 1, st, k), kAttn);
 }
 
-template <int NB, bool LOW>
+template <typename T, int NB>
 bool launch_attn_tc(const Kv4AttnArgs &k, uint32_t ctas, cudaStream_t st) {
     static bool ready[64] = {};
-    constexpr uint32_t smem = kt_smem<NB, LOW>();
+    constexpr uint32_t smem = kt_smem<NB>();
     static_assert(smem <= 227 * 1024, "shared memory");
-    if (!opt_in(kv4_attn_tc_kernel<NB, LOW>, smem, ready, kAttn)) return false;
-    return launched(launch_after(kv4_attn_tc_kernel<NB, LOW>, dim3(ctas), kKtThreads, smem, 1, st, k), kAttn);
+    if (!opt_in(kv4_attn_tc_kernel<T, NB>, smem, ready, kAttn)) return false;
+    return launched(launch_after(kv4_attn_tc_kernel<T, NB>, dim3(ctas), kKtThreads, smem, 1, st, k), kAttn);
 }
 
 template <bool SPLIT, int NB>
@@ -331,8 +331,8 @@ int fwb_kv4_attention_dev(const fwb_kv4_attn_t *a, void *workspace, size_t works
         k.snap = 16;
         k.least = 32;
         k.whole = 0x3fffffff;
-        const bool ok = a->type == 1 ? (L.nb == 4 ? launch_attn_tc<4, true>(k, L.ctas, st) : launch_attn_tc<2, true>(k, L.ctas, st))
-                                     : (L.nb == 4 ? launch_attn_tc<4, false>(k, L.ctas, st) : launch_attn_tc<2, false>(k, L.ctas, st));
+        const bool ok = a->type == 1 ? (L.nb == 4 ? launch_attn_tc<__half, 4>(k, L.ctas, st) : launch_attn_tc<__half, 2>(k, L.ctas, st))
+                                     : (L.nb == 4 ? launch_attn_tc<__nv_bfloat16, 4>(k, L.ctas, st) : launch_attn_tc<__nv_bfloat16, 2>(k, L.ctas, st));
         return ok ? 0 : -1;
     }
     return (a->type == 0 ? pick_blocks<true>(k, L, st) : pick_blocks<false>(k, L, st)) ? 0 : -1;

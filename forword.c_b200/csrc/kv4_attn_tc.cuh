@@ -15,9 +15,10 @@
 //
 // The scales of a position's key are taken times a power of two, which leaves the
 // largest in [2^14, 2^15) and multiplies its scores in fp32: unpacked keys do not
-// overflow, and lose 2^-33 of the largest at most.  LOW (fp16 calls): a key d *
-// (code - 8) has up to 15 bits and goes in as two halves, the second exactly the
-// first's rounding; bf16 calls take the first alone.  A position's values go in
+// overflow, and lose 2^-33 of the largest at most.  A key d * (code - 8) has up to
+// 15 bits and goes in as two halves, the second exactly the first's rounding (the
+// first alone took 220 us for bf16's 233 below and cost scores 2^-11 of sum |q||k|,
+// which a call of fewer rows, in kv4_attn.cuh, does not lose).  A position's values go in
 // as they are, in two parts of bf16 that hold them exactly, and the weights in two
 // parts, 16 bits of them (three of the four products are formed): with bf16's
 // range neither a block's small scales nor a row's vanish beside larger ones.
@@ -26,10 +27,10 @@
 // see, or of other blocks, took bits of a result.)
 //
 // Bound: the chain of a tile's products, softmax and products beside its
-// unpacking, 1.9 us a tile (bf16 1.7); the tensor pipe is 31 % busy, and 2.1
+// unpacking, 1.9 us a tile; the tensor pipe is 31 % busy, and 2.1
 // instructions issue a cycle.  Measured on a B200: 512 tokens of 32
 // fp16 heads on 8 of 128 at 8191 positions 246 us (271 TFLOP/s of the formula's,
-// two and a half times that in products), bf16 220 us.
+// two and a half times that in products), bf16 233 us.
 //
 // The reference of a row is raised, and its part of O rescaled in tensor memory,
 // only when a score of it exceeds it by 2^7 (see kv4_attn.cuh).  Values that are not
@@ -44,14 +45,13 @@ namespace fwb {
 constexpr int kKtRows = 128, kKtKeys = 64;
 constexpr int kKtSoft = kKtRows, kKtMake = 4 * kKtKeys, kKtThreads = kKtSoft + kKtMake + 64;
 
-template <int NB, bool LOW>
+template <int NB>
 struct KtSmem {
-    static constexpr int kDims = 32 * NB, kSub = kDims / 64, kHalves = LOW ? 2 : 1;
+    static constexpr int kDims = 32 * NB, kSub = kDims / 64;
     static constexpr uint32_t kSubBytes = kKtKeys * 128;               // 64 dimensions of a tile's keys or values
     static constexpr uint32_t kPart = kSub * kSubBytes;                // one half, or part, of them all
-    static constexpr uint32_t kStage = kHalves * kPart;                // of keys
-    static constexpr uint32_t kStageV = 2 * kPart;
-    static constexpr uint32_t kOffV = 2 * kStage, kOffTail = kOffV + 2 * kStageV;
+    static constexpr uint32_t kStage = 2 * kPart;                      // of keys or values
+    static constexpr uint32_t kOffV = 2 * kStage, kOffTail = 4 * kStage;
 };
 struct KtTail {
     uint64_t kfull[2], vfull[2], sfull[2], sfree[2], pfull[2], pdone[2], qfull, ofree;
@@ -61,8 +61,8 @@ struct KtTail {
     alignas(8) uint8_t odd[2][4][8];                   // values that are not finite, by block
     KaScan scan;
 };
-template <int NB, bool LOW>
-constexpr uint32_t kt_smem() { return KtSmem<NB, LOW>::kOffTail + sizeof(KtTail); }
+template <int NB>
+constexpr uint32_t kt_smem() { return KtSmem<NB>::kOffTail + sizeof(KtTail); }
 
 // What a thread of the making warps reads of a position: 16 bytes of codes
 // (8 for 64 dimensions) and all scales of its key and value.
@@ -120,8 +120,7 @@ __device__ __forceinline__ float kt_scales(const uint32_t (&raw)[NB / 2], __half
     for (int b = 0; b < NB; ++b) d[b] = __half2half2(__float2half_rn(x[b] * up));
     return top == 0.f ? 0.f : __uint_as_float((ex - 5u) << 23);
 }
-// A key's codes times a scale, in one half or two, to a swizzled row.
-template <bool LOW>
+// A key's codes times a scale, in two halves, to a swizzled row.
 __device__ __forceinline__ void kt_key(uint32_t word, __half2 d, uint32_t at, uint32_t part) {
     uint32_t code[4], hi[4], lo[4];
     ka_codes(word, code);
@@ -132,7 +131,7 @@ __device__ __forceinline__ void kt_key(uint32_t word, __half2 d, uint32_t at, ui
         lo[j] = *reinterpret_cast<const uint32_t *>(&r);
     }
     kt_store16(at, hi);
-    if constexpr (LOW) kt_store16(at + part, lo);
+    kt_store16(at + part, lo);
 }
 // A value's in two parts of bf16.  The scale has 11 bits: 8 and what is left; the
 // first product rounded to 8, and what is left of both, which 8 hold: exact.
@@ -152,21 +151,21 @@ __device__ __forceinline__ void kt_value(uint32_t word, float scale, uint32_t at
     kt_store16(at + part, lo);
 }
 // A position's quarter of keys into a stage; eight positions a warp at a time.
-template <int NB, bool LOW>
+template <int NB>
 __device__ __forceinline__ float kt_make_keys(const KtRaw<NB> &raw, uint32_t stage, uint32_t p, uint32_t c) {
-    using S = KtSmem<NB, LOW>;
+    using S = KtSmem<NB>;
     __half2 d[NB];
     const float ek = kt_scales<NB>(raw.dk, d);
 #pragma unroll
     for (int b = 0; b < NB; ++b)
-        kt_key<LOW>(raw.k[b], d[b], stage + p * 128 + (b / 2) * S::kSubBytes + (((4 * (b % 2) + c) ^ (p & 7)) << 4), S::kPart);
+        kt_key(raw.k[b], d[b], stage + p * 128 + (b / 2) * S::kSubBytes + (((4 * (b % 2) + c) ^ (p & 7)) << 4), S::kPart);
     return ek;
 }
 // Its values, and what the softmax needs of the position (which stays until the
 // tile's weights are used, as its values do; its keys go earlier).
 template <int NB>
 __device__ __forceinline__ void kt_make_values(const KtRaw<NB> &raw, float ek, uint32_t stage, KtTail &t, uint32_t s, uint32_t p, uint32_t c) {
-    using S = KtSmem<NB, true>;
+    using S = KtSmem<NB>;
     uint32_t odd = 0;
     const uint32_t chunk = c ^ (p & 2);  // units 2c and 2c + 1 as they lie: dimensions 8 chunk.. of every block
 #pragma unroll
@@ -193,10 +192,9 @@ __device__ __forceinline__ void kt_make_values(const KtRaw<NB> &raw, float ek, u
     }
 }
 
-template <int NB, bool LOW>
+template <typename T, int NB>
 __global__ void __launch_bounds__(kKtThreads, 1) kv4_attn_tc_kernel(const __grid_constant__ Kv4AttnArgs a) {
-    using S = KtSmem<NB, LOW>;
-    using T = typename std::conditional<LOW, __half, __nv_bfloat16>::type;
+    using S = KtSmem<NB>;
     constexpr uint32_t kTmem = 512, kO = 2 * kKtKeys, kQ = kO + 128, kP = kQ + 64;  // columns: scores, O, queries, weights (128)
     extern __shared__ __align__(1024) uint8_t kt_sm[];
     KtTail &t = *reinterpret_cast<KtTail *>(kt_sm + S::kOffTail);
@@ -270,12 +268,12 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv4_attn_tc_kernel(const __grid
                 }
                 // keys once the scores of the tile before last are formed, values once its weights are used
                 if (i >= 2) ok = mbar_wait_warp(&t.sfull[s], (i >> 1 & 1) ^ 1, a.wait_err, ERR_WAIT_EMPTY) && ok;
-                const float ek = kt_make_keys<NB, LOW>(now, smem + s * S::kStage, p, c);
+                const float ek = kt_make_keys<NB>(now, smem + s * S::kStage, p, c);
                 bt_fence_proxy();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&t.kfull[s]);
                 if (i >= 2) ok = mbar_wait_warp(&t.pdone[s], (i >> 1 & 1) ^ 1, a.wait_err, ERR_WAIT_EMPTY) && ok;
-                kt_make_values<NB>(now, ek, smem + S::kOffV + s * S::kStageV, t, s, p, c);
+                kt_make_values<NB>(now, ek, smem + S::kOffV + s * S::kStage, t, s, p, c);
                 bt_fence_proxy();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&t.vfull[s]);
@@ -299,12 +297,12 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv4_attn_tc_kernel(const __grid
                     bt_fence_proxy();
                     if (ok)
 #pragma unroll
-                        for (int h = S::kHalves - 1; h >= 0; --h)
+                        for (int h = 1; h >= 0; --h)
 #pragma unroll
                             for (int d = 0; d < S::kDims / 16; ++d)
                                 bt_mma_ta(tmem + b * kKtKeys, tmem + kQ + d * 8,
                                           bt_desc(k + h * S::kPart + (d / 4) * S::kSubBytes + (d % 4) * 32, 16), ids,
-                                          d != 0 || h != S::kHalves - 1);
+                                          d != 0 || h != 1);
                     bt_commit(&t.sfull[b]);
                 }
             } while (ln.next());
@@ -321,7 +319,7 @@ __global__ void __launch_bounds__(kKtThreads, 1) kv4_attn_tc_kernel(const __grid
                 if (seg) ok = mbar_wait(&t.ofree, (seg - 1) & 1, a.wait_err, ERR_WAIT_EMPTY) && ok;
                 ++seg;
                 for (uint32_t k = 0; k < n; ++k, ++i) {
-                    const uint32_t b = i & 1, ph = i >> 1 & 1, v = smem + S::kOffV + b * S::kStageV, ps = tmem + kP + b * kKtKeys;
+                    const uint32_t b = i & 1, ph = i >> 1 & 1, v = smem + S::kOffV + b * S::kStage, ps = tmem + kP + b * kKtKeys;
                     ok = mbar_wait(&t.vfull[b], ph, a.wait_err, ERR_WAIT_FULL) && ok;
                     ok = mbar_wait(&t.pfull[b], ph, a.wait_err, ERR_WAIT_FULL) && ok;
                     bt_fence_after();
