@@ -348,8 +348,18 @@ struct KaSmem {
     static constexpr int kStages = NT == 2 ? 2 : 3;
     static constexpr uint32_t kRows = 8 * NT, kTile = kv4_tile(NB), kStage = 2 * kTile, kStride = 32 * NB + 4;
     static constexpr uint32_t kRing = kKaWarps * kStages * kStage, kJoin = kKaWarps * kRows * kStride * 4;
+    // with an item's end, which uses the rings' memory: the warps' references and sums, their weights, the rows'
+    static constexpr uint32_t kSums = kJoin, kWeights = kSums + kKaWarps * kRows * 8, kRowSums = kWeights + kKaWarps * kRows * 4,
+                              kEnd = kRowSums + kRows * 8;
     static constexpr uint32_t kQueries = NT * NB * (SPLIT ? 2 : 1) * 32 * 16;  // after the ring
-    static constexpr uint32_t kRingBytes = kRing > kJoin ? kRing : kJoin, kBytes = kRingBytes + kQueries;
+    static constexpr uint32_t kRingBytes = kRing > kEnd ? kRing : kEnd, kBytes = kRingBytes + kQueries;
+};
+// What a CTA holds besides.
+template <uint32_t ROWS>
+struct KaStatic {
+    float qs[ROWS];  // of its queries
+    KaScan scan;
+    uint32_t last;
 };
 
 // H tiles of 16 positions.  (Keys' codes as they lie under a mask, with sums that
@@ -583,18 +593,18 @@ __global__ void __launch_bounds__(kKaThreads, NT <= 2 ? 2 : 1) kv4_attn_kernel(c
     constexpr uint32_t ROWS = S::kRows;
     constexpr int kKaStages = S::kStages;
     extern __shared__ __align__(128) uint8_t ring[];
-    __shared__ float2 sml[kKaWarps][ROWS];
-    __shared__ float sw[kKaWarps][ROWS];   // weights of the warps' results
-    __shared__ float2 srow[ROWS];          // an item's references and sums
-    __shared__ float sqs[ROWS];            // of its queries
-    __shared__ KaScan scan;
-    __shared__ uint32_t slast;
+    __shared__ KaStatic<ROWS> sh;
+    // two CTAs of an SM's 228 KB, 1 KB of each the system's, static memory in steps of 1 KB
+    static_assert(NT > 2 || 2 * (S::kBytes + (sizeof sh + 1023) / 1024 * 1024 + 1024) <= 228 * 1024, "shared memory of two CTAs");
+    float2(*const sml)[ROWS] = reinterpret_cast<float2(*)[ROWS]>(ring + S::kSums);
+    float(*const sw)[ROWS] = reinterpret_cast<float(*)[ROWS]>(ring + S::kWeights);
+    float2 *const srow = reinterpret_cast<float2 *>(ring + S::kRowSums);
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
     uint4 *const sq = reinterpret_cast<uint4 *>(ring + S::kRingBytes);
     pdl_wait();
 
     KaLine<ROWS, kKaPair> ln(a);
-    if (!ln.begin(scan)) return;
+    if (!ln.begin(sh.scan)) return;
     do {
         if (!ln.item()) break;
         if (ln.last >= blockIdx.x) {
@@ -683,7 +693,7 @@ __global__ void __launch_bounds__(kKaThreads, NT <= 2 ? 2 : 1) kv4_attn_kernel(c
                     if constexpr (SPLIT) sq[at + NB * 32] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                 }
                 // codes stand there as multiples of 2^-9
-                if (ch == 0) sqs[r] = (__uint_as_float((ex - 13u) << 23) + (ex < 227 ? odd : NAN)) * (a.scale * 1.4426950408889634f) * kKaCode;
+                if (ch == 0) sh.qs[r] = (__uint_as_float((ex - 13u) << 23) + (ex < 227 ? odd : NAN)) * (a.scale * 1.4426950408889634f) * kKaCode;
             }
             float qs[NT][2], mm[NT][2], thr[NT][2], l[NT][2], o[NT][NB][2][4];
             __syncthreads();
@@ -691,7 +701,7 @@ __global__ void __launch_bounds__(kKaThreads, NT <= 2 ? 2 : 1) kv4_attn_kernel(c
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    qs[n][j] = sqs[n * 8 + 2 * c + j];
+                    qs[n][j] = sh.qs[n * 8 + 2 * c + j];
                     mm[n][j] = thr[n][j] = -INFINITY;  // nothing seen yet
                     l[n][j] = 0.f;
                 }
@@ -782,9 +792,9 @@ __global__ void __launch_bounds__(kKaThreads, NT <= 2 ? 2 : 1) kv4_attn_kernel(c
             if (parts > 1) {
                 __threadfence();
                 __syncthreads();
-                if (tid == 0) slast = atomicAdd(a.ticket + ln.first, 1u) == parts - 1;
+                if (tid == 0) sh.last = atomicAdd(a.ticket + ln.first, 1u) == parts - 1;
                 __syncthreads();
-                if (slast) {
+                if (sh.last) {
                     __threadfence();
                     if (tid == 0) a.ticket[ln.first] = 0;
                     ka_add_parts<NB, kKaThreads>(ln, tid);
