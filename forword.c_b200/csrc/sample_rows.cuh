@@ -582,6 +582,9 @@ __global__ void __launch_bounds__(kSrThreads, 2) sample_rows_kernel(const __grid
     uint32_t all = light ? near_c : 0xffffffffu, bins = kSrNear, keep_k;
     bool by_k;
     const bool by_p = top_p < 1., by_low = low > 0.f && !(light && deep_low);
+    // (a u of 1 or more asks for the last entry by its rank: by their masses, whose
+    // sums are rounded, entries below 2^-53 of the row's are not told apart)
+    const double drawn = u >= 1.f ? INFINITY : (double)u;
     auto last_bin = [&](bool any) {
         by_k = top_k > 0 && (uint32_t)top_k < all;
         keep_k = by_k ? (uint32_t)top_k : all;
@@ -589,7 +592,7 @@ __global__ void __launch_bounds__(kSrThreads, 2) sample_rows_kernel(const __grid
         uint32_t at = bins;
         if (by_p) at = pass(sh.cum_c, sh.cum_w, bins, false, 0, top_p * total, any);
         if (by_low) at = min(at, low_bin + 1);
-        return by_p || by_low ? at : pass(sh.cum_c, sh.cum_w, bins, false, 0, (double)u * total, any);
+        return by_p || by_low ? at : pass(sh.cum_c, sh.cum_w, bins, false, 0, drawn * total, any);
     };
     uint32_t far = last_bin(light);
     const bool few = far < kSrNear && sh.cum_c[far] <= kSrList;  // (the same in every block)
@@ -638,7 +641,7 @@ __global__ void __launch_bounds__(kSrThreads, 2) sample_rows_kernel(const __grid
                            return i == 0 || s.high(t, rest);
                        }));
         if (by_k || by_p || by_low) kept = sh.list_w[stay - 1];
-        const double limit = (double)u * kept;
+        const double limit = drawn * kept;
         pick = min(prefix([&](uint32_t i) { return sh.list_w[i] <= limit; }), stay - 1);
     };
     bool listed = few;
@@ -698,10 +701,14 @@ __global__ void __launch_bounds__(kSrThreads, 2) sample_rows_kernel(const __grid
             }
             __syncthreads();
         }
-        const double limit = (double)u * kept;
-        near(pass(sh.cum_c, sh.cum_w, bins, false, 0, limit, true), false, 0, limit);
-        pick = prefix([&](uint32_t i) { return base_w + sh.list_w[i] <= limit; });
-        if (base_c + pick >= stay) {  // u is 1, or rounding: the last that stays
+        bool last = u >= 1.f;
+        if (!last) {
+            const double limit = drawn * kept;
+            near(pass(sh.cum_c, sh.cum_w, bins, false, 0, limit, true), false, 0, limit);
+            pick = prefix([&](uint32_t i) { return base_w + sh.list_w[i] <= limit; });
+            last = base_c + pick >= stay;  // (rounding)
+        }
+        if (last) {
             near(pass(sh.cum_c, sh.cum_w, bins, true, stay - 1, 0., true), true, stay - 1, 0.);
             pick = stay - 1 - base_c;
         }
