@@ -713,11 +713,15 @@ __global__ void __launch_bounds__(kSrThreads, 2) sample_rows_kernel(const __grid
             pick = stay - 1 - base_c;
         }
     }
-    const uint32_t index = ~(uint32_t)sh.list[pick];
     if (tid == 0) {
-        const double w = sh.list_w[pick] - (pick ? sh.list_w[pick - 1] : 0.);
-        a.token[row] = (int32_t)index;
-        if (a.logprob) a.logprob[row] = (float)log(w / kept);
+        const unsigned long long e = sh.list[pick];
+        a.token[row] = (int32_t)~(uint32_t)e;
+        if (a.logprob) {  // its own weight: in the running mass it may be below the last bit
+            float t, rest;
+            s.of(sr_value((uint32_t)(e >> 32)), t, rest);
+            const uint32_t k = s.bin(t);
+            a.logprob[row] = (float)log(sr_mass(sh.steps, k, 1, s.frac(t, rest, k)) / kept);
+        }
     }
     if (!few) ask(kSrDone, {}, 0);
 }
