@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(kSrThreads, 2) sample_rows_kernel(const __grid
     s.top = sr_value((uint32_t)(best >> 32));
     if (dead || s.top == -INFINITY || temp != temp || u != u || temp <= 0.f) {  // (the same in every block)
         if (rank == 0 && tid == 0) {
-            const bool greedy = !dead && s.top != -INFINITY && temp <= 0.f;
+            const bool greedy = !dead && s.top != -INFINITY && temp <= 0.f && u == u;
             a.token[row] = greedy ? (int32_t)~(uint32_t)best : -1;
             if (a.logprob) a.logprob[row] = greedy ? 0.f : -INFINITY;
         }
