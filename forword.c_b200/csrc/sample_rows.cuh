@@ -705,8 +705,9 @@ __global__ void __launch_bounds__(kSrThreads, 2) sample_rows_kernel(const __grid
         if (!last) {
             const double limit = drawn * kept;
             near(pass(sh.cum_c, sh.cum_w, bins, false, 0, limit, true), false, 0, limit);
-            pick = prefix([&](uint32_t i) { return base_w + sh.list_w[i] <= limit; });
-            last = base_c + pick >= stay;  // (rounding)
+            // (the bin's sum and the list's are rounded apart: the limit may lie between them, past the list)
+            pick = min(prefix([&](uint32_t i) { return base_w + sh.list_w[i] <= limit; }), n - 1);
+            last = base_c + pick >= stay;
         }
         if (last) {
             near(pass(sh.cum_c, sh.cum_w, bins, true, stay - 1, 0., true), true, stay - 1, 0.);
