@@ -11,6 +11,7 @@
 #include "kv4_attn.cuh"
 #include "kv4_attn_tc.cuh"
 #include "launch.h"
+#include "runs.h"
 
 namespace fwb {
 namespace {
@@ -95,6 +96,27 @@ bool rows_ok(const char *who, uint32_t type, uint32_t n_seq, uint32_t n_tok, uin
     auto step = [&](uint64_t n, uint64_t stride) { return n > 1 ? stride * e : 0; };
     if (((uintptr_t)r.p | step(n_seq, r.seq) | step(n_tok, r.tok) | step(heads, r.head)) % 16)
         return refuse(who, "rows and their strides must be multiples of 16 bytes");
+    return true;
+}
+
+// Rotated queries: rows of their own that do not lie over one another, and the
+// queries' own memory or memory apart from it.
+bool rows_out_ok(const char *who, uint64_t run, const size_t (&n)[3], const Kv4Rows &from, const Kv4Rows &to, uint64_t e) {
+    const size_t in[3] = {from.seq * e, from.tok * e, from.head * e}, out[3] = {to.seq * e, to.tok * e, to.head * e};
+    Runs runs;
+    if (!runs.nested(run, n, out)) return refuse(who, "q_out's rows overlap one another");
+    bool alike = true;
+    uint64_t span = run;  // of the queries
+    for (int i = 0; i < 3; ++i) {
+        if (n[i] == 1) continue;
+        alike = alike && in[i] == out[i];
+        uint64_t over;
+        if (__builtin_mul_overflow(n[i] - 1, in[i], &over) || __builtin_add_overflow(span, over, &span)) span = UINT64_MAX / 2;
+    }
+    const uint64_t at = (uintptr_t)from.p, to_at = (uintptr_t)to.p;
+    const bool near = to_at < at ? at - to_at < runs.span : to_at - at < span;
+    if (near && (!alike || (at != to_at && runs.meets((int64_t)(to_at - at), run))))
+        return refuse(who, "q_out must be q itself or memory apart from it");
     return true;
 }
 
@@ -239,6 +261,8 @@ int fwb_kv4_append_dev(const fwb_kv4_append_t *a, void *stream) {
         (heads && (!rows_ok(who, a->type, a->n_seq, a->n_query, heads, k.q) || !rows_ok(who, a->type, a->n_seq, a->n_query, heads, k.q_out))))
         return -1;
     if (heads > 65535) { refuse(who, "too many heads"); return -1; }
+    const uint64_t e = elem_bytes(a->type);
+    if (heads && !rows_out_ok(who, a->head_dim * e, {a->n_seq, a->n_query, heads}, k.q, k.q_out, e)) return -1;
     k.cache = static_cast<uint8_t *>(a->cache);
     k.pages = a->pages; k.len = a->lengths; k.n_new = a->n_new;
     k.cos = a->cos; k.sin = a->sin;

@@ -292,7 +292,7 @@ typedef struct fwb_kv4_append {
     const void *k, *v;                  /* [n_seq][n_query][n_head_kv][head_dim] */
     uint64_t k_seq_stride, k_token_stride, k_head_stride;
     uint64_t v_seq_stride, v_token_stride, v_head_stride;
-    void *q_out;                        /* as q; q itself, or memory apart from it */
+    void *q_out;                        /* as q, rows of its own; q itself, or memory apart from all that is read */
     uint64_t q_out_seq_stride, q_out_token_stride, q_out_head_stride;
     void *cache;
     const int32_t *pages;               /* [n_seq][max_pages], pages_stride apart */
