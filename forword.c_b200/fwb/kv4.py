@@ -116,13 +116,27 @@ def _ints(t, what: str, shape, dev: int) -> int:
     return t.data_ptr()
 
 
+def _meet(levels, off: int, run: int) -> bool:
+    """Whether runs share a byte with ones of the same layout `off` bytes on; levels: (count, stride) of them, the widest
+    stride first, each level not reaching past the stride before it."""
+    if not levels:
+        return -run < off < run
+    (n, stride), *inner = levels
+    i = off // stride
+    return any(-n < j < n and _meet(inner, off - j * stride, run) for j in (i, i + 1))
+
+
 def _overlap(a, b) -> bool:
-    """Whether the bytes from first to last of two tensors meet."""
-    def end(t):
-        if t.is_contiguous():
-            return t.data_ptr() + t.numel() * t.element_size()
-        return t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
-    return a.data_ptr() < end(b) and b.data_ptr() < end(a)
+    """Whether rows of two tensors of one shape share memory without being the same rows."""
+    off, size = b.data_ptr() - a.data_ptr(), a.element_size()
+    if a.is_contiguous() and b.is_contiguous():
+        return off != 0 and abs(off) < a.numel() * size
+    run = a.shape[3] * size
+    one, other = ([(n, s * size) for n, s in zip(t.shape[:3], t.stride()) if n > 1] for t in (a, b))
+    if one == other:
+        levels = sorted(one, key=lambda level: -level[1])
+        return off != 0 and all(s for _, s in levels) and _meet(levels, off, run)
+    return -sum((n - 1) * s for n, s in other) - run < off < sum((n - 1) * s for n, s in one) + run
 
 
 def append(q, k, v, cache, pages, lengths, cos=None, sin=None, halves: bool = False, n_new=None, q_out=None):
@@ -132,8 +146,10 @@ def append(q, k, v, cache, pages, lengths, cos=None, sin=None, halves: bool = Fa
     n_head_kv, head_dim]: views with a contiguous last dimension, addresses
     and strides multiples of 16 bytes.  cos and sin fp32 [n_pos, head_dim/2],
     None: no rotation; halves: pairs (i, i + head_dim/2) are turned instead of
-    neighbours.  q_out may be q itself; rows of tokens that a padded batch
-    lacks are left as they were (zeros where q_out is None).
+    neighbours.  q_out may be q itself, or memory apart from all that is read, in
+    the gaps between q's rows too; rows of tokens without a position (of a padded
+    batch, below position 0, past the tables) are left as they were: where q_out is
+    None zeros, but with n_new None whatever was there.
     """
     if k is None or k.dim() != 4:
         raise ValueError("k must be [n_seq, n_query, n_head_kv, head_dim]")
