@@ -152,10 +152,12 @@ bool attn_layout(const fwb_kv4_attn_t *a, AttnLayout &L) {
     // More rows than half a tile of the tcgen05 kernel, and tiles for three
     // quarters of the SMs (their items are better left whole: a part is 64 KB).
     // Measured, us for warp-level products / tcgen05 (fp16, 8 KV heads of 128, 4
-    // query heads each): 512 tokens at 8191 positions (128 tiles) 346 / 234, at 512
-    // 56 / 28; 16 sequences of 1000 positions with 16, 32, 64 tokens (128, 128, 256
-    // tiles) 46 / 38, 69 / 39, 124 / 73; of one sequence 32, 64, 128 tokens at 8191 (8,
-    // 16, 32 tiles) 42 / 125, 66 / 134, 105 / 143.
+    // query heads each): 512 tokens at 8191 positions (128 tiles) 420 / 244, at 512
+    // 63 / 28; 16 sequences of 1000 positions with 16, 32, 64 tokens (128, 128, 256
+    // tiles) 55 / 42, 94 / 43, 167 / 82, 12 with 32 (96) 76 / 41; of one sequence 32, 64,
+    // 128, 256 tokens at 8191 (8, 16, 32, 64 tiles) 47 / 215, 70 / 218, 120 / 217, 222 / 222.
+    // (Between half and three quarters of the SMs equal lengths would gain, unequal
+    // ones, whose longest item is one CTA's, lose.)
     const uint64_t tiles = (uint64_t)a->n_seq * a->n_head_kv * ((rows + kKtRows - 1) / kKtRows);
     L.tc = a->type != 0 && (L.nb == 2 || L.nb == 4) && rows >= kKtRows / 2 && 4 * tiles >= 3 * (uint64_t)device_sms();
     L.rows = L.tc ? kKtRows : 8 * L.nt;
@@ -333,10 +335,10 @@ int fwb_kv4_attention_dev(const fwb_kv4_attn_t *a, void *workspace, size_t works
     k.rtiles = L.rtiles;
     // How the line is cut, in pairs of tiles.  Measured (us on the device): an
     // item's ends counted as 8 / 16 / 24 / 32 pairs, 64 sequences of up to 8191
-    // 110 / 87 / 81 / 83; parts of at least 16 / 24 / 40 pairs, one sequence of
-    // 4000 positions 11.9 / 15.3 / 16.3, of 16000 15.9 / 18.3 / 17.1; items of up
-    // to 48 pairs left whole where there is a CTA for each: 1000 positions 11.3,
-    // cut 13.0 (2000: whole 16.3, cut 12.3).
+    // 110 / 96 / 93 / 95; parts of at least 16 / 24 / 40 pairs, one sequence of
+    // 4000 positions 12.7 / 14.8 / 16.8, of 16000 17.4 / 18.9 / 17.6; items of up
+    // to 48 pairs left whole where there is a CTA for each: 1000 positions 12.2,
+    // cut 12.6 (2000: whole 17.7, cut 13.2).
     k.cost = 24;
     k.snap = 8;
     k.least = 16;

@@ -15,14 +15,17 @@
 // exact comparisons, so that a cache's content does not depend on how a sum was
 // rounded.
 //
-// Bound: DRAM for prompts, the launch for steps.  Four lanes hold a block, eight
+// Bound: the launch for steps, the latency of loads for prompts.  Four lanes hold a block, eight
 // values each: its scale is two shuffles of each extreme, a lane has a whole
 // word of a key's codes, and every store goes to bytes of this position alone.
 // Measured on a B200 (us; graphs of calls on alternating inputs), to append and to
 // read back: 64 fp16 sequences of one token, 32 heads of 128 on 8, 3.0 and 2.1; a
-// prompt of 2048 fp32 tokens 20.9 and 8.9; 7 padded bf16 chunks of up to 333
+// prompt of 2048 fp32 tokens 20.9 and 8.9; 7 bf16 chunks of 333
 // tokens, 64 heads on 8, 23.5 and 9.9: 3.5 and 3.0 TB/s together, the ends of two
-// launches in them; exact products and divisions take the rest.
+// launches in them.  Of the prompt's append half of the stall cycles wait for loads,
+// at 64 registers and 42 % of the warps (2.0 instructions a cycle, integer pipe 37 %,
+// the products in 64 bits 1 %); the read spends its time on the indexes of four
+// values a thread (four divisions each) and the same waits (2.6 a cycle).
 #pragma once
 #include "kv4_format.cuh"
 

@@ -12,10 +12,11 @@
 // comes of the latter goes into its products in two or three parts of bf16.
 //
 // Bound: at head_dim 128 a position is 144 bytes for a KV head, 6 cycles of an SM
-// at the memory's rate, and 24 instructions of a warp, three in ten of them on
-// codes, 10 cycles at the 2.4 a cycle that issue: large batches are bound by
-// issue (integer pipe 46 % busy, tensor pipe 20 %), small ones by latency, a
-// launch of one item 7.5 us.  Positions are the rows of the m16n8k16 products and
+// at the memory's rate, and 26 instructions of a warp, 11 cycles at the 2.3 a cycle
+// that issue: large batches wait for instructions' results and for one another's
+// pipes with the 16 warps an SM that 128 registers leave (integer pipe 50 % busy,
+// tensor pipe 27 %, DRAM 38 %: none is full), small ones for their loads, a launch
+// of one item 7.5 us.  Instances of 16 rows spill up to 300 bytes.  Positions are the rows of the m16n8k16 products and
 // query rows the columns: a group's few rows fill 8 columns, and an instruction
 // multiplies 256 values of K or V as they come unpacked into registers.  (On
 // tcgen05 they would pass through shared memory, which pays from 64 rows on:
@@ -32,8 +33,9 @@
 //
 // Measured on a B200 (us; graphs of calls on alternating inputs; heads of 128
 // dimensions): 64 bf16 sequences of up to 8191 positions, 64 heads on 8, 93 (308
-// MB: 3.3 TB/s); one fp16 token, 32 heads on 8, at 8000 positions 14.2; one fp32
-// token at 200 8.0; 9 bf16 sequences of 7 tokens at 4099 38.7.  (With weights as one
+// MB: 3.3 TB/s); one fp16 token, 32 heads on 8, at 8000 positions 14.5; one fp32
+// token at 200 8.2; 9 bf16 sequences of 7 tokens at 4099 39; 64 fp32 sequences of
+// up to 2000, 32 heads on 8, 48.  (With weights as one
 // fp16 relative to the largest value scale 84, 14.0, 8.1, 35.1: where scales lie
 // 2^14 and more apart, in blocks beside one another or in positions that only later
 // tokens see, results were off by up to 400 times their bounds.)

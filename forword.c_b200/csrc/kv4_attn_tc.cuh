@@ -23,13 +23,14 @@
 // parts, 16 bits of them (three of the four products are formed): with bf16's
 // range neither a block's small scales nor a row's vanish beside larger ones.
 // (One part of fp16 each, weights relative to the largest scale so far of all
-// rows' positions: 234 us for the 246 below, and values that only later tokens
+// rows' positions: 234 us for the 245 below, and values that only later tokens
 // see, or of other blocks, took bits of a result.)
 //
 // Bound: the chain of a tile's products, softmax and products beside its
-// unpacking, 1.9 us a tile; the tensor pipe is 31 % busy, and 2.1
-// instructions issue a cycle.  Measured on a B200: 512 tokens of 32
-// fp16 heads on 8 of 128 at 8191 positions 246 us (271 TFLOP/s of the formula's,
+// unpacking, 1.9 us a tile; the tensor pipe is 37 % busy, and 2.1
+// instructions issue a cycle.  All roles have the softmax's 128 registers, of which
+// it spills 220 bytes.  Measured on a B200: 512 tokens of 32
+// fp16 heads on 8 of 128 at 8191 positions 245 us (272 TFLOP/s of the formula's,
 // two and a half times that in products), bf16 233 us.
 //
 // The reference of a row is raised, and its part of O rescaled in tensor memory,

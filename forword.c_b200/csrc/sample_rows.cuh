@@ -23,10 +23,12 @@
 //
 // Bound: latency for few rows (loads, four barriers of the cluster, a short
 // sort; 6 us more where top_k reaches below the near bins beside one token that
-// holds nearly all), instruction issue for many: three passes over a row from the
-// caches, 10 to 20 instructions an entry.  Measured on a B200 (us; graphs of calls
-// on alternating inputs): a row of 128256 fp32 logits 16.8, 64 of bf16 with
-// settings of their own 38.9, 256 of 32000 in fp16 without filters 28.5.
+// holds nearly all), for many the instructions of three passes over a row from the
+// caches, 53 an entry in all: 2.2 issue a cycle (integer pipe 32 % busy, DRAM 7 %),
+// which wait for one another's results, additions in shared memory and barriers.
+// 68 to 120 bytes a thread are spilled.  Measured on a B200 (us; graphs of calls
+// on alternating inputs): a row of 128256 fp32 logits 16.9, 64 of bf16 with
+// settings of their own 39.2, 256 of 32000 in fp16 without filters 28.6.
 #pragma once
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>

@@ -347,7 +347,7 @@ typedef struct fwb_kv4_attn {
     uint64_t pages_stride;
     const int32_t *lengths, *n_new;     /* [n_seq]; held to 0..max_pages * page_size and 0..n_query */
     void *out;                          /* [n_seq][n_query][n_head][head_dim], contiguous */
-    float *lse;                         /* [n_seq][n_query][n_head], or NULL */
+    float *lse;                         /* [n_seq][n_query][n_head], or NULL; both apart from all that is read */
 } fwb_kv4_attn_t;
 
 /*
@@ -390,9 +390,10 @@ size_t fwb_kv4_attention_workspace(const fwb_kv4_attn_t *a);
  * nor in a mass; ones below 2^-32 are not drawn where they make up less than
  * 2^-24 of the mass, and a top_k or min_p that would keep some of them keeps none
  * where they make up less than 2^-20 of the mass besides the first entry's.
- * Weights carry 22 bits and are added exactly, so a token can differ from exact
- * arithmetic's only where a limit falls within about 2^-22 of the mass of a
- * border.  n_vocab at most 262144.
+ * Weights carry 22 bits (fewer below 2^-8, by the rounding of an exponent to 24 bits:
+ * 19 at 2^-64) and are added exactly, so a token can differ from exact arithmetic's
+ * only where a limit falls within about 2^-22 of the mass of a border (2^-20 where
+ * the mass is in such weights).  n_vocab at most 262144.
  */
 int fwb_sample_rows_dev(const void *d_logits, uint32_t type, size_t n_row, size_t n_vocab, size_t row_stride,
                         const float *d_uniform, const float *d_temperature, const int32_t *d_top_k, const float *d_top_p,
