@@ -249,7 +249,8 @@ class Attention(_Plan):
            dimension, address and strides multiples of 16 bytes)
     cache  uint8 [n_page, n_head_kv, page bytes]
     pages  int32 [n_seq, max_pages], lengths and n_new int32 [n_seq]
-    out    like q, contiguous; lse fp32 [n_seq, n_query, n_head].  Rows of
+    out    like q, contiguous; lse fp32 [n_seq, n_query, n_head]: memory apart
+           from all that is read.  Rows of
            tokens that a padded batch lacks are left as they were (zeros
            where out and lse are None)
 

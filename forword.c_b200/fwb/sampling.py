@@ -20,7 +20,8 @@ def sample_rows(logits, uniform, temperature=None, top_k=None, top_p=None, min_p
     stay are ranked by logit, equal ones by index; the token is the first at
     which their running mass exceeds uniform times all their mass, logprob the
     log of its share.  Temperature 0: the largest logit.  -1 and -inf where a
-    row holds a NaN or +inf or nothing but -inf.
+    row holds a NaN or +inf or nothing but -inf, or its uniform number or
+    temperature is NaN.
     """
     if logits is None or logits.dim() != 2:
         raise ValueError("logits must be [n_row, n_vocab]")
